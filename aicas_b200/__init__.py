@@ -4,10 +4,13 @@ Public surface = the reference package ``triton_qwen3vl``'s ``__all__``
 (triton_qwen3vl/__init__.py:1-16 in the reference project) plus the operators
 it leaves to Hugging Face or lacks: :func:`rope_kv_append`,
 :func:`gqa_decode_partial` and :func:`merge_partials`, and the decode-side
-products of its native decode path (:func:`decode_linear`).
+products of its native decode path (:func:`decode_linear`).  A paged cache
+(:func:`paged_rope_kv_append`, :func:`paged_gqa_decode_attention`) and 4-bit
+weights (:func:`decode_linear_int4`) serve more requests in the same memory.
 """
 from . import _native
 from .backends import TEXT_BACKEND_KEY, VISION_BACKEND_KEY, text_triton_attention, vision_triton_attention
+from .int4 import Int4Weight, decode_linear_int4, quantize_int4
 from .ops import (
     decode_linear,
     gqa_decode_attention,
@@ -18,6 +21,7 @@ from .ops import (
     varlen_flash_attention,
     vision_rope,
 )
+from .paged import paged_gqa_decode_attention, paged_rope_kv_append
 from .patch import install_qwen3vl_triton_attention
 
 
@@ -31,16 +35,21 @@ def __getattr__(name: str):
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 __all__ = [
+    "Int4Weight",
     "NATIVE_AVAILABLE",
     "TEXT_BACKEND_KEY",
     "TRITON_AVAILABLE",
     "VISION_BACKEND_KEY",
     "decode_linear",
+    "decode_linear_int4",
     "gqa_decode_attention",
     "gqa_decode_partial",
     "gqa_flash_attention",
     "install_qwen3vl_triton_attention",
     "merge_partials",
+    "paged_gqa_decode_attention",
+    "paged_rope_kv_append",
+    "quantize_int4",
     "rope_kv_append",
     "text_triton_attention",
     "varlen_flash_attention",

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libaicas_b200.so"
@@ -36,6 +37,8 @@ CAP_PEER_EXCHANGE = 32
 CAP_DECODE_LINEAR = 64
 CAP_VISION_ROPE = 128
 CAP_VISION_QKV = 256
+CAP_PAGED = 512
+CAP_LINEAR_INT4 = 1024
 
 LINEAR_MAX_SEGMENTS = 4
 LINEAR_MAX_ROWS = 32
@@ -155,6 +158,75 @@ class LinearParams(ctypes.Structure):
     ]
 
 
+class PagedAppendParams(ctypes.Structure):
+    _fields_ = [
+        ("q_in", _vp), ("q_out", _vp), ("k_in", _vp), ("v_in", _vp), ("cos", _vp), ("sin", _vp),
+        ("k_pages", _vp), ("v_pages", _vp), ("page_table", _vp), ("positions", _vp), ("num_new", _vp),
+        ("kv_lens_out", _vp), ("q_norm_weight", _vp), ("k_norm_weight", _vp),
+        ("qi_stride_b", _i64), ("qi_stride_h", _i64), ("qi_stride_s", _i64),
+        ("qo_stride_b", _i64), ("qo_stride_h", _i64), ("qo_stride_s", _i64),
+        ("k_stride_b", _i64), ("k_stride_h", _i64), ("k_stride_s", _i64),
+        ("v_stride_b", _i64), ("v_stride_h", _i64), ("v_stride_s", _i64),
+        ("cs_stride_b", _i64), ("cs_stride_s", _i64),
+        ("kp_stride_p", _i64), ("kp_stride_h", _i64), ("kp_stride_t", _i64),
+        ("vp_stride_p", _i64), ("vp_stride_h", _i64), ("vp_stride_t", _i64),
+        ("table_stride", _i64),
+        ("batch", _i32), ("num_q_heads", _i32), ("num_kv_heads", _i32), ("seq_len", _i32), ("head_dim", _i32),
+        ("num_pages", _i32), ("page_size", _i32), ("max_pages", _i32), ("dtype", _i32), ("cs_dtype", _i32),
+        ("norm_eps", _f32),
+    ]
+
+
+class PagedDecodeParams(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("k_pages", _vp), ("v_pages", _vp), ("out", _vp), ("lse", _vp),
+        ("page_table", _vp), ("kv_lens", _vp), ("kv_starts", _vp),
+        ("q_stride_b", _i64), ("q_stride_h", _i64), ("o_stride_b", _i64), ("o_stride_h", _i64),
+        ("kp_stride_p", _i64), ("kp_stride_h", _i64), ("kp_stride_t", _i64),
+        ("vp_stride_p", _i64), ("vp_stride_h", _i64), ("vp_stride_t", _i64),
+        ("table_stride", _i64),
+        ("batch", _i32), ("num_q_heads", _i32), ("num_kv_heads", _i32), ("head_dim", _i32),
+        ("num_pages", _i32), ("page_size", _i32), ("max_pages", _i32), ("dtype", _i32), ("sm_scale", _f32),
+    ]
+
+
+class Int4WeightRef(ctypes.Structure):
+    _fields_ = [("q", _vp), ("scales", _vp), ("zeros", _vp), ("q_stride", _i64)]
+
+
+class LinearInt4Params(ctypes.Structure):
+    _fields_ = [
+        ("x", _vp), ("x_stride", _i64), ("norm_weight", _vp), ("residual", _vp), ("residual_stride", _i64),
+        ("out", _vp), ("out_stride", _i64), ("w", Int4WeightRef * 2),
+        ("rows", _i32), ("in_features", _i32), ("out_features", _i32), ("group_size", _i32),
+        ("mode", _i32), ("dtype", _i32), ("eps", _f32),
+    ]
+
+
+def packer(params) -> struct.Struct:
+    """The layout of a parameter struct as one ``struct`` format, every field in
+    order: filling all fields in one call costs a fraction of as many ctypes
+    attribute assignments, which weigh in the calls that run a few microseconds."""
+
+    def codes(cls):
+        for _, kind in cls._fields_:
+            if kind in _CODES:
+                yield _CODES[kind]
+            else:  # an array of structs
+                yield "".join(codes(kind._type_)) * kind._length_
+
+    made = struct.Struct("@" + "".join(codes(params)) + "0q")
+    assert made.size == ctypes.sizeof(params)
+    return made
+
+
+_CODES = {_vp: "P", _i64: "q", _i32: "i", _f32: "f"}
+
+PACK_PAGED_APPEND = packer(PagedAppendParams)
+PACK_PAGED_DECODE = packer(PagedDecodeParams)
+PACK_LINEAR_INT4 = packer(LinearInt4Params)
+
+
 # name -> (restype, argtypes); exactly the functions declared in include/aicas_b200.h
 EXPORTS = {
     "aicas_decode_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(DecodeParams)]),
@@ -177,6 +249,11 @@ EXPORTS = {
     "aicas_vision_qkv_rope": (ctypes.c_int, [ctypes.POINTER(VisionQkvParams), _vp]),
     "aicas_linear_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(LinearParams)]),
     "aicas_decode_linear": (ctypes.c_int, [ctypes.POINTER(LinearParams), _vp, ctypes.c_size_t, _vp]),
+    # parameters as a packed bytes object (packer) or byref of the struct
+    "aicas_paged_rope_append": (ctypes.c_int, [_vp, _vp]),
+    "aicas_paged_decode_workspace_bytes": (ctypes.c_size_t, [_vp]),
+    "aicas_paged_decode_gqa": (ctypes.c_int, [_vp, _vp, ctypes.c_size_t, _vp]),
+    "aicas_linear_int4": (ctypes.c_int, [_vp, _vp]),
     "aicas_version": (ctypes.c_char_p, []),
     "aicas_capabilities": (ctypes.c_uint32, []),
     "aicas_last_error": (ctypes.c_char_p, []),

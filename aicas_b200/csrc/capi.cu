@@ -12,6 +12,8 @@
 #include "common.cuh"
 #include "fmha.cuh"
 #include "linear.cuh"
+#include "linear_int4.cuh"
+#include "paged.cuh"
 #include "vision_qkv.cuh"
 
 namespace aicas {
@@ -382,13 +384,131 @@ int check_linear(const aicas_linear_params* p) {
   return AICAS_OK;
 }
 
+// What the two paged entry points share: the pools, the page table, the sizes.
+int check_pages(const void* k_pages, const void* v_pages, const int32_t* table, int64_t table_stride, const int64_t* st,
+                int dtype, int batch, int hq, int hkv, int head_dim, int num_pages, int page_size, int max_pages) {
+  if (k_pages == nullptr || v_pages == nullptr || table == nullptr)
+    return fail(AICAS_ERR_INVALID, "k_pages, v_pages and page_table must be set");
+  const int eb = elem_bytes(dtype);
+  if (eb == 0) return fail(AICAS_ERR_UNSUPPORTED, "unknown dtype %d", dtype);
+  if (batch < 1 || hq < 1 || hkv < 1 || num_pages < 1 || max_pages < 1)
+    return fail(AICAS_ERR_INVALID, "batch=%d num_q_heads=%d num_kv_heads=%d num_pages=%d max_pages=%d", batch, hq, hkv,
+                num_pages, max_pages);
+  if (hq % hkv != 0) return fail(AICAS_ERR_INVALID, "num_q_heads=%d is not a multiple of num_kv_heads=%d", hq, hkv);
+  if (!head_dim_ok(head_dim)) return fail(AICAS_ERR_UNSUPPORTED, "head_dim %d not in {16,32,64,128}", head_dim);
+  if (page_size < 8 || page_size % 8 != 0)
+    return fail(AICAS_ERR_UNSUPPORTED, "page_size must be a positive multiple of 8 (got %d)", page_size);
+  if ((int64_t)max_pages * page_size > (int64_t)INT32_MAX - 4096)
+    return fail(AICAS_ERR_UNSUPPORTED, "max_pages * page_size = %lld slots a request is past 2^31",
+                (long long)max_pages * page_size);
+  if (!aligned16(k_pages) || !aligned16(v_pages)) return fail(AICAS_ERR_INVALID, "the pages must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(table) & 3u) != 0 || table_stride < 0)
+    return fail(AICAS_ERR_INVALID, "page_table must be 4-byte aligned with a non-negative stride");
+  for (int i = 0; i < 6; ++i)
+    if (st[i] < 0 || !stride_ok(st[i], eb) || st[i] * eb >= ((int64_t)1 << 40))
+      return fail(AICAS_ERR_INVALID, "page strides must be non-negative multiples of 16 bytes below 2^40");
+  return AICAS_OK;
+}
+
+int check_paged_append(const aicas_paged_append_params* p) {
+  if (p == nullptr) return fail(AICAS_ERR_INVALID, "params is NULL");
+  if (p->q_in == nullptr || p->q_out == nullptr || p->k_in == nullptr || p->v_in == nullptr || p->cos == nullptr ||
+      p->sin == nullptr || p->positions == nullptr)
+    return fail(AICAS_ERR_INVALID, "q_in, q_out, k_in, v_in, cos, sin and positions must be set");
+  const int64_t st[6] = {p->kp_stride_p, p->kp_stride_h, p->kp_stride_t, p->vp_stride_p, p->vp_stride_h, p->vp_stride_t};
+  const int rc = check_pages(p->k_pages, p->v_pages, p->page_table, p->table_stride, st, p->dtype, p->batch,
+                             p->num_q_heads, p->num_kv_heads, p->head_dim, p->num_pages, p->page_size, p->max_pages);
+  if (rc != AICAS_OK) return rc;
+  if (p->cs_dtype != p->dtype && p->cs_dtype != AICAS_DTYPE_F32)
+    return fail(AICAS_ERR_UNSUPPORTED, "cos/sin dtype must equal the tensor dtype or be fp32");
+  if (p->seq_len < 1 || (int64_t)p->batch * p->seq_len > (int64_t)INT32_MAX)
+    return fail(AICAS_ERR_INVALID, "seq_len=%d of batch %d", p->seq_len, p->batch);
+  const int eb = elem_bytes(p->dtype), ceb = elem_bytes(p->cs_dtype);
+  const void* ptr[] = {p->q_in, p->q_out, p->k_in, p->v_in, p->cos, p->sin, p->q_norm_weight, p->k_norm_weight};
+  for (const void* x : ptr)
+    if (!aligned16(x)) return fail(AICAS_ERR_INVALID, "device pointers must be 16-byte aligned");
+  const int64_t rows[] = {p->qi_stride_b, p->qi_stride_h, p->qi_stride_s, p->qo_stride_b, p->qo_stride_h, p->qo_stride_s,
+                          p->k_stride_b,  p->k_stride_h,  p->k_stride_s,  p->v_stride_b,  p->v_stride_h,  p->v_stride_s};
+  for (int64_t s : rows)
+    if (s < 0 || !stride_ok(s, eb)) return fail(AICAS_ERR_INVALID, "q/k/v strides must be non-negative multiples of 16 bytes");
+  if (p->cs_stride_b < 0 || p->cs_stride_s < 0 || !stride_ok(p->cs_stride_b, ceb) || !stride_ok(p->cs_stride_s, ceb))
+    return fail(AICAS_ERR_INVALID, "cos/sin strides must be non-negative multiples of 16 bytes");
+  if ((p->q_norm_weight != nullptr || p->k_norm_weight != nullptr) && !(p->norm_eps >= 0.0f))
+    return fail(AICAS_ERR_INVALID, "norm_eps must be >= 0");
+  return AICAS_OK;
+}
+
+int check_paged_decode(const aicas_paged_decode_params* p) {
+  if (p == nullptr) return fail(AICAS_ERR_INVALID, "params is NULL");
+  if (p->q == nullptr || p->out == nullptr) return fail(AICAS_ERR_INVALID, "q and out must be non-NULL");
+  const int64_t st[6] = {p->kp_stride_p, p->kp_stride_h, p->kp_stride_t, p->vp_stride_p, p->vp_stride_h, p->vp_stride_t};
+  const int rc = check_pages(p->k_pages, p->v_pages, p->page_table, p->table_stride, st, p->dtype, p->batch,
+                             p->num_q_heads, p->num_kv_heads, p->head_dim, p->num_pages, p->page_size, p->max_pages);
+  if (rc != AICAS_OK) return rc;
+  const int eb = elem_bytes(p->dtype);
+  if (!aligned16(p->q) || !aligned16(p->out)) return fail(AICAS_ERR_INVALID, "q and out must be 16-byte aligned");
+  const int64_t qo[] = {p->q_stride_b, p->q_stride_h, p->o_stride_b, p->o_stride_h};
+  for (int64_t s : qo)
+    if (s < 0 || !stride_ok(s, eb)) return fail(AICAS_ERR_INVALID, "q/out strides must be non-negative multiples of 16 bytes");
+  if (!(p->sm_scale == p->sm_scale) || p->sm_scale == INFINITY || p->sm_scale == -INFINITY)
+    return fail(AICAS_ERR_INVALID, "sm_scale must be finite");
+  // the kernel numbers 16-slot tiles of (request, KV head, block of query heads) with 32-bit ints
+  const int64_t tiles = (((int64_t)p->max_pages * p->page_size + 15) / 16 + 1) * p->batch *
+                        ((int64_t)p->num_kv_heads * ((p->num_q_heads / p->num_kv_heads + 15) / 16));
+  if (tiles > (int64_t)INT32_MAX / 2)
+    return fail(AICAS_ERR_UNSUPPORTED, "%lld tiles of 16 slots exceed the 2^30 of one launch", (long long)tiles);
+  return AICAS_OK;
+}
+
+int check_linear_int4(const aicas_linear_int4_params* p) {
+  if (p == nullptr) return fail(AICAS_ERR_INVALID, "params is NULL");
+  if (p->dtype != AICAS_DTYPE_F16 && p->dtype != AICAS_DTYPE_BF16)
+    return fail(AICAS_ERR_UNSUPPORTED, "int4 linear needs fp16 or bf16 activations (dtype %d)", p->dtype);
+  if (p->rows < 0 || p->rows > AICAS_LINEAR_MAX_ROWS)
+    return fail(AICAS_ERR_UNSUPPORTED, "int4 linear takes 0..%d rows (got %d)", AICAS_LINEAR_MAX_ROWS, p->rows);
+  if (p->group_size != 32 && p->group_size != 64 && p->group_size != 128)
+    return fail(AICAS_ERR_UNSUPPORTED, "group_size %d not in {32,64,128}", p->group_size);
+  if (p->in_features <= 0 || p->in_features % p->group_size != 0)
+    return fail(AICAS_ERR_UNSUPPORTED, "in_features=%d must be a positive multiple of group_size=%d", p->in_features,
+                p->group_size);
+  if (p->out_features <= 0) return fail(AICAS_ERR_INVALID, "out_features=%d", p->out_features);
+  if (p->mode != AICAS_LINEAR_STORE && p->mode != AICAS_LINEAR_RESIDUAL && p->mode != AICAS_LINEAR_SWIGLU)
+    return fail(AICAS_ERR_INVALID, "unknown mode %d", p->mode);
+  if (p->x == nullptr || !aligned16(p->x)) return fail(AICAS_ERR_INVALID, "x must be a 16-byte aligned pointer");
+  if (p->x_stride < p->in_features || !stride_ok(p->x_stride, 2))
+    return fail(AICAS_ERR_INVALID, "x_stride must be >= in_features and a multiple of 8 elements");
+  if (p->norm_weight != nullptr && !aligned16(p->norm_weight))
+    return fail(AICAS_ERR_INVALID, "norm_weight must be 16-byte aligned");
+  if (p->norm_weight != nullptr && !(p->eps >= 0.0f)) return fail(AICAS_ERR_INVALID, "eps must be >= 0");
+  if (p->out == nullptr || (reinterpret_cast<uintptr_t>(p->out) & 1u) != 0)
+    return fail(AICAS_ERR_INVALID, "out must be a 2-byte aligned pointer");
+  if (p->rows > 1 && p->out_stride < p->out_features) return fail(AICAS_ERR_INVALID, "out_stride must be >= out_features");
+  if (p->mode == AICAS_LINEAR_RESIDUAL) {
+    if (p->residual == nullptr || (reinterpret_cast<uintptr_t>(p->residual) & 1u) != 0)
+      return fail(AICAS_ERR_INVALID, "the residual epilogue needs a 2-byte aligned residual");
+    if (p->residual_stride < 0) return fail(AICAS_ERR_INVALID, "residual_stride must be >= 0");
+  }
+  for (int j = 0; j < (p->mode == AICAS_LINEAR_SWIGLU ? 2 : 1); ++j) {
+    const aicas_int4_weight& w = p->w[j];
+    if (w.q == nullptr || !aligned16(w.q)) return fail(AICAS_ERR_INVALID, "weight %d: q must be a 16-byte aligned pointer", j);
+    if (w.q_stride < p->in_features / 2 || w.q_stride % 16 != 0)
+      return fail(AICAS_ERR_INVALID, "weight %d: q_stride must be >= in_features / 2 and a multiple of 16", j);
+    if (w.scales == nullptr || (reinterpret_cast<uintptr_t>(w.scales) & 1u) != 0)
+      return fail(AICAS_ERR_INVALID, "weight %d: scales must be a 2-byte aligned pointer", j);
+  }
+  if (p->mode == AICAS_LINEAR_SWIGLU && (p->w[0].zeros == nullptr) != (p->w[1].zeros == nullptr))
+    return fail(AICAS_ERR_INVALID, "both weights of the SwiGLU epilogue have zeros, or neither");
+  return AICAS_OK;
+}
+
 extern "C" {
 
 const char* aicas_version(void) { return "aicas_b200 0.2.0 sm_100a abi 2"; }
 
 uint32_t aicas_capabilities(void) {
   return AICAS_CAP_DECODE | AICAS_CAP_MERGE | AICAS_CAP_ROPE_APPEND | AICAS_CAP_PEER_EXCHANGE |
-         AICAS_CAP_DECODE_LINEAR | AICAS_CAP_VISION_ROPE | AICAS_CAP_VISION_QKV | aicas::fmha_capabilities();
+         AICAS_CAP_DECODE_LINEAR | AICAS_CAP_VISION_ROPE | AICAS_CAP_VISION_QKV | AICAS_CAP_PAGED |
+         AICAS_CAP_LINEAR_INT4 | aicas::fmha_capabilities();
 }
 
 const char* aicas_last_error(void) { return g_err; }
@@ -775,6 +895,38 @@ int aicas_decode_linear(const aicas_linear_params* p, void* workspace, size_t wo
   if (rc != AICAS_OK) return rc;
   return aicas::run_linear(p, sm_count(), workspace, workspace_bytes, static_cast<cudaStream_t>(stream),
                            device_error_word(), g_err, sizeof(g_err));
+}
+
+int aicas_paged_rope_append(const aicas_paged_append_params* p, void* stream) {
+  const int rc = check_paged_append(p);
+  if (rc != AICAS_OK) return rc;
+  return aicas::run_paged_append(p, static_cast<cudaStream_t>(stream), g_err, sizeof(g_err));
+}
+
+size_t aicas_paged_decode_workspace_bytes(const aicas_paged_decode_params* p) {
+  if (check_paged_decode(p) != AICAS_OK) return 0;
+  return aicas::paged_decode_workspace(p, sm_count());
+}
+
+int aicas_paged_decode_gqa(const aicas_paged_decode_params* p, void* workspace, size_t workspace_bytes, void* stream) {
+  const int rc = check_paged_decode(p);
+  if (rc != AICAS_OK) return rc;
+  const size_t need = aicas::paged_decode_workspace(p, sm_count());
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(AICAS_ERR_WORKSPACE, "paged decode needs %zu bytes of zero-initialised workspace (got %zu)", need,
+                workspace_bytes);
+  if (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+    return fail(AICAS_ERR_INVALID, "workspace must be 256-byte aligned");
+  return aicas::run_paged_decode(p, sm_count(), workspace, static_cast<cudaStream_t>(stream), device_error_word(),
+                                 g_err, sizeof(g_err));
+}
+
+int aicas_linear_int4(const aicas_linear_int4_params* p, void* stream) {
+  const int rc = check_linear_int4(p);
+  if (rc != AICAS_OK) return rc;
+  if (p->rows == 0) return AICAS_OK;
+  return aicas::run_linear_int4(p, sm_count(), static_cast<cudaStream_t>(stream), device_error_word(), g_err,
+                                sizeof(g_err));
 }
 
 }  // extern "C"

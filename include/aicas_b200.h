@@ -54,6 +54,13 @@
  *                             residual add of HF Qwen3VLTextDecoderLayer
  *                             (modeling_qwen3_vl.py:545-563)
  *
+ * and add these, which the reference lacks (its caches are contiguous and its
+ * weights 16-bit):
+ *
+ *   aicas_paged_rope_append   aicas_rope_kv_append into a paged cache
+ *   aicas_paged_decode_gqa    aicas_decode_gqa over a paged cache
+ *   aicas_linear_int4         aicas_decode_linear with 4-bit weights
+ *
  * Layout conventions: attention tensors are 4-D [batch, heads, tokens, head_dim]
  * with head_dim contiguous (stride 1).  Strides are given in ELEMENTS.  All
  * device pointers must be 16-byte aligned and every stride times the element
@@ -394,6 +401,111 @@ AICAS_API int aicas_decode_linear(const aicas_linear_params* p, void* workspace,
                                   void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Paged KV cache: a pool of pages [P, Hkv, page_size, D] for the keys and one  */
+/* for the values, and a page table [B, max_pages] of int32: slot t of request  */
+/* b is row t % page_size of page page_table[b, t / page_size].  The strides of */
+/* pages, heads and rows are free (multiples of 16 bytes; D is contiguous), so  */
+/* a [P, page_size, Hkv, D] pool is passed by its strides.  page_size is a      */
+/* multiple of 8.                                                               */
+/* ------------------------------------------------------------------------ */
+typedef struct aicas_paged_append_params {
+  const void* q_in;         /* [B, Hq, S, D] */
+  void* q_out;              /* [B, Hq, S, D] rotated q (may alias q_in) */
+  const void* k_in;         /* [B, Hkv, S, D] new keys (before RoPE) */
+  const void* v_in;         /* [B, Hkv, S, D] new values */
+  const void* cos;          /* [B, S, D] */
+  const void* sin;          /* [B, S, D] */
+  void* k_pages;
+  void* v_pages;
+  const int32_t* page_table; /* [B, max_pages], table_stride elements between requests */
+  const int32_t* positions; /* [B] slot of the first new token per request */
+  const int32_t* num_new;   /* optional [B]: how many of the S tokens are real (a padded batch); NULL = S */
+  int32_t* kv_lens_out;     /* optional [B]: receives min(max(positions[b], 0) + num_new[b], capacity) */
+  const void* q_norm_weight; /* optional [D] (dtype of q): per-head RMSNorm before RoPE */
+  const void* k_norm_weight; /* optional [D] */
+  int64_t qi_stride_b, qi_stride_h, qi_stride_s;
+  int64_t qo_stride_b, qo_stride_h, qo_stride_s;
+  int64_t k_stride_b, k_stride_h, k_stride_s;
+  int64_t v_stride_b, v_stride_h, v_stride_s;
+  int64_t cs_stride_b, cs_stride_s;  /* strides of cos and sin (same for both) */
+  int64_t kp_stride_p, kp_stride_h, kp_stride_t; /* k_pages: page, head, row */
+  int64_t vp_stride_p, vp_stride_h, vp_stride_t;
+  int64_t table_stride;
+  int32_t batch, num_q_heads, num_kv_heads, seq_len, head_dim; /* head_dim 16, 32, 64 or 128 */
+  int32_t num_pages, page_size, max_pages;
+  int32_t dtype;            /* dtype of q, k, v, pages and norm weights */
+  int32_t cs_dtype;         /* dtype of cos/sin.  AICAS_DTYPE_F32: norm and rotation in fp32, rounded once.
+                               The 16-bit dtype of the tensors: rounded after every operation, as HF's
+                               modules and aicas_rope_kv_append round */
+  float norm_eps;
+} aicas_paged_append_params;
+
+/* Tokens whose slot is negative or past max_pages * page_size, or whose page
+   number is outside [0, num_pages), are dropped; pages shared by two requests
+   must not be appended to by both in one call. */
+AICAS_API int aicas_paged_rope_append(const aicas_paged_append_params* p, void* stream);
+
+typedef struct aicas_paged_decode_params {
+  const void* q;            /* [B, Hq, 1, D] */
+  const void* k_pages;
+  const void* v_pages;
+  void* out;                /* [B, Hq, 1, D] */
+  float* lse;               /* optional [B, Hq] fp32 base-2 log-sum-exp of the scaled logits (-inf for no slot) */
+  const int32_t* page_table; /* [B, max_pages], table_stride elements between requests */
+  const int32_t* kv_lens;   /* optional [B] cached length per request (clamped to 0..capacity); NULL = capacity */
+  const int32_t* kv_starts; /* optional [B] first slot attended to; NULL = 0 */
+  int64_t q_stride_b, q_stride_h;
+  int64_t o_stride_b, o_stride_h;
+  int64_t kp_stride_p, kp_stride_h, kp_stride_t; /* k_pages: page, head, row */
+  int64_t vp_stride_p, vp_stride_h, vp_stride_t;
+  int64_t table_stride;
+  int32_t batch, num_q_heads, num_kv_heads, head_dim; /* any whole num_q_heads / num_kv_heads; head_dim 16, 32, 64, 128 */
+  int32_t num_pages, page_size, max_pages;
+  int32_t dtype;
+  float sm_scale;
+} aicas_paged_decode_params;
+
+/* Bytes of workspace for these parameters: the layout and the rules of
+   aicas_decode_workspace_bytes (the same zero-initialised buffer serves both).
+   A request with no slot (kv_lens[b] <= kv_starts[b]) gets zeros.  Page numbers
+   outside [0, num_pages) read as rows of zeros. */
+AICAS_API size_t aicas_paged_decode_workspace_bytes(const aicas_paged_decode_params* p);
+AICAS_API int aicas_paged_decode_gqa(const aicas_paged_decode_params* p, void* workspace, size_t workspace_bytes,
+                                     void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Decode-side products with 4-bit weights:                                   */
+/*   W[n, k] = scales[n, k / g] * (q[n, k] - zeros[n, k / g]),  q in 0..15.     */
+/* ------------------------------------------------------------------------ */
+typedef struct aicas_int4_weight {
+  const void* q;            /* [N, K / 2] bytes: even k in the low half, q_stride bytes between rows */
+  const void* scales;       /* [N, K / g] of the dtype of x, contiguous */
+  const void* zeros;        /* optional [N, K / g] uint8 in 0..15, contiguous; NULL = 8 */
+  int64_t q_stride;
+} aicas_int4_weight;
+
+typedef struct aicas_linear_int4_params {
+  const void* x;            /* [rows, in_features], x_stride elements between rows */
+  int64_t x_stride;
+  const void* norm_weight;  /* optional [in_features]: x' = round(x * rsqrt(mean x^2 + eps) * norm_weight) */
+  const void* residual;     /* RESIDUAL: [rows, out_features] */
+  int64_t residual_stride;
+  void* out;                /* [rows, out_features] */
+  int64_t out_stride;
+  aicas_int4_weight w[2];   /* w[1]: the up projection of SWIGLU, else unused */
+  int32_t rows;             /* 1 .. AICAS_LINEAR_MAX_ROWS (0: nothing to do) */
+  int32_t in_features;      /* a multiple of group_size */
+  int32_t out_features;
+  int32_t group_size;       /* g: 32, 64 or 128 */
+  int32_t mode;             /* AICAS_LINEAR_*: x' W^T; residual + x' W^T; silu(x' W0^T) * (x' W1^T).
+                               Held in fp32 and rounded once to the output */
+  int32_t dtype;            /* AICAS_DTYPE_F16 or AICAS_DTYPE_BF16, shared by x, scales, norm_weight, residual, out */
+  float eps;
+} aicas_linear_int4_params;
+
+AICAS_API int aicas_linear_int4(const aicas_linear_int4_params* p, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Library queries.                                                           */
 /* ------------------------------------------------------------------------ */
 /* "aicas_b200 <version> sm_100a abi <n>" */
@@ -409,6 +521,8 @@ AICAS_API const char* aicas_version(void);
 #define AICAS_CAP_DECODE_LINEAR 64u
 #define AICAS_CAP_VISION_ROPE 128u
 #define AICAS_CAP_VISION_QKV 256u
+#define AICAS_CAP_PAGED 512u
+#define AICAS_CAP_LINEAR_INT4 1024u
 AICAS_API uint32_t aicas_capabilities(void);
 
 /* Message of the last failed call on this thread ("" if none). */
