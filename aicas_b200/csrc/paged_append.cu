@@ -42,7 +42,7 @@ __device__ __forceinline__ void load_table(const CS* p, float* f) {
   constexpr int kV = Elem<CS>::kPerVec;
   if constexpr (N >= kV) {
 #pragma unroll
-    for (int i = 0; i < N / kV; ++i) Elem<CS>::unpack(__ldg(reinterpret_cast<const uint4*>(p) + i), f + i * kV);
+    for (int i = 0; i < N / kV; ++i) Elem<CS>::unpack(reinterpret_cast<const uint4*>(p)[i], f + i * kV);
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) f[i] = Elem<CS>::to_float(p[i]);
