@@ -13,7 +13,8 @@ from typing import NamedTuple, Sequence
 import torch
 
 from . import _native as nat
-from .ops import _LINEAR_DTYPES, _call_in_device, _overlaps, _reject_grad, _row_major, _stream_handle
+from ._hostpath import launch, pointer
+from .ops import _LINEAR_DTYPES, _overlaps, _reject_grad
 
 INT4_GROUP_SIZES = (32, 64, 128)
 
@@ -62,22 +63,25 @@ def quantize_int4(weight: torch.Tensor, group_size: int = 128, *, symmetric: boo
     return Int4Weight(q[:, 0::2] | (q[:, 1::2] << 4), scales.contiguous(), zeros)
 
 
-def _check_weight(w, x: torch.Tensor, k: int):
-    """(qweight, scales, zeros, N, groups) of one weight, checked against x."""
+def _check_weight(w, dtype: torch.dtype, index: int, k: int):
+    """(qweight, its row stride, scales, zeros, N, groups) of one weight, checked against x."""
     q, scales, zeros = w
-    if not (q.is_cuda and scales.is_cuda) or q.device != x.device or scales.device != x.device:
+    if q.get_device() != index or scales.get_device() != index:
         raise ValueError("decode_linear_int4 needs CUDA tensors on one device")
-    if q.dtype != torch.uint8 or q.ndim != 2 or q.shape[1] * 2 != k:
+    q_shape = q.shape
+    if q.dtype is not torch.uint8 or len(q_shape) != 2 or q_shape[1] * 2 != k:
         raise ValueError(f"decode_linear_int4: qweight must be uint8 [N, {k // 2}]")
-    n, groups = q.shape[0], scales.shape[-1]
-    if scales.ndim != 2 or scales.shape[0] != n or scales.dtype != x.dtype or not scales.is_contiguous():
+    n, shape = q_shape[0], scales.shape
+    if len(shape) != 2 or shape[0] != n or scales.dtype is not dtype or not scales.is_contiguous():
         raise ValueError(f"decode_linear_int4: scales must be contiguous [{n}, K / g] of the dtype of x")
-    if q.stride(1) != 1 or q.stride(0) % 16 or q.data_ptr() % 16:
-        q = q.contiguous()
-    if zeros is not None and (zeros.shape != scales.shape or zeros.dtype != torch.uint8
-                              or zeros.device != x.device or not zeros.is_contiguous()):
+    s = q.stride()
+    if s[1] != 1 or (s[0] | q.data_ptr()) & 15 or s[0] * 2 < k:
+        q = q.contiguous().clone()
+        s = q.stride()
+    if zeros is not None and (zeros.shape != shape or zeros.dtype is not torch.uint8
+                              or zeros.get_device() != index or not zeros.is_contiguous()):
         raise ValueError("decode_linear_int4: zeros must be contiguous uint8 of the shape of the scales")
-    return q, scales, zeros, n, groups
+    return q, s[0], scales, zeros, n, shape[1]
 
 
 def decode_linear_int4(
@@ -95,79 +99,78 @@ def decode_linear_int4(
     * ``x`` ``[R, K]`` fp16 or bf16, R <= 32; ``weight`` an :class:`Int4Weight` of
       ``[N, K]`` with scales of the dtype of x -> ``[R, N]``.  Several weights of
       one x (q, k and v) are one weight with their rows one after the other.
-    * ``norm_weight`` ``[K]``: x' = RMSNorm(x) with that weight and ``eps``,
-      computed in fp32 and rounded once (the tensor cores take 16-bit operands).
+    * ``norm_weight`` ``[K]``: x' = RMSNorm(x) with that weight and ``eps``
+      in fp32, not rounded (two 16-bit parts go through the tensor cores).
     * ``residual`` ``[R, N]``: returns ``residual + x' W^T``; ``out=residual`` updates
       it in place.
     * ``swiglu=True`` with ``weight=(gate, up)``: ``silu(x' Wg^T) * (x' Wu^T)``.
 
     Sums are held in fp32 and the result is rounded once.  ``ValueError`` for
     what the kernel cannot take."""
-    pair = swiglu
-    weights = list(weight) if pair else [weight]
-    if pair and (len(weights) != 2 or isinstance(weight, Int4Weight)):
-        raise ValueError("swiglu needs weight=(gate, up)")
-    if not pair and (len(weight) != 3 or not isinstance(weight[0], torch.Tensor)):
-        raise ValueError("decode_linear_int4 takes one Int4Weight, or with swiglu=True a (gate, up) pair")
-    _reject_grad(x)
-    if not x.is_cuda:
-        raise ValueError("decode_linear_int4 needs CUDA tensors")
+    if swiglu:
+        if len(weight) != 2 or isinstance(weight, Int4Weight):
+            raise ValueError("swiglu needs weight=(gate, up)")
+        first = weight[0]
+    else:
+        first = weight
+        if len(weight) != 3 or not isinstance(weight[0], torch.Tensor):
+            raise ValueError("decode_linear_int4 takes one Int4Weight, or with swiglu=True a (gate, up) pair")
+    if x.requires_grad:
+        _reject_grad(x)
     dtype, device = x.dtype, x.device
+    if device.type != "cuda":
+        raise ValueError("decode_linear_int4 needs CUDA tensors")
     if dtype not in _LINEAR_DTYPES:
         raise ValueError("decode_linear_int4 needs fp16 or bf16 x")
-    x = _row_major(x, "x")
+    if x.ndim != 2:
+        raise ValueError("x must be 2-D")
     R, K = x.shape
-    if R > 1 and x.stride(0) < K:  # rows that overlap (an expanded x)
-        x = x.contiguous()
+    index = x.get_device()
+    xs = x.stride()
+    if xs[1] != 1 or (xs[0] * 2 | x.data_ptr()) & 15 or xs[0] < K:  # unaligned, or rows that overlap
+        x = x.contiguous().clone()
+        xs = x.stride()
     if R > nat.LINEAR_MAX_ROWS:
         raise ValueError(f"decode_linear_int4 takes at most {nat.LINEAR_MAX_ROWS} rows (got {R})")
-    checked = [_check_weight(w, x, K) for w in weights]
-    q, scales, zeros, N, groups = checked[0]
+    q, q_stride, scales, zeros, N, groups = _check_weight(first, dtype, index, K)
     if not groups or K % groups or K // groups not in INT4_GROUP_SIZES:
         raise ValueError(f"decode_linear_int4: {groups} scales a row of {K}: groups must be of {INT4_GROUP_SIZES}")
-    if pair and (checked[1][3:] != (N, groups) or (checked[1][2] is None) != (zeros is None)):
-        raise ValueError("decode_linear_int4: gate and up must be of one shape and kind")
-    if residual is not None:
-        if pair:
+    second = (0, 0, 0, 0)
+    if swiglu:
+        if residual is not None:
             raise ValueError("decode_linear_int4: residual and swiglu exclude each other")
-        if residual.shape != (R, N) or residual.dtype != dtype or residual.device != device or residual.stride(1) != 1:
+        q2, q2_stride, scales2, zeros2, *sizes = _check_weight(weight[1], dtype, index, K)
+        if sizes != [N, groups] or (zeros2 is None) != (zeros is None):
+            raise ValueError("decode_linear_int4: gate and up must be of one shape and kind")
+        second = (q2.data_ptr(), scales2.data_ptr(), pointer(zeros2), q2_stride)
+    mode, res, res_stride = nat.LINEAR_SWIGLU if swiglu else nat.LINEAR_STORE, 0, 0
+    if residual is not None:
+        mode, res, res_stride = nat.LINEAR_RESIDUAL, residual.data_ptr(), residual.stride(0)
+        if residual.shape != (R, N) or residual.dtype is not dtype or residual.get_device() != index or residual.stride(1) != 1:
             raise ValueError(f"residual must be [{R}, {N}] of the dtype of x with unit stride on the last dimension")
     if norm_weight is not None:
-        if norm_weight.shape != (K,) or norm_weight.dtype != dtype or norm_weight.device != device:
+        if norm_weight.shape != (K,) or norm_weight.dtype is not dtype or norm_weight.get_device() != index:
             raise ValueError(f"norm_weight must be a [{K}] tensor of the dtype of x")
-        if not norm_weight.is_contiguous() or norm_weight.data_ptr() % 16:
+        if not norm_weight.is_contiguous() or norm_weight.data_ptr() & 15:
             norm_weight = norm_weight.contiguous().clone()
     if out is None:
-        out = torch.empty((R, N), dtype=dtype, device=device)
+        out, out_stride = torch.empty_strided((R, N), (N, 1), dtype=dtype, device=device), N
     else:
         if out.shape != (R, N) or out.dtype != dtype or out.device != device or out.stride(1) != 1 \
                 or (R > 1 and out.stride(0) < N):
             raise ValueError(f"out must be [{R}, {N}] of the dtype of x with rows apart and unit stride within")
+        out_stride = out.stride(0)
         # every CTA reads all of x while others already write their outputs
         if _overlaps(out, x) or (norm_weight is not None and _shares(out, norm_weight)):
             raise ValueError("decode_linear_int4: out must not overlap x or norm_weight")
         # a residual is read where its sum is written: the same elements, or others altogether
-        if residual is not None and _overlaps(out, residual) and (
-                out.data_ptr() != residual.data_ptr() or out.stride() != residual.stride()):
+        if residual is not None and _overlaps(out, residual) and (res != out.data_ptr() or (R > 1 and res_stride != out_stride)):
             raise ValueError("decode_linear_int4: out must be the residual or not overlap it")
-    if R == 0 or N == 0:
-        return out
-    q2, scales2, zeros2 = checked[1][:3] if pair else (None, None, None)
-    args = nat.PACK_LINEAR_INT4.pack(
-        x.data_ptr(), x.stride(0) if R > 1 else K, 0 if norm_weight is None else norm_weight.data_ptr(),
-        0 if residual is None else residual.data_ptr(), 0 if residual is None else residual.stride(0),
-        out.data_ptr(), out.stride(0),
-        q.data_ptr(), scales.data_ptr(), 0 if zeros is None else zeros.data_ptr(), q.stride(0),
-        0 if q2 is None else q2.data_ptr(), 0 if q2 is None else scales2.data_ptr(),
-        0 if zeros2 is None else zeros2.data_ptr(), 0 if q2 is None else q2.stride(0),
-        R, K, N, K // groups,
-        nat.LINEAR_SWIGLU if pair else nat.LINEAR_STORE if residual is None else nat.LINEAR_RESIDUAL,
-        _LINEAR_DTYPES[dtype], eps)
-
-    def run():
-        nat.check(nat.lib().aicas_linear_int4(args, _stream_handle(device)), "aicas_linear_int4")
-
-    _call_in_device(device, run)
+    if R and N:
+        launch(device, "aicas_linear_int4", nat.PACK_LINEAR_INT4.pack(
+            x.data_ptr(), xs[0], pointer(norm_weight), res, res_stride, out.data_ptr(), out_stride,
+            q.data_ptr(), scales.data_ptr(), pointer(zeros), q_stride, *second,
+            R, K, N, K // groups, mode, _LINEAR_DTYPES[dtype], eps))
     return out
 
 

@@ -487,7 +487,8 @@ typedef struct aicas_int4_weight {
 typedef struct aicas_linear_int4_params {
   const void* x;            /* [rows, in_features], x_stride elements between rows */
   int64_t x_stride;
-  const void* norm_weight;  /* optional [in_features]: x' = round(x * rsqrt(mean x^2 + eps) * norm_weight) */
+  const void* norm_weight;  /* optional [in_features]: x' = x * rsqrt(mean x^2 + eps) * norm_weight, in fp32
+                               (carried as two 16-bit parts); NULL: x' = x */
   const void* residual;     /* RESIDUAL: [rows, out_features] */
   int64_t residual_stride;
   void* out;                /* [rows, out_features] */

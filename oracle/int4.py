@@ -4,8 +4,6 @@ from __future__ import annotations
 
 import numpy as np
 
-from .rope import round_to
-
 
 def widen(qweight: np.ndarray, scales: np.ndarray, zeros: np.ndarray | None) -> np.ndarray:
     """W[n, k] = scales[n, k // g] * (q[n, k] - zeros[n, k // g])."""
@@ -17,26 +15,19 @@ def widen(qweight: np.ndarray, scales: np.ndarray, zeros: np.ndarray | None) -> 
     return (q - z) * np.repeat(scales.astype(np.float64), g, axis=1)
 
 
-def norm_rows(x: np.ndarray, weight: np.ndarray, eps: float, dtype: str) -> np.ndarray:
-    """RMSNorm rounded once to the dtype, as the kernel's 16-bit operand is."""
+def norm_rows(x: np.ndarray, weight: np.ndarray, eps: float) -> np.ndarray:
     y = x.astype(np.float64)
-    y = y / np.sqrt((y * y).mean(axis=-1, keepdims=True) + eps) * weight.astype(np.float64)
-    return round_to(y.astype(np.float32), dtype).astype(np.float64)
+    return y / np.sqrt((y * y).mean(axis=-1, keepdims=True) + eps) * weight.astype(np.float64)
 
 
-def linear(x, weights, *, norm_weight=None, eps=1e-6, residual=None, swiglu=False, dtype="bf16"):
-    """(y, bound): the product before its last rounding, and a bound of what fp32
+def linear(x, weights, *, norm_weight=None, eps=1e-6, residual=None, swiglu=False):
+    """(y, bound): the product before its one rounding, and a bound of what fp32
     sums may be off: every sum of K terms, in whatever order, within 2^-15 of the
     sum of the terms' magnitudes (chains of up to 512 additions of relative error
-    2^-24), plus, with a norm, two operands a row whose rounding went the other way."""
-    xd = norm_rows(x, norm_weight, eps, dtype) if norm_weight is not None else np.asarray(x, np.float64)
-    ys, offs = [], []
-    for w in weights:
-        y, off = xd @ w.T, 2.0 ** -15 * (np.abs(xd) @ np.abs(w).T)
-        if norm_weight is not None:
-            off = off + 2 * (2.0 ** -7 if dtype == "bf16" else 2.0 ** -10) * np.abs(xd).max() * np.abs(w).max()
-        ys.append(y)
-        offs.append(off)
+    2^-24; a normalised x in two 16-bit parts is within 2^-16 of itself)."""
+    xd = norm_rows(x, norm_weight, eps) if norm_weight is not None else np.asarray(x, np.float64)
+    ys = [xd @ w.T for w in weights]
+    offs = [2.0 ** -15 * (np.abs(xd) @ np.abs(w).T) for w in weights]
     if swiglu:
         s = ys[0] / (1.0 + np.exp(-ys[0]))
         # |silu'| <= 1.1

@@ -41,8 +41,7 @@ def _case(device, rows, k, n, group=128, dtype="bf16", zeros=False, norm=False, 
     res = torch.randn(rows, n, generator=g).to(DT[dtype]).to(device) if residual else None
     y = ab.decode_linear_int4(x, w if swiglu else w[0], norm_weight=nw, residual=res, swiglu=swiglu)
     assert y.shape == (rows, n) and y.dtype == x.dtype
-    ref, off = oi.linear(_np(x), [_wide(v) for v in w], norm_weight=_np(nw), residual=_np(res), swiglu=swiglu,
-                         dtype=dtype)
+    ref, off = oi.linear(_np(x), [_wide(v) for v in w], norm_weight=_np(nw), residual=_np(res), swiglu=swiglu)
     over = np.abs(_np(y).astype(np.float64) - ref) - (HALF_ULP[dtype] * (np.abs(ref) + off) + off)
     assert over.max() <= 2.0 ** -24, f"{over.max():.3e} over the bound at {np.unravel_index(over.argmax(), over.shape)}"
     assert nat.device_error_flags() == 0
