@@ -5,18 +5,25 @@
 // HBM bound: N K / 2 bytes of weights for at most 2 * 32 * N K flops.  What it
 // takes is turning 4-bit numbers into tensor-core operands as fast as they come.
 //
-//   * Operands: mma.sync m16n8k16 with the weights as the 16 x 16 side, in
+//   * Operands: mma.sync m16n8k16 in fp16 with the weights as the 16 x 16 side, in
 //     registers, and the activations as columns.  A 32-bit word of weights holds
-//     k0..k7 of a row; (word >> 4 j) & 0x000f000f is the pair (k_j, k_{j+4}), and
-//     or-ing the bits of 128 (bf16) or 1024 (fp16), whose units are 1, and
-//     subtracting 128 + zero gives the exact q - zero.  The products do not care
-//     in what order k goes by, so the weights stay as stored and the activations
-//     are laid out in shared memory to match, once a CTA.  tcgen05 would need the
-//     widened weights written back to shared or tensor memory: four times the
-//     bytes that came from HBM.
-//   * Sums: a group's products are summed in fp32 over whole numbers, multiplied
-//     by the group's scale in fp32 and added up in fp32; one rounding at the end.
-//     A normalised x' is carried as two 16-bit parts in neighbouring columns.
+//     k0..k7 of a row.  word & 0x000f000f is the pair (k0, k4) as it stands: a
+//     4-bit number in the low bits of an fp16 is that number times 2^-24, a
+//     subnormal that the tensor cores take exactly.  word & 0x00f000f0 is (k1, k5)
+//     times 2^-20, and the word shifted by 8 gives the other two pairs: 5
+//     instructions for 8 weights.  The odd k's activations are held times 2^-4 to
+//     match, and the products do not care in what order k goes by, so the weights
+//     stay as stored and the activations are laid out in shared memory to suit.
+//     tcgen05 would need the widened weights written back to shared or tensor
+//     memory: four times the bytes that came from HBM.
+//   * Activations: x' of a row times a power of two that brings its largest
+//     element to [2^9, 2^10), as fp16.  16-bit x is exact so (an element 2^30
+//     times smaller than the row's largest loses its last bits).  A normalised x'
+//     is rounded to fp16's 11 bits where the result has bf16's 8, and carried as
+//     two fp16 parts in neighbouring columns where the result is fp16.
+//   * Sums: a group's sum over the whole numbers q in fp32, less zero point times
+//     the group's sum of activations, times the scale in fp32; groups, warps and
+//     CTAs are added up in fp32; one rounding at the end.
 //   * Work: a cluster of S CTAs takes a run of 16-row tiles (8 gate + 8 up rows
 //     for SiLU * up), each CTA one S-th of K, so that its share of x' fits beside
 //     the ring (S = 1 wherever all of it does).  Tiles are taken in rounds; a
@@ -26,6 +33,7 @@
 //     a private TMA ring that runs on across rounds.
 #include <cstdio>
 #include <cstring>
+#include <type_traits>
 
 #include "common.cuh"
 #include "linear_int4.cuh"
@@ -34,13 +42,15 @@
 namespace aicas {
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
 constexpr int kJobK = 256;              // k of a job: 128 bytes of a row
 constexpr int kJobBytes = 16 * 128;     // 16 rows
 constexpr int kPitch = 20;              // floats a column of a partial tile (16 rows; 20 keeps stores conflict free)
 constexpr int kMaxSmem = 232448;
-constexpr int kTwoPerSm = 115712;       // shared memory of a CTA of which two fit on an SM
+constexpr int kVarBytes = 64 + 4 * 160;  // abort flag; rows' statistics, scales and their inverses
+
+// Warps of a CTA: more of them hide the products' latency, fewer leave shared
+// memory for the columns of many rows.
+constexpr int warps_for(int nt) { return nt <= 2 ? 16 : 8; }
 
 struct Int4Args {
   CUtensorMap tm_w[2];
@@ -58,39 +68,16 @@ struct Int4Args {
   int kb;                  // jobs of a tile for each of them
   int tiles, tiles_round;  // 16-row tiles of the launch; tiles of a round
   int stages;
-  int off_part, off_x, off_bars;
+  int off_part, off_x, off_sum, off_bars;
   unsigned int* err;
 };
 
-template <typename T> struct Int4Type;
-template <> struct Int4Type<__nv_bfloat16> {
-  static constexpr uint32_t kMagic = 0x4300u;  // 128: its unit in the last place is 1
-  __device__ __forceinline__ static uint32_t sub(uint32_t a, uint32_t b) {
-    __nv_bfloat162 x = *reinterpret_cast<__nv_bfloat162*>(&a), y = *reinterpret_cast<__nv_bfloat162*>(&b);
-    x = __hsub2(x, y);
-    return *reinterpret_cast<uint32_t*>(&x);
-  }
-  __device__ __forceinline__ static void mma(float c[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                             uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  }
-};
-template <> struct Int4Type<__half> {
-  static constexpr uint32_t kMagic = 0x6400u;  // 1024: its unit in the last place is 1
-  __device__ __forceinline__ static uint32_t sub(uint32_t a, uint32_t b) {
-    __half2 x = *reinterpret_cast<__half2*>(&a), y = *reinterpret_cast<__half2*>(&b);
-    x = __hsub2(x, y);
-    return *reinterpret_cast<uint32_t*>(&x);
-  }
-  __device__ __forceinline__ static void mma(float c[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                             uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  }
-};
+__device__ __forceinline__ void mma_f16(float c[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 
 template <typename T>
 __device__ __forceinline__ float low_half(uint32_t v) {
@@ -124,49 +111,65 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ int tile_row(int g) { return (g & 1) << 2 | (g & 2) | g >> 2; }
 
 // A warp's jobs: those of each round's (tile, job along K) list that fall to it.
+template <int WARPS>
 struct Jobs {
-  int tile0, tile_end;  // tiles of the cluster
-  int round;            // first tile of the round
-  int at, end;          // jobs of the round: this warp's [at, end)
+  int round;       // first tile of the round
+  int left;        // jobs of the round still this warp's
+  int tile, jk;    // the next one: tile of the round, job along K
 
-  __device__ __forceinline__ void cut(const Int4Args& a) {
+  __device__ __forceinline__ void cut(const Int4Args& a, int tile_end) {
     const int warp = threadIdx.x >> 5;
     const int total = min(a.tiles_round, tile_end - round) * a.kb;
-    at = warp * total / kWarps;
-    end = (warp + 1) * total / kWarps;
+    const int begin = warp * total / WARPS;
+    left = (warp + 1) * total / WARPS - begin;
+    tile = begin / a.kb;
+    jk = begin - tile * a.kb;
   }
-  // Moves to the next job, over the rounds; false after the last.
-  __device__ __forceinline__ bool settle(const Int4Args& a) {
-    while (at >= end) {
+  // Finds the next job, over the rounds; false after the last.
+  __device__ __forceinline__ bool settle(const Int4Args& a, int tile_end) {
+    while (left == 0) {
       round += a.tiles_round;
-      if (round >= tile_end) return false;
-      cut(a);
+      if (round >= tile_end) {
+        round -= a.tiles_round;
+        return false;
+      }
+      cut(a, tile_end);
     }
     return true;
+  }
+  __device__ __forceinline__ void step(const Int4Args& a) {
+    --left;
+    if (++jk == a.kb) jk = 0, ++tile;
   }
 };
 
 // W: 32-bit words of weights that a lane takes side by side (4 W lanes' words
 // = 32 W of k share a group of g = 32 W).  NT: blocks of 8 columns.
 template <typename T, int NT, int W>
-__global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1) linear_int4_kernel(const __grid_constant__ Int4Args a) {
-  using E = Int4Type<T>;
+__global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(const __grid_constant__ Int4Args a) {
+  constexpr int kWarps = warps_for(NT), kThreads = kWarps * 32;
   constexpr int kSegs = 8 / W;          // groups of a job
   constexpr int kHold = kSegs / 2;      // (scale, zero) pairs a lane holds of a job: two rows' kSegs over four lanes
+  constexpr int kTileFloats = NT * 8 * kPitch;
   extern __shared__ __align__(1024) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, i = lane & 3;
   const bool pair = a.mode == AICAS_LINEAR_SWIGLU;
   const int tile_n = pair ? 8 : 16;     // output features of a tile
   const uint32_t ring = smem_u32(smem) + warp * a.stages * kJobBytes;
   const uint32_t bars = smem_u32(smem + a.off_bars) + warp * a.stages * 8;
-  float* part = reinterpret_cast<float*>(smem + a.off_part);  // [tiles_round tiles][NT * 8][kPitch], then [kWarps] heads
-  float* heads = part + a.tiles_round * NT * 8 * kPitch;
+  float* part = reinterpret_cast<float*>(smem + a.off_part);  // [tiles_round][kTileFloats], then [kWarps] heads
+  float* heads = part + a.tiles_round * kTileFloats;
   uint8_t* xs = smem + a.off_x;
+  float* xsum = reinterpret_cast<float*>(smem + a.off_sum);   // [group of this CTA's K][NT * 8 columns]
   int* s_abort = reinterpret_cast<int*>(smem + a.off_bars + kWarps * a.stages * 8);
-  float* s_rstd = reinterpret_cast<float*>(s_abort + 1);
+  float* s_stat = reinterpret_cast<float*>(s_abort + 16);     // [(row, part), 32 at most][max, sums of squares]
+  float* s_scale = s_stat + 96;                               // [32]
+  float* s_inv = s_scale + 32;                                // [32]
   const int rank = a.s > 1 ? (int)cluster_rank() : 0;
   const int cluster = (int)blockIdx.x / a.s, clusters = (int)gridDim.x / a.s;
   const int kb0 = rank * a.kb;  // this CTA's first job along K
+  const T* nw = static_cast<const T*>(a.norm_weight);
+  const bool split = nw != nullptr && std::is_same<T, __half>::value;  // two parts a row
 
   if (tid == 0) *s_abort = 0;
   if (lane == 0) {
@@ -176,17 +179,17 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1) linear_int4_kernel(
   __syncwarp();
   grid_launch_dependents();
 
-  Jobs ld;
-  ld.tile0 = (int)((int64_t)cluster * a.tiles / clusters);
-  ld.tile_end = (int)((int64_t)(cluster + 1) * a.tiles / clusters);
-  ld.round = ld.tile0;
-  ld.cut(a);
-  Jobs job = ld;
+  const int tile0 = (int)((int64_t)cluster * a.tiles / clusters);
+  const int tile_end = (int)((int64_t)(cluster + 1) * a.tiles / clusters);
+  Jobs<kWarps> ld;
+  ld.round = tile0;
+  ld.cut(a, tile_end);
+  Jobs<kWarps> job = ld;
   // the first weights into L2 (where every earlier write is seen) while the kernel before this one ends
   if (lane == 0) {
-    Jobs pf = ld;
-    for (int s = 0; s < a.stages && pf.settle(a); ++s, ++pf.at) {
-      const int t = pf.round + pf.at / a.kb, x = (kb0 + pf.at % a.kb) * 128;
+    Jobs<kWarps> pf = ld;
+    for (int s = 0; s < a.stages && pf.settle(a, tile_end); ++s, pf.step(a)) {
+      const int t = pf.round + pf.tile, x = (kb0 + pf.jk) * 128;
       tma_prefetch_l2_2d(&a.tm_w[0], x, t * tile_n);
       if (pair) tma_prefetch_l2_2d(&a.tm_w[1], x, t * tile_n);
     }
@@ -195,15 +198,15 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1) linear_int4_kernel(
 
   const uint64_t policy = l2_policy_evict_first();
   const auto issue = [&](int stage) -> int {
-    if (!ld.settle(a)) return 0;
+    if (!ld.settle(a, tile_end)) return 0;
     if (lane == 0) {
-      const int t = ld.round + ld.at / a.kb, x = (kb0 + ld.at % a.kb) * 128;
+      const int t = ld.round + ld.tile, x = (kb0 + ld.jk) * 128;
       const uint32_t dst = ring + stage * kJobBytes, bar = bars + 8 * stage;
       mbar_arrive_expect_tx(bar, kJobBytes);
       tma_load_2d_hint(dst, &a.tm_w[0], x, t * tile_n, bar, policy);
       if (pair) tma_load_2d_hint(dst + 1024, &a.tm_w[1], x, t * tile_n, bar, policy);
     }
-    ++ld.at;
+    ld.step(a);
     return 1;
   };
   int flying = 0;
@@ -211,26 +214,29 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1) linear_int4_kernel(
   for (int s = 0; s < a.stages; ++s) flying += issue(s);
 
   // ---- (scale, zero) of a job: lane i of a row's four holds rows g + 8 (i / 2), groups (i % 2) kHold ..
-  Jobs sj = job;  // next job whose scales are fetched
+  Jobs<kWarps> sj = job;  // next job whose scales are fetched
   const int my_row = tile_row(g), hi_row = i >> 1;
+  const uint8_t* const my_zeros = pair && hi_row ? a.zeros[1] : a.zeros[0];
+  const uint16_t* const my_scales = static_cast<const uint16_t*>(pair && hi_row ? a.scales[1] : a.scales[0]);
+  const int n_off = my_row + (pair ? 0 : 8 * hi_row);
   const auto fetch = [&](uint32_t (&v)[kHold]) {
 #pragma unroll
-    for (int j = 0; j < kHold; ++j) v[j] = E::kMagic << 16;
-    if (!sj.settle(a)) return;
-    const int t = sj.round + sj.at / a.kb, jk = kb0 + sj.at % a.kb;
-    const int n = t * tile_n + my_row + (pair ? 0 : 8 * hi_row);
-    const bool up = pair && hi_row;
-    const uint8_t* zeros = up ? a.zeros[1] : a.zeros[0];
-    const uint16_t* scales = static_cast<const uint16_t*>(up ? a.scales[1] : a.scales[0]);
-    ++sj.at;
+    for (int j = 0; j < kHold; ++j) v[j] = 0u;
+    if (!sj.settle(a, tile_end)) return;
+    const int n = (sj.round + sj.tile) * tile_n + n_off, grp0 = (kb0 + sj.jk) * kSegs + (i & 1) * kHold;
+    sj.step(a);
     if (n >= a.n) return;
+    const int64_t at = (int64_t)n * a.groups + grp0;
 #pragma unroll
     for (int j = 0; j < kHold; ++j) {
-      const int grp = jk * kSegs + (i & 1) * kHold + j;
-      if (grp >= a.groups) continue;
-      const int64_t at = (int64_t)n * a.groups + grp;
-      const uint32_t z = zeros != nullptr ? zeros[at] : 8u;
-      v[j] = scales[at] | (E::kMagic | z) << 16;
+      if (grp0 + j >= a.groups) continue;
+      const float z = my_zeros != nullptr ? (float)my_zeros[at + j] : 8.f;
+      union {
+        T t;
+        uint16_t u;
+      } zb;
+      zb.t = Elem<T>::from_float(z);  // 0..15: exact
+      v[j] = my_scales[at + j] | (uint32_t)zb.u << 16;
     }
   };
   uint32_t sz0[kHold], sz1[kHold], sz2[kHold];
@@ -238,63 +244,121 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1) linear_int4_kernel(
   fetch(sz1);
   fetch(sz2);
 
-  // ---- x' into shared memory, in the order in which the products take it
+  // ---- rows' largest element (of this CTA's K) and sum of squares (of all K)
   const T* x = static_cast<const T*>(a.x);
-  const T* nw = static_cast<const T*>(a.norm_weight);
-  if (nw != nullptr) {
-    for (int r = warp; r < a.rows; r += kWarps) {
-      float ss = 0.f;
-      for (int v = lane; v < a.k / 8; v += 32) {
-        float f[8];
-        Elem<T>::unpack(*reinterpret_cast<const uint4*>(x + r * a.x_stride + 8 * v), f);
+  constexpr int kFly = NT <= 2 ? 4 : 8;  // vectors in flight a thread
+  const int parts = a.rows >= kWarps ? 1 : kWarps / a.rows;  // warps a row
+  const int vec0 = kb0 * (kJobK / 8), vecs = a.kb * (kJobK / 8), all_vecs = a.k / 8;
+  for (int u = warp; u < a.rows * parts; u += kWarps) {
+    const int r = u / parts, first = (u - r * parts) * 32 + lane;
+    const uint4* row = reinterpret_cast<const uint4*>(x + r * a.x_stride);
+    const int lo = nw != nullptr ? 0 : vec0, hi = nw != nullptr ? all_vecs : min(vec0 + vecs, all_vecs);
+    float ss = 0.f, far = 0.f, top = 0.f;  // far: of elements times 2^-70, where squares pass fp32's range
+    for (int v0 = lo + first; v0 < hi; v0 += kFly * parts * 32) {
+      uint4 q[kFly], wq[kFly];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss);
+      for (int j = 0; j < kFly; ++j) {
+        const int v = v0 + j * parts * 32;
+        q[j] = wq[j] = make_uint4(0, 0, 0, 0);
+        if (v < hi) {
+          q[j] = row[v];
+          if (nw != nullptr) wq[j] = reinterpret_cast<const uint4*>(nw)[v];
+        }
       }
 #pragma unroll
-      for (int off = 16; off >= 1; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-      if (lane == 0) s_rstd[r] = rsqrtf(ss / (float)a.k + a.eps);
-    }
-    __syncthreads();
-  }
-  const int vecs = a.kb * 32;
-  for (int at = tid; at < a.rows * vecs; at += kThreads) {
-    const int r = at / vecs, v = at - r * vecs;
-    const int k = kb0 * kJobK + 8 * v;
-    uint4 u = make_uint4(0, 0, 0, 0), lo = u;
-    if (k < a.k) {
-      u = *reinterpret_cast<const uint4*>(x + r * a.x_stride + k);
-      if (nw != nullptr) {
+      for (int j = 0; j < kFly; ++j) {
+        const int v = v0 + j * parts * 32;
         float f[8], w[8];
-        Elem<T>::unpack(u, f);
-        Elem<T>::unpack(*reinterpret_cast<const uint4*>(nw + k), w);
-        union {
-          T t[8];
-          uint4 u;
-        } h, l;
-        const float rstd = s_rstd[r];
+        Elem<T>::unpack(q[j], f);
+        Elem<T>::unpack(wq[j], w);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float y = f[e] * rstd * w[e];
-          h.t[e] = Elem<T>::from_float(y);
-          l.t[e] = Elem<T>::from_float(y - Elem<T>::to_float(h.t[e]));
+          ss = fmaf(f[e], f[e], ss);
+          const float small = f[e] * 8.470329472543003e-22f;
+          far = fmaf(small, small, far);
+          if (nw != nullptr) f[e] *= w[e];
+          if (v >= vec0 && v < vec0 + vecs) top = fmaxf(top, fabsf(f[e]));
         }
-        u = h.u;
-        lo = l.u;
       }
     }
-    const int wd = v & 31, rem = wd % (4 * W);
-    const int step = (v >> 5) * 8 + wd / (4 * W) * W + rem % W, li = rem / W;
-    // pairs (k0, k4), (k1, k5), (k2, k6), (k3, k7)
-    const auto put = [&](int col, const uint4& d) {
-      *reinterpret_cast<uint4*>(xs + ((step * NT + (col >> 3)) * 32 + (col & 7) * 4 + li) * 16) =
-          make_uint4(__byte_perm(d.x, d.z, 0x5410), __byte_perm(d.x, d.z, 0x7632), __byte_perm(d.y, d.w, 0x5410),
-                     __byte_perm(d.y, d.w, 0x7632));
-    };
-    if (nw != nullptr) {
-      put(2 * r, u);
-      put(2 * r + 1, lo);
-    } else {
-      put(r, u);
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) {
+      ss += __shfl_xor_sync(0xffffffffu, ss, off);
+      far += __shfl_xor_sync(0xffffffffu, far, off);
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    }
+    if (lane == 0) s_stat[3 * u] = top, s_stat[3 * u + 1] = ss, s_stat[3 * u + 2] = far;
+  }
+  __syncthreads();
+  if (tid < a.rows) {
+    float ss = 0.f, far = 0.f, top = 0.f;
+    for (int u = tid * parts; u < (tid + 1) * parts; ++u)
+      top = fmaxf(top, s_stat[3 * u]), ss += s_stat[3 * u + 1], far += s_stat[3 * u + 2];
+    float rstd = 1.f;
+    if (nw != nullptr)
+      rstd = ss < INFINITY ? rsqrtf(ss / (float)a.k + a.eps) : rsqrtf(far / (float)a.k) * 8.470329472543003e-22f;
+    // 2^e that brings the largest element to [2^9, 2^10); 1 for a row of zeros or one with inf
+    const uint32_t bits = __float_as_uint(top * rstd) >> 23;
+    const int e = bits == 0u || bits >= 255u ? 0 : min(136 - (int)bits, 100);
+    s_scale[tid] = rstd * __uint_as_float((uint32_t)(127 + e) << 23);
+    s_inv[tid] = __uint_as_float((uint32_t)(127 - e) << 23);
+  }
+  __syncthreads();
+
+  // ---- x' into shared memory, in the order in which the products take it
+  for (int at0 = tid; at0 < a.rows * vecs; at0 += kFly * kThreads) {
+    uint4 q[kFly], wq[kFly];
+#pragma unroll
+    for (int j = 0; j < kFly; ++j) {
+      const int at = at0 + j * kThreads, r = at / vecs, v = vec0 + at - r * vecs;
+      q[j] = wq[j] = make_uint4(0, 0, 0, 0);
+      if (r < a.rows && v < all_vecs) {
+        q[j] = reinterpret_cast<const uint4*>(x + r * a.x_stride)[v];
+        if (nw != nullptr) wq[j] = reinterpret_cast<const uint4*>(nw)[v];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kFly; ++j) {
+      const int at = at0 + j * kThreads, r = at / vecs, v = at - r * vecs;
+      if (r >= a.rows) break;  // whole warps: vecs is a multiple of 32
+      float f[8], w[8], lo[8], sum = 0.f, low_sum = 0.f;
+      Elem<T>::unpack(q[j], f);
+      Elem<T>::unpack(wq[j], w);
+      const float scale = s_scale[r];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = (nw != nullptr ? f[e] * w[e] : f[e]) * scale;
+        f[e] = __half2float(__float2half_rn(y));
+        lo[e] = split ? __half2float(__float2half_rn(y - f[e])) : 0.f;
+        sum += f[e];
+        low_sum += lo[e];
+      }
+      const int wd = v & 31, rem = wd % (4 * W);
+      const int step = (v >> 5) * 8 + wd / (4 * W) * W + rem % W, li = rem / W;
+      // pairs (k0, k4), (k1, k5) / 16, (k2, k6), (k3, k7) / 16
+      const auto put = [&](int col, const float* y) {
+        union {
+          __half2 h[4];
+          uint4 u;
+        } d;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          d.h[e] = __floats2half2_rn(y[e] * (e & 1 ? 0.0625f : 1.f), y[e + 4] * (e & 1 ? 0.0625f : 1.f));
+        *reinterpret_cast<uint4*>(xs + ((step * NT + (col >> 3)) * 32 + (col & 7) * 4 + li) * 16) = d.u;
+      };
+      put(split ? 2 * r : r, f);
+      if (split) put(2 * r + 1, lo);
+      // the group's sum: 4 W neighbouring lanes hold it
+#pragma unroll
+      for (int off = 2 * W; off >= 1; off >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        low_sum += __shfl_xor_sync(0xffffffffu, low_sum, off);
+      }
+      if (rem == 0) {
+        float* d = xsum + (v / (4 * W)) * NT * 8 + (split ? 2 * r : r);
+        d[0] = sum * 5.9604644775390625e-8f;  // 2^-24, as the weights
+        if (split) d[1] = low_sum * 5.9604644775390625e-8f;
+      }
     }
   }
   __syncthreads();
@@ -304,12 +368,12 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1) linear_int4_kernel(
   uint32_t phase = 0;
   bool bad = false;
   for (;;) {
-    const int first = job.at;
     float tot[NT][4];
+    bool head = job.jk != 0;  // a tile begun by an earlier warp is this warp's head; its own tiles have a place each
+    bool fresh = true;
 #pragma unroll 1
-    for (; job.at < job.end; ++job.at) {
-      const int tile = job.at / a.kb, jk = job.at - tile * a.kb;
-      if (job.at == first || jk == 0) {
+    while (job.left > 0) {
+      if (fresh) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -318,12 +382,12 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1) linear_int4_kernel(
       if (!bad && !mbar_wait(bars + 8 * stage, phase, s_abort, a.err)) bad = true;  // computes no more, keeps to the barriers
       if (!bad) {
         const uint32_t wrow = ring + stage * kJobBytes + my_row * 128;
-        const uint8_t* xf = xs + (size_t)(jk * 8 * NT * 32 + lane) * 16;
+        const uint8_t* xf = xs + (size_t)(job.jk * 8 * NT * 32 + lane) * 16;
+        const float* gs = xsum + job.jk * kSegs * NT * 8 + 2 * i;
 #pragma unroll
         for (int seg = 0; seg < kSegs; ++seg) {
           const uint32_t s_lo = __shfl_sync(0xffffffffu, sz0[seg % kHold], (lane & ~3) | seg / kHold);
           const uint32_t s_hi = __shfl_sync(0xffffffffu, sz0[seg % kHold], (lane & ~3) | 2 | seg / kHold);
-          const uint32_t z_lo = __byte_perm(s_lo, 0, 0x3232), z_hi = __byte_perm(s_hi, 0, 0x3232);
           // this lane's W words of rows my_row and my_row + 8
           uint32_t w0[4], w1[4];
           {
@@ -345,24 +409,23 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1) linear_int4_kernel(
           float acc[NT][4] = {};
 #pragma unroll
           for (int w = 0; w < W; ++w) {
-            uint32_t q0[4], q1[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              q0[j] = E::sub(((w0[w] >> (4 * j)) & 0x000f000fu) | E::kMagic * 0x10001u, z_lo);
-              q1[j] = E::sub(((w1[w] >> (4 * j)) & 0x000f000fu) | E::kMagic * 0x10001u, z_hi);
-            }
+            const uint32_t lo8 = w0[w] >> 8, hi8 = w1[w] >> 8;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               const uint4 b = *reinterpret_cast<const uint4*>(xf + ((seg * W + w) * NT + n) * 512);
-              E::mma(acc[n], q0[0], q1[0], q0[1], q1[1], b.x, b.y);
-              E::mma(acc[n], q0[2], q1[2], q0[3], q1[3], b.z, b.w);
+              mma_f16(acc[n], w0[w] & 0x000f000fu, w1[w] & 0x000f000fu, w0[w] & 0x00f000f0u, w1[w] & 0x00f000f0u, b.x, b.y);
+              mma_f16(acc[n], lo8 & 0x000f000fu, hi8 & 0x000f000fu, lo8 & 0x00f000f0u, hi8 & 0x00f000f0u, b.z, b.w);
             }
           }
-          const float f_lo = low_half<T>(s_lo), f_hi = low_half<T>(s_hi);
+          const float f_lo = low_half<T>(s_lo) * 16777216.f, f_hi = low_half<T>(s_hi) * 16777216.f;  // the weights' 2^24
+          const float z_lo = low_half<T>(s_lo >> 16), z_hi = low_half<T>(s_hi >> 16);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            tot[n][0] = fmaf(f_lo, acc[n][0], tot[n][0]), tot[n][1] = fmaf(f_lo, acc[n][1], tot[n][1]);
-            tot[n][2] = fmaf(f_hi, acc[n][2], tot[n][2]), tot[n][3] = fmaf(f_hi, acc[n][3], tot[n][3]);
+            const float2 xg = *reinterpret_cast<const float2*>(gs + (seg * NT + n) * 8);
+            tot[n][0] = fmaf(f_lo, fmaf(-z_lo, xg.x, acc[n][0]), tot[n][0]);
+            tot[n][1] = fmaf(f_lo, fmaf(-z_lo, xg.y, acc[n][1]), tot[n][1]);
+            tot[n][2] = fmaf(f_hi, fmaf(-z_hi, xg.x, acc[n][2]), tot[n][2]);
+            tot[n][3] = fmaf(f_hi, fmaf(-z_hi, xg.y, acc[n][3]), tot[n][3]);
           }
         }
         __syncwarp();  // every lane has read the stage
@@ -372,10 +435,12 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1) linear_int4_kernel(
         for (int j = 0; j < kHold; ++j) sz0[j] = sz1[j], sz1[j] = sz2[j];
         fetch(sz2);
       }
-      if (jk == a.kb - 1 || job.at == job.end - 1) {
-        // a tile begun by an earlier warp is this warp's head; its own tiles have a place each
-        const bool head = job.at - jk < first;
-        float* dst = (head ? heads + warp * NT * 8 * kPitch : part + tile * NT * 8 * kPitch) + my_row;
+      const int tile = job.tile;
+      job.step(a);
+      fresh = job.jk == 0;
+      if (fresh || job.left == 0) {
+        float* dst = (head ? heads + warp * kTileFloats : part + tile * kTileFloats) + my_row;
+        head = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           dst[(8 * n + 2 * i) * kPitch] = tot[n][0], dst[(8 * n + 2 * i + 1) * kPitch] = tot[n][1];
@@ -386,31 +451,41 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1) linear_int4_kernel(
     if (a.s > 1) cluster_sync_all(); else __syncthreads();
 
     // ---- the round's outputs: partial tiles of the warps and CTAs added in their order
-    const int tiles = min(a.tiles_round, job.tile_end - job.round), total_jobs = tiles * a.kb;
+    const int tiles = min(a.tiles_round, tile_end - job.round), total_jobs = tiles * a.kb;
     const int n0 = job.round * tile_n, width = min(tiles * tile_n, a.n - n0);
-    const uint32_t part_at = smem_u32(part), heads_at = smem_u32(heads);
     for (int at = rank * kThreads + tid; at < width * a.rows; at += a.s * kThreads) {
       const int r = at / width, c = at - r * width, tile = c / tile_n, row = c - tile * tile_n;
-      const int col = nw != nullptr ? 2 * r : r;
+      const int place = (split ? 2 * r : r) * kPitch + row;
+      // warps that hold a head of this tile: those whose first job lies inside it
+      int w0 = (tile * a.kb + 1) * kWarps / total_jobs;  // no smaller w begins after the tile's first job
       float y[2] = {0.f, 0.f};
-      for (int q = 0; q < a.s; ++q) {
-        const auto add = [&](uint32_t base) {
-          // the low parts of a normalised x' are the next column; up's rows come 8 after gate's
+      const auto add = [&](int where) {
+        float v[2][2][8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          if (q >= a.s) break;
 #pragma unroll
           for (int m = 0; m < 2; ++m)
-            if (m == 0 || pair) {
-              const uint32_t p = base + (col * kPitch + row + 8 * m) * 4;
-              y[m] += a.s > 1 ? ld_cluster(p, q) : *reinterpret_cast<const float*>(smem + (p - smem_u32(smem)));
-              if (nw != nullptr)
-                y[m] += a.s > 1 ? ld_cluster(p + kPitch * 4, q)
-                                : *reinterpret_cast<const float*>(smem + (p + kPitch * 4 - smem_u32(smem)));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              v[m][h][q] = 0.f;
+              if ((m == 1 && !pair) || (h == 1 && !split)) continue;
+              const float* p = part + where + place + 8 * m + h * kPitch;
+              v[m][h][q] = a.s > 1 ? ld_cluster(smem_u32(p), q) * ld_cluster(smem_u32(s_inv + r), q) : *p * s_inv[r];
             }
-        };
-        add(part_at + tile * NT * 8 * kPitch * 4);
-        for (int w = 1; w < kWarps; ++w) {
-          const int begin = w * total_jobs / kWarps, end = (w + 1) * total_jobs / kWarps;
-          if (begin < end && begin > tile * a.kb && begin < (tile + 1) * a.kb) add(heads_at + w * NT * 8 * kPitch * 4);
         }
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          if (q >= a.s) break;
+          y[0] += v[0][0][q] + v[0][1][q];
+          y[1] += v[1][0][q] + v[1][1][q];
+        }
+      };
+      add(tile * kTileFloats);
+      for (int w = w0; w < kWarps; ++w) {
+        const int begin = w * total_jobs / kWarps;
+        if (begin >= (tile + 1) * a.kb) break;
+        if (begin > tile * a.kb && begin < (w + 1) * total_jobs / kWarps) add((a.tiles_round + w) * kTileFloats);
       }
       float v = y[0];
       if (pair) v = v / (1.f + expf(-v)) * y[1];
@@ -419,8 +494,8 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1) linear_int4_kernel(
       static_cast<T*>(a.out)[r * a.out_stride + n0 + c] = Elem<T>::from_float(v);
     }
     job.round += a.tiles_round;
-    if (job.round >= job.tile_end) break;
-    job.cut(a);
+    if (job.round >= tile_end) break;
+    job.cut(a, tile_end);
     if (a.s > 1) cluster_sync_all(); else __syncthreads();  // the partial tiles have been read
   }
   if (bad)
@@ -457,7 +532,7 @@ int log2_of(int v) { return v <= 1 ? 0 : 1 + log2_of(v / 2); }
 template <typename T, int NT, int W>
 cudaError_t launch_int4(Int4Args a, int smem, int sms, cudaStream_t st) {
   static bool attr_set[64] = {false};
-  static int max_clusters[64][4][2] = {};  // by device, cluster size and CTAs an SM
+  static int max_clusters[64][4] = {};  // by device and cluster size
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
@@ -467,8 +542,7 @@ cudaError_t launch_int4(Int4Args a, int smem, int sms, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     if (known) attr_set[dev] = true;
   }
-  const bool two = smem <= kTwoPerSm;
-  int clusters = sms * (two ? 2 : 1);
+  int clusters = sms;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -477,13 +551,13 @@ cudaError_t launch_int4(Int4Args a, int smem, int sms, cudaStream_t st) {
   attr[1].val.clusterDim.x = (unsigned)a.s;
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(warps_for(NT) * 32);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = a.s > 1 ? 2 : 1;
   if (a.s > 1) {
-    int* cached = known ? &max_clusters[dev][log2_of(a.s)][two] : nullptr;
+    int* cached = known ? &max_clusters[dev][log2_of(a.s)] : nullptr;
     if (cached != nullptr && *cached > 0) {
       clusters = *cached;
     } else {
@@ -520,8 +594,9 @@ cudaError_t dispatch_int4(int nt, int group, const Int4Args& a, int smem, int sm
     case 1: return dispatch_group<T, 1>(group, a, smem, sms, st);
     case 2: return dispatch_group<T, 2>(group, a, smem, sms, st);
     case 4: return dispatch_group<T, 4>(group, a, smem, sms, st);
-    case 8: return dispatch_group<T, 8>(group, a, smem, sms, st);
   }
+  if constexpr (std::is_same<T, __half>::value)  // 32 rows in two parts
+    if (nt == 8) return dispatch_group<T, 8>(group, a, smem, sms, st);
   return cudaErrorInvalidValue;
 }
 
@@ -531,15 +606,17 @@ int plan_int4(Int4Args* a, int nt, int s) {
   a->s = s;
   a->kb = (jobs + s - 1) / s;
   a->tiles_round = nt == 1 ? 16 : nt == 2 ? 8 : 4;
-  const int part = (a->tiles_round + kWarps) * nt * 8 * kPitch * 4, xs = a->kb * nt * 4096, tail = 2048;
-  const int rest = part + xs + tail, ring = kWarps * kJobBytes;
-  a->stages = (kTwoPerSm - rest) / ring;  // two CTAs an SM, if their rings hold four jobs a warp
-  if (a->stages < 4) a->stages = (kMaxSmem - rest) / ring;
+  const int warps = warps_for(nt);
+  const int part = (a->tiles_round + warps) * nt * 8 * kPitch * 4, xs = a->kb * nt * 4096;
+  const int sums = a->kb * (kJobK / (a->k / a->groups)) * nt * 32;
+  const int tail = warps * 8 * 8 + kVarBytes, rest = part + xs + sums + tail, ring = warps * kJobBytes;
+  a->stages = (kMaxSmem - rest) / ring;
   if (a->stages < 3) return 0;
   if (a->stages > 8) a->stages = 8;
   a->off_part = a->stages * ring;
   a->off_x = a->off_part + part;
-  a->off_bars = a->off_x + xs;
+  a->off_sum = a->off_x + xs;
+  a->off_bars = a->off_sum + sums;
   return a->off_bars + tail;
 }
 
@@ -562,8 +639,8 @@ int run_linear_int4(const aicas_linear_int4_params* p, int sms, cudaStream_t str
   a.mode = p->mode, a.eps = p->eps, a.err = dev_err;
   const int tile_n = pair ? 8 : 16;
   a.tiles = (p->out_features + tile_n - 1) / tile_n;
-  // every row at once where x' fits on chip over a cluster of up to 8 CTAs (K up to 14336 for 32 rows), else fewer
-  const int columns = p->norm_weight != nullptr ? 2 : 1;
+  // every row at once where x' fits on chip over a cluster of up to 8 CTAs, else fewer rows a launch
+  const int columns = p->norm_weight != nullptr && !bf16 ? 2 : 1;  // a normalised x' for an fp16 result: two parts
   int batch = p->rows, nt = 0, smem = 0;
   for (;; batch = (batch + 1) / 2) {
     const int blocks = (batch * columns + 7) / 8;

@@ -20,14 +20,17 @@ def norm_rows(x: np.ndarray, weight: np.ndarray, eps: float) -> np.ndarray:
     return y / np.sqrt((y * y).mean(axis=-1, keepdims=True) + eps) * weight.astype(np.float64)
 
 
-def linear(x, weights, *, norm_weight=None, eps=1e-6, residual=None, swiglu=False):
-    """(y, bound): the product before its one rounding, and a bound of what fp32
-    sums may be off: every sum of K terms, in whatever order, within 2^-15 of the
-    sum of the terms' magnitudes (chains of up to 512 additions of relative error
-    2^-24; a normalised x in two 16-bit parts is within 2^-16 of itself)."""
+def linear(x, weights, *, norm_weight=None, eps=1e-6, residual=None, swiglu=False, dtype="bf16"):
+    """(y, bound): the product before its one rounding, and a bound of what it may
+    be off before that.  fp32 sums of K terms, in whatever order: within 2^-15 of
+    the sum of the terms' magnitudes (chains of up to 512 additions of relative
+    error 2^-24, of terms up to 16 times larger while the zero point is still in).
+    A normalised x for a bf16 result is rounded to 11 bits: within 2^-11 of itself;
+    for an fp16 result it has two such parts, within 2^-22."""
     xd = norm_rows(x, norm_weight, eps) if norm_weight is not None else np.asarray(x, np.float64)
     ys = [xd @ w.T for w in weights]
-    offs = [2.0 ** -15 * (np.abs(xd) @ np.abs(w).T) for w in weights]
+    rel = 2.0 ** -15 + (2.0 ** -11 if norm_weight is not None and dtype == "bf16" else 0.0)
+    offs = [rel * (np.abs(xd) @ np.abs(w).T) for w in weights]
     if swiglu:
         s = ys[0] / (1.0 + np.exp(-ys[0]))
         # |silu'| <= 1.1

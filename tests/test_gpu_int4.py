@@ -41,7 +41,8 @@ def _case(device, rows, k, n, group=128, dtype="bf16", zeros=False, norm=False, 
     res = torch.randn(rows, n, generator=g).to(DT[dtype]).to(device) if residual else None
     y = ab.decode_linear_int4(x, w if swiglu else w[0], norm_weight=nw, residual=res, swiglu=swiglu)
     assert y.shape == (rows, n) and y.dtype == x.dtype
-    ref, off = oi.linear(_np(x), [_wide(v) for v in w], norm_weight=_np(nw), residual=_np(res), swiglu=swiglu)
+    ref, off = oi.linear(_np(x), [_wide(v) for v in w], norm_weight=_np(nw), residual=_np(res), swiglu=swiglu,
+                         dtype=dtype)
     over = np.abs(_np(y).astype(np.float64) - ref) - (HALF_ULP[dtype] * (np.abs(ref) + off) + off)
     assert over.max() <= 2.0 ** -24, f"{over.max():.3e} over the bound at {np.unravel_index(over.argmax(), over.shape)}"
     assert nat.device_error_flags() == 0
@@ -68,6 +69,34 @@ def test_odd_sizes(cuda_device, k, group, n):
 def test_prologue_and_epilogues(cuda_device, rows, zeros, kind):
     _case(cuda_device, rows, 512, 333, 64, zeros=zeros, norm="norm" in kind, residual="residual" in kind,
           swiglu="swiglu" in kind, seed=rows)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_norm_of_many_rows(cuda_device, dtype):
+    _case(cuda_device, 32, 1536, 90, 64, dtype, zeros=True, norm=True, residual=True)
+    _case(cuda_device, 27, 8192, 40, 128, dtype, norm=True)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("norm", [False, True])
+def test_rows_of_every_size(cuda_device, dtype, norm):
+    """Rows of any magnitude the type has, zeros and single large elements, in one batch."""
+    g = torch.Generator().manual_seed(12)
+    k, top = 512, 1e36 if dtype == "bf16" else 2e3
+    size = torch.tensor([1.0, top / 30, 1e-3 if dtype == "fp16" else 1e-30, 0.0, 37.0, 1e-2, 1.0, 5.0])
+    x = (torch.randn(8, k, generator=g) * size[:, None]).to(DT[dtype])
+    x[6, 100] = top  # one element far above the others
+    x = x.to(cuda_device)
+    w = _weight(g, 64, k, 64, dtype, True, cuda_device)
+    nw = torch.ones(k, dtype=DT[dtype], device=cuda_device) if norm else None
+    y = ab.decode_linear_int4(x, w, norm_weight=nw, eps=1e-6 if norm else 0.0)
+    ref, off = oi.linear(_np(x), [_wide(w)], norm_weight=_np(nw), dtype=dtype)
+    # elements 2^30 below their row's largest may lose bits: 2^-34 of the largest, K times
+    xd = oi.norm_rows(_np(x), _np(nw), 1e-6) if norm else _np(x).astype(np.float64)
+    off = off + 2.0 ** -34 * k * np.abs(xd).max(1, keepdims=True) * np.abs(_wide(w)).max()
+    off = off + (2.0 ** -25 if dtype == "fp16" else 0.0)
+    assert np.all(np.abs(_np(y).astype(np.float64) - ref) <= HALF_ULP[dtype] * (np.abs(ref) + off) + off)
+    assert (y[3] == 0).all()
 
 
 @pytest.mark.parametrize("rows,k,n", [(1, 2048, 4096), (8, 2048, 6144), (32, 6144, 2048), (1, 2048, 40000),
