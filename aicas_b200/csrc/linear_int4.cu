@@ -46,11 +46,14 @@ constexpr int kJobK = 256;              // k of a job: 128 bytes of a row
 constexpr int kJobBytes = 16 * 128;     // 16 rows
 constexpr int kPitch = 20;              // floats a column of a partial tile (16 rows; 20 keeps stores conflict free)
 constexpr int kMaxSmem = 232448;
-constexpr int kVarBytes = 64 + 4 * 160;  // abort flag; rows' statistics, scales and their inverses
+
+constexpr int kMaxRound = 80;           // tiles of a round
+constexpr int kEntries = 128;           // rows' statistics: (largest element, sum of squares) of 256 k each
+constexpr int kVarBytes = 64 + kEntries * 8 + 2 * 32 * 4 + kMaxRound * 4;
 
 // Warps of a CTA: more of them hide the products' latency, fewer leave shared
 // memory for the columns of many rows.
-constexpr int warps_for(int nt) { return nt <= 2 ? 16 : 8; }
+constexpr int warps_for(int nt) { return nt <= 4 ? 16 : 8; }
 
 struct Int4Args {
   CUtensorMap tm_w[2];
@@ -67,6 +70,7 @@ struct Int4Args {
   int s;                   // CTAs of a cluster
   int kb;                  // jobs of a tile for each of them
   int tiles, tiles_round;  // 16-row tiles of the launch; tiles of a round
+  int tiles_each, tiles_more;  // tiles of a cluster; the first tiles_more clusters take one more
   int stages;
   int off_part, off_x, off_sum, off_bars;
   unsigned int* err;
@@ -143,6 +147,31 @@ struct Jobs {
   }
 };
 
+// Largest |x * w| over the vectors in [lo, hi) of those first, first + 32, .. below
+// end, and the sum of squares of x * by over all of them, over the warp.  w: ones where null.
+template <typename T>
+__device__ __noinline__ float2 row_stats(const T* row, const T* w, int first, int end, int lo, int hi, float by) {
+  float top = 0.f, ss = 0.f;
+#pragma unroll 4
+  for (int v = first; v < end; v += 32) {
+    float f[8], g[8];
+    Elem<T>::unpack(reinterpret_cast<const uint4*>(row)[v], f);
+    if (w != nullptr) Elem<T>::unpack(reinterpret_cast<const uint4*>(w)[v], g);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float y = f[e] * by;
+      ss = fmaf(y, y, ss);
+      if (v >= lo && v < hi) top = fmaxf(top, fabsf(w != nullptr ? f[e] * g[e] : f[e]));
+    }
+  }
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) {
+    ss += __shfl_xor_sync(0xffffffffu, ss, off);
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+  }
+  return make_float2(top, ss);
+}
+
 // W: 32-bit words of weights that a lane takes side by side (4 W lanes' words
 // = 32 W of k share a group of g = 32 W).  NT: blocks of 8 columns.
 template <typename T, int NT, int W>
@@ -151,6 +180,7 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
   constexpr int kSegs = 8 / W;          // groups of a job
   constexpr int kHold = kSegs / 2;      // (scale, zero) pairs a lane holds of a job: two rows' kSegs over four lanes
   constexpr int kTileFloats = NT * 8 * kPitch;
+  constexpr int kFly = NT <= 2 ? 4 : 8; // vectors of x a thread holds at once
   extern __shared__ __align__(1024) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, i = lane & 3;
   const bool pair = a.mode == AICAS_LINEAR_SWIGLU;
@@ -158,209 +188,270 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
   const uint32_t ring = smem_u32(smem) + warp * a.stages * kJobBytes;
   const uint32_t bars = smem_u32(smem + a.off_bars) + warp * a.stages * 8;
   float* part = reinterpret_cast<float*>(smem + a.off_part);  // [tiles_round][kTileFloats], then [kWarps] heads
-  float* heads = part + a.tiles_round * kTileFloats;
   uint8_t* xs = smem + a.off_x;
   float* xsum = reinterpret_cast<float*>(smem + a.off_sum);   // [group of this CTA's K][NT * 8 columns]
   int* s_abort = reinterpret_cast<int*>(smem + a.off_bars + kWarps * a.stages * 8);
-  float* s_stat = reinterpret_cast<float*>(s_abort + 16);     // [(row, part), 32 at most][max, sums of squares]
-  float* s_scale = s_stat + 96;                               // [32]
+  float2* s_stat = reinterpret_cast<float2*>(s_abort + 16);   // [kEntries]
+  float* s_scale = reinterpret_cast<float*>(s_stat + kEntries);  // [32]
   float* s_inv = s_scale + 32;                                // [32]
+  int* s_heads = reinterpret_cast<int*>(s_inv + 32);          // [tile of the round] the warps after the tile's first
   const int rank = a.s > 1 ? (int)cluster_rank() : 0;
-  const int cluster = (int)blockIdx.x / a.s, clusters = (int)gridDim.x / a.s;
+  const int cluster = (int)blockIdx.x / a.s;
   const int kb0 = rank * a.kb;  // this CTA's first job along K
   const T* nw = static_cast<const T*>(a.norm_weight);
   const bool split = nw != nullptr && std::is_same<T, __half>::value;  // two parts a row
 
   if (tid == 0) *s_abort = 0;
-  if (lane == 0) {
-    for (int s = 0; s < a.stages; ++s) mbar_init(bars + 8 * s, 1);
-    fence_mbar_init();
-  }
-  __syncwarp();
+  if (lane < a.stages) mbar_init(bars + 8 * lane, 1);
   grid_launch_dependents();
 
-  const int tile0 = (int)((int64_t)cluster * a.tiles / clusters);
-  const int tile_end = (int)((int64_t)(cluster + 1) * a.tiles / clusters);
-  Jobs<kWarps> ld;
-  ld.round = tile0;
-  ld.cut(a, tile_end);
-  Jobs<kWarps> job = ld;
-  // the first weights into L2 (where every earlier write is seen) while the kernel before this one ends
-  if (lane == 0) {
-    Jobs<kWarps> pf = ld;
-    for (int s = 0; s < a.stages && pf.settle(a, tile_end); ++s, pf.step(a)) {
-      const int t = pf.round + pf.tile, x = (kb0 + pf.jk) * 128;
-      tma_prefetch_l2_2d(&a.tm_w[0], x, t * tile_n);
-      if (pair) tma_prefetch_l2_2d(&a.tm_w[1], x, t * tile_n);
-    }
+  const int tile0 = cluster * a.tiles_each + min(cluster, a.tiles_more);
+  const int tile_end = tile0 + a.tiles_each + (cluster < a.tiles_more ? 1 : 0);
+  Jobs<kWarps> job;
+  job.round = tile0;
+  job.cut(a, tile_end);
+  // the ring's first jobs, a lane each
+  Jobs<kWarps> mine = job;
+  const bool fill = lane < min(a.stages, job.left);
+  mine.jk += lane;
+  while (mine.jk >= a.kb) mine.jk -= a.kb, ++mine.tile;
+  const int fill_x = (kb0 + mine.jk) * 128, fill_n = (mine.round + mine.tile) * tile_n;
+  if (fill) {
+    // into L2 (where every earlier write is seen) while the kernel before this one ends
+    tma_prefetch_l2_2d(&a.tm_w[0], fill_x, fill_n);
+    if (pair) tma_prefetch_l2_2d(&a.tm_w[1], fill_x, fill_n);
   }
+  fence_mbar_init();
+  __syncwarp();
   grid_dependency_wait();
 
+  // ---- x: this thread's vectors of the CTA's share of K, ahead of the weights
+  const T* x = static_cast<const T*>(a.x);
+  const int vec0 = kb0 * (kJobK / 8), vecs = a.kb * (kJobK / 8), all_vecs = a.k / 8;
+  // at once, where they fit and nothing else of the rows is needed; else in passes
+  const bool once = a.rows * vecs <= kFly * kThreads && (nw == nullptr || a.s == 1);
+  uint4 xq[kFly], wq[kFly];
+  int xr[kFly];
+  if (once) {
+#pragma unroll
+    for (int j = 0; j < kFly; ++j) {
+      const int entry = warp + j * kWarps;  // 32 vectors: of one row
+      xr[j] = entry / a.kb;
+      const int v = vec0 + (entry - xr[j] * a.kb) * 32 + lane;
+      xq[j] = wq[j] = make_uint4(0, 0, 0, 0);
+      if (xr[j] < a.rows && v < all_vecs) {
+        xq[j] = reinterpret_cast<const uint4*>(x + xr[j] * a.x_stride)[v];
+        if (nw != nullptr) wq[j] = reinterpret_cast<const uint4*>(nw)[v];
+      }
+    }
+  }
+
   const uint64_t policy = l2_policy_evict_first();
+  if (fill) {
+    const uint32_t dst = ring + lane * kJobBytes, bar = bars + 8 * lane;
+    mbar_arrive_expect_tx(bar, kJobBytes);
+    tma_load_2d_hint(dst, &a.tm_w[0], fill_x, fill_n, bar, policy);
+    if (pair) tma_load_2d_hint(dst + 1024, &a.tm_w[1], fill_x, fill_n, bar, policy);
+  }
+  Jobs<kWarps> ld = job;  // next job to copy
+  int flying = min(a.stages, job.left);
+  ld.left -= flying;
+  ld.jk += flying;
+  while (ld.jk >= a.kb) ld.jk -= a.kb, ++ld.tile;
   const auto issue = [&](int stage) -> int {
     if (!ld.settle(a, tile_end)) return 0;
     if (lane == 0) {
-      const int t = ld.round + ld.tile, x = (kb0 + ld.jk) * 128;
+      const int n = (ld.round + ld.tile) * tile_n, xk = (kb0 + ld.jk) * 128;
       const uint32_t dst = ring + stage * kJobBytes, bar = bars + 8 * stage;
       mbar_arrive_expect_tx(bar, kJobBytes);
-      tma_load_2d_hint(dst, &a.tm_w[0], x, t * tile_n, bar, policy);
-      if (pair) tma_load_2d_hint(dst + 1024, &a.tm_w[1], x, t * tile_n, bar, policy);
+      tma_load_2d_hint(dst, &a.tm_w[0], xk, n, bar, policy);
+      if (pair) tma_load_2d_hint(dst + 1024, &a.tm_w[1], xk, n, bar, policy);
     }
     ld.step(a);
     return 1;
   };
-  int flying = 0;
-#pragma unroll 1
-  for (int s = 0; s < a.stages; ++s) flying += issue(s);
 
-  // ---- (scale, zero) of a job: lane i of a row's four holds rows g + 8 (i / 2), groups (i % 2) kHold ..
+  // ---- (scale, zero) of a job: lane i of a row's four holds rows g + 8 (i / 2), groups (i % 2) kHold ..;
+  // fetched a job ahead, from L2 where the round before asked for them
   Jobs<kWarps> sj = job;  // next job whose scales are fetched
   const int my_row = tile_row(g), hi_row = i >> 1;
   const uint8_t* const my_zeros = pair && hi_row ? a.zeros[1] : a.zeros[0];
   const uint16_t* const my_scales = static_cast<const uint16_t*>(pair && hi_row ? a.scales[1] : a.scales[0]);
   const int n_off = my_row + (pair ? 0 : 8 * hi_row);
-  const auto fetch = [&](uint32_t (&v)[kHold]) {
-#pragma unroll
-    for (int j = 0; j < kHold; ++j) v[j] = 0u;
+  uint32_t sz[kHold], next_s[kHold], next_z[kHold];
+  const auto fetch = [&]() {
     if (!sj.settle(a, tile_end)) return;
-    const int n = (sj.round + sj.tile) * tile_n + n_off, grp0 = (kb0 + sj.jk) * kSegs + (i & 1) * kHold;
+    const int t = sj.round + sj.tile, n = t * tile_n + n_off, grp0 = (kb0 + sj.jk) * kSegs + (i & 1) * kHold;
     sj.step(a);
-    if (n >= a.n) return;
     const int64_t at = (int64_t)n * a.groups + grp0;
+    if (t + a.tiles_round < tile_end && n + a.tiles_round * tile_n < a.n && grp0 < a.groups) {
+      const int64_t next = at + (int64_t)a.tiles_round * tile_n * a.groups;
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(my_scales + next));
+      if (my_zeros != nullptr) asm volatile("prefetch.global.L2 [%0];" ::"l"(my_zeros + next));
+    }
 #pragma unroll
     for (int j = 0; j < kHold; ++j) {
-      if (grp0 + j >= a.groups) continue;
-      const float z = my_zeros != nullptr ? (float)my_zeros[at + j] : 8.f;
+      next_s[j] = 0u;
+      next_z[j] = 8u;
+      if (n >= a.n || grp0 + j >= a.groups) continue;
+      next_s[j] = my_scales[at + j];
+      if (my_zeros != nullptr) next_z[j] = my_zeros[at + j];
+    }
+  };
+  const auto take = [&]() {  // the fetched ones become the next job's
+#pragma unroll
+    for (int j = 0; j < kHold; ++j) {
       union {
         T t;
         uint16_t u;
-      } zb;
-      zb.t = Elem<T>::from_float(z);  // 0..15: exact
-      v[j] = my_scales[at + j] | (uint32_t)zb.u << 16;
+      } z;
+      z.t = Elem<T>::from_float((float)next_z[j]);  // 0..15: exact
+      sz[j] = next_s[j] | (uint32_t)z.u << 16;
     }
   };
-  uint32_t sz0[kHold], sz1[kHold], sz2[kHold];
-  fetch(sz0);
-  fetch(sz1);
-  fetch(sz2);
+  fetch();
+
+  // ---- which warps share a tile of a full round, for the sums at its end
+  const auto find_heads = [&](int tiles) {
+    const int total = tiles * a.kb;
+    if (tid < tiles) {
+      // job j is warp ((j + 1) kWarps - 1) / total's
+      const int w0 = ((tid * a.kb + 1) * kWarps - 1) / total, w1 = ((tid + 1) * a.kb * kWarps - 1) / total;
+      s_heads[tid] = w0 | w1 << 16;
+    }
+  };
+  find_heads(min(a.tiles_round, tile_end - tile0));
 
   // ---- rows' largest element (of this CTA's K) and sum of squares (of all K)
-  const T* x = static_cast<const T*>(a.x);
-  constexpr int kFly = NT <= 2 ? 4 : 8;  // vectors in flight a thread
-  const int parts = a.rows >= kWarps ? 1 : kWarps / a.rows;  // warps a row
-  const int vec0 = kb0 * (kJobK / 8), vecs = a.kb * (kJobK / 8), all_vecs = a.k / 8;
-  for (int u = warp; u < a.rows * parts; u += kWarps) {
-    const int r = u / parts, first = (u - r * parts) * 32 + lane;
-    const uint4* row = reinterpret_cast<const uint4*>(x + r * a.x_stride);
-    const int lo = nw != nullptr ? 0 : vec0, hi = nw != nullptr ? all_vecs : min(vec0 + vecs, all_vecs);
-    float ss = 0.f, far = 0.f, top = 0.f;  // far: of elements times 2^-70, where squares pass fp32's range
-    for (int v0 = lo + first; v0 < hi; v0 += kFly * parts * 32) {
-      uint4 q[kFly], wq[kFly];
-#pragma unroll
-      for (int j = 0; j < kFly; ++j) {
-        const int v = v0 + j * parts * 32;
-        q[j] = wq[j] = make_uint4(0, 0, 0, 0);
-        if (v < hi) {
-          q[j] = row[v];
-          if (nw != nullptr) wq[j] = reinterpret_cast<const uint4*>(nw)[v];
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < kFly; ++j) {
-        const int v = v0 + j * parts * 32;
-        float f[8], w[8];
-        Elem<T>::unpack(q[j], f);
-        Elem<T>::unpack(wq[j], w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          ss = fmaf(f[e], f[e], ss);
-          const float small = f[e] * 8.470329472543003e-22f;
-          far = fmaf(small, small, far);
-          if (nw != nullptr) f[e] *= w[e];
-          if (v >= vec0 && v < vec0 + vecs) top = fmaxf(top, fabsf(f[e]));
-        }
-      }
-    }
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) {
-      ss += __shfl_xor_sync(0xffffffffu, ss, off);
-      far += __shfl_xor_sync(0xffffffffu, far, off);
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-    }
-    if (lane == 0) s_stat[3 * u] = top, s_stat[3 * u + 1] = ss, s_stat[3 * u + 2] = far;
-  }
-  __syncthreads();
-  if (tid < a.rows) {
-    float ss = 0.f, far = 0.f, top = 0.f;
-    for (int u = tid * parts; u < (tid + 1) * parts; ++u)
-      top = fmaxf(top, s_stat[3 * u]), ss += s_stat[3 * u + 1], far += s_stat[3 * u + 2];
+  const auto row_scale = [&](int r, float top, float ss) {
     float rstd = 1.f;
-    if (nw != nullptr)
-      rstd = ss < INFINITY ? rsqrtf(ss / (float)a.k + a.eps) : rsqrtf(far / (float)a.k) * 8.470329472543003e-22f;
+    if (nw != nullptr) {
+      rstd = rsqrtf(ss / (float)a.k + a.eps);
+      if (!(ss < INFINITY)) {  // squares past fp32's range: of the elements times 2^-70
+        const float by = 8.470329472543003e-22f;
+        rstd = rsqrtf(row_stats<T>(x + r * a.x_stride, nw, lane, all_vecs, 0, 0, by).y / (float)a.k) * by;
+      }
+    }
     // 2^e that brings the largest element to [2^9, 2^10); 1 for a row of zeros or one with inf
     const uint32_t bits = __float_as_uint(top * rstd) >> 23;
     const int e = bits == 0u || bits >= 255u ? 0 : min(136 - (int)bits, 100);
-    s_scale[tid] = rstd * __uint_as_float((uint32_t)(127 + e) << 23);
-    s_inv[tid] = __uint_as_float((uint32_t)(127 - e) << 23);
+    if (lane == 0) {
+      s_scale[r] = rstd * __uint_as_float((uint32_t)(127 + e) << 23);
+      s_inv[r] = __uint_as_float((uint32_t)(127 - e) << 23);
+    }
+  };
+  if (once) {
+#pragma unroll
+    for (int j = 0; j < kFly; ++j) {
+      if (xr[j] >= a.rows) break;
+      float f[8], w[8], top = 0.f, ss = 0.f;
+      Elem<T>::unpack(xq[j], f);
+      if (nw != nullptr) {
+        Elem<T>::unpack(wq[j], w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss), f[e] *= w[e];
+#pragma unroll
+        for (int off = 16; off >= 1; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[e]));
+      const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(top));  // magnitudes order as their bits
+      if (lane == 0) s_stat[warp + j * kWarps] = make_float2(__uint_as_float(most), ss);
+    }
+    __syncthreads();
+    for (int r = warp; r < a.rows; r += kWarps) {
+      float top = 0.f, ss = 0.f;
+      for (int e = lane; e < a.kb; e += 32) {
+        const float2 st = s_stat[r * a.kb + e];
+        top = fmaxf(top, st.x);
+        ss += st.y;
+      }
+#pragma unroll
+      for (int off = 16; off >= 1; off >>= 1) {
+        ss += __shfl_xor_sync(0xffffffffu, ss, off);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+      }
+      row_scale(r, top, ss);
+    }
+  } else {
+    for (int r = warp; r < a.rows; r += kWarps) {
+      const float2 st = nw != nullptr
+                            ? row_stats<T>(x + r * a.x_stride, nw, lane, all_vecs, vec0, vec0 + vecs, 1.f)
+                            : row_stats<T>(x + r * a.x_stride, nullptr, vec0 + lane, min(vec0 + vecs, all_vecs), vec0, vec0 + vecs, 1.f);
+      row_scale(r, st.x, st.y);
+    }
   }
   __syncthreads();
 
   // ---- x' into shared memory, in the order in which the products take it
-  for (int at0 = tid; at0 < a.rows * vecs; at0 += kFly * kThreads) {
-    uint4 q[kFly], wq[kFly];
+  const auto lay_out = [&](const uint4& q, const uint4& wv, int r, int v) {
+    float f[8];
+    Elem<T>::unpack(q, f);
+    const float scale = s_scale[r];
 #pragma unroll
-    for (int j = 0; j < kFly; ++j) {
-      const int at = at0 + j * kThreads, r = at / vecs, v = vec0 + at - r * vecs;
-      q[j] = wq[j] = make_uint4(0, 0, 0, 0);
-      if (r < a.rows && v < all_vecs) {
-        q[j] = reinterpret_cast<const uint4*>(x + r * a.x_stride)[v];
-        if (nw != nullptr) wq[j] = reinterpret_cast<const uint4*>(nw)[v];
-      }
+    for (int e = 0; e < 8; ++e) f[e] *= scale;
+    if (nw != nullptr) {
+      float w[8];
+      Elem<T>::unpack(wv, w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] *= w[e];
     }
+    const int wd = v & 31, rem = wd % (4 * W);
+    const int step = (v >> 5) * 8 + wd / (4 * W) * W + rem % W, li = rem / W;
+    // pairs (k0, k4), (k1, k5) / 16, (k2, k6), (k3, k7) / 16
+    const auto put = [&](int col) {
+      union {
+        __half2 h[4];
+        uint4 u;
+      } d;
 #pragma unroll
-    for (int j = 0; j < kFly; ++j) {
-      const int at = at0 + j * kThreads, r = at / vecs, v = at - r * vecs;
-      if (r >= a.rows) break;  // whole warps: vecs is a multiple of 32
-      float f[8], w[8], lo[8], sum = 0.f, low_sum = 0.f;
-      Elem<T>::unpack(q[j], f);
-      Elem<T>::unpack(wq[j], w);
-      const float scale = s_scale[r];
+      for (int e = 0; e < 4; ++e)
+        d.h[e] = e & 1 ? __floats2half2_rn(f[e] * 0.0625f, f[e + 4] * 0.0625f) : __floats2half2_rn(f[e], f[e + 4]);
+      *reinterpret_cast<uint4*>(xs + ((step * NT + (col >> 3)) * 32 + (col & 7) * 4 + li) * 16) = d.u;
+    };
+    if (split) {
+      put(2 * r);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float y = (nw != nullptr ? f[e] * w[e] : f[e]) * scale;
-        f[e] = __half2float(__float2half_rn(y));
-        lo[e] = split ? __half2float(__float2half_rn(y - f[e])) : 0.f;
-        sum += f[e];
-        low_sum += lo[e];
+      for (int e = 0; e < 8; ++e) f[e] -= __half2float(__float2half_rn(f[e]));
+      put(2 * r + 1);
+    } else {
+      put(r);
+    }
+  };
+  if (once) {
+#pragma unroll
+    for (int j = 0; j < kFly; ++j)
+      if (xr[j] < a.rows) lay_out(xq[j], wq[j], xr[j], (warp + j * kWarps - xr[j] * a.kb) * 32 + lane);
+  } else {
+#pragma unroll 4
+    for (int at = tid; at < a.rows * vecs; at += kThreads) {
+      const int r = at / vecs, v = at - r * vecs;
+      uint4 q = make_uint4(0, 0, 0, 0), w = q;
+      if (vec0 + v < all_vecs) {
+        q = reinterpret_cast<const uint4*>(x + r * a.x_stride)[vec0 + v];
+        if (nw != nullptr) w = reinterpret_cast<const uint4*>(nw)[vec0 + v];
       }
-      const int wd = v & 31, rem = wd % (4 * W);
-      const int step = (v >> 5) * 8 + wd / (4 * W) * W + rem % W, li = rem / W;
-      // pairs (k0, k4), (k1, k5) / 16, (k2, k6), (k3, k7) / 16
-      const auto put = [&](int col, const float* y) {
-        union {
-          __half2 h[4];
-          uint4 u;
-        } d;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          d.h[e] = __floats2half2_rn(y[e] * (e & 1 ? 0.0625f : 1.f), y[e + 4] * (e & 1 ? 0.0625f : 1.f));
-        *reinterpret_cast<uint4*>(xs + ((step * NT + (col >> 3)) * 32 + (col & 7) * 4 + li) * 16) = d.u;
-      };
-      put(split ? 2 * r : r, f);
-      if (split) put(2 * r + 1, lo);
-      // the group's sum: 4 W neighbouring lanes hold it
-#pragma unroll
-      for (int off = 2 * W; off >= 1; off >>= 1) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        low_sum += __shfl_xor_sync(0xffffffffu, low_sum, off);
-      }
-      if (rem == 0) {
-        float* d = xsum + (v / (4 * W)) * NT * 8 + (split ? 2 * r : r);
-        d[0] = sum * 5.9604644775390625e-8f;  // 2^-24, as the weights
-        if (split) d[1] = low_sum * 5.9604644775390625e-8f;
-      }
+      lay_out(q, w, r, v);
     }
   }
+  __syncthreads();
+  // a group's sums of x', times the weights' 2^-24: products with ones in the weights' place
+  for (int grp = warp; grp < a.kb * kSegs; grp += kWarps) {
+    float acc[NT][4] = {};
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const uint4 b = *reinterpret_cast<const uint4*>(xs + (((grp * W + w) * NT + n) * 32 + lane) * 16);
+        mma_f16(acc[n], 0x00010001u, 0u, 0x00100010u, 0u, b.x, b.y);
+        mma_f16(acc[n], 0x00010001u, 0u, 0x00100010u, 0u, b.z, b.w);
+      }
+    if (g == 0)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        *reinterpret_cast<float2*>(xsum + (grp * NT + n) * 8 + 2 * i) = make_float2(acc[n][0], acc[n][1]);
+  }
+  take();
   __syncthreads();
 
   // ---- rounds
@@ -381,13 +472,14 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
       }
       if (!bad && !mbar_wait(bars + 8 * stage, phase, s_abort, a.err)) bad = true;  // computes no more, keeps to the barriers
       if (!bad) {
+        fetch();
         const uint32_t wrow = ring + stage * kJobBytes + my_row * 128;
         const uint8_t* xf = xs + (size_t)(job.jk * 8 * NT * 32 + lane) * 16;
         const float* gs = xsum + job.jk * kSegs * NT * 8 + 2 * i;
 #pragma unroll
         for (int seg = 0; seg < kSegs; ++seg) {
-          const uint32_t s_lo = __shfl_sync(0xffffffffu, sz0[seg % kHold], (lane & ~3) | seg / kHold);
-          const uint32_t s_hi = __shfl_sync(0xffffffffu, sz0[seg % kHold], (lane & ~3) | 2 | seg / kHold);
+          const uint32_t s_lo = __shfl_sync(0xffffffffu, sz[seg % kHold], (lane & ~3) | seg / kHold);
+          const uint32_t s_hi = __shfl_sync(0xffffffffu, sz[seg % kHold], (lane & ~3) | 2 | seg / kHold);
           // this lane's W words of rows my_row and my_row + 8
           uint32_t w0[4], w1[4];
           {
@@ -431,15 +523,13 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
         __syncwarp();  // every lane has read the stage
         flying += issue(stage) - 1;
         if (++stage == a.stages) stage = 0, phase ^= 1;
-#pragma unroll
-        for (int j = 0; j < kHold; ++j) sz0[j] = sz1[j], sz1[j] = sz2[j];
-        fetch(sz2);
+        take();
       }
       const int tile = job.tile;
       job.step(a);
       fresh = job.jk == 0;
       if (fresh || job.left == 0) {
-        float* dst = (head ? heads + warp * kTileFloats : part + tile * kTileFloats) + my_row;
+        float* dst = part + (head ? a.tiles_round + warp : tile) * kTileFloats + my_row;
         head = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -451,52 +541,47 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
     if (a.s > 1) cluster_sync_all(); else __syncthreads();
 
     // ---- the round's outputs: partial tiles of the warps and CTAs added in their order
-    const int tiles = min(a.tiles_round, tile_end - job.round), total_jobs = tiles * a.kb;
-    const int n0 = job.round * tile_n, width = min(tiles * tile_n, a.n - n0);
+    const int total = min(a.tiles_round, tile_end - job.round) * a.kb;
+    const int n0 = job.round * tile_n, width = min(min(a.tiles_round, tile_end - job.round) * tile_n, a.n - n0);
     for (int at = rank * kThreads + tid; at < width * a.rows; at += a.s * kThreads) {
-      const int r = at / width, c = at - r * width, tile = c / tile_n, row = c - tile * tile_n;
-      const int place = (split ? 2 * r : r) * kPitch + row;
-      // warps that hold a head of this tile: those whose first job lies inside it
-      int w0 = (tile * a.kb + 1) * kWarps / total_jobs;  // no smaller w begins after the tile's first job
-      float y[2] = {0.f, 0.f};
-      const auto add = [&](int where) {
-        float v[2][2][8];
+      const int r = at / width, c = at - r * width, tile = c / tile_n;
+      const int place = (split ? 2 * r : r) * kPitch + c - tile * tile_n;
+      const int heads = s_heads[tile], w0 = heads & 0xffff, w1 = heads >> 16;
+      float y0 = 0.f, y1 = 0.f;
+#pragma unroll 1
+      for (int w = w0; w <= w1; ++w) {
+        if (w * total / kWarps == (w + 1) * total / kWarps) continue;  // a warp without jobs
+        const float* p = part + (w == w0 ? tile : a.tiles_round + w) * kTileFloats + place;
+        if (a.s == 1) {
+          y0 += split ? p[0] + p[kPitch] : p[0];
+          if (pair) y1 += split ? p[8] + p[kPitch + 8] : p[8];
+        } else {
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          if (q >= a.s) break;
-#pragma unroll
-          for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              v[m][h][q] = 0.f;
-              if ((m == 1 && !pair) || (h == 1 && !split)) continue;
-              const float* p = part + where + place + 8 * m + h * kPitch;
-              v[m][h][q] = a.s > 1 ? ld_cluster(smem_u32(p), q) * ld_cluster(smem_u32(s_inv + r), q) : *p * s_inv[r];
+          for (int q = 0; q < 8; ++q) {
+            if (q >= a.s) break;
+            const float inv = ld_cluster(smem_u32(s_inv + r), q);
+            float t = ld_cluster(smem_u32(p), q);
+            if (split) t += ld_cluster(smem_u32(p + kPitch), q);
+            y0 = fmaf(t, inv, y0);
+            if (pair) {
+              t = ld_cluster(smem_u32(p + 8), q);
+              if (split) t += ld_cluster(smem_u32(p + 8 + kPitch), q);
+              y1 = fmaf(t, inv, y1);
             }
+          }
         }
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          if (q >= a.s) break;
-          y[0] += v[0][0][q] + v[0][1][q];
-          y[1] += v[1][0][q] + v[1][1][q];
-        }
-      };
-      add(tile * kTileFloats);
-      for (int w = w0; w < kWarps; ++w) {
-        const int begin = w * total_jobs / kWarps;
-        if (begin >= (tile + 1) * a.kb) break;
-        if (begin > tile * a.kb && begin < (w + 1) * total_jobs / kWarps) add((a.tiles_round + w) * kTileFloats);
       }
-      float v = y[0];
-      if (pair) v = v / (1.f + expf(-v)) * y[1];
+      if (a.s == 1) y0 *= s_inv[r], y1 *= s_inv[r];
+      if (pair) y0 = y0 / (1.f + expf(-y0)) * y1;
       if (a.mode == AICAS_LINEAR_RESIDUAL)
-        v += Elem<T>::to_float(static_cast<const T*>(a.residual)[r * a.res_stride + n0 + c]);
-      static_cast<T*>(a.out)[r * a.out_stride + n0 + c] = Elem<T>::from_float(v);
+        y0 += Elem<T>::to_float(static_cast<const T*>(a.residual)[r * a.res_stride + n0 + c]);
+      static_cast<T*>(a.out)[r * a.out_stride + n0 + c] = Elem<T>::from_float(y0);
     }
     job.round += a.tiles_round;
     if (job.round >= tile_end) break;
     job.cut(a, tile_end);
     if (a.s > 1) cluster_sync_all(); else __syncthreads();  // the partial tiles have been read
+    if (tile_end - job.round < a.tiles_round) find_heads(tile_end - job.round);  // read after the next barrier
   }
   if (bad)
     for (; flying > 0; --flying) {  // leave once this warp's copies have landed (bounded again)
@@ -574,6 +659,8 @@ cudaError_t launch_int4(Int4Args a, int smem, int sms, cudaStream_t st) {
     }
   }
   if (clusters > a.tiles) clusters = a.tiles;
+  a.tiles_each = a.tiles / clusters;
+  a.tiles_more = a.tiles % clusters;
   cfg.gridDim = dim3((unsigned)(clusters * a.s));
   return cudaLaunchKernelEx(&cfg, linear_int4_kernel<T, NT, W>, a);
 }
@@ -601,11 +688,13 @@ cudaError_t dispatch_int4(int nt, int group, const Int4Args& a, int smem, int sm
 }
 
 // Shared memory of a launch of nt column blocks with K split s ways; 0: does not fit.
-int plan_int4(Int4Args* a, int nt, int s) {
+int plan_int4(Int4Args* a, int nt, int s, int sms) {
   const int jobs = (a->k + kJobK - 1) / kJobK;
   a->s = s;
   a->kb = (jobs + s - 1) / s;
-  a->tiles_round = nt == 1 ? 16 : nt == 2 ? 8 : 4;
+  // a round holds a cluster's tiles, if shared memory does
+  const int most = nt == 8 ? 8 : kMaxRound / nt, want = (int)((int64_t)a->tiles * s * 4 / (3 * sms)) + 1;
+  a->tiles_round = want < most ? want : most;
   const int warps = warps_for(nt);
   const int part = (a->tiles_round + warps) * nt * 8 * kPitch * 4, xs = a->kb * nt * 4096;
   const int sums = a->kb * (kJobK / (a->k / a->groups)) * nt * 32;
@@ -645,7 +734,7 @@ int run_linear_int4(const aicas_linear_int4_params* p, int sms, cudaStream_t str
   for (;; batch = (batch + 1) / 2) {
     const int blocks = (batch * columns + 7) / 8;
     nt = blocks <= 1 ? 1 : blocks <= 2 ? 2 : blocks <= 4 ? 4 : 8;
-    for (int s = 1; s <= 8 && smem == 0; s *= 2) smem = plan_int4(&a, nt, s);
+    for (int s = 1; s <= 8 && smem == 0; s *= 2) smem = plan_int4(&a, nt, s, sms);
     if (smem != 0) break;
     if (batch == 1) {
       snprintf(err, errlen, "int4 linear: in_features %d is more than shared memory holds", p->in_features);
