@@ -24,7 +24,7 @@
 //   * Sums: a group's sum over the whole numbers q in fp32, less zero point times
 //     the group's sum of activations, times the scale in fp32; groups, warps and
 //     CTAs are added up in fp32; one rounding at the end.
-//   * Work: a cluster of S CTAs takes a run of 16-row tiles (8 gate + 8 up rows
+//   * Work: a cluster of S CTAs takes a run of 32-row tiles (16 gate + 16 up rows
 //     for SiLU * up), each CTA one S-th of K, so that its share of x' fits beside
 //     the ring (S = 1 wherever all of it does).  Tiles are taken in rounds; a
 //     round's (tile, 256 k) jobs are cut evenly over the warps, whatever tile
@@ -43,17 +43,17 @@ namespace aicas {
 namespace {
 
 constexpr int kJobK = 256;              // k of a job: 128 bytes of a row
-constexpr int kJobBytes = 16 * 128;     // 16 rows
-constexpr int kPitch = 20;              // floats a column of a partial tile (16 rows; 20 keeps stores conflict free)
+constexpr int kTileRows = 32;
+constexpr int kJobBytes = kTileRows * 128;
+constexpr int kPitch = 36;              // floats a column of a partial tile (32 rows; 36 keeps stores conflict free)
 constexpr int kMaxSmem = 232448;
 
-constexpr int kMaxRound = 80;           // tiles of a round
-constexpr int kEntries = 128;           // rows' statistics: (largest element, sum of squares) of 256 k each
-constexpr int kVarBytes = 64 + kEntries * 8 + 2 * 32 * 4 + kMaxRound * 4;
+constexpr int kMaxRound = 40;           // tiles of a round
+constexpr int kVarBytes = 64 + 3 * 32 * 4 + kMaxRound * 4;
 
 // Warps of a CTA: more of them hide the products' latency, fewer leave shared
 // memory for the columns of many rows.
-constexpr int warps_for(int nt) { return nt <= 4 ? 16 : 8; }
+constexpr int warps_for(int nt) { return nt <= 2 ? 12 : 8; }
 
 struct Int4Args {
   CUtensorMap tm_w[2];
@@ -69,10 +69,12 @@ struct Int4Args {
   float eps;
   int s;                   // CTAs of a cluster
   int kb;                  // jobs of a tile for each of them
-  int tiles, tiles_round;  // 16-row tiles of the launch; tiles of a round
+  int tiles, tiles_round;  // 32-row tiles of the launch; tiles of a round
+  int out_quads;           // four outputs may be stored at once
+  int whole;               // K is whole jobs and scales and zeros are aligned: vector loads
   int tiles_each, tiles_more;  // tiles of a cluster; the first tiles_more clusters take one more
   int stages;
-  int off_part, off_x, off_sum, off_bars;
+  int off_part, off_recv, off_x, off_sum, off_bars;
   unsigned int* err;
 };
 
@@ -83,23 +85,31 @@ __device__ __forceinline__ void mma_f16(float c[4], uint32_t a0, uint32_t a1, ui
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// Element `odd` of a packed pair.
 template <typename T>
-__device__ __forceinline__ float low_half(uint32_t v) {
+__device__ __forceinline__ float half_of(uint32_t v, int odd) {
   union {
-    uint16_t u;
-    T t;
+    uint16_t u[2];
+    T t[2];
   } r;
-  r.u = (uint16_t)v;
-  return Elem<T>::to_float(r.t);
+  r.u[0] = (uint16_t)v, r.u[1] = (uint16_t)(v >> 16);
+  return Elem<T>::to_float(r.t[odd]);
 }
 
-__device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
-  uint32_t a;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-  return v;
+// Byte b of v as a float: its bits under those of 2^23, less 2^23.
+__device__ __forceinline__ float byte_of(uint32_t v, int b) {
+  return __uint_as_float(__byte_perm(v, 0x4b000000u, 0x7440 | b)) - 8388608.f;
 }
+
+__device__ __forceinline__ void st_cluster(float* p, uint32_t rank, const float4& v) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+               : "memory");
+}
+// In two halves: every CTA of the cluster has started once the wait returns.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync_all() {
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -178,21 +188,21 @@ template <typename T, int NT, int W>
 __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(const __grid_constant__ Int4Args a) {
   constexpr int kWarps = warps_for(NT), kThreads = kWarps * 32;
   constexpr int kSegs = 8 / W;          // groups of a job
-  constexpr int kHold = kSegs / 2;      // (scale, zero) pairs a lane holds of a job: two rows' kSegs over four lanes
-  constexpr int kTileFloats = NT * 8 * kPitch;
-  constexpr int kFly = NT <= 2 ? 4 : 8; // vectors of x a thread holds at once
+  constexpr int kFly = NT <= 2 ? 6 : 12;  // vectors of x a thread holds at once
   extern __shared__ __align__(1024) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, i = lane & 3;
   const bool pair = a.mode == AICAS_LINEAR_SWIGLU;
-  const int tile_n = pair ? 8 : 16;     // output features of a tile
+  const int tile_n = pair ? 16 : 32;    // output features of a tile
   const uint32_t ring = smem_u32(smem) + warp * a.stages * kJobBytes;
   const uint32_t bars = smem_u32(smem + a.off_bars) + warp * a.stages * 8;
-  float* part = reinterpret_cast<float*>(smem + a.off_part);  // [tiles_round][kTileFloats], then [kWarps] heads
+  float* part = reinterpret_cast<float*>(smem + a.off_part);  // [tiles_round][cols][kPitch], then [kWarps] heads
+  float* s_sums = part;  // before the first round: a row's sums of squares, by blocks of 256
+  float* recv = reinterpret_cast<float*>(smem + a.off_recv);  // cluster: [from rank][this CTA's share of the outputs]
   uint8_t* xs = smem + a.off_x;
   float* xsum = reinterpret_cast<float*>(smem + a.off_sum);   // [group of this CTA's K][NT * 8 columns]
   int* s_abort = reinterpret_cast<int*>(smem + a.off_bars + kWarps * a.stages * 8);
-  float2* s_stat = reinterpret_cast<float2*>(s_abort + 16);   // [kEntries]
-  float* s_scale = reinterpret_cast<float*>(s_stat + kEntries);  // [32]
+  uint32_t* s_top = reinterpret_cast<uint32_t*>(s_abort + 16);   // [32] a row's largest magnitude
+  float* s_scale = reinterpret_cast<float*>(s_top + 32);      // [32]
   float* s_inv = s_scale + 32;                                // [32]
   int* s_heads = reinterpret_cast<int*>(s_inv + 32);          // [tile of the round] the warps after the tile's first
   const int rank = a.s > 1 ? (int)cluster_rank() : 0;
@@ -200,8 +210,11 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
   const int kb0 = rank * a.kb;  // this CTA's first job along K
   const T* nw = static_cast<const T*>(a.norm_weight);
   const bool split = nw != nullptr && std::is_same<T, __half>::value;  // two parts a row
+  const int cols = split ? 2 * a.rows : a.rows, tile_floats = cols * kPitch;
 
   if (tid == 0) *s_abort = 0;
+  if (tid < 32) s_top[tid] = 0u;
+  if (a.s > 1) cluster_arrive();  // waited for before the first store to another CTA
   if (lane < a.stages) mbar_init(bars + 8 * lane, 1);
   grid_launch_dependents();
 
@@ -222,36 +235,39 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
     if (pair) tma_prefetch_l2_2d(&a.tm_w[1], fill_x, fill_n);
   }
   fence_mbar_init();
-  __syncwarp();
+  __syncthreads();
   grid_dependency_wait();
 
-  // ---- x: this thread's vectors of the CTA's share of K, ahead of the weights
+  // ---- x, ahead of the weights: blocks of 256 k of a row, a 16-byte vector a lane, kFly blocks a warp at once
   const T* x = static_cast<const T*>(a.x);
-  const int vec0 = kb0 * (kJobK / 8), vecs = a.kb * (kJobK / 8), all_vecs = a.k / 8;
-  // at once, where they fit and nothing else of the rows is needed; else in passes
-  const bool once = a.rows * vecs <= kFly * kThreads && (nw == nullptr || a.s == 1);
+  const int all_vecs = a.k / 8, all_kb = (a.k + kJobK - 1) / kJobK;
+  const int row_kb = nw != nullptr ? all_kb : a.kb, row_kb0 = nw != nullptr ? 0 : kb0;  // blocks of a row for its statistics
+  const bool once = a.rows * a.kb <= kFly * kWarps && row_kb == a.kb;  // the vectors stay in registers in between
   uint4 xq[kFly], wq[kFly];
-  int xr[kFly];
-  if (once) {
+  int xr[kFly], xb[kFly];
+  const auto load = [&](int block, int per, int first) {  // blocks block, block + kWarps, .. of rows of `per` blocks
+    int r = block / per, at = block - r * per;
 #pragma unroll
     for (int j = 0; j < kFly; ++j) {
-      const int entry = warp + j * kWarps;  // 32 vectors: of one row
-      xr[j] = entry / a.kb;
-      const int v = vec0 + (entry - xr[j] * a.kb) * 32 + lane;
+      xr[j] = r, xb[j] = at;
+      const int v = (first + at) * 32 + lane;
       xq[j] = wq[j] = make_uint4(0, 0, 0, 0);
-      if (xr[j] < a.rows && v < all_vecs) {
-        xq[j] = reinterpret_cast<const uint4*>(x + xr[j] * a.x_stride)[v];
+      if (r < a.rows && v < all_vecs) {
+        xq[j] = reinterpret_cast<const uint4*>(x + r * a.x_stride)[v];
         if (nw != nullptr) wq[j] = reinterpret_cast<const uint4*>(nw)[v];
       }
+      at += kWarps;
+      while (at >= per) at -= per, ++r;
     }
-  }
+  };
+  load(warp, row_kb, row_kb0);
 
   const uint64_t policy = l2_policy_evict_first();
   if (fill) {
     const uint32_t dst = ring + lane * kJobBytes, bar = bars + 8 * lane;
     mbar_arrive_expect_tx(bar, kJobBytes);
     tma_load_2d_hint(dst, &a.tm_w[0], fill_x, fill_n, bar, policy);
-    if (pair) tma_load_2d_hint(dst + 1024, &a.tm_w[1], fill_x, fill_n, bar, policy);
+    if (pair) tma_load_2d_hint(dst + 2048, &a.tm_w[1], fill_x, fill_n, bar, policy);
   }
   Jobs<kWarps> ld = job;  // next job to copy
   int flying = min(a.stages, job.left);
@@ -265,49 +281,66 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
       const uint32_t dst = ring + stage * kJobBytes, bar = bars + 8 * stage;
       mbar_arrive_expect_tx(bar, kJobBytes);
       tma_load_2d_hint(dst, &a.tm_w[0], xk, n, bar, policy);
-      if (pair) tma_load_2d_hint(dst + 1024, &a.tm_w[1], xk, n, bar, policy);
+      if (pair) tma_load_2d_hint(dst + 2048, &a.tm_w[1], xk, n, bar, policy);
     }
     ld.step(a);
     return 1;
   };
 
-  // ---- (scale, zero) of a job: lane i of a row's four holds rows g + 8 (i / 2), groups (i % 2) kHold ..;
+  // ---- scales and zero points of a job: lane i of a lane group holds those of row my_row + 8 i;
   // fetched a job ahead, from L2 where the round before asked for them
   Jobs<kWarps> sj = job;  // next job whose scales are fetched
-  const int my_row = tile_row(g), hi_row = i >> 1;
-  const uint8_t* const my_zeros = pair && hi_row ? a.zeros[1] : a.zeros[0];
-  const uint16_t* const my_scales = static_cast<const uint16_t*>(pair && hi_row ? a.scales[1] : a.scales[0]);
-  const int n_off = my_row + (pair ? 0 : 8 * hi_row);
-  uint32_t sz[kHold], next_s[kHold], next_z[kHold];
+  const int my_row = tile_row(g);
+  const bool up = pair && i >= 2;
+  const uint8_t* const my_zeros = up ? a.zeros[1] : a.zeros[0];
+  const uint16_t* const my_scales = static_cast<const uint16_t*>(up ? a.scales[1] : a.scales[0]);
+  const int n_off = my_row + 8 * (pair ? i & 1 : i);
+  uint32_t sc[kSegs / 2], zp[(kSegs + 3) / 4], next_s[kSegs / 2], next_z[(kSegs + 3) / 4];
   const auto fetch = [&]() {
     if (!sj.settle(a, tile_end)) return;
-    const int t = sj.round + sj.tile, n = t * tile_n + n_off, grp0 = (kb0 + sj.jk) * kSegs + (i & 1) * kHold;
+    const int t = sj.round + sj.tile, n = t * tile_n + n_off, grp0 = (kb0 + sj.jk) * kSegs;
     sj.step(a);
     const int64_t at = (int64_t)n * a.groups + grp0;
+#pragma unroll
+    for (int j = 0; j < (kSegs + 3) / 4; ++j) next_z[j] = 0x08080808u;
+    if (n < a.n && a.whole) {
+      // K is whole jobs: a row's groups of a job are one aligned vector
+      if constexpr (kSegs == 2) {
+        next_s[0] = *reinterpret_cast<const uint32_t*>(my_scales + at);
+        if (my_zeros != nullptr) next_z[0] = *reinterpret_cast<const uint16_t*>(my_zeros + at);
+      } else if constexpr (kSegs == 4) {
+        const uint2 v = *reinterpret_cast<const uint2*>(my_scales + at);
+        next_s[0] = v.x, next_s[1] = v.y;
+        if (my_zeros != nullptr) next_z[0] = *reinterpret_cast<const uint32_t*>(my_zeros + at);
+      } else {
+        const uint4 v = *reinterpret_cast<const uint4*>(my_scales + at);
+        next_s[0] = v.x, next_s[1] = v.y, next_s[2] = v.z, next_s[3] = v.w;
+        if (my_zeros != nullptr) {
+          const uint2 z = *reinterpret_cast<const uint2*>(my_zeros + at);
+          next_z[0] = z.x, next_z[1] = z.y;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kSegs / 2; ++j) next_s[j] = 0u;
+#pragma unroll
+      for (int j = 0; j < kSegs; ++j) {
+        if (n >= a.n || grp0 + j >= a.groups) continue;
+        next_s[j / 2] |= (uint32_t)my_scales[at + j] << (16 * (j & 1));
+        if (my_zeros != nullptr) next_z[j / 4] ^= (8u ^ my_zeros[at + j]) << (8 * (j & 3));
+      }
+    }
     if (t + a.tiles_round < tile_end && n + a.tiles_round * tile_n < a.n && grp0 < a.groups) {
       const int64_t next = at + (int64_t)a.tiles_round * tile_n * a.groups;
       asm volatile("prefetch.global.L2 [%0];" ::"l"(my_scales + next));
       if (my_zeros != nullptr) asm volatile("prefetch.global.L2 [%0];" ::"l"(my_zeros + next));
     }
-#pragma unroll
-    for (int j = 0; j < kHold; ++j) {
-      next_s[j] = 0u;
-      next_z[j] = 8u;
-      if (n >= a.n || grp0 + j >= a.groups) continue;
-      next_s[j] = my_scales[at + j];
-      if (my_zeros != nullptr) next_z[j] = my_zeros[at + j];
-    }
   };
   const auto take = [&]() {  // the fetched ones become the next job's
 #pragma unroll
-    for (int j = 0; j < kHold; ++j) {
-      union {
-        T t;
-        uint16_t u;
-      } z;
-      z.t = Elem<T>::from_float((float)next_z[j]);  // 0..15: exact
-      sz[j] = next_s[j] | (uint32_t)z.u << 16;
-    }
+    for (int j = 0; j < kSegs / 2; ++j) sc[j] = next_s[j];
+#pragma unroll
+    for (int j = 0; j < (kSegs + 3) / 4; ++j) zp[j] = next_z[j];
   };
   fetch();
 
@@ -340,99 +373,81 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
       s_inv[r] = __uint_as_float((uint32_t)(127 - e) << 23);
     }
   };
-  if (once) {
+  for (int block = warp;;) {
 #pragma unroll
     for (int j = 0; j < kFly; ++j) {
       if (xr[j] >= a.rows) break;
-      float f[8], w[8], top = 0.f, ss = 0.f;
+      float f[8], top = 0.f, ss = 0.f;
       Elem<T>::unpack(xq[j], f);
       if (nw != nullptr) {
+        float w[8];
         Elem<T>::unpack(wq[j], w);
 #pragma unroll
         for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss), f[e] *= w[e];
 #pragma unroll
         for (int off = 16; off >= 1; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+        if (lane == 0) s_sums[xr[j] * row_kb + xb[j]] = ss;
       }
+      const int mine_kb = row_kb0 + xb[j] - kb0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[e]));
       const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(top));  // magnitudes order as their bits
-      if (lane == 0) s_stat[warp + j * kWarps] = make_float2(__uint_as_float(most), ss);
+      if (lane == 0 && mine_kb >= 0 && mine_kb < a.kb) atomicMax(s_top + xr[j], most);
     }
-    __syncthreads();
-    for (int r = warp; r < a.rows; r += kWarps) {
-      float top = 0.f, ss = 0.f;
-      for (int e = lane; e < a.kb; e += 32) {
-        const float2 st = s_stat[r * a.kb + e];
-        top = fmaxf(top, st.x);
-        ss += st.y;
-      }
+    block += kFly * kWarps;
+    if (block >= a.rows * row_kb) break;
+    load(block, row_kb, row_kb0);
+  }
+  __syncthreads();
+  for (int r = warp; r < a.rows; r += kWarps) {
+    float ss = 0.f;
+    if (nw != nullptr) {
+      for (int e = lane; e < row_kb; e += 32) ss += s_sums[r * row_kb + e];
 #pragma unroll
-      for (int off = 16; off >= 1; off >>= 1) {
-        ss += __shfl_xor_sync(0xffffffffu, ss, off);
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-      }
-      row_scale(r, top, ss);
+      for (int off = 16; off >= 1; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
     }
-  } else {
-    for (int r = warp; r < a.rows; r += kWarps) {
-      const float2 st = nw != nullptr
-                            ? row_stats<T>(x + r * a.x_stride, nw, lane, all_vecs, vec0, vec0 + vecs, 1.f)
-                            : row_stats<T>(x + r * a.x_stride, nullptr, vec0 + lane, min(vec0 + vecs, all_vecs), vec0, vec0 + vecs, 1.f);
-      row_scale(r, st.x, st.y);
-    }
+    row_scale(r, __uint_as_float(s_top[r]), ss);
   }
   __syncthreads();
 
   // ---- x' into shared memory, in the order in which the products take it
-  const auto lay_out = [&](const uint4& q, const uint4& wv, int r, int v) {
-    float f[8];
-    Elem<T>::unpack(q, f);
-    const float scale = s_scale[r];
+  const int my_step = lane / (4 * W) * W + lane % W, my_i = lane % (4 * W) / W;  // of this lane's vector of a block
+  for (int block = warp;;) {
+    if (!once) load(block, a.kb, kb0);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] *= scale;
-    if (nw != nullptr) {
-      float w[8];
-      Elem<T>::unpack(wv, w);
+    for (int j = 0; j < kFly; ++j) {
+      if (xr[j] >= a.rows) break;
+      float f[8];
+      Elem<T>::unpack(xq[j], f);
+      const float scale = s_scale[xr[j]], odd = scale * 0.0625f;  // odd k's times 2^-4
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] *= w[e];
-    }
-    const int wd = v & 31, rem = wd % (4 * W);
-    const int step = (v >> 5) * 8 + wd / (4 * W) * W + rem % W, li = rem / W;
-    // pairs (k0, k4), (k1, k5) / 16, (k2, k6), (k3, k7) / 16
-    const auto put = [&](int col) {
-      union {
-        __half2 h[4];
-        uint4 u;
-      } d;
+      for (int e = 0; e < 8; ++e) f[e] *= e & 1 ? odd : scale;
+      if (nw != nullptr) {
+        float w[8];
+        Elem<T>::unpack(wq[j], w);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        d.h[e] = e & 1 ? __floats2half2_rn(f[e] * 0.0625f, f[e + 4] * 0.0625f) : __floats2half2_rn(f[e], f[e + 4]);
-      *reinterpret_cast<uint4*>(xs + ((step * NT + (col >> 3)) * 32 + (col & 7) * 4 + li) * 16) = d.u;
-    };
-    if (split) {
-      put(2 * r);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] -= __half2float(__float2half_rn(f[e]));
-      put(2 * r + 1);
-    } else {
-      put(r);
-    }
-  };
-  if (once) {
-#pragma unroll
-    for (int j = 0; j < kFly; ++j)
-      if (xr[j] < a.rows) lay_out(xq[j], wq[j], xr[j], (warp + j * kWarps - xr[j] * a.kb) * 32 + lane);
-  } else {
-#pragma unroll 4
-    for (int at = tid; at < a.rows * vecs; at += kThreads) {
-      const int r = at / vecs, v = at - r * vecs;
-      uint4 q = make_uint4(0, 0, 0, 0), w = q;
-      if (vec0 + v < all_vecs) {
-        q = reinterpret_cast<const uint4*>(x + r * a.x_stride)[vec0 + v];
-        if (nw != nullptr) w = reinterpret_cast<const uint4*>(nw)[vec0 + v];
+        for (int e = 0; e < 8; ++e) f[e] *= w[e];
       }
-      lay_out(q, w, r, v);
+      const auto put = [&](int col) {  // pairs (k0, k4), (k1, k5), (k2, k6), (k3, k7)
+        union {
+          __half2 h[4];
+          uint4 u;
+        } d;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d.h[e] = __floats2half2_rn(f[e], f[e + 4]);
+        *reinterpret_cast<uint4*>(xs + (((xb[j] * 8 + my_step) * NT + (col >> 3)) * 32 + (col & 7) * 4 + my_i) * 16) = d.u;
+      };
+      if (split) {
+        put(2 * xr[j]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] -= __half2float(__float2half_rn(f[e]));
+        put(2 * xr[j] + 1);
+      } else {
+        put(xr[j]);
+      }
     }
+    block += kFly * kWarps;
+    if (block >= a.rows * a.kb) break;
   }
   __syncthreads();
   // a group's sums of x', times the weights' 2^-24: products with ones in the weights' place
@@ -459,16 +474,18 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
   uint32_t phase = 0;
   bool bad = false;
   for (;;) {
-    float tot[NT][4];
+    float tot[2][NT][4];  // rows my_row + 16 m, + 8; columns 8 n + 2 i, + 1
     bool head = job.jk != 0;  // a tile begun by an earlier warp is this warp's head; its own tiles have a place each
     bool fresh = true;
 #pragma unroll 1
     while (job.left > 0) {
       if (fresh) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int m = 0; m < 2; ++m)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) tot[n][e] = 0.f;
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) tot[m][n][e] = 0.f;
       }
       if (!bad && !mbar_wait(bars + 8 * stage, phase, s_abort, a.err)) bad = true;  // computes no more, keeps to the barriers
       if (!bad) {
@@ -478,46 +495,55 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
         const float* gs = xsum + job.jk * kSegs * NT * 8 + 2 * i;
 #pragma unroll
         for (int seg = 0; seg < kSegs; ++seg) {
-          const uint32_t s_lo = __shfl_sync(0xffffffffu, sz[seg % kHold], (lane & ~3) | seg / kHold);
-          const uint32_t s_hi = __shfl_sync(0xffffffffu, sz[seg % kHold], (lane & ~3) | 2 | seg / kHold);
-          // this lane's W words of rows my_row and my_row + 8
-          uint32_t w0[4], w1[4];
-          {
-            const int byte = (seg * 4 + i) * W * 4;
-            const uint32_t at = wrow + ((byte & ~15) ^ ((my_row & 7) << 4)) + (byte & 15);
-            if constexpr (W == 4) {
-              asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                           : "=r"(w0[0]), "=r"(w0[1]), "=r"(w0[2]), "=r"(w0[3]) : "r"(at) : "memory");
-              asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                           : "=r"(w1[0]), "=r"(w1[1]), "=r"(w1[2]), "=r"(w1[3]) : "r"(at + 1024) : "memory");
-            } else if constexpr (W == 2) {
-              asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w0[0]), "=r"(w0[1]) : "r"(at) : "memory");
-              asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w1[0]), "=r"(w1[1]) : "r"(at + 1024) : "memory");
-            } else {
-              asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w0[0]) : "r"(at) : "memory");
-              asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w1[0]) : "r"(at + 1024) : "memory");
-            }
-          }
-          float acc[NT][4] = {};
+          // this lane's W words of rows my_row + 8 r
+          uint32_t w[4][4];
+          const int byte = (seg * 4 + i) * W * 4;
+          const uint32_t at = wrow + ((byte & ~15) ^ (my_row << 4)) + (byte & 15);
 #pragma unroll
-          for (int w = 0; w < W; ++w) {
-            const uint32_t lo8 = w0[w] >> 8, hi8 = w1[w] >> 8;
+          for (int r = 0; r < 4; ++r) {
+            if constexpr (W == 4)
+              asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                           : "=r"(w[r][0]), "=r"(w[r][1]), "=r"(w[r][2]), "=r"(w[r][3]) : "r"(at + 1024 * r) : "memory");
+            else if constexpr (W == 2)
+              asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[r][0]), "=r"(w[r][1]) : "r"(at + 1024 * r) : "memory");
+            else
+              asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[r][0]) : "r"(at + 1024 * r) : "memory");
+          }
+          float acc[2][NT][4] = {};
+#pragma unroll
+          for (int j = 0; j < W; ++j) {
+            uint32_t h[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) h[r] = w[r][j] >> 8;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              const uint4 b = *reinterpret_cast<const uint4*>(xf + ((seg * W + w) * NT + n) * 512);
-              mma_f16(acc[n], w0[w] & 0x000f000fu, w1[w] & 0x000f000fu, w0[w] & 0x00f000f0u, w1[w] & 0x00f000f0u, b.x, b.y);
-              mma_f16(acc[n], lo8 & 0x000f000fu, hi8 & 0x000f000fu, lo8 & 0x00f000f0u, hi8 & 0x00f000f0u, b.z, b.w);
+              const uint4 b = *reinterpret_cast<const uint4*>(xf + ((seg * W + j) * NT + n) * 512);
+#pragma unroll
+              for (int m = 0; m < 2; ++m) {
+                const uint32_t p = w[2 * m][j], q = w[2 * m + 1][j];
+                mma_f16(acc[m][n], p & 0x000f000fu, q & 0x000f000fu, p & 0x00f000f0u, q & 0x00f000f0u, b.x, b.y);
+              }
+#pragma unroll
+              for (int m = 0; m < 2; ++m) {
+                const uint32_t p = h[2 * m], q = h[2 * m + 1];
+                mma_f16(acc[m][n], p & 0x000f000fu, q & 0x000f000fu, p & 0x00f000f0u, q & 0x00f000f0u, b.z, b.w);
+              }
             }
           }
-          const float f_lo = low_half<T>(s_lo) * 16777216.f, f_hi = low_half<T>(s_hi) * 16777216.f;  // the weights' 2^24
-          const float z_lo = low_half<T>(s_lo >> 16), z_hi = low_half<T>(s_hi >> 16);
+          float f[4], z[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            f[r] = half_of<T>(__shfl_sync(0xffffffffu, sc[seg / 2], (lane & ~3) | r), seg & 1) * 16777216.f;  // the weights' 2^24
+            z[r] = byte_of(__shfl_sync(0xffffffffu, zp[seg / 4], (lane & ~3) | r), seg & 3);
+          }
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             const float2 xg = *reinterpret_cast<const float2*>(gs + (seg * NT + n) * 8);
-            tot[n][0] = fmaf(f_lo, fmaf(-z_lo, xg.x, acc[n][0]), tot[n][0]);
-            tot[n][1] = fmaf(f_lo, fmaf(-z_lo, xg.y, acc[n][1]), tot[n][1]);
-            tot[n][2] = fmaf(f_hi, fmaf(-z_hi, xg.x, acc[n][2]), tot[n][2]);
-            tot[n][3] = fmaf(f_hi, fmaf(-z_hi, xg.y, acc[n][3]), tot[n][3]);
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                tot[m][n][e] = fmaf(f[2 * m + e / 2], fmaf(-z[2 * m + e / 2], e & 1 ? xg.y : xg.x, acc[m][n][e]), tot[m][n][e]);
           }
         }
         __syncwarp();  // every lane has read the stage
@@ -529,58 +555,98 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
       job.step(a);
       fresh = job.jk == 0;
       if (fresh || job.left == 0) {
-        float* dst = part + (head ? a.tiles_round + warp : tile) * kTileFloats + my_row;
+        float* dst = part + (head ? a.tiles_round + warp : tile) * tile_floats + my_row;
         head = false;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          dst[(8 * n + 2 * i) * kPitch] = tot[n][0], dst[(8 * n + 2 * i + 1) * kPitch] = tot[n][1];
-          dst[(8 * n + 2 * i) * kPitch + 8] = tot[n][2], dst[(8 * n + 2 * i + 1) * kPitch + 8] = tot[n][3];
-        }
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int col = 8 * n + 2 * i + (e & 1);
+              if (col < cols) dst[col * kPitch + 16 * m + 8 * (e / 2)] = tot[m][n][e];
+            }
       }
     }
-    if (a.s > 1) cluster_sync_all(); else __syncthreads();
+    __syncthreads();
 
-    // ---- the round's outputs: partial tiles of the warps and CTAs added in their order
+    if (a.s > 1 && job.round == tile0) cluster_wait();
+    // ---- the round's outputs: the warps' partial tiles, then the CTAs', added in their order
     const int total = min(a.tiles_round, tile_end - job.round) * a.kb;
     const int n0 = job.round * tile_n, width = min(min(a.tiles_round, tile_end - job.round) * tile_n, a.n - n0);
-    for (int at = rank * kThreads + tid; at < width * a.rows; at += a.s * kThreads) {
-      const int r = at / width, c = at - r * width, tile = c / tile_n;
-      const int place = (split ? 2 * r : r) * kPitch + c - tile * tile_n;
+    // four neighbouring outputs a thread
+    const int quads = (width + 3) / 4, count = quads * a.rows, share = (count + a.s - 1) / a.s;
+    const float per_row = 1.f / (float)quads;
+    const auto add4 = [](float4& y, const float* p) {
+      const float4 v = *reinterpret_cast<const float4*>(p);
+      y.x += v.x, y.y += v.y, y.z += v.z, y.w += v.w;
+    };
+    const auto finish = [&](int r, int c, float4 y, const float4& u) {
+      float v[4] = {y.x, y.y, y.z, y.w};
+      const float w[4] = {u.x, u.y, u.z, u.w};
+      T* out = static_cast<T*>(a.out) + r * a.out_stride + n0 + c;
+      const T* res = static_cast<const T*>(a.residual) + r * a.res_stride + n0 + c;
+      union {
+        T t[4];
+        uint2 u;
+      } d;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (pair) v[e] = v[e] / (1.f + expf(-v[e])) * w[e];
+        if (a.mode == AICAS_LINEAR_RESIDUAL && c + e < width) v[e] += Elem<T>::to_float(res[e]);
+        d.t[e] = Elem<T>::from_float(v[e]);
+      }
+      if (a.out_quads && c + 3 < width) {
+        *reinterpret_cast<uint2*>(out) = d.u;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (c + e < width) out[e] = d.t[e];
+      }
+    };
+    for (int at = tid; at < count; at += kThreads) {
+      const int r = (int)((at + 0.5f) * per_row), c = 4 * (at - r * quads);  // at / quads: below 2^14 and 2^9
+      const int tile = c / tile_n, place = (split ? 2 * r : r) * kPitch + c - tile * tile_n;
       const int heads = s_heads[tile], w0 = heads & 0xffff, w1 = heads >> 16;
-      float y0 = 0.f, y1 = 0.f;
-#pragma unroll 1
+      float4 y = make_float4(0.f, 0.f, 0.f, 0.f), u = y;
       for (int w = w0; w <= w1; ++w) {
         if (w * total / kWarps == (w + 1) * total / kWarps) continue;  // a warp without jobs
-        const float* p = part + (w == w0 ? tile : a.tiles_round + w) * kTileFloats + place;
-        if (a.s == 1) {
-          y0 += split ? p[0] + p[kPitch] : p[0];
-          if (pair) y1 += split ? p[8] + p[kPitch + 8] : p[8];
-        } else {
-#pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            if (q >= a.s) break;
-            const float inv = ld_cluster(smem_u32(s_inv + r), q);
-            float t = ld_cluster(smem_u32(p), q);
-            if (split) t += ld_cluster(smem_u32(p + kPitch), q);
-            y0 = fmaf(t, inv, y0);
-            if (pair) {
-              t = ld_cluster(smem_u32(p + 8), q);
-              if (split) t += ld_cluster(smem_u32(p + 8 + kPitch), q);
-              y1 = fmaf(t, inv, y1);
-            }
-          }
+        const float* p = part + (w == w0 ? tile : a.tiles_round + w) * tile_floats + place;
+        add4(y, p);
+        if (split) add4(y, p + kPitch);
+        if (pair) {
+          add4(u, p + 16);
+          if (split) add4(u, p + kPitch + 16);
         }
       }
-      if (a.s == 1) y0 *= s_inv[r], y1 *= s_inv[r];
-      if (pair) y0 = y0 / (1.f + expf(-y0)) * y1;
-      if (a.mode == AICAS_LINEAR_RESIDUAL)
-        y0 += Elem<T>::to_float(static_cast<const T*>(a.residual)[r * a.res_stride + n0 + c]);
-      static_cast<T*>(a.out)[r * a.out_stride + n0 + c] = Elem<T>::from_float(y0);
+      const float inv = s_inv[r];
+      y.x *= inv, y.y *= inv, y.z *= inv, y.w *= inv;
+      u.x *= inv, u.y *= inv, u.z *= inv, u.w *= inv;
+      if (a.s == 1) {
+        finish(r, c, y, u);
+      } else {  // to the CTA that finishes these outputs
+        const int owner = at / share, slot = rank * share + at - owner * share;
+        st_cluster(recv + 4 * slot, owner, y);
+        if (pair) st_cluster(recv + 4 * (a.s * share + slot), owner, u);
+      }
+    }
+    if (a.s > 1) {
+      cluster_sync_all();
+      for (int at = rank * share + tid; at < min(count, (rank + 1) * share); at += kThreads) {
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f), u = y;
+        for (int q = 0; q < a.s; ++q) {
+          add4(y, recv + 4 * (q * share + at - rank * share));
+          if (pair) add4(u, recv + 4 * ((a.s + q) * share + at - rank * share));
+        }
+        const int r = (int)((at + 0.5f) * per_row);
+        finish(r, 4 * (at - r * quads), y, u);
+      }
     }
     job.round += a.tiles_round;
     if (job.round >= tile_end) break;
     job.cut(a, tile_end);
-    if (a.s > 1) cluster_sync_all(); else __syncthreads();  // the partial tiles have been read
+    // the partial tiles have been read, the received ones in every CTA
+    if (a.s > 1) cluster_sync_all(); else __syncthreads();
     if (tile_end - job.round < a.tiles_round) find_heads(tile_end - job.round);  // read after the next barrier
   }
   if (bad)
@@ -588,7 +654,6 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
       mbar_wait(bars + 8 * stage, phase, nullptr, a.err);
       if (++stage == a.stages) stage = 0, phase ^= 1;
     }
-  if (a.s > 1) cluster_sync_all();  // no CTA leaves while its partial tiles are read
 }
 
 // ------------------------------------------------------------------ host side
@@ -687,23 +752,25 @@ cudaError_t dispatch_int4(int nt, int group, const Int4Args& a, int smem, int sm
   return cudaErrorInvalidValue;
 }
 
-// Shared memory of a launch of nt column blocks with K split s ways; 0: does not fit.
-int plan_int4(Int4Args* a, int nt, int s, int sms) {
+// Shared memory of a launch of nt column blocks with K split s ways and rings of at least `deep` jobs; 0: does not fit.
+int plan_int4(Int4Args* a, int nt, int s, int rows, int cols, int deep, int sms) {
   const int jobs = (a->k + kJobK - 1) / kJobK;
   a->s = s;
   a->kb = (jobs + s - 1) / s;
   // a round holds a cluster's tiles, if shared memory does
-  const int most = nt == 8 ? 8 : kMaxRound / nt, want = (int)((int64_t)a->tiles * s * 4 / (3 * sms)) + 1;
+  const int most = cols <= 8 ? kMaxRound : kMaxRound * 8 / cols, want = (int)((int64_t)a->tiles * s * 4 / (3 * sms)) + 1;
   a->tiles_round = want < most ? want : most;
   const int warps = warps_for(nt);
-  const int part = (a->tiles_round + warps) * nt * 8 * kPitch * 4, xs = a->kb * nt * 4096;
+  const int part = (a->tiles_round + warps) * cols * kPitch * 4, xs = a->kb * nt * 4096;
+  const int recv = s > 1 ? a->tiles_round * (a->mode == AICAS_LINEAR_SWIGLU ? 2 * 16 : 32) * rows * 4 + 32 * s : 0;
   const int sums = a->kb * (kJobK / (a->k / a->groups)) * nt * 32;
-  const int tail = warps * 8 * 8 + kVarBytes, rest = part + xs + sums + tail, ring = warps * kJobBytes;
+  const int tail = warps * 8 * 8 + kVarBytes + 16, rest = part + recv + xs + sums + tail, ring = warps * kJobBytes;
   a->stages = (kMaxSmem - rest) / ring;
-  if (a->stages < 3) return 0;
+  if (a->stages < deep) return 0;
   if (a->stages > 8) a->stages = 8;
   a->off_part = a->stages * ring;
-  a->off_x = a->off_part + part;
+  a->off_recv = a->off_part + part;
+  a->off_x = a->off_recv + (recv + 15) / 16 * 16;
   a->off_sum = a->off_x + xs;
   a->off_bars = a->off_sum + sums;
   return a->off_bars + tail;
@@ -716,17 +783,22 @@ int run_linear_int4(const aicas_linear_int4_params* p, int sms, cudaStream_t str
   const bool pair = p->mode == AICAS_LINEAR_SWIGLU, bf16 = p->dtype == AICAS_DTYPE_BF16;
   Int4Args a;
   memset(&a, 0, sizeof(a));
+  a.whole = 1;
   for (int j = 0; j < (pair ? 2 : 1); ++j) {
-    if (!weight_map(&a.tm_w[j], p->w[j], p->out_features, p->in_features, pair ? 8 : 16, err, errlen))
+    if (!weight_map(&a.tm_w[j], p->w[j], p->out_features, p->in_features, pair ? 16 : 32, err, errlen))
       return AICAS_ERR_UNSUPPORTED;
     a.scales[j] = p->w[j].scales;
     a.zeros[j] = static_cast<const uint8_t*>(p->w[j].zeros);
+    const int segs = kJobK / p->group_size;
+    if (p->in_features % kJobK != 0 || reinterpret_cast<uintptr_t>(a.scales[j]) % (2 * segs) != 0 ||
+        reinterpret_cast<uintptr_t>(a.zeros[j]) % segs != 0)
+      a.whole = 0;
   }
   a.norm_weight = p->norm_weight;
   a.x_stride = p->x_stride, a.res_stride = p->residual_stride, a.out_stride = p->out_stride;
   a.k = p->in_features, a.n = p->out_features, a.groups = p->in_features / p->group_size;
   a.mode = p->mode, a.eps = p->eps, a.err = dev_err;
-  const int tile_n = pair ? 8 : 16;
+  const int tile_n = pair ? 16 : 32;
   a.tiles = (p->out_features + tile_n - 1) / tile_n;
   // every row at once where x' fits on chip over a cluster of up to 8 CTAs, else fewer rows a launch
   const int columns = p->norm_weight != nullptr && !bf16 ? 2 : 1;  // a normalised x' for an fp16 result: two parts
@@ -734,7 +806,8 @@ int run_linear_int4(const aicas_linear_int4_params* p, int sms, cudaStream_t str
   for (;; batch = (batch + 1) / 2) {
     const int blocks = (batch * columns + 7) / 8;
     nt = blocks <= 1 ? 1 : blocks <= 2 ? 2 : blocks <= 4 ? 4 : 8;
-    for (int s = 1; s <= 8 && smem == 0; s *= 2) smem = plan_int4(&a, nt, s, sms);
+    for (int deep = 3; deep >= 2 && smem == 0; --deep)  // rings of three jobs a warp, if some split leaves room for them
+      for (int s = 1; s <= 8 && smem == 0; s *= 2) smem = plan_int4(&a, nt, s, batch, batch * columns, deep, sms);
     if (smem != 0) break;
     if (batch == 1) {
       snprintf(err, errlen, "int4 linear: in_features %d is more than shared memory holds", p->in_features);
@@ -745,6 +818,7 @@ int run_linear_int4(const aicas_linear_int4_params* p, int sms, cudaStream_t str
     a.rows = p->rows - r < batch ? p->rows - r : batch;
     a.x = static_cast<const uint16_t*>(p->x) + r * p->x_stride;
     a.out = static_cast<uint16_t*>(p->out) + r * p->out_stride;
+    a.out_quads = reinterpret_cast<uintptr_t>(a.out) % 8 == 0 && (a.rows == 1 || p->out_stride % 4 == 0);
     a.residual = p->residual != nullptr ? static_cast<const uint16_t*>(p->residual) + r * p->residual_stride : nullptr;
     const cudaError_t e = bf16 ? dispatch_int4<__nv_bfloat16>(nt, p->group_size, a, smem, sms, stream)
                                : dispatch_int4<__half>(nt, p->group_size, a, smem, sms, stream);
