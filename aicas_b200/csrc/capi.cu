@@ -433,6 +433,8 @@ int check_paged_append(const aicas_paged_append_params* p) {
     if (s < 0 || !stride_ok(s, eb)) return fail(AICAS_ERR_INVALID, "q/k/v strides must be non-negative multiples of 16 bytes");
   if (p->cs_stride_b < 0 || p->cs_stride_s < 0 || !stride_ok(p->cs_stride_b, ceb) || !stride_ok(p->cs_stride_s, ceb))
     return fail(AICAS_ERR_INVALID, "cos/sin strides must be non-negative multiples of 16 bytes");
+  if (p->kv_lens_out != nullptr && p->kv_lens_out == p->positions)
+    return fail(AICAS_ERR_INVALID, "kv_lens_out must not be positions");
   if ((p->q_norm_weight != nullptr || p->k_norm_weight != nullptr) && !(p->norm_eps >= 0.0f))
     return fail(AICAS_ERR_INVALID, "norm_eps must be >= 0");
   return AICAS_OK;

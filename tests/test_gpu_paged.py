@@ -437,6 +437,8 @@ def test_append_refusals(cuda_device):
         ("kv_lens_out", {"kv_lens_out": torch.zeros(2, dtype=torch.int64, device=cuda_device)}),
         ("norm weights", {"q_norm_weight": torch.ones(64, device=cuda_device)}),
         ("q_out", {"q_out": ok["query"][:, :, :, :32]}),
+        ("must not be positions", dict.fromkeys(["positions", "kv_lens_out"],
+                                                torch.zeros(2, dtype=torch.int32, device=cuda_device))),
         ("not a multiple", {"query": torch.zeros(2, 3, 1, 64, dtype=torch.bfloat16, device=cuda_device)}),
     ]:
         with pytest.raises(ValueError, match=text):
