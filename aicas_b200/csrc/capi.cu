@@ -454,8 +454,8 @@ int check_paged_decode(const aicas_paged_decode_params* p) {
     if (s < 0 || !stride_ok(s, eb)) return fail(AICAS_ERR_INVALID, "q/out strides must be non-negative multiples of 16 bytes");
   if (!(p->sm_scale == p->sm_scale) || p->sm_scale == INFINITY || p->sm_scale == -INFINITY)
     return fail(AICAS_ERR_INVALID, "sm_scale must be finite");
-  // the kernel numbers 16-slot tiles of (request, KV head, block of query heads) with 32-bit ints
-  const int64_t tiles = (((int64_t)p->max_pages * p->page_size + 15) / 16 + 1) * p->batch *
+  // the kernel numbers 16-slot tiles of (request, KV head, block of query heads), and a few more each, with 32-bit ints
+  const int64_t tiles = (((int64_t)p->max_pages * p->page_size + 15) / 16 + 16) * p->batch *
                         ((int64_t)p->num_kv_heads * ((p->num_q_heads / p->num_kv_heads + 15) / 16));
   if (tiles > (int64_t)INT32_MAX / 2)
     return fail(AICAS_ERR_UNSUPPORTED, "%lld tiles of 16 slots exceed the 2^30 of one launch", (long long)tiles);

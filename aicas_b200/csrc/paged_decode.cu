@@ -10,15 +10,18 @@
 //   * Work: the 16-slot tiles of all (request, KV head) pairs, numbered pair by
 //     pair, are cut into equal ranges, one per CTA (one CTA an SM).  The cut is
 //     made on the device from the lengths, so the host neither knows nor bounds
-//     them and ragged batches balance to a tile.  A pair inside one range is
-//     finished there; a pair that crosses ranges leaves one fp32 partial a CTA
-//     (a CTA has at most two: its first and its last pair), and the last CTA to
-//     arrive adds them in CTA order, so results repeat to the bit.
-//   * Copies: each warp streams its own tiles (every kWarps-th of the CTA's
-//     range) through a private ring of TMA boxes, swizzled so that ldmatrix
-//     reads them without bank conflicts; no warp waits for another inside a
-//     pair.  Page numbers for the next 32 tiles are fetched by the lanes at
-//     once.  A page number outside the pool is an out-of-range box: zeros.
+//     them and ragged batches balance to a tile; a pair counts kPairCost tiles more
+//     for its beginning and end (64 ragged caches of up to 4096 slots, while the warps
+//     still copied for themselves: 96 us against 101 without it).  A pair inside one range is finished there; a pair that crosses ranges
+//     leaves one fp32 partial a CTA (a CTA has at most two: its first and its last
+//     pair), and the last CTA to arrive adds them in CTA order, so results repeat to
+//     the bit.  A small launch of few pairs gives each pair CTAs of its own.
+//   * Copies: two warps stream the range's K and V tiles as TMA boxes, swizzled so
+//     that ldmatrix reads them without bank conflicts, into a ring of its own for
+//     each of the other warps, which take the tiles in turn; no warp waits for
+//     another inside a pair.  (Warps that copied for themselves spent as long, 900
+//     cycles a tile, at issuing the copies as at the products.)  A page number
+//     outside the pool is an out-of-range box: zeros.
 //   * Products: mma.sync m16n8k16 with the group's query heads as rows (a
 //     larger group takes several blocks of 16).  At a few percent of the SM's
 //     tensor rate the legacy path is not the bound, and it keeps scores and
@@ -39,12 +42,14 @@ namespace aicas {
 namespace {
 
 constexpr int kTile = 16;       // slots a tile
+constexpr int kPairCost = 6;    // what beginning and ending a pair costs a CTA, in tiles (3: 95.2, 6: 93.9, 10: 93.4 us)
 constexpr int kMinChunk = 16;   // fewest tiles a CTA takes
+constexpr int kSmallTiles = 32;   // most tiles a CTA of a launch that gives pairs whole CTAs
 constexpr int kRowsMax = 16;    // query heads of a block
 constexpr size_t kWsCounters = (size_t)1 << 20;  // counter region shared with the contiguous decode
 
 struct PagedArgs {
-  CUtensorMap tm_k, tm_v;
+  CUtensorMap tm_k, tm_v;  // 5-D: (128 bytes of D, rows, parts of D, heads, pages), a box all of D of 16 (or 8) rows
   const void* q;
   void* out;
   float* lse;
@@ -54,8 +59,10 @@ struct PagedArgs {
   int64_t q_sb, q_sh, o_sb, o_sh, table_stride;
   int batch, hq, hkv, group, row_blocks;
   int page_size, cap;
-  int k_rows_first, v_rows_first;  // 1: map dims (D, rows, heads, pages); 0: (D, heads, rows, pages)
+  int few;                         // at most half as many pairs as CTAs
   int boxes;                       // boxes of a tile: 1 (16 rows) or 2 (8 rows: page sizes of 8, 24, ...)
+  // a tile in shared memory: bytes from one 128-byte part of D to the next, and from rows 0..7 to rows 8..15
+  int part_bytes, rows8_bytes;
   float scale_log2;
   float* ws_o;             // [2 * grid][kRowsMax][D]
   float* ws_ml;            // [2 * grid][kRowsMax][2]
@@ -68,22 +75,20 @@ struct PagedCfg {
   static constexpr bool kF32 = sizeof(T) == 4;
   static constexpr int kRowBytes = D * (int)sizeof(T);
   static constexpr int kInner = kRowBytes < 128 ? kRowBytes : 128;  // bytes of a box's row (the swizzle's width)
-  static constexpr int kHalves = kRowBytes / kInner;                // boxes along D
   static constexpr int kSwzMask = kInner / 16 - 1;
   static constexpr int kTileBytes = kTile * kRowBytes;
   static constexpr int kStageBytes = 2 * kTileBytes;  // K tile, V tile
-  static constexpr int kWarps = kF32 ? 4 : 8;
-  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kWarps = kF32 ? 4 : 8;              // warps at the products; two more copy K and V
+  static constexpr int kConsumers = kWarps * 32, kThreads = kConsumers + 64;
   static constexpr int kRing = 196608 / kWarps / kStageBytes;
   static constexpr int kStages = kRing < 8 ? kRing : 8;
-  static constexpr int kRedRow = D + 8;  // the 8 keeps the fragment stores free of bank conflicts
+  static constexpr int kRedRow = D + 4;  // a row's output, its maximum and its sum
   static constexpr int kOffRed = kWarps * kStages * kStageBytes;
-  static constexpr int kOffMl = kOffRed + kWarps * 8 * kRedRow * 4;
-  static constexpr int kOffQ = kOffMl + kWarps * 8 * 2 * 4;  // fp32: the block's query rows
-  static constexpr int kOffBars = kOffQ + (kF32 ? kRowsMax * D * 4 : 0);
-  static constexpr int kOffVars = kOffBars + kWarps * kStages * 8;
+  static constexpr int kOffQ = kOffRed + kWarps * 8 * kRedRow * 4;  // fp32: the block's query rows
+  static constexpr int kOffBars = kOffQ + (kF32 ? kRowsMax * D * 4 : 0);  // [warp][stage] full, then empty
+  static constexpr int kOffVars = kOffBars + 2 * kWarps * kStages * 8;
   // no static shared memory beside it: the ring starts 1024-byte aligned, as the swizzle wants
-  static constexpr int kSmem = kOffVars + 64;
+  static constexpr int kSmem = kOffVars + 16;
   static_assert(kStages >= 3 && kSmem <= 232448, "shared memory");
 };
 
@@ -135,15 +140,29 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint3
 
 // ------------------------------------------------------------------ the CTA's range
 
-// The tiles [t0, t1) of one (request, KV head, row block) in a CTA's range.
-// Tiles count from the one that holds the request's first slot.
+// Units of work: a pair counts its tiles and, before them, kPairCost units for
+// beginning and ending it, so that a CTA with many short pairs gets fewer tiles.
+//
+// The tiles [t0, t1) of one pair (request, KV head and row block) in a CTA's
+// range; none where the range ends in the pair's cost.  Tiles count from the one
+// that holds the request's first slot.
 struct Segment {
   int b, pair;        // request; KV head * row_blocks + row block
   int t0, t1, nt;     // this CTA's tiles, all tiles of the pair
   int first_tile;     // tile of the first slot
   int start, len;     // slots [start, len)
-  int base;           // number of the request's first tile in the launch
-  int left;           // tiles of the CTA's range after this segment
+  int base;           // number of the request's first unit in the launch
+  int left;           // units of the CTA's range after this segment
+
+  __device__ __forceinline__ int units() const { return nt + kPairCost; }
+  __device__ __forceinline__ int pair_base() const { return base + pair * units(); }
+  // The pair's units [from, from + count), as far as it has them.
+  __device__ __forceinline__ void take(int from, int count) {
+    const int to = min(units(), from + count);
+    left = count - (to - from);
+    t0 = max(0, from - kPairCost);
+    t1 = max(0, to - kPairCost);
+  }
 };
 
 __device__ __forceinline__ void request_bounds(const PagedArgs& a, int b, int& start, int& len, int& nt) {
@@ -152,110 +171,128 @@ __device__ __forceinline__ void request_bounds(const PagedArgs& a, int b, int& s
   nt = len > start ? (len + kTile - 1) / kTile - start / kTile : 0;
 }
 
-// Fills a segment from tile `tile` of the launch, which lies in request s.b.
-__device__ __forceinline__ void segment_at(const PagedArgs& a, Segment& s, int tile, int count) {
+__device__ __forceinline__ int request_units(const PagedArgs& a, int nt) {
+  return nt == 0 ? 0 : (nt + kPairCost) * a.hkv * a.row_blocks;
+}
+
+// Fills a segment from unit `unit` of the launch, which lies in request s.b.
+__device__ __forceinline__ void segment_at(const PagedArgs& a, Segment& s, int unit, int count) {
   request_bounds(a, s.b, s.start, s.len, s.nt);
   s.first_tile = s.start / kTile;
-  const int off = tile - s.base;
-  s.pair = off / s.nt;
-  s.t0 = off - s.pair * s.nt;
-  s.t1 = min(s.nt, s.t0 + count);
-  s.left = count - (s.t1 - s.t0);
+  const int off = unit - s.base;
+  s.pair = off / s.units();
+  s.take(off - s.pair * s.units(), count);
 }
 
 __device__ __forceinline__ bool segment_next(const PagedArgs& a, Segment& s) {
   if (s.left == 0) return false;
   if (++s.pair == a.hkv * a.row_blocks) {
-    s.base += s.nt * a.hkv * a.row_blocks;
+    s.base += s.units() * a.hkv * a.row_blocks;
     s.pair = 0;
     do {
-      ++s.b;  // tiles are left, so a request with some follows
+      ++s.b;  // units are left, so a request with some follows
       request_bounds(a, s.b, s.start, s.len, s.nt);
     } while (s.nt == 0);
     s.first_tile = s.start / kTile;
   }
-  s.t0 = 0;
-  s.t1 = min(s.nt, s.left);
-  s.left -= s.t1;
+  s.take(0, s.left);
   return true;
 }
 
-// ------------------------------------------------------------------ a warp's copies
+// The warps at the products among themselves.
+template <int THREADS>
+__device__ __forceinline__ void consumers_sync() {
+  asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
+}
 
-template <typename T, int D>
-struct Loader {
-  using C = PagedCfg<T, D>;
-  Segment seg;
-  int tile;          // next tile of the segment to copy
-  int batch;         // tile whose page this warp's lane 0 holds
-  int page0, row0, page1, row1;  // this lane's tile: page and row of its (up to) two boxes
-  bool done;
+// ------------------------------------------------------------------ the copying warps
 
-  __device__ __forceinline__ void fetch_pages(const PagedArgs& a) {
-    const int lane = threadIdx.x & 31;
-    batch = tile;
-    const int t = tile + lane * C::kWarps;
-    page0 = page1 = -1;
-    row0 = row1 = 0;
-    if (t < seg.t1) {
-      const int slot = (seg.first_tile + t) * kTile;
-      const int32_t* row = a.table + seg.b * a.table_stride;
-      const int i = slot / a.page_size;
-      row0 = slot - i * a.page_size;
-      page0 = row[i];
-      if (a.boxes == 2 && slot + 8 < seg.len) {
-        const bool same = row0 + 8 < a.page_size;
-        row1 = same ? row0 + 8 : 0;
-        page1 = same ? page0 : row[i + 1];
-      }
-    }
-  }
+__device__ __forceinline__ void copy_box(const CUtensorMap& m, uint32_t dst, int row, int head, int page, uint32_t bar,
+                                         uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%2, %3, %2, %4, %5}], [%6], %7;" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(&m)), "r"(0), "r"(row), "r"(head), "r"(page),
+      "r"(bar), "l"(policy)
+      : "memory");
+}
 
-  // Copies this warp's next tile into a stage; false when none is left.
-  __device__ __forceinline__ bool issue(const PagedArgs& a, uint32_t dst, uint32_t bar, uint64_t policy) {
-    if (done) return false;
-    const int warp = threadIdx.x >> 5;
-    while (tile >= seg.t1) {
-      if (!segment_next(a, seg)) {
-        done = true;
-        return false;
-      }
-      tile = seg.t0 + warp;
-      fetch_pages(a);
-    }
-    if (tile - batch >= 32 * C::kWarps) fetch_pages(a);
-    const int src = (tile - batch) / C::kWarps;
-    const int p0 = __shfl_sync(0xffffffffu, page0, src), r0 = __shfl_sync(0xffffffffu, row0, src);
-    const int p1 = __shfl_sync(0xffffffffu, page1, src), r1 = __shfl_sync(0xffffffffu, row1, src);
-    if ((threadIdx.x & 31) == 0) {
-      mbar_arrive_expect_tx(bar, C::kStageBytes);
-      const int head = seg.pair / a.row_blocks;
-#pragma unroll
-      for (int h = 0; h < C::kHalves; ++h) {
-        const int x = h * (C::kInner / (int)sizeof(T));
-        const uint32_t d = dst + h * kTile * C::kInner;
-        box(a.tm_k, a.k_rows_first, d, x, r0, head, p0, bar, policy);
-        box(a.tm_v, a.v_rows_first, d + C::kTileBytes, x, r0, head, p0, bar, policy);
-        if (a.boxes == 2) {
-          box(a.tm_k, a.k_rows_first, d + 8 * C::kInner, x, r1, head, p1, bar, policy);
-          box(a.tm_v, a.v_rows_first, d + C::kTileBytes + 8 * C::kInner, x, r1, head, p1, bar, policy);
-        }
-      }
-    }
-    tile += C::kWarps;
-    return true;
-  }
-
-  __device__ __forceinline__ static void box(const CUtensorMap& m, int rows_first, uint32_t dst, int x, int row,
-                                             int head, int page, uint32_t bar, uint64_t policy) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
-        " [%0], [%1, {%2, %3, %4, %5}], [%6], %7;" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(&m)), "r"(x), "r"(rows_first ? row : head), "r"(rows_first ? head : row),
-        "r"(page), "r"(bar), "l"(policy)
-        : "memory");
-  }
+// A lane's tile of a batch of 32: page and row of its (up to) two boxes.
+struct Pages {
+  int page0, row0, page1, row1;
 };
+
+__device__ __forceinline__ Pages pages_of(const PagedArgs& a, const Segment& s, int t) {
+  Pages p = {-1, 0, -1, 0};
+  if (t < s.t1) {
+    const int slot = (s.first_tile + t) * kTile;
+    const int32_t* row = a.table + s.b * a.table_stride;
+    const int i = slot / a.page_size;
+    p.row0 = slot - i * a.page_size;
+    p.page0 = row[i];
+    if (a.boxes == 2 && slot + 8 < s.len) {
+      const bool same = p.row0 + 8 < a.page_size;
+      p.row1 = same ? p.row0 + 8 : 0;
+      p.page1 = same ? p.page0 : row[i + 1];
+    }
+  }
+  return p;
+}
+
+// Copies all K (or V) tiles of the CTA's range: tile number n of it to stage
+// (n / kWarps) % kStages of warp n % kWarps.  A lane a tile, kWarps lanes at a time, so that the
+// wait for a free stage and the page numbers' way are paid once for kWarps tiles
+// (a tile at a time took 0.42 us each).  bars: full barriers, then empty ones.
+template <typename T, int D>
+__device__ void copy_range(const PagedArgs& a, const CUtensorMap& map, Segment seg, uint32_t ring, uint32_t bars,
+                           volatile int* abort) {
+  using C = PagedCfg<T, D>;
+  const int lane = threadIdx.x & 31;
+  const uint64_t policy = l2_policy_evict_first();
+  const uint32_t empty = bars + C::kWarps * C::kStages * 8;
+  int number = 0;  // of the segment's next tile
+  bool ok = true;
+  Pages at = pages_of(a, seg, seg.t0 + lane);
+  while (ok) {
+    const int head = seg.pair / a.row_blocks;
+    Segment next = seg;
+    bool more = true;
+    for (int t = seg.t0; t < seg.t1 && ok; t += 32) {
+      // the next batch's page numbers are on their way while this one is copied
+      Pages ahead = {};
+      if (t + 32 < seg.t1) {
+        ahead = pages_of(a, seg, t + 32 + lane);
+      } else {
+        do more = segment_next(a, next);
+        while (more && next.t0 == next.t1);
+        if (more) ahead = pages_of(a, next, next.t0 + lane);
+      }
+      const int count = min(32, seg.t1 - t);
+      const int n = number + lane, turn = n / C::kWarps, round = turn / C::kStages;
+      const int place = n % C::kWarps * C::kStages + turn % C::kStages;
+      const uint32_t dst = ring + place * C::kStageBytes, bar = bars + 8 * place;
+      for (int first = 0; first < count && ok; first += C::kWarps) {
+        if (lane >= first && lane < min(first + C::kWarps, count)) {
+          if (round > 0) ok = mbar_wait(empty + 8 * place, (round - 1) & 1, abort, a.err);
+          if (ok) {
+            mbar_arrive_expect_tx(bar, C::kTileBytes);
+            copy_box(map, dst, at.row0, head, at.page0, bar, policy);
+            if (a.boxes == 2) copy_box(map, dst + C::kTileBytes / 2, at.row1, head, at.page1, bar, policy);
+          }
+        }
+        ok = __all_sync(0xffffffffu, ok);
+      }
+      number += count;
+      at = ahead;
+    }
+    if (seg.t0 == seg.t1) {  // the range begins in a pair's cost: nothing of it to copy
+      more = segment_next(a, next);
+      if (more) at = pages_of(a, next, next.t0 + lane);
+    }
+    if (!more) break;
+    seg = next;
+  }
+}
 
 // ------------------------------------------------------------------ a warp's state, 16-bit caches
 
@@ -271,13 +308,12 @@ struct WarpState {
   uint32_t k_off, v_off;  // this lane's row of the ldmatrix tiles, with its share of the swizzle
   uint32_t k_swz, v_swz;
 
-  __device__ __forceinline__ void init(const uint8_t*) {
+  __device__ __forceinline__ void init(const PagedArgs& a, const uint8_t*) {
     const int lane = threadIdx.x & 31, mat = lane >> 3, r = lane & 7;
-    const int krow = (mat >> 1) * 8 + r, vrow = (mat & 1) * 8 + r;
-    k_off = krow * C::kInner;
-    v_off = vrow * C::kInner;
-    k_swz = ((((krow * C::kInner) >> 7) & C::kSwzMask) << 4) ^ ((mat & 1) << 4);
-    v_swz = ((((vrow * C::kInner) >> 7) & C::kSwzMask) << 4) ^ ((mat >> 1) << 4);
+    k_off = (mat >> 1) * a.rows8_bytes + r * C::kInner;
+    v_off = (mat & 1) * a.rows8_bytes + r * C::kInner + C::kTileBytes;
+    k_swz = ((((r * C::kInner) >> 7) & C::kSwzMask) << 4) ^ ((mat & 1) << 4);
+    v_swz = ((((r * C::kInner) >> 7) & C::kSwzMask) << 4) ^ ((mat >> 1) << 4);
   }
 
   __device__ __forceinline__ void begin(const PagedArgs& a, const Segment& s, uint8_t*) {
@@ -307,10 +343,10 @@ struct WarpState {
   __device__ __forceinline__ void tile(const PagedArgs& a, uint32_t at, int lo, int hi) {
     const int i = threadIdx.x & 3;
     // ---- scores of 16 slots: s[n][0..1] = (row g, slots 8 n + 2 i, + 1), s[n][2..3] = row g + 8
-    float s[2][4] = {};
+    float s[2][4] = {}, s2[2][4] = {};  // even and odd steps: two shorter chains of products
 #pragma unroll
     for (int j = 0; j < kSteps; ++j) {
-      const uint32_t sub = (uint32_t)(j * 32 / C::kInner) * kTile * C::kInner;
+      const uint32_t sub = (uint32_t)(j * 32 / C::kInner) * a.part_bytes;
       uint32_t kf[4];
       ldsm_x4(at + sub + k_off + (((j * 32) & (C::kInner - 1)) ^ k_swz), kf);
       uint32_t af[4];
@@ -319,15 +355,15 @@ struct WarpState {
       } else {
         af[0] = qf[j][0], af[1] = qf[j][1], af[2] = qf[j][2], af[3] = qf[j][3];
       }
-      Mma<T>::run(s[0], af, kf[0], kf[1]);
-      Mma<T>::run(s[1], af, kf[2], kf[3]);
+      Mma<T>::run(j & 1 ? s2[0] : s[0], af, kf[0], kf[1]);
+      Mma<T>::run(j & 1 ? s2[1] : s[1], af, kf[2], kf[3]);
     }
     const bool edge = lo > 0 || hi < kTile;
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 2 * kH; ++e) {
-        s[n][e] *= a.scale_log2;
+        s[n][e] = (s[n][e] + s2[n][e]) * a.scale_log2;
         const int slot = 8 * n + 2 * i + (e & 1);
         if (edge && (slot < lo || slot >= hi)) s[n][e] = -INFINITY;
       }
@@ -383,9 +419,9 @@ struct WarpState {
     }
 #pragma unroll
     for (int c = 0; c < D / 8; c += 2) {
-      const uint32_t sub = (uint32_t)(c * 16 / C::kInner) * kTile * C::kInner;
+      const uint32_t sub = (uint32_t)(c * 16 / C::kInner) * a.part_bytes;
       uint32_t vf[4];
-      ldsm_x4_t(at + C::kTileBytes + sub + v_off + (((c * 16) & (C::kInner - 1)) ^ v_swz), vf);
+      ldsm_x4_t(at + sub + v_off + (((c * 16) & (C::kInner - 1)) ^ v_swz), vf);
 #pragma unroll
       for (int e = 0; e < 4; ++e) vf[e] &= keep[e & 1];
       Mma<T>::run(o[c], ph, vf[0], vf[1]);
@@ -398,7 +434,7 @@ struct WarpState {
   }
 
   // Rows 8 h .. 8 h + 7 into this warp's part of the reduction buffer.
-  __device__ __forceinline__ void put(int h, float* red, float* ml) {
+  __device__ __forceinline__ void put(int h, float* red) {
     const int lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3;
     float sum = l[RM == 8 ? 0 : h];
     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
@@ -414,7 +450,7 @@ struct WarpState {
       }
       *reinterpret_cast<float2*>(row + 8 * n) = v;
     }
-    if (i == 0) ml[2 * g] = m[RM == 8 ? 0 : h], ml[2 * g + 1] = sum;
+    if (i == 0) *reinterpret_cast<float2*>(red + g * C::kRedRow + D) = make_float2(m[RM == 8 ? 0 : h], sum);
   }
 };
 
@@ -429,7 +465,7 @@ struct WarpState<float, D, RM> {
   float m[RM], l[RM];
   const float* qs;
 
-  __device__ __forceinline__ void init(const uint8_t* q_smem) { qs = reinterpret_cast<const float*>(q_smem); }
+  __device__ __forceinline__ void init(const PagedArgs&, const uint8_t* q_smem) { qs = reinterpret_cast<const float*>(q_smem); }
 
   // Every thread of the CTA copies a share of the block's query rows (zeros past the group).
   __device__ __forceinline__ void begin(const PagedArgs& a, const Segment& s, uint8_t* q_smem) {
@@ -437,8 +473,8 @@ struct WarpState<float, D, RM> {
     const int rows = min(kRowsMax, a.group - h0);
     const float* q = static_cast<const float*>(a.q) + s.b * a.q_sb + (int64_t)(kvh * a.group + h0) * a.q_sh;
     float* dst = reinterpret_cast<float*>(q_smem);
-    for (int x = threadIdx.x; x < RM * D; x += C::kThreads) dst[x] = x / D < rows ? q[(x / D) * a.q_sh + x % D] : 0.f;
-    __syncthreads();
+    for (int x = threadIdx.x; x < RM * D; x += C::kConsumers) dst[x] = x / D < rows ? q[(x / D) * a.q_sh + x % D] : 0.f;
+    consumers_sync<C::kConsumers>();
 #pragma unroll
     for (int r = 0; r < RM; ++r) {
       m[r] = -INFINITY, l[r] = 0.f;
@@ -447,9 +483,10 @@ struct WarpState<float, D, RM> {
     }
   }
 
-  __device__ __forceinline__ static uint32_t at_col(int row, int col) {  // byte offset of a 16-byte column
-    const int byte = col * 16, sub = byte / C::kInner, in = byte % C::kInner;
-    return sub * kTile * C::kInner + row * C::kInner + (in ^ ((((row * C::kInner) >> 7) & C::kSwzMask) << 4));
+  __device__ __forceinline__ static uint32_t at_col(const PagedArgs& a, int row, int col) {  // byte offset of a 16-byte column
+    const int byte = col * 16, r = row & 7;
+    return byte / C::kInner * a.part_bytes + (row >> 3) * a.rows8_bytes + r * C::kInner +
+           (byte % C::kInner ^ ((((r * C::kInner) >> 7) & C::kSwzMask) << 4));
   }
 
   __device__ __forceinline__ static float4 lds4(uint32_t addr) {
@@ -465,7 +502,7 @@ struct WarpState<float, D, RM> {
     const int lane = threadIdx.x & 31, slot = lane & 15, half = lane >> 4;
     float s[RM] = {};
     for (int c = half; c < kCols; c += 2) {
-      const float4 k = lds4(at + at_col(slot, c));
+      const float4 k = lds4(at + at_col(a, slot, c));
 #pragma unroll
       for (int r = 0; r < RM; ++r) {
         const float4 q = *reinterpret_cast<const float4*>(qs + r * D + 4 * c);
@@ -490,7 +527,7 @@ struct WarpState<float, D, RM> {
     const int col = lane % kCols, kg = lane / kCols;
     for (int t0 = 0; t0 < kTile; t0 += kGroups) {
       const int t = t0 + kg;
-      float4 v = lds4(at + C::kTileBytes + at_col(t, col));
+      float4 v = lds4(at + C::kTileBytes + at_col(a, t, col));
       if (t < lo || t >= hi) v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int r = 0; r < RM; ++r) {
@@ -501,7 +538,7 @@ struct WarpState<float, D, RM> {
     }
   }
 
-  __device__ __forceinline__ void put(int h, float* red, float* ml) {
+  __device__ __forceinline__ void put(int h, float* red) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int r = 0; r < RM; ++r) {
@@ -515,7 +552,7 @@ struct WarpState<float, D, RM> {
         for (int off = kCols; off < 32; off <<= 1) o[r][e] += __shfl_xor_sync(0xffffffffu, o[r][e], off);
       if (lane < kCols) *reinterpret_cast<float4*>(red + (r & 7) * C::kRedRow + 4 * lane) =
           make_float4(o[r][0], o[r][1], o[r][2], o[r][3]);
-      if (lane == 0) ml[2 * (r & 7)] = m[r], ml[2 * (r & 7) + 1] = sum;
+      if (lane == 0) *reinterpret_cast<float2*>(red + (r & 7) * C::kRedRow + D) = make_float2(m[r], sum);
     }
   }
 };
@@ -553,35 +590,42 @@ __global__ void __launch_bounds__(PagedCfg<T, D>::kThreads, 1) paged_decode_kern
   int* vars = reinterpret_cast<int*>(smem + C::kOffVars);
   int& s_abort = vars[0];
   int& s_last = vars[1];
-  int* s_find = vars + 2;
-  int* s_warp = vars + 4;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
-  const uint32_t ring = smem_u32(smem) + warp * C::kStages * C::kStageBytes;
-  const uint32_t bars = smem_u32(smem + C::kOffBars) + warp * C::kStages * 8;
+  const uint32_t all_bars = smem_u32(smem + C::kOffBars);
   float* red = reinterpret_cast<float*>(smem + C::kOffRed);
-  float* ml = reinterpret_cast<float*>(smem + C::kOffMl);
   if (tid == 0) s_abort = 0;
-  if (lane == 0) {
-    for (int s = 0; s < C::kStages; ++s) mbar_init(bars + 8 * s, 1);
-    fence_mbar_init();
-  }
+  if (tid < 2 * C::kWarps * C::kStages) mbar_init(all_bars + 8 * tid, tid < C::kWarps * C::kStages ? 2 : 1);  // K and V; the reader
+  fence_mbar_init();
   grid_launch_dependents();
+  __syncthreads();
   grid_dependency_wait();
 
-  // ---- the launch's tiles before each thread's requests (a run of requests a thread)
-  const int per = a.hkv * a.row_blocks;
-  const int run = (a.batch + C::kThreads - 1) / C::kThreads;
-  const int b0 = min(a.batch, tid * run), b1 = min(a.batch, b0 + run);
+  // ---- the launch's units before each lane's requests (a run of requests a lane; every warp for itself)
+  const int run = (a.batch + 31) / 32, per = a.hkv * a.row_blocks, pairs = a.batch * per;
+  const int b0 = min(a.batch, lane * run), b1 = min(a.batch, b0 + run);
+  int tiles = 0, full_pairs = 0;
+#pragma unroll 4
+  for (int b = b0; b < b1; ++b) {
+    int start, len, nt;
+    request_bounds(a, b, start, len, nt);
+    tiles += nt * per;
+    full_pairs += nt > 0 ? per : 0;
+  }
+  tiles = __reduce_add_sync(0xffffffffu, tiles);
+  full_pairs = __reduce_add_sync(0xffffffffu, full_pairs);
+  // A small launch of few pairs: whole CTAs a pair, as short as they go (latency); else equal ranges (bandwidth).
+  const bool small = a.few && tiles <= (int)gridDim.x * kSmallTiles;
+  const int ctas = (int)gridDim.x - (small ? pairs : 0);  // small: at most tiles / chunk + pairs are needed
+  const int units = tiles + (small ? 0 : full_pairs * kPairCost);
+  int chunk = max((units + ctas - 1) / ctas, kMinChunk);  // units of a CTA; small: its tiles
+  if (small) chunk = (chunk + C::kWarps - 1) / C::kWarps * C::kWarps;
+  // what a request counts: units, or (small) CTAs
+  const auto share = [&](int nt) { return small ? (nt + chunk - 1) / chunk * per : request_units(a, nt); };
   int mine = 0;
   for (int b = b0; b < b1; ++b) {
     int start, len, nt;
     request_bounds(a, b, start, len, nt);
-    mine += nt * per;
-    if (nt == 0 && b % (int)gridDim.x == (int)blockIdx.x) {
-      // nothing to attend to: zeros (few requests: one thread a request)
-      for (int x = 0; x < a.hq * D / 4; ++x)
-        write_result<T>(a, b, x / (D / 4), x % (D / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, 0.f);
-    }
+    mine += share(nt);
   }
   int before = mine;
 #pragma unroll
@@ -589,70 +633,86 @@ __global__ void __launch_bounds__(PagedCfg<T, D>::kThreads, 1) paged_decode_kern
     const int v = __shfl_up_sync(0xffffffffu, before, off);
     if (lane >= off) before += v;
   }
-  if (lane == 31) s_warp[warp] = before;
-  __syncthreads();
-  int total = 0;
+  const int total = __shfl_sync(0xffffffffu, before, 31);
   before -= mine;
-#pragma unroll
-  for (int w = 0; w < C::kWarps; ++w) {
-    if (w < warp) before += s_warp[w];
-    total += s_warp[w];
-  }
-  const int chunk = max((total + (int)gridDim.x - 1) / (int)gridDim.x, kMinChunk);
-  const int64_t r64 = (int64_t)blockIdx.x * chunk;
-  if (r64 >= total) return;  // the same for every thread of the CTA
-  const int r0 = (int)r64, count = min(chunk, total - r0);
-  if (r0 >= before && r0 < before + mine) {
-    int at = before;
-    for (int b = b0; b < b1; ++b) {
-      int start, len, nt;
-      request_bounds(a, b, start, len, nt);
-      if (r0 < at + nt * per) {
-        s_find[0] = b;
-        s_find[1] = at;
-        break;
-      }
-      at += nt * per;
-    }
-  }
-  __syncthreads();
+  const int64_t r64 = small ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * chunk;
+  const bool busy = r64 < total;
 
   Segment seg;
-  seg.b = s_find[0];
-  seg.base = s_find[1];
-  segment_at(a, seg, r0, count);
+  int split_first = 0, split_last = 0;  // small: the CTAs of this CTA's pair
+  if (busy) {
+    const int r0 = (int)r64;
+    int b = 0, at = before;
+    const bool here = r0 >= before && r0 < before + mine;
+    if (here)
+      for (b = b0;; ++b) {
+        int start, len, nt;
+        request_bounds(a, b, start, len, nt);
+        if (r0 < at + share(nt)) break;
+        at += share(nt);
+      }
+    const int src = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+    seg.b = __shfl_sync(0xffffffffu, b, src);
+    seg.base = __shfl_sync(0xffffffffu, at, src);
+    if (small) {
+      request_bounds(a, seg.b, seg.start, seg.len, seg.nt);
+      seg.first_tile = seg.start / kTile;
+      const int splits = (seg.nt + chunk - 1) / chunk, off = r0 - seg.base;
+      seg.pair = off / splits;
+      seg.t0 = (off - seg.pair * splits) * chunk;
+      seg.t1 = min(seg.nt, seg.t0 + chunk);
+      seg.left = 0;
+      split_first = seg.base + seg.pair * splits;
+      split_last = split_first + splits - 1;
+    } else {
+      segment_at(a, seg, r0, min(chunk, total - r0));
+    }
+    if (warp >= C::kWarps) {
+      const bool v = warp > C::kWarps;
+      copy_range<T, D>(a, v ? a.tm_v : a.tm_k, seg, smem_u32(smem) + (v ? C::kTileBytes : 0), all_bars, &s_abort);
+      return;
+    }
+  } else if (warp >= C::kWarps) {
+    return;
+  }
 
-  // ---- fill the ring
-  const uint64_t policy = l2_policy_evict_first();
-  Loader<T, D> ld;
-  ld.seg = seg;
-  ld.tile = seg.t0 + warp;
-  ld.done = false;
-  ld.fetch_pages(a);
-  int flying = 0;  // copies issued and not yet waited for
-#pragma unroll 1
-  for (int s = 0; s < C::kStages; ++s) flying += ld.issue(a, ring + s * C::kStageBytes, bars + 8 * s, policy);
+  if (full_pairs < pairs)  // requests with nothing to attend to: zeros
+    for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+      int start, len, nt;
+      request_bounds(a, b, start, len, nt);
+      if (nt == 0)
+        for (int x = tid; x < a.hq * (D / 4); x += C::kConsumers)
+          write_result<T>(a, b, x / (D / 4), x % (D / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, 0.f);
+    }
+  if (!busy) return;
 
+  const uint32_t ring = smem_u32(smem) + warp * C::kStages * C::kStageBytes;
+  const uint32_t full = all_bars + warp * C::kStages * 8, empty = full + C::kWarps * C::kStages * 8;
   WarpState<T, D, RM> st;
-  st.init(smem + C::kOffQ);
-  int stage = 0;
+  st.init(a, smem + C::kOffQ);
+  int stage = 0, turn = 0;  // turn: the warp that takes the segment's first tile
   uint32_t phase = 0;
   bool bad = false;
-  for (bool first = true;; first = false) {
+  for (bool first = true;;) {
+    if (seg.t0 == seg.t1) {
+      if (!segment_next(a, seg)) break;
+      continue;
+    }
     st.begin(a, seg, smem + C::kOffQ);
 #pragma unroll 1
-    for (int t = seg.t0 + warp; t < seg.t1; t += C::kWarps) {
+    for (int t = seg.t0 + (warp - turn + C::kWarps) % C::kWarps; t < seg.t1; t += C::kWarps) {
       if (bad) continue;
-      if (!mbar_wait(bars + 8 * stage, phase, &s_abort, a.err)) {
-        bad = true;  // this warp computes and copies no more, but keeps to the barriers below
+      if (!mbar_wait(full + 8 * stage, phase, &s_abort, a.err)) {
+        bad = true;  // this warp computes no more, but keeps to the barriers below
         continue;
       }
       const int slot = (seg.first_tile + t) * kTile;
       st.tile(a, ring + stage * C::kStageBytes, seg.start - slot, seg.len - slot);
       __syncwarp();  // every lane has read the stage
-      flying += ld.issue(a, ring + stage * C::kStageBytes, bars + 8 * stage, policy) - 1;
+      if (lane == 0) mbar_arrive(empty + 8 * stage);
       if (++stage == C::kStages) stage = 0, phase ^= 1;
     }
+    turn = (turn + seg.t1 - seg.t0) % C::kWarps;
 
     // ---- the warps' states into one, 8 rows a round
     const int kvh = seg.pair / a.row_blocks, h0 = (seg.pair - kvh * a.row_blocks) * kRowsMax;
@@ -663,20 +723,22 @@ __global__ void __launch_bounds__(PagedCfg<T, D>::kThreads, 1) paged_decode_kern
 #pragma unroll
     for (int h = 0; h < RM / 8; ++h) {
       if (h * 8 >= rows) break;
-      st.put(h, red + warp * 8 * C::kRedRow, ml + warp * 16);
-      __syncthreads();
-      for (int x = tid; x < min(8, rows - 8 * h) * (D / 4); x += C::kThreads) {
+      st.put(h, red + warp * 8 * C::kRedRow);
+      consumers_sync<C::kConsumers>();
+      for (int x = tid; x < min(8, rows - 8 * h) * (D / 4); x += C::kConsumers) {
         const int r = x / (D / 4), d = x % (D / 4) * 4;
         float M = -INFINITY, L = 0.f;
 #pragma unroll
-        for (int w = 0; w < C::kWarps; ++w) M = fmaxf(M, ml[w * 16 + 2 * r]);
+        for (int w = 0; w < C::kWarps; ++w) M = fmaxf(M, red[(w * 8 + r) * C::kRedRow + D]);
         const float use = M == -INFINITY ? 0.f : M;
         float4 o4 = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < C::kWarps; ++w) {
-          const float f = exp2f(ml[w * 16 + 2 * r] - use);
-          const float4 v = *reinterpret_cast<const float4*>(red + (w * 8 + r) * C::kRedRow + d);
-          L = fmaf(f, ml[w * 16 + 2 * r + 1], L);
+          const float* row = red + (w * 8 + r) * C::kRedRow;
+          const float2 ml = *reinterpret_cast<const float2*>(row + D);
+          const float f = exp2f(ml.x - use);
+          const float4 v = *reinterpret_cast<const float4*>(row + d);
+          L = fmaf(f, ml.y, L);
           o4.x = fmaf(f, v.x, o4.x), o4.y = fmaf(f, v.y, o4.y);
           o4.z = fmaf(f, v.z, o4.z), o4.w = fmaf(f, v.w, o4.w);
         }
@@ -687,13 +749,15 @@ __global__ void __launch_bounds__(PagedCfg<T, D>::kThreads, 1) paged_decode_kern
           if (d == 0) *reinterpret_cast<float2*>(a.ws_ml + (ws_row + 8 * h + r) * 2) = make_float2(M, L);
         }
       }
-      __syncthreads();
+      consumers_sync<C::kConsumers>();
     }
 
     // ---- a pair cut by ranges: the last CTA to arrive joins the partials in CTA order
     if (!whole) {
-      const int pair0 = seg.base + seg.pair * seg.nt;                     // the pair's first tile in the launch
-      const int c0 = pair0 / chunk, c1 = (pair0 + seg.nt - 1) / chunk;    // the CTAs it crosses
+      const int pair0 = seg.pair_base();
+      // the CTAs with tiles of it
+      const int c0 = small ? split_first : (pair0 + kPairCost) / chunk;
+      const int c1 = small ? split_last : (pair0 + seg.units() - 1) / chunk;
       if (tid == 0) {
         unsigned int prev;
         // after the barrier, so cumulative over the CTA's stores of its partial
@@ -701,10 +765,10 @@ __global__ void __launch_bounds__(PagedCfg<T, D>::kThreads, 1) paged_decode_kern
         s_last = prev == (unsigned int)(c1 - c0);
         if (s_last) a.ws_count[c0] = 0u;  // as the next call expects it
       }
-      __syncthreads();
+      consumers_sync<C::kConsumers>();
       if (s_last) {
-        const int first_slot = pair0 % chunk == 0 ? 0 : 1;  // of CTA c0; the others hold it as their first
-        for (int x = tid; x < rows * (D / 4); x += C::kThreads) {
+        const int first_slot = small || c0 * chunk >= pair0 ? 0 : 1;  // of CTA c0; the others hold it as their first
+        for (int x = tid; x < rows * (D / 4); x += C::kConsumers) {
           const int r = x / (D / 4), d = x % (D / 4) * 4;
           float M = -INFINITY, L = 0.f;
           float4 o4 = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -740,20 +804,15 @@ __global__ void __launch_bounds__(PagedCfg<T, D>::kThreads, 1) paged_decode_kern
         }
       }
     }
+    first = false;
     if (!segment_next(a, seg)) break;
   }
-  // a warp that gave up leaves once its copies have landed (bounded again)
-  if (bad)
-    for (; flying > 0; --flying) {
-      mbar_wait(bars + 8 * stage, phase, nullptr, a.err);
-      if (++stage == C::kStages) stage = 0, phase ^= 1;
-    }
 }
 
 // ------------------------------------------------------------------ host side
 
 bool pages_map(CUtensorMap* m, const void* ptr, const aicas_paged_decode_params* p, int64_t sp, int64_t sh, int64_t st,
-               int box_rows, int* rows_first, char* err, size_t errlen) {
+               int box_rows, char* err, size_t errlen) {
   EncodeTiledFn enc = tensor_map_encoder();
   if (enc == nullptr) {
     snprintf(err, errlen, "cuTensorMapEncodeTiled is unavailable from the driver");
@@ -763,23 +822,19 @@ bool pages_map(CUtensorMap* m, const void* ptr, const aicas_paged_decode_params*
   // a dimension of one entry may carry any stride: give it a valid one
   if (p->num_kv_heads == 1) sh = st * p->page_size;
   if (p->num_pages == 1) sp = st * p->page_size + sh * p->num_kv_heads;
-  *rows_first = st <= sh;
-  const cuuint64_t rows = (cuuint64_t)p->page_size, heads = (cuuint64_t)p->num_kv_heads;
-  const cuuint64_t dims[4] = {(cuuint64_t)p->head_dim, *rows_first ? rows : heads, *rows_first ? heads : rows,
-                              (cuuint64_t)p->num_pages};
-  const cuuint64_t strides[3] = {(cuuint64_t)(*rows_first ? st : sh) * eb, (cuuint64_t)(*rows_first ? sh : st) * eb,
-                                 (cuuint64_t)sp * eb};
   const int row_bytes = p->head_dim * eb, inner = row_bytes < 128 ? row_bytes : 128;
-  const cuuint32_t box[4] = {(cuuint32_t)(inner / eb), *rows_first ? (cuuint32_t)box_rows : 1u,
-                             *rows_first ? 1u : (cuuint32_t)box_rows, 1u};
-  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const cuuint64_t dims[5] = {(cuuint64_t)(inner / eb), (cuuint64_t)p->page_size, (cuuint64_t)(row_bytes / inner),
+                              (cuuint64_t)p->num_kv_heads, (cuuint64_t)p->num_pages};
+  const cuuint64_t strides[4] = {(cuuint64_t)st * eb, (cuuint64_t)inner, (cuuint64_t)sh * eb, (cuuint64_t)sp * eb};
+  const cuuint32_t box[5] = {(cuuint32_t)(inner / eb), (cuuint32_t)box_rows, (cuuint32_t)(row_bytes / inner), 1u, 1u};
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   const CUtensorMapDataType type = p->dtype == AICAS_DTYPE_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                    : p->dtype == AICAS_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                                  : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const CUtensorMapSwizzle swz = inner == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
                                  : inner == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
                                                : CU_TENSOR_MAP_SWIZZLE_32B;
-  const CUresult r = enc(m, type, 4, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
+  const CUresult r = enc(m, type, 5, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     snprintf(err, errlen, "cuTensorMapEncodeTiled failed (%d) for pages of strides %lld, %lld, %lld", (int)r,
@@ -789,11 +844,12 @@ bool pages_map(CUtensorMap* m, const void* ptr, const aicas_paged_decode_params*
   return true;
 }
 
-// CTAs of a launch: an SM each, or fewer where even full caches have fewer runs of kMinChunk tiles.
+// CTAs of a launch: as many as the SMs hold, or fewer where even full caches have fewer runs of kMinChunk tiles.
 int paged_grid(const aicas_paged_decode_params* p, int sms) {
   const int64_t cap_tiles = ((int64_t)p->max_pages * p->page_size + kTile - 1) / kTile;
   const int blocks = (p->num_q_heads / p->num_kv_heads + kRowsMax - 1) / kRowsMax;
-  const int64_t runs = (cap_tiles * p->batch * p->num_kv_heads * blocks + kMinChunk - 1) / kMinChunk;
+  const int64_t pairs = (int64_t)p->batch * p->num_kv_heads * blocks;
+  const int64_t runs = (cap_tiles * pairs + kMinChunk - 1) / kMinChunk + pairs;
   return (int)(runs < sms ? runs : sms);
 }
 
@@ -835,10 +891,8 @@ int run_paged_decode(const aicas_paged_decode_params* p, int sms, void* workspac
   PagedArgs a;
   memset(&a, 0, sizeof(a));
   const int box_rows = p->page_size % kTile == 0 ? kTile : 8;
-  if (!pages_map(&a.tm_k, p->k_pages, p, p->kp_stride_p, p->kp_stride_h, p->kp_stride_t, box_rows, &a.k_rows_first, err,
-                 errlen) ||
-      !pages_map(&a.tm_v, p->v_pages, p, p->vp_stride_p, p->vp_stride_h, p->vp_stride_t, box_rows, &a.v_rows_first, err,
-                 errlen))
+  if (!pages_map(&a.tm_k, p->k_pages, p, p->kp_stride_p, p->kp_stride_h, p->kp_stride_t, box_rows, err, errlen) ||
+      !pages_map(&a.tm_v, p->v_pages, p, p->vp_stride_p, p->vp_stride_h, p->vp_stride_t, box_rows, err, errlen))
     return AICAS_ERR_UNSUPPORTED;
   a.q = p->q, a.out = p->out, a.lse = p->lse;
   a.table = p->page_table, a.lens = p->kv_lens, a.starts = p->kv_starts;
@@ -850,8 +904,12 @@ int run_paged_decode(const aicas_paged_decode_params* p, int sms, void* workspac
   a.page_size = p->page_size;
   a.cap = p->max_pages * p->page_size;
   a.boxes = kTile / box_rows;
+  const int row_bytes = p->head_dim * (p->dtype == AICAS_DTYPE_F32 ? 4 : 2), inner = row_bytes < 128 ? row_bytes : 128;
+  a.part_bytes = box_rows * inner;
+  a.rows8_bytes = a.boxes == 2 ? 8 * row_bytes : 8 * inner;
   a.scale_log2 = p->sm_scale * 1.4426950408889634f;
   const int grid = paged_grid(p, sms);
+  a.few = 2 * (int64_t)a.batch * a.hkv * a.row_blocks <= grid;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   a.ws_count = reinterpret_cast<unsigned int*>(ws);
   a.ws_o = reinterpret_cast<float*>(ws + kWsCounters);

@@ -241,6 +241,13 @@ def test_decode_pages_and_lengths(cuda_device, layout, size):
     _decode_case(cuda_device, "bf16", 64, 4, 2, size, lens, layout=layout, seed=size)
 
 
+@pytest.mark.parametrize("dtype,dim", [("bf16", 16), ("fp16", 32), ("bf16", 128), ("fp32", 16), ("fp32", 32), ("fp32", 64),
+                                       ("fp32", 128)])
+@pytest.mark.parametrize("size", [8, 24, 48])
+def test_decode_page_sizes_at_every_row_width(cuda_device, dtype, dim, size):
+    _decode_case(cuda_device, dtype, dim, 4, 2, size, [1, 8, 9, 23, 24, 25, 100, 256, 333], seed=dim)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 @pytest.mark.parametrize("size", [8, 16, 24])
 def test_decode_skips_the_first_slots(cuda_device, dtype, size):
@@ -263,6 +270,40 @@ def test_decode_long_caches(cuda_device, dtype, size, lens):
 def test_decode_many_short_requests(cuda_device):
     rng = np.random.RandomState(0)
     _decode_case(cuda_device, "bf16", 32, 4, 2, 8, rng.randint(0, 60, 700).tolist(), spoil=False)
+
+
+@pytest.mark.parametrize("lens", [
+    [1] * 2500,                                    # one tile a request: most warps have nothing to copy
+    [20, 1, 0, 33] * 500 + [3000],                 # and a long cache after them
+    [9000] + [0] * 300 + [17] * 1500 + [6000, 2],
+    [16] * 40 + [30000] + [16] * 40 + [1] * 2000 + [15000],
+])
+@pytest.mark.parametrize("dim,dtype", [(16, "fp16"), (64, "bf16"), (32, "fp32")])
+def test_decode_claimed_ranges(cuda_device, lens, dim, dtype):
+    """Launches large enough for ranges that the CTAs claim, of short and long requests mixed."""
+    g = torch.Generator().manual_seed(len(lens))
+    B, hkv, size = len(lens), 8, 16
+    pages = 400
+    kp, vp = _pool(g, pages, hkv, size, dim, dtype, "hnd", cuda_device)
+    per = -(-max(lens) // size)
+    table = torch.randint(0, pages, (B, per), generator=g, dtype=torch.int32).to(cuda_device)
+    q = torch.randn(B, 16, 1, dim, generator=g).to(DT[dtype]).to(cuda_device)
+    kw = dict(sm_scale=dim ** -0.5, num_key_value_groups=2, kv_lens=torch.tensor(lens, dtype=torch.int32))
+    out, lse = ab.paged_gqa_decode_attention(q, kp, vp, table, return_lse=True, **kw)
+    for _ in range(3):
+        again = ab.paged_gqa_decode_attention(q, kp, vp, table, **kw)
+        assert torch.equal(again, out)
+    assert nat.device_error_flags() == 0
+    pick = sorted(set([0, 1, 2, 3, 40, 41, 300, 301, B // 2, B - 3, B - 2, B - 1]))
+    ref, ref_lse = op.decode(_np(q[pick]), _np(kp), _np(vp), table[pick].cpu().numpy(), [lens[b] for b in pick],
+                             [0] * len(pick), dim ** -0.5, 2)
+    _near(out[pick], ref, dtype, 2e-5 if dtype == "fp32" else 1e-3)
+    _near(lse[pick], ref_lse, "fp32", 1e-4)
+    # every request: a batch of few requests takes equal ranges without claims
+    for b0 in range(0, B, 250):
+        part = ab.paged_gqa_decode_attention(q[b0:b0 + 250], kp, vp, table[b0:b0 + 250],
+                                             **(kw | {"kv_lens": torch.tensor(lens[b0:b0 + 250], dtype=torch.int32)}))
+        assert (part.float() - out[b0:b0 + 250].float()).abs().max().item() <= 2e-2
 
 
 def test_decode_large_scores(cuda_device):
