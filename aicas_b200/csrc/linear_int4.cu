@@ -80,7 +80,7 @@ struct Int4Args {
 
 __device__ __forceinline__ void mma_f16(float c[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -296,45 +296,61 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
   const uint16_t* const my_scales = static_cast<const uint16_t*>(up ? a.scales[1] : a.scales[0]);
   const int n_off = my_row + 8 * (pair ? i & 1 : i);
   uint32_t sc[kSegs / 2], zp[(kSegs + 3) / 4], next_s[kSegs / 2], next_z[(kSegs + 3) / 4];
+  int64_t s_at = 0;     // of the next job's first group
+  bool s_row = false;   // this lane's row exists
+  bool s_new = true;    // the next job begins a tile, a round or the range
   const auto fetch = [&]() {
-    if (!sj.settle(a, tile_end)) return;
-    const int t = sj.round + sj.tile, n = t * tile_n + n_off, grp0 = (kb0 + sj.jk) * kSegs;
-    sj.step(a);
-    const int64_t at = (int64_t)n * a.groups + grp0;
+    if (sj.left == 0) {
+      if (!sj.settle(a, tile_end)) return;
+      s_new = true;
+    }
+    const int grp0 = (kb0 + sj.jk) * kSegs;
+    if (s_new) {
+      const int t = sj.round + sj.tile, n = t * tile_n + n_off;
+      s_at = (int64_t)n * a.groups + grp0;
+      s_row = n < a.n;
+      if (t + a.tiles_round < tile_end && n + a.tiles_round * tile_n < a.n) {  // the next round's, a line of each kind
+        const int64_t next = s_at + (int64_t)a.tiles_round * tile_n * a.groups;
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(my_scales + next));
+        if (my_zeros != nullptr) asm volatile("prefetch.global.L2 [%0];" ::"l"(my_zeros + next));
+      }
+    }
 #pragma unroll
     for (int j = 0; j < (kSegs + 3) / 4; ++j) next_z[j] = 0x08080808u;
-    if (n < a.n && a.whole) {
+    if (s_row && a.whole) {
       // K is whole jobs: a row's groups of a job are one aligned vector
       if constexpr (kSegs == 2) {
-        next_s[0] = *reinterpret_cast<const uint32_t*>(my_scales + at);
-        if (my_zeros != nullptr) next_z[0] = *reinterpret_cast<const uint16_t*>(my_zeros + at);
+        next_s[0] = *reinterpret_cast<const uint32_t*>(my_scales + s_at);
+        if (my_zeros != nullptr) next_z[0] = *reinterpret_cast<const uint16_t*>(my_zeros + s_at);
       } else if constexpr (kSegs == 4) {
-        const uint2 v = *reinterpret_cast<const uint2*>(my_scales + at);
+        const uint2 v = *reinterpret_cast<const uint2*>(my_scales + s_at);
         next_s[0] = v.x, next_s[1] = v.y;
-        if (my_zeros != nullptr) next_z[0] = *reinterpret_cast<const uint32_t*>(my_zeros + at);
+        if (my_zeros != nullptr) next_z[0] = *reinterpret_cast<const uint32_t*>(my_zeros + s_at);
       } else {
-        const uint4 v = *reinterpret_cast<const uint4*>(my_scales + at);
+        const uint4 v = *reinterpret_cast<const uint4*>(my_scales + s_at);
         next_s[0] = v.x, next_s[1] = v.y, next_s[2] = v.z, next_s[3] = v.w;
         if (my_zeros != nullptr) {
-          const uint2 z = *reinterpret_cast<const uint2*>(my_zeros + at);
+          const uint2 z = *reinterpret_cast<const uint2*>(my_zeros + s_at);
           next_z[0] = z.x, next_z[1] = z.y;
         }
       }
     } else {
 #pragma unroll
       for (int j = 0; j < kSegs / 2; ++j) next_s[j] = 0u;
-#pragma unroll
+#pragma unroll 1
       for (int j = 0; j < kSegs; ++j) {
-        if (n >= a.n || grp0 + j >= a.groups) continue;
-        next_s[j / 2] |= (uint32_t)my_scales[at + j] << (16 * (j & 1));
-        if (my_zeros != nullptr) next_z[j / 4] ^= (8u ^ my_zeros[at + j]) << (8 * (j & 3));
+        if (!s_row || grp0 + j >= a.groups) break;
+        const uint32_t v = (uint32_t)my_scales[s_at + j] << (16 * (j & 1));
+        const uint32_t z = my_zeros != nullptr ? (8u ^ my_zeros[s_at + j]) << (8 * (j & 3)) : 0u;
+#pragma unroll
+        for (int q = 0; q < kSegs / 2; ++q) next_s[q] |= q == j / 2 ? v : 0u;
+#pragma unroll
+        for (int q = 0; q < (kSegs + 3) / 4; ++q) next_z[q] ^= q == j / 4 ? z : 0u;
       }
     }
-    if (t + a.tiles_round < tile_end && n + a.tiles_round * tile_n < a.n && grp0 < a.groups) {
-      const int64_t next = at + (int64_t)a.tiles_round * tile_n * a.groups;
-      asm volatile("prefetch.global.L2 [%0];" ::"l"(my_scales + next));
-      if (my_zeros != nullptr) asm volatile("prefetch.global.L2 [%0];" ::"l"(my_zeros + next));
-    }
+    s_at += kSegs;
+    sj.step(a);
+    s_new = sj.jk == 0;
   };
   const auto take = [&]() {  // the fetched ones become the next job's
 #pragma unroll
@@ -503,11 +519,11 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
           for (int r = 0; r < 4; ++r) {
             if constexpr (W == 4)
               asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                           : "=r"(w[r][0]), "=r"(w[r][1]), "=r"(w[r][2]), "=r"(w[r][3]) : "r"(at + 1024 * r) : "memory");
+                           : "=r"(w[r][0]), "=r"(w[r][1]), "=r"(w[r][2]), "=r"(w[r][3]) : "r"(at + 1024 * r));
             else if constexpr (W == 2)
-              asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[r][0]), "=r"(w[r][1]) : "r"(at + 1024 * r) : "memory");
+              asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[r][0]), "=r"(w[r][1]) : "r"(at + 1024 * r));
             else
-              asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[r][0]) : "r"(at + 1024 * r) : "memory");
+              asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[r][0]) : "r"(at + 1024 * r));
           }
           float acc[2][NT][4] = {};
 #pragma unroll
