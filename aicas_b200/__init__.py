@@ -21,7 +21,7 @@ from .ops import (
     varlen_flash_attention,
     vision_rope,
 )
-from .paged import paged_gqa_decode_attention, paged_rope_kv_append
+from .paged import PagedKVCache, paged_gqa_decode_attention, paged_rope_kv_append
 from .patch import install_qwen3vl_triton_attention
 
 
@@ -37,6 +37,7 @@ def __getattr__(name: str):
 __all__ = [
     "Int4Weight",
     "NATIVE_AVAILABLE",
+    "PagedKVCache",
     "TEXT_BACKEND_KEY",
     "TRITON_AVAILABLE",
     "VISION_BACKEND_KEY",

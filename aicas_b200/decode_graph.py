@@ -193,10 +193,13 @@ class GraphGreedyDecoder:
         mm_token_type_ids, pixel_values, image_grid_thw).  Afterwards
         ``last_step_ms`` holds the mean device time of one replayed decode step
         (CUDA events around the replays)."""
-        graph, st = self.prefill_and_capture(inputs, max_new_tokens)
+        return self._replay(*self.prefill_and_capture(inputs, max_new_tokens))
+
+    def _replay(self, graph: torch.cuda.CUDAGraph | None, st: dict) -> torch.Tensor:
+        """All the replays that ``state["log"]`` has room for, timed; its tokens."""
         if graph is None:
             return st["log"]
-        device = st["log"].device
+        device, max_new_tokens = st["log"].device, st["log"].shape[1]
         stream = torch.cuda.current_stream(device)
         e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
         e0.record(stream)
@@ -244,23 +247,25 @@ class GraphGreedyDecoder:
             "log": log,
             "caches": [(layer.keys, layer.values) for layer in cache.layers],
         }
-        # warm-up run of the step on the capture stream (allocations, library
-        # set-up, the decode workspace of that stream), then the state is put
-        # back and the step captured
-        saved = {k: st[k].clone() for k in ("tok", "pos", "lens", "step", "log")}
-        saved_kv = [(kc[:, :, S].clone(), vc[:, :, S].clone()) for kc, vc in st["caches"]]
+        keep = [st[k] for k in ("tok", "pos", "lens", "step", "log")]
+        keep += [c[:, :, S] for kv in st["caches"] for c in kv]
+        return self._capture(st, keep), st
+
+    def _capture(self, st: dict, keep: list[torch.Tensor]) -> torch.cuda.CUDAGraph:
+        """Warm-up run of the step on the capture stream (allocations, library
+        set-up, the decode workspace of that stream); then what it changed,
+        ``keep``, is put back and the step captured."""
+        device = st["tok"].device
+        saved = [t.clone() for t in keep]
         stream = torch.cuda.Stream(device)
         stream.wait_stream(torch.cuda.current_stream(device))
         with torch.cuda.stream(stream):
             self._step(st)
         torch.cuda.current_stream(device).wait_stream(stream)
-        for k, v in saved.items():
-            st[k].copy_(v)
-        for (kc, vc), (k0, v0) in zip(st["caches"], saved_kv):
-            kc[:, :, S].copy_(k0)
-            vc[:, :, S].copy_(v0)
+        for t, v in zip(keep, saved):
+            t.copy_(v)
         torch.cuda.synchronize(device)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, stream=stream):
             self._step(st)
-        return graph, st
+        return graph

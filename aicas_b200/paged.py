@@ -1,5 +1,6 @@
 """Paged key-value cache: the append with the position rotation on the way, the
-single-token attention that reads it, and the pool that hands out the pages.
+single-token attention that reads it, and :class:`PagedKVCache`, which owns the
+pages and hands them out.
 
 A pool is a pair of tensors ``[P, Hkv, page_size, D]`` (or any view of that
 shape whose strides are multiples of 16 bytes with a contiguous ``D``, so a
@@ -201,3 +202,97 @@ def paged_gqa_decode_attention(
                 ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], table_stride,
                 B, Hq, Hkv, D, shape[0], shape[2], max_pages, _DTYPE_CODES[dtype], sm_scale))
     return (out, lse) if return_lse else out
+
+
+class PagedKVCache:
+    """Page pools of every layer and the host's account of who holds which page.
+
+    ``keys[i]`` / ``values[i]`` are the layers' pools ``[P, Hkv, page_size, D]``,
+    allocated once; a page number means the same page in each layer.  Requests
+    come (:meth:`add`), grow (:meth:`grow`) and go (:meth:`release`) on the host;
+    :meth:`page_table` writes their rows for the kernels.  Released pages keep
+    what they held: a kernel reads only the slots under the lengths it is given.
+    Work that reads a released page and is already on a stream must be ordered
+    before the work that writes its next holder's tokens (one stream does)."""
+
+    def __init__(self, num_layers: int, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, *,
+                 dtype: torch.dtype, device: torch.device | str):
+        if min(num_layers, num_pages, num_kv_heads) < 1:
+            raise ValueError("PagedKVCache needs a positive number of layers, pages and heads")
+        if page_size < 8 or page_size % 8:
+            raise ValueError(f"PagedKVCache: page_size must be a positive multiple of 8 (got {page_size})")
+        if dtype not in _DTYPE_CODES or head_dim not in SUPPORTED_HEAD_DIMS:
+            raise ValueError(f"PagedKVCache: dtype {dtype}, head_dim {head_dim} are not ones that the kernels take")
+        shape = (num_pages, num_kv_heads, page_size, head_dim)
+        self.page_size, self.num_pages = page_size, num_pages
+        self.keys = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(num_layers)]
+        self.values = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(num_layers)]
+        self._free = list(range(num_pages - 1, -1, -1))  # the lowest page goes out first
+        self._held: dict[int, list[int]] = {}
+        self._next = 0
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def pages(self, request: int) -> list[int]:
+        """The pages that ``request`` holds, in the order of its tokens."""
+        if request not in self._held:
+            raise ValueError(f"request {request} holds no pages in this cache")
+        return list(self._held[request])
+
+    def add(self, tokens: int) -> int:
+        """A new request with room for ``tokens`` tokens; its number."""
+        request = self._next
+        self._held[request] = []
+        try:
+            self.grow(request, tokens)
+        except ValueError:
+            del self._held[request]
+            raise
+        self._next += 1
+        return request
+
+    def grow(self, request: int, tokens: int) -> None:
+        """Gives ``request`` room for ``tokens`` tokens in all (never takes any away).
+        ``ValueError``, and nothing taken, where the pool has too few pages left."""
+        have = len(self.pages(request))
+        need = -(-tokens // self.page_size) - have
+        if tokens < 0:
+            raise ValueError("tokens must not be negative")
+        if need > len(self._free):
+            raise ValueError(f"paged cache is full: {need} pages needed, {len(self._free)} of {self.num_pages} free")
+        for _ in range(need):
+            self._held[request].append(self._free.pop())
+
+    def release(self, request: int) -> None:
+        """Takes all pages of ``request`` back."""
+        self.pages(request)
+        self._free.extend(reversed(self._held.pop(request)))
+
+    def page_table(self, requests: Sequence[int], max_pages: int | None = None) -> torch.Tensor:
+        """int32 ``[len(requests), max_pages]`` on the pools' device (``max_pages``
+        defaults to the longest row's); -1, a page outside the pool, past a row's end."""
+        rows = [self.pages(r) for r in requests]
+        width = max([len(r) for r in rows], default=0) if max_pages is None else max_pages
+        if any(len(r) > width for r in rows):
+            raise ValueError(f"page_table: a request holds more than max_pages = {width} pages")
+        width = max(width, 1)
+        table = torch.tensor([r + [-1] * (width - len(r)) for r in rows], dtype=torch.int32).view(len(rows), width)
+        return table.to(self.keys[0].device)
+
+    def store(self, layer: int, request: int, key: torch.Tensor, value: torch.Tensor) -> None:
+        """Copies rotated keys and values ``[Hkv, S, D]`` (a prompt's, from another
+        cache) to the first S slots of ``request``: a set-up step, in plain copies."""
+        S, held = key.shape[1], self.pages(request)
+        if S > len(held) * self.page_size:
+            raise ValueError(f"store: {S} tokens do not fit the {len(held)} pages of request {request}")
+        for pool, rows in ((self.keys[layer], key), (self.values[layer], value)):
+            if rows.shape != (pool.shape[1], S, pool.shape[3]) or rows.dtype != pool.dtype:
+                raise ValueError(f"store: keys and values must be [{pool.shape[1]}, {S}, {pool.shape[3]}] {pool.dtype}")
+            full, rest = divmod(S, self.page_size)
+            if full:
+                where = torch.tensor(held[:full], device=pool.device)
+                pool[where] = rows[:, :S - rest].reshape(pool.shape[1], full, self.page_size, -1).transpose(0, 1)
+            if rest:
+                pool[held[full], :, :rest] = rows[:, S - rest:]
