@@ -124,6 +124,15 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 // so that the rows of a shared-memory phase differ where the swizzle looks.
 __device__ __forceinline__ int tile_row(int g) { return (g & 1) << 2 | (g & 2) | g >> 2; }
 
+// x' lies as 512 bytes a step of 16 k and block of 8 columns, a lane's 16 bytes
+// after the other.  The lanes that write neighbouring vectors of a row write them
+// to different steps; each step's lanes are turned so that these fall in
+// different banks (without it four met in one).
+template <int W>
+__device__ __forceinline__ constexpr int turn(int step) {
+  return W == 4 ? (step & 3) * 2 : (step & 1) * 4;
+}
+
 // A warp's jobs: those of each round's (tile, job along K) list that fall to it.
 template <int WARPS>
 struct Jobs {
@@ -134,8 +143,9 @@ struct Jobs {
   __device__ __forceinline__ void cut(const Int4Args& a, int tile_end) {
     const int warp = threadIdx.x >> 5;
     const int total = min(a.tiles_round, tile_end - round) * a.kb;
-    const int begin = warp * total / WARPS;
-    left = (warp + 1) * total / WARPS - begin;
+    const int each = total / WARPS, more = total - each * WARPS;  // the first `more` warps take one more
+    const int begin = warp * each + min(warp, more);
+    left = each + (warp < more ? 1 : 0);
     tile = begin / a.kb;
     jk = begin - tile * a.kb;
   }
@@ -189,6 +199,7 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
   constexpr int kWarps = warps_for(NT), kThreads = kWarps * 32;
   constexpr int kSegs = 8 / W;          // groups of a job
   constexpr int kFly = NT <= 2 ? 6 : 12;  // vectors of x a thread holds at once
+  constexpr int kAtOnce = 3;            // and works on side by side
   extern __shared__ __align__(1024) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, i = lane & 3;
   const bool pair = a.mode == AICAS_LINEAR_SWIGLU;
@@ -362,12 +373,12 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
 
   // ---- which warps share a tile of a full round, for the sums at its end
   const auto find_heads = [&](int tiles) {
-    const int total = tiles * a.kb;
-    if (tid < tiles) {
-      // job j is warp ((j + 1) kWarps - 1) / total's
-      const int w0 = ((tid * a.kb + 1) * kWarps - 1) / total, w1 = ((tid + 1) * a.kb * kWarps - 1) / total;
-      s_heads[tid] = w0 | w1 << 16;
-    }
+    const int total = tiles * a.kb, each = total / kWarps, more = total - each * kWarps;
+    const auto warp_of = [&](int j) {
+      const int first = j / (each + 1);
+      return first < more ? first : more + (j - more * (each + 1)) / max(each, 1);
+    };
+    if (tid < tiles) s_heads[tid] = warp_of(tid * a.kb) | warp_of((tid + 1) * a.kb - 1) << 16;
   };
   find_heads(min(a.tiles_round, tile_end - tile0));
 
@@ -391,24 +402,40 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
   };
   for (int block = warp;;) {
 #pragma unroll
-    for (int j = 0; j < kFly; ++j) {
-      if (xr[j] >= a.rows) break;
-      float f[8], top = 0.f, ss = 0.f;
-      Elem<T>::unpack(xq[j], f);
-      if (nw != nullptr) {
-        float w[8];
-        Elem<T>::unpack(wq[j], w);
+    for (int j0 = 0; j0 < kFly; j0 += kAtOnce) {  // reductions side by side hide each other's latency
+      if (xr[j0] >= a.rows) break;
+      float ss[kAtOnce];
+      uint32_t most[kAtOnce];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss), f[e] *= w[e];
+      for (int j = 0; j < kAtOnce; ++j) {
+        float f[8], top = 0.f;
+        Elem<T>::unpack(xq[j0 + j], f);
+        ss[j] = 0.f;
+        if (nw != nullptr) {
+          float w[8];
+          Elem<T>::unpack(wq[j0 + j], w);
 #pragma unroll
-        for (int off = 16; off >= 1; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-        if (lane == 0) s_sums[xr[j] * row_kb + xb[j]] = ss;
+          for (int e = 0; e < 8; ++e) ss[j] = fmaf(f[e], f[e], ss[j]), f[e] *= w[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[e]));
+        most[j] = __float_as_uint(top);  // magnitudes order as their bits
       }
-      const int mine_kb = row_kb0 + xb[j] - kb0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[e]));
-      const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(top));  // magnitudes order as their bits
-      if (lane == 0 && mine_kb >= 0 && mine_kb < a.kb) atomicMax(s_top + xr[j], most);
+      for (int j = 0; j < kAtOnce; ++j) most[j] = __reduce_max_sync(0xffffffffu, most[j]);
+      if (nw != nullptr)
+#pragma unroll
+        for (int off = 16; off >= 1; off >>= 1)
+#pragma unroll
+          for (int j = 0; j < kAtOnce; ++j) ss[j] += __shfl_xor_sync(0xffffffffu, ss[j], off);
+      if (lane == 0)
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+          const int r = xr[j0 + j], mine_kb = row_kb0 + xb[j0 + j] - kb0;
+          if (r >= a.rows) break;
+          if (nw != nullptr) s_sums[r * row_kb + xb[j0 + j]] = ss[j];
+          if (mine_kb >= 0 && mine_kb < a.kb) atomicMax(s_top + r, most[j]);
+        }
     }
     block += kFly * kWarps;
     if (block >= a.rows * row_kb) break;
@@ -428,6 +455,7 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
 
   // ---- x' into shared memory, in the order in which the products take it
   const int my_step = lane / (4 * W) * W + lane % W, my_i = lane % (4 * W) / W;  // of this lane's vector of a block
+  const int my_place = my_i ^ turn<W>(my_step);
   for (int block = warp;;) {
     if (!once) load(block, a.kb, kb0);
 #pragma unroll
@@ -451,7 +479,7 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
         } d;
 #pragma unroll
         for (int e = 0; e < 4; ++e) d.h[e] = __floats2half2_rn(f[e], f[e + 4]);
-        *reinterpret_cast<uint4*>(xs + (((xb[j] * 8 + my_step) * NT + (col >> 3)) * 32 + (col & 7) * 4 + my_i) * 16) = d.u;
+        *reinterpret_cast<uint4*>(xs + (((xb[j] * 8 + my_step) * NT + (col >> 3)) * 32 + ((col & 7) * 4 ^ my_place)) * 16) = d.u;
       };
       if (split) {
         put(2 * xr[j]);
@@ -473,7 +501,7 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
     for (int w = 0; w < W; ++w)
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const uint4 b = *reinterpret_cast<const uint4*>(xs + (((grp * W + w) * NT + n) * 32 + lane) * 16);
+        const uint4 b = *reinterpret_cast<const uint4*>(xs + (((grp * W + w) * NT + n) * 32 + (lane ^ turn<W>(grp * W + w))) * 16);
         mma_f16(acc[n], 0x00010001u, 0u, 0x00100010u, 0u, b.x, b.y);
         mma_f16(acc[n], 0x00010001u, 0u, 0x00100010u, 0u, b.z, b.w);
       }
@@ -507,7 +535,7 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
       if (!bad) {
         fetch();
         const uint32_t wrow = ring + stage * kJobBytes + my_row * 128;
-        const uint8_t* xf = xs + (size_t)(job.jk * 8 * NT * 32 + lane) * 16;
+        const uint8_t* xf = xs + job.jk * 8 * NT * 512;
         const float* gs = xsum + job.jk * kSegs * NT * 8 + 2 * i;
 #pragma unroll
         for (int seg = 0; seg < kSegs; ++seg) {
@@ -533,7 +561,7 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
             for (int r = 0; r < 4; ++r) h[r] = w[r][j] >> 8;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              const uint4 b = *reinterpret_cast<const uint4*>(xf + ((seg * W + j) * NT + n) * 512);
+              const uint4 b = *reinterpret_cast<const uint4*>(xf + ((seg * W + j) * NT + n) * 512 + (lane ^ turn<W>(seg * W + j)) * 16);
 #pragma unroll
               for (int m = 0; m < 2; ++m) {
                 const uint32_t p = w[2 * m][j], q = w[2 * m + 1][j];
@@ -588,7 +616,6 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
 
     if (a.s > 1 && job.round == tile0) cluster_wait();
     // ---- the round's outputs: the warps' partial tiles, then the CTAs', added in their order
-    const int total = min(a.tiles_round, tile_end - job.round) * a.kb;
     const int n0 = job.round * tile_n, width = min(min(a.tiles_round, tile_end - job.round) * tile_n, a.n - n0);
     // four neighbouring outputs a thread
     const int quads = (width + 3) / 4, count = quads * a.rows, share = (count + a.s - 1) / a.s;
@@ -625,15 +652,17 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
       const int tile = c / tile_n, place = (split ? 2 * r : r) * kPitch + c - tile * tile_n;
       const int heads = s_heads[tile], w0 = heads & 0xffff, w1 = heads >> 16;
       float4 y = make_float4(0.f, 0.f, 0.f, 0.f), u = y;
-      for (int w = w0; w <= w1; ++w) {
-        if (w * total / kWarps == (w + 1) * total / kWarps) continue;  // a warp without jobs
-        const float* p = part + (w == w0 ? tile : a.tiles_round + w) * tile_floats + place;
+      const float* p = part + tile * tile_floats + place;
+      const float* const heads_at = part + (a.tiles_round + w0) * tile_floats + place;
+#pragma unroll 4
+      for (int w = 0; w <= w1 - w0; ++w) {
         add4(y, p);
         if (split) add4(y, p + kPitch);
         if (pair) {
           add4(u, p + 16);
           if (split) add4(u, p + kPitch + 16);
         }
+        p = heads_at + (w + 1) * tile_floats;
       }
       const float inv = s_inv[r];
       y.x *= inv, y.y *= inv, y.z *= inv, y.w *= inv;
