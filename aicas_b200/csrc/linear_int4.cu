@@ -319,8 +319,8 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
     if (s_new) {
       const int t = sj.round + sj.tile, n = t * tile_n + n_off;
       s_at = (int64_t)n * a.groups + grp0;
-      s_row = n < a.n;
-      if (t + a.tiles_round < tile_end && n + a.tiles_round * tile_n < a.n) {  // the next round's, a line of each kind
+      s_row = n < a.n && grp0 < a.groups;  // K may end before the last CTA's share of it does
+      if (t + a.tiles_round < tile_end && n + a.tiles_round * tile_n < a.n && grp0 < a.groups) {  // the next round's, a line of each kind
         const int64_t next = s_at + (int64_t)a.tiles_round * tile_n * a.groups;
         asm volatile("prefetch.global.L2 [%0];" ::"l"(my_scales + next));
         if (my_zeros != nullptr) asm volatile("prefetch.global.L2 [%0];" ::"l"(my_zeros + next));
@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
     }
 #pragma unroll
     for (int j = 0; j < (kSegs + 3) / 4; ++j) next_z[j] = 0x08080808u;
-    if (s_row && a.whole) {
+    if (s_row && a.whole && grp0 < a.groups) {
       // K is whole jobs: a row's groups of a job are one aligned vector
       if constexpr (kSegs == 2) {
         next_s[0] = *reinterpret_cast<const uint32_t*>(my_scales + s_at);

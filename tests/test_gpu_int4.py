@@ -238,3 +238,22 @@ def test_refusals(cuda_device):
     ]:
         with pytest.raises(ValueError, match=text):
             call()
+
+
+@pytest.mark.parametrize("rows,k,dtype", [(32, 2304, "bf16"), (32, 2816, "bf16"), (20, 1280, "fp16"), (32, 6400, "fp16")])
+def test_scales_past_the_end_of_k_are_not_read(cuda_device, rows, k, dtype):
+    """K in an odd number of 256s, many rows: the last CTA of a cluster has less of
+    K than the others.  What follows the scales and zero points counts for nothing."""
+    n, group = 96, 128
+    g = torch.Generator().manual_seed(k)
+    w = _weight(g, n, k, group, dtype, True, cuda_device)
+    count = n * (k // group)
+    scales = torch.full((count + 64,), float("nan"), dtype=DT[dtype], device=cuda_device)
+    zeros = torch.full((count + 64,), 255, dtype=torch.uint8, device=cuda_device)
+    scales[:count], zeros[:count] = w.scales.flatten(), w.zeros.flatten()
+    inside = ab.Int4Weight(w.qweight, scales[:count].view(n, -1), zeros[:count].view(n, -1))
+    x = torch.randn(rows, k, generator=g).to(DT[dtype]).to(cuda_device)
+    nw = torch.ones(k, dtype=DT[dtype], device=cuda_device)
+    for norm in (None, nw):
+        y = ab.decode_linear_int4(x, inside, norm_weight=norm)
+        assert torch.equal(y, ab.decode_linear_int4(x, w, norm_weight=norm)) and bool(y.isfinite().all())
