@@ -297,6 +297,9 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
     ld.step(a);
     return 1;
   };
+  // a first round with fewer jobs than stages: the next rounds' jobs fill the rest, so that
+  // from here on the stage just read is the only free one, or nothing is left to copy
+  while (flying < a.stages && issue(flying) != 0) ++flying;
 
   // ---- scales and zero points of a job: lane i of a lane group holds those of row my_row + 8 i;
   // fetched a job ahead, from L2 where the round before asked for them

@@ -257,3 +257,11 @@ def test_scales_past_the_end_of_k_are_not_read(cuda_device, rows, k, dtype):
     for norm in (None, nw):
         y = ab.decode_linear_int4(x, inside, norm_weight=norm)
         assert torch.equal(y, ab.decode_linear_int4(x, w, norm_weight=norm)) and bool(y.isfinite().all())
+
+
+@pytest.mark.parametrize("rows,k,n,group,swiglu", [(32, 256, 60000, 128, False), (16, 512, 120000, 128, False),
+                                                   (1, 256, 100000, 32, True), (25, 128, 50001, 64, False),
+                                                   (32, 256, 30001, 64, True)])
+def test_rounds_with_fewer_jobs_than_the_ring_has_stages(cuda_device, rows, k, n, group, swiglu):
+    """Short K, many output features: a warp has one or two jobs in each of several rounds."""
+    _case(cuda_device, rows, k, n, group, zeros=True, swiglu=swiglu, seed=rows)
