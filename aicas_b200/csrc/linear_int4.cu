@@ -55,6 +55,9 @@ constexpr int kVarBytes = 64 + 3 * 32 * 4 + kMaxRound * 4;
 // memory for the columns of many rows.
 constexpr int warps_for(int nt) { return nt <= 2 ? 12 : 8; }
 
+// 16-byte vectors of x that a thread holds at once while x' is laid out.
+constexpr int fly_for(int nt) { return nt <= 2 ? 6 : 12; }
+
 struct Int4Args {
   CUtensorMap tm_w[2];
   const void* x;
@@ -198,7 +201,7 @@ template <typename T, int NT, int W>
 __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(const __grid_constant__ Int4Args a) {
   constexpr int kWarps = warps_for(NT), kThreads = kWarps * 32;
   constexpr int kSegs = 8 / W;          // groups of a job
-  constexpr int kFly = NT <= 2 ? 6 : 12;  // vectors of x a thread holds at once
+  constexpr int kFly = fly_for(NT);     // vectors of x a thread holds at once
   constexpr int kAtOnce = 3;            // and works on side by side
   extern __shared__ __align__(1024) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, i = lane & 3;
@@ -805,16 +808,21 @@ int plan_int4(Int4Args* a, int nt, int s, int rows, int cols, int deep, int sms)
   const int jobs = (a->k + kJobK - 1) / kJobK;
   a->s = s;
   a->kb = (jobs + s - 1) / s;
-  // a round holds a cluster's tiles, if shared memory does
+  const int warps = warps_for(nt), ring = warps * kJobBytes;
+  const int place = cols * kPitch * 4, recv_tile = s > 1 ? kTileRows * rows * 4 : 0;  // a tile's partial sums, received ones
+  const int xs = a->kb * nt * 4096, sums = a->kb * (kJobK / (a->k / a->groups)) * nt * 32;
+  const int tail = warps * 8 * 8 + kVarBytes + 16;
+  // a round holds a cluster's tiles, if shared memory does beside rings of `deep` jobs; two jobs a warp at least
   const int most = cols <= 8 ? kMaxRound : kMaxRound * 8 / cols, want = (int)((int64_t)a->tiles * s * 4 / (3 * sms)) + 1;
+  const int fixed = warps * place + (s > 1 ? 32 * s + 16 : 0) + xs + sums + tail, room = kMaxSmem - deep * ring - fixed;
+  const int hold = room < 0 ? 0 : room / (place + recv_tile), least = (2 * warps + a->kb - 1) / a->kb;
   a->tiles_round = want < most ? want : most;
-  const int warps = warps_for(nt);
-  const int part = (a->tiles_round + warps) * cols * kPitch * 4, xs = a->kb * nt * 4096;
-  const int recv = s > 1 ? a->tiles_round * (a->mode == AICAS_LINEAR_SWIGLU ? 2 * 16 : 32) * rows * 4 + 32 * s : 0;
-  const int sums = a->kb * (kJobK / (a->k / a->groups)) * nt * 32;
-  const int tail = warps * 8 * 8 + kVarBytes + 16, rest = part + recv + xs + sums + tail, ring = warps * kJobBytes;
-  a->stages = (kMaxSmem - rest) / ring;
-  if (a->stages < deep) return 0;
+  if (a->tiles_round > hold) {
+    if (hold < least || hold < 1) return 0;
+    a->tiles_round = hold;
+  }
+  const int part = (a->tiles_round + warps) * place, recv = s > 1 ? a->tiles_round * recv_tile + 32 * s : 0;
+  a->stages = (kMaxSmem - fixed - a->tiles_round * (place + recv_tile)) / ring;
   if (a->stages > 8) a->stages = 8;
   a->off_part = a->stages * ring;
   a->off_recv = a->off_part + part;
@@ -854,8 +862,16 @@ int run_linear_int4(const aicas_linear_int4_params* p, int sms, cudaStream_t str
   for (;; batch = (batch + 1) / 2) {
     const int blocks = (batch * columns + 7) / 8;
     nt = blocks <= 1 ? 1 : blocks <= 2 ? 2 : blocks <= 4 ? 4 : 8;
-    for (int deep = 3; deep >= 2 && smem == 0; --deep)  // rings of three jobs a warp, if some split leaves room for them
-      for (int s = 1; s <= 8 && smem == 0; s *= 2) smem = plan_int4(&a, nt, s, batch, batch * columns, deep, sms);
+    // Rings of three jobs a warp, if some split leaves room for them; before that, without a norm, a split that
+    // lets x stay in registers between its statistics and its place in shared memory (with a norm each CTA's
+    // statistics take all of K whatever the split).  8 rows of 6144 -> 2048: 8.2 us over 4 CTAs, 10.3 over the
+    // 2 that would hold x'; 32 rows of 2048 -> 2048: 10.1 over 4, 13.9 over 2; 32 of 6144 -> 20000: 87 and 100.
+    for (int lean = p->norm_weight == nullptr; lean >= 0 && smem == 0; --lean)
+      for (int deep = 3; deep >= 2 && smem == 0; --deep)
+        for (int s = 1; s <= 8 && smem == 0; s *= 2) {
+          smem = plan_int4(&a, nt, s, batch, batch * columns, deep, sms);
+          if (lean && batch * a.kb > fly_for(nt) * warps_for(nt)) smem = 0;
+        }
     if (smem != 0) break;
     if (batch == 1) {
       snprintf(err, errlen, "int4 linear: in_features %d is more than shared memory holds", p->in_features);
