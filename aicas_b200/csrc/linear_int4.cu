@@ -49,7 +49,7 @@ constexpr int kPitch = 36;              // floats a column of a partial tile (32
 constexpr int kMaxSmem = 232448;
 
 constexpr int kMaxRound = 40;           // tiles of a round
-constexpr int kVarBytes = 64 + 3 * 32 * 4 + kMaxRound * 4;
+constexpr int kVarBytes = 64 + 3 * 32 * 4 + kMaxRound * 4 + 8 * 32 * 4;
 
 // Warps of a CTA: more of them hide the products' latency, fewer leave shared
 // memory for the columns of many rows.
@@ -109,6 +109,11 @@ __device__ __forceinline__ void st_cluster(float* p, uint32_t rank, const float4
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
   asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
                : "memory");
+}
+__device__ __forceinline__ void st_cluster(float* p, uint32_t rank, float v) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
 }
 // In two halves: every CTA of the cluster has started once the wait returns.
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
@@ -218,7 +223,8 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
   uint32_t* s_top = reinterpret_cast<uint32_t*>(s_abort + 16);   // [32] a row's largest magnitude
   float* s_scale = reinterpret_cast<float*>(s_top + 32);      // [32]
   float* s_inv = s_scale + 32;                                // [32]
-  int* s_heads = reinterpret_cast<int*>(s_inv + 32);          // [tile of the round] the warps after the tile's first
+  float* s_ss = s_inv + 32;                                   // [8][32] cluster: [from rank] a row's sum of squares over its K
+  int* s_heads = reinterpret_cast<int*>(s_ss + 8 * 32);       // [tile of the round] the warps after the tile's first
   const int rank = a.s > 1 ? (int)cluster_rank() : 0;
   const int cluster = (int)blockIdx.x / a.s;
   const int kb0 = rank * a.kb;  // this CTA's first job along K
@@ -254,27 +260,26 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
 
   // ---- x, ahead of the weights: blocks of 256 k of a row, a 16-byte vector a lane, kFly blocks a warp at once
   const T* x = static_cast<const T*>(a.x);
-  const int all_vecs = a.k / 8, all_kb = (a.k + kJobK - 1) / kJobK;
-  const int row_kb = nw != nullptr ? all_kb : a.kb, row_kb0 = nw != nullptr ? 0 : kb0;  // blocks of a row for its statistics
-  const bool once = a.rows * a.kb <= kFly * kWarps && row_kb == a.kb;  // the vectors stay in registers in between
+  const int all_vecs = a.k / 8;
+  const bool once = a.rows * a.kb <= kFly * kWarps;  // the vectors stay in registers between statistics and staging
   uint4 xq[kFly], wq[kFly];
   int xr[kFly], xb[kFly];
-  const auto load = [&](int block, int per, int first) {  // blocks block, block + kWarps, .. of rows of `per` blocks
-    int r = block / per, at = block - r * per;
+  const auto load = [&](int block) {  // blocks block, block + kWarps, .. of rows of kb
+    int r = block / a.kb, at = block - r * a.kb;
 #pragma unroll
     for (int j = 0; j < kFly; ++j) {
       xr[j] = r, xb[j] = at;
-      const int v = (first + at) * 32 + lane;
+      const int v = (kb0 + at) * 32 + lane;
       xq[j] = wq[j] = make_uint4(0, 0, 0, 0);
       if (r < a.rows && v < all_vecs) {
         xq[j] = reinterpret_cast<const uint4*>(x + r * a.x_stride)[v];
         if (nw != nullptr) wq[j] = reinterpret_cast<const uint4*>(nw)[v];
       }
       at += kWarps;
-      while (at >= per) at -= per, ++r;
+      while (at >= a.kb) at -= a.kb, ++r;
     }
   };
-  load(warp, row_kb, row_kb0);
+  load(warp);
 
   const uint64_t policy = l2_policy_evict_first();
   if (fill) {
@@ -437,24 +442,39 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
       if (lane == 0)
 #pragma unroll
         for (int j = 0; j < kAtOnce; ++j) {
-          const int r = xr[j0 + j], mine_kb = row_kb0 + xb[j0 + j] - kb0;
+          const int r = xr[j0 + j];
           if (r >= a.rows) break;
-          if (nw != nullptr) s_sums[r * row_kb + xb[j0 + j]] = ss[j];
-          if (mine_kb >= 0 && mine_kb < a.kb) atomicMax(s_top + r, most[j]);
+          if (nw != nullptr) s_sums[r * a.kb + xb[j0 + j]] = ss[j];
+          atomicMax(s_top + r, most[j]);
         }
     }
     block += kFly * kWarps;
-    if (block >= a.rows * row_kb) break;
-    load(block, row_kb, row_kb0);
+    if (block >= a.rows * a.kb) break;
+    load(block);
   }
   __syncthreads();
+  const auto row_sum = [&](int r) {
+    float ss = 0.f;
+    for (int e = lane; e < a.kb; e += 32) ss += s_sums[r * a.kb + e];
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+    return ss;
+  };
+  const bool shared_rows = nw != nullptr && a.s > 1;  // the other CTAs have the rest of a row's squares
+  if (shared_rows) {
+    cluster_wait();
+    for (int r = warp; r < a.rows; r += kWarps) {
+      const float ss = row_sum(r);
+      if (lane < a.s) st_cluster(s_ss + rank * 32 + r, lane, ss);
+    }
+    cluster_sync_all();
+  }
   for (int r = warp; r < a.rows; r += kWarps) {
     float ss = 0.f;
-    if (nw != nullptr) {
-      for (int e = lane; e < row_kb; e += 32) ss += s_sums[r * row_kb + e];
-#pragma unroll
-      for (int off = 16; off >= 1; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-    }
+    if (shared_rows)
+      for (int q = 0; q < a.s; ++q) ss += s_ss[q * 32 + r];
+    else if (nw != nullptr)
+      ss = row_sum(r);
     row_scale(r, __uint_as_float(s_top[r]), ss);
   }
   __syncthreads();
@@ -463,7 +483,7 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
   const int my_step = lane / (4 * W) * W + lane % W, my_i = lane % (4 * W) / W;  // of this lane's vector of a block
   const int my_place = my_i ^ turn<W>(my_step);
   for (int block = warp;;) {
-    if (!once) load(block, a.kb, kb0);
+    if (!once) load(block);
 #pragma unroll
     for (int j = 0; j < kFly; ++j) {
       if (xr[j] >= a.rows) break;
@@ -620,7 +640,7 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
     }
     __syncthreads();
 
-    if (a.s > 1 && job.round == tile0) cluster_wait();
+    if (a.s > 1 && !shared_rows && job.round == tile0) cluster_wait();
     // ---- the round's outputs: the warps' partial tiles, then the CTAs', added in their order
     const int n0 = job.round * tile_n, width = min(min(a.tiles_round, tile_end - job.round) * tile_n, a.n - n0);
     // four neighbouring outputs a thread
@@ -803,8 +823,9 @@ cudaError_t dispatch_int4(int nt, int group, const Int4Args& a, int smem, int sm
   return cudaErrorInvalidValue;
 }
 
-// Shared memory of a launch of nt column blocks with K split s ways and rings of at least `deep` jobs; 0: does not fit.
-int plan_int4(Int4Args* a, int nt, int s, int rows, int cols, int deep, int sms) {
+// Shared memory of a launch of nt column blocks with K split s ways and rings of at least `deep` jobs; 0: does
+// not fit.  lean: x has to stay in registers and one round to do.
+int plan_int4(Int4Args* a, int nt, int s, int rows, int cols, int deep, bool lean, int sms) {
   const int jobs = (a->k + kJobK - 1) / kJobK;
   a->s = s;
   a->kb = (jobs + s - 1) / s;
@@ -816,6 +837,7 @@ int plan_int4(Int4Args* a, int nt, int s, int rows, int cols, int deep, int sms)
   const int most = cols <= 8 ? kMaxRound : kMaxRound * 8 / cols, want = (int)((int64_t)a->tiles * s * 4 / (3 * sms)) + 1;
   const int fixed = warps * place + (s > 1 ? 32 * s + 16 : 0) + xs + sums + tail, room = kMaxSmem - deep * ring - fixed;
   const int hold = room < 0 ? 0 : room / (place + recv_tile), least = (2 * warps + a->kb - 1) / a->kb;
+  if (lean && (rows * a->kb > fly_for(nt) * warps || want > most || want > hold)) return 0;
   a->tiles_round = want < most ? want : most;
   if (a->tiles_round > hold) {
     if (hold < least || hold < 1) return 0;
@@ -862,16 +884,14 @@ int run_linear_int4(const aicas_linear_int4_params* p, int sms, cudaStream_t str
   for (;; batch = (batch + 1) / 2) {
     const int blocks = (batch * columns + 7) / 8;
     nt = blocks <= 1 ? 1 : blocks <= 2 ? 2 : blocks <= 4 ? 4 : 8;
-    // Rings of three jobs a warp, if some split leaves room for them; before that, without a norm, a split that
-    // lets x stay in registers between its statistics and its place in shared memory (with a norm each CTA's
-    // statistics take all of K whatever the split).  8 rows of 6144 -> 2048: 8.2 us over 4 CTAs, 10.3 over the
-    // 2 that would hold x'; 32 rows of 2048 -> 2048: 10.1 over 4, 13.9 over 2; 32 of 6144 -> 20000: 87 and 100.
-    for (int lean = p->norm_weight == nullptr; lean >= 0 && smem == 0; --lean)
+    // Rings of three jobs a warp, if some split leaves room for them.  Before that a split that lets x stay in
+    // registers between its statistics and its place in shared memory, if the work is one round (else each round
+    // pays for the split).  8 rows of 6144 -> 2048: 8.1 us over 4 CTAs, 10.3 over the 2 that would hold x'; 32 of
+    // 2048 -> 2048: 10.1 over 4, 14.1 over 2; 32 of 4096 -> 4096 with the norm 19.5 over 8, 21.8 over 4; but 32 of
+    // 2048 -> 40000 with the norm, several rounds: 57 over 4, 49 over 2.
+    for (int lean = 1; lean >= 0 && smem == 0; --lean)
       for (int deep = 3; deep >= 2 && smem == 0; --deep)
-        for (int s = 1; s <= 8 && smem == 0; s *= 2) {
-          smem = plan_int4(&a, nt, s, batch, batch * columns, deep, sms);
-          if (lean && batch * a.kb > fly_for(nt) * warps_for(nt)) smem = 0;
-        }
+        for (int s = 1; s <= 8 && smem == 0; s *= 2) smem = plan_int4(&a, nt, s, batch, batch * columns, deep, lean, sms);
     if (smem != 0) break;
     if (batch == 1) {
       snprintf(err, errlen, "int4 linear: in_features %d is more than shared memory holds", p->in_features);
