@@ -200,9 +200,11 @@ __device__ __noinline__ float2 row_stats(const T* row, const T* w, int first, in
   return make_float2(top, ss);
 }
 
+// CLUSTER: K is split over a cluster (a kernel of its own, so that calls of one row, bound by the way to their
+// first instruction and back, do not carry the exchange).
 // W: 32-bit words of weights that a lane takes side by side (4 W lanes' words
 // = 32 W of k share a group of g = 32 W).  NT: blocks of 8 columns.
-template <typename T, int NT, int W>
+template <typename T, int NT, int W, bool CLUSTER>
 __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(const __grid_constant__ Int4Args a) {
   constexpr int kWarps = warps_for(NT), kThreads = kWarps * 32;
   constexpr int kSegs = 8 / W;          // groups of a job
@@ -225,8 +227,8 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
   float* s_inv = s_scale + 32;                                // [32]
   float* s_ss = s_inv + 32;                                   // [8][32] cluster: [from rank] a row's sum of squares over its K
   int* s_heads = reinterpret_cast<int*>(s_ss + 8 * 32);       // [tile of the round] the warps after the tile's first
-  const int rank = a.s > 1 ? (int)cluster_rank() : 0;
-  const int cluster = (int)blockIdx.x / a.s;
+  const int rank = CLUSTER ? (int)cluster_rank() : 0;
+  const int cluster = CLUSTER ? (int)blockIdx.x / a.s : (int)blockIdx.x;
   const int kb0 = rank * a.kb;  // this CTA's first job along K
   const T* nw = static_cast<const T*>(a.norm_weight);
   const bool split = nw != nullptr && std::is_same<T, __half>::value;  // two parts a row
@@ -234,7 +236,7 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
 
   if (tid == 0) *s_abort = 0;
   if (tid < 32) s_top[tid] = 0u;
-  if (a.s > 1) cluster_arrive();  // waited for before the first store to another CTA
+  if (CLUSTER) cluster_arrive();  // waited for before the first store to another CTA
   if (lane < a.stages) mbar_init(bars + 8 * lane, 1);
   grid_launch_dependents();
 
@@ -460,7 +462,7 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
     for (int off = 16; off >= 1; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
     return ss;
   };
-  const bool shared_rows = nw != nullptr && a.s > 1;  // the other CTAs have the rest of a row's squares
+  const bool shared_rows = CLUSTER && nw != nullptr;  // the other CTAs have the rest of a row's squares
   if (shared_rows) {
     cluster_wait();
     for (int r = warp; r < a.rows; r += kWarps) {
@@ -640,11 +642,11 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
     }
     __syncthreads();
 
-    if (a.s > 1 && !shared_rows && job.round == tile0) cluster_wait();
+    if (CLUSTER && !shared_rows && job.round == tile0) cluster_wait();
     // ---- the round's outputs: the warps' partial tiles, then the CTAs', added in their order
     const int n0 = job.round * tile_n, width = min(min(a.tiles_round, tile_end - job.round) * tile_n, a.n - n0);
     // four neighbouring outputs a thread
-    const int quads = (width + 3) / 4, count = quads * a.rows, share = (count + a.s - 1) / a.s;
+    const int quads = (width + 3) / 4, count = quads * a.rows, share = CLUSTER ? (count + a.s - 1) / a.s : count;
     const float per_row = 1.f / (float)quads;
     const auto add4 = [](float4& y, const float* p) {
       const float4 v = *reinterpret_cast<const float4*>(p);
@@ -678,22 +680,30 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
       const int tile = c / tile_n, place = (split ? 2 * r : r) * kPitch + c - tile * tile_n;
       const int heads = s_heads[tile], w0 = heads & 0xffff, w1 = heads >> 16;
       float4 y = make_float4(0.f, 0.f, 0.f, 0.f), u = y;
-      const float* p = part + tile * tile_floats + place;
+      const float* const first = part + tile * tile_floats + place;
       const float* const heads_at = part + (a.tiles_round + w0) * tile_floats + place;
-#pragma unroll 4
-      for (int w = 0; w <= w1 - w0; ++w) {
-        add4(y, p);
-        if (split) add4(y, p + kPitch);
-        if (pair) {
-          add4(u, p + 16);
-          if (split) add4(u, p + kPitch + 16);
+      const auto add_all = [&](float4& sum, int off) {  // up to four loads at once; few tiles have more
+        float4 v[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          v[w] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (w <= w1 - w0) v[w] = *reinterpret_cast<const float4*>((w == 0 ? first : heads_at + w * tile_floats) + off);
         }
-        p = heads_at + (w + 1) * tile_floats;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) sum.x += v[w].x, sum.y += v[w].y, sum.z += v[w].z, sum.w += v[w].w;
+#pragma unroll 1
+        for (int w = 4; w <= w1 - w0; ++w) add4(sum, heads_at + w * tile_floats + off);
+      };
+      add_all(y, 0);
+      if (split) add_all(y, kPitch);
+      if (pair) {
+        add_all(u, 16);
+        if (split) add_all(u, kPitch + 16);
       }
       const float inv = s_inv[r];
       y.x *= inv, y.y *= inv, y.z *= inv, y.w *= inv;
       u.x *= inv, u.y *= inv, u.z *= inv, u.w *= inv;
-      if (a.s == 1) {
+      if (!CLUSTER) {
         finish(r, c, y, u);
       } else {  // to the CTA that finishes these outputs
         const int owner = at / share, slot = rank * share + at - owner * share;
@@ -701,7 +711,7 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
         if (pair) st_cluster(recv + 4 * (a.s * share + slot), owner, u);
       }
     }
-    if (a.s > 1) {
+    if (CLUSTER) {
       cluster_sync_all();
       for (int at = rank * share + tid; at < min(count, (rank + 1) * share); at += kThreads) {
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f), u = y;
@@ -717,7 +727,7 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
     if (job.round >= tile_end) break;
     job.cut(a, tile_end);
     // the partial tiles have been read, the received ones in every CTA
-    if (a.s > 1) cluster_sync_all(); else __syncthreads();
+    if (CLUSTER) cluster_sync_all(); else __syncthreads();
     if (tile_end - job.round < a.tiles_round) find_heads(tile_end - job.round);  // read after the next barrier
   }
   if (bad)
@@ -750,7 +760,7 @@ bool weight_map(CUtensorMap* m, const aicas_int4_weight& w, int n, int k, int bo
 
 int log2_of(int v) { return v <= 1 ? 0 : 1 + log2_of(v / 2); }
 
-template <typename T, int NT, int W>
+template <typename T, int NT, int W, bool CLUSTER>
 cudaError_t launch_int4(Int4Args a, int smem, int sms, cudaStream_t st) {
   static bool attr_set[64] = {false};
   static int max_clusters[64][4] = {};  // by device and cluster size
@@ -759,7 +769,7 @@ cudaError_t launch_int4(Int4Args a, int smem, int sms, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   const bool known = dev >= 0 && dev < 64;
   if (!known || !attr_set[dev]) {
-    e = cudaFuncSetAttribute(linear_int4_kernel<T, NT, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+    e = cudaFuncSetAttribute(linear_int4_kernel<T, NT, W, CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
     if (e != cudaSuccess) return e;
     if (known) attr_set[dev] = true;
   }
@@ -776,8 +786,8 @@ cudaError_t launch_int4(Int4Args a, int smem, int sms, cudaStream_t st) {
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = a.s > 1 ? 2 : 1;
-  if (a.s > 1) {
+  cfg.numAttrs = CLUSTER ? 2 : 1;
+  if (CLUSTER) {
     int* cached = known ? &max_clusters[dev][log2_of(a.s)] : nullptr;
     if (cached != nullptr && *cached > 0) {
       clusters = *cached;
@@ -786,7 +796,7 @@ cudaError_t launch_int4(Int4Args a, int smem, int sms, cudaStream_t st) {
       cudaLaunchAttribute only = attr[1];
       cfg.attrs = &only;
       cfg.numAttrs = 1;
-      e = cudaOccupancyMaxActiveClusters(&clusters, linear_int4_kernel<T, NT, W>, &cfg);
+      e = cudaOccupancyMaxActiveClusters(&clusters, linear_int4_kernel<T, NT, W, CLUSTER>, &cfg);
       if (e != cudaSuccess) return e;
       if (clusters < 1) return cudaErrorInvalidConfiguration;
       if (cached != nullptr) *cached = clusters;
@@ -798,15 +808,15 @@ cudaError_t launch_int4(Int4Args a, int smem, int sms, cudaStream_t st) {
   a.tiles_each = a.tiles / clusters;
   a.tiles_more = a.tiles % clusters;
   cfg.gridDim = dim3((unsigned)(clusters * a.s));
-  return cudaLaunchKernelEx(&cfg, linear_int4_kernel<T, NT, W>, a);
+  return cudaLaunchKernelEx(&cfg, linear_int4_kernel<T, NT, W, CLUSTER>, a);
 }
 
 template <typename T, int NT>
 cudaError_t dispatch_group(int group, const Int4Args& a, int smem, int sms, cudaStream_t st) {
   switch (group) {
-    case 32: return launch_int4<T, NT, 1>(a, smem, sms, st);
-    case 64: return launch_int4<T, NT, 2>(a, smem, sms, st);
-    case 128: return launch_int4<T, NT, 4>(a, smem, sms, st);
+    case 32: return a.s > 1 ? launch_int4<T, NT, 1, true>(a, smem, sms, st) : launch_int4<T, NT, 1, false>(a, smem, sms, st);
+    case 64: return a.s > 1 ? launch_int4<T, NT, 2, true>(a, smem, sms, st) : launch_int4<T, NT, 2, false>(a, smem, sms, st);
+    case 128: return a.s > 1 ? launch_int4<T, NT, 4, true>(a, smem, sms, st) : launch_int4<T, NT, 4, false>(a, smem, sms, st);
   }
   return cudaErrorInvalidValue;
 }
