@@ -11,11 +11,11 @@
 //     pair, are cut into equal ranges, one per CTA (one CTA an SM).  The cut is
 //     made on the device from the lengths, so the host neither knows nor bounds
 //     them and ragged batches balance to a tile; a pair counts kPairCost tiles more
-//     for its beginning and end (64 ragged caches of up to 4096 slots, while the warps
-//     still copied for themselves: 96 us against 101 without it).  A pair inside one range is finished there; a pair that crosses ranges
-//     leaves one fp32 partial a CTA (a CTA has at most two: its first and its last
-//     pair), and the last CTA to arrive adds them in CTA order, so results repeat to
-//     the bit.  A small launch of few pairs gives each pair CTAs of its own.
+//     for its beginning and end.  A pair inside one range is finished there; a pair
+//     that crosses ranges leaves one fp32 partial a CTA (a CTA has at most two: its
+//     first and its last pair), and the last CTA to arrive adds them in CTA order, so
+//     results repeat to the bit.  A small launch of few pairs gives each pair CTAs of
+//     its own.
 //   * Copies: two warps stream the range's K and V tiles as TMA boxes, swizzled so
 //     that ldmatrix reads them without bank conflicts, into a ring of its own for
 //     each of the other warps, which take the tiles in turn; no warp waits for
@@ -31,6 +31,11 @@
 //     heads the lo parts ride in the 8 unused rows of the same products.
 //   * Slots out of range: scores replaced by -inf and V's elements by 0 before
 //     the products (0 * NaN), in the tiles at the range's ends only.
+//
+// Measured (16 query over 8 KV heads of 128, bf16): 4 caches of 131072 slots 320 us,
+// 6700 GB/s; 64 ragged ones of up to 4096 slots 94.5 us, 6090 GB/s (the measured copy
+// rate is 6450 GB/s); one cache of 1024 slots 7.9 us, which is a chain of latencies:
+// lengths, page numbers, first tiles, a join over CTAs.
 #include <cstdio>
 #include <cstring>
 

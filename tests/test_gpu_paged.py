@@ -279,8 +279,8 @@ def test_decode_many_short_requests(cuda_device):
     [16] * 40 + [30000] + [16] * 40 + [1] * 2000 + [15000],
 ])
 @pytest.mark.parametrize("dim,dtype", [(16, "fp16"), (64, "bf16"), (32, "fp32")])
-def test_decode_claimed_ranges(cuda_device, lens, dim, dtype):
-    """Launches large enough for ranges that the CTAs claim, of short and long requests mixed."""
+def test_decode_ranges_over_mixed_requests(cuda_device, lens, dim, dtype):
+    """More requests than CTAs, short and long ones mixed: ranges that hold many, or a part of one."""
     g = torch.Generator().manual_seed(len(lens))
     B, hkv, size = len(lens), 8, 16
     pages = 400
@@ -299,7 +299,7 @@ def test_decode_claimed_ranges(cuda_device, lens, dim, dtype):
                              [0] * len(pick), dim ** -0.5, 2)
     _near(out[pick], ref, dtype, 2e-5 if dtype == "fp32" else 1e-3)
     _near(lse[pick], ref_lse, "fp32", 1e-4)
-    # every request: a batch of few requests takes equal ranges without claims
+    # every request, cut differently: in batches of 250
     for b0 in range(0, B, 250):
         part = ab.paged_gqa_decode_attention(q[b0:b0 + 250], kp, vp, table[b0:b0 + 250],
                                              **(kw | {"kv_lens": torch.tensor(lens[b0:b0 + 250], dtype=torch.int32)}))
