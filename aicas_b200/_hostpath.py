@@ -1,8 +1,11 @@
 """The host side of a launch for operators that run a few microseconds: what they
 check and look up on every call, at the least cost torch allows.  A tensor
 attribute is 40-100 ns, ``torch.cuda.current_stream`` 1.2 us and a strided view
-1 us, against kernels of 3-5 us."""
+1 us, against kernels of 2-10 us.  Calls whose arguments need nothing done to
+them take the compiled ``fast_*`` way; the others the Python operators' own."""
 from __future__ import annotations
+
+import ctypes
 
 import torch
 
@@ -15,6 +18,29 @@ except ImportError:  # pragma: no cover - torch without the binding
 
     def raw_stream(index: int) -> int:
         return torch.cuda.current_stream(index).cuda_stream
+
+
+try:  # the common calls' checks and packing, compiled; each function returns None where it leaves a call to Python
+    from . import _hostcalls
+    fast_append, fast_decode, fast_int4 = _hostcalls.append, _hostcalls.decode, _hostcalls.int4
+except ImportError:  # not built, or for another torch: the Python operators do it all
+    _hostcalls = None
+
+    def fast_append(*args):
+        return None
+
+    fast_decode = fast_int4 = fast_append
+
+
+def library():
+    """The native library, its entry points known to the compiled calls too."""
+    global _hostcalls
+    lib = nat.lib()
+    if _hostcalls is not None:
+        _hostcalls.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
+            lib.aicas_paged_rope_append, lib.aicas_paged_decode_gqa, lib.aicas_linear_int4)))
+        _hostcalls = None
+    return lib
 
 
 def rows_ready(t: torch.Tensor, item: int):
@@ -53,7 +79,7 @@ def launch(device: torch.device, name: str, args: bytes) -> None:
     if torch.cuda.current_device() != index:
         with torch.cuda.device(device):
             return launch(device, name, args)
-    rc = getattr(nat.lib(), name)(args, raw_stream(index))
+    rc = getattr(library(), name)(args, raw_stream(index))
     if rc:
         nat.check(rc, name)
 
@@ -64,7 +90,7 @@ def launch_with_workspace(device: torch.device, name: str, bytes_name: str, args
     if torch.cuda.current_device() != device.index:
         with torch.cuda.device(device):
             return launch_with_workspace(device, name, bytes_name, args)
-    lib = nat.lib()
+    lib = library()
     stream = raw_stream(device.index)
     ws = _WORKSPACES.get((device.index, stream))
     if ws is not None:

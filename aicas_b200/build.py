@@ -5,6 +5,10 @@ source under ``aicas_b200/csrc`` is compiled by nvcc for
 ``-gencode arch=compute_100a,code=sm_100a`` and linked with the static CUDA
 runtime, so any host language can bind it through ``include/aicas_b200.h``.
 
+Beside it ``csrc/hostcalls.cpp`` becomes ``aicas_b200/_hostcalls.so``, a small
+extension (g++, torch's headers) that makes the common calls of the short
+operators cheap for this package's Python operators; they work without it.
+
 Usage: ``python -m aicas_b200.build [--force] [--verbose]``.
 """
 from __future__ import annotations
@@ -15,6 +19,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -23,6 +28,8 @@ CSRC = PKG_DIR / "csrc"
 LIB_DIR = PKG_DIR / "lib"
 OBJ_DIR = REPO_DIR / "_build" / "obj"
 LIB_PATH = LIB_DIR / "libaicas_b200.so"
+HOST_SOURCE = CSRC / "hostcalls.cpp"
+HOST_PATH = PKG_DIR / "_hostcalls.so"
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
     "-O3",
@@ -103,6 +110,29 @@ def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = Fals
     return LIB_PATH
 
 
+def build_hostcalls(force: bool = False, verbose: bool = False) -> Path:
+    """Compiles the host extension against the installed torch; returns its path."""
+    import torch
+
+    torch_dir = Path(torch.__file__).resolve().parent
+    inputs = [HOST_SOURCE, REPO_DIR / "include" / "aicas_b200.h", torch_dir / "version.py"]
+    if not force and HOST_PATH.exists() and HOST_PATH.stat().st_mtime >= max(p.stat().st_mtime for p in inputs):
+        return HOST_PATH
+    include = [REPO_DIR / "include", torch_dir / "include", torch_dir / "include/torch/csrc/api/include",
+               Path(nvcc_path()).resolve().parent.parent / "include", sysconfig.get_paths()["include"]]
+    tmp = HOST_PATH.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in include),
+           str(HOST_SOURCE), "-o", str(tmp), f"-L{torch_dir / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed on {HOST_SOURCE.name}:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, HOST_PATH)
+    return HOST_PATH
+
+
 def main(argv: list[str] | None = None) -> int:
     ap = argparse.ArgumentParser(description=__doc__)
     ap.add_argument("--force", action="store_true")
@@ -111,6 +141,7 @@ def main(argv: list[str] | None = None) -> int:
     args = ap.parse_args(argv)
     path = build(force=args.force, verbose=args.verbose, ptxas_verbose=args.ptxas_verbose)
     print(path)
+    print(build_hostcalls(force=args.force, verbose=args.verbose))
     return 0
 
 

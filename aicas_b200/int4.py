@@ -13,7 +13,7 @@ from typing import NamedTuple, Sequence
 import torch
 
 from . import _native as nat
-from ._hostpath import launch, pointer
+from ._hostpath import fast_int4, launch, pointer
 from .ops import _LINEAR_DTYPES, _overlaps, _reject_grad
 
 INT4_GROUP_SIZES = (32, 64, 128)
@@ -108,6 +108,9 @@ def decode_linear_int4(
 
     Sums are held in fp32 and the result is rounded once.  ``ValueError`` for
     what the kernel cannot take."""
+    done = fast_int4(x, weight, norm_weight, eps, residual, swiglu, out)
+    if done is not None:
+        return done
     if swiglu:
         if len(weight) != 2 or isinstance(weight, Int4Weight):
             raise ValueError("swiglu needs weight=(gate, up)")

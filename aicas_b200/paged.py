@@ -22,8 +22,8 @@ from typing import Sequence
 import torch
 
 from . import _native as nat
-from ._hostpath import heads_out, launch, launch_with_workspace, lengths, pointer, rows_ready
-from .ops import _DTYPE_CODES, SUPPORTED_HEAD_DIMS, _reject_grad
+from ._hostpath import fast_append, fast_decode, heads_out, launch, launch_with_workspace, lengths, pointer, rows_ready
+from .ops import _DTYPE_CODES, _WORKSPACES, SUPPORTED_HEAD_DIMS, _reject_grad
 
 _ITEM = {torch.float32: 4, torch.float16: 2, torch.bfloat16: 2}
 
@@ -95,6 +95,10 @@ def paged_rope_kv_append(
     cos/sin of the tensors' 16-bit dtype every operation is rounded, as Hugging
     Face's modules and :func:`rope_kv_append` round, so such a model's keys are
     the same in either cache."""
+    done = fast_append(query, key, value, cos, sin, k_pages, v_pages, page_table, positions, num_new, q_out, kv_lens_out,
+                       q_norm_weight, k_norm_weight, eps)
+    if done is not None:
+        return done
     if query.requires_grad or key.requires_grad or value.requires_grad:
         _reject_grad(query, key, value)
     what = "paged_rope_kv_append"
@@ -179,6 +183,10 @@ def paged_gqa_decode_attention(
     prompt, otherwise).  Slots outside the range may hold anything, NaN among it.
     A request without a slot gets zeros.  With ``return_lse`` the base-2 log-sum-exp
     ``[B, Hq]`` is returned too.  Page numbers outside the pool read as zeros."""
+    done = fast_decode(query, k_pages, v_pages, page_table, sm_scale, num_key_value_groups, kv_lens, kv_starts, return_lse,
+                       _WORKSPACES)
+    if done is not None:
+        return done
     if query.requires_grad or k_pages.requires_grad or v_pages.requires_grad:
         _reject_grad(query, k_pages, v_pages)
     (B, Hq, q_len, D), shape, ks, vs, page_table, max_pages, table_stride = _check_pool(
