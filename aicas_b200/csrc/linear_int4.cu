@@ -25,8 +25,9 @@
 //   * Activations: x' of a row times a power of two that brings its largest
 //     element to [2^9, 2^10), as fp16.  16-bit x is exact so (an element 2^30
 //     times smaller than the row's largest loses its last bits).  A normalised x'
-//     is rounded to fp16's 11 bits where the result has bf16's 8, and carried as
-//     two fp16 parts in neighbouring columns where the result is fp16.
+//     is carried as two fp16 parts in neighbouring columns where the result is fp16
+//     or the parts of all rows fit one block of columns (run_linear_int4), and
+//     rounded to fp16's 11 bits for the bf16 results of more rows.
 //   * Sums: a group's sum over the whole numbers q in fp32, less zero point times
 //     the group's sum of activations, times the scale in fp32; groups, warps and
 //     CTAs are added up in fp32; one rounding at the end.
@@ -76,6 +77,7 @@ struct Int4Args {
   int rows, k, n, groups;  // groups along K
   int mode;
   float eps;
+  int split;               // a row's x' is two parts, in neighbouring columns
   int s;                   // CTAs of a cluster
   int kb;                  // jobs of a tile for each of them
   int tiles, tiles_round;  // 32-row tiles of the launch; tiles of a round
@@ -237,7 +239,7 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
   const int cluster = CLUSTER ? (int)blockIdx.x / a.s : (int)blockIdx.x;
   const int kb0 = rank * a.kb;  // this CTA's first job along K
   const T* nw = static_cast<const T*>(a.norm_weight);
-  const bool split = nw != nullptr && std::is_same<T, __half>::value;  // two parts a row
+  const bool split = a.split != 0;
   const int cols = split ? 2 * a.rows : a.rows, tile_floats = cols * kPitch;
 
   if (tid == 0) *s_abort = 0;
@@ -899,7 +901,13 @@ int run_linear_int4(const aicas_linear_int4_params* p, int sms, cudaStream_t str
   const int tile_n = pair ? 16 : 32;
   a.tiles = (p->out_features + tile_n - 1) / tile_n;
   // every row at once where x' fits on chip over a cluster of up to 8 CTAs, else fewer rows a launch
-  const int columns = p->norm_weight != nullptr && !bf16 ? 2 : 1;  // a normalised x' for an fp16 result: two parts
+  // A normalised x' in two parts for an fp16 result, and for a bf16 one where both parts of every row fit the 8
+  // columns that are multiplied anyway.  One part there changes a tenth of the results of 2048 terms by a unit in the
+  // last place, two one in a hundred, for 0.4 us of staging (one row of 2048 -> 4096 6.1 against 5.6 us, 2048 ->
+  // 151936 38.3 against 38.3).  From 5 rows on two parts are twice the columns: 8 rows of 2048 -> 4096 7.8 against
+  // 6.8 us, 32 of 2048 -> 4096 23.3 against 13.4, 8 of 2048 -> 151936 81 against 42.
+  a.split = p->norm_weight != nullptr && (!bf16 || p->rows <= 4);
+  const int columns = a.split ? 2 : 1;
   int batch = p->rows, nt = 0, smem = 0;
   for (;; batch = (batch + 1) / 2) {
     const int blocks = (batch * columns + 7) / 8;

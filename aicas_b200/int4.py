@@ -100,8 +100,8 @@ def decode_linear_int4(
       ``[N, K]`` with scales of the dtype of x -> ``[R, N]``.  Several weights of
       one x (q, k and v) are one weight with their rows one after the other.
     * ``norm_weight`` ``[K]``: x' = RMSNorm(x) with that weight and ``eps`` in
-      fp32; it enters the products with fp16's 11 bits where the result has bf16's
-      8, as two fp16 parts where the result is fp16.
+      fp32; it enters the products as two fp16 parts, but with fp16's 11 bits for
+      a bf16 result of more than 4 rows.
     * ``residual`` ``[R, N]``: returns ``residual + x' W^T``; ``out=residual`` updates
       it in place.
     * ``swiglu=True`` with ``weight=(gate, up)``: ``silu(x' Wg^T) * (x' Wu^T)``.

@@ -488,7 +488,7 @@ typedef struct aicas_linear_int4_params {
   const void* x;            /* [rows, in_features], x_stride elements between rows */
   int64_t x_stride;
   const void* norm_weight;  /* optional [in_features]: x' = x * rsqrt(mean x^2 + eps) * norm_weight, in fp32
-                               (fp16's 11 bits for a bf16 result, two fp16 parts for an fp16 one); NULL: x' = x */
+                               (two fp16 parts; fp16's 11 bits for a bf16 result of more than 4 rows); NULL: x' = x */
   const void* residual;     /* RESIDUAL: [rows, out_features] */
   int64_t residual_stride;
   void* out;                /* [rows, out_features] */

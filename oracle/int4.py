@@ -25,11 +25,11 @@ def linear(x, weights, *, norm_weight=None, eps=1e-6, residual=None, swiglu=Fals
     be off before that.  fp32 sums of K terms, in whatever order: within 2^-15 of
     the sum of the terms' magnitudes (chains of up to 512 additions of relative
     error 2^-24, of terms up to 16 times larger while the zero point is still in).
-    A normalised x for a bf16 result is rounded to 11 bits: within 2^-11 of itself;
-    for an fp16 result it has two such parts, within 2^-22."""
+    A normalised x of more than 4 rows for a bf16 result is rounded to 11 bits:
+    within 2^-11 of itself; any other has two such parts, within 2^-22."""
     xd = norm_rows(x, norm_weight, eps) if norm_weight is not None else np.asarray(x, np.float64)
     ys = [xd @ w.T for w in weights]
-    rel = 2.0 ** -15 + (2.0 ** -11 if norm_weight is not None and dtype == "bf16" else 0.0)
+    rel = 2.0 ** -15 + (2.0 ** -11 if norm_weight is not None and dtype == "bf16" and xd.shape[0] > 4 else 0.0)
     offs = [rel * (np.abs(xd) @ np.abs(w).T) for w in weights]
     if swiglu:
         s = ys[0] / (1.0 + np.exp(-ys[0]))

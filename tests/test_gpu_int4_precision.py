@@ -1,0 +1,45 @@
+"""How near the 4-bit products come to their definition, beyond a bound of the
+largest error: shares of results, extreme magnitudes and infinities."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import aicas_b200 as ab
+from oracle import int4 as oi
+
+pytestmark = pytest.mark.gpu
+
+
+def _np(t):
+    return None if t is None else t.detach().float().cpu().numpy()
+
+
+def _weight(g, n, k, group, dtype, zeros, device):
+    q = torch.randint(0, 256, (n, k // 2), generator=g, dtype=torch.int32).to(torch.uint8)
+    s = ((0.5 + torch.rand(n, k // group, generator=g)) / (4 * k ** 0.5)).to(dtype)
+    z = torch.randint(0, 16, (n, k // group), generator=g, dtype=torch.int32).to(torch.uint8) if zeros else None
+    return ab.Int4Weight(q.to(device), s.to(device), None if z is None else z.to(device))
+
+
+def _wide(w):
+    return oi.widen(w.qweight.cpu().numpy(), _np(w.scales), None if w.zeros is None else w.zeros.cpu().numpy())
+
+
+@pytest.mark.parametrize("rows", [1, 2, 3, 4])
+@pytest.mark.parametrize("k,zeros,swiglu", [(2048, False, False), (1024, True, False), (640, True, True)])
+def test_normalised_rows_give_the_rounded_definition(cuda_device, rows, k, zeros, swiglu):
+    """Nearly every bf16 result is the definition's, rounded once.  Errors of the fp32
+    sums of 2^-18 of the results' size (twice as much after SiLU * up) move a result
+    over a rounding boundary, 2^-8 of it apart, in E[2 * 2^-18 / (2^-8 |y|)] of the
+    cases, about 2^-9 * 5.5 = 1.1 % for normal y: 1 in 32 is allowed (an x' of 11 bits
+    has errors of 2^-12.8 and moves one in ten)."""
+    g = torch.Generator().manual_seed(10 * k + rows)
+    x = torch.randn(rows, k, generator=g).to(torch.bfloat16).to(cuda_device)
+    nw = (1 + 0.2 * torch.randn(k, generator=g)).to(torch.bfloat16).to(cuda_device)
+    w = [_weight(g, 4096, k, 128 if k % 128 == 0 else 64, torch.bfloat16, zeros, cuda_device) for _ in range(1 + swiglu)]
+    y = ab.decode_linear_int4(x, w if swiglu else w[0], norm_weight=nw, swiglu=swiglu)
+    ref, _ = oi.linear(_np(x), [_wide(v) for v in w], norm_weight=_np(nw), swiglu=swiglu)
+    rounded = torch.from_numpy(ref).to(torch.bfloat16).float().numpy()
+    assert np.mean(_np(y) != rounded) <= 1 / 32
