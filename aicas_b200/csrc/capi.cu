@@ -433,8 +433,13 @@ int check_paged_append(const aicas_paged_append_params* p) {
     if (s < 0 || !stride_ok(s, eb)) return fail(AICAS_ERR_INVALID, "q/k/v strides must be non-negative multiples of 16 bytes");
   if (p->cs_stride_b < 0 || p->cs_stride_s < 0 || !stride_ok(p->cs_stride_b, ceb) || !stride_ok(p->cs_stride_s, ceb))
     return fail(AICAS_ERR_INVALID, "cos/sin strides must be non-negative multiples of 16 bytes");
-  if (p->kv_lens_out != nullptr && p->kv_lens_out == p->positions)
-    return fail(AICAS_ERR_INVALID, "kv_lens_out must not be positions");
+  // the first token's CTA writes a length while the other tokens' still read these
+  const auto written = [&](const int32_t* at, int64_t count) {
+    return p->kv_lens_out != nullptr && at != nullptr && p->kv_lens_out < at + count && at < p->kv_lens_out + p->batch;
+  };
+  if (written(p->positions, p->batch) || written(p->num_new, p->batch) ||
+      written(p->page_table, (p->batch - 1) * p->table_stride + p->max_pages))
+    return fail(AICAS_ERR_INVALID, "kv_lens_out must not be positions, num_new or page_table, nor share memory with them");
   if ((p->q_norm_weight != nullptr || p->k_norm_weight != nullptr) && !(p->norm_eps >= 0.0f))
     return fail(AICAS_ERR_INVALID, "norm_eps must be >= 0");
   return AICAS_OK;

@@ -121,7 +121,7 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t count) {
       sin.sizes() != cos.sizes() || !same(sin, cos) || sin.strides() != cos.strides() || !rows_ready(cos) || !rows_ready(sin))
     return none();
   if (!vector32(pos, B, q) || (fresh != nullptr && !vector32(*fresh, B, q))) return none();
-  if (lens_out != nullptr && (!vector32(*lens_out, B, q) || lens_out->data_ptr() == pos.data_ptr())) return none();
+  if (lens_out != nullptr && !vector32(*lens_out, B, q)) return none();
   for (const Tensor* w : {qw, kw})
     if (w != nullptr && (!same(*w, q) || !shaped(*w, {D}) || !w->is_contiguous())) return none();
   if (q_out != nullptr && (!same(*q_out, q) || q_out->sizes() != q.sizes() || q_out->stride(3) != 1)) return none();

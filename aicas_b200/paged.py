@@ -87,7 +87,8 @@ def paged_rope_kv_append(
     (or ``[1, S, D]``), pages ``[P, Hkv, page_size, D]``, page_table int32
     ``[B, max_pages]``, positions int32 ``[B]``.  ``num_new`` (int32 ``[B]``): only
     the first ``num_new[b]`` tokens of row ``b`` are real, the others (padding)
-    are rotated but not written.  ``kv_lens_out[b]`` receives the new length.
+    are rotated but not written.  ``kv_lens_out[b]`` receives the new length, in
+    memory of its own (not that of ``positions``, ``num_new`` or the page table).
     Tokens past the page table's end, at negative slots or with a page number
     outside the pool are dropped.
 
@@ -135,8 +136,6 @@ def paged_rope_kv_append(
     if kv_lens_out is not None and (kv_lens_out.shape != (B,) or kv_lens_out.dtype is not torch.int32
                                     or kv_lens_out.get_device() != index or not kv_lens_out.is_contiguous()):
         raise ValueError(f"{what}: kv_lens_out must be a contiguous int32 [{B}] tensor on the device")
-    if kv_lens_out is not None and kv_lens_out.data_ptr() == pos.data_ptr():
-        raise ValueError(f"{what}: kv_lens_out must not be positions (each is read while the other is written)")
     for w in (q_norm_weight, k_norm_weight):
         if w is not None and (w.shape != (D,) or w.dtype is not dtype or w.get_device() != index
                               or not w.is_contiguous()):
