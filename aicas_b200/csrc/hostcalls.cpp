@@ -160,7 +160,8 @@ PyObject* decode(PyObject*, PyObject* const* args, Py_ssize_t count) {
   for (int i = 0; i < 4; ++i)
     if ((t[i] = tensor(args[i])) == nullptr) return none();
   const Tensor *lens, *starts;
-  if (!optional(args[6], &lens) || !optional(args[7], &starts)) return none();
+  const bool want_lse = args[8] == Py_True;
+  if ((!want_lse && args[8] != Py_False) || !optional(args[6], &lens) || !optional(args[7], &starts)) return none();
   const Tensor &q = *t[0], &kp = *t[1], &vp = *t[2], &table = *t[3];
   if (q.requires_grad() || kp.requires_grad() || vp.requires_grad() || !pool_ok(q, kp, vp, table) || !sizes_ok(q)) return none();
   const int64_t B = q.size(0), Hq = q.size(1), D = q.size(3), Hkv = kp.size(1);
@@ -178,7 +179,6 @@ PyObject* decode(PyObject*, PyObject* const* args, Py_ssize_t count) {
   if (ws == nullptr) return none();
   const Tensor out = heads_out(q);
   Tensor lse;
-  const bool want_lse = args[8] == Py_True;
   if (want_lse) lse = at::empty_strided({B, Hq}, {Hq, 1}, q.options().dtype(at::kFloat));
   aicas_paged_decode_params p;
   memset(&p, 0, sizeof(p));

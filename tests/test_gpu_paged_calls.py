@@ -2,6 +2,7 @@
 however they are made."""
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
 
@@ -35,3 +36,21 @@ def test_append_refuses_lengths_over_what_it_reads(cuda_device):
         with pytest.raises(ValueError, match="nor share memory"):
             ab.paged_rope_kv_append(**(ok | more))
     ab.paged_rope_kv_append(**(ok | dict(page_table=table, kv_lens_out=buf[6:9])))
+
+
+@pytest.mark.parametrize("batch", [1, 2])
+def test_decode_returns_the_lse_for_any_true_value(cuda_device, batch):
+    """Values that are true without being True, on a stream's first call and later ones."""
+    ok = _append_args(cuda_device, batch, 1)
+    g = torch.Generator().manual_seed(2)
+    q = torch.randn(batch, 4, 1, 64, generator=g).to(torch.bfloat16).to(cuda_device)
+    kp, vp = (torch.randn(7, 2, 16, 64, generator=g).to(torch.bfloat16).to(cuda_device) for _ in range(2))
+    call = lambda flag: ab.paged_gqa_decode_attention(q, kp, vp, ok["page_table"], sm_scale=0.125,  # noqa: E731
+                                                      num_key_value_groups=2, return_lse=flag)
+    out, lse = call(True)
+    for flag in (1, np.bool_(True), "yes", torch.tensor(True)):
+        for _ in range(2):
+            got = call(flag)
+            assert isinstance(got, tuple) and torch.equal(got[0], out) and torch.equal(got[1], lse)
+    for flag in (0, np.bool_(False), None, ""):
+        assert torch.equal(call(flag), out)
