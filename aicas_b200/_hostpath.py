@@ -20,26 +20,41 @@ except ImportError:  # pragma: no cover - torch without the binding
         return torch.cuda.current_stream(index).cuda_stream
 
 
-try:  # the common calls' checks and packing, compiled; each function returns None where it leaves a call to Python
-    from . import _hostcalls
-    fast_append, fast_decode, fast_int4 = _hostcalls.append, _hostcalls.decode, _hostcalls.int4
-except ImportError:  # not built, or for another torch: the Python operators do it all
-    _hostcalls = None
+# The common calls' checks and packing, compiled.  Loaded and bound with the native
+# library (importing the package maps neither); until then, or where it was not
+# built or was built for another torch, the Python operators do it all.
+_calls = None
 
-    def fast_append(*args):
-        return None
 
-    fast_decode = fast_int4 = fast_append
+def fast_append(*args):
+    """The compiled ``paged_rope_kv_append``; None where it leaves a call to Python."""
+    return None if _calls is None else _calls.append(*args)
+
+
+def fast_decode(*args):
+    return None if _calls is None else _calls.decode(*args)
+
+
+def fast_int4(*args):
+    return None if _calls is None else _calls.int4(*args)
+
+
+_bound = False
 
 
 def library():
     """The native library, its entry points known to the compiled calls too."""
-    global _hostcalls
+    global _bound, _calls
     lib = nat.lib()
-    if _hostcalls is not None:
+    if not _bound:
+        _bound = True
+        try:
+            from . import _hostcalls
+        except ImportError:
+            return lib
         _hostcalls.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
             lib.aicas_paged_rope_append, lib.aicas_paged_decode_gqa, lib.aicas_linear_int4)))
-        _hostcalls = None
+        _calls = _hostcalls
     return lib
 
 
