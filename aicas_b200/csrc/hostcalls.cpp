@@ -12,6 +12,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty_strided.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -50,6 +51,12 @@ int dtype_code(const Tensor& t) {
 
 bool same(const Tensor& t, const Tensor& like) {
   return t.is_cuda() && t.get_device() == like.get_device() && t.scalar_type() == like.scalar_type();
+}
+
+// Autograd would have to follow one of them: the operators refuse that.
+template <typename... Ts>
+bool recorded(const Ts*... t) {
+  return c10::GradMode::is_enabled() && ((t != nullptr && t->requires_grad()) || ...);
 }
 
 bool shaped(const Tensor& t, at::IntArrayRef shape) { return t.sizes() == shape; }
@@ -111,7 +118,7 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t count) {
     return none();
   const Tensor &q = *t[0], &k = *t[1], &v = *t[2], &cos = *t[3], &sin = *t[4], &kp = *t[5], &vp = *t[6], &table = *t[7],
                &pos = *t[8];
-  if (q.requires_grad() || k.requires_grad() || v.requires_grad() || !pool_ok(q, kp, vp, table) || !sizes_ok(q)) return none();
+  if (recorded(&q, &k, &v) || !pool_ok(q, kp, vp, table) || !sizes_ok(q)) return none();
   const int64_t B = q.size(0), Hq = q.size(1), S = q.size(2), D = q.size(3), Hkv = kp.size(1);
   if (Hkv < 1 || Hq % Hkv != 0 || !shaped(k, {B, Hkv, S, D}) || !shaped(v, {B, Hkv, S, D}) || !same(k, q) || !same(v, q) ||
       !rows_ready(q) || !rows_ready(k) || !rows_ready(v))
@@ -163,7 +170,7 @@ PyObject* decode(PyObject*, PyObject* const* args, Py_ssize_t count) {
   const bool want_lse = args[8] == Py_True;
   if ((!want_lse && args[8] != Py_False) || !optional(args[6], &lens) || !optional(args[7], &starts)) return none();
   const Tensor &q = *t[0], &kp = *t[1], &vp = *t[2], &table = *t[3];
-  if (q.requires_grad() || kp.requires_grad() || vp.requires_grad() || !pool_ok(q, kp, vp, table) || !sizes_ok(q)) return none();
+  if (recorded(&q, &kp, &vp) || !pool_ok(q, kp, vp, table) || !sizes_ok(q)) return none();
   const int64_t B = q.size(0), Hq = q.size(1), D = q.size(3), Hkv = kp.size(1);
   const double scale = PyFloat_AsDouble(args[4]);
   const long long groups = PyLong_AsLongLong(args[5]);
@@ -208,7 +215,7 @@ bool weight_ok(PyObject* o, const Tensor& x, int64_t* n, int64_t* groups, aicas_
   if (!q->is_cuda() || q->get_device() != x.get_device() || q->scalar_type() != at::kByte || q->dim() != 2 ||
       q->size(1) * 2 != x.size(1) || !rows_ready(*q) || q->stride(0) * 2 < x.size(1))
     return false;
-  if (!same(*s, x) || s->dim() != 2 || s->size(0) != q->size(0) || !s->is_contiguous()) return false;
+  if (recorded(s) || !same(*s, x) || s->dim() != 2 || s->size(0) != q->size(0) || !s->is_contiguous()) return false;
   if (z != nullptr && (!z->is_cuda() || z->get_device() != x.get_device() || z->scalar_type() != at::kByte ||
                        z->sizes() != s->sizes() || !z->is_contiguous()))
     return false;
@@ -226,7 +233,7 @@ PyObject* int4(PyObject*, PyObject* const* args, Py_ssize_t count) {
   if (xp == nullptr || !optional(args[2], &nw) || !optional(args[4], &res) || !optional(args[6], &outp)) return none();
   const Tensor& x = *xp;
   const bool pair = args[5] == Py_True;
-  if ((!pair && args[5] != Py_False) || x.requires_grad() || !x.is_cuda() || x.dim() != 2) return none();
+  if ((!pair && args[5] != Py_False) || recorded(&x, nw, res) || !x.is_cuda() || x.dim() != 2) return none();
   const int code = dtype_code(x);
   const int64_t R = x.size(0), K = x.size(1);
   if ((code != AICAS_DTYPE_F16 && code != AICAS_DTYPE_BF16) || R < 1 || R > AICAS_LINEAR_MAX_ROWS || K < 1 || K > INT32_MAX ||

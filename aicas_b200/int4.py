@@ -66,6 +66,7 @@ def quantize_int4(weight: torch.Tensor, group_size: int = 128, *, symmetric: boo
 def _check_weight(w, dtype: torch.dtype, index: int, k: int):
     """(qweight, its row stride, scales, zeros, N, groups) of one weight, checked against x."""
     q, scales, zeros = w
+    _reject_grad(scales)
     if q.get_device() != index or scales.get_device() != index:
         raise ValueError("decode_linear_int4 needs CUDA tensors on one device")
     q_shape = q.shape
@@ -107,7 +108,7 @@ def decode_linear_int4(
     * ``swiglu=True`` with ``weight=(gate, up)``: ``silu(x' Wg^T) * (x' Wu^T)``.
 
     Sums are held in fp32 and the result is rounded once.  ``ValueError`` for
-    what the kernel cannot take."""
+    what the kernel cannot take, and for tensors that autograd would have to follow."""
     done = fast_int4(x, weight, norm_weight, eps, residual, swiglu, out)
     if done is not None:
         return done
@@ -119,8 +120,7 @@ def decode_linear_int4(
         first = weight
         if len(weight) != 3 or not isinstance(weight[0], torch.Tensor):
             raise ValueError("decode_linear_int4 takes one Int4Weight, or with swiglu=True a (gate, up) pair")
-    if x.requires_grad:
-        _reject_grad(x)
+    _reject_grad(x, *(t for t in (norm_weight, residual) if t is not None))
     dtype, device = x.dtype, x.device
     if device.type != "cuda":
         raise ValueError("decode_linear_int4 needs CUDA tensors")
