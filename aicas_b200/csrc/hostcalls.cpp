@@ -31,6 +31,15 @@ decltype(&aicas_linear_int4) g_int4 = nullptr;
 
 PyObject* none() { Py_RETURN_NONE; }
 
+// A launch without the GIL: one into a full queue waits for the GPU.
+template <typename F, typename... Args>
+int launch(F* entry, Args... args) {
+  PyThreadState* const thread = PyEval_SaveThread();
+  const int rc = entry(args...);
+  PyEval_RestoreThread(thread);
+  return rc;
+}
+
 // A plain tensor (or parameter), else null.
 const Tensor* tensor(PyObject* o) { return THPVariable_CheckExact(o) ? &THPVariable_Unpack(o) : nullptr; }
 
@@ -154,7 +163,7 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t count) {
   p.max_pages = (int32_t)table.size(1), p.dtype = dtype_code(q), p.cs_dtype = dtype_code(cos);
   p.norm_eps = (float)PyFloat_AsDouble(args[14]);
   if (PyErr_Occurred() != nullptr) return PyErr_Clear(), none();
-  if (g_append(&p, stream(q)) != AICAS_OK) return none();
+  if (launch(g_append, &p, stream(q)) != AICAS_OK) return none();
   return q_out != nullptr ? Py_NewRef(args[10]) : THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS
 }
@@ -182,8 +191,8 @@ PyObject* decode(PyObject*, PyObject* const* args, Py_ssize_t count) {
   THPObjectPtr key(Py_BuildValue("(iK)", (int)q.get_device(), (unsigned long long)reinterpret_cast<uintptr_t>(st)));
   PyObject* found = key ? PyDict_GetItemWithError(args[9], key.get()) : nullptr;
   if (found == nullptr) return PyErr_Clear(), none();
-  const Tensor* ws = tensor(found);
-  if (ws == nullptr) return none();
+  if (tensor(found) == nullptr) return none();
+  const Tensor ws = *tensor(found);  // held: another thread may enlarge the stream's workspace during the launch
   const Tensor out = heads_out(q);
   Tensor lse;
   if (want_lse) lse = at::empty_strided({B, Hq}, {Hq, 1}, q.options().dtype(at::kFloat));
@@ -200,7 +209,7 @@ PyObject* decode(PyObject*, PyObject* const* args, Py_ssize_t count) {
   p.batch = (int32_t)B, p.num_q_heads = (int32_t)Hq, p.num_kv_heads = (int32_t)Hkv, p.head_dim = (int32_t)D;
   p.num_pages = (int32_t)kp.size(0), p.page_size = (int32_t)kp.size(2), p.max_pages = (int32_t)table.size(1);
   p.dtype = dtype_code(q), p.sm_scale = (float)scale;
-  if (g_decode(&p, ws->data_ptr(), (size_t)ws->numel(), st) != AICAS_OK) return none();
+  if (launch(g_decode, &p, ws.data_ptr(), (size_t)ws.numel(), st) != AICAS_OK) return none();
   if (!want_lse) return THPVariable_Wrap(out);
   THPObjectPtr a(THPVariable_Wrap(out)), b(THPVariable_Wrap(lse));
   return a && b ? PyTuple_Pack(2, a.get(), b.get()) : nullptr;
@@ -275,7 +284,7 @@ PyObject* int4(PyObject*, PyObject* const* args, Py_ssize_t count) {
   p.rows = (int32_t)R, p.in_features = (int32_t)K, p.out_features = (int32_t)N, p.group_size = (int32_t)g;
   p.mode = pair ? AICAS_LINEAR_SWIGLU : res != nullptr ? AICAS_LINEAR_RESIDUAL : AICAS_LINEAR_STORE;
   p.dtype = code;
-  if (g_int4(&p, stream(x)) != AICAS_OK) return none();
+  if (launch(g_int4, &p, stream(x)) != AICAS_OK) return none();
   return outp != nullptr ? Py_NewRef(args[6]) : THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS
 }
