@@ -912,13 +912,13 @@ int aicas_paged_rope_append(const aicas_paged_append_params* p, void* stream) {
 
 size_t aicas_paged_decode_workspace_bytes(const aicas_paged_decode_params* p) {
   if (check_paged_decode(p) != AICAS_OK) return 0;
-  return aicas::paged_decode_workspace(p, sm_count());
+  return aicas::paged_decode_workspace(sm_count());
 }
 
 int aicas_paged_decode_gqa(const aicas_paged_decode_params* p, void* workspace, size_t workspace_bytes, void* stream) {
   const int rc = check_paged_decode(p);
   if (rc != AICAS_OK) return rc;
-  const size_t need = aicas::paged_decode_workspace(p, sm_count());
+  const size_t need = aicas::paged_decode_workspace(sm_count());
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(AICAS_ERR_WORKSPACE, "paged decode needs %zu bytes of zero-initialised workspace (got %zu)", need,
                 workspace_bytes);

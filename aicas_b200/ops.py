@@ -36,6 +36,11 @@ _DTYPE_CODES = {torch.float32: nat.DTYPE_F32, torch.float16: nat.DTYPE_F16, torc
 # decode kernel leaves it zeroed after every call
 _WORKSPACES: dict[tuple[int, int], torch.Tensor] = {}
 
+# Workspaces that larger ones replaced.  A CUDA graph captured before holds their
+# addresses and needs them zeroed and nobody else's; each is at most half as large
+# as the next, so they never add up to more than those in use.
+_REPLACED: list[torch.Tensor] = []
+
 
 def _stream_handle(device: torch.device) -> int:
     # an integer index: torch resolves a torch.device argument through a much
@@ -85,22 +90,35 @@ def _call_in_device(device: torch.device, fn, *args):
 def _reset_workspaces() -> None:
     """Zero-fills every workspace of this module (after a device error: a kernel
     whose bounded wait gave up may have left split counters behind)."""
-    for (dev, _), ws in list(_WORKSPACES.items()) + list(_LINEAR_WORKSPACES.items()):
-        with torch.cuda.device(dev):
+    for ws in [*_WORKSPACES.values(), *_LINEAR_WORKSPACES.values(), *_REPLACED]:
+        with torch.cuda.device(ws.device):
             ws.zero_()
-            torch.cuda.synchronize(dev)
+            torch.cuda.synchronize(ws.device)
 
 
 nat.add_device_error_hook(_reset_workspaces)
 
 
-def _workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
+def _stream_workspace(table: dict, device: torch.device, stream: int, nbytes: int, least: int) -> torch.Tensor:
+    """The stream's zeroed buffer of ``nbytes`` or more, enlarged where it is smaller.
+    Inside a capture a buffer made now would be zeroed by the graph alone, at each
+    replay: it is the graph's then, not the stream's."""
     key = (device.index, stream)
-    ws = _WORKSPACES.get(key)
-    if ws is None or ws.numel() < nbytes:
-        ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
-        _WORKSPACES[key] = ws
-    return ws
+    ws = table.get(key)
+    if ws is not None and ws.numel() >= nbytes:
+        return ws
+    if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    old = 0 if ws is None else ws.numel()
+    new = torch.zeros(max(nbytes, least, 2 * old), dtype=torch.uint8, device=device)
+    if ws is not None:
+        _REPLACED.append(ws)
+    table[key] = new
+    return new
+
+
+def _workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
+    return _stream_workspace(_WORKSPACES, device, stream, nbytes, 1 << 20)
 
 
 def _as_lens(kv_lens, batch: int, device: torch.device) -> torch.Tensor | None:
@@ -549,12 +567,7 @@ _LINEAR_DTYPES = {torch.float16: nat.DTYPE_F16, torch.bfloat16: nat.DTYPE_BF16}
 
 
 def _linear_workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
-    key = (device.index, stream)
-    ws = _LINEAR_WORKSPACES.get(key)
-    if ws is None or ws.numel() < nbytes:
-        ws = torch.zeros(max(nbytes, 4 << 20), dtype=torch.uint8, device=device)
-        _LINEAR_WORKSPACES[key] = ws
-    return ws
+    return _stream_workspace(_LINEAR_WORKSPACES, device, stream, nbytes, 4 << 20)
 
 
 def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:

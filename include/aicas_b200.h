@@ -466,8 +466,8 @@ typedef struct aicas_paged_decode_params {
   float sm_scale;
 } aicas_paged_decode_params;
 
-/* Bytes of workspace for these parameters: the layout and the rules of
-   aicas_decode_workspace_bytes (the same zero-initialised buffer serves both).
+/* Bytes of workspace, the same for all valid parameters on a device: the layout and the
+   rules of aicas_decode_workspace_bytes (the same zero-initialised buffer serves both).
    A request with no slot (kv_lens[b] <= kv_starts[b]) gets zeros.  Page numbers
    outside [0, num_pages) read as rows of zeros. */
 AICAS_API size_t aicas_paged_decode_workspace_bytes(const aicas_paged_decode_params* p);
