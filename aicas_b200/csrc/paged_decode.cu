@@ -28,7 +28,9 @@
 //     output in registers, where the softmax is.  fp32 caches use the FMA pipes.
 //   * Rounding: fp32 scores and statistics.  A probability enters P V as two
 //     16-bit parts (hi + lo), so that only the result is rounded; with up to 8
-//     heads the lo parts ride in the 8 unused rows of the same products.
+//     heads the lo parts ride in the 8 unused rows of the same products.  fp16's
+//     smallest step is 2^-24: there probabilities are held times 2^14 (up to the
+//     end of the pair), so that a weight is within 2^-39 of the largest one.
 //   * Slots out of range: scores replaced by -inf and V's elements by 0 before
 //     the products (0 * NaN), in the tiles at the range's ends only.
 //
@@ -38,6 +40,7 @@
 // lengths, page numbers, first tiles, a join over CTAs.
 #include <cstdio>
 #include <cstring>
+#include <type_traits>
 
 #include "common.cuh"
 #include "paged.cuh"
@@ -305,6 +308,8 @@ struct WarpState {
   using C = PagedCfg<T, D>;
   static constexpr int kSteps = D / 16;
   static constexpr int kH = RM / 8;  // row halves with heads in them
+  // what probabilities, and with them o and l, are multiplied by
+  static constexpr float kLift = std::is_same<T, __half>::value ? 16384.f : 1.f;
   uint32_t qf[kSteps][RM == 8 ? 2 : 4];
   float o[D / 8][4];
   float m[kH], l[kH];
@@ -388,7 +393,7 @@ struct WarpState {
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          s[n][2 * h + e] = exp2f(s[n][2 * h + e] - use);
+          s[n][2 * h + e] = exp2f(s[n][2 * h + e] - use) * kLift;
           sum += s[n][2 * h + e];
         }
       l[h] = l[h] * alpha[h] + sum;
@@ -451,9 +456,9 @@ struct WarpState {
       } else {
         v = h == 0 ? make_float2(o[n][0], o[n][1]) : make_float2(o[n][2], o[n][3]);
       }
-      *reinterpret_cast<float2*>(row + 8 * n) = v;
+      *reinterpret_cast<float2*>(row + 8 * n) = make_float2(v.x * (1.f / kLift), v.y * (1.f / kLift));
     }
-    if (i == 0) *reinterpret_cast<float2*>(red + g * C::kRedRow + D) = make_float2(m[RM == 8 ? 0 : h], sum);
+    if (i == 0) *reinterpret_cast<float2*>(red + g * C::kRedRow + D) = make_float2(m[RM == 8 ? 0 : h], sum * (1.f / kLift));
   }
 };
 
