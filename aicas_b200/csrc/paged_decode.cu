@@ -30,7 +30,10 @@
 //     16-bit parts (hi + lo), so that only the result is rounded; with up to 8
 //     heads the lo parts ride in the 8 unused rows of the same products.  fp16's
 //     smallest step is 2^-24: there probabilities are held times 2^14 (up to the
-//     end of the pair), so that a weight is within 2^-39 of the largest one.
+//     end of the pair), so that a weight is within 2^-38 of the largest one.
+//   * An infinite element of V in a live slot gives that infinity (split_pair), as long
+//     as the slot's weight is one of the numbers above: not below 2^-38 of the
+//     largest (fp16) or 2^-102 (bf16).
 //   * Slots out of range: scores replaced by -inf and V's elements by 0 before
 //     the products (0 * NaN), in the tiles at the range's ends only.
 //
@@ -129,18 +132,37 @@ template <> struct Mma<__half> {
   }
 };
 
-// hi = (T(x), T(y)) and lo = what that rounding left, as packed pairs.
+// Packed pairs hi = (x, y) cut to 16 bits and lo = what that left, rounded.  Both parts
+// of a positive weight are positive (hi is cut, not rounded; a lo of 0 becomes the
+// smallest part there is): with a 0 among them or opposite signs, an infinite element
+// of V would make a NaN (0 inf, inf - inf) where the sum is that infinity.
 template <typename T>
-__device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint32_t& lo) {
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint32_t& lo);
+template <>
+__device__ __forceinline__ void split_pair<__nv_bfloat16>(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const uint32_t bx = __float_as_uint(x), by = __float_as_uint(y);
+  hi = __byte_perm(bx, by, 0x7632);
+  constexpr float kLeast = 5.9604644775390625e-08f;  // 2^-24 of the weight, far below lo's own rounding
+  const float lx = fmaxf(x - __uint_as_float(bx & 0xffff0000u), x * kLeast);
+  const float ly = fmaxf(y - __uint_as_float(by & 0xffff0000u), y * kLeast);
   union {
-    T t[2];
+    __nv_bfloat162 b;
     uint32_t u;
-  } h, l;
-  h.t[0] = Elem<T>::from_float(x);
-  h.t[1] = Elem<T>::from_float(y);
-  l.t[0] = Elem<T>::from_float(x - Elem<T>::to_float(h.t[0]));
-  l.t[1] = Elem<T>::from_float(y - Elem<T>::to_float(h.t[1]));
-  hi = h.u;
+  } l;
+  l.b = __floats2bfloat162_rn(lx, ly);
+  lo = l.u;
+}
+template <>
+__device__ __forceinline__ void split_pair<__half>(float x, float y, uint32_t& hi, uint32_t& lo) {
+  union {
+    __half2 h;
+    uint32_t u;
+  } p, l;
+  asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(p.u) : "f"(y), "f"(x));
+  constexpr float kLeast = 5.9604644775390625e-08f;  // fp16's smallest step, 2^-24
+  const float2 f = __half22float2(p.h);
+  l.h = __floats2half2_rn(fmaxf(x - f.x, fminf(x, kLeast)), fmaxf(y - f.y, fminf(y, kLeast)));
+  hi = p.u;
   lo = l.u;
 }
 
