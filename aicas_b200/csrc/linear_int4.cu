@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
   const int cluster = CLUSTER ? (int)blockIdx.x / a.s : (int)blockIdx.x;
   const int kb0 = rank * a.kb;  // this CTA's first job along K
   const T* nw = static_cast<const T*>(a.norm_weight);
-  const bool split = a.split != 0;
+  const bool split = nw != nullptr && (std::is_same<T, __half>::value || (NT == 1 && a.split != 0));
   const int cols = split ? 2 * a.rows : a.rows, tile_floats = cols * kPitch;
 
   if (tid == 0) *s_abort = 0;
@@ -903,8 +903,8 @@ int run_linear_int4(const aicas_linear_int4_params* p, int sms, cudaStream_t str
   // every row at once where x' fits on chip over a cluster of up to 8 CTAs, else fewer rows a launch
   // A normalised x' in two parts for an fp16 result, and for a bf16 one where both parts of every row fit the 8
   // columns that are multiplied anyway.  One part there changes a tenth of the results of 2048 terms by a unit in the
-  // last place, two one in a hundred, for 0.4 us of staging (one row of 2048 -> 4096 6.1 against 5.6 us, 2048 ->
-  // 151936 38.3 against 38.3).  From 5 rows on two parts are twice the columns: 8 rows of 2048 -> 4096 7.8 against
+  // last place, two one in a hundred, for 0.3 us (one row of 2048 -> 4096 6.0 against 5.7 us, 2048 -> 151936 38.9
+  // against 38.5; products without a norm, of the same kernel, 0.2-0.3 us).  From 5 rows on two parts are twice the columns: 8 rows of 2048 -> 4096 7.8 against
   // 6.8 us, 32 of 2048 -> 4096 23.3 against 13.4, 8 of 2048 -> 151936 81 against 42.
   a.split = p->norm_weight != nullptr && (!bf16 || p->rows <= 4);
   const int columns = a.split ? 2 : 1;
