@@ -23,8 +23,11 @@
 //     tcgen05 would need the widened weights written back to shared or tensor
 //     memory: four times the bytes that came from HBM.
 //   * Activations: x' of a row times a power of two that brings its largest
-//     element to [2^9, 2^10), as fp16.  16-bit x is exact so (an element 2^30
-//     times smaller than the row's largest loses its last bits).  A normalised x'
+//     element to [2^9, 2^10), as fp16.  16-bit x is exact so down to 2^20 (fp16) or
+//     2^23 (bf16) below its row's largest element; smaller ones are off by up to
+//     2^-30 of the largest, which is half of fp16's smallest step at an odd k.  (Of a
+//     row below 2^-117, whose largest element gets no further than 2^126 times
+//     itself, by up to 2^-147.)  A normalised x'
 //     is carried as two fp16 parts in neighbouring columns where the result is fp16
 //     or the parts of all rows fit one block of columns (run_linear_int4), and
 //     rounded to fp16's 11 bits for the bf16 results of more rows.
@@ -33,7 +36,7 @@
 //     CTAs are added up in fp32; one rounding at the end.
 //   * Work: a cluster of S CTAs takes a run of 32-row tiles (16 gate + 16 up rows
 //     for SiLU * up), each CTA one S-th of K, so that its share of x' fits beside
-//     the ring (S = 1 wherever all of it does).  Tiles are taken in rounds; a
+//     the ring (run_linear_int4 chooses S).  Tiles are taken in rounds; a
 //     round's (tile, 256 k) jobs are cut evenly over the warps, whatever tile
 //     they belong to, and the warps' and CTAs' partial sums are added in a fixed
 //     order, so results repeat to the bit.  Each warp streams its own jobs through
@@ -183,29 +186,23 @@ struct Jobs {
   }
 };
 
-// Largest |x * w| over the vectors in [lo, hi) of those first, first + 32, .. below
-// end, and the sum of squares of x * by over all of them, over the warp.  w: ones where null.
+// Sum of squares of x * by over the vectors first, first + 32, .. below end, over the warp.
 template <typename T>
-__device__ __noinline__ float2 row_stats(const T* row, const T* w, int first, int end, int lo, int hi, float by) {
-  float top = 0.f, ss = 0.f;
+__device__ __noinline__ float sum_squares(const T* row, int first, int end, float by) {
+  float ss = 0.f;
 #pragma unroll 4
   for (int v = first; v < end; v += 32) {
-    float f[8], g[8];
+    float f[8];
     Elem<T>::unpack(reinterpret_cast<const uint4*>(row)[v], f);
-    if (w != nullptr) Elem<T>::unpack(reinterpret_cast<const uint4*>(w)[v], g);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float y = f[e] * by;
       ss = fmaf(y, y, ss);
-      if (v >= lo && v < hi) top = fmaxf(top, fabsf(w != nullptr ? f[e] * g[e] : f[e]));
     }
   }
 #pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) {
-    ss += __shfl_xor_sync(0xffffffffu, ss, off);
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-  }
-  return make_float2(top, ss);
+  for (int off = 16; off >= 1; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+  return ss;
 }
 
 // CLUSTER: K is split over a cluster (a kernel of its own, so that calls of one row, bound by the way to their
@@ -410,14 +407,15 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
       rstd = rsqrtf(ss / (float)a.k + a.eps);
       if (!(ss < INFINITY)) {  // squares past fp32's range: of the elements times 2^-70
         const float by = 8.470329472543003e-22f;
-        rstd = rsqrtf(row_stats<T>(x + r * a.x_stride, nw, lane, all_vecs, 0, 0, by).y / (float)a.k) * by;
+        rstd = rsqrtf(sum_squares<T>(x + r * a.x_stride, lane, all_vecs, by) / (float)a.k) * by;
       }
     }
-    // 2^e that brings the largest element to [2^9, 2^10); 1 for a row of zeros or one with inf
+    // 2^e that brings the largest element to [2^9, 2^10), or as near as 2^126 does (2^-126 to 1); 1 for a row with inf
+    // (or normalised to subnormal numbers, whose top may be far off)
     const uint32_t bits = __float_as_uint(top * rstd) >> 23;
-    const int e = bits == 0u || bits >= 255u ? 0 : min(136 - (int)bits, 100);
+    const int e = bits >= 255u || (bits == 0u && nw != nullptr) ? 0 : min(136 - (int)bits, 126);
     if (lane == 0) {
-      s_scale[r] = rstd * __uint_as_float((uint32_t)(127 + e) << 23);
+      s_scale[r] = nw != nullptr ? rstd : __uint_as_float((uint32_t)(127 + e) << 23);  // their product may be past fp32
       s_inv[r] = __uint_as_float((uint32_t)(127 - e) << 23);
     }
   };
@@ -505,8 +503,9 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
       if (nw != nullptr) {
         float w[8];
         Elem<T>::unpack(wq[j], w);
+        const float power = __uint_as_float(0x7f000000u - __float_as_uint(s_inv[xr[j]]));  // the 2^e
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] *= w[e];
+        for (int e = 0; e < 8; ++e) f[e] = f[e] * w[e] * power;
       }
       const auto put = [&](int col) {  // pairs (k0, k4), (k1, k5), (k2, k6), (k3, k7)
         union {
@@ -900,14 +899,15 @@ int run_linear_int4(const aicas_linear_int4_params* p, int sms, cudaStream_t str
   a.mode = p->mode, a.eps = p->eps, a.err = dev_err;
   const int tile_n = pair ? 16 : 32;
   a.tiles = (p->out_features + tile_n - 1) / tile_n;
-  // every row at once where x' fits on chip over a cluster of up to 8 CTAs, else fewer rows a launch
   // A normalised x' in two parts for an fp16 result, and for a bf16 one where both parts of every row fit the 8
   // columns that are multiplied anyway.  One part there changes a tenth of the results of 2048 terms by a unit in the
   // last place, two one in a hundred, for 0.3 us (one row of 2048 -> 4096 6.0 against 5.7 us, 2048 -> 151936 38.9
-  // against 38.5; products without a norm, of the same kernel, 0.2-0.3 us).  From 5 rows on two parts are twice the columns: 8 rows of 2048 -> 4096 7.8 against
-  // 6.8 us, 32 of 2048 -> 4096 23.3 against 13.4, 8 of 2048 -> 151936 81 against 42.
+  // against 38.5; products without a norm, of the same kernel, 0.2-0.3 us).  From 5 rows on two parts are twice the
+  // columns: 8 rows of 2048 -> 4096 7.8 against 6.8 us, 32 of 2048 -> 4096 23.3 against 13.4, 8 of 2048 -> 151936 81
+  // against 42.
   a.split = p->norm_weight != nullptr && (!bf16 || p->rows <= 4);
   const int columns = a.split ? 2 : 1;
+  // every row at once where x' fits on chip over a cluster of up to 8 CTAs, else fewer rows a launch
   int batch = p->rows, nt = 0, smem = 0;
   for (;; batch = (batch + 1) / 2) {
     const int blocks = (batch * columns + 7) / 8;

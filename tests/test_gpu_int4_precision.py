@@ -43,3 +43,43 @@ def test_normalised_rows_give_the_rounded_definition(cuda_device, rows, k, zeros
     ref, _ = oi.linear(_np(x), [_wide(v) for v in w], norm_weight=_np(nw), swiglu=swiglu)
     rounded = torch.from_numpy(ref).to(torch.bfloat16).float().numpy()
     assert np.mean(_np(y) != rounded) <= 1 / 32
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e-34, 1e-36, 1e-37, 2e-38, 3e-39])
+@pytest.mark.parametrize("rows", [1, 9])
+def test_rows_near_the_smallest_numbers(cuda_device, size, rows):
+    """bf16 rows down to subnormal ones.  An element may be off by 2^-30 of its row's
+    largest or by 2^-147, whichever is more, before fp32 sums and one rounding (to
+    2^-8 of the result, or half of the smallest bf16, 2^-134)."""
+    k, n = 512, 200
+    g = torch.Generator().manual_seed(int(-np.log10(size) * 10))
+    x = (size * torch.randn(rows, k, generator=g)).to(torch.bfloat16).to(cuda_device)
+    w = _weight(g, n, k, 64, torch.bfloat16, True, cuda_device)
+    w = w._replace(scales=w.scales * 16)
+    y = ab.decode_linear_int4(x, w)
+    ref, off = oi.linear(_np(x), [_wide(w)])
+    each = np.maximum(2.0 ** -30 * np.abs(_np(x)).max(1, keepdims=True).astype(np.float64), 2.0 ** -147)
+    off = off + each * np.abs(_wide(w)).sum(1)
+    over = np.abs(_np(y).astype(np.float64) - ref) - (2.0 ** -8 * (np.abs(ref) + off) + off + 2.0 ** -134)
+    assert over.max() <= 0 and np.abs(ref).max() > 0
+
+
+@pytest.mark.parametrize("rows", [1, 9])
+def test_small_rows_under_large_norm_weights(cuda_device, rows):
+    """Rows of zeros, and rows whose large norm weights meet zeros, beside tiny ones:
+    no factor on the way is infinite.  x' is fp32: what is normalised to less than its
+    smallest normal number, 2^-126, may be lost."""
+    k, n = 256, 64
+    g = torch.Generator().manual_seed(rows)
+    x = torch.randn(rows, k, generator=g) * 1e-30
+    nw = torch.full((k,), 1e-20)
+    x[:, ::5], nw[::5] = 0.0, 3e38
+    x[-1] = 0.0
+    x, nw = x.to(torch.bfloat16).to(cuda_device), nw.to(torch.bfloat16).to(cuda_device)
+    w = _weight(g, n, k, 64, torch.bfloat16, True, cuda_device)
+    w = w._replace(scales=w.scales * 2.0 ** 60)
+    y = ab.decode_linear_int4(x, w, norm_weight=nw)
+    ref, off = oi.linear(_np(x), [_wide(w)], norm_weight=_np(nw))
+    off = off + 2.0 ** -126 * np.abs(_wide(w)).sum(1)
+    assert (y[-1] == 0).all() and bool(y.isfinite().all())
+    assert np.all(np.abs(_np(y).astype(np.float64) - ref) <= 2.0 ** -8 * (np.abs(ref) + off) + off + 2.0 ** -134)
