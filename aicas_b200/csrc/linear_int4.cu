@@ -33,7 +33,8 @@
 //     rounded to fp16's 11 bits for the bf16 results of more rows.
 //   * Sums: a group's sum over the whole numbers q in fp32, less zero point times
 //     the group's sum of activations, times the scale in fp32; groups, warps and
-//     CTAs are added up in fp32; one rounding at the end.
+//     CTAs are added up in fp32; one rounding at the end.  Rows with an infinity are
+//     summed by the definition instead (define_rows), at a few us an output.
 //   * Work: a cluster of S CTAs takes a run of 32-row tiles (16 gate + 16 up rows
 //     for SiLU * up), each CTA one S-th of K, so that its share of x' fits beside
 //     the ring (run_linear_int4 chooses S).  Tiles are taken in rounds; a
@@ -74,6 +75,8 @@ struct Int4Args {
   const void* norm_weight;
   const void* residual;
   void* out;
+  const uint8_t* q[2];     // as under the tensor maps
+  int64_t q_stride[2];
   const void* scales[2];
   const uint8_t* zeros[2];
   int64_t x_stride, res_stride, out_stride;
@@ -205,6 +208,50 @@ __device__ __noinline__ float sum_squares(const T* row, int first, int end, floa
   return ss;
 }
 
+// Up to four neighbouring outputs' sums over [k0, k1) by the definition.
+template <typename T>
+__device__ __noinline__ float4 defined_sums(const Int4Args& a, int j, int r, int n, int count, int k0, int k1) {
+  const T* x = static_cast<const T*>(a.x) + r * a.x_stride;
+  const int size = a.k / a.groups;
+  float v[4] = {};
+  for (int k = k0; k < k1; k += 8) {
+    float f[8];
+    Elem<T>::unpack(*reinterpret_cast<const uint4*>(x + k), f);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (e >= count) break;
+      const int64_t grp = (int64_t)(n + e) * a.groups + k / size;
+      const uint32_t word = *reinterpret_cast<const uint32_t*>(a.q[j] + (n + e) * a.q_stride[j] + k / 2);
+      const float s = Elem<T>::to_float(static_cast<const T*>(a.scales[j])[grp]);
+      const int z = a.zeros[j] != nullptr ? a.zeros[j][grp] : 8;
+#pragma unroll
+      for (int b = 0; b < 8; ++b) v[e] = fmaf((float)((int)(word >> 4 * b & 15) - z) * s, f[b], v[e]);
+    }
+  }
+  return make_float4(v[0], v[1], v[2], v[3]);
+}
+
+// Rows with an infinity: the products' sum q x' less zero point times sum x' is inf - inf there,
+// where the definition has (q - zero) inf, an infinity unless q is the zero point.  Puts the definition's sums in
+// the place of a round's partial ones, each thread for the outputs that it adds up next.
+template <typename T, int THREADS>
+__device__ __noinline__ void define_rows(const Int4Args& a, float* part, const int* heads, const uint32_t* top, int quads,
+                                         int width, int n0, int k0, int k1) {
+  const bool pair = a.mode == AICAS_LINEAR_SWIGLU;
+  const int tile_n = pair ? 16 : 32, tile_floats = a.rows * kPitch;
+  for (int at = threadIdx.x; at < quads * a.rows; at += THREADS) {
+    const int r = at / quads, c = 4 * (at - r * quads), tile = c / tile_n;
+    if (top[r] != 0x7f800000u) continue;
+    const int place = r * kPitch + c - tile * tile_n, w0 = heads[tile] & 0xffff, w1 = heads[tile] >> 16;
+    for (int j = 0; j < (pair ? 2 : 1); ++j) {
+      *reinterpret_cast<float4*>(part + tile * tile_floats + place + 16 * j) =
+          defined_sums<T>(a, j, r, n0 + c, min(4, width - c), k0, k1);
+      for (int w = w0 + 1; w <= w1; ++w)
+        *reinterpret_cast<float4*>(part + (a.tiles_round + w) * tile_floats + place + 16 * j) = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  }
+}
+
 // CLUSTER: K is split over a cluster (a kernel of its own, so that calls of one row, bound by the way to their
 // first instruction and back, do not carry the exchange).
 // W: 32-bit words of weights that a lane takes side by side (4 W lanes' words
@@ -227,6 +274,7 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
   uint8_t* xs = smem + a.off_x;
   float* xsum = reinterpret_cast<float*>(smem + a.off_sum);   // [group of this CTA's K][NT * 8 columns]
   int* s_abort = reinterpret_cast<int*>(smem + a.off_bars + kWarps * a.stages * 8);
+  int* s_infinite = s_abort + 1;                              // some row has an infinity
   uint32_t* s_top = reinterpret_cast<uint32_t*>(s_abort + 16);   // [32] a row's largest magnitude
   float* s_scale = reinterpret_cast<float*>(s_top + 32);      // [32]
   float* s_inv = s_scale + 32;                                // [32]
@@ -239,7 +287,7 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
   const bool split = nw != nullptr && (std::is_same<T, __half>::value || (NT == 1 && a.split != 0));
   const int cols = split ? 2 * a.rows : a.rows, tile_floats = cols * kPitch;
 
-  if (tid == 0) *s_abort = 0;
+  if (tid == 0) *s_abort = 0, *s_infinite = 0;
   if (tid < 32) s_top[tid] = 0u;
   if (CLUSTER) cluster_arrive();  // waited for before the first store to another CTA
   if (lane < a.stages) mbar_init(bars + 8 * lane, 1);
@@ -417,6 +465,7 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
     if (lane == 0) {
       s_scale[r] = nw != nullptr ? rstd : __uint_as_float((uint32_t)(127 + e) << 23);  // their product may be past fp32
       s_inv[r] = __uint_as_float((uint32_t)(127 - e) << 23);
+      if (nw == nullptr && top == INFINITY) *s_infinite = 1;  // normalised, it is NaN, as the products make it
     }
   };
   for (int block = warp;;) {
@@ -682,6 +731,8 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
           if (c + e < width) out[e] = d.t[e];
       }
     };
+    if (*s_infinite != 0)
+      define_rows<T, kThreads>(a, part, s_heads, s_top, quads, width, n0, kb0 * kJobK, min(a.k, (kb0 + a.kb) * kJobK));
     for (int at = tid; at < count; at += kThreads) {
       const int r = (int)((at + 0.5f) * per_row), c = 4 * (at - r * quads);  // at / quads: below 2^14 and 2^9
       const int tile = c / tile_n, place = (split ? 2 * r : r) * kPitch + c - tile * tile_n;
@@ -886,6 +937,8 @@ int run_linear_int4(const aicas_linear_int4_params* p, int sms, cudaStream_t str
   for (int j = 0; j < (pair ? 2 : 1); ++j) {
     if (!weight_map(&a.tm_w[j], p->w[j], p->out_features, p->in_features, pair ? 16 : 32, err, errlen))
       return AICAS_ERR_UNSUPPORTED;
+    a.q[j] = static_cast<const uint8_t*>(p->w[j].q);
+    a.q_stride[j] = p->w[j].q_stride;
     a.scales[j] = p->w[j].scales;
     a.zeros[j] = static_cast<const uint8_t*>(p->w[j].zeros);
     const int segs = kJobK / p->group_size;

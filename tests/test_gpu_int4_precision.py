@@ -83,3 +83,35 @@ def test_small_rows_under_large_norm_weights(cuda_device, rows):
     off = off + 2.0 ** -126 * np.abs(_wide(w)).sum(1)
     assert (y[-1] == 0).all() and bool(y.isfinite().all())
     assert np.all(np.abs(_np(y).astype(np.float64) - ref) <= 2.0 ** -8 * (np.abs(ref) + off) + off + 2.0 ** -134)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,k,n", [(1, 256, 200), (3, 640, 100), (9, 2048, 130), (32, 6144, 70)])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("kind", ["store", "residual", "swiglu"])
+def test_infinite_elements_of_x(cuda_device, dtype, rows, k, n, zeros, kind):
+    """An infinite x comes out as the definition has it: an infinity, or NaN where it
+    meets its zero point or an opposite one.  Rows with NaN are NaN, the others are what
+    they are without either."""
+    g = torch.Generator().manual_seed(rows + k)
+    clean = torch.randn(rows, k, generator=g)
+    x = clean.clone()
+    inf = float("inf")
+    x[0, k // 3] = -inf
+    if rows > 2:
+        x[1, 5], x[1, k - 1] = inf, inf
+        x[2, 0], x[2, k - 2] = inf, float("nan")
+    if rows > 8:
+        x[4, 1::2] = inf
+        x[7, 3], x[7, k - 9] = inf, -inf
+        x[rows - 1, k // 2:] = -inf
+    w = [_weight(g, n, k, 64, dtype, zeros, cuda_device) for _ in range(1 + (kind == "swiglu"))]
+    res = torch.randn(rows, n, generator=g).to(dtype).to(cuda_device) if kind == "residual" else None
+    run = lambda t: ab.decode_linear_int4(t.to(dtype).to(cuda_device), w if kind == "swiglu" else w[0],  # noqa: E731
+                                          residual=res, swiglu=kind == "swiglu")
+    got, base = run(x), run(clean)
+    with np.errstate(all="ignore"):
+        ref, _ = oi.linear(_np(x.to(dtype)), [_wide(v) for v in w], residual=_np(res), swiglu=kind == "swiglu")
+    hit = ~x.isfinite().all(1).numpy()
+    assert np.array_equal(_np(got)[hit], ref[hit].astype(np.float32), equal_nan=True)
+    assert torch.equal(got[torch.from_numpy(~hit)], base[torch.from_numpy(~hit)]) and bool(base.isfinite().all())
