@@ -58,16 +58,26 @@ def library():
     return lib
 
 
+def steps(t: torch.Tensor) -> tuple[int, ...]:
+    """The strides of a tensor, 0 for a dimension of one entry, whose stride may be
+    any number and means nothing."""
+    return tuple([0 if n == 1 else s for n, s in zip(t.shape, t.stride())])
+
+
+def plain(t: torch.Tensor) -> torch.Tensor:
+    """A copy with the strides of its shape (``contiguous`` and ``clone`` keep odd
+    strides of dimensions of one entry)."""
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 def rows_ready(t: torch.Tensor, item: int):
-    """(t, its strides) for a 4-D tensor of ``item``-byte elements whose rows lie
+    """(t, its steps) for a 4-D tensor of ``item``-byte elements whose rows lie
     on 16 bytes, copying it where they do not."""
-    s = t.stride()
-    if s[3] == 1 and not ((s[0] | s[1] | s[2]) * item | t.data_ptr()) & 15:
-        return t, s
-    t = t.contiguous()
-    if t.data_ptr() & 15:
-        t = t.clone()
-    return t, t.stride()
+    s = steps(t)
+    if s[3] != 1 or ((s[0] | s[1] | s[2]) * item | t.data_ptr()) & 15:
+        t = plain(t)
+        s = t.stride()
+    return t, s
 
 
 def heads_out(batch: int, heads: int, seq: int, dim: int, dtype: torch.dtype, device: torch.device):

@@ -13,7 +13,7 @@ from typing import NamedTuple, Sequence
 import torch
 
 from . import _native as nat
-from ._hostpath import fast_int4, launch, pointer
+from ._hostpath import fast_int4, launch, plain, pointer
 from .ops import _LINEAR_DTYPES, _overlaps, _reject_grad
 
 INT4_GROUP_SIZES = (32, 64, 128)
@@ -77,7 +77,7 @@ def _check_weight(w, dtype: torch.dtype, index: int, k: int):
         raise ValueError(f"decode_linear_int4: scales must be contiguous [{n}, K / g] of the dtype of x")
     s = q.stride()
     if s[1] != 1 or (s[0] | q.data_ptr()) & 15 or s[0] * 2 < k:
-        q = q.contiguous().clone()
+        q = plain(q)
         s = q.stride()
     if zeros is not None and (zeros.shape != shape or zeros.dtype is not torch.uint8
                               or zeros.get_device() != index or not zeros.is_contiguous()):
@@ -132,7 +132,7 @@ def decode_linear_int4(
     index = x.get_device()
     xs = x.stride()
     if xs[1] != 1 or (xs[0] * 2 | x.data_ptr()) & 15 or xs[0] < K:  # unaligned, or rows that overlap
-        x = x.contiguous().clone()
+        x = plain(x)
         xs = x.stride()
     if R > nat.LINEAR_MAX_ROWS:
         raise ValueError(f"decode_linear_int4 takes at most {nat.LINEAR_MAX_ROWS} rows (got {R})")
@@ -156,7 +156,7 @@ def decode_linear_int4(
         if norm_weight.shape != (K,) or norm_weight.dtype is not dtype or norm_weight.get_device() != index:
             raise ValueError(f"norm_weight must be a [{K}] tensor of the dtype of x")
         if not norm_weight.is_contiguous() or norm_weight.data_ptr() & 15:
-            norm_weight = norm_weight.contiguous().clone()
+            norm_weight = plain(norm_weight)
     if out is None:
         out, out_stride = torch.empty_strided((R, N), (N, 1), dtype=dtype, device=device), N
     else:

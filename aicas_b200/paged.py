@@ -22,7 +22,8 @@ from typing import Sequence
 import torch
 
 from . import _native as nat
-from ._hostpath import fast_append, fast_decode, heads_out, launch, launch_with_workspace, lengths, pointer, rows_ready
+from ._hostpath import (fast_append, fast_decode, heads_out, launch, launch_with_workspace, lengths, plain, pointer,
+                        rows_ready, steps)
 from .ops import _DTYPE_CODES, _WORKSPACES, SUPPORTED_HEAD_DIMS, _reject_grad
 
 _ITEM = {torch.float32: 4, torch.float16: 2, torch.bfloat16: 2}
@@ -47,7 +48,7 @@ def _check_pool(what: str, query, k_pages, v_pages, page_table):
                          f"both must be one of {sorted(SUPPORTED_HEAD_DIMS)}")
     if shape[2] < 8 or shape[2] % 8:
         raise ValueError(f"{what}: page_size must be a positive multiple of 8 (got {shape[2]})")
-    ks, vs = k_pages.stride(), v_pages.stride()
+    ks, vs = steps(k_pages), steps(v_pages)
     if ks[3] != 1 or vs[3] != 1:
         raise ValueError(f"{what}: head_dim must be the unit-stride dimension of the pages")
     t_shape = page_table.shape
@@ -124,10 +125,9 @@ def paged_rope_kv_append(
     query, qi = rows_ready(query, item)
     key, ki = rows_ready(key, item)
     value, vi = rows_ready(value, item)
-    cs = cos.stride()
-    if sin.stride() != cs or cs[2] != 1 \
-            or ((cs[0] | cs[1]) * _ITEM[cs_dtype] | cos.data_ptr() | sin.data_ptr()) & 15:
-        cos, sin = cos.contiguous().clone(), sin.contiguous().clone()
+    cs = steps(cos)
+    if steps(sin) != cs or cs[2] != 1 or ((cs[0] | cs[1]) * _ITEM[cs_dtype] | cos.data_ptr() | sin.data_ptr()) & 15:
+        cos, sin = plain(cos), plain(sin)
         cs = cos.stride()
     pos = lengths(positions, B, device)
     if pos is None:
@@ -143,7 +143,7 @@ def paged_rope_kv_append(
     if q_out is None:
         q_out, qo = heads_out(B, Hq, S, D, dtype, device)
     else:
-        qo = q_out.stride()
+        qo = steps(q_out)
         if q_out.shape != (B, Hq, S, D) or q_out.dtype != dtype or q_out.device != device or qo[3] != 1:
             raise ValueError(f"{what}: q_out must be [{B}, {Hq}, {S}, {D}] with a unit-stride head_dim")
     if B == 0 or S == 0:

@@ -37,3 +37,19 @@ def test_every_tensor_that_needs_a_gradient_is_refused(cuda_device):
             assert hp._calls is None or hp.fast_int4(xx, ww, kw.get("norm_weight"), 1e-6, kw.get("residual"),
                                                      kw.get("swiglu", False), None) is not None
     assert torch.equal(ab.decode_linear_int4(x, w[0]), first)
+
+
+def test_strides_of_single_entries_mean_nothing(cuda_device):
+    """One row of x, one output feature: whatever the stride of that dimension."""
+    x, w, nw, res = _call_args(cuda_device)
+    want = ab.decode_linear_int4(x[:1], w[0], norm_weight=nw, residual=res[:1])
+    for stride in (1, 3, 256, 999):
+        row = torch.as_strided(x, (1, 256), (stride, 1))
+        got = ab.decode_linear_int4(row, w[0], norm_weight=nw, residual=torch.as_strided(res, (1, 96), (stride, 1)),
+                                    out=torch.as_strided(torch.empty_like(want), (1, 96), (stride, 1)))
+        assert torch.equal(got, want)
+    first = ab.Int4Weight(w[0].qweight[:1], w[0].scales[:1], w[0].zeros[:1])
+    one = ab.decode_linear_int4(x, first)
+    for stride in (1, 5, 48):
+        odd = first._replace(qweight=torch.as_strided(first.qweight, (1, 128), (stride, 1)))
+        assert torch.equal(ab.decode_linear_int4(x, odd), one)

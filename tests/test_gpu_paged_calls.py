@@ -54,3 +54,28 @@ def test_decode_returns_the_lse_for_any_true_value(cuda_device, batch):
             assert isinstance(got, tuple) and torch.equal(got[0], out) and torch.equal(got[1], lse)
     for flag in (0, np.bool_(False), None, ""):
         assert torch.equal(call(flag), out)
+
+
+def test_strides_of_single_entries_mean_nothing(cuda_device):
+    """A dimension of one entry may carry any stride (views, slices and transposes leave
+    odd ones): batch, heads, tokens, pages and the tables of the rotation."""
+    g = torch.Generator().manual_seed(3)
+    mk = lambda *s: torch.randn(*s, generator=g).to(torch.bfloat16).to(cuda_device)  # noqa: E731
+    odd = lambda t, *s: torch.as_strided(t, t.shape, s)  # noqa: E731
+    q, k, v = mk(1, 4, 1, 64), mk(1, 1, 1, 64), mk(1, 1, 1, 64)
+    cos, sin = (torch.randn(1, 1, 64, generator=g).to(cuda_device) for _ in range(2))
+    table = torch.zeros(1, 1, dtype=torch.int32, device=cuda_device)
+    pos = torch.tensor([2], dtype=torch.int32, device=cuda_device)
+    out = []
+    for strange in (False, True):
+        kp, vp = torch.zeros(2, 1, 1, 16, 64, dtype=torch.bfloat16, device=cuda_device)
+        a, to = [q, k, v, cos, sin, kp, vp, table], torch.zeros_like(q)
+        if strange:
+            a = [odd(q, 7, 64, 1, 1), odd(k, 3, 5, 1, 1), odd(v, 1, 1, 1, 1), odd(cos, 3, 1, 1), odd(sin, 5, 7, 1),
+                 odd(kp, 9, 1, 64, 1), odd(vp, 1, 3, 64, 1), odd(table, 11, 3)]
+            to = odd(to, 5, 64, 3, 1)
+        r = ab.paged_rope_kv_append(*a, pos, q_out=to)
+        o = ab.paged_gqa_decode_attention(a[0], *a[5:], sm_scale=0.125, num_key_value_groups=4, kv_lens=[3])
+        out.append([r, kp, vp, o])
+    for x, y in zip(*out):
+        assert torch.equal(x, y) and bool((x != 0).any())
