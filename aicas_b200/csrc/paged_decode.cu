@@ -279,6 +279,8 @@ __device__ void copy_range(const PagedArgs& a, const CUtensorMap& map, Segment s
   const uint64_t policy = l2_policy_evict_first();
   const uint32_t empty = bars + C::kWarps * C::kStages * 8;
   int number = 0;  // of the segment's next tile
+  int sent = 0;    // tiles copied by whole turns of kWarps lanes
+  int last = -1;   // the lane's tile in a turn that was not whole
   bool ok = true;
   Pages at = pages_of(a, seg, seg.t0 + lane);
   while (ok) {
@@ -306,9 +308,11 @@ __device__ void copy_range(const PagedArgs& a, const CUtensorMap& map, Segment s
             mbar_arrive_expect_tx(bar, C::kTileBytes);
             copy_box(map, dst, at.row0, head, at.page0, bar, policy);
             if (a.boxes == 2) copy_box(map, dst + C::kTileBytes / 2, at.row1, head, at.page1, bar, policy);
+            last = n;
           }
         }
         ok = __all_sync(0xffffffffu, ok);
+        if (ok) sent = number + min(first + C::kWarps, count);
       }
       number += count;
       at = ahead;
@@ -320,6 +324,13 @@ __device__ void copy_range(const PagedArgs& a, const CUtensorMap& map, Segment s
     if (!more) break;
     seg = next;
   }
+  // Leave once this warp's last copies have landed: the products' warps wait for them too, unless a wait gave up.
+  const auto landed = [&](int n) {
+    const int turn = n / C::kWarps;
+    mbar_wait(bars + 8 * (n % C::kWarps * C::kStages + turn % C::kStages), turn / C::kStages & 1, nullptr, a.err);
+  };
+  for (int n = max(0, sent - C::kWarps * C::kStages) + lane; n < sent; n += 32) landed(n);
+  if (last >= sent) landed(last);
 }
 
 // ------------------------------------------------------------------ a warp's state, 16-bit caches
