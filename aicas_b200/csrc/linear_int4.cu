@@ -83,7 +83,6 @@ struct Int4Args {
   int rows, k, n, groups;  // groups along K
   int mode;
   float eps;
-  int split;               // a row's x' is two parts, in neighbouring columns
   int s;                   // CTAs of a cluster
   int kb;                  // jobs of a tile for each of them
   int tiles, tiles_round;  // 32-row tiles of the launch; tiles of a round
@@ -255,8 +254,9 @@ __device__ __noinline__ void define_rows(const Int4Args& a, float* part, const i
 // CLUSTER: K is split over a cluster (a kernel of its own, so that calls of one row, bound by the way to their
 // first instruction and back, do not carry the exchange).
 // W: 32-bit words of weights that a lane takes side by side (4 W lanes' words
-// = 32 W of k share a group of g = 32 W).  NT: blocks of 8 columns.
-template <typename T, int NT, int W, bool CLUSTER>
+// = 32 W of k share a group of g = 32 W).  NT: blocks of 8 columns.  PARTS: a
+// normalised row is two columns.
+template <typename T, int NT, int W, bool CLUSTER, bool PARTS>
 __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(const __grid_constant__ Int4Args a) {
   constexpr int kWarps = warps_for(NT), kThreads = kWarps * 32;
   constexpr int kSegs = 8 / W;          // groups of a job
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
   const int tile_n = pair ? 16 : 32;    // output features of a tile
   const uint32_t ring = smem_u32(smem) + warp * a.stages * kJobBytes;
   const uint32_t bars = smem_u32(smem + a.off_bars) + warp * a.stages * 8;
-  float* part = reinterpret_cast<float*>(smem + a.off_part);  // [tiles_round][cols][kPitch], then [kWarps] heads
+  float* part = reinterpret_cast<float*>(smem + a.off_part);  // [tiles_round][rows][kPitch], then [kWarps] heads
   float* s_sums = part;  // before the first round: a row's sums of squares, by blocks of 256
   float* recv = reinterpret_cast<float*>(smem + a.off_recv);  // cluster: [from rank][this CTA's share of the outputs]
   uint8_t* xs = smem + a.off_x;
@@ -284,8 +284,8 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
   const int cluster = CLUSTER ? (int)blockIdx.x / a.s : (int)blockIdx.x;
   const int kb0 = rank * a.kb;  // this CTA's first job along K
   const T* nw = static_cast<const T*>(a.norm_weight);
-  const bool split = nw != nullptr && (std::is_same<T, __half>::value || (NT == 1 && a.split != 0));
-  const int cols = split ? 2 * a.rows : a.rows, tile_floats = cols * kPitch;
+  const bool split = PARTS && nw != nullptr;
+  const int tile_floats = a.rows * kPitch;
 
   if (tid == 0) *s_abort = 0, *s_infinite = 0;
   if (tid < 32) s_top[tid] = 0u;
@@ -690,9 +690,15 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int col = 8 * n + 2 * i + (e & 1);
-              if (col < cols) dst[col * kPitch + 16 * m + 8 * (e / 2)] = tot[m][n][e];
+            for (int h = 0; h < 2; ++h) {
+              float* const at = dst + 16 * m + 8 * h;
+              const float x0 = tot[m][n][2 * h], x1 = tot[m][n][2 * h + 1];
+              if (split) {  // a row's two parts are this lane's two columns
+                if (4 * n + i < a.rows) at[(4 * n + i) * kPitch] = x0 + x1;
+              } else {
+                if (8 * n + 2 * i < a.rows) at[(8 * n + 2 * i) * kPitch] = x0;
+                if (8 * n + 2 * i + 1 < a.rows) at[(8 * n + 2 * i + 1) * kPitch] = x1;
+              }
             }
       }
     }
@@ -735,7 +741,7 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
       define_rows<T, kThreads>(a, part, s_heads, s_top, quads, width, n0, kb0 * kJobK, min(a.k, (kb0 + a.kb) * kJobK));
     for (int at = tid; at < count; at += kThreads) {
       const int r = (int)((at + 0.5f) * per_row), c = 4 * (at - r * quads);  // at / quads: below 2^14 and 2^9
-      const int tile = c / tile_n, place = (split ? 2 * r : r) * kPitch + c - tile * tile_n;
+      const int tile = c / tile_n, place = r * kPitch + c - tile * tile_n;
       const int heads = s_heads[tile], w0 = heads & 0xffff, w1 = heads >> 16;
       float4 y = make_float4(0.f, 0.f, 0.f, 0.f), u = y;
       const float* const first = part + tile * tile_floats + place;
@@ -753,11 +759,7 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, 1) linear_int4_kernel(cons
         for (int w = 4; w <= w1 - w0; ++w) add4(sum, heads_at + w * tile_floats + off);
       };
       add_all(y, 0);
-      if (split) add_all(y, kPitch);
-      if (pair) {
-        add_all(u, 16);
-        if (split) add_all(u, kPitch + 16);
-      }
+      if (pair) add_all(u, 16);
       const float inv = s_inv[r];
       y.x *= inv, y.y *= inv, y.z *= inv, y.w *= inv;
       u.x *= inv, u.y *= inv, u.z *= inv, u.w *= inv;
@@ -818,7 +820,7 @@ bool weight_map(CUtensorMap* m, const aicas_int4_weight& w, int n, int k, int bo
 
 int log2_of(int v) { return v <= 1 ? 0 : 1 + log2_of(v / 2); }
 
-template <typename T, int NT, int W, bool CLUSTER>
+template <typename T, int NT, int W, bool CLUSTER, bool PARTS>
 cudaError_t launch_int4(Int4Args a, int smem, int sms, cudaStream_t st) {
   static bool attr_set[64] = {false};
   static int max_clusters[64][4] = {};  // by device and cluster size
@@ -827,7 +829,7 @@ cudaError_t launch_int4(Int4Args a, int smem, int sms, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   const bool known = dev >= 0 && dev < 64;
   if (!known || !attr_set[dev]) {
-    e = cudaFuncSetAttribute(linear_int4_kernel<T, NT, W, CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+    e = cudaFuncSetAttribute(linear_int4_kernel<T, NT, W, CLUSTER, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
     if (e != cudaSuccess) return e;
     if (known) attr_set[dev] = true;
   }
@@ -854,7 +856,7 @@ cudaError_t launch_int4(Int4Args a, int smem, int sms, cudaStream_t st) {
       cudaLaunchAttribute only = attr[1];
       cfg.attrs = &only;
       cfg.numAttrs = 1;
-      e = cudaOccupancyMaxActiveClusters(&clusters, linear_int4_kernel<T, NT, W, CLUSTER>, &cfg);
+      e = cudaOccupancyMaxActiveClusters(&clusters, linear_int4_kernel<T, NT, W, CLUSTER, PARTS>, &cfg);
       if (e != cudaSuccess) return e;
       if (clusters < 1) return cudaErrorInvalidConfiguration;
       if (cached != nullptr) *cached = clusters;
@@ -866,28 +868,33 @@ cudaError_t launch_int4(Int4Args a, int smem, int sms, cudaStream_t st) {
   a.tiles_each = a.tiles / clusters;
   a.tiles_more = a.tiles % clusters;
   cfg.gridDim = dim3((unsigned)(clusters * a.s));
-  return cudaLaunchKernelEx(&cfg, linear_int4_kernel<T, NT, W, CLUSTER>, a);
+  return cudaLaunchKernelEx(&cfg, linear_int4_kernel<T, NT, W, CLUSTER, PARTS>, a);
 }
 
-template <typename T, int NT>
+template <typename T, int NT, bool PARTS>
 cudaError_t dispatch_group(int group, const Int4Args& a, int smem, int sms, cudaStream_t st) {
   switch (group) {
-    case 32: return a.s > 1 ? launch_int4<T, NT, 1, true>(a, smem, sms, st) : launch_int4<T, NT, 1, false>(a, smem, sms, st);
-    case 64: return a.s > 1 ? launch_int4<T, NT, 2, true>(a, smem, sms, st) : launch_int4<T, NT, 2, false>(a, smem, sms, st);
-    case 128: return a.s > 1 ? launch_int4<T, NT, 4, true>(a, smem, sms, st) : launch_int4<T, NT, 4, false>(a, smem, sms, st);
+    case 32: return a.s > 1 ? launch_int4<T, NT, 1, true, PARTS>(a, smem, sms, st) : launch_int4<T, NT, 1, false, PARTS>(a, smem, sms, st);
+    case 64: return a.s > 1 ? launch_int4<T, NT, 2, true, PARTS>(a, smem, sms, st) : launch_int4<T, NT, 2, false, PARTS>(a, smem, sms, st);
+    case 128: return a.s > 1 ? launch_int4<T, NT, 4, true, PARTS>(a, smem, sms, st) : launch_int4<T, NT, 4, false, PARTS>(a, smem, sms, st);
   }
   return cudaErrorInvalidValue;
 }
 
+// parts: the rows of bf16 calls are few enough for two parts, normalised or not (a layer's products share a kernel)
 template <typename T>
-cudaError_t dispatch_int4(int nt, int group, const Int4Args& a, int smem, int sms, cudaStream_t st) {
+cudaError_t dispatch_int4(int nt, bool parts, int group, const Int4Args& a, int smem, int sms, cudaStream_t st) {
+  constexpr bool kHalf = std::is_same<T, __half>::value;
   switch (nt) {
-    case 1: return dispatch_group<T, 1>(group, a, smem, sms, st);
-    case 2: return dispatch_group<T, 2>(group, a, smem, sms, st);
-    case 4: return dispatch_group<T, 4>(group, a, smem, sms, st);
+    case 1:
+      if constexpr (!kHalf)
+        if (!parts) return dispatch_group<T, 1, false>(group, a, smem, sms, st);
+      return dispatch_group<T, 1, true>(group, a, smem, sms, st);
+    case 2: return dispatch_group<T, 2, kHalf>(group, a, smem, sms, st);
+    case 4: return dispatch_group<T, 4, kHalf>(group, a, smem, sms, st);
   }
-  if constexpr (std::is_same<T, __half>::value)  // 32 rows in two parts
-    if (nt == 8) return dispatch_group<T, 8>(group, a, smem, sms, st);
+  if constexpr (kHalf)  // 32 rows in two parts
+    if (nt == 8) return dispatch_group<T, 8, true>(group, a, smem, sms, st);
   return cudaErrorInvalidValue;
 }
 
@@ -954,12 +961,12 @@ int run_linear_int4(const aicas_linear_int4_params* p, int sms, cudaStream_t str
   a.tiles = (p->out_features + tile_n - 1) / tile_n;
   // A normalised x' in two parts for an fp16 result, and for a bf16 one where both parts of every row fit the 8
   // columns that are multiplied anyway.  One part there changes a tenth of the results of 2048 terms by a unit in the
-  // last place, two one in a hundred, for 0.3 us (one row of 2048 -> 4096 6.0 against 5.7 us, 2048 -> 151936 38.9
-  // against 38.5; products without a norm, of the same kernel, 0.2-0.3 us).  From 5 rows on two parts are twice the
-  // columns: 8 rows of 2048 -> 4096 7.8 against 6.8 us, 32 of 2048 -> 4096 23.3 against 13.4, 8 of 2048 -> 151936 81
-  // against 42.
-  a.split = p->norm_weight != nullptr && (!bf16 || p->rows <= 4);
-  const int columns = a.split ? 2 : 1;
+  // last place, two one in a hundred, for 0.2 us (one row of 2048 -> 4096 5.8 against 5.6 us, 2048 -> 151936 38.4
+  // against 38.3; products without a norm, of the same kernel, 5.1 against 5.0 for 2048 -> 2048).  From 5 rows on two
+  // parts are twice the columns: 8 rows of 2048 -> 4096 7.8 against 6.8 us, 32 of 2048 -> 4096 23.3 against 13.4, 8 of
+  // 2048 -> 151936 81 against 42, 32 263 against 136 (16-bit weights: 181).
+  const bool parts = !bf16 || p->rows <= 4;
+  const int columns = parts && p->norm_weight != nullptr ? 2 : 1;
   // every row at once where x' fits on chip over a cluster of up to 8 CTAs, else fewer rows a launch
   int batch = p->rows, nt = 0, smem = 0;
   for (;; batch = (batch + 1) / 2) {
@@ -985,8 +992,8 @@ int run_linear_int4(const aicas_linear_int4_params* p, int sms, cudaStream_t str
     a.out = static_cast<uint16_t*>(p->out) + r * p->out_stride;
     a.out_quads = reinterpret_cast<uintptr_t>(a.out) % 8 == 0 && (a.rows == 1 || p->out_stride % 4 == 0);
     a.residual = p->residual != nullptr ? static_cast<const uint16_t*>(p->residual) + r * p->residual_stride : nullptr;
-    const cudaError_t e = bf16 ? dispatch_int4<__nv_bfloat16>(nt, p->group_size, a, smem, sms, stream)
-                               : dispatch_int4<__half>(nt, p->group_size, a, smem, sms, stream);
+    const cudaError_t e = bf16 ? dispatch_int4<__nv_bfloat16>(nt, parts, p->group_size, a, smem, sms, stream)
+                               : dispatch_int4<__half>(nt, parts, p->group_size, a, smem, sms, stream);
     if (e != cudaSuccess) {
       snprintf(err, errlen, "int4 linear launch: %s (%s)", cudaGetErrorString(e), cudaGetErrorName(e));
       return AICAS_ERR_CUDA;
