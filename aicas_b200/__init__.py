@@ -5,8 +5,9 @@ Public surface = the reference package ``triton_qwen3vl``'s ``__all__``
 it leaves to Hugging Face or lacks: :func:`rope_kv_append`,
 :func:`gqa_decode_partial` and :func:`merge_partials`, and the decode-side
 products of its native decode path (:func:`decode_linear`).  A paged cache
-(:func:`paged_rope_kv_append`, :func:`paged_gqa_decode_attention`) and 4-bit
-weights (:func:`decode_linear_int4`) serve more requests in the same memory.
+(:func:`paged_rope_kv_append`, :func:`paged_gqa_decode_attention`) holds more
+requests in the same memory, and 4-bit weights (:func:`decode_linear_int4`) make
+a decode step read a quarter of the bytes.
 """
 from . import _native
 from .backends import TEXT_BACKEND_KEY, VISION_BACKEND_KEY, text_triton_attention, vision_triton_attention

@@ -2,14 +2,16 @@
 //   y[r, n] = sum_k x'[r, k] * scale[n, k / g] * (q[n, k] - zero[n, k / g])
 // with x' = x or its RMSNorm, and a residual or SiLU(gate) * up epilogue.
 //
-// HBM bound by its bytes (N K / 2 of weights for at most 2 * 32 * N K flops).  At one
-// row and many features it is near that; small products are bound by the way to the
+// HBM bound by its bytes (N K / 2 of weights for at most 2 * 32 * N K flops).  One row of
+// many features comes to 70 % of the copy rate, held back by the instructions of the
+// product loop (47 % of the issue slots); small products are bound by the way to the
 // first product (x, its statistics, x' in shared memory: 2.5 us) and the partial sums'
-// way out (1 us, 2.5 over a cluster), many rows by the products themselves.
+// way out (1 us, 2.5 over a cluster); many rows by the latency of reading x' from
+// shared memory for every 32 rows of weights (tensor pipe 8 %, issue 19 %).
 // Measured (bf16, groups of 128, norm where a layer has it; zero points but in the
-// first two): 2048 -> 151936 at one row 35.7 us, 4500 GB/s; 2048 -> 4096 at one row 5.7;
-// SiLU * up 2048 -> 6144 at 8 rows 9.0 us; 6144 -> 2048 at 32 rows 13.4 us;
-// 2048 -> 40000 at 32 rows 45 us (116 TFLOP/s).
+// first two): 2048 -> 151936 at one row 35.9 us, 4480 GB/s, at 32 rows 133 us;
+// 2048 -> 4096 at one row 5.9; SiLU * up 2048 -> 6144 at 8 rows 9.2 us; 6144 -> 2048 at
+// 32 rows 13.4 us; 2048 -> 40000 at 32 rows 46 us (114 TFLOP/s).
 //
 //   * Operands: mma.sync m16n8k16 in fp16 with the weights as the 16 x 16 side, in
 //     registers, and the activations as columns.  A 32-bit word of weights holds

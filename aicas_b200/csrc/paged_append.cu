@@ -194,8 +194,9 @@ template <typename T, typename CS>
 cudaError_t launch_append(const aicas_paged_append_params& p, cudaStream_t st) {
   // Few tokens (a decode step): a row a thread, 256 threads, the shortest way through (64 tokens of 16 + 2 * 8 heads of
   // 128: 2.6 against 5.1 us).  Many: one warp a CTA with four rows in flight each, 18 CTAs an SM (8192 tokens: 28.6
-  // against 60.3 us).  They cross between 256 (2.8, 5.1) and 1024 tokens (7.9, 7.8); with 6 + 2 * 2 heads of 64 between
-  // 256 (2.3, 2.7) and 512 (4.0, 2.7).
+  // against 60.3 us).  Where they cross depends on a token's bytes and the tables' type, and 384 tokens are a middle:
+  // 6 + 2 * 2 heads of 64 cross between 256 (2.4, 2.6) and 384 (3.8, 2.7); 16 + 2 * 8 heads of 128 near 1024 (7.7, 7.8;
+  // 512: 4.8, 5.8) with fp32 tables and below 2048 (16.7, 14.9; 1024: 9.2, 13.2) with 16-bit ones.
   return p.batch * p.seq_len <= 384 ? launch_append_rows<T, CS, 256, 1>(p, st) : launch_append_rows<T, CS, 32, 4>(p, st);
 }
 

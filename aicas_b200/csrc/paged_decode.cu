@@ -3,9 +3,10 @@
 //   t being row t % page_size of page table[b, t / page_size];
 //   lse = log2(sum_j 2^(scale log2(e) q.k_j)).
 //
-// HBM bound: every cached row is read once for the whole group of query heads
-// and used for 4 G flops a pair of elements, far below what the tensor cores
-// take, so the design is about keeping copies in flight.
+// HBM bound: every cached row is read once for up to 16 query heads of its group
+// (a larger group reads it once for each block of 16) and used for 4 flops a head
+// and pair of elements, far below what the tensor cores take, so the design is about
+// keeping copies in flight.
 //
 //   * Work: the 16-slot tiles of all (request, KV head) pairs, numbered pair by
 //     pair, are cut into equal ranges, one per CTA (one CTA an SM).  The cut is
@@ -37,8 +38,8 @@
 //   * Slots out of range: scores replaced by -inf and V's elements by 0 before
 //     the products (0 * NaN), in the tiles at the range's ends only.
 //
-// Measured (16 query over 8 KV heads of 128, bf16): 4 caches of 131072 slots 320 us,
-// 6700 GB/s; 64 ragged ones of up to 4096 slots 94.5 us, 6090 GB/s (the measured copy
+// Measured (16 query over 8 KV heads of 128, bf16): 4 caches of 131072 slots 326 us,
+// 6590 GB/s; 64 ragged ones of up to 4096 slots 94.4 us, 6090 GB/s (the measured copy
 // rate is 6450 GB/s); one cache of 1024 slots 7.9 us, which is a chain of latencies:
 // lengths, page numbers, first tiles, a join over CTAs.
 #include <cstdio>
@@ -53,9 +54,14 @@ namespace aicas {
 namespace {
 
 constexpr int kTile = 16;       // slots a tile
-constexpr int kPairCost = 6;    // what beginning and ending a pair costs a CTA, in tiles (3: 95.2, 6: 93.9, 10: 93.4 us)
-constexpr int kMinChunk = 16;   // fewest tiles a CTA takes
-constexpr int kSmallTiles = 32;   // most tiles a CTA of a launch that gives pairs whole CTAs
+// What beginning and ending a pair costs a CTA, in tiles.  3, 6, 10: 64 ragged caches of up to 4096 slots 94.6, 93.4,
+// 93.6 us; 128 of 2048 with heads of 64 89.0, 86.3, 90.0.
+constexpr int kPairCost = 6;
+// Fewest tiles a CTA takes.  8, 16, 32: one cache of 1024 slots 7.2, 7.9, 9.2 us, one of 256 6.9, 5.7, 11.5.
+constexpr int kMinChunk = 16;
+// Most tiles a CTA of a launch that gives pairs whole CTAs.  16, 32, 64: one cache of 8192 slots 12.7, 10.6, 10.7 us, 8
+// ragged ones of up to 2048 15.9, 15.9, 13.8, 128 of 2048 with heads of 64 89.2, 86.3, 89.2.
+constexpr int kSmallTiles = 32;
 constexpr int kRowsMax = 16;    // query heads of a block
 constexpr size_t kWsCounters = (size_t)1 << 20;  // counter region shared with the contiguous decode
 

@@ -91,7 +91,9 @@ def paged_rope_kv_append(
     are rotated but not written.  ``kv_lens_out[b]`` receives the new length, in
     memory of its own (not that of ``positions``, ``num_new`` or the page table).
     Tokens past the page table's end, at negative slots or with a page number
-    outside the pool are dropped.
+    outside the pool are dropped, but count: the length is ``max(positions[b], 0) +
+    num_new[b]``, at most the table's slots, as :func:`rope_kv_append` counts.  A
+    request that has nothing to append gets ``num_new[b] = 0``.
 
     With fp32 cos/sin norm and rotation are held in fp32 and rounded once; with
     cos/sin of the tensors' 16-bit dtype every operation is rounded, as Hugging

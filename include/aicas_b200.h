@@ -420,7 +420,8 @@ typedef struct aicas_paged_append_params {
   const int32_t* page_table; /* [B, max_pages], table_stride elements between requests */
   const int32_t* positions; /* [B] slot of the first new token per request */
   const int32_t* num_new;   /* optional [B]: how many of the S tokens are real (a padded batch); NULL = S */
-  int32_t* kv_lens_out;     /* optional [B]: receives min(max(positions[b], 0) + num_new[b], capacity); shares no
+  int32_t* kv_lens_out;     /* optional [B]: receives min(max(positions[b], 0) + num_new[b], capacity), also where
+                               tokens were dropped (num_new[b] = 0 leaves a request as it is); shares no
                                memory with positions, num_new or page_table */
   const void* q_norm_weight; /* optional [D] (dtype of q): per-head RMSNorm before RoPE */
   const void* k_norm_weight; /* optional [D] */
