@@ -7,10 +7,14 @@ it leaves to Hugging Face or lacks: :func:`rope_kv_append`,
 products of its native decode path (:func:`decode_linear`).  A paged cache
 (:func:`paged_rope_kv_append`, :func:`paged_gqa_decode_attention`) holds more
 requests in the same memory, and 4-bit weights (:func:`decode_linear_int4`) make
-a decode step read a quarter of the bytes.
+a decode step read a quarter of the bytes.  A cache of 4-bit rows
+(:func:`paged_rope_kv_append_int4`, :func:`paged_gqa_decode_attention_int4`) does the
+same for long contexts, and eviction by attention weight
+(:func:`paged_attention_weights`, :func:`paged_kv_evict`) bounds their length.
 """
 from . import _native
 from .backends import TEXT_BACKEND_KEY, VISION_BACKEND_KEY, text_triton_attention, vision_triton_attention
+from .eviction import paged_attention_weights, paged_kv_evict
 from .int4 import Int4Weight, decode_linear_int4, quantize_int4
 from .ops import (
     decode_linear,
@@ -23,6 +27,14 @@ from .ops import (
     vision_rope,
 )
 from .paged import PagedKVCache, paged_gqa_decode_attention, paged_rope_kv_append
+from .paged_int4 import (
+    Int4Pages,
+    int4_pages,
+    paged_gqa_decode_attention_int4,
+    paged_kv_read_int4,
+    paged_rope_kv_append_int4,
+    quantize_kv_int4,
+)
 from .patch import install_qwen3vl_triton_attention
 
 
@@ -36,6 +48,7 @@ def __getattr__(name: str):
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 __all__ = [
+    "Int4Pages",
     "Int4Weight",
     "NATIVE_AVAILABLE",
     "PagedKVCache",
@@ -48,10 +61,17 @@ __all__ = [
     "gqa_decode_partial",
     "gqa_flash_attention",
     "install_qwen3vl_triton_attention",
+    "int4_pages",
     "merge_partials",
+    "paged_attention_weights",
     "paged_gqa_decode_attention",
+    "paged_gqa_decode_attention_int4",
+    "paged_kv_evict",
+    "paged_kv_read_int4",
     "paged_rope_kv_append",
+    "paged_rope_kv_append_int4",
     "quantize_int4",
+    "quantize_kv_int4",
     "rope_kv_append",
     "text_triton_attention",
     "varlen_flash_attention",

@@ -39,6 +39,8 @@ CAP_VISION_ROPE = 128
 CAP_VISION_QKV = 256
 CAP_PAGED = 512
 CAP_LINEAR_INT4 = 1024
+CAP_PAGED_INT4 = 2048
+CAP_PAGED_EVICT = 4096
 
 LINEAR_MAX_SEGMENTS = 4
 LINEAR_MAX_ROWS = 32
@@ -190,6 +192,78 @@ class PagedDecodeParams(ctypes.Structure):
     ]
 
 
+class Int4PagesRef(ctypes.Structure):
+    _fields_ = [("codes", _vp), ("scales", _vp), ("cs_p", _i64), ("cs_h", _i64), ("cs_t", _i64),
+                ("ss_p", _i64), ("ss_h", _i64), ("ss_t", _i64)]
+
+
+class PagedAppendInt4Params(ctypes.Structure):
+    _fields_ = [
+        ("q_in", _vp), ("q_out", _vp), ("k_in", _vp), ("v_in", _vp), ("cos", _vp), ("sin", _vp),
+        ("kv", Int4PagesRef * 2), ("page_table", _vp), ("positions", _vp), ("num_new", _vp),
+        ("kv_lens_out", _vp), ("q_norm_weight", _vp), ("k_norm_weight", _vp),
+        ("qi_stride_b", _i64), ("qi_stride_h", _i64), ("qi_stride_s", _i64),
+        ("qo_stride_b", _i64), ("qo_stride_h", _i64), ("qo_stride_s", _i64),
+        ("k_stride_b", _i64), ("k_stride_h", _i64), ("k_stride_s", _i64),
+        ("v_stride_b", _i64), ("v_stride_h", _i64), ("v_stride_s", _i64),
+        ("cs_stride_b", _i64), ("cs_stride_s", _i64), ("table_stride", _i64),
+        ("batch", _i32), ("num_q_heads", _i32), ("num_kv_heads", _i32), ("seq_len", _i32), ("head_dim", _i32),
+        ("group_size", _i32), ("num_pages", _i32), ("page_size", _i32), ("max_pages", _i32), ("dtype", _i32),
+        ("cs_dtype", _i32), ("norm_eps", _f32),
+    ]
+
+
+class PagedReadInt4Params(ctypes.Structure):
+    _fields_ = [
+        ("kv", Int4PagesRef * 2), ("out", _vp * 2), ("page_table", _vp), ("positions", _vp), ("num_tokens", _vp),
+        ("out_stride_b", _i64), ("out_stride_h", _i64), ("out_stride_s", _i64), ("table_stride", _i64),
+        ("batch", _i32), ("num_kv_heads", _i32), ("seq_len", _i32), ("head_dim", _i32), ("group_size", _i32),
+        ("num_pages", _i32), ("page_size", _i32), ("max_pages", _i32), ("dtype", _i32),
+    ]
+
+
+class PagedDecodeInt4Params(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("kv", Int4PagesRef * 2), ("out", _vp), ("lse", _vp),
+        ("page_table", _vp), ("kv_lens", _vp), ("kv_starts", _vp),
+        ("q_stride_b", _i64), ("q_stride_h", _i64), ("o_stride_b", _i64), ("o_stride_h", _i64), ("table_stride", _i64),
+        ("batch", _i32), ("num_q_heads", _i32), ("num_kv_heads", _i32), ("head_dim", _i32), ("group_size", _i32),
+        ("num_pages", _i32), ("page_size", _i32), ("max_pages", _i32), ("dtype", _i32), ("sm_scale", _f32),
+    ]
+
+
+class PagedWeightsParams(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("k_pages", _vp), ("k_scales", _vp), ("lse", _vp), ("weights", _vp),
+        ("page_table", _vp), ("kv_lens", _vp), ("kv_starts", _vp),
+        ("q_stride_b", _i64), ("q_stride_h", _i64), ("q_stride_s", _i64),
+        ("lse_stride_b", _i64), ("lse_stride_h", _i64), ("lse_stride_s", _i64),
+        ("w_stride_b", _i64), ("w_stride_h", _i64),
+        ("kp_stride_p", _i64), ("kp_stride_h", _i64), ("kp_stride_t", _i64),
+        ("ks_stride_p", _i64), ("ks_stride_h", _i64), ("ks_stride_t", _i64), ("table_stride", _i64),
+        ("batch", _i32), ("num_q_heads", _i32), ("num_kv_heads", _i32), ("seq_len", _i32), ("head_dim", _i32),
+        ("group_size", _i32), ("num_pages", _i32), ("page_size", _i32), ("max_pages", _i32), ("dtype", _i32),
+        ("sm_scale", _f32),
+    ]
+
+
+EVICT_MAX_PLANES = 4
+
+
+class EvictPlane(ctypes.Structure):
+    _fields_ = [("data", _vp), ("stride_p", _i64), ("stride_h", _i64), ("stride_t", _i64), ("row_bytes", _i64)]
+
+
+class PagedEvictParams(ctypes.Structure):
+    _fields_ = [
+        ("plane", EvictPlane * EVICT_MAX_PLANES), ("weights", _vp), ("weights_out", _vp), ("kept", _vp),
+        ("page_table", _vp), ("kv_lens", _vp), ("kv_lens_out", _vp),
+        ("w_stride_b", _i64), ("w_stride_h", _i64), ("wo_stride_b", _i64), ("wo_stride_h", _i64), ("table_stride", _i64),
+        ("num_planes", _i32), ("batch", _i32), ("num_kv_heads", _i32), ("num_pages", _i32), ("page_size", _i32),
+        ("max_pages", _i32), ("keep", _i32), ("keep_first", _i32), ("keep_last", _i32), ("longer_than", _i32),
+    ]
+
+
 class Int4WeightRef(ctypes.Structure):
     _fields_ = [("q", _vp), ("scales", _vp), ("zeros", _vp), ("q_stride", _i64)]
 
@@ -212,6 +286,8 @@ def packer(params) -> struct.Struct:
         for _, kind in cls._fields_:
             if kind in _CODES:
                 yield _CODES[kind]
+            elif kind._type_ in _CODES:  # an array
+                yield _CODES[kind._type_] * kind._length_
             else:  # an array of structs
                 yield "".join(codes(kind._type_)) * kind._length_
 
@@ -225,6 +301,11 @@ _CODES = {_vp: "P", _i64: "q", _i32: "i", _f32: "f"}
 PACK_PAGED_APPEND = packer(PagedAppendParams)
 PACK_PAGED_DECODE = packer(PagedDecodeParams)
 PACK_LINEAR_INT4 = packer(LinearInt4Params)
+PACK_PAGED_APPEND_INT4 = packer(PagedAppendInt4Params)
+PACK_PAGED_READ_INT4 = packer(PagedReadInt4Params)
+PACK_PAGED_DECODE_INT4 = packer(PagedDecodeInt4Params)
+PACK_PAGED_WEIGHTS = packer(PagedWeightsParams)
+PACK_PAGED_EVICT = packer(PagedEvictParams)
 
 
 # name -> (restype, argtypes); exactly the functions declared in include/aicas_b200.h
@@ -253,6 +334,12 @@ EXPORTS = {
     "aicas_paged_rope_append": (ctypes.c_int, [_vp, _vp]),
     "aicas_paged_decode_workspace_bytes": (ctypes.c_size_t, [_vp]),
     "aicas_paged_decode_gqa": (ctypes.c_int, [_vp, _vp, ctypes.c_size_t, _vp]),
+    "aicas_paged_append_int4": (ctypes.c_int, [_vp, _vp]),
+    "aicas_paged_read_int4": (ctypes.c_int, [_vp, _vp]),
+    "aicas_paged_decode_int4_workspace_bytes": (ctypes.c_size_t, [_vp]),
+    "aicas_paged_decode_int4": (ctypes.c_int, [_vp, _vp, ctypes.c_size_t, _vp]),
+    "aicas_paged_weights": (ctypes.c_int, [_vp, _vp]),
+    "aicas_paged_evict": (ctypes.c_int, [_vp, _vp]),
     "aicas_linear_int4": (ctypes.c_int, [_vp, _vp]),
     "aicas_version": (ctypes.c_char_p, []),
     "aicas_capabilities": (ctypes.c_uint32, []),

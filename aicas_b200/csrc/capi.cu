@@ -14,6 +14,7 @@
 #include "linear.cuh"
 #include "linear_int4.cuh"
 #include "paged.cuh"
+#include "paged_int4.cuh"
 #include "vision_qkv.cuh"
 
 namespace aicas {
@@ -467,6 +468,206 @@ int check_paged_decode(const aicas_paged_decode_params* p) {
   return AICAS_OK;
 }
 
+// What the entry points over pages share beside the pools: sizes and the page table.
+int check_table(const int32_t* table, int64_t table_stride, int batch, int hkv, int num_pages, int page_size, int max_pages) {
+  if (table == nullptr) return fail(AICAS_ERR_INVALID, "page_table must be set");
+  if (batch < 1 || hkv < 1 || num_pages < 1 || max_pages < 1)
+    return fail(AICAS_ERR_INVALID, "batch=%d num_kv_heads=%d num_pages=%d max_pages=%d", batch, hkv, num_pages, max_pages);
+  if (page_size < 8 || page_size % 8 != 0)
+    return fail(AICAS_ERR_UNSUPPORTED, "page_size must be a positive multiple of 8 (got %d)", page_size);
+  if ((int64_t)max_pages * page_size > (int64_t)INT32_MAX - 4096)
+    return fail(AICAS_ERR_UNSUPPORTED, "max_pages * page_size = %lld slots a request is past 2^31",
+                (long long)max_pages * page_size);
+  if ((reinterpret_cast<uintptr_t>(table) & 3u) != 0 || table_stride < 0)
+    return fail(AICAS_ERR_INVALID, "page_table must be 4-byte aligned with a non-negative stride");
+  return AICAS_OK;
+}
+
+int check_int4_shape(int dtype, int head_dim, int group) {
+  if (dtype != AICAS_DTYPE_F16 && dtype != AICAS_DTYPE_BF16)
+    return fail(AICAS_ERR_UNSUPPORTED, "a 4-bit cache needs fp16 or bf16 tensors (dtype %d)", dtype);
+  if (head_dim != 64 && head_dim != 128) return fail(AICAS_ERR_UNSUPPORTED, "4-bit head_dim %d not in {64,128}", head_dim);
+  if (group != 64 && group != head_dim)
+    return fail(AICAS_ERR_UNSUPPORTED, "group_size %d must be 64 or head_dim %d", group, head_dim);
+  return AICAS_OK;
+}
+
+int check_codes(const void* codes, const void* scales, const int64_t cs[3], const int64_t ss[3], int pairs) {
+  if (codes == nullptr || scales == nullptr) return fail(AICAS_ERR_INVALID, "codes and scales of the pages must be set");
+  if (!aligned16(codes)) return fail(AICAS_ERR_INVALID, "the codes must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(scales) % (4 * pairs) != 0)
+    return fail(AICAS_ERR_INVALID, "the scales must be aligned to a row's pairs");
+  for (int i = 0; i < 3; ++i) {
+    if (cs[i] < 0 || cs[i] % 16 != 0 || cs[i] >= ((int64_t)1 << 40))
+      return fail(AICAS_ERR_INVALID, "strides of the codes must be non-negative multiples of 16 bytes below 2^40");
+    if (ss[i] < 0 || ss[i] % (2 * pairs) != 0 || ss[i] >= ((int64_t)1 << 40))
+      return fail(AICAS_ERR_INVALID, "strides of the scales must be non-negative multiples of a row's pairs below 2^40");
+  }
+  return AICAS_OK;
+}
+
+int check_int4_pages(const aicas_int4_pages kv[2], int dtype, int head_dim, int group, const int32_t* table,
+                     int64_t table_stride, int batch, int hkv, int num_pages, int page_size, int max_pages) {
+  int rc = check_table(table, table_stride, batch, hkv, num_pages, page_size, max_pages);
+  if (rc == AICAS_OK) rc = check_int4_shape(dtype, head_dim, group);
+  for (int i = 0; i < 2 && rc == AICAS_OK; ++i) {
+    const int64_t cs[3] = {kv[i].cs_p, kv[i].cs_h, kv[i].cs_t}, ss[3] = {kv[i].ss_p, kv[i].ss_h, kv[i].ss_t};
+    rc = check_codes(kv[i].codes, kv[i].scales, cs, ss, head_dim / group);
+  }
+  return rc;
+}
+
+// Lengths that a call writes may not lie in what its other CTAs still read.
+bool lengths_overlap(const int32_t* out, int batch, const int32_t* at, int64_t count) {
+  return out != nullptr && at != nullptr && out < at + count && at < out + batch;
+}
+
+int check_paged_append_int4(const aicas_paged_append_int4_params* p) {
+  if (p == nullptr) return fail(AICAS_ERR_INVALID, "params is NULL");
+  if (p->q_in == nullptr || p->q_out == nullptr || p->k_in == nullptr || p->v_in == nullptr || p->cos == nullptr ||
+      p->sin == nullptr || p->positions == nullptr)
+    return fail(AICAS_ERR_INVALID, "q_in, q_out, k_in, v_in, cos, sin and positions must be set");
+  const int rc = check_int4_pages(p->kv, p->dtype, p->head_dim, p->group_size, p->page_table, p->table_stride, p->batch,
+                                  p->num_kv_heads, p->num_pages, p->page_size, p->max_pages);
+  if (rc != AICAS_OK) return rc;
+  if (p->num_q_heads < 1 || p->num_q_heads % p->num_kv_heads != 0)
+    return fail(AICAS_ERR_INVALID, "num_q_heads=%d is not a multiple of num_kv_heads=%d", p->num_q_heads, p->num_kv_heads);
+  if (p->cs_dtype != p->dtype && p->cs_dtype != AICAS_DTYPE_F32)
+    return fail(AICAS_ERR_UNSUPPORTED, "cos/sin dtype must equal the tensor dtype or be fp32");
+  if (p->seq_len < 1 || (int64_t)p->batch * p->seq_len > (int64_t)INT32_MAX)
+    return fail(AICAS_ERR_INVALID, "seq_len=%d of batch %d", p->seq_len, p->batch);
+  const int ceb = elem_bytes(p->cs_dtype);
+  const void* ptr[] = {p->q_in, p->q_out, p->k_in, p->v_in, p->cos, p->sin, p->q_norm_weight, p->k_norm_weight};
+  for (const void* x : ptr)
+    if (!aligned16(x)) return fail(AICAS_ERR_INVALID, "device pointers must be 16-byte aligned");
+  const int64_t rows[] = {p->qi_stride_b, p->qi_stride_h, p->qi_stride_s, p->qo_stride_b, p->qo_stride_h, p->qo_stride_s,
+                          p->k_stride_b,  p->k_stride_h,  p->k_stride_s,  p->v_stride_b,  p->v_stride_h,  p->v_stride_s};
+  for (int64_t s : rows)
+    if (s < 0 || !stride_ok(s, 2)) return fail(AICAS_ERR_INVALID, "q/k/v strides must be non-negative multiples of 16 bytes");
+  if (p->cs_stride_b < 0 || p->cs_stride_s < 0 || !stride_ok(p->cs_stride_b, ceb) || !stride_ok(p->cs_stride_s, ceb))
+    return fail(AICAS_ERR_INVALID, "cos/sin strides must be non-negative multiples of 16 bytes");
+  if (lengths_overlap(p->kv_lens_out, p->batch, p->positions, p->batch) ||
+      lengths_overlap(p->kv_lens_out, p->batch, p->num_new, p->batch) ||
+      lengths_overlap(p->kv_lens_out, p->batch, p->page_table, (p->batch - 1) * p->table_stride + p->max_pages))
+    return fail(AICAS_ERR_INVALID, "kv_lens_out must not be positions, num_new or page_table, nor share memory with them");
+  if ((p->q_norm_weight != nullptr || p->k_norm_weight != nullptr) && !(p->norm_eps >= 0.0f))
+    return fail(AICAS_ERR_INVALID, "norm_eps must be >= 0");
+  return AICAS_OK;
+}
+
+int check_paged_read_int4(const aicas_paged_read_int4_params* p) {
+  if (p == nullptr) return fail(AICAS_ERR_INVALID, "params is NULL");
+  if (p->out[0] == nullptr || p->out[1] == nullptr || p->positions == nullptr)
+    return fail(AICAS_ERR_INVALID, "out and positions must be set");
+  const int rc = check_int4_pages(p->kv, p->dtype, p->head_dim, p->group_size, p->page_table, p->table_stride, p->batch,
+                                  p->num_kv_heads, p->num_pages, p->page_size, p->max_pages);
+  if (rc != AICAS_OK) return rc;
+  if (p->seq_len < 1) return fail(AICAS_ERR_INVALID, "seq_len=%d", p->seq_len);
+  if (!aligned16(p->out[0]) || !aligned16(p->out[1])) return fail(AICAS_ERR_INVALID, "out must be 16-byte aligned");
+  const int64_t st[] = {p->out_stride_b, p->out_stride_h, p->out_stride_s};
+  for (int64_t s : st)
+    if (s < 0 || !stride_ok(s, 2)) return fail(AICAS_ERR_INVALID, "out strides must be non-negative multiples of 16 bytes");
+  return AICAS_OK;
+}
+
+int check_scale(float sm_scale) {
+  return sm_scale == sm_scale && sm_scale != INFINITY && sm_scale != -INFINITY
+             ? AICAS_OK
+             : fail(AICAS_ERR_INVALID, "sm_scale must be finite");
+}
+
+int check_paged_decode_int4(const aicas_paged_decode_int4_params* p) {
+  if (p == nullptr) return fail(AICAS_ERR_INVALID, "params is NULL");
+  if (p->q == nullptr || p->out == nullptr) return fail(AICAS_ERR_INVALID, "q and out must be non-NULL");
+  const int rc = check_int4_pages(p->kv, p->dtype, p->head_dim, p->group_size, p->page_table, p->table_stride, p->batch,
+                                  p->num_kv_heads, p->num_pages, p->page_size, p->max_pages);
+  if (rc != AICAS_OK) return rc;
+  if (p->num_q_heads < 1 || p->num_q_heads % p->num_kv_heads != 0)
+    return fail(AICAS_ERR_INVALID, "num_q_heads=%d is not a multiple of num_kv_heads=%d", p->num_q_heads, p->num_kv_heads);
+  if (!aligned16(p->q) || !aligned16(p->out)) return fail(AICAS_ERR_INVALID, "q and out must be 16-byte aligned");
+  const int64_t qo[] = {p->q_stride_b, p->q_stride_h, p->o_stride_b, p->o_stride_h};
+  for (int64_t s : qo)
+    if (s < 0 || !stride_ok(s, 2)) return fail(AICAS_ERR_INVALID, "q/out strides must be non-negative multiples of 16 bytes");
+  // tiles of (request, KV head, block of query heads), and a few more each, are numbered with 32-bit ints
+  const int64_t tiles = (((int64_t)p->max_pages * p->page_size + 15) / 16 + 16) * p->batch *
+                        ((int64_t)p->num_kv_heads * ((p->num_q_heads / p->num_kv_heads + 7) / 8));
+  if (tiles > (int64_t)INT32_MAX / 2)
+    return fail(AICAS_ERR_UNSUPPORTED, "%lld tiles of 16 slots exceed the 2^30 of one launch", (long long)tiles);
+  return check_scale(p->sm_scale);
+}
+
+int check_paged_weights(const aicas_paged_weights_params* p) {
+  if (p == nullptr) return fail(AICAS_ERR_INVALID, "params is NULL");
+  if (p->q == nullptr || p->lse == nullptr || p->weights == nullptr || p->k_pages == nullptr)
+    return fail(AICAS_ERR_INVALID, "q, k_pages, lse and weights must be set");
+  int rc = check_table(p->page_table, p->table_stride, p->batch, p->num_kv_heads, p->num_pages, p->page_size, p->max_pages);
+  if (rc != AICAS_OK) return rc;
+  const int eb = elem_bytes(p->dtype);
+  if (eb == 0) return fail(AICAS_ERR_UNSUPPORTED, "unknown dtype %d", p->dtype);
+  const int64_t kp[3] = {p->kp_stride_p, p->kp_stride_h, p->kp_stride_t}, ks[3] = {p->ks_stride_p, p->ks_stride_h, p->ks_stride_t};
+  if (p->group_size != 0) {
+    rc = check_int4_shape(p->dtype, p->head_dim, p->group_size);
+    if (rc == AICAS_OK) rc = check_codes(p->k_pages, p->k_scales, kp, ks, p->head_dim / p->group_size);
+    if (rc != AICAS_OK) return rc;
+  } else {
+    if (!head_dim_ok(p->head_dim)) return fail(AICAS_ERR_UNSUPPORTED, "head_dim %d not in {16,32,64,128}", p->head_dim);
+    if (!aligned16(p->k_pages)) return fail(AICAS_ERR_INVALID, "the pages must be 16-byte aligned");
+    for (int64_t s : kp)
+      if (s < 0 || !stride_ok(s, eb) || s * eb >= ((int64_t)1 << 40))
+        return fail(AICAS_ERR_INVALID, "page strides must be non-negative multiples of 16 bytes below 2^40");
+  }
+  if (p->num_q_heads < 1 || p->num_q_heads % p->num_kv_heads != 0)
+    return fail(AICAS_ERR_INVALID, "num_q_heads=%d is not a multiple of num_kv_heads=%d", p->num_q_heads, p->num_kv_heads);
+  if (p->seq_len < 1 || (int64_t)p->seq_len * p->num_q_heads > INT32_MAX)
+    return fail(AICAS_ERR_INVALID, "seq_len=%d of %d heads", p->seq_len, p->num_q_heads);
+  if (!aligned16(p->q) || !stride_ok(p->q_stride_b, eb) || !stride_ok(p->q_stride_h, eb) || !stride_ok(p->q_stride_s, eb) ||
+      p->q_stride_b < 0 || p->q_stride_h < 0 || p->q_stride_s < 0)
+    return fail(AICAS_ERR_INVALID, "q must be 16-byte aligned with strides that are non-negative multiples of 16 bytes");
+  const int64_t st[] = {p->lse_stride_b, p->lse_stride_h, p->lse_stride_s, p->w_stride_b, p->w_stride_h};
+  for (int64_t s : st)
+    if (s < 0) return fail(AICAS_ERR_INVALID, "strides of lse and weights must not be negative");
+  if (((reinterpret_cast<uintptr_t>(p->lse) | reinterpret_cast<uintptr_t>(p->weights)) & 3u) != 0)
+    return fail(AICAS_ERR_INVALID, "lse and weights must be 4-byte aligned");
+  const int64_t tiles = (((int64_t)p->max_pages * p->page_size + 15) / 16 + 1) * p->batch * p->num_kv_heads;
+  if (tiles > (int64_t)INT32_MAX / 2)
+    return fail(AICAS_ERR_UNSUPPORTED, "%lld tiles of 16 slots exceed the 2^30 of one launch", (long long)tiles);
+  return check_scale(p->sm_scale);
+}
+
+int check_paged_evict(const aicas_paged_evict_params* p) {
+  if (p == nullptr) return fail(AICAS_ERR_INVALID, "params is NULL");
+  if (p->weights == nullptr || p->weights_out == nullptr || p->kept == nullptr || p->kv_lens == nullptr)
+    return fail(AICAS_ERR_INVALID, "weights, weights_out, kept and kv_lens must be set");
+  const int rc = check_table(p->page_table, p->table_stride, p->batch, p->num_kv_heads, p->num_pages, p->page_size, p->max_pages);
+  if (rc != AICAS_OK) return rc;
+  if (p->num_planes < 1 || p->num_planes > AICAS_EVICT_MAX_PLANES)
+    return fail(AICAS_ERR_INVALID, "num_planes=%d not in 1..%d", p->num_planes, AICAS_EVICT_MAX_PLANES);
+  for (int i = 0; i < p->num_planes; ++i) {
+    const aicas_evict_plane& pl = p->plane[i];
+    const int64_t bytes = pl.row_bytes;
+    if (pl.data == nullptr || (bytes != 4 && bytes != 8 && (bytes < 16 || bytes > 512 || bytes % 16 != 0 || (bytes > 128 && bytes % 128 != 0))))
+      return fail(AICAS_ERR_INVALID, "a plane needs rows of 4, 8, or a multiple of 16 (above 128: of 128) up to 512 bytes (got %lld)",
+                  (long long)bytes);
+    const int64_t unit = bytes < 16 ? bytes : 16, st[] = {pl.stride_p, pl.stride_h, pl.stride_t};
+    if (reinterpret_cast<uintptr_t>(pl.data) % unit != 0) return fail(AICAS_ERR_INVALID, "a plane must be aligned to %lld bytes", (long long)unit);
+    for (int64_t s : st)
+      if (s < 0 || s % unit != 0 || s >= ((int64_t)1 << 41))
+        return fail(AICAS_ERR_INVALID, "plane strides must be non-negative multiples of %lld bytes below 2^41", (long long)unit);
+  }
+  if (p->keep < 1 || p->keep_first < 0 || p->keep_last < 0 || (int64_t)p->keep_first + p->keep_last > p->keep ||
+      p->longer_than < p->keep)
+    return fail(AICAS_ERR_INVALID, "keep=%d keep_first=%d keep_last=%d longer_than=%d: 1 <= keep_first + keep_last <= keep <= "
+                "longer_than is needed", p->keep, p->keep_first, p->keep_last, p->longer_than);
+  const int64_t st[] = {p->w_stride_b, p->w_stride_h, p->wo_stride_b, p->wo_stride_h};
+  for (int64_t s : st)
+    if (s < 0) return fail(AICAS_ERR_INVALID, "strides of the weights must not be negative");
+  if ((int64_t)p->batch * p->num_kv_heads > (1 << 24)) return fail(AICAS_ERR_UNSUPPORTED, "batch=%d of %d heads", p->batch, p->num_kv_heads);
+  if (lengths_overlap(p->kv_lens_out, p->batch, p->page_table, (p->batch - 1) * p->table_stride + p->max_pages) ||
+      (p->kv_lens_out != p->kv_lens && lengths_overlap(p->kv_lens_out, p->batch, p->kv_lens, p->batch)))
+    return fail(AICAS_ERR_INVALID, "kv_lens_out must be kv_lens or share no memory with it, nor with page_table");
+  return AICAS_OK;
+}
+
 int check_linear_int4(const aicas_linear_int4_params* p) {
   if (p == nullptr) return fail(AICAS_ERR_INVALID, "params is NULL");
   if (p->dtype != AICAS_DTYPE_F16 && p->dtype != AICAS_DTYPE_BF16)
@@ -515,7 +716,7 @@ const char* aicas_version(void) { return "aicas_b200 0.2.0 sm_100a abi 2"; }
 uint32_t aicas_capabilities(void) {
   return AICAS_CAP_DECODE | AICAS_CAP_MERGE | AICAS_CAP_ROPE_APPEND | AICAS_CAP_PEER_EXCHANGE |
          AICAS_CAP_DECODE_LINEAR | AICAS_CAP_VISION_ROPE | AICAS_CAP_VISION_QKV | AICAS_CAP_PAGED |
-         AICAS_CAP_LINEAR_INT4 | aicas::fmha_capabilities();
+         AICAS_CAP_LINEAR_INT4 | AICAS_CAP_PAGED_INT4 | AICAS_CAP_PAGED_EVICT | aicas::fmha_capabilities();
 }
 
 const char* aicas_last_error(void) { return g_err; }
@@ -926,6 +1127,47 @@ int aicas_paged_decode_gqa(const aicas_paged_decode_params* p, void* workspace, 
     return fail(AICAS_ERR_INVALID, "workspace must be 256-byte aligned");
   return aicas::run_paged_decode(p, sm_count(), workspace, static_cast<cudaStream_t>(stream), device_error_word(),
                                  g_err, sizeof(g_err));
+}
+
+int aicas_paged_append_int4(const aicas_paged_append_int4_params* p, void* stream) {
+  const int rc = check_paged_append_int4(p);
+  if (rc != AICAS_OK) return rc;
+  return aicas::run_paged_append_int4(p, static_cast<cudaStream_t>(stream), g_err, sizeof(g_err));
+}
+
+int aicas_paged_read_int4(const aicas_paged_read_int4_params* p, void* stream) {
+  const int rc = check_paged_read_int4(p);
+  if (rc != AICAS_OK) return rc;
+  return aicas::run_paged_read_int4(p, static_cast<cudaStream_t>(stream), g_err, sizeof(g_err));
+}
+
+size_t aicas_paged_decode_int4_workspace_bytes(const aicas_paged_decode_int4_params* p) {
+  if (check_paged_decode_int4(p) != AICAS_OK) return 0;
+  return aicas::paged_decode_int4_workspace(sm_count());
+}
+
+int aicas_paged_decode_int4(const aicas_paged_decode_int4_params* p, void* workspace, size_t workspace_bytes, void* stream) {
+  const int rc = check_paged_decode_int4(p);
+  if (rc != AICAS_OK) return rc;
+  const size_t need = aicas::paged_decode_int4_workspace(sm_count());
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(AICAS_ERR_WORKSPACE, "paged 4-bit decode needs %zu bytes of zero-initialised workspace (got %zu)", need,
+                workspace_bytes);
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+    return fail(AICAS_ERR_INVALID, "workspace must be 256-byte aligned");
+  return aicas::run_paged_decode_int4(p, sm_count(), workspace, static_cast<cudaStream_t>(stream), g_err, sizeof(g_err));
+}
+
+int aicas_paged_weights(const aicas_paged_weights_params* p, void* stream) {
+  const int rc = check_paged_weights(p);
+  if (rc != AICAS_OK) return rc;
+  return aicas::run_paged_weights(p, sm_count(), static_cast<cudaStream_t>(stream), g_err, sizeof(g_err));
+}
+
+int aicas_paged_evict(const aicas_paged_evict_params* p, void* stream) {
+  const int rc = check_paged_evict(p);
+  if (rc != AICAS_OK) return rc;
+  return aicas::run_paged_evict(p, static_cast<cudaStream_t>(stream), g_err, sizeof(g_err));
 }
 
 int aicas_linear_int4(const aicas_linear_int4_params* p, void* stream) {

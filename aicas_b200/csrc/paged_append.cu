@@ -15,49 +15,10 @@
 
 #include "common.cuh"
 #include "paged.cuh"
+#include "paged_rows.cuh"
 
 namespace aicas {
 namespace {
-
-template <typename T>
-__device__ __forceinline__ float rounded(float x) {
-  return Elem<T>::to_float(Elem<T>::from_float(x));
-}
-
-// 16 bytes of T from floats, two a conversion.
-template <typename T>
-__device__ __forceinline__ uint4 pack_vec(const float* f) {
-  union {
-    uint4 u;
-    __nv_bfloat162 b[4];
-    __half2 h[4];
-    float f[4];
-  } r;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (std::is_same<T, __nv_bfloat16>::value)
-      r.b[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-    else if constexpr (std::is_same<T, __half>::value)
-      r.h[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-    else
-      r.f[i] = f[i];
-  }
-  return r.u;
-}
-
-// N floats of a cos/sin row.
-template <typename CS, int N>
-__device__ __forceinline__ void load_table(const CS* p, float* f) {
-  constexpr int kV = Elem<CS>::kPerVec;
-  if constexpr (N >= kV) {
-#pragma unroll
-    for (int i = 0; i < N / kV; ++i) Elem<CS>::unpack(reinterpret_cast<const uint4*>(p)[i], f + i * kV);
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = Elem<CS>::to_float(p[i]);
-  }
-}
-
 
 // HBM bound: every row is read and written once (8 prompts of 2048 tokens, 16 + 2 * 8
 // heads of 128: 285 MB in 50 us, 5700 GB/s, 88 % of the measured copy rate).  One CTA
@@ -112,10 +73,10 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendThreads == 32 ? 18 : 1)
     if (!tables) {
       const CS* cp = static_cast<const CS*>(a.cos) + b * a.cs_stride_b + s * a.cs_stride_s + c;
       const CS* sp = static_cast<const CS*>(a.sin) + b * a.cs_stride_b + s * a.cs_stride_s + c;
-      load_table<CS, kV>(cp, c1);
-      load_table<CS, kV>(cp + D / 2, c2);
-      load_table<CS, kV>(sp, s1);
-      load_table<CS, kV>(sp + D / 2, s2);
+      load_floats<CS, kV>(cp, c1);
+      load_floats<CS, kV>(cp + D / 2, c2);
+      load_floats<CS, kV>(sp, s1);
+      load_floats<CS, kV>(sp + D / 2, s2);
       tables = true;
     }
 #pragma unroll
@@ -139,36 +100,17 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendThreads == 32 ? 18 : 1)
         Elem<T>::unpack(u2[j], x2);
         if (w != nullptr) {
           float w1[kV], w2[kV];
-          load_table<T, kV>(w + c, w1);
-          load_table<T, kV>(w + c + D / 2, w2);
+          load_floats<T, kV>(w + c, w1);
+          load_floats<T, kV>(w + c + D / 2, w2);
           float ss = 0.f;
 #pragma unroll
           for (int i = 0; i < kV; ++i) ss += x1[i] * x1[i] + x2[i] * x2[i];
 #pragma unroll
           for (int off = kTpr / 2; off >= 1; off >>= 1) ss += __shfl_xor_sync(row_lanes, ss, off);
           const float inv = rsqrtf(ss / (float)D + a.norm_eps);
-#pragma unroll
-          for (int i = 0; i < kV; ++i) {
-            if (kRoundEach) {
-              x1[i] = rounded<T>(__fmul_rn(w1[i], rounded<T>(__fmul_rn(x1[i], inv))));
-              x2[i] = rounded<T>(__fmul_rn(w2[i], rounded<T>(__fmul_rn(x2[i], inv))));
-            } else {
-              x1[i] *= inv * w1[i];
-              x2[i] *= inv * w2[i];
-            }
-          }
+          normed_pair<T, kRoundEach, kV>(x1, x2, w1, w2, inv);
         }
-#pragma unroll
-        for (int i = 0; i < kV; ++i) {
-          const float p1 = x1[i], p2 = x2[i];
-          if (kRoundEach) {
-            x1[i] = __fadd_rn(rounded<T>(__fmul_rn(p1, c1[i])), rounded<T>(__fmul_rn(-p2, s1[i])));
-            x2[i] = __fadd_rn(rounded<T>(__fmul_rn(p2, c2[i])), rounded<T>(__fmul_rn(p1, s2[i])));
-          } else {
-            x1[i] = p1 * c1[i] - p2 * s1[i];
-            x2[i] = p2 * c2[i] + p1 * s2[i];
-          }
-        }
+        rotated_pair<T, kRoundEach, kV>(x1, x2, c1, c2, s1, s2);
         u1[j] = pack_vec<T>(x1);
         u2[j] = pack_vec<T>(x2);
       }

@@ -108,7 +108,26 @@ def paged_rope_kv_append(
     what = "paged_rope_kv_append"
     (B, Hq, S, D), shape, ks, vs, page_table, max_pages, table_stride = _check_pool(what, query, k_pages, v_pages,
                                                                                     page_table)
-    device, dtype, Hkv = query.device, query.dtype, shape[1]
+    device, Hkv = query.device, shape[1]
+    rows, steps_of_rows, per_request, dtypes, pos, q_out, _held = _new_rows(
+        what, query, key, value, cos, sin, Hkv, positions, num_new, q_out, kv_lens_out, q_norm_weight, k_norm_weight)
+    if B == 0 or S == 0:
+        if kv_lens_out is not None and B:
+            kv_lens_out.copy_(pos.clamp(0, max_pages * shape[2]))
+        return q_out
+    launch(device, "aicas_paged_rope_append", nat.PACK_PAGED_APPEND.pack(
+        *rows, k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), *per_request, *steps_of_rows,
+        ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], table_stride,
+        B, Hq, Hkv, S, D, shape[0], shape[2], max_pages, *dtypes, eps))
+    return q_out
+
+
+def _new_rows(what: str, query, key, value, cos, sin, Hkv, positions, num_new, q_out, kv_lens_out, q_norm_weight,
+              k_norm_weight):
+    """What the appends check and pack beside the pages: the rows' addresses (q, q_out,
+    k, v, cos, sin), their strides, the per-request vectors' and the norm weights'
+    addresses, the dtype codes, the positions, q_out, and what has to live until the launch."""
+    (B, Hq, S, D), device, dtype = query.shape, query.device, query.dtype
     if key.shape != (B, Hkv, S, D) or value.shape != (B, Hkv, S, D):
         raise ValueError(f"{what}: key and value must be [{B}, {Hkv}, {S}, {D}]")
     if Hkv == 0 or Hq % Hkv:
@@ -148,18 +167,10 @@ def paged_rope_kv_append(
         qo = steps(q_out)
         if q_out.shape != (B, Hq, S, D) or q_out.dtype != dtype or q_out.device != device or qo[3] != 1:
             raise ValueError(f"{what}: q_out must be [{B}, {Hq}, {S}, {D}] with a unit-stride head_dim")
-    if B == 0 or S == 0:
-        if kv_lens_out is not None and B:
-            kv_lens_out.copy_(pos.clamp(0, max_pages * shape[2]))
-        return q_out
-    launch(device, "aicas_paged_rope_append", nat.PACK_PAGED_APPEND.pack(
-        query.data_ptr(), q_out.data_ptr(), key.data_ptr(), value.data_ptr(), cos.data_ptr(), sin.data_ptr(),
-        k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), pos.data_ptr(), pointer(new),
-        pointer(kv_lens_out), pointer(q_norm_weight), pointer(k_norm_weight),
-        qi[0], qi[1], qi[2], qo[0], qo[1], qo[2], ki[0], ki[1], ki[2], vi[0], vi[1], vi[2],
-        cs[0] if cs_shape[0] == B else 0, cs[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], table_stride,
-        B, Hq, Hkv, S, D, shape[0], shape[2], max_pages, _DTYPE_CODES[dtype], _DTYPE_CODES[cs_dtype], eps))
-    return q_out
+    return ((query.data_ptr(), q_out.data_ptr(), key.data_ptr(), value.data_ptr(), cos.data_ptr(), sin.data_ptr()),
+            (*qi[:3], *qo[:3], *ki[:3], *vi[:3], cs[0] if cs_shape[0] == B else 0, cs[1]),
+            (pos.data_ptr(), pointer(new), pointer(kv_lens_out), pointer(q_norm_weight), pointer(k_norm_weight)),
+            (_DTYPE_CODES[dtype], _DTYPE_CODES[cs_dtype]), pos, q_out, (query, key, value, cos, sin, new))
 
 
 def paged_gqa_decode_attention(
@@ -222,10 +233,15 @@ class PagedKVCache:
     :meth:`page_table` writes their rows for the kernels.  Released pages keep
     what they held: a kernel reads only the slots under the lengths it is given.
     Work that reads a released page and is already on a stream must be ordered
-    before the work that writes its next holder's tokens (one stream does)."""
+    before the work that writes its next holder's tokens (one stream does).
+
+    With ``int4_group_size`` (64, or the head dim of 64 or 128) the pools are
+    :class:`aicas_b200.Int4Pages`, a quarter of the bytes and their scales, for
+    :func:`aicas_b200.paged_rope_kv_append_int4` and
+    :func:`aicas_b200.paged_gqa_decode_attention_int4`."""
 
     def __init__(self, num_layers: int, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, *,
-                 dtype: torch.dtype, device: torch.device | str):
+                 dtype: torch.dtype, device: torch.device | str, int4_group_size: int | None = None):
         if min(num_layers, num_pages, num_kv_heads) < 1:
             raise ValueError("PagedKVCache needs a positive number of layers, pages and heads")
         if page_size < 8 or page_size % 8:
@@ -234,8 +250,15 @@ class PagedKVCache:
             raise ValueError(f"PagedKVCache: dtype {dtype}, head_dim {head_dim} are not ones that the kernels take")
         shape = (num_pages, num_kv_heads, page_size, head_dim)
         self.page_size, self.num_pages = page_size, num_pages
-        self.keys = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(num_layers)]
-        self.values = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(num_layers)]
+        self.device, self.int4_group_size = torch.device(device), int4_group_size
+        if int4_group_size is None:
+            pool = lambda: torch.zeros(shape, dtype=dtype, device=device)  # noqa: E731
+        else:
+            from .paged_int4 import int4_pages
+
+            pool = lambda: int4_pages(*shape, int4_group_size, dtype=dtype, device=device)  # noqa: E731
+        self.keys = [pool() for _ in range(num_layers)]
+        self.values = [pool() for _ in range(num_layers)]
         self._free = list(range(num_pages - 1, -1, -1))  # the lowest page goes out first
         self._held: dict[int, list[int]] = {}
         self._next = 0
@@ -274,6 +297,16 @@ class PagedKVCache:
         for _ in range(need):
             self._held[request].append(self._free.pop())
 
+    def shrink(self, request: int, tokens: int) -> None:
+        """Takes back the pages of ``request`` that its first ``tokens`` tokens do not
+        need (after :func:`aicas_b200.paged_kv_evict`); never gives it any."""
+        if tokens < 0:
+            raise ValueError("tokens must not be negative")
+        self.pages(request)
+        held, need = self._held[request], -(-tokens // self.page_size)
+        self._free.extend(reversed(held[need:]))
+        del held[need:]
+
     def release(self, request: int) -> None:
         """Takes all pages of ``request`` back."""
         self.pages(request)
@@ -288,20 +321,31 @@ class PagedKVCache:
             raise ValueError(f"page_table: a request holds more than max_pages = {width} pages")
         width = max(width, 1)
         table = torch.tensor([r + [-1] * (width - len(r)) for r in rows], dtype=torch.int32).view(len(rows), width)
-        return table.to(self.keys[0].device)
+        return table.to(self.device)
 
     def store(self, layer: int, request: int, key: torch.Tensor, value: torch.Tensor) -> None:
         """Copies rotated keys and values ``[Hkv, S, D]`` (a prompt's, from another
-        cache) to the first S slots of ``request``: a set-up step, in plain copies."""
+        cache) to the first S slots of ``request`` (rounded first where the pools are of
+        4 bits): a set-up step, in plain copies."""
         S, held = key.shape[1], self.pages(request)
         if S > len(held) * self.page_size:
             raise ValueError(f"store: {S} tokens do not fit the {len(held)} pages of request {request}")
         for pool, rows in ((self.keys[layer], key), (self.values[layer], value)):
-            if rows.shape != (pool.shape[1], S, pool.shape[3]) or rows.dtype != pool.dtype:
-                raise ValueError(f"store: keys and values must be [{pool.shape[1]}, {S}, {pool.shape[3]}] {pool.dtype}")
+            if self.int4_group_size is None:
+                shape, dtype, parts = pool.shape, pool.dtype, [(pool, rows)]
+            else:
+                from .paged_int4 import quantize_kv_int4
+
+                shape, dtype = (*pool.codes.shape[:3], pool.codes.shape[3] * 2), pool.scales.dtype
+                parts = None
+            if rows.shape != (shape[1], S, shape[3]) or rows.dtype != dtype:
+                raise ValueError(f"store: keys and values must be [{shape[1]}, {S}, {shape[3]}] {dtype}")
+            if parts is None:
+                parts = list(zip(pool, quantize_kv_int4(rows, self.int4_group_size)))
             full, rest = divmod(S, self.page_size)
-            if full:
-                where = torch.tensor(held[:full], device=pool.device)
-                pool[where] = rows[:, :S - rest].reshape(pool.shape[1], full, self.page_size, -1).transpose(0, 1)
-            if rest:
-                pool[held[full], :, :rest] = rows[:, S - rest:]
+            for into, part in parts:
+                if full:
+                    where = torch.tensor(held[:full], device=into.device)
+                    into[where] = part[:, :S - rest].unflatten(1, (full, self.page_size)).transpose(0, 1)
+                if rest:
+                    into[held[full], :, :rest] = part[:, S - rest:]

@@ -59,6 +59,11 @@
  *
  *   aicas_paged_rope_append   aicas_rope_kv_append into a paged cache
  *   aicas_paged_decode_gqa    aicas_decode_gqa over a paged cache
+ *   aicas_paged_append_int4   aicas_paged_rope_append into a paged cache of 4-bit rows
+ *   aicas_paged_read_int4     rows of such a cache as 16-bit values
+ *   aicas_paged_decode_int4   aicas_paged_decode_gqa over such a cache
+ *   aicas_paged_weights       what attention gave to each cached slot, added up
+ *   aicas_paged_evict         cuts caches to their slots of the largest weights
  *   aicas_linear_int4         aicas_decode_linear with 4-bit weights
  *
  * Layout conventions: attention tensors are 4-D [batch, heads, tokens, head_dim]
@@ -476,6 +481,155 @@ AICAS_API int aicas_paged_decode_gqa(const aicas_paged_decode_params* p, void* w
                                      void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Paged KV cache in 4 bits: a row of D = 64 or 128 elements is D / 2 bytes of  */
+/* codes 0..15 (even d in the low half of a byte) and, for each group of        */
+/* group_size elements (64, or all D), a pair (scale, least) of the 16-bit type */
+/* of the calls' tensors: element d stands for scale * code[d] + least.         */
+/* ------------------------------------------------------------------------ */
+typedef struct aicas_int4_pages {
+  void* codes;              /* uint8 [P, Hkv, page_size, D / 2] */
+  void* scales;             /* dtype [P, Hkv, page_size, D / group_size, 2], a row's pairs contiguous */
+  int64_t cs_p, cs_h, cs_t; /* codes, in bytes: page, head, row (multiples of 16) */
+  int64_t ss_p, ss_h, ss_t; /* scales, in elements: page, head, row (multiples of 2 * D / group_size) */
+} aicas_int4_pages;
+
+typedef struct aicas_paged_append_int4_params {
+  const void* q_in;         /* as in aicas_paged_append_params, but for the pages */
+  void* q_out;
+  const void* k_in;
+  const void* v_in;
+  const void* cos;
+  const void* sin;
+  aicas_int4_pages kv[2];   /* keys, values */
+  const int32_t* page_table;
+  const int32_t* positions;
+  const int32_t* num_new;
+  int32_t* kv_lens_out;
+  const void* q_norm_weight;
+  const void* k_norm_weight;
+  int64_t qi_stride_b, qi_stride_h, qi_stride_s;
+  int64_t qo_stride_b, qo_stride_h, qo_stride_s;
+  int64_t k_stride_b, k_stride_h, k_stride_s;
+  int64_t v_stride_b, v_stride_h, v_stride_s;
+  int64_t cs_stride_b, cs_stride_s;
+  int64_t table_stride;
+  int32_t batch, num_q_heads, num_kv_heads, seq_len, head_dim, group_size;
+  int32_t num_pages, page_size, max_pages;
+  int32_t dtype;            /* fp16 or bf16 */
+  int32_t cs_dtype;         /* fp32, or the tensors' type with aicas_paged_append_params' rounding */
+  float norm_eps;
+} aicas_paged_append_int4_params;
+
+/* aicas_paged_rope_append with rounded rows: of a group's values (keys after norm and
+   rotation) least = their least and scale = (their largest - least) / 15, each rounded to
+   dtype, code = (value - least) / scale to the nearest of 0..15 (0 where scale is 0).  A
+   group with a value that is not finite, or a range past fp32's, has scale and least NaN. */
+AICAS_API int aicas_paged_append_int4(const aicas_paged_append_int4_params* p, void* stream);
+
+typedef struct aicas_paged_read_int4_params {
+  aicas_int4_pages kv[2];
+  void* out[2];             /* [B, Hkv, S, D] keys, values of dtype */
+  const int32_t* page_table;
+  const int32_t* positions; /* [B] first slot read per request */
+  const int32_t* num_tokens; /* optional [B]: how many of the S rows are read; NULL = S */
+  int64_t out_stride_b, out_stride_h, out_stride_s; /* of both outputs */
+  int64_t table_stride;
+  int32_t batch, num_kv_heads, seq_len, head_dim, group_size;
+  int32_t num_pages, page_size, max_pages;
+  int32_t dtype;
+} aicas_paged_read_int4_params;
+
+/* Row s of request b is slot positions[b] + s; rows past num_tokens[b], slots outside the
+   table and pages outside the pool read as zeros. */
+AICAS_API int aicas_paged_read_int4(const aicas_paged_read_int4_params* p, void* stream);
+
+typedef struct aicas_paged_decode_int4_params {
+  const void* q;            /* as in aicas_paged_decode_params, but for the pages */
+  aicas_int4_pages kv[2];
+  void* out;
+  float* lse;
+  const int32_t* page_table;
+  const int32_t* kv_lens;
+  const int32_t* kv_starts;
+  int64_t q_stride_b, q_stride_h;
+  int64_t o_stride_b, o_stride_h;
+  int64_t table_stride;
+  int32_t batch, num_q_heads, num_kv_heads, head_dim, group_size;
+  int32_t num_pages, page_size, max_pages;
+  int32_t dtype;
+  float sm_scale;
+} aicas_paged_decode_int4_params;
+
+/* The rules of aicas_paged_decode_gqa, workspace included (the same buffer serves both). */
+AICAS_API size_t aicas_paged_decode_int4_workspace_bytes(const aicas_paged_decode_int4_params* p);
+AICAS_API int aicas_paged_decode_int4(const aicas_paged_decode_int4_params* p, void* workspace, size_t workspace_bytes,
+                                      void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Eviction from a paged cache by attention weight.                            */
+/* ------------------------------------------------------------------------ */
+typedef struct aicas_paged_weights_params {
+  const void* q;            /* [B, Hq, S, D]: query s of request b is the token at slot kv_lens[b] - S + s */
+  const void* k_pages;      /* 16-bit [P, Hkv, page_size, D], or the codes of 4-bit pages */
+  const void* k_scales;     /* scales of 4-bit pages; NULL: 16-bit (or fp32) pages */
+  const float* lse;         /* [B, Hq, S] base-2 log-sum-exp of each query's attention (-inf: it saw nothing) */
+  float* weights;           /* [B, Hkv, C], C >= max_pages * page_size: added to */
+  const int32_t* page_table;
+  const int32_t* kv_lens;   /* optional [B], NULL = capacity */
+  const int32_t* kv_starts; /* optional [B], NULL = 0 */
+  int64_t q_stride_b, q_stride_h, q_stride_s;
+  int64_t lse_stride_b, lse_stride_h, lse_stride_s;
+  int64_t w_stride_b, w_stride_h;
+  int64_t kp_stride_p, kp_stride_h, kp_stride_t; /* elements of the pages (bytes of 4-bit codes) */
+  int64_t ks_stride_p, ks_stride_h, ks_stride_t; /* elements of the scales */
+  int64_t table_stride;
+  int32_t batch, num_q_heads, num_kv_heads, seq_len, head_dim;
+  int32_t group_size;       /* of 4-bit pages; 0: pages of the dtype of q */
+  int32_t num_pages, page_size, max_pages;
+  int32_t dtype;
+  float sm_scale;
+} aicas_paged_weights_params;
+
+/* weights[b, h, t] += sum over the queries (s, j) of head h that see slot t, slots
+   kv_starts[b] <= t <= kv_lens[b] - S + s, of 2^(sm_scale log2(e) q[b, j, s].k[b, h, t] - lse[b, j, s]). */
+AICAS_API int aicas_paged_weights(const aicas_paged_weights_params* p, void* stream);
+
+typedef struct aicas_evict_plane {
+  void* data;               /* [P, Hkv, page_size] rows of row_bytes bytes */
+  int64_t stride_p, stride_h, stride_t; /* in bytes */
+  int64_t row_bytes;        /* 4, 8 or a multiple of 16 up to 512; data and strides are multiples of it or of 16 */
+} aicas_evict_plane;
+
+#define AICAS_EVICT_MAX_PLANES 4
+
+typedef struct aicas_paged_evict_params {
+  aicas_evict_plane plane[AICAS_EVICT_MAX_PLANES]; /* what a slot has: keys, values, their scales */
+  const float* weights;     /* [B, Hkv, C], C >= max_pages * page_size */
+  float* weights_out;       /* the same shape; may be weights */
+  int32_t* kept;            /* [B, Hkv, keep], contiguous */
+  const int32_t* page_table;
+  const int32_t* kv_lens;   /* [B], clamped to 0..capacity */
+  int32_t* kv_lens_out;     /* optional [B]; may be kv_lens */
+  int64_t w_stride_b, w_stride_h;
+  int64_t wo_stride_b, wo_stride_h;
+  int64_t table_stride;
+  int32_t num_planes;
+  int32_t batch, num_kv_heads;
+  int32_t num_pages, page_size, max_pages;
+  int32_t keep;             /* slots that a cut cache has left */
+  int32_t keep_first, keep_last; /* of them the first and the last of the cache, whatever their weights */
+  int32_t longer_than;      /* caches of at most so many slots are left as they are (>= keep) */
+} aicas_paged_evict_params;
+
+/* For each (request, KV head) with more than longer_than slots: the first keep_first slots, the
+   last keep_last and, of those between, the ones of the largest weights (the lower slot where two
+   are equal; NaN counts as less than all numbers) move to slots 0 .. keep - 1 in their order, with
+   their weights; the weights of the slots behind become 0.  kept[b, h, i] is the slot that became i;
+   in a cache that is not cut, i, and -1 past its length.  Rows behind the kept ones stay as they
+   were.  A page is in one place of one request's row of the table. */
+AICAS_API int aicas_paged_evict(const aicas_paged_evict_params* p, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Decode-side products with 4-bit weights:                                   */
 /*   W[n, k] = scales[n, k / g] * (q[n, k] - zeros[n, k / g]),  q in 0..15.     */
 /* ------------------------------------------------------------------------ */
@@ -526,6 +680,8 @@ AICAS_API const char* aicas_version(void);
 #define AICAS_CAP_VISION_QKV 256u
 #define AICAS_CAP_PAGED 512u
 #define AICAS_CAP_LINEAR_INT4 1024u
+#define AICAS_CAP_PAGED_INT4 2048u
+#define AICAS_CAP_PAGED_EVICT 4096u
 AICAS_API uint32_t aicas_capabilities(void);
 
 /* Message of the last failed call on this thread ("" if none). */
