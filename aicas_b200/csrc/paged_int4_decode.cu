@@ -3,106 +3,691 @@
 //   o = softmax(scale * q K^T) V over the slots [start, len) of a request,
 //   lse = log2(sum_j 2^(scale log2(e) q.k_j)).
 //
-// One CTA a (request, KV head, block of up to 8 query heads), a slot a warp at a time.
+// A row is a quarter of a 16-bit one and its products are as many, so what has to be kept
+// low beside the bytes is the work on a code.  The codes enter mma.sync as they are:
+//   q.k_t = sk_t (q.ck_t) + lk_t (sum q),   sum_t p_t v_t = sum_t (p_t sv_t) cv_t + sum_t p_t lv_t,
+// so a code costs a mask (and half a shift): the 4 bits in the low end of an fp16 are the
+// subnormal number code * 2^-24, 4 bits further up code * 2^-20, both exact, as are their
+// products in the fp32 accumulators.  The 1 / 16 of the latter is taken on the other operand
+// (q) or at the end (o).  Scales and least values act on a score or a probability, not on an
+// element.
+//
+//   * Work: paged_split.cuh's equal ranges of tiles of 32 slots, one CTA an SM; partials of a
+//     pair cut by ranges are joined by the last CTA to arrive, in CTA order, so results
+//     repeat to the bit.
+//   * Copies: each warp streams its tiles with 16-byte cp.async into a ring of its own,
+//     rows swizzled so that the fragment loads below meet no bank twice.  A row is 64
+//     bytes (D = 128) and a page may be 8 rows, too small for a tensor copy each.
+//   * Products: m16n8k16 with K (16 slots) and V^T (16 dims) as the 16-row operand and the
+//     heads as the 8 columns; a probability moves from the scores' accumulator layout to
+//     the operand layout by a transposing 8 x 8 move in registers.
+//   * Rounding: a 16-bit q is exact in one fp16 after scaling by a power of two a head (down
+//     to 2^-29 of its largest element).  A probability times its scale enters P V as two
+//     fp16 parts (22 bits; down to 2^-37 of the largest), scaled by a power of two that
+//     follows the largest scale.  Everything else is fp32.
+//   * Slots out of range: score -inf, V's scale and least 0.
 #include <cstdio>
 #include <cstring>
+#include <type_traits>
 
 #include "common.cuh"
 #include "paged_int4.cuh"
+#include "paged_split.cuh"
 
 namespace aicas {
 namespace {
 
-constexpr int kWarps = 8, kHeads = 8;
+constexpr int kTile = 32;      // slots a tile
+constexpr int kPairCost = 3;   // what beginning and ending a pair costs a CTA, in tiles
+constexpr int kMinChunk = 16;  // fewest tiles a CTA takes
+constexpr int kSmallTiles = 16;  // most tiles a CTA of a launch that gives pairs whole CTAs
+constexpr int kHeads = 8;      // query heads of a block
+constexpr size_t kWsCounters = (size_t)1 << 20;  // counter region shared with the other decode kernels
+constexpr float kCodeUnit = 16777216.f;  // 2^24: a code in an fp16's low bits is code / kCodeUnit
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kWarps * 32) paged_decode_int4_kernel(const __grid_constant__ aicas_paged_decode_int4_params a) {
-  constexpr int kE = D / 32;  // elements a lane
-  __shared__ float red[kWarps][kHeads][D + 2];
-  const int group = a.num_q_heads / a.num_kv_heads, blocks = (group + kHeads - 1) / kHeads;
-  const int blk = blockIdx.x % blocks, kvh = blockIdx.x / blocks % a.num_kv_heads, b = blockIdx.x / blocks / a.num_kv_heads;
-  const int h0 = kvh * group + blk * kHeads, heads = min(kHeads, group - blk * kHeads);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, d0 = lane * kE;
-  grid_launch_dependents();
-  grid_dependency_wait();
-  const int cap = a.max_pages * a.page_size;
-  const int len = a.kv_lens != nullptr ? min(max(a.kv_lens[b], 0), cap) : cap;
-  const int start = a.kv_starts != nullptr ? max(a.kv_starts[b], 0) : 0;
-  const float c = a.sm_scale * 1.4426950408889634f;
-  float q[kHeads][kE], o[kHeads][kE], m[kHeads], l[kHeads];
-#pragma unroll
-  for (int h = 0; h < kHeads; ++h) {
-    m[h] = -INFINITY, l[h] = 0.f;
-#pragma unroll
-    for (int e = 0; e < kE; ++e) {
-      o[h][e] = 0.f;
-      q[h][e] = h < heads ? Elem<T>::to_float(static_cast<const T*>(a.q)[b * a.q_stride_b + (h0 + h) * a.q_stride_h + d0 + e]) : 0.f;
-    }
-  }
-  for (int t = start + warp; t < len; t += kWarps) {
-    const int i = t / a.page_size, row = t - i * a.page_size, page = a.page_table[b * a.table_stride + i];
-    float kv[2][kE] = {};
-    if (page >= 0 && page < a.num_pages) {
-#pragma unroll
-      for (int side = 0; side < 2; ++side) {
-        const aicas_int4_pages& p = a.kv[side];
-        const uint8_t* codes = static_cast<const uint8_t*>(p.codes) + page * p.cs_p + kvh * p.cs_h + row * p.cs_t;
-        const T* pair = static_cast<const T*>(p.scales) + page * p.ss_p + kvh * p.ss_h + row * p.ss_t + d0 / a.group_size * 2;
-        const float s = Elem<T>::to_float(pair[0]), least = Elem<T>::to_float(pair[1]);
-#pragma unroll
-        for (int e = 0; e < kE; ++e) kv[side][e] = fmaf(s, (float)(codes[(d0 + e) / 2] >> (4 * ((d0 + e) & 1)) & 15), least);
-      }
-    }
-#pragma unroll
-    for (int h = 0; h < kHeads; ++h) {
-      float s = 0.f;
-#pragma unroll
-      for (int e = 0; e < kE; ++e) s = fmaf(q[h][e], kv[0][e], s);
-#pragma unroll
-      for (int off = 16; off >= 1; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-      s *= c;
-      const float mn = fmaxf(m[h], s), use = mn == -INFINITY ? 0.f : mn;
-      const float alpha = exp2f(m[h] - use), p = exp2f(s - use);
-      m[h] = mn, l[h] = fmaf(l[h], alpha, p);
-#pragma unroll
-      for (int e = 0; e < kE; ++e) o[h][e] = fmaf(o[h][e], alpha, p * kv[1][e]);
-    }
-  }
-#pragma unroll
-  for (int h = 0; h < kHeads; ++h) {
-#pragma unroll
-    for (int e = 0; e < kE; ++e) red[warp][h][d0 + e] = o[h][e];
-    if (lane == 0) red[warp][h][D] = m[h], red[warp][h][D + 1] = l[h];
-  }
-  __syncthreads();
-  for (int x = threadIdx.x; x < heads * D; x += kWarps * 32) {
-    const int h = x / D, d = x % D;
-    float M = -INFINITY, L = 0.f, O = 0.f;
-    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, red[w][h][D]);
-    const float use = M == -INFINITY ? 0.f : M;
-    for (int w = 0; w < kWarps; ++w) {
-      const float f = exp2f(red[w][h][D] - use);
-      L = fmaf(f, red[w][h][D + 1], L), O = fmaf(f, red[w][h][d], O);
-    }
-    static_cast<T*>(a.out)[b * a.o_stride_b + (h0 + h) * a.o_stride_h + d] = Elem<T>::from_float(L == 0.f ? 0.f : O / L);
-    if (a.lse != nullptr && d == 0) a.lse[(int64_t)b * a.num_q_heads + h0 + h] = L == 0.f ? -INFINITY : M + log2f(L);
+struct Int4Args {
+  aicas_int4_pages kv[2];
+  const void* q;
+  void* out;
+  float* lse;
+  const int32_t* table;
+  const int32_t* lens;
+  const int32_t* starts;
+  int64_t q_sb, q_sh, o_sb, o_sh, table_stride;
+  int batch, hq, hkv, group, row_blocks;
+  int num_pages, cap;
+  int octets;              // of 8 rows a page has
+  uint32_t octets_mul;     // n / octets = (umulhi(n, octets_mul) + n) >> octets_shift
+  int octets_shift;
+  int few;                 // at most half as many pairs as CTAs
+  float scale_log2;
+  float* ws_o;             // [2 * grid][kHeads][D]
+  float* ws_ml;            // [2 * grid][kHeads][2]
+  unsigned int* ws_count;  // [grid]
+};
+
+template <int D, int GD>
+struct Int4Cfg {
+  static constexpr int kRow = D / 2;          // bytes of a row's codes
+  static constexpr int kChunks = kRow / 16;   // its 16-byte chunks
+  static constexpr int kPair = 4 * GD;        // bytes of a row's pairs
+  static constexpr int kOffV = kTile * kRow;
+  static constexpr int kOffKs = 2 * kTile * kRow, kOffVs = kOffKs + kTile * kPair;
+  static constexpr int kStage = kOffVs + kTile * kPair;
+  static constexpr int kWarps = 16, kThreads = kWarps * 32;
+  static constexpr int kStages = GD == 1 ? 3 : 2;
+  static constexpr int kRedHeads = 2;         // heads that the warps' states are joined of at a time
+  static constexpr int kRedRow = D + 4;
+  static constexpr int kOffRed = kWarps * kStages * kStage;
+  static constexpr int kOffVars = kOffRed + kWarps * kRedHeads * kRedRow * 4;
+  static constexpr int kSmem = kOffVars + 16;
+  static_assert(kSmem <= 232448, "shared memory");
+};
+
+using Seg = Segment<kTile, kPairCost>;
+
+// The 16-byte chunk where chunk c of row r is kept.  K's fragments take the same chunk of 8
+// rows, V's half of the chunks of 4 rows: both meet all banks once.
+template <int D>
+__device__ __forceinline__ int swizzled(int r, int c) {
+  if constexpr (D == 128) {
+    const int p = (r >> 1) & 3;  // 0, 1, 2, 3 -> 0, 2, 1, 3
+    return c ^ ((p >> 1) | ((p & 1) << 1));
+  } else {
+    return c ^ ((r >> 2) & 1);
   }
 }
 
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool there) {
+  if constexpr (BYTES == 16) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+  } else {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(there ? BYTES : 0)
+                 : "memory");
+  }
+}
+
+__device__ __forceinline__ void mma(float c[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t pack_half(float x, float y) {
+  union {
+    __half2 h;
+    uint32_t u;
+  } r;
+  r.h = __floats2half2_rn(x, y);
+  return r.u;
+}
+
+// hi = fp16(x), lo = fp16(x - hi) of two numbers: hi's and lo's packed.
+__device__ __forceinline__ void split_half(float x, float y, uint32_t& hi, uint32_t& lo) {
+  union {
+    __half2 h;
+    uint32_t u;
+  } r;
+  r.h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(r.h);
+  hi = r.u;
+  lo = pack_half(x - f.x, y - f.y);
+}
+
 template <typename T>
-cudaError_t launch_decode_int4(const aicas_paged_decode_int4_params& p, cudaStream_t st) {
-  const int blocks = (p.num_q_heads / p.num_kv_heads + kHeads - 1) / kHeads;
-  const dim3 grid((unsigned)(p.batch * p.num_kv_heads * blocks)), block(kWarps * 32);
-  return p.head_dim == 64 ? launch_pdl(paged_decode_int4_kernel<T, 64>, grid, block, 0, st, p)
-                          : launch_pdl(paged_decode_int4_kernel<T, 128>, grid, block, 0, st, p);
+__device__ __forceinline__ float2 pair_of(uint32_t u) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+  } else {
+    return __half22float2(*reinterpret_cast<const __half2*>(&u));
+  }
+}
+
+// ------------------------------------------------------------------ copies
+
+// A warp's way through its tiles, ahead of the products.
+template <int D, int GD>
+struct Cursor {
+  using C = Int4Cfg<D, GD>;
+  Seg seg;
+  int t;      // its next tile, in seg
+  int turn;   // the warp that takes seg's first tile
+  bool more;
+  int page;   // page number and octet of the lane's 8 rows of that tile
+  int octet;
+
+  __device__ __forceinline__ void look(const Int4Args& a) {
+    const int lane = threadIdx.x & 31;
+    page = -1;
+    if (!more) return;
+    const int n = (seg.first_tile + t) * (kTile / 8) + (lane >> 3);
+    const int i = (int)((__umulhi((uint32_t)n, a.octets_mul) + (uint32_t)n) >> a.octets_shift);
+    octet = n - i * a.octets;
+    if (8 * n < seg.len && 8 * n + 8 > seg.start) page = a.table[seg.b * a.table_stride + i];
+  }
+
+  // To the warp's first tile at or after the segment.
+  __device__ __forceinline__ void settle(const Int4Args& a, int warp) {
+    for (;;) {
+      t = seg.t0 + ((warp - turn) & (C::kWarps - 1));
+      if (t < seg.t1) break;
+      turn = (turn + seg.t1 - seg.t0) & (C::kWarps - 1);
+      if (!seg.next(a)) {
+        more = false;
+        break;
+      }
+    }
+  }
+
+  __device__ __forceinline__ void begin(const Int4Args& a, const Seg& first, int warp) {
+    seg = first, turn = 0, more = true;
+    settle(a, warp);
+    look(a);
+  }
+
+  // Asks for the tile and goes on to the next one.
+  __device__ __forceinline__ void copy(const Int4Args& a, uint32_t stage, int warp) {
+    if (more) {
+      const int lane = threadIdx.x & 31, o = lane >> 3, sub = lane & 7;
+      const int head = seg.pair / a.row_blocks;
+      const bool there = page >= 0 && page < a.num_pages;
+      const int64_t pg = there ? page : 0;
+      constexpr int kAtOnce = 8 / C::kChunks;  // rows of an octet in one go
+      const int r = sub / C::kChunks, c = sub % C::kChunks;
+#pragma unroll
+      for (int side = 0; side < 2; ++side) {
+        const aicas_int4_pages& p = a.kv[side];
+        const uint8_t* codes = static_cast<const uint8_t*>(p.codes) + pg * p.cs_p + head * p.cs_h + (int64_t)(8 * octet + r) * p.cs_t + 16 * c;
+        const uint32_t dst = stage + side * C::kOffV + (8 * o + r) * C::kRow;
+#pragma unroll
+        for (int k = 0; k < C::kChunks; ++k)
+          copy_async<16>(dst + kAtOnce * k * C::kRow + 16 * swizzled<D>(r + kAtOnce * k, c), codes + (int64_t)kAtOnce * k * p.cs_t, there);
+        const uint16_t* pair = static_cast<const uint16_t*>(p.scales) + pg * p.ss_p + head * p.ss_h + (int64_t)(8 * octet + sub) * p.ss_t;
+        copy_async<C::kPair>(stage + (side ? C::kOffVs : C::kOffKs) + lane * C::kPair, pair, there);
+      }
+      t += C::kWarps;
+      if (t >= seg.t1) {
+        turn = (turn + seg.t1 - seg.t0) & (C::kWarps - 1);
+        more = seg.next(a);
+        if (more) settle(a, warp);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    look(a);
+  }
+};
+
+// ------------------------------------------------------------------ a warp's state
+
+// WIDE: up to 8 heads, a column each, lo parts in products of their own; else up to 4
+// heads, head j's hi and lo parts in columns 2 j and 2 j + 1 of the same products.
+// A lane's heads: WIDE 2 i and 2 i + 1, else i; slots (rows g and g + 8 of a product) of
+// 16 are g / 2 + 4 (g % 2) and 8 more, an order that lets V's loads meet no bank twice.
+template <typename T, int D, int GD, bool WIDE>
+struct Int4State {
+  using C = Int4Cfg<D, GD>;
+  static constexpr int kN = WIDE ? 2 : 1;  // heads a lane
+  uint32_t q[D / 32][4];  // the lane's 8 dims of each 32, as (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16
+  float fq[kN], qs[kN][GD];  // of the lane's heads: factor of q.code, sum of q, both with the softmax's scale
+  float o[D / 16][4];
+  float m[kN], l[kN], z[kN][GD];
+  float lift;             // power of two on scales of V; 0: none seen yet
+
+  __device__ __forceinline__ void begin(const Int4Args& a, const Seg& s) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3;
+    const int kvh = s.pair / a.row_blocks, h0 = (s.pair - kvh * a.row_blocks) * kHeads;
+    const int heads = min(kHeads, a.group - h0);
+    const int col = WIDE ? g : g >> 1;  // the head of column g
+    float x[D / 32][8], top = 0.f, sum[GD] = {};
+    const T* src = static_cast<const T*>(a.q) + s.b * a.q_sb + (int64_t)(kvh * a.group + h0 + min(col, heads - 1)) * a.q_sh + 8 * i;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+      Elem<T>::unpack(*reinterpret_cast<const uint4*>(src + 32 * c), x[c]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        top = fmaxf(top, fabsf(x[c][e]));
+        sum[c * GD / (D / 32)] += x[c][e];
+      }
+    }
+#pragma unroll
+    for (int off = 1; off < 4; off <<= 1) {
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+#pragma unroll
+      for (int e = 0; e < GD; ++e) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], off);
+    }
+    // top in [2^14, 2^15) after scaling: with an exponent E, times 2^(14 - E)
+    const int E = (int)(__float_as_uint(top) >> 23) - 127;
+    const bool plain = top > 0.f && E < 128 && E > -100;  // else 0, infinite, NaN, or so small that it may be lost
+    const int up = plain ? 14 - E : 0;
+    const float by = __uint_as_float((uint32_t)(up + 127) << 23);
+    const float back = __uint_as_float((uint32_t)(127 - up) << 23) * kCodeUnit * a.scale_log2;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[c][e] *= by;
+      q[c][0] = pack_half(x[c][0], x[c][4]);
+      q[c][1] = pack_half(x[c][1] * 0.0625f, x[c][5] * 0.0625f);
+      q[c][2] = pack_half(x[c][2], x[c][6]);
+      q[c][3] = pack_half(x[c][3] * 0.0625f, x[c][7] * 0.0625f);
+    }
+    // from the lanes of column g to the lanes that hold the column's scores
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      const int from = 4 * (WIDE ? 2 * i + n : 2 * i);
+      fq[n] = __shfl_sync(0xffffffffu, back, from);
+#pragma unroll
+      for (int e = 0; e < GD; ++e) qs[n][e] = __shfl_sync(0xffffffffu, sum[e], from) * a.scale_log2;
+      m[n] = -INFINITY, l[n] = 0.f;
+#pragma unroll
+      for (int e = 0; e < GD; ++e) z[n][e] = 0.f;
+    }
+    lift = 0.f;
+#pragma unroll
+    for (int n = 0; n < D / 16; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+  }
+
+  // One tile at shared-memory address `at`; lo..hi: its slots in range.
+  __device__ __forceinline__ void tile(uint32_t at, int lo, int hi) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3;
+    const int slot0 = (g >> 1) + 4 * (g & 1);
+    float s[2][2][kN];  // [16 slots][row half][head]
+    float2 v[2][2][GD];  // scale and least of V
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+      float acc[GD][4] = {};
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        const int r = 16 * mt + slot0;  // row r + 8 has the same swizzle
+        const uint32_t from = at + r * C::kRow + 16 * swizzled<D>(r, c) + 4 * i;
+        uint32_t w0 = lds32(from), w1 = lds32(from + 8 * C::kRow);
+        float* t = acc[c * GD / (D / 32)];
+        mma(t, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, q[c][0], q[c][1]);
+        w0 >>= 8, w1 >>= 8;
+        mma(t, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, q[c][2], q[c][3]);
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int r = 16 * mt + 8 * half + slot0;
+        const bool live = r >= lo && r < hi;
+#pragma unroll
+        for (int n = 0; n < kN; ++n) s[mt][half][n] = 0.f;
+#pragma unroll
+        for (int e = 0; e < GD; ++e) {
+          const float2 k = pair_of<T>(lds32(at + C::kOffKs + r * C::kPair + 4 * e));
+          v[mt][half][e] = live ? pair_of<T>(lds32(at + C::kOffVs + r * C::kPair + 4 * e)) : make_float2(0.f, 0.f);
+#pragma unroll
+          for (int n = 0; n < kN; ++n)
+            s[mt][half][n] = fmaf(acc[e][2 * half + n] * fq[n], k.x, fmaf(k.y, qs[n][e], s[mt][half][n]));
+        }
+        if (!live)
+#pragma unroll
+          for (int n = 0; n < kN; ++n) s[mt][half][n] = -INFINITY;
+      }
+    }
+    // ---- online softmax: a head's state is agreed on by its eight lanes, l and z are the lane's shares
+    float alpha[kN];
+    bool moved = false;
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      float mt = fmaxf(fmaxf(s[0][0][n], s[0][1][n]), fmaxf(s[1][0][n], s[1][1][n]));
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, off));
+      const float mn = fmaxf(m[n], mt), use = mn == -INFINITY ? 0.f : mn;
+      moved |= mn != m[n];
+      alpha[n] = exp2f(m[n] - use);
+      m[n] = mn;
+      float sum = 0.f;
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) sum += s[a][b][n] = exp2f(s[a][b][n] - use);
+      l[n] = fmaf(l[n], alpha[n], sum);
+    }
+    // ---- the power of two on V's scales: the largest is kept below 2^15
+    float top = 0.f;
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < GD; ++e) top = fmaxf(top, fabsf(v[a][b][e].x));
+    const uint32_t largest = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+    float again = 1.f;
+    if (largest != 0u && (lift == 0.f || __uint_as_float(largest) * lift >= 32768.f) && largest < 0x7f800000u) {
+      // the largest to [2^12, 2^13), so that it may grow eightfold before the next time
+      const int E = min(max((int)(largest >> 23) - 127, -100), 127);
+      const float to = __uint_as_float((uint32_t)(12 - E + 127) << 23);
+      again = lift == 0.f ? 1.f : to / lift;
+      lift = to;
+    }
+    if (__any_sync(0xffffffffu, moved) || again != 1.f) {
+      float f[2];  // of the columns 2 i and 2 i + 1
+      f[0] = alpha[0] * again, f[1] = alpha[kN - 1] * again;
+#pragma unroll
+      for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int e = 0; e < GD; ++e) z[n][e] *= alpha[n];
+#pragma unroll
+      for (int n = 0; n < D / 16; ++n) o[n][0] *= f[0], o[n][1] *= f[1], o[n][2] *= f[0], o[n][3] *= f[1];
+    }
+    // ---- o += V^T P^T
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+      uint32_t ph[GD][2], pl[GD][2];  // operands of slots 0..7 and 8..15
+#pragma unroll
+      for (int e = 0; e < GD; ++e) {
+        const float2 v0 = v[mt][0][e], v1 = v[mt][1][e];
+        const float u0 = v0.x * lift, u1 = v1.x * lift;
+#pragma unroll
+        for (int n = 0; n < kN; ++n) z[n][e] = fmaf(s[mt][0][n], v0.y, fmaf(s[mt][1][n], v1.y, z[n][e]));
+        uint32_t h, lw;
+        if constexpr (WIDE) {
+          split_half(s[mt][0][0] * u0, s[mt][0][1] * u0, h, lw);
+          ph[e][0] = transposed(h), pl[e][0] = transposed(lw);
+          split_half(s[mt][1][0] * u1, s[mt][1][1] * u1, h, lw);
+          ph[e][1] = transposed(h), pl[e][1] = transposed(lw);
+        } else {
+          split_half(s[mt][0][0] * u0, s[mt][1][0] * u1, h, lw);
+          ph[e][0] = transposed(__byte_perm(h, lw, 0x5410));
+          ph[e][1] = transposed(__byte_perm(h, lw, 0x7632));
+        }
+      }
+#pragma unroll
+      for (int half = 0; half < D / 64; ++half) {
+        const int e = GD == 2 ? half : 0;
+        uint32_t w[4];  // the lane's word of slots i, i + 4, i + 8, i + 12
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int r = 16 * mt + 4 * k + i;
+          w[k] = lds32(at + C::kOffV + r * C::kRow + 16 * swizzled<D>(r, 2 * half + (g >> 2)) + 4 * (g & 3));
+        }
+        uint32_t a0 = __byte_perm(w[0], w[1], 0x5410), a1 = __byte_perm(w[0], w[1], 0x7632);  // dims 0..3, 4..7 of the word
+        uint32_t a2 = __byte_perm(w[2], w[3], 0x5410), a3 = __byte_perm(w[2], w[3], 0x7632);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const uint32_t mask = t & 1 ? 0x00f000f0u : 0x000f000fu;
+          mma(o[4 * half + t], a0 & mask, a1 & mask, a2 & mask, a3 & mask, ph[e][0], ph[e][1]);
+          if constexpr (WIDE) mma(o[4 * half + t], a0 & mask, a1 & mask, a2 & mask, a3 & mask, pl[e][0], pl[e][1]);
+          if (t == 1) a0 >>= 8, a1 >>= 8, a2 >>= 8, a3 >>= 8;
+        }
+      }
+    }
+  }
+
+  // Heads h0, h0 + 1 of the block into this warp's part of the reduction buffer.
+  __device__ __forceinline__ void put(int h0, float* red) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3;
+    const float unit = lift == 0.f ? 0.f : kCodeUnit / lift;
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      const int h = WIDE ? 2 * i + n : i;
+      float sum = l[n], least[GD];
+#pragma unroll
+      for (int e = 0; e < GD; ++e) least[e] = z[n][e];
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, off);
+#pragma unroll
+        for (int e = 0; e < GD; ++e) least[e] += __shfl_xor_sync(0xffffffffu, least[e], off);
+      }
+      if (h < h0 || h >= h0 + C::kRedHeads) continue;
+      float* row = red + (h - h0) * C::kRedRow;
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t) {
+        const float by = t & 1 ? unit * 0.0625f : unit;
+        const int d = 64 * (t / 4) + 8 * g + t % 4;
+        const float x = WIDE ? o[t][n] : o[t][0] + o[t][1], y = WIDE ? o[t][2 + n] : o[t][2] + o[t][3];
+        row[d] = fmaf(x, by, least[GD == 2 ? t / 4 : 0]);
+        row[d + 4] = fmaf(y, by, least[GD == 2 ? t / 4 : 0]);
+      }
+      if (g == 0) *reinterpret_cast<float2*>(row + D) = make_float2(m[n], sum);
+    }
+  }
+};
+
+// ------------------------------------------------------------------ the kernel
+
+template <typename T>
+__device__ __forceinline__ void write_result(const Int4Args& a, int b, int head, int d, float4 o4, float M, float L) {
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  union {
+    T t[4];
+    uint2 u;
+  } r;
+  r.t[0] = Elem<T>::from_float(o4.x * inv), r.t[1] = Elem<T>::from_float(o4.y * inv);
+  r.t[2] = Elem<T>::from_float(o4.z * inv), r.t[3] = Elem<T>::from_float(o4.w * inv);
+  *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + b * a.o_sb + head * a.o_sh + d) = r.u;
+  if (a.lse != nullptr && d == 0) a.lse[(int64_t)b * a.hq + head] = L == 0.f ? -INFINITY : M + log2f(L);
+}
+
+template <typename T, int D, int GD, bool WIDE>
+__global__ void __launch_bounds__(Int4Cfg<D, GD>::kThreads, 1) paged_decode_int4_kernel(const __grid_constant__ Int4Args a) {
+  using C = Int4Cfg<D, GD>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  int& s_last = *reinterpret_cast<int*>(smem + C::kOffVars);
+  float* red = reinterpret_cast<float*>(smem + C::kOffRed);
+  const int tid = threadIdx.x, warp = tid >> 5;
+  grid_launch_dependents();
+  grid_dependency_wait();
+  Split<kTile, kPairCost> split = {};
+  split.template find<C::kWarps, kMinChunk, kSmallTiles>(a);
+  const uint32_t ring = smem_u32(smem) + warp * C::kStages * C::kStage;
+  Cursor<D, GD> ahead;
+  if (split.busy) {
+    ahead.begin(a, split.seg, warp);
+#pragma unroll
+    for (int k = 0; k < C::kStages; ++k) ahead.copy(a, ring + k * C::kStage, warp);
+  }
+  if (split.empty_rows)  // requests with nothing to attend to: zeros
+    for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+      int start, len, nt;
+      request_bounds<kTile>(a, b, start, len, nt);
+      if (nt == 0)
+        for (int x = tid; x < a.hq * (D / 4); x += C::kThreads)
+          write_result<T>(a, b, x / (D / 4), x % (D / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, 0.f);
+    }
+  if (!split.busy) return;
+
+  Seg seg = split.seg;
+  const int chunk = split.chunk;
+  const bool small = split.small;
+  Int4State<T, D, GD, WIDE> st;
+  int stage = 0, turn = 0;  // turn: the warp that takes the segment's first tile
+  for (bool first = true;;) {
+    if (seg.t0 == seg.t1) {
+      if (!seg.next(a)) break;
+      continue;
+    }
+    st.begin(a, seg);
+#pragma unroll 1
+    for (int t = seg.t0 + ((warp - turn) & (C::kWarps - 1)); t < seg.t1; t += C::kWarps) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 1) : "memory");
+      __syncwarp();  // every lane's copies have landed
+      const uint32_t at = ring + stage * C::kStage;
+      const int slot = (seg.first_tile + t) * kTile;
+      st.tile(at, seg.start - slot, seg.len - slot);
+      __syncwarp();  // every lane has read the stage
+      ahead.copy(a, at, warp);
+      if (++stage == C::kStages) stage = 0;
+    }
+    turn = (turn + seg.t1 - seg.t0) & (C::kWarps - 1);
+
+    // ---- the warps' states into one
+    const int kvh = seg.pair / a.row_blocks, h0 = (seg.pair - kvh * a.row_blocks) * kHeads;
+    const int heads = min(kHeads, a.group - h0), head0 = kvh * a.group + h0;
+    const bool whole = seg.t0 == 0 && seg.t1 == seg.nt;
+    // a pair that starts inside this range is its last: slot 1, unless it is the first, too
+    const int64_t ws_row = ((int64_t)blockIdx.x * 2 + (first ? 0 : 1)) * kHeads;
+    for (int h = 0; h < heads; h += C::kRedHeads) {
+      st.put(h, red + warp * C::kRedHeads * C::kRedRow);
+      __syncthreads();
+      for (int x = tid; x < min(C::kRedHeads, heads - h) * (D / 4); x += C::kThreads) {
+        const int r = x / (D / 4), d = x % (D / 4) * 4;
+        float M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < C::kWarps; ++w) M = fmaxf(M, red[(w * C::kRedHeads + r) * C::kRedRow + D]);
+        const float use = M == -INFINITY ? 0.f : M;
+        float4 o4 = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < C::kWarps; ++w) {
+          const float* row = red + (w * C::kRedHeads + r) * C::kRedRow;
+          const float2 ml = *reinterpret_cast<const float2*>(row + D);
+          const float f = exp2f(ml.x - use);
+          const float4 v = *reinterpret_cast<const float4*>(row + d);
+          L = fmaf(f, ml.y, L);
+          o4.x = fmaf(f, v.x, o4.x), o4.y = fmaf(f, v.y, o4.y);
+          o4.z = fmaf(f, v.z, o4.z), o4.w = fmaf(f, v.w, o4.w);
+        }
+        if (whole) {
+          write_result<T>(a, seg.b, head0 + h + r, d, o4, M, L);
+        } else {
+          *reinterpret_cast<float4*>(a.ws_o + (ws_row + h + r) * D + d) = o4;
+          if (d == 0) *reinterpret_cast<float2*>(a.ws_ml + (ws_row + h + r) * 2) = make_float2(M, L);
+        }
+      }
+      __syncthreads();
+    }
+
+    // ---- a pair cut by ranges: the last CTA to arrive joins the partials in CTA order
+    if (!whole) {
+      const int pair0 = seg.pair_base();
+      // the CTAs with tiles of it
+      const int c0 = small ? split.first_cta : (pair0 + kPairCost) / chunk;
+      const int c1 = small ? split.last_cta : (pair0 + seg.units() - 1) / chunk;
+      if (tid == 0) {
+        unsigned int prev;
+        // after the barrier, so cumulative over the CTA's stores of its partial
+        asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(prev) : "l"(a.ws_count + c0) : "memory");
+        s_last = prev == (unsigned int)(c1 - c0);
+        if (s_last) a.ws_count[c0] = 0u;  // as the next call expects it
+      }
+      __syncthreads();
+      if (s_last) {
+        const int first_slot = small || c0 * chunk >= pair0 ? 0 : 1;  // of CTA c0; the others hold it as their first
+        for (int x = tid; x < heads * (D / 4); x += C::kThreads) {
+          const int r = x / (D / 4), d = x % (D / 4) * 4;
+          float M = -INFINITY, L = 0.f;
+          float4 o4 = make_float4(0.f, 0.f, 0.f, 0.f);
+          constexpr int kMany = 8;  // partials in flight
+          for (int c = c0; c <= c1; c += kMany) {
+            float2 s[kMany];
+            float4 v[kMany];
+            float Mn = M;
+#pragma unroll
+            for (int k = 0; k < kMany; ++k) {
+              s[k] = make_float2(-INFINITY, 0.f);
+              v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (c + k <= c1) {
+                const int64_t row = ((int64_t)(c + k) * 2 + (c + k == c0 ? first_slot : 0)) * kHeads + r;
+                s[k] = __ldcg(reinterpret_cast<const float2*>(a.ws_ml + row * 2));
+                v[k] = __ldcg(reinterpret_cast<const float4*>(a.ws_o + row * D + d));
+              }
+            }
+#pragma unroll
+            for (int k = 0; k < kMany; ++k) Mn = fmaxf(Mn, s[k].x);
+            const float use = Mn == -INFINITY ? 0.f : Mn, old = exp2f(M - use);
+            L *= old, o4.x *= old, o4.y *= old, o4.z *= old, o4.w *= old;
+#pragma unroll
+            for (int k = 0; k < kMany; ++k) {
+              const float f = exp2f(s[k].x - use);
+              L = fmaf(f, s[k].y, L);
+              o4.x = fmaf(f, v[k].x, o4.x), o4.y = fmaf(f, v[k].y, o4.y);
+              o4.z = fmaf(f, v[k].z, o4.z), o4.w = fmaf(f, v[k].w, o4.w);
+            }
+            M = Mn;
+          }
+          write_result<T>(a, seg.b, head0 + r, d, o4, M, L);
+        }
+      }
+      __syncthreads();  // s_last is free again
+    }
+    first = false;
+    if (!seg.next(a)) break;
+  }
+}
+
+// ------------------------------------------------------------------ host side
+
+// CTAs of a launch: as many as the SMs hold, or fewer where even full caches have fewer runs of kMinChunk tiles.
+int decode_grid(const aicas_paged_decode_int4_params* p, int sms) {
+  const int64_t cap_tiles = ((int64_t)p->max_pages * p->page_size + kTile - 1) / kTile;
+  const int blocks = (p->num_q_heads / p->num_kv_heads + kHeads - 1) / kHeads;
+  const int64_t pairs = (int64_t)p->batch * p->num_kv_heads * blocks;
+  const int64_t runs = (cap_tiles * pairs + kMinChunk - 1) / kMinChunk + pairs;
+  return (int)(runs < sms ? runs : sms);
+}
+
+template <typename T, int D, int GD, bool WIDE>
+cudaError_t launch_one(const Int4Args& a, int grid, cudaStream_t st) {
+  using C = Int4Cfg<D, GD>;
+  static bool attr_set[64] = {false};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    e = cudaFuncSetAttribute(paged_decode_int4_kernel<T, D, GD, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
+  }
+  return launch_pdl(paged_decode_int4_kernel<T, D, GD, WIDE>, dim3(grid), dim3(C::kThreads), C::kSmem, st, a);
+}
+
+template <typename T>
+cudaError_t dispatch(int head_dim, int group_size, const Int4Args& a, int grid, cudaStream_t st) {
+  const bool wide = a.group > 4;
+  if (head_dim == 64) return wide ? launch_one<T, 64, 1, true>(a, grid, st) : launch_one<T, 64, 1, false>(a, grid, st);
+  if (group_size == 64) return wide ? launch_one<T, 128, 2, true>(a, grid, st) : launch_one<T, 128, 2, false>(a, grid, st);
+  return wide ? launch_one<T, 128, 1, true>(a, grid, st) : launch_one<T, 128, 1, false>(a, grid, st);
 }
 
 }  // namespace
 
-size_t paged_decode_int4_workspace(int) { return 256; }
+// The same for every call, so that a stream's buffer never has to grow for another shape.
+size_t paged_decode_int4_workspace(int sms) {
+  return kWsCounters + (size_t)sms * 2 * kHeads * (128 + 2) * sizeof(float);
+}
 
-int run_paged_decode_int4(const aicas_paged_decode_int4_params* p, int, void*, cudaStream_t stream, char* err, size_t errlen) {
-  const cudaError_t e = p->dtype == AICAS_DTYPE_F16 ? launch_decode_int4<__half>(*p, stream) : launch_decode_int4<__nv_bfloat16>(*p, stream);
+int run_paged_decode_int4(const aicas_paged_decode_int4_params* p, int sms, void* workspace, cudaStream_t stream, char* err,
+                          size_t errlen) {
+  Int4Args a;
+  memset(&a, 0, sizeof(a));
+  a.kv[0] = p->kv[0], a.kv[1] = p->kv[1];
+  a.q = p->q, a.out = p->out, a.lse = p->lse;
+  a.table = p->page_table, a.lens = p->kv_lens, a.starts = p->kv_starts;
+  a.q_sb = p->q_stride_b, a.q_sh = p->q_stride_h, a.o_sb = p->o_stride_b, a.o_sh = p->o_stride_h;
+  a.table_stride = p->table_stride;
+  a.batch = p->batch, a.hq = p->num_q_heads, a.hkv = p->num_kv_heads;
+  a.group = p->num_q_heads / p->num_kv_heads;
+  a.row_blocks = (a.group + kHeads - 1) / kHeads;
+  a.num_pages = p->num_pages, a.cap = p->max_pages * p->page_size;
+  // n / d for n < 2^28: with s = ceil(log2 d), (n + floor(n M / 2^32)) >> s, M = floor(2^32 (2^s - d) / d) + 1
+  a.octets = p->page_size / 8;
+  while ((1ll << a.octets_shift) < a.octets) ++a.octets_shift;
+  a.octets_mul = (uint32_t)((((1ull << a.octets_shift) - a.octets) << 32) / a.octets + 1);
+  a.scale_log2 = p->sm_scale * 1.4426950408889634f;
+  const int grid = decode_grid(p, sms);
+  a.few = 2 * (int64_t)a.batch * a.hkv * a.row_blocks <= grid;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  a.ws_count = reinterpret_cast<unsigned int*>(ws);
+  a.ws_o = reinterpret_cast<float*>(ws + kWsCounters);
+  a.ws_ml = a.ws_o + (size_t)grid * 2 * kHeads * p->head_dim;
+  const cudaError_t e = p->dtype == AICAS_DTYPE_F16 ? dispatch<__half>(p->head_dim, p->group_size, a, grid, stream)
+                                                    : dispatch<__nv_bfloat16>(p->head_dim, p->group_size, a, grid, stream);
   if (e == cudaSuccess) return AICAS_OK;
   snprintf(err, errlen, "paged 4-bit decode launch: %s (%s)", cudaGetErrorString(e), cudaGetErrorName(e));
   return AICAS_ERR_CUDA;
