@@ -589,7 +589,7 @@ int check_paged_decode_int4(const aicas_paged_decode_int4_params* p) {
   for (int64_t s : qo)
     if (s < 0 || !stride_ok(s, 2)) return fail(AICAS_ERR_INVALID, "q/out strides must be non-negative multiples of 16 bytes");
   // tiles of (request, KV head, block of query heads), and a few more each, are numbered with 32-bit ints
-  const int64_t tiles = (((int64_t)p->max_pages * p->page_size + 15) / 16 + 16) * p->batch *
+  const int64_t tiles = (((int64_t)p->max_pages * p->page_size + 15) / 16 + 40) * p->batch *
                         ((int64_t)p->num_kv_heads * ((p->num_q_heads / p->num_kv_heads + 7) / 8));
   if (tiles > (int64_t)INT32_MAX / 2)
     return fail(AICAS_ERR_UNSUPPORTED, "%lld tiles of 16 slots exceed the 2^30 of one launch", (long long)tiles);
@@ -1143,13 +1143,13 @@ int aicas_paged_read_int4(const aicas_paged_read_int4_params* p, void* stream) {
 
 size_t aicas_paged_decode_int4_workspace_bytes(const aicas_paged_decode_int4_params* p) {
   if (check_paged_decode_int4(p) != AICAS_OK) return 0;
-  return aicas::paged_decode_int4_workspace(sm_count());
+  return aicas::paged_decode_int4_workspace(p, sm_count());
 }
 
 int aicas_paged_decode_int4(const aicas_paged_decode_int4_params* p, void* workspace, size_t workspace_bytes, void* stream) {
   const int rc = check_paged_decode_int4(p);
   if (rc != AICAS_OK) return rc;
-  const size_t need = aicas::paged_decode_int4_workspace(sm_count());
+  const size_t need = aicas::paged_decode_int4_workspace(p, sm_count());
   if (workspace == nullptr || workspace_bytes < need)
     return fail(AICAS_ERR_WORKSPACE, "paged 4-bit decode needs %zu bytes of zero-initialised workspace (got %zu)", need,
                 workspace_bytes);

@@ -13,8 +13,8 @@ namespace aicas {
 int run_paged_append_int4(const aicas_paged_append_int4_params* p, cudaStream_t stream, char* err, size_t errlen);
 int run_paged_read_int4(const aicas_paged_read_int4_params* p, cudaStream_t stream, char* err, size_t errlen);
 
-// Bytes of workspace run_paged_decode_int4 needs on a device with `sms` SMs, whatever the call.
-size_t paged_decode_int4_workspace(int sms);
+// Bytes of workspace run_paged_decode_int4 needs on a device with `sms` SMs.
+size_t paged_decode_int4_workspace(const aicas_paged_decode_int4_params* p, int sms);
 int run_paged_decode_int4(const aicas_paged_decode_int4_params* p, int sms, void* workspace, cudaStream_t stream,
                           char* err, size_t errlen);
 

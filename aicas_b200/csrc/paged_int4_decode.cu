@@ -38,15 +38,23 @@ namespace aicas {
 namespace {
 
 constexpr int kTile = 32;      // slots a tile
-constexpr int kPairCost = 3;   // what beginning and ending a pair costs a CTA, in tiles
-constexpr int kMinChunk = 16;  // fewest tiles a CTA takes
+constexpr int kRanges = 6;     // ranges that a pair is cut into, about
+constexpr int kPairCost = 2;   // what beginning and ending a pair costs a warp, in tiles
+constexpr int kLeast = 1;      // fewest tiles a warp takes
 constexpr int kSmallTiles = 16;  // most tiles a CTA of a launch that gives pairs whole CTAs
 constexpr int kHeads = 8;      // query heads of a block
 constexpr size_t kWsCounters = (size_t)1 << 20;  // counter region shared with the other decode kernels
 constexpr float kCodeUnit = 16777216.f;  // 2^24: a code in an fp16's low bits is code / kCodeUnit
 
+// One side's pages: strides of the codes in 16 bytes, of the pairs in kPair bytes.
+struct Side {
+  const uint8_t* codes;
+  const uint8_t* pairs;
+  uint32_t cs_p, cs_h, cs_t, ss_p, ss_h, ss_t;
+};
+
 struct Int4Args {
-  aicas_int4_pages kv[2];
+  Side kv[2];
   const void* q;
   void* out;
   float* lse;
@@ -60,10 +68,11 @@ struct Int4Args {
   uint32_t octets_mul;     // n / octets = (umulhi(n, octets_mul) + n) >> octets_shift
   int octets_shift;
   int few;                 // at most half as many pairs as CTAs
+  int part_heads;          // heads that a partial result has room for
   float scale_log2;
-  float* ws_o;             // [2 * grid][kHeads][D]
-  float* ws_ml;            // [2 * grid][kHeads][2]
-  unsigned int* ws_count;  // [grid]
+  float* ws_o;             // [2 * teams][part_heads][D]
+  float* ws_ml;            // [2 * teams][part_heads][2]
+  unsigned int* ws_count;  // [teams]
 };
 
 template <int D, int GD>
@@ -72,19 +81,19 @@ struct Int4Cfg {
   static constexpr int kChunks = kRow / 16;   // its 16-byte chunks
   static constexpr int kPair = 4 * GD;        // bytes of a row's pairs
   static constexpr int kOffV = kTile * kRow;
-  static constexpr int kOffKs = 2 * kTile * kRow, kOffVs = kOffKs + kTile * kPair;
-  static constexpr int kStage = kOffVs + kTile * kPair;
+  static constexpr int kOffPairs = 2 * kTile * kRow;  // a slot's pairs of K, then of V
+  static constexpr int kStage = kOffPairs + 2 * kTile * kPair;
   static constexpr int kWarps = 16, kThreads = kWarps * 32;
   static constexpr int kStages = GD == 1 ? 3 : 2;
   static constexpr int kRedHeads = 2;         // heads that the warps' states are joined of at a time
   static constexpr int kRedRow = D + 4;
   static constexpr int kOffRed = kWarps * kStages * kStage;
   static constexpr int kOffVars = kOffRed + kWarps * kRedHeads * kRedRow * 4;
-  static constexpr int kSmem = kOffVars + 16;
+  static constexpr int kSmem = kOffVars + 4 * kWarps;
   static_assert(kSmem <= 232448, "shared memory");
 };
 
-using Seg = Segment<kTile, kPairCost>;
+using Seg = Segment<kTile>;
 
 // The 16-byte chunk where chunk c of row r is kept.  K's fragments take the same chunk of 8
 // rows, V's half of the chunks of 4 rows: both meet all banks once.
@@ -118,6 +127,12 @@ __device__ __forceinline__ void mma(float c[4], uint32_t a0, uint32_t a1, uint32
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
@@ -180,11 +195,11 @@ struct Cursor {
   }
 
   // To the warp's first tile at or after the segment.
-  __device__ __forceinline__ void settle(const Int4Args& a, int warp) {
+  __device__ __forceinline__ void settle(const Int4Args& a, int rank, int team) {
     for (;;) {
-      t = seg.t0 + ((warp - turn) & (C::kWarps - 1));
+      t = seg.t0 + ((rank - turn) & (team - 1));
       if (t < seg.t1) break;
-      turn = (turn + seg.t1 - seg.t0) & (C::kWarps - 1);
+      turn = (turn + seg.t1 - seg.t0) & (team - 1);
       if (!seg.next(a)) {
         more = false;
         break;
@@ -192,37 +207,38 @@ struct Cursor {
     }
   }
 
-  __device__ __forceinline__ void begin(const Int4Args& a, const Seg& first, int warp) {
+  __device__ __forceinline__ void begin(const Int4Args& a, const Seg& first, int rank, int team) {
     seg = first, turn = 0, more = true;
-    settle(a, warp);
+    settle(a, rank, team);
     look(a);
   }
 
   // Asks for the tile and goes on to the next one.
-  __device__ __forceinline__ void copy(const Int4Args& a, uint32_t stage, int warp) {
+  __device__ __forceinline__ void copy(const Int4Args& a, uint32_t stage, int rank, int team) {
     if (more) {
       const int lane = threadIdx.x & 31, o = lane >> 3, sub = lane & 7;
-      const int head = seg.pair / a.row_blocks;
+      const uint32_t head = a.row_blocks == 1 ? seg.pair : seg.pair / a.row_blocks;
       const bool there = page >= 0 && page < a.num_pages;
-      const int64_t pg = there ? page : 0;
+      const uint32_t pg = there ? page : 0;
       constexpr int kAtOnce = 8 / C::kChunks;  // rows of an octet in one go
       const int r = sub / C::kChunks, c = sub % C::kChunks;
 #pragma unroll
       for (int side = 0; side < 2; ++side) {
-        const aicas_int4_pages& p = a.kv[side];
-        const uint8_t* codes = static_cast<const uint8_t*>(p.codes) + pg * p.cs_p + head * p.cs_h + (int64_t)(8 * octet + r) * p.cs_t + 16 * c;
+        const Side& p = a.kv[side];
+        const uint8_t* codes = p.codes + 16 * ((uint64_t)pg * p.cs_p + (uint64_t)head * p.cs_h + (uint64_t)(uint32_t)(8 * octet + r) * p.cs_t + c);
+        const uint64_t step = (uint64_t)p.cs_t * (16 * kAtOnce);
         const uint32_t dst = stage + side * C::kOffV + (8 * o + r) * C::kRow;
 #pragma unroll
         for (int k = 0; k < C::kChunks; ++k)
-          copy_async<16>(dst + kAtOnce * k * C::kRow + 16 * swizzled<D>(r + kAtOnce * k, c), codes + (int64_t)kAtOnce * k * p.cs_t, there);
-        const uint16_t* pair = static_cast<const uint16_t*>(p.scales) + pg * p.ss_p + head * p.ss_h + (int64_t)(8 * octet + sub) * p.ss_t;
-        copy_async<C::kPair>(stage + (side ? C::kOffVs : C::kOffKs) + lane * C::kPair, pair, there);
+          copy_async<16>(dst + kAtOnce * k * C::kRow + 16 * swizzled<D>(r + kAtOnce * k, c), codes + k * step, there);
+        const uint8_t* pair = p.pairs + C::kPair * ((uint64_t)pg * p.ss_p + (uint64_t)head * p.ss_h + (uint64_t)(uint32_t)(8 * octet + sub) * p.ss_t);
+        copy_async<C::kPair>(stage + C::kOffPairs + (2 * lane + side) * C::kPair, pair, there);
       }
-      t += C::kWarps;
+      t += team;
       if (t >= seg.t1) {
-        turn = (turn + seg.t1 - seg.t0) & (C::kWarps - 1);
+        turn = (turn + seg.t1 - seg.t0) & (team - 1);
         more = seg.next(a);
-        if (more) settle(a, warp);
+        if (more) settle(a, rank, team);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -236,30 +252,43 @@ struct Cursor {
 // heads, head j's hi and lo parts in columns 2 j and 2 j + 1 of the same products.
 // A lane's heads: WIDE 2 i and 2 i + 1, else i; slots (rows g and g + 8 of a product) of
 // 16 are g / 2 + 4 (g % 2) and 8 more, an order that lets V's loads meet no bank twice.
+//
+// With one group a row (GD = 1) lane i takes the 32 dims of chunk i of K, lane g the 16 of
+// words 2 g and 2 g + 1 of V; with two, so that a product stays within a group, 8 dims of
+// each 32 and words g and g + 8.
 template <typename T, int D, int GD, bool WIDE>
 struct Int4State {
   using C = Int4Cfg<D, GD>;
   static constexpr int kN = WIDE ? 2 : 1;  // heads a lane
-  uint32_t q[D / 32][4];  // the lane's 8 dims of each 32, as (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16
+  static constexpr bool kWhole = GD == 1;
+  static constexpr int kWords = D / 32;    // words of K a lane takes of a row: 8 dims each
+  uint32_t q[kWords][4];  // of a word's dims (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16
   float fq[kN], qs[kN][GD];  // of the lane's heads: factor of q.code, sum of q, both with the softmax's scale
   float o[D / 16][4];
-  float m[kN], l[kN], z[kN][GD];
-  float lift;             // power of two on scales of V; 0: none seen yet
+  float ref[kN];           // what scores are taken against; within kSlack of the largest so far, or above
+  float l[kN], z[kN][GD];  // the lane's shares of sum p, sum p least
+  float lift;              // power of two on scales of V
+  float bound;             // the largest scale of V that lift is good for; -1: no tile yet
+
+  // p stays below 2^kSlack: the reference is moved when a score passes it by more.
+  static constexpr float kSlack = 4.f;
+
+  __device__ __forceinline__ static int dim_of(int i, int w) { return kWhole ? 8 * (kWords * i + w) : 32 * w + 8 * i; }
 
   __device__ __forceinline__ void begin(const Int4Args& a, const Seg& s) {
     const int lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3;
     const int kvh = s.pair / a.row_blocks, h0 = (s.pair - kvh * a.row_blocks) * kHeads;
     const int heads = min(kHeads, a.group - h0);
     const int col = WIDE ? g : g >> 1;  // the head of column g
-    float x[D / 32][8], top = 0.f, sum[GD] = {};
-    const T* src = static_cast<const T*>(a.q) + s.b * a.q_sb + (int64_t)(kvh * a.group + h0 + min(col, heads - 1)) * a.q_sh + 8 * i;
+    float x[kWords][8], top = 0.f, sum[GD] = {};
+    const T* src = static_cast<const T*>(a.q) + s.b * a.q_sb + (int64_t)(kvh * a.group + h0 + min(col, heads - 1)) * a.q_sh;
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c) {
-      Elem<T>::unpack(*reinterpret_cast<const uint4*>(src + 32 * c), x[c]);
+    for (int c = 0; c < kWords; ++c) {
+      Elem<T>::unpack(*reinterpret_cast<const uint4*>(src + dim_of(i, c)), x[c]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         top = fmaxf(top, fabsf(x[c][e]));
-        sum[c * GD / (D / 32)] += x[c][e];
+        sum[c * GD / kWords] += x[c][e];
       }
     }
 #pragma unroll
@@ -275,7 +304,7 @@ struct Int4State {
     const float by = __uint_as_float((uint32_t)(up + 127) << 23);
     const float back = __uint_as_float((uint32_t)(127 - up) << 23) * kCodeUnit * a.scale_log2;
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c) {
+    for (int c = 0; c < kWords; ++c) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[c][e] *= by;
       q[c][0] = pack_half(x[c][0], x[c][4]);
@@ -290,101 +319,136 @@ struct Int4State {
       fq[n] = __shfl_sync(0xffffffffu, back, from);
 #pragma unroll
       for (int e = 0; e < GD; ++e) qs[n][e] = __shfl_sync(0xffffffffu, sum[e], from) * a.scale_log2;
-      m[n] = -INFINITY, l[n] = 0.f;
+      ref[n] = 0.f, l[n] = 0.f;
 #pragma unroll
       for (int e = 0; e < GD; ++e) z[n][e] = 0.f;
     }
-    lift = 0.f;
+    lift = 0.f, bound = -1.f;
 #pragma unroll
     for (int n = 0; n < D / 16; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
   }
 
-  // One tile at shared-memory address `at`; lo..hi: its slots in range.
-  __device__ __forceinline__ void tile(uint32_t at, int lo, int hi) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3;
-    const int slot0 = (g >> 1) + 4 * (g & 1);
-    float s[2][2][kN];  // [16 slots][row half][head]
-    float2 v[2][2][GD];  // scale and least of V
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-      float acc[GD][4] = {};
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        const int r = 16 * mt + slot0;  // row r + 8 has the same swizzle
-        const uint32_t from = at + r * C::kRow + 16 * swizzled<D>(r, c) + 4 * i;
-        uint32_t w0 = lds32(from), w1 = lds32(from + 8 * C::kRow);
-        float* t = acc[c * GD / (D / 32)];
-        mma(t, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, q[c][0], q[c][1]);
-        w0 >>= 8, w1 >>= 8;
-        mma(t, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, q[c][2], q[c][3]);
-      }
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int r = 16 * mt + 8 * half + slot0;
-        const bool live = r >= lo && r < hi;
-#pragma unroll
-        for (int n = 0; n < kN; ++n) s[mt][half][n] = 0.f;
-#pragma unroll
-        for (int e = 0; e < GD; ++e) {
-          const float2 k = pair_of<T>(lds32(at + C::kOffKs + r * C::kPair + 4 * e));
-          v[mt][half][e] = live ? pair_of<T>(lds32(at + C::kOffVs + r * C::kPair + 4 * e)) : make_float2(0.f, 0.f);
-#pragma unroll
-          for (int n = 0; n < kN; ++n)
-            s[mt][half][n] = fmaf(acc[e][2 * half + n] * fq[n], k.x, fmaf(k.y, qs[n][e], s[mt][half][n]));
-        }
-        if (!live)
-#pragma unroll
-          for (int n = 0; n < kN; ++n) s[mt][half][n] = -INFINITY;
-      }
-    }
-    // ---- online softmax: a head's state is agreed on by its eight lanes, l and z are the lane's shares
-    float alpha[kN];
-    bool moved = false;
-#pragma unroll
-    for (int n = 0; n < kN; ++n) {
-      float mt = fmaxf(fmaxf(s[0][0][n], s[0][1][n]), fmaxf(s[1][0][n], s[1][1][n]));
-#pragma unroll
-      for (int off = 4; off < 32; off <<= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, off));
-      const float mn = fmaxf(m[n], mt), use = mn == -INFINITY ? 0.f : mn;
-      moved |= mn != m[n];
-      alpha[n] = exp2f(m[n] - use);
-      m[n] = mn;
-      float sum = 0.f;
-#pragma unroll
-      for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int b = 0; b < 2; ++b) sum += s[a][b][n] = exp2f(s[a][b][n] - use);
-      l[n] = fmaf(l[n], alpha[n], sum);
-    }
-    // ---- the power of two on V's scales: the largest is kept below 2^15
-    float top = 0.f;
+  // A score passes the reference by more than kSlack, or a scale of V the bound: both anew.
+  __device__ __forceinline__ void move(float (&s)[2][2][kN], const float2 (&v)[2][2][GD]) {
+    float f[kN], top = 0.f;
 #pragma unroll
     for (int a = 0; a < 2; ++a)
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int e = 0; e < GD; ++e) top = fmaxf(top, fabsf(v[a][b][e].x));
+        for (int e = 0; e < GD; ++e) top = fmaxf(top, fabsf(v[a][b][e].x) < INFINITY ? fabsf(v[a][b][e].x) : 0.f);
     const uint32_t largest = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+    const bool first = bound < 0.f;
     float again = 1.f;
-    if (largest != 0u && (lift == 0.f || __uint_as_float(largest) * lift >= 32768.f) && largest < 0x7f800000u) {
-      // the largest to [2^12, 2^13), so that it may grow eightfold before the next time
+    if (__uint_as_float(largest) > bound) {
+      // the largest to [2^7, 2^8), so that it may grow 16-fold, and p to 2^kSlack, below 2^16
       const int E = min(max((int)(largest >> 23) - 127, -100), 127);
-      const float to = __uint_as_float((uint32_t)(12 - E + 127) << 23);
+      const float to = __uint_as_float((uint32_t)(7 - E + 127) << 23);
       again = lift == 0.f ? 1.f : to / lift;
       lift = to;
+      bound = __uint_as_float(min((uint32_t)(E + 4 + 127) << 23, 0x7f7fffffu));
     }
-    if (__any_sync(0xffffffffu, moved) || again != 1.f) {
-      float f[2];  // of the columns 2 i and 2 i + 1
-      f[0] = alpha[0] * again, f[1] = alpha[kN - 1] * again;
 #pragma unroll
-      for (int n = 0; n < kN; ++n)
+    for (int n = 0; n < kN; ++n) {
+      float mt = fmaxf(fmaxf(s[0][0][n], s[0][1][n]), fmaxf(s[1][0][n], s[1][1][n]));
 #pragma unroll
-        for (int e = 0; e < GD; ++e) z[n][e] *= alpha[n];
+      for (int off = 4; off < 32; off <<= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, off));
+      // scores are less the old reference; the first tile sets it, down too
+      const float up = mt == -INFINITY ? 0.f : first ? mt : fmaxf(mt, 0.f);
+      ref[n] += up;
+      const float alpha = exp2f(-up);
+      l[n] *= alpha;
 #pragma unroll
-      for (int n = 0; n < D / 16; ++n) o[n][0] *= f[0], o[n][1] *= f[1], o[n][2] *= f[0], o[n][3] *= f[1];
+      for (int e = 0; e < GD; ++e) z[n][e] *= alpha;
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) s[a][b][n] -= up;
+      f[n] = alpha * again;
     }
+    if (first) return;  // nothing added up yet
+#pragma unroll
+    for (int n = 0; n < D / 16; ++n)
+      o[n][0] *= f[0], o[n][1] *= f[kN - 1], o[n][2] *= f[0], o[n][3] *= f[kN - 1];
+  }
+
+  // One tile at shared-memory address `at`; lo..hi: its slots in range.
+  __device__ __forceinline__ void tile(uint32_t at, int lo, int hi) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3;
+    const int slot0 = (g >> 1) + 4 * (g & 1);
+    float s[2][2][kN];  // [16 slots][row half][head], less ref
+    float2 v[2][2][GD];  // scale and least of V
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+      const int r = 16 * mt + slot0;  // row r + 8 has the same swizzle
+      float acc[GD][4] = {};
+      uint32_t w0[kWords], w1[kWords];
+      if constexpr (kWhole) {
+        lds_words<kWords>(at + r * C::kRow + 4 * kWords * i, w0, slot0, i);
+        lds_words<kWords>(at + (r + 8) * C::kRow + 4 * kWords * i, w1, slot0, i);
+      } else {
+#pragma unroll
+        for (int c = 0; c < kWords; ++c) {
+          const uint32_t from = at + r * C::kRow + 16 * swizzled<D>(slot0, c) + 4 * i;
+          w0[c] = lds32(from), w1[c] = lds32(from + 8 * C::kRow);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < kWords; ++c) {
+        float* t = acc[c * GD / kWords];
+        mma(t, w0[c] & 0x000f000fu, w1[c] & 0x000f000fu, w0[c] & 0x00f000f0u, w1[c] & 0x00f000f0u, q[c][0], q[c][1]);
+        const uint32_t u0 = w0[c] >> 8, u1 = w1[c] >> 8;
+        mma(t, u0 & 0x000f000fu, u1 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x00f000f0u, q[c][2], q[c][3]);
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t kp[GD], vp[GD];
+        lds_pairs(at + C::kOffPairs + (r + 8 * half) * 2 * C::kPair, kp, vp);
+#pragma unroll
+        for (int n = 0; n < kN; ++n) s[mt][half][n] = -ref[n];
+#pragma unroll
+        for (int e = 0; e < GD; ++e) {
+          const float2 k = pair_of<T>(kp[e]);
+          v[mt][half][e] = pair_of<T>(vp[e]);
+#pragma unroll
+          for (int n = 0; n < kN; ++n)
+            s[mt][half][n] = fmaf(acc[e][2 * half + n] * fq[n], k.x, fmaf(k.y, qs[n][e], s[mt][half][n]));
+        }
+      }
+    }
+    if (lo > 0 || hi < kTile) {  // an end of the range
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int r = 16 * mt + 8 * half + slot0;
+          if (r >= lo && r < hi) continue;
+#pragma unroll
+          for (int n = 0; n < kN; ++n) s[mt][half][n] = -INFINITY;
+#pragma unroll
+          for (int e = 0; e < GD; ++e) v[mt][half][e] = make_float2(0.f, 0.f);
+        }
+    }
+    // ---- online softmax: a head's reference is agreed on by its eight lanes
+    float top = 0.f, most = -INFINITY;
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+#pragma unroll
+        for (int n = 0; n < kN; ++n) most = fmaxf(most, s[a][b][n]);
+#pragma unroll
+        for (int e = 0; e < GD; ++e) top = fmaxf(top, fabsf(v[a][b][e].x));
+      }
+    if (__any_sync(0xffffffffu, most > kSlack || top > bound)) move(s, v);
+#pragma unroll
+    for (int n = 0; n < kN; ++n)
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) l[n] += s[a][b][n] = exp2_fast(s[a][b][n]);
     // ---- o += V^T P^T
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
@@ -407,17 +471,25 @@ struct Int4State {
           ph[e][1] = transposed(__byte_perm(h, lw, 0x7632));
         }
       }
+      uint32_t w[4][D / 64];  // the lane's words of slots i, i + 4, i + 8, i + 12
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int r = 16 * mt + 4 * k + i;
+        const uint32_t row = at + C::kOffV + r * C::kRow;
+        if constexpr (kWhole && D == 128) {
+          asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[k][0]), "=r"(w[k][1])
+                       : "r"(row + 16 * swizzled<D>(4 * k + i, g >> 1) + 8 * (g & 1)) : "memory");
+        } else {
+#pragma unroll
+          for (int half = 0; half < D / 64; ++half)
+            w[k][half] = lds32(row + 16 * swizzled<D>(4 * k + i, 2 * half + (g >> 2)) + 4 * (g & 3));
+        }
+      }
 #pragma unroll
       for (int half = 0; half < D / 64; ++half) {
         const int e = GD == 2 ? half : 0;
-        uint32_t w[4];  // the lane's word of slots i, i + 4, i + 8, i + 12
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int r = 16 * mt + 4 * k + i;
-          w[k] = lds32(at + C::kOffV + r * C::kRow + 16 * swizzled<D>(r, 2 * half + (g >> 2)) + 4 * (g & 3));
-        }
-        uint32_t a0 = __byte_perm(w[0], w[1], 0x5410), a1 = __byte_perm(w[0], w[1], 0x7632);  // dims 0..3, 4..7 of the word
-        uint32_t a2 = __byte_perm(w[2], w[3], 0x5410), a3 = __byte_perm(w[2], w[3], 0x7632);
+        uint32_t a0 = __byte_perm(w[0][half], w[1][half], 0x5410), a1 = __byte_perm(w[0][half], w[1][half], 0x7632);  // dims 0..3, 4..7 of the word
+        uint32_t a2 = __byte_perm(w[2][half], w[3][half], 0x5410), a3 = __byte_perm(w[2][half], w[3][half], 0x7632);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           const uint32_t mask = t & 1 ? 0x00f000f0u : 0x000f000fu;
@@ -426,6 +498,27 @@ struct Int4State {
           if (t == 1) a0 >>= 8, a1 >>= 8, a2 >>= 8, a3 >>= 8;
         }
       }
+    }
+  }
+
+  // The words of chunk i of row `slot0` of 16.
+  template <int N>
+  __device__ __forceinline__ static void lds_words(uint32_t from, uint32_t* w, int slot0, int i) {
+    if constexpr (N == 4) {
+      const uint32_t addr = from + 16 * (swizzled<D>(slot0, i) - i);
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr) : "memory");
+    } else {  // half a chunk
+      const uint32_t addr = from + 16 * (swizzled<D>(slot0, i >> 1) - (i >> 1));
+      asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr) : "memory");
+    }
+  }
+
+  // A slot's pairs of K and V.
+  __device__ __forceinline__ static void lds_pairs(uint32_t addr, uint32_t* k, uint32_t* v) {
+    if constexpr (GD == 1) {
+      asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(k[0]), "=r"(v[0]) : "r"(addr) : "memory");
+    } else {
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(k[0]), "=r"(k[1]), "=r"(v[0]), "=r"(v[1]) : "r"(addr) : "memory");
     }
   }
 
@@ -450,12 +543,12 @@ struct Int4State {
 #pragma unroll
       for (int t = 0; t < D / 16; ++t) {
         const float by = t & 1 ? unit * 0.0625f : unit;
-        const int d = 64 * (t / 4) + 8 * g + t % 4;
+        const int d = kWhole && D == 128 ? 16 * g + 8 * (t / 4) + t % 4 : 64 * (t / 4) + 8 * g + t % 4;
         const float x = WIDE ? o[t][n] : o[t][0] + o[t][1], y = WIDE ? o[t][2 + n] : o[t][2] + o[t][3];
         row[d] = fmaf(x, by, least[GD == 2 ? t / 4 : 0]);
         row[d + 4] = fmaf(y, by, least[GD == 2 ? t / 4 : 0]);
       }
-      if (g == 0) *reinterpret_cast<float2*>(row + D) = make_float2(m[n], sum);
+      if (g == 0) *reinterpret_cast<float2*>(row + D) = make_float2(bound < 0.f ? -INFINITY : ref[n], sum);
     }
   }
 };
@@ -479,19 +572,27 @@ template <typename T, int D, int GD, bool WIDE>
 __global__ void __launch_bounds__(Int4Cfg<D, GD>::kThreads, 1) paged_decode_int4_kernel(const __grid_constant__ Int4Args a) {
   using C = Int4Cfg<D, GD>;
   extern __shared__ __align__(128) uint8_t smem[];
-  int& s_last = *reinterpret_cast<int*>(smem + C::kOffVars);
+  int* s_last = reinterpret_cast<int*>(smem + C::kOffVars);  // of a team, at its first warp's place
   float* red = reinterpret_cast<float*>(smem + C::kOffRed);
   const int tid = threadIdx.x, warp = tid >> 5;
   grid_launch_dependents();
   grid_dependency_wait();
-  Split<kTile, kPairCost> split = {};
-  split.template find<C::kWarps, kMinChunk, kSmallTiles>(a);
+  Split<kTile> split = {};
+  split.template find<C::kWarps, kRanges, kLeast, kPairCost, kSmallTiles>(a);
+  const int team = split.team, rank = warp & (team - 1), threads = 32 * team, lane_id = tid & (threads - 1);
+  const auto team_sync = [&] {
+    if (team == 1) {
+      __syncwarp();
+    } else {
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / team), "r"(threads) : "memory");
+    }
+  };
   const uint32_t ring = smem_u32(smem) + warp * C::kStages * C::kStage;
   Cursor<D, GD> ahead;
   if (split.busy) {
-    ahead.begin(a, split.seg, warp);
+    ahead.begin(a, split.seg, rank, team);
 #pragma unroll
-    for (int k = 0; k < C::kStages; ++k) ahead.copy(a, ring + k * C::kStage, warp);
+    for (int k = 0; k < C::kStages; ++k) ahead.copy(a, ring + k * C::kStage, rank, team);
   }
   if (split.empty_rows)  // requests with nothing to attend to: zeros
     for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
@@ -506,6 +607,7 @@ __global__ void __launch_bounds__(Int4Cfg<D, GD>::kThreads, 1) paged_decode_int4
   Seg seg = split.seg;
   const int chunk = split.chunk;
   const bool small = split.small;
+  float* const team_red = red + (warp - rank) * C::kRedHeads * C::kRedRow;
   Int4State<T, D, GD, WIDE> st;
   int stage = 0, turn = 0;  // turn: the warp that takes the segment's first tile
   for (bool first = true;;) {
@@ -515,37 +617,37 @@ __global__ void __launch_bounds__(Int4Cfg<D, GD>::kThreads, 1) paged_decode_int4
     }
     st.begin(a, seg);
 #pragma unroll 1
-    for (int t = seg.t0 + ((warp - turn) & (C::kWarps - 1)); t < seg.t1; t += C::kWarps) {
+    for (int t = seg.t0 + ((rank - turn) & (team - 1)); t < seg.t1; t += team) {
       asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 1) : "memory");
       __syncwarp();  // every lane's copies have landed
       const uint32_t at = ring + stage * C::kStage;
       const int slot = (seg.first_tile + t) * kTile;
       st.tile(at, seg.start - slot, seg.len - slot);
       __syncwarp();  // every lane has read the stage
-      ahead.copy(a, at, warp);
+      ahead.copy(a, at, rank, team);
       if (++stage == C::kStages) stage = 0;
     }
-    turn = (turn + seg.t1 - seg.t0) & (C::kWarps - 1);
+    turn = (turn + seg.t1 - seg.t0) & (team - 1);
 
     // ---- the warps' states into one
     const int kvh = seg.pair / a.row_blocks, h0 = (seg.pair - kvh * a.row_blocks) * kHeads;
     const int heads = min(kHeads, a.group - h0), head0 = kvh * a.group + h0;
     const bool whole = seg.t0 == 0 && seg.t1 == seg.nt;
     // a pair that starts inside this range is its last: slot 1, unless it is the first, too
-    const int64_t ws_row = ((int64_t)blockIdx.x * 2 + (first ? 0 : 1)) * kHeads;
+    const int64_t ws_row = ((int64_t)split.id * 2 + (first ? 0 : 1)) * a.part_heads;
     for (int h = 0; h < heads; h += C::kRedHeads) {
       st.put(h, red + warp * C::kRedHeads * C::kRedRow);
-      __syncthreads();
-      for (int x = tid; x < min(C::kRedHeads, heads - h) * (D / 4); x += C::kThreads) {
+      team_sync();
+      for (int x = lane_id; x < min(C::kRedHeads, heads - h) * (D / 4); x += threads) {
         const int r = x / (D / 4), d = x % (D / 4) * 4;
         float M = -INFINITY, L = 0.f;
-#pragma unroll
-        for (int w = 0; w < C::kWarps; ++w) M = fmaxf(M, red[(w * C::kRedHeads + r) * C::kRedRow + D]);
+#pragma unroll 4
+        for (int w = 0; w < team; ++w) M = fmaxf(M, team_red[(w * C::kRedHeads + r) * C::kRedRow + D]);
         const float use = M == -INFINITY ? 0.f : M;
         float4 o4 = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < C::kWarps; ++w) {
-          const float* row = red + (w * C::kRedHeads + r) * C::kRedRow;
+#pragma unroll 4
+        for (int w = 0; w < team; ++w) {
+          const float* row = team_red + (w * C::kRedHeads + r) * C::kRedRow;
           const float2 ml = *reinterpret_cast<const float2*>(row + D);
           const float f = exp2f(ml.x - use);
           const float4 v = *reinterpret_cast<const float4*>(row + d);
@@ -560,26 +662,34 @@ __global__ void __launch_bounds__(Int4Cfg<D, GD>::kThreads, 1) paged_decode_int4
           if (d == 0) *reinterpret_cast<float2*>(a.ws_ml + (ws_row + h + r) * 2) = make_float2(M, L);
         }
       }
-      __syncthreads();
+      team_sync();
     }
 
-    // ---- a pair cut by ranges: the last CTA to arrive joins the partials in CTA order
+    // ---- a pair cut by ranges: the last team to arrive joins the partials in their order
     if (!whole) {
       const int pair0 = seg.pair_base();
-      // the CTAs with tiles of it
-      const int c0 = small ? split.first_cta : (pair0 + kPairCost) / chunk;
-      const int c1 = small ? split.last_cta : (pair0 + seg.units() - 1) / chunk;
-      if (tid == 0) {
-        unsigned int prev;
-        // after the barrier, so cumulative over the CTA's stores of its partial
-        asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(prev) : "l"(a.ws_count + c0) : "memory");
-        s_last = prev == (unsigned int)(c1 - c0);
-        if (s_last) a.ws_count[c0] = 0u;  // as the next call expects it
+      // the teams with tiles of it
+      const int c0 = small ? split.first_id : (pair0 + seg.cost) / chunk;
+      const int c1 = small ? split.last_id : (pair0 + seg.units() - 1) / chunk;
+      unsigned int last = 0;
+      if (lane_id < 32) {
+        if (lane_id == 0) {
+          unsigned int prev;
+          // after the barrier, so cumulative over the team's stores of its partial
+          asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(prev) : "l"(a.ws_count + c0) : "memory");
+          last = prev == (unsigned int)(c1 - c0);
+          if (last) a.ws_count[c0] = 0u;  // as the next call expects it
+        }
+        last = __shfl_sync(0xffffffffu, last, 0);
+        if (team > 1 && lane_id == 0) s_last[warp] = last;
       }
-      __syncthreads();
-      if (s_last) {
-        const int first_slot = small || c0 * chunk >= pair0 ? 0 : 1;  // of CTA c0; the others hold it as their first
-        for (int x = tid; x < heads * (D / 4); x += C::kThreads) {
+      if (team > 1) {
+        team_sync();
+        last = s_last[warp - rank];
+      }
+      if (last) {
+        const int first_slot = small || c0 * chunk >= pair0 ? 0 : 1;  // of team c0; the others hold it as their first
+        for (int x = lane_id; x < heads * (D / 4); x += threads) {
           const int r = x / (D / 4), d = x % (D / 4) * 4;
           float M = -INFINITY, L = 0.f;
           float4 o4 = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -593,7 +703,7 @@ __global__ void __launch_bounds__(Int4Cfg<D, GD>::kThreads, 1) paged_decode_int4
               s[k] = make_float2(-INFINITY, 0.f);
               v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
               if (c + k <= c1) {
-                const int64_t row = ((int64_t)(c + k) * 2 + (c + k == c0 ? first_slot : 0)) * kHeads + r;
+                const int64_t row = ((int64_t)(c + k) * 2 + (c + k == c0 ? first_slot : 0)) * a.part_heads + r;
                 s[k] = __ldcg(reinterpret_cast<const float2*>(a.ws_ml + row * 2));
                 v[k] = __ldcg(reinterpret_cast<const float4*>(a.ws_o + row * D + d));
               }
@@ -614,7 +724,7 @@ __global__ void __launch_bounds__(Int4Cfg<D, GD>::kThreads, 1) paged_decode_int4
           write_result<T>(a, seg.b, head0 + r, d, o4, M, L);
         }
       }
-      __syncthreads();  // s_last is free again
+      if (team > 1) team_sync();  // s_last is free again
     }
     first = false;
     if (!seg.next(a)) break;
@@ -623,13 +733,21 @@ __global__ void __launch_bounds__(Int4Cfg<D, GD>::kThreads, 1) paged_decode_int4
 
 // ------------------------------------------------------------------ host side
 
-// CTAs of a launch: as many as the SMs hold, or fewer where even full caches have fewer runs of kMinChunk tiles.
+constexpr int kMaxWarps = 16;
+
+int row_blocks_of(const aicas_paged_decode_int4_params* p) { return (p->num_q_heads / p->num_kv_heads + kHeads - 1) / kHeads; }
+
+// CTAs of a launch: as many as the SMs hold, or fewer where even full caches have fewer tiles for their warps.
 int decode_grid(const aicas_paged_decode_int4_params* p, int sms) {
   const int64_t cap_tiles = ((int64_t)p->max_pages * p->page_size + kTile - 1) / kTile;
-  const int blocks = (p->num_q_heads / p->num_kv_heads + kHeads - 1) / kHeads;
-  const int64_t pairs = (int64_t)p->batch * p->num_kv_heads * blocks;
-  const int64_t runs = (cap_tiles * pairs + kMinChunk - 1) / kMinChunk + pairs;
+  const int64_t pairs = (int64_t)p->batch * p->num_kv_heads * row_blocks_of(p);
+  const int64_t runs = (cap_tiles * pairs + kMaxWarps - 1) / kMaxWarps + pairs;
   return (int)(runs < sms ? runs : sms);
+}
+
+int part_heads_of(const aicas_paged_decode_int4_params* p) {
+  const int group = p->num_q_heads / p->num_kv_heads;
+  return group < kHeads ? group : kHeads;
 }
 
 template <typename T, int D, int GD, bool WIDE>
@@ -657,16 +775,31 @@ cudaError_t dispatch(int head_dim, int group_size, const Int4Args& a, int grid, 
 
 }  // namespace
 
-// The same for every call, so that a stream's buffer never has to grow for another shape.
-size_t paged_decode_int4_workspace(int sms) {
-  return kWsCounters + (size_t)sms * 2 * kHeads * (128 + 2) * sizeof(float);
+// Two partial results a team; the device makes teams no smaller than for all pairs.
+size_t paged_decode_int4_workspace(const aicas_paged_decode_int4_params* p, int sms) {
+  const int grid = decode_grid(p, sms);
+  const int64_t pairs = (int64_t)p->batch * p->num_kv_heads * row_blocks_of(p);
+  const int team = team_warps<kMaxWarps, kRanges>((int)(pairs < INT32_MAX ? pairs : INT32_MAX), grid);
+  return kWsCounters + (size_t)grid * (kMaxWarps / team) * 2 * part_heads_of(p) * (p->head_dim + 2) * sizeof(float);
 }
 
 int run_paged_decode_int4(const aicas_paged_decode_int4_params* p, int sms, void* workspace, cudaStream_t stream, char* err,
                           size_t errlen) {
+  const size_t workspace_bytes = paged_decode_int4_workspace(p, sms);
   Int4Args a;
   memset(&a, 0, sizeof(a));
-  a.kv[0] = p->kv[0], a.kv[1] = p->kv[1];
+  for (int i = 0; i < 2; ++i) {
+    const aicas_int4_pages& from = p->kv[i];
+    const int64_t pair = 2 * (p->head_dim / p->group_size);  // elements
+    const int64_t st[] = {from.cs_p / 16, from.cs_h / 16, from.cs_t / 16, from.ss_p / pair, from.ss_h / pair, from.ss_t / pair};
+    for (int64_t s : st)
+      if (s > (int64_t)UINT32_MAX) {
+        snprintf(err, errlen, "page strides of 64 GB or more are not supported");
+        return AICAS_ERR_UNSUPPORTED;
+      }
+    a.kv[i] = {static_cast<const uint8_t*>(from.codes), static_cast<const uint8_t*>(from.scales), (uint32_t)st[0], (uint32_t)st[1],
+               (uint32_t)st[2], (uint32_t)st[3], (uint32_t)st[4], (uint32_t)st[5]};
+  }
   a.q = p->q, a.out = p->out, a.lse = p->lse;
   a.table = p->page_table, a.lens = p->kv_lens, a.starts = p->kv_starts;
   a.q_sb = p->q_stride_b, a.q_sh = p->q_stride_h, a.o_sb = p->o_stride_b, a.o_sh = p->o_stride_h;
@@ -685,7 +818,8 @@ int run_paged_decode_int4(const aicas_paged_decode_int4_params* p, int sms, void
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   a.ws_count = reinterpret_cast<unsigned int*>(ws);
   a.ws_o = reinterpret_cast<float*>(ws + kWsCounters);
-  a.ws_ml = a.ws_o + (size_t)grid * 2 * kHeads * p->head_dim;
+  a.part_heads = part_heads_of(p);
+  a.ws_ml = a.ws_o + (workspace_bytes - kWsCounters) / sizeof(float) / (p->head_dim + 2) * p->head_dim;
   const cudaError_t e = p->dtype == AICAS_DTYPE_F16 ? dispatch<__half>(p->head_dim, p->group_size, a, grid, stream)
                                                     : dispatch<__nv_bfloat16>(p->head_dim, p->group_size, a, grid, stream);
   if (e == cudaSuccess) return AICAS_OK;
