@@ -68,6 +68,7 @@ struct Int4Args {
   uint32_t octets_mul;     // n / octets = (umulhi(n, octets_mul) + n) >> octets_shift
   int octets_shift;
   int few;                 // at most half as many pairs as CTAs
+  int dense;               // rows follow one another within a page and head, on both sides
   int part_heads;          // heads that a partial result has room for
   float scale_log2;
   float* ws_o;             // [2 * teams][part_heads][D]
@@ -95,22 +96,24 @@ struct Int4Cfg {
 
 using Seg = Segment<kTile>;
 
-// The 16-byte chunk where chunk c of row r is kept.  K's fragments take the same chunk of 8
-// rows, V's half of the chunks of 4 rows: both meet all banks once.
+// The 16-byte chunk where chunk c of row r is kept: the same chunk of 8 rows, which a
+// fragment load takes, lies in all banks once.
 template <int D>
 __device__ __forceinline__ int swizzled(int r, int c) {
-  if constexpr (D == 128) {
-    const int p = (r >> 1) & 3;  // 0, 1, 2, 3 -> 0, 2, 1, 3
-    return c ^ ((p >> 1) | ((p & 1) << 1));
-  } else {
-    return c ^ ((r >> 2) & 1);
-  }
+  return c ^ (D == 128 ? (r >> 1) & 3 : (r >> 2) & 1);
 }
 
-__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t r[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t r[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
 }
 
 template <int BYTES>
@@ -173,76 +176,94 @@ __device__ __forceinline__ float2 pair_of(uint32_t u) {
 
 // ------------------------------------------------------------------ copies
 
-// A warp's way through its tiles, ahead of the products.
+// A warp's way through its tiles, ahead of the products.  The pages of 8 of its tiles are
+// looked up at once, a lane an octet (8 rows) of slots, so that the page table's way and the
+// division are paid once for them.
 template <int D, int GD>
 struct Cursor {
   using C = Int4Cfg<D, GD>;
   Seg seg;
   int t;      // its next tile, in seg
   int turn;   // the warp that takes seg's first tile
-  bool more;
-  int page;   // page number and octet of the lane's 8 rows of that tile
-  int octet;
+  int known;  // tiles from t on whose pages are looked up; -1: no tile left
+  int page;   // of lane's octet lane % 4 of the tile lane / 4 of those 8: page number, -1: nothing to copy,
+  int row;    // and first row in the page
 
-  __device__ __forceinline__ void look(const Int4Args& a) {
+  __device__ __forceinline__ void look(const Int4Args& a, int team) {
     const int lane = threadIdx.x & 31;
-    page = -1;
-    if (!more) return;
-    const int n = (seg.first_tile + t) * (kTile / 8) + (lane >> 3);
+    const int n = (seg.first_tile + t + (lane >> 2) * team) * (kTile / 8) + (lane & 3);
     const int i = (int)((__umulhi((uint32_t)n, a.octets_mul) + (uint32_t)n) >> a.octets_shift);
-    octet = n - i * a.octets;
+    row = 8 * (n - i * a.octets);
+    page = -1;
     if (8 * n < seg.len && 8 * n + 8 > seg.start) page = a.table[seg.b * a.table_stride + i];
+    if (page >= a.num_pages) page = -1;
+    known = 8;
   }
 
   // To the warp's first tile at or after the segment.
   __device__ __forceinline__ void settle(const Int4Args& a, int rank, int team) {
     for (;;) {
       t = seg.t0 + ((rank - turn) & (team - 1));
-      if (t < seg.t1) break;
+      if (t < seg.t1) return look(a, team);
       turn = (turn + seg.t1 - seg.t0) & (team - 1);
       if (!seg.next(a)) {
-        more = false;
-        break;
+        known = -1;
+        return;
       }
     }
   }
 
   __device__ __forceinline__ void begin(const Int4Args& a, const Seg& first, int rank, int team) {
-    seg = first, turn = 0, more = true;
+    seg = first, turn = 0;
     settle(a, rank, team);
-    look(a);
+  }
+
+  template <bool DENSE>
+  __device__ __forceinline__ void rows(const Int4Args& a, uint32_t stage, int pg, int first_row) {
+    const int lane = threadIdx.x & 31, o = lane >> 3, sub = lane & 7;
+    const uint32_t head = a.row_blocks == 1 ? seg.pair : seg.pair / a.row_blocks;
+    const bool there = pg >= 0;
+    const uint32_t at = there ? pg : 0;
+    constexpr int kAtOnce = 8 / C::kChunks;  // rows of an octet in one go
+    const int r = sub / C::kChunks, c = sub % C::kChunks;
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      const Side& p = a.kv[side];
+      const uint64_t unit = (uint64_t)at * p.cs_p + (uint64_t)head * p.cs_h +
+                            (DENSE ? (uint64_t)(uint32_t)((first_row + r) * C::kChunks + c) : (uint64_t)(uint32_t)(first_row + r) * p.cs_t + c);
+      const uint8_t* codes = p.codes + 16 * unit;
+      const uint64_t step = DENSE ? kAtOnce * C::kRow : (uint64_t)p.cs_t * (16 * kAtOnce);
+      const uint32_t dst = stage + side * C::kOffV + (8 * o + r) * C::kRow;
+#pragma unroll
+      for (int k = 0; k < C::kChunks; ++k)
+        copy_async<16>(dst + kAtOnce * k * C::kRow + 16 * swizzled<D>(r + kAtOnce * k, c), codes + k * step, there);
+      const uint64_t pair = (uint64_t)at * p.ss_p + (uint64_t)head * p.ss_h +
+                            (DENSE ? (uint64_t)(uint32_t)(first_row + sub) : (uint64_t)(uint32_t)(first_row + sub) * p.ss_t);
+      copy_async<C::kPair>(stage + C::kOffPairs + (2 * lane + side) * C::kPair, p.pairs + C::kPair * pair, there);
+    }
   }
 
   // Asks for the tile and goes on to the next one.
   __device__ __forceinline__ void copy(const Int4Args& a, uint32_t stage, int rank, int team) {
-    if (more) {
-      const int lane = threadIdx.x & 31, o = lane >> 3, sub = lane & 7;
-      const uint32_t head = a.row_blocks == 1 ? seg.pair : seg.pair / a.row_blocks;
-      const bool there = page >= 0 && page < a.num_pages;
-      const uint32_t pg = there ? page : 0;
-      constexpr int kAtOnce = 8 / C::kChunks;  // rows of an octet in one go
-      const int r = sub / C::kChunks, c = sub % C::kChunks;
-#pragma unroll
-      for (int side = 0; side < 2; ++side) {
-        const Side& p = a.kv[side];
-        const uint8_t* codes = p.codes + 16 * ((uint64_t)pg * p.cs_p + (uint64_t)head * p.cs_h + (uint64_t)(uint32_t)(8 * octet + r) * p.cs_t + c);
-        const uint64_t step = (uint64_t)p.cs_t * (16 * kAtOnce);
-        const uint32_t dst = stage + side * C::kOffV + (8 * o + r) * C::kRow;
-#pragma unroll
-        for (int k = 0; k < C::kChunks; ++k)
-          copy_async<16>(dst + kAtOnce * k * C::kRow + 16 * swizzled<D>(r + kAtOnce * k, c), codes + k * step, there);
-        const uint8_t* pair = p.pairs + C::kPair * ((uint64_t)pg * p.ss_p + (uint64_t)head * p.ss_h + (uint64_t)(uint32_t)(8 * octet + sub) * p.ss_t);
-        copy_async<C::kPair>(stage + C::kOffPairs + (2 * lane + side) * C::kPair, pair, there);
-      }
+    if (known >= 0) {
+      const int from = 4 * (8 - known) + ((threadIdx.x & 31) >> 3);
+      const int pg = __shfl_sync(0xffffffffu, page, from), first_row = __shfl_sync(0xffffffffu, row, from);
+      if (a.dense)
+        rows<true>(a, stage, pg, first_row);
+      else
+        rows<false>(a, stage, pg, first_row);
       t += team;
       if (t >= seg.t1) {
         turn = (turn + seg.t1 - seg.t0) & (team - 1);
-        more = seg.next(a);
-        if (more) settle(a, rank, team);
+        if (seg.next(a))
+          settle(a, rank, team);
+        else
+          known = -1;
+      } else if (--known == 0) {
+        look(a, team);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
-    look(a);
   }
 };
 
@@ -250,17 +271,13 @@ struct Cursor {
 
 // WIDE: up to 8 heads, a column each, lo parts in products of their own; else up to 4
 // heads, head j's hi and lo parts in columns 2 j and 2 j + 1 of the same products.
-// A lane's heads: WIDE 2 i and 2 i + 1, else i; slots (rows g and g + 8 of a product) of
-// 16 are g / 2 + 4 (g % 2) and 8 more, an order that lets V's loads meet no bank twice.
-//
-// With one group a row (GD = 1) lane i takes the 32 dims of chunk i of K, lane g the 16 of
-// words 2 g and 2 g + 1 of V; with two, so that a product stays within a group, 8 dims of
-// each 32 and words g and g + 8.
+// A lane's heads: WIDE 2 i and 2 i + 1, else i; its slots of 16: rows g and g + 8 of a product.
+// K's fragments are words: lane i has 8 dims of each 32.  V's are 16-bit units of 4 dims,
+// paired over two slots by the transposing load: lane g has units g of each 32.
 template <typename T, int D, int GD, bool WIDE>
 struct Int4State {
   using C = Int4Cfg<D, GD>;
   static constexpr int kN = WIDE ? 2 : 1;  // heads a lane
-  static constexpr bool kWhole = GD == 1;
   static constexpr int kWords = D / 32;    // words of K a lane takes of a row: 8 dims each
   uint32_t q[kWords][4];  // of a word's dims (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16
   float fq[kN], qs[kN][GD];  // of the lane's heads: factor of q.code, sum of q, both with the softmax's scale
@@ -273,7 +290,15 @@ struct Int4State {
   // p stays below 2^kSlack: the reference is moved when a score passes it by more.
   static constexpr float kSlack = 4.f;
 
-  __device__ __forceinline__ static int dim_of(int i, int w) { return kWhole ? 8 * (kWords * i + w) : 32 * w + 8 * i; }
+  uint32_t k_off, v_off, p_off;  // this lane's places in a stage: rows of the fragment loads, pairs
+
+  __device__ __forceinline__ void init() {
+    const int lane = threadIdx.x & 31, mat = lane >> 3, r = lane & 7;
+    // K, D = 128: chunk mat of rows 0..7; D = 64: chunk mat / 2 of rows 0..7 and 8..15
+    k_off = D == 128 ? r * C::kRow + 16 * swizzled<D>(r, mat) : (r + 8 * (mat & 1)) * C::kRow + 16 * swizzled<D>(r, mat >> 1);
+    v_off = C::kOffV + (r + 8 * (mat & 1)) * C::kRow + 16 * swizzled<D>(r, mat >> 1);
+    p_off = C::kOffPairs + (lane >> 2) * 2 * C::kPair;
+  }
 
   __device__ __forceinline__ void begin(const Int4Args& a, const Seg& s) {
     const int lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3;
@@ -284,7 +309,7 @@ struct Int4State {
     const T* src = static_cast<const T*>(a.q) + s.b * a.q_sb + (int64_t)(kvh * a.group + h0 + min(col, heads - 1)) * a.q_sh;
 #pragma unroll
     for (int c = 0; c < kWords; ++c) {
-      Elem<T>::unpack(*reinterpret_cast<const uint4*>(src + dim_of(i, c)), x[c]);
+      Elem<T>::unpack(*reinterpret_cast<const uint4*>(src + 32 * c + 8 * i), x[c]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         top = fmaxf(top, fabsf(x[c][e]));
@@ -376,36 +401,31 @@ struct Int4State {
 
   // One tile at shared-memory address `at`; lo..hi: its slots in range.
   __device__ __forceinline__ void tile(uint32_t at, int lo, int hi) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3;
-    const int slot0 = (g >> 1) + 4 * (g & 1);
     float s[2][2][kN];  // [16 slots][row half][head], less ref
     float2 v[2][2][GD];  // scale and least of V
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
-      const int r = 16 * mt + slot0;  // row r + 8 has the same swizzle
       float acc[GD][4] = {};
-      uint32_t w0[kWords], w1[kWords];
-      if constexpr (kWhole) {
-        lds_words<kWords>(at + r * C::kRow + 4 * kWords * i, w0, slot0, i);
-        lds_words<kWords>(at + (r + 8) * C::kRow + 4 * kWords * i, w1, slot0, i);
+      uint32_t w[2][4];  // rows g and g + 8
+      if constexpr (D == 128) {
+        ldsm_x4(at + k_off + 16 * mt * C::kRow, w[0]);
+        ldsm_x4(at + k_off + (16 * mt + 8) * C::kRow, w[1]);
       } else {
-#pragma unroll
-        for (int c = 0; c < kWords; ++c) {
-          const uint32_t from = at + r * C::kRow + 16 * swizzled<D>(slot0, c) + 4 * i;
-          w0[c] = lds32(from), w1[c] = lds32(from + 8 * C::kRow);
-        }
+        uint32_t u[4];
+        ldsm_x4(at + k_off + 16 * mt * C::kRow, u);
+        w[0][0] = u[0], w[1][0] = u[1], w[0][1] = u[2], w[1][1] = u[3];
       }
 #pragma unroll
       for (int c = 0; c < kWords; ++c) {
         float* t = acc[c * GD / kWords];
-        mma(t, w0[c] & 0x000f000fu, w1[c] & 0x000f000fu, w0[c] & 0x00f000f0u, w1[c] & 0x00f000f0u, q[c][0], q[c][1]);
-        const uint32_t u0 = w0[c] >> 8, u1 = w1[c] >> 8;
+        const uint32_t w0 = w[0][c], w1 = w[1][c], u0 = w0 >> 8, u1 = w1 >> 8;
+        mma(t, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, q[c][0], q[c][1]);
         mma(t, u0 & 0x000f000fu, u1 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x00f000f0u, q[c][2], q[c][3]);
       }
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         uint32_t kp[GD], vp[GD];
-        lds_pairs(at + C::kOffPairs + (r + 8 * half) * 2 * C::kPair, kp, vp);
+        lds_pairs(at + p_off + (16 * mt + 8 * half) * 2 * C::kPair, kp, vp);
 #pragma unroll
         for (int n = 0; n < kN; ++n) s[mt][half][n] = -ref[n];
 #pragma unroll
@@ -423,7 +443,7 @@ struct Int4State {
       for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          const int r = 16 * mt + 8 * half + slot0;
+          const int r = 16 * mt + 8 * half + ((threadIdx.x & 31) >> 2);
           if (r >= lo && r < hi) continue;
 #pragma unroll
           for (int n = 0; n < kN; ++n) s[mt][half][n] = -INFINITY;
@@ -471,45 +491,21 @@ struct Int4State {
           ph[e][1] = transposed(__byte_perm(h, lw, 0x7632));
         }
       }
-      uint32_t w[4][D / 64];  // the lane's words of slots i, i + 4, i + 8, i + 12
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int r = 16 * mt + 4 * k + i;
-        const uint32_t row = at + C::kOffV + r * C::kRow;
-        if constexpr (kWhole && D == 128) {
-          asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[k][0]), "=r"(w[k][1])
-                       : "r"(row + 16 * swizzled<D>(4 * k + i, g >> 1) + 8 * (g & 1)) : "memory");
-        } else {
-#pragma unroll
-          for (int half = 0; half < D / 64; ++half)
-            w[k][half] = lds32(row + 16 * swizzled<D>(4 * k + i, 2 * half + (g >> 2)) + 4 * (g & 3));
-        }
-      }
-#pragma unroll
-      for (int half = 0; half < D / 64; ++half) {
-        const int e = GD == 2 ? half : 0;
-        uint32_t a0 = __byte_perm(w[0][half], w[1][half], 0x5410), a1 = __byte_perm(w[0][half], w[1][half], 0x7632);  // dims 0..3, 4..7 of the word
-        uint32_t a2 = __byte_perm(w[2][half], w[3][half], 0x5410), a3 = __byte_perm(w[2][half], w[3][half], 0x7632);
+      for (int cp = 0; cp < D / 64; ++cp) {  // 64 dims: units of chunks 2 cp (rows 0..7 of the products) and 2 cp + 1
+        const int e = GD == 2 ? cp : 0;
+        uint32_t w[4];  // chunk 2 cp: slots 0..7, 8..15; chunk 2 cp + 1: the same
+        ldsm_x4_t(at + (v_off ^ (32 * cp)) + 16 * mt * C::kRow, w);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           const uint32_t mask = t & 1 ? 0x00f000f0u : 0x000f000fu;
-          mma(o[4 * half + t], a0 & mask, a1 & mask, a2 & mask, a3 & mask, ph[e][0], ph[e][1]);
-          if constexpr (WIDE) mma(o[4 * half + t], a0 & mask, a1 & mask, a2 & mask, a3 & mask, pl[e][0], pl[e][1]);
-          if (t == 1) a0 >>= 8, a1 >>= 8, a2 >>= 8, a3 >>= 8;
+          mma(o[4 * cp + t], w[0] & mask, w[2] & mask, w[1] & mask, w[3] & mask, ph[e][0], ph[e][1]);
+          if constexpr (WIDE) mma(o[4 * cp + t], w[0] & mask, w[2] & mask, w[1] & mask, w[3] & mask, pl[e][0], pl[e][1]);
+          if (t == 1)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[k] >>= 8;
         }
       }
-    }
-  }
-
-  // The words of chunk i of row `slot0` of 16.
-  template <int N>
-  __device__ __forceinline__ static void lds_words(uint32_t from, uint32_t* w, int slot0, int i) {
-    if constexpr (N == 4) {
-      const uint32_t addr = from + 16 * (swizzled<D>(slot0, i) - i);
-      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr) : "memory");
-    } else {  // half a chunk
-      const uint32_t addr = from + 16 * (swizzled<D>(slot0, i >> 1) - (i >> 1));
-      asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr) : "memory");
     }
   }
 
@@ -541,13 +537,17 @@ struct Int4State {
       if (h < h0 || h >= h0 + C::kRedHeads) continue;
       float* row = red + (h - h0) * C::kRedRow;
 #pragma unroll
-      for (int t = 0; t < D / 16; ++t) {
-        const float by = t & 1 ? unit * 0.0625f : unit;
-        const int d = kWhole && D == 128 ? 16 * g + 8 * (t / 4) + t % 4 : 64 * (t / 4) + 8 * g + t % 4;
-        const float x = WIDE ? o[t][n] : o[t][0] + o[t][1], y = WIDE ? o[t][2 + n] : o[t][2] + o[t][3];
-        row[d] = fmaf(x, by, least[GD == 2 ? t / 4 : 0]);
-        row[d + 4] = fmaf(y, by, least[GD == 2 ? t / 4 : 0]);
-      }
+      for (int cp = 0; cp < D / 64; ++cp)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float x[4];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const float* c = o[4 * cp + t] + 2 * half;
+            x[t] = fmaf(WIDE ? c[n] : c[0] + c[1], t & 1 ? unit * 0.0625f : unit, least[GD == 2 ? cp : 0]);
+          }
+          *reinterpret_cast<float4*>(row + 64 * cp + 32 * half + 4 * g) = make_float4(x[0], x[1], x[2], x[3]);
+        }
       if (g == 0) *reinterpret_cast<float2*>(row + D) = make_float2(bound < 0.f ? -INFINITY : ref[n], sum);
     }
   }
@@ -609,6 +609,7 @@ __global__ void __launch_bounds__(Int4Cfg<D, GD>::kThreads, 1) paged_decode_int4
   const bool small = split.small;
   float* const team_red = red + (warp - rank) * C::kRedHeads * C::kRedRow;
   Int4State<T, D, GD, WIDE> st;
+  st.init();
   int stage = 0, turn = 0;  // turn: the warp that takes the segment's first tile
   for (bool first = true;;) {
     if (seg.t0 == seg.t1) {
@@ -813,6 +814,8 @@ int run_paged_decode_int4(const aicas_paged_decode_int4_params* p, int sms, void
   while ((1ll << a.octets_shift) < a.octets) ++a.octets_shift;
   a.octets_mul = (uint32_t)((((1ull << a.octets_shift) - a.octets) << 32) / a.octets + 1);
   a.scale_log2 = p->sm_scale * 1.4426950408889634f;
+  a.dense = 1;
+  for (const Side& x : a.kv) a.dense &= x.cs_t == (uint32_t)p->head_dim / 32 && x.ss_t == 1;
   const int grid = decode_grid(p, sms);
   a.few = 2 * (int64_t)a.batch * a.hkv * a.row_blocks <= grid;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
