@@ -39,7 +39,7 @@ namespace {
 
 constexpr int kTile = 32;      // slots a tile
 constexpr int kRanges = 6;     // ranges that a pair is cut into, about
-constexpr int kPairCost = 2;   // what beginning and ending a pair costs a warp, in tiles
+constexpr int kPairCost = 4;   // what beginning and ending a pair costs a warp, in tiles
 constexpr int kLeast = 1;      // fewest tiles a warp takes
 constexpr int kSmallTiles = 16;  // most tiles a CTA of a launch that gives pairs whole CTAs
 constexpr int kHeads = 8;      // query heads of a block
@@ -85,7 +85,7 @@ struct Int4Cfg {
   static constexpr int kOffPairs = 2 * kTile * kRow;  // a slot's pairs of K, then of V
   static constexpr int kStage = kOffPairs + 2 * kTile * kPair;
   static constexpr int kWarps = 16, kThreads = kWarps * 32;
-  static constexpr int kStages = GD == 1 ? 3 : 2;
+  static constexpr int kStages = 2;
   static constexpr int kRedHeads = 2;         // heads that the warps' states are joined of at a time
   static constexpr int kRedRow = D + 4;
   static constexpr int kOffRed = kWarps * kStages * kStage;
