@@ -38,10 +38,11 @@ namespace aicas {
 namespace {
 
 constexpr int kTile = 32;      // slots a tile
-constexpr int kRanges = 6;     // ranges that a pair is cut into, about
-constexpr int kPairCost = 4;   // what beginning and ending a pair costs a warp, in tiles
-constexpr int kLeast = 1;      // fewest tiles a warp takes
-constexpr int kSmallTiles = 16;  // most tiles a CTA of a launch that gives pairs whole CTAs
+constexpr int kRanges = 4;     // ranges that a pair is cut into, about
+constexpr int kPairCost = 3;   // what beginning and ending a pair costs a warp, in tiles
+constexpr int kSmallTiles = 32;  // most tiles a CTA of a launch that gives pairs whole CTAs
+constexpr int kLogWarps = 4, kMaxWarps = 1 << kLogWarps;
+constexpr int kSmallLog = 2;   // warps of a team in a small launch
 constexpr int kHeads = 8;      // query heads of a block
 constexpr size_t kWsCounters = (size_t)1 << 20;  // counter region shared with the other decode kernels
 constexpr float kCodeUnit = 16777216.f;  // 2^24: a code in an fp16's low bits is code / kCodeUnit
@@ -84,12 +85,11 @@ struct Int4Cfg {
   static constexpr int kOffV = kTile * kRow;
   static constexpr int kOffPairs = 2 * kTile * kRow;  // a slot's pairs of K, then of V
   static constexpr int kStage = kOffPairs + 2 * kTile * kPair;
-  static constexpr int kWarps = 16, kThreads = kWarps * 32;
+  static constexpr int kWarps = kMaxWarps, kThreads = kWarps * 32;
   static constexpr int kStages = 2;
-  static constexpr int kRedHeads = 2;         // heads that the warps' states are joined of at a time
   static constexpr int kRedRow = D + 4;
   static constexpr int kOffRed = kWarps * kStages * kStage;
-  static constexpr int kOffVars = kOffRed + kWarps * kRedHeads * kRedRow * 4;
+  static constexpr int kOffVars = kOffRed + kWarps * kHeads * kRedRow * 4;
   static constexpr int kSmem = kOffVars + 4 * kWarps;
   static_assert(kSmem <= 232448, "shared memory");
 };
@@ -300,16 +300,23 @@ struct Int4State {
     p_off = C::kOffPairs + (lane >> 2) * 2 * C::kPair;
   }
 
-  __device__ __forceinline__ void begin(const Int4Args& a, const Seg& s) {
+  // Asks for the query heads of a segment's pair.
+  __device__ __forceinline__ static void ask(const Int4Args& a, const Seg& s, uint4 (&raw)[kWords]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3;
     const int kvh = s.pair / a.row_blocks, h0 = (s.pair - kvh * a.row_blocks) * kHeads;
     const int heads = min(kHeads, a.group - h0);
     const int col = WIDE ? g : g >> 1;  // the head of column g
-    float x[kWords][8], top = 0.f, sum[GD] = {};
     const T* src = static_cast<const T*>(a.q) + s.b * a.q_sb + (int64_t)(kvh * a.group + h0 + min(col, heads - 1)) * a.q_sh;
 #pragma unroll
+    for (int c = 0; c < kWords; ++c) raw[c] = *reinterpret_cast<const uint4*>(src + 32 * c + 8 * i);
+  }
+
+  __device__ __forceinline__ void begin(const Int4Args& a, const uint4 (&raw)[kWords]) {
+    const int i = threadIdx.x & 3;
+    float x[kWords][8], top = 0.f, sum[GD] = {};
+#pragma unroll
     for (int c = 0; c < kWords; ++c) {
-      Elem<T>::unpack(*reinterpret_cast<const uint4*>(src + 32 * c + 8 * i), x[c]);
+      Elem<T>::unpack(raw[c], x[c]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         top = fmaxf(top, fabsf(x[c][e]));
@@ -383,7 +390,7 @@ struct Int4State {
       // scores are less the old reference; the first tile sets it, down too
       const float up = mt == -INFINITY ? 0.f : first ? mt : fmaxf(mt, 0.f);
       ref[n] += up;
-      const float alpha = exp2f(-up);
+      const float alpha = exp2_fast(-up);
       l[n] *= alpha;
 #pragma unroll
       for (int e = 0; e < GD; ++e) z[n][e] *= alpha;
@@ -518,8 +525,8 @@ struct Int4State {
     }
   }
 
-  // Heads h0, h0 + 1 of the block into this warp's part of the reduction buffer.
-  __device__ __forceinline__ void put(int h0, float* red) {
+  // The block's heads into this warp's part of the reduction buffer.
+  __device__ __forceinline__ void put(int heads, float* red) {
     const int lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3;
     const float unit = lift == 0.f ? 0.f : kCodeUnit / lift;
 #pragma unroll
@@ -534,8 +541,8 @@ struct Int4State {
 #pragma unroll
         for (int e = 0; e < GD; ++e) least[e] += __shfl_xor_sync(0xffffffffu, least[e], off);
       }
-      if (h < h0 || h >= h0 + C::kRedHeads) continue;
-      float* row = red + (h - h0) * C::kRedRow;
+      if (h >= heads) continue;
+      float* row = red + h * C::kRedRow;
 #pragma unroll
       for (int cp = 0; cp < D / 64; ++cp)
 #pragma unroll
@@ -578,18 +585,21 @@ __global__ void __launch_bounds__(Int4Cfg<D, GD>::kThreads, 1) paged_decode_int4
   grid_launch_dependents();
   grid_dependency_wait();
   Split<kTile> split = {};
-  split.template find<C::kWarps, kRanges, kLeast, kPairCost, kSmallTiles>(a);
-  const int team = split.team, rank = warp & (team - 1), threads = 32 * team, lane_id = tid & (threads - 1);
+  split.template find<kLogWarps, kSmallLog, kRanges, kPairCost, kSmallTiles>(a);
+  const int team = 1 << split.log, rank = warp & (team - 1), threads = 32 * team, lane_id = tid & (threads - 1);
   const auto team_sync = [&] {
     if (team == 1) {
       __syncwarp();
     } else {
-      asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / team), "r"(threads) : "memory");
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + (warp >> split.log)), "r"(threads) : "memory");
     }
   };
   const uint32_t ring = smem_u32(smem) + warp * C::kStages * C::kStage;
+  using State = Int4State<T, D, GD, WIDE>;
+  uint4 raw[State::kWords];
   Cursor<D, GD> ahead;
   if (split.busy) {
+    State::ask(a, split.seg, raw);  // on its way while the tiles are asked for
     ahead.begin(a, split.seg, rank, team);
 #pragma unroll
     for (int k = 0; k < C::kStages; ++k) ahead.copy(a, ring + k * C::kStage, rank, team);
@@ -607,16 +617,17 @@ __global__ void __launch_bounds__(Int4Cfg<D, GD>::kThreads, 1) paged_decode_int4
   Seg seg = split.seg;
   const int chunk = split.chunk;
   const bool small = split.small;
-  float* const team_red = red + (warp - rank) * C::kRedHeads * C::kRedRow;
-  Int4State<T, D, GD, WIDE> st;
+  float* const team_red = red + (warp - rank) * kHeads * C::kRedRow;
+  State st;
   st.init();
   int stage = 0, turn = 0;  // turn: the warp that takes the segment's first tile
   for (bool first = true;;) {
     if (seg.t0 == seg.t1) {
       if (!seg.next(a)) break;
+      State::ask(a, seg, raw);
       continue;
     }
-    st.begin(a, seg);
+    st.begin(a, raw);
 #pragma unroll 1
     for (int t = seg.t0 + ((rank - turn) & (team - 1)); t < seg.t1; t += team) {
       asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 1) : "memory");
@@ -636,42 +647,40 @@ __global__ void __launch_bounds__(Int4Cfg<D, GD>::kThreads, 1) paged_decode_int4
     const bool whole = seg.t0 == 0 && seg.t1 == seg.nt;
     // a pair that starts inside this range is its last: slot 1, unless it is the first, too
     const int64_t ws_row = ((int64_t)split.id * 2 + (first ? 0 : 1)) * a.part_heads;
-    for (int h = 0; h < heads; h += C::kRedHeads) {
-      st.put(h, red + warp * C::kRedHeads * C::kRedRow);
-      team_sync();
-      for (int x = lane_id; x < min(C::kRedHeads, heads - h) * (D / 4); x += threads) {
-        const int r = x / (D / 4), d = x % (D / 4) * 4;
-        float M = -INFINITY, L = 0.f;
+    st.put(heads, red + warp * kHeads * C::kRedRow);
+    team_sync();
+    for (int x = lane_id; x < heads * (D / 4); x += threads) {
+      const int r = x / (D / 4), d = x % (D / 4) * 4;
+      float M = -INFINITY, L = 0.f;
 #pragma unroll 4
-        for (int w = 0; w < team; ++w) M = fmaxf(M, team_red[(w * C::kRedHeads + r) * C::kRedRow + D]);
-        const float use = M == -INFINITY ? 0.f : M;
-        float4 o4 = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int w = 0; w < team; ++w) M = fmaxf(M, team_red[(w * kHeads + r) * C::kRedRow + D]);
+      const float use = M == -INFINITY ? 0.f : M;
+      float4 o4 = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-        for (int w = 0; w < team; ++w) {
-          const float* row = team_red + (w * C::kRedHeads + r) * C::kRedRow;
-          const float2 ml = *reinterpret_cast<const float2*>(row + D);
-          const float f = exp2f(ml.x - use);
-          const float4 v = *reinterpret_cast<const float4*>(row + d);
-          L = fmaf(f, ml.y, L);
-          o4.x = fmaf(f, v.x, o4.x), o4.y = fmaf(f, v.y, o4.y);
-          o4.z = fmaf(f, v.z, o4.z), o4.w = fmaf(f, v.w, o4.w);
-        }
-        if (whole) {
-          write_result<T>(a, seg.b, head0 + h + r, d, o4, M, L);
-        } else {
-          *reinterpret_cast<float4*>(a.ws_o + (ws_row + h + r) * D + d) = o4;
-          if (d == 0) *reinterpret_cast<float2*>(a.ws_ml + (ws_row + h + r) * 2) = make_float2(M, L);
-        }
+      for (int w = 0; w < team; ++w) {
+        const float* row = team_red + (w * kHeads + r) * C::kRedRow;
+        const float2 ml = *reinterpret_cast<const float2*>(row + D);
+        const float f = exp2_fast(ml.x - use);
+        const float4 v = *reinterpret_cast<const float4*>(row + d);
+        L = fmaf(f, ml.y, L);
+        o4.x = fmaf(f, v.x, o4.x), o4.y = fmaf(f, v.y, o4.y);
+        o4.z = fmaf(f, v.z, o4.z), o4.w = fmaf(f, v.w, o4.w);
       }
-      team_sync();
+      if (whole) {
+        write_result<T>(a, seg.b, head0 + r, d, o4, M, L);
+      } else {
+        *reinterpret_cast<float4*>(a.ws_o + (ws_row + r) * D + d) = o4;
+        if (d == 0) *reinterpret_cast<float2*>(a.ws_ml + (ws_row + r) * 2) = make_float2(M, L);
+      }
     }
+    team_sync();
 
     // ---- a pair cut by ranges: the last team to arrive joins the partials in their order
     if (!whole) {
       const int pair0 = seg.pair_base();
       // the teams with tiles of it
-      const int c0 = small ? split.first_id : (pair0 + seg.cost) / chunk;
-      const int c1 = small ? split.last_id : (pair0 + seg.units() - 1) / chunk;
+      const int c0 = small ? split.first_id : (int)((uint32_t)(pair0 + seg.cost) / (uint32_t)chunk);
+      const int c1 = small ? split.last_id : (int)((uint32_t)(pair0 + seg.units() - 1) / (uint32_t)chunk);
       unsigned int last = 0;
       if (lane_id < 32) {
         if (lane_id == 0) {
@@ -694,7 +703,7 @@ __global__ void __launch_bounds__(Int4Cfg<D, GD>::kThreads, 1) paged_decode_int4
           const int r = x / (D / 4), d = x % (D / 4) * 4;
           float M = -INFINITY, L = 0.f;
           float4 o4 = make_float4(0.f, 0.f, 0.f, 0.f);
-          constexpr int kMany = 8;  // partials in flight
+          constexpr int kMany = 4;  // partials in flight
           for (int c = c0; c <= c1; c += kMany) {
             float2 s[kMany];
             float4 v[kMany];
@@ -711,11 +720,11 @@ __global__ void __launch_bounds__(Int4Cfg<D, GD>::kThreads, 1) paged_decode_int4
             }
 #pragma unroll
             for (int k = 0; k < kMany; ++k) Mn = fmaxf(Mn, s[k].x);
-            const float use = Mn == -INFINITY ? 0.f : Mn, old = exp2f(M - use);
+            const float use = Mn == -INFINITY ? 0.f : Mn, old = exp2_fast(M - use);
             L *= old, o4.x *= old, o4.y *= old, o4.z *= old, o4.w *= old;
 #pragma unroll
             for (int k = 0; k < kMany; ++k) {
-              const float f = exp2f(s[k].x - use);
+              const float f = exp2_fast(s[k].x - use);
               L = fmaf(f, s[k].y, L);
               o4.x = fmaf(f, v[k].x, o4.x), o4.y = fmaf(f, v[k].y, o4.y);
               o4.z = fmaf(f, v[k].z, o4.z), o4.w = fmaf(f, v[k].w, o4.w);
@@ -729,12 +738,11 @@ __global__ void __launch_bounds__(Int4Cfg<D, GD>::kThreads, 1) paged_decode_int4
     }
     first = false;
     if (!seg.next(a)) break;
+    State::ask(a, seg, raw);
   }
 }
 
 // ------------------------------------------------------------------ host side
-
-constexpr int kMaxWarps = 16;
 
 int row_blocks_of(const aicas_paged_decode_int4_params* p) { return (p->num_q_heads / p->num_kv_heads + kHeads - 1) / kHeads; }
 
@@ -742,7 +750,7 @@ int row_blocks_of(const aicas_paged_decode_int4_params* p) { return (p->num_q_he
 int decode_grid(const aicas_paged_decode_int4_params* p, int sms) {
   const int64_t cap_tiles = ((int64_t)p->max_pages * p->page_size + kTile - 1) / kTile;
   const int64_t pairs = (int64_t)p->batch * p->num_kv_heads * row_blocks_of(p);
-  const int64_t runs = (cap_tiles * pairs + kMaxWarps - 1) / kMaxWarps + pairs;
+  const int64_t runs = (cap_tiles * pairs + (1 << kSmallLog) - 1) / (1 << kSmallLog) + pairs;
   return (int)(runs < sms ? runs : sms);
 }
 
@@ -780,8 +788,9 @@ cudaError_t dispatch(int head_dim, int group_size, const Int4Args& a, int grid, 
 size_t paged_decode_int4_workspace(const aicas_paged_decode_int4_params* p, int sms) {
   const int grid = decode_grid(p, sms);
   const int64_t pairs = (int64_t)p->batch * p->num_kv_heads * row_blocks_of(p);
-  const int team = team_warps<kMaxWarps, kRanges>((int)(pairs < INT32_MAX ? pairs : INT32_MAX), grid);
-  return kWsCounters + (size_t)grid * (kMaxWarps / team) * 2 * part_heads_of(p) * (p->head_dim + 2) * sizeof(float);
+  const int least = team_log<kLogWarps, kRanges>((int)(pairs < INT32_MAX ? pairs : INT32_MAX), grid);
+  const int log = least < kSmallLog ? least : kSmallLog;
+  return kWsCounters + ((size_t)grid << (kLogWarps - log)) * 2 * part_heads_of(p) * (p->head_dim + 2) * sizeof(float);
 }
 
 int run_paged_decode_int4(const aicas_paged_decode_int4_params* p, int sms, void* workspace, cudaStream_t stream, char* err,

@@ -21,7 +21,7 @@ template <int TILE, typename A>
 __device__ __forceinline__ void request_bounds(const A& a, int b, int& start, int& len, int& nt) {
   len = a.lens != nullptr ? min(max(a.lens[b], 0), a.cap) : a.cap;
   start = a.starts != nullptr ? min(max(a.starts[b], 0), len) : 0;
-  nt = len > start ? (len + TILE - 1) / TILE - start / TILE : 0;
+  nt = len > start ? (int)((uint32_t)(len + TILE - 1) / TILE - (uint32_t)start / TILE) : 0;
 }
 
 // The tiles [t0, t1) of one pair in a team's range; none where the range ends in the pair's
@@ -47,16 +47,6 @@ struct Segment {
     t1 = max(0, to - cost);
   }
 
-  // From unit `unit` of the launch, which lies in request b.
-  template <typename A>
-  __device__ __forceinline__ void at(const A& a, int unit, int count) {
-    request_bounds<TILE>(a, b, start, len, nt);
-    first_tile = start / TILE;
-    const int off = unit - base;
-    pair = off / units();
-    take(off - pair * units(), count);
-  }
-
   template <typename A>
   __device__ __forceinline__ bool next(const A& a) {
     if (left == 0) return false;
@@ -67,105 +57,115 @@ struct Segment {
         ++b;  // units are left, so a request with some follows
         request_bounds<TILE>(a, b, start, len, nt);
       } while (nt == 0);
-      first_tile = start / TILE;
+      first_tile = (uint32_t)start / TILE;
     }
     take(0, left);
     return true;
   }
 };
 
-// Warps of a team for so many pairs: the least that leaves a pair about RANGES ranges.
-template <int WARPS, int RANGES>
-__host__ __device__ __forceinline__ int team_warps(int pairs, int ctas) {
-  int team = 1;
-  while (team < WARPS && (int64_t)pairs * RANGES * team < (int64_t)ctas * WARPS) team *= 2;
-  return team;
+// Warps of a team, as a power of two, for so many pairs: the least that leaves a pair about RANGES ranges.
+template <int LOG_WARPS, int RANGES>
+__host__ __device__ __forceinline__ int team_log(int pairs, int ctas) {
+  int log = 0;
+#pragma unroll
+  for (int k = 0; k < LOG_WARPS; ++k) log += (int64_t)pairs * RANGES << k < (int64_t)ctas << LOG_WARPS;
+  return log;
 }
 
 // A team's place in the launch.  Small launches of few pairs (a.few, and at most MOST tiles
-// a CTA) give each pair whole CTAs, as short as WARPS tiles allow: latency; the others
-// equal ranges: bandwidth.
+// a CTA) give each pair whole teams, as short as the warps' tiles allow, of 1 << SMALL warps
+// where that leaves each team a CTA: latency; the others equal ranges: bandwidth.
 template <int TILE>
 struct Split {
   bool small, busy, empty_rows;  // empty_rows: some request has no slot
-  int team;                      // warps of a team, a power of two
+  int log;                       // warps of a team: 1 << log
   int id;                        // this team's number
   int chunk;                     // units of a range; small: its tiles
   int first_id, last_id;         // small: the teams of this team's pair
   Segment<TILE> seg;             // this team's first, if it is busy
 
-  // Every warp for itself: a run of requests a lane.  LEAST: fewest tiles a warp; COST: a pair's, for each warp of a team.
-  template <int WARPS, int RANGES, int LEAST, int COST, int MOST, typename A>
+  // Every warp for itself, a run of requests a lane.  The chain of a launch of few
+  // tiles, so loads and divisions are few.  COST: a pair's, for each warp of a team.
+  template <int LOG_WARPS, int SMALL, int RANGES, int COST, int MOST, typename A>
   __device__ __forceinline__ void find(const A& a) {
-    const int lane = threadIdx.x & 31, per = a.hkv * a.row_blocks, pairs = a.batch * per;
-    const int run = (a.batch + 31) / 32, b0 = min(a.batch, lane * run), b1 = min(a.batch, b0 + run);
-    int tiles = 0, full_pairs = 0;
-#pragma unroll 4
-    for (int b = b0; b < b1; ++b) {
-      int start, len, nt;
-      request_bounds<TILE>(a, b, start, len, nt);
-      tiles += nt * per;
-      full_pairs += nt > 0 ? per : 0;
+    const int lane = threadIdx.x & 31, per = a.hkv * a.row_blocks;
+    const int run = (a.batch + 31) >> 5, b0 = min(a.batch, lane * run), b1 = min(a.batch, b0 + run);
+    int start = 0, len = 0, nt0 = 0;  // of the lane's first request
+    if (b0 < b1) request_bounds<TILE>(a, b0, start, len, nt0);
+    int tiles = nt0, full = nt0 > 0;
+    for (int b = b0 + 1; b < b1; ++b) {
+      int st, ln, nt;
+      request_bounds<TILE>(a, b, st, ln, nt);
+      tiles += nt;
+      full += nt > 0;
     }
-    tiles = __reduce_add_sync(0xffffffffu, tiles);
-    full_pairs = __reduce_add_sync(0xffffffffu, full_pairs);
-    empty_rows = full_pairs < pairs;
-    small = a.few && tiles <= (int)gridDim.x * MOST;
-    team = small ? WARPS : team_warps<WARPS, RANGES>(full_pairs, (int)gridDim.x);
-    const int teams = (int)gridDim.x * (WARPS / team);
-    id = (int)blockIdx.x * (WARPS / team) + (int)(threadIdx.x >> 5) / team;
-    const int ranges = teams - (small ? pairs : 0);  // small: at most tiles / chunk + pairs are needed
-    const int cost = small ? 0 : COST * team;
-    const int units = tiles + full_pairs * cost;
-    chunk = max((units + ranges - 1) / ranges, LEAST * team);
-    if (small) chunk = (chunk + WARPS - 1) / WARPS * WARPS;
-    // what a request counts: units, or (small) teams
+    tiles = __reduce_add_sync(0xffffffffu, tiles) * per;
+    full = __reduce_add_sync(0xffffffffu, full);
+    empty_rows = full < a.batch;
+    full *= per;
+    const int grid = (int)gridDim.x;
+    small = a.few && tiles <= grid * MOST;
+    log = small ? (tiles <= grid << SMALL ? SMALL : LOG_WARPS) : team_log<LOG_WARPS, RANGES>(full, grid);
+    const int teams = grid << (LOG_WARPS - log);
+    const int of_cta = (int)(threadIdx.x >> (5 + log));
+    id = small ? (int)blockIdx.x + grid * of_cta : (int)(blockIdx.x << (LOG_WARPS - log)) + of_cta;
+    const int ranges = teams - (small ? a.batch * per : 0);  // small: at most tiles / chunk + pairs are needed
+    const int cost = small ? 0 : COST << log;
+    const uint32_t units = (uint32_t)(tiles + full * cost);
+    chunk = max((int)((units + ranges - 1) / (uint32_t)ranges), 1 << log);
+    if (small) chunk = (chunk + (1 << log) - 1) & -(1 << log);
+    const float inv = 1.f / (float)chunk;
+    // what a request counts: units, or (small; numbers below 2^16, so the quotient is exact) teams
     const auto share = [&](int nt) {
-      return small ? (nt + chunk - 1) / chunk * per : nt == 0 ? 0 : (nt + cost) * per;
+      return small ? (int)(((float)(nt + chunk - 1) + 0.5f) * inv) * per : nt == 0 ? 0 : (nt + cost) * per;
     };
-    int mine = 0;
-    for (int b = b0; b < b1; ++b) {
-      int start, len, nt;
-      request_bounds<TILE>(a, b, start, len, nt);
+    int mine = b0 < b1 ? share(nt0) : 0;
+    for (int b = b0 + 1; b < b1; ++b) {
+      int st, ln, nt;
+      request_bounds<TILE>(a, b, st, ln, nt);
       mine += share(nt);
     }
     int before = mine;
+    if (a.batch > 1)
 #pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, before, off);
-      if (lane >= off) before += v;
-    }
-    const int total = __shfl_sync(0xffffffffu, before, 31);
+      for (int off = 1; off < 32; off <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, before, off);
+        if (lane >= off) before += v;
+      }
+    const int total = __shfl_sync(0xffffffffu, before, 31 < a.batch - 1 ? 31 : a.batch - 1);
     before -= mine;
     const int64_t r64 = small ? (int64_t)id : (int64_t)id * chunk;
     busy = r64 < total;
     if (!busy) return;
     const int r0 = (int)r64;
-    int b = 0, at = before;
+    int b = b0, at = before, nt = nt0;
     const bool here = r0 >= before && r0 < before + mine;
     if (here)
-      for (b = b0;; ++b) {
-        int start, len, nt;
-        request_bounds<TILE>(a, b, start, len, nt);
-        if (r0 < at + share(nt)) break;
+      while (r0 >= at + share(nt)) {
         at += share(nt);
+        request_bounds<TILE>(a, ++b, start, len, nt);
       }
     const int src = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
     seg.b = __shfl_sync(0xffffffffu, b, src);
     seg.base = __shfl_sync(0xffffffffu, at, src);
+    seg.start = __shfl_sync(0xffffffffu, start, src);
+    seg.len = __shfl_sync(0xffffffffu, len, src);
+    seg.nt = __shfl_sync(0xffffffffu, nt, src);
+    seg.first_tile = (uint32_t)seg.start / TILE;
     seg.cost = cost;
+    const uint32_t off = (uint32_t)(r0 - seg.base);
     if (small) {
-      request_bounds<TILE>(a, seg.b, seg.start, seg.len, seg.nt);
-      seg.first_tile = seg.start / TILE;
-      const int splits = (seg.nt + chunk - 1) / chunk, off = r0 - seg.base;
-      seg.pair = off / splits;
-      seg.t0 = (off - seg.pair * splits) * chunk;
+      const uint32_t splits = (uint32_t)(((float)(seg.nt + chunk - 1) + 0.5f) * inv);
+      seg.pair = (int)(off / splits);
+      seg.t0 = (int)(off - seg.pair * splits) * chunk;
       seg.t1 = min(seg.nt, seg.t0 + chunk);
       seg.left = 0;
-      first_id = seg.base + seg.pair * splits;
-      last_id = first_id + splits - 1;
+      first_id = seg.base + seg.pair * (int)splits;
+      last_id = first_id + (int)splits - 1;
     } else {
-      seg.at(a, r0, min(chunk, total - r0));
+      seg.pair = (int)(off / (uint32_t)seg.units());
+      seg.take((int)off - seg.pair * seg.units(), min(chunk, total - r0));
     }
   }
 };
