@@ -39,6 +39,11 @@ def fast_int4(*args):
     return None if _calls is None else _calls.int4(*args)
 
 
+def fast(name: str, *args):
+    """The compiled call ``name`` of 4-bit pages and eviction; None as above."""
+    return None if _calls is None else getattr(_calls, name)(*args)
+
+
 _bound = False
 
 
@@ -54,6 +59,9 @@ def library():
             return lib
         _hostcalls.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
             lib.aicas_paged_rope_append, lib.aicas_paged_decode_gqa, lib.aicas_linear_int4)))
+        _hostcalls.bind_int4(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
+            lib.aicas_paged_append_int4, lib.aicas_paged_read_int4, lib.aicas_paged_decode_int4, lib.aicas_paged_weights,
+            lib.aicas_paged_evict)))
         _calls = _hostcalls
     return lib
 

@@ -15,13 +15,14 @@ The reference's caches keep every token (dujunbaoV1/evaluation_wrapper.py:54-112
 """
 from __future__ import annotations
 
+import operator
 from typing import Sequence
 
 import torch
 
 from . import _native as nat
-from ._hostpath import launch, lengths, plain, pointer, rows_ready, steps
-from .ops import _DTYPE_CODES, _LINEAR_DTYPES, SUPPORTED_HEAD_DIMS, _overlaps, _reject_grad
+from ._hostpath import fast, launch, lengths, pointer, rows_ready, steps
+from .ops import _DTYPE_CODES, SUPPORTED_HEAD_DIMS, _reject_grad
 from .paged import _ITEM
 from .paged_int4 import Int4Pages, _side, _table
 
@@ -54,7 +55,9 @@ def _check_weights(what: str, name: str, weights, B: int, Hkv: int, slots: int, 
         raise ValueError(f"{what}: {name} must be a CUDA fp32 [{B}, {Hkv}, C] tensor, C at least the {slots} slots of the "
                          "page table")
     s = steps(weights)
-    if s[2] not in (0, 1) or (Hkv > 1 and s[1] < weights.shape[2]) or (B > 1 and s[0] < weights.shape[2]):
+    C = weights.shape[2]
+    if s[2] not in (0, 1) or (Hkv > 1 and s[1] < C) or (B > 1 and s[0] < C) \
+            or (Hkv > 1 and B > 1 and s[0] < s[1] * Hkv and s[1] < s[0] * B):
         raise ValueError(f"{what}: {name} must have contiguous slots and rows apart from one another")
     return s[0], s[1]
 
@@ -83,6 +86,9 @@ def paged_attention_weights(
     ``[B, Hkv, C]``, C at least the page table's slots, updated in place and returned;
     slots outside the range keep what they hold.  ``kv_lens`` and ``kv_starts`` are the
     attention's.  Each slot is summed in one order, so results repeat to the bit."""
+    done = fast("weigh", query, k_pages, page_table, lse, weights, sm_scale, num_key_value_groups, kv_lens, kv_starts)
+    if done is not None:
+        return done
     what = "paged_attention_weights"
     if query.requires_grad or lse.requires_grad or weights.requires_grad:
         _reject_grad(query, lse, weights)
@@ -149,6 +155,10 @@ def paged_kv_evict(
 
     A page that a cut request holds must be in one place of one row of the page table:
     pages that requests share have to be copied first."""
+    done = fast("evict", k_pages, v_pages, page_table, weights, kv_lens, keep, keep_first, keep_last, longer_than, kv_lens_out,
+                weights_out)
+    if done is not None:
+        return done
     what = "paged_kv_evict"
     int4 = not isinstance(k_pages, torch.Tensor)
     first = (k_pages[0] if isinstance(k_pages, tuple) and len(k_pages) == 2 else page_table) if int4 else k_pages
@@ -172,7 +182,8 @@ def paged_kv_evict(
         raise ValueError(f"{what}: keys' and values' pages must be of one shape")
     P, Hkv, size = shapes[0][:3]
     page_table, max_pages, table_stride = _table(what, page_table, B, index)
-    longer_than = keep if longer_than is None else longer_than
+    keep, keep_first, keep_last, longer_than = (
+        operator.index(n) for n in (keep, keep_first, keep_last, keep if longer_than is None else longer_than))
     if keep < 1 or keep_first < 0 or keep_last < 0 or keep_first + keep_last > keep or longer_than < keep:
         raise ValueError(f"{what}: keep must be positive, keep_first + keep_last at most keep, and longer_than not below it")
     # no cache is longer than the table: numbers beyond it all mean the same

@@ -15,13 +15,14 @@ The reference has 16-bit contiguous caches in its served path
 """
 from __future__ import annotations
 
+import operator
 from typing import NamedTuple, Sequence
 
 import torch
 
 from . import _native as nat
-from ._hostpath import heads_out, launch, launch_with_workspace, lengths, plain, pointer, rows_ready, steps
-from .ops import _DTYPE_CODES, _LINEAR_DTYPES, _reject_grad
+from ._hostpath import fast, heads_out, launch, launch_with_workspace, lengths, pointer, rows_ready, steps
+from .ops import _DTYPE_CODES, _LINEAR_DTYPES, _WORKSPACES, _reject_grad
 from .paged import _new_rows
 
 INT4_HEAD_DIMS = (64, 128)
@@ -164,6 +165,10 @@ def paged_rope_kv_append_int4(
     A group's least value, and a fifteenth of its range above it, are rounded to that
     dtype; each element becomes the nearest of the 16 levels.  A group that is all one
     value gets that value, one with an element that is not finite reads back as NaN."""
+    done = fast("append_int4", query, key, value, cos, sin, k_pages, v_pages, page_table, positions, num_new, q_out,
+                kv_lens_out, q_norm_weight, k_norm_weight, eps)
+    if done is not None:
+        return done
     if query.requires_grad or key.requires_grad or value.requires_grad:
         _reject_grad(query, key, value)
     what = "paged_rope_kv_append_int4"
@@ -199,6 +204,9 @@ def paged_kv_read_int4(
     modules, :func:`aicas_b200.gqa_flash_attention` or another cache take.  Rows past
     ``num_tokens[b]`` (int32 ``[B]``, default all), slots outside the page table and
     pages outside the pool read as zeros."""
+    done = fast("read_int4", k_pages, v_pages, page_table, positions, seq_len, num_tokens)
+    if done is not None:
+        return done
     what = "paged_kv_read_int4"
     if not isinstance(k_pages, tuple) or len(k_pages) != 2 or page_table.ndim != 2:
         raise ValueError(f"{what} needs Int4Pages and a page_table [B, max_pages]")
@@ -206,6 +214,7 @@ def paged_kv_read_int4(
     (P, Hkv, size, D, group), refs, page_table, max_pages, table_stride = _pools(
         what, page_table, k_pages, v_pages, page_table, B, None)
     device, dtype = page_table.device, k_pages[1].dtype
+    seq_len = operator.index(seq_len)
     if seq_len < 0:
         raise ValueError(f"{what}: seq_len must not be negative")
     pos = lengths(positions, B, device)
@@ -237,6 +246,10 @@ def paged_gqa_decode_attention_int4(
     arguments, masks and results, but for the pages, whose scales are of the query's
     dtype (fp16 or bf16).  The codes enter the products as they are; scores, statistics
     and sums are held in fp32 and the result is rounded once."""
+    done = fast("decode_int4", query, k_pages, v_pages, page_table, sm_scale, num_key_value_groups, kv_lens, kv_starts,
+                return_lse, _WORKSPACES)
+    if done is not None:
+        return done
     if query.requires_grad:
         _reject_grad(query)
     what = "paged_gqa_decode_attention_int4"
