@@ -563,6 +563,8 @@ int check_paged_read_int4(const aicas_paged_read_int4_params* p) {
                                   p->num_kv_heads, p->num_pages, p->page_size, p->max_pages);
   if (rc != AICAS_OK) return rc;
   if (p->seq_len < 1) return fail(AICAS_ERR_INVALID, "seq_len=%d", p->seq_len);
+  if (p->num_kv_heads > 32767 || (int64_t)p->batch * p->seq_len > (int64_t)INT32_MAX)
+    return fail(AICAS_ERR_UNSUPPORTED, "num_kv_heads=%d, seq_len=%d of batch %d", p->num_kv_heads, p->seq_len, p->batch);
   if (!aligned16(p->out[0]) || !aligned16(p->out[1])) return fail(AICAS_ERR_INVALID, "out must be 16-byte aligned");
   const int64_t st[] = {p->out_stride_b, p->out_stride_h, p->out_stride_s};
   for (int64_t s : st)

@@ -4,7 +4,7 @@
 //   r = y * cos + rotate_half(y) * sin,      rotate_half(y) = cat(-y[D/2:], y[:D/2])
 //   of each group of 64 (or D) elements of r (keys) and v:
 //     least = T(min r),  scale = T((max r - least) / 15)
-//     code  = (r - least) / scale to the nearest of 0..15   (0 where scale is 0)
+//     code  = (r - least) / scale to the nearest of 0..15   (0 where scale is no normal fp32 number)
 //   read back as fma(scale, code, least), rounded to T.
 //
 // Rounding of r: paged_append.cu's (fp32 tables: fp32 to the code; 16-bit tables: every
@@ -20,183 +20,239 @@
 namespace aicas {
 namespace {
 
-// Least and largest of a group over its TPR lanes; NaN as least where an element is no finite number.
+// Least and largest of three; NaN if one is.
+__device__ __forceinline__ float min_nan(float a, float b, float c) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// And of 8 elements.
+__device__ __forceinline__ void range8(const float* x, float& lo, float& hi) {
+  lo = min_nan(min_nan(x[0], x[1], x[2]), min_nan(x[3], x[4], x[5]), min_nan(x[6], x[7], x[7]));
+  hi = max_nan(max_nan(x[0], x[1], x[2]), max_nan(x[3], x[4], x[5]), max_nan(x[6], x[7], x[7]));
+}
+
+// Least and largest of a group over its TPR lanes; NaN where an element is.
 template <int TPR>
-__device__ __forceinline__ void group_range(uint32_t lanes, float& lo, float& hi, bool bad) {
+__device__ __forceinline__ void group_range(uint32_t lanes, float& lo, float& hi) {
 #pragma unroll
   for (int off = TPR / 2; off >= 1; off >>= 1) {
-    lo = fminf(lo, __shfl_xor_sync(lanes, lo, off));
-    hi = fmaxf(hi, __shfl_xor_sync(lanes, hi, off));
+    lo = min_nan(lo, lo, __shfl_xor_sync(lanes, lo, off));
+    hi = max_nan(hi, hi, __shfl_xor_sync(lanes, hi, off));
   }
-  if (__any_sync(lanes, bad)) lo = __int_as_float(0x7fc00000);
 }
 
-// (scale, least) of a group as the cache holds them, and as floats.
-template <typename T>
-__device__ __forceinline__ uint32_t group_levels(float lo, float hi, float& scale, float& least) {
-  const T l = Elem<T>::from_float(lo);
-  least = Elem<T>::to_float(l);
-  const T s = Elem<T>::from_float((hi - least) / 15.f);
-  scale = Elem<T>::to_float(s);
-  if (!(fabsf(scale) < INFINITY)) scale = least = __int_as_float(0x7fc00000);  // infinities, NaN
-  union {
-    T t[2];
-    uint32_t u;
-  } r;
-  r.t[0] = Elem<T>::from_float(scale), r.t[1] = Elem<T>::from_float(least);
-  return r.u;
-}
+// A group's (scale, least) as the cache holds them, and what its codes are taken by.
+struct Levels {
+  float scale, least, inv;
+  uint32_t pair;
 
-__device__ __forceinline__ uint32_t codes_of(const float* x, float scale, float least) {
-  // the reciprocal of a scale near the least normal number would be infinite
-  const float lift = scale < 1e-30f ? 0x1p64f : 1.f;
-  const float inv = scale > 0.f ? 1.f / (scale * lift) : 0.f;
-  scale *= lift;
-  // 1.5 x 2^23: a sum with it has the number, rounded to a whole one, in its low bits
-  constexpr float kWhole = 12582912.f;
-  uint32_t u = 0;
+  template <typename T>
+  __device__ __forceinline__ void set(float lo, float hi) {
+    const T l = Elem<T>::from_float(lo);
+    least = Elem<T>::to_float(l);
+    const T s = Elem<T>::from_float((hi - least) / 15.f);
+    scale = Elem<T>::to_float(s);
+    if (!(fabsf(scale) < INFINITY)) scale = least = __int_as_float(0x7fc00000);  // an infinity or NaN among the elements
+    inv = scale >= 0x1p-126f ? __frcp_rn(scale) : 0.f;
+    union {
+      T t[2];
+      uint32_t u;
+    } r;
+    r.t[0] = Elem<T>::from_float(scale), r.t[1] = Elem<T>::from_float(least);
+    pair = r.u;
+  }
+
+  // The codes of 8 elements, 4 bits each.  EXACT: elements that are 16-bit values often lie
+  // on the border between two codes, where the quotient by the reciprocal may fall on
+  // either side; what a nearby code leaves, which fma gives exactly, corrects it.
+  template <bool EXACT>
+  __device__ __forceinline__ uint32_t codes(const float* x) const {
+    if (inv == 0.f) return 0u;  // one value, or NaN
+    // 1.5 x 2^23: a sum with it has the number, rounded to a whole one, in its low bits
+    constexpr float kWhole = 12582912.f;
+    const float at = fmaf(-least, inv, kWhole);
+    int q[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    // 16-bit values often lie on the border between two codes, where a product with the
-    // reciprocal may fall on either side: what the nearest code leaves, which fma gives
-    // exactly, brings the quotient back to the border
-    const float d = (x[i] - least) * lift, t = d * inv, near = (t + kWhole) - kWhole;
-    const float q = fmaf(fmaf(-near, scale, d), inv, near);
-    u |= (__float_as_uint(fminf(fmaxf(q, 0.f), 15.f) + kWhole) & 15u) << (4 * i);
+    for (int i = 0; i < 8; ++i) {
+      const float d = x[i] - least;
+      float w;
+      if constexpr (EXACT) {
+        const float near = fmaf(x[i], inv, at) - kWhole;
+        w = fmaf(fmaf(-near, scale, d), inv, near) + kWhole;
+      } else {
+        w = fmaf(d, inv, kWhole);
+      }
+      q[i] = __float_as_int(w) - 0x4b400000;
+    }
+    uint32_t u = 0;
+#pragma unroll
+    for (int i = 6; i >= 0; i -= 2)  // two numbers, held to 0..15, below what is there
+      asm("cvt.pack.sat.u4.s32.b32 %0, %1, %2, %0;" : "+r"(u) : "r"(q[i + 1]), "r"(q[i]));
+    return u;
   }
-  return u;
-}
+};
 
-// HBM bound: the token's rows are read once, q written in 16 and k and v in 4 bits.  The
-// CTA, its threads and the rows in flight are paged_append.cu's: a row (one head of q, k
-// or v) belongs to D / 16 threads, each with one 16-byte vector of the row's first half
-// and the matching one of its second half, so that the rotation needs no exchange, and
-// with groups of 64 in rows of 128 each half is a group.
-template <typename T, typename CS, int D, bool HALVES, int THREADS, int ROWS>
-__global__ void __launch_bounds__(THREADS) paged_append_int4_kernel(const __grid_constant__ aicas_paged_append_int4_params a) {
-  constexpr bool kRoundEach = std::is_same<T, CS>::value;
-  constexpr int kV = 8;
-  constexpr int kTpr = D / (2 * kV);
-  constexpr int kSlots = THREADS / kTpr;
-  const int b = blockIdx.x / a.seq_len, s = blockIdx.x - b * a.seq_len;
-  const int c = threadIdx.x % kTpr * kV;
-  const uint32_t row_lanes = ((1u << kTpr) - 1u) << (threadIdx.x % 32 / kTpr * kTpr);
-  const int hq = a.num_q_heads, hkv = a.num_kv_heads, rows = hq + 2 * hkv;
-  grid_launch_dependents();
-  grid_dependency_wait();
-  // the token's slot; asked for first, needed last
-  const int pos = a.positions[b];
-  const int fresh = a.num_new != nullptr ? min(max(a.num_new[b], 0), a.seq_len) : a.seq_len;
-  const int cap = a.max_pages * a.page_size;
-  const long long slot = (long long)pos + s;
-  int page = -1, row = 0;  // -1: nowhere
-  if (s < fresh && slot >= 0 && slot < cap) {
-    const int i = (int)slot / a.page_size;
-    row = (int)slot - i * a.page_size;
-    page = a.page_table[b * a.table_stride + i];
-    if (page >= a.num_pages) page = -1;
-  }
-  if (a.kv_lens_out != nullptr && s == 0 && threadIdx.x == 0)
-    a.kv_lens_out[b] = (int)min((long long)max(pos, 0) + fresh, (long long)cap);
-
+// The lane's part of one token: c is its place in a row's halves, lanes those of its row.
+template <typename CS, int D>
+struct Token {
+  static constexpr int kV = 8, kTpr = D / (2 * kV);
+  int b, s, c;
+  uint32_t lanes;
+  int page, row;  // page -1: nowhere to write
   float c1[kV], c2[kV], s1[kV], s2[kV];
-  bool tables = false;
-  for (int r0 = threadIdx.x / kTpr; r0 - (int)threadIdx.x / kTpr < rows; r0 += kSlots * ROWS) {
-    uint4 u1[ROWS], u2[ROWS];
+};
+
+// Rows h, h + step, ... (COUNT of them, below `heads`) of the token's q (KIND 0), k (1) or v (2).
+template <typename T, typename CS, int D, bool HALVES, int KIND, int COUNT>
+__device__ __forceinline__ void token_rows(const aicas_paged_append_int4_params& a, const Token<CS, D>& t, int h, int step, int heads) {
+  using K = Token<CS, D>;
+  constexpr int kV = K::kV, kTpr = K::kTpr;
+  constexpr bool kRoundEach = std::is_same<T, CS>::value;
+  const T* src = static_cast<const T*>(KIND == 0 ? a.q_in : KIND == 1 ? a.k_in : a.v_in) +
+                 t.b * (KIND == 0 ? a.qi_stride_b : KIND == 1 ? a.k_stride_b : a.v_stride_b) +
+                 t.s * (KIND == 0 ? a.qi_stride_s : KIND == 1 ? a.k_stride_s : a.v_stride_s) + t.c;
+  const int64_t src_h = KIND == 0 ? a.qi_stride_h : KIND == 1 ? a.k_stride_h : a.v_stride_h;
+  uint4 u1[COUNT], u2[COUNT];
 #pragma unroll
-    for (int j = 0; j < ROWS; ++j) {
-      const int r = r0 + j * kSlots;
-      u1[j] = u2[j] = make_uint4(0, 0, 0, 0);
-      if (r >= rows) continue;
-      const T* src = r < hq ? static_cast<const T*>(a.q_in) + b * a.qi_stride_b + r * a.qi_stride_h + s * a.qi_stride_s
-                     : r < hq + hkv
-                         ? static_cast<const T*>(a.k_in) + b * a.k_stride_b + (r - hq) * a.k_stride_h + s * a.k_stride_s
-                         : static_cast<const T*>(a.v_in) + b * a.v_stride_b + (r - hq - hkv) * a.v_stride_h + s * a.v_stride_s;
-      u1[j] = *reinterpret_cast<const uint4*>(src + c);
-      u2[j] = *reinterpret_cast<const uint4*>(src + c + D / 2);
-    }
-    if (!tables) {
-      const CS* cp = static_cast<const CS*>(a.cos) + b * a.cs_stride_b + s * a.cs_stride_s + c;
-      const CS* sp = static_cast<const CS*>(a.sin) + b * a.cs_stride_b + s * a.cs_stride_s + c;
-      load_floats<CS, kV>(cp, c1);
-      load_floats<CS, kV>(cp + D / 2, c2);
-      load_floats<CS, kV>(sp, s1);
-      load_floats<CS, kV>(sp + D / 2, s2);
-      tables = true;
-    }
+  for (int j = 0; j < COUNT; ++j) {
+    u1[j] = u2[j] = make_uint4(0, 0, 0, 0);
+    if (h + j * step >= heads) continue;
+    const T* p = src + (h + j * step) * src_h;
+    u1[j] = *reinterpret_cast<const uint4*>(p);
+    u2[j] = *reinterpret_cast<const uint4*>(p + D / 2);
+  }
+  const T* w = static_cast<const T*>(KIND == 0 ? a.q_norm_weight : a.k_norm_weight);
+  uint4 w1 = {}, w2 = {};
+  if (KIND < 2 && w != nullptr) {
+    w1 = *reinterpret_cast<const uint4*>(w + t.c);
+    w2 = *reinterpret_cast<const uint4*>(w + t.c + D / 2);
+  }
 #pragma unroll
-    for (int j = 0; j < ROWS; ++j) {
-      const int r = r0 + j * kSlots;
-      if (r >= rows || (r >= hq && page < 0)) continue;  // the lanes of a row stay together
-      float x1[kV], x2[kV];
-      Elem<T>::unpack(u1[j], x1);
-      Elem<T>::unpack(u2[j], x2);
-      if (r < hq + hkv) {
-        const T* w = static_cast<const T*>(r < hq ? a.q_norm_weight : a.k_norm_weight);
-        if (w != nullptr) {
-          float w1[kV], w2[kV];
-          load_floats<T, kV>(w + c, w1);
-          load_floats<T, kV>(w + c + D / 2, w2);
-          float ss = 0.f;
+  for (int j = 0; j < COUNT; ++j) {
+    const int head = h + j * step;
+    if (head >= heads || (KIND > 0 && t.page < 0)) continue;  // the lanes of a row stay together
+    float x1[kV], x2[kV];
+    Elem<T>::unpack(u1[j], x1);
+    Elem<T>::unpack(u2[j], x2);
+    if constexpr (KIND < 2) {
+      if (w != nullptr) {
+        float f1[kV], f2[kV];
+        Elem<T>::unpack(w1, f1);
+        Elem<T>::unpack(w2, f2);
+        float ss = 0.f;
 #pragma unroll
-          for (int i = 0; i < kV; ++i) ss += x1[i] * x1[i] + x2[i] * x2[i];
+        for (int i = 0; i < kV; ++i) ss += x1[i] * x1[i] + x2[i] * x2[i];
 #pragma unroll
-          for (int off = kTpr / 2; off >= 1; off >>= 1) ss += __shfl_xor_sync(row_lanes, ss, off);
-          const float inv = rsqrtf(ss / (float)D + a.norm_eps);
-          normed_pair<T, kRoundEach, kV>(x1, x2, w1, w2, inv);
-        }
-        rotated_pair<T, kRoundEach, kV>(x1, x2, c1, c2, s1, s2);
+        for (int off = kTpr / 2; off >= 1; off >>= 1) ss += __shfl_xor_sync(t.lanes, ss, off);
+        normed_pair<T, kRoundEach, kV>(x1, x2, f1, f2, rsqrtf(ss / (float)D + a.norm_eps));
       }
-      if (r < hq) {
-        T* dst = static_cast<T*>(a.q_out) + b * a.qo_stride_b + r * a.qo_stride_h + s * a.qo_stride_s;
-        *reinterpret_cast<uint4*>(dst + c) = pack_vec<T>(x1);
-        *reinterpret_cast<uint4*>(dst + c + D / 2) = pack_vec<T>(x2);
-        continue;
-      }
-      const aicas_int4_pages& to = a.kv[r >= hq + hkv];
-      const int h = r >= hq + hkv ? r - hq - hkv : r - hq;
-      if (kRoundEach && r < hq + hkv) {
+      rotated_pair<T, kRoundEach, kV>(x1, x2, t.c1, t.c2, t.s1, t.s2);
+    }
+    if constexpr (KIND == 0) {
+      T* dst = static_cast<T*>(a.q_out) + t.b * a.qo_stride_b + t.s * a.qo_stride_s + head * a.qo_stride_h + t.c;
+      *reinterpret_cast<uint4*>(dst) = pack_vec<T>(x1);
+      *reinterpret_cast<uint4*>(dst + D / 2) = pack_vec<T>(x2);
+    } else {
+      if constexpr (KIND == 1 && kRoundEach) {
 #pragma unroll
         for (int i = 0; i < kV; ++i) x1[i] = rounded<T>(x1[i]), x2[i] = rounded<T>(x2[i]);
       }
-      float lo1 = x1[0], hi1 = x1[0], lo2 = x2[0], hi2 = x2[0], bad1 = 0.f, bad2 = 0.f;
-#pragma unroll
-      for (int i = 0; i < kV; ++i) {
-        lo1 = fminf(lo1, x1[i]), hi1 = fmaxf(hi1, x1[i]), bad1 = fmaf(x1[i], 0.f, bad1);
-        lo2 = fminf(lo2, x2[i]), hi2 = fmaxf(hi2, x2[i]), bad2 = fmaf(x2[i], 0.f, bad2);
-      }
+      constexpr bool kExact = KIND == 2 || kRoundEach;
+      const aicas_int4_pages& to = a.kv[KIND - 1];
+      uint8_t* codes = static_cast<uint8_t*>(to.codes) + t.page * to.cs_p + t.row * to.cs_t + head * to.cs_h + t.c / 2;
+      T* pair = static_cast<T*>(to.scales) + t.page * to.ss_p + t.row * to.ss_t + head * to.ss_h;
+      float lo1, hi1, lo2, hi2;
+      range8(x1, lo1, hi1);
+      range8(x2, lo2, hi2);
+      Levels v1 = {}, v2 = {};
       if constexpr (HALVES) {
-        group_range<kTpr>(row_lanes, lo1, hi1, bad1 != 0.f);  // 0 but where an element is no finite number
-        group_range<kTpr>(row_lanes, lo2, hi2, bad2 != 0.f);
+        group_range<kTpr>(t.lanes, lo1, hi1);
+        group_range<kTpr>(t.lanes, lo2, hi2);
+        v1.set<T>(lo1, hi1);
+        v2.set<T>(lo2, hi2);
+        if (t.c == 0) *reinterpret_cast<uint2*>(pair) = make_uint2(v1.pair, v2.pair);
       } else {
-        lo1 = fminf(lo1, lo2), hi1 = fmaxf(hi1, hi2);
-        group_range<kTpr>(row_lanes, lo1, hi1, bad1 + bad2 != 0.f);
+        lo1 = min_nan(lo1, lo1, lo2), hi1 = max_nan(hi1, hi1, hi2);
+        group_range<kTpr>(t.lanes, lo1, hi1);
+        v1.set<T>(lo1, hi1);
+        v2 = v1;
+        if (t.c == 0) *reinterpret_cast<uint32_t*>(pair) = v1.pair;
       }
-      float scale1, least1, scale2, least2;
-      const uint32_t p1 = group_levels<T>(lo1, hi1, scale1, least1);
-      const uint32_t p2 = HALVES ? group_levels<T>(lo2, hi2, scale2, least2) : (scale2 = scale1, least2 = least1, 0u);
-      uint8_t* codes = static_cast<uint8_t*>(to.codes) + page * to.cs_p + h * to.cs_h + row * to.cs_t;
-      *reinterpret_cast<uint32_t*>(codes + c / 2) = codes_of(x1, scale1, least1);
-      *reinterpret_cast<uint32_t*>(codes + c / 2 + D / 4) = codes_of(x2, scale2, least2);
-      if (c == 0) {
-        T* pair = static_cast<T*>(to.scales) + page * to.ss_p + h * to.ss_h + row * to.ss_t;
-        if constexpr (HALVES) {
-          *reinterpret_cast<uint2*>(pair) = make_uint2(p1, p2);
-        } else {
-          *reinterpret_cast<uint32_t*>(pair) = p1;
-        }
-      }
+      *reinterpret_cast<uint32_t*>(codes) = v1.codes<kExact>(x1);
+      *reinterpret_cast<uint32_t*>(codes + D / 4) = v2.codes<kExact>(x2);
     }
   }
 }
+
+// HBM bound: the token's rows are read once, q written in 16 and k and v in 4 bits.  One
+// CTA a token, as in paged_append.cu: a row (one head of q, k or v) belongs to D / 16
+// threads, each with one 16-byte vector of the row's first half and the matching one of its
+// second half, so that the rotation needs no exchange, and with groups of 64 in rows of 128
+// each half is a group.  PROMPT: one warp, and q's, k's and v's rows one after the other
+// with several in flight; else a row a thread, all at once.
+template <typename T, typename CS, int D, bool HALVES, bool PROMPT>
+__global__ void __launch_bounds__(PROMPT ? 32 : 256, PROMPT ? 18 : 1)
+    paged_append_int4_kernel(const __grid_constant__ aicas_paged_append_int4_params a) {
+  using K = Token<CS, D>;
+  constexpr int kV = K::kV, kTpr = K::kTpr, kSlots = (PROMPT ? 32 : 256) / kTpr;
+  K t;
+  t.b = blockIdx.x / a.seq_len, t.s = blockIdx.x - t.b * a.seq_len;
+  t.c = threadIdx.x % kTpr * kV;
+  t.lanes = ((1u << kTpr) - 1u) << (threadIdx.x % 32 / kTpr * kTpr);
+  const int hq = a.num_q_heads, hkv = a.num_kv_heads;
+  grid_launch_dependents();
+  grid_dependency_wait();
+  // the token's slot; asked for first, needed last
+  const int pos = a.positions[t.b];
+  const int fresh = a.num_new != nullptr ? min(max(a.num_new[t.b], 0), a.seq_len) : a.seq_len;
+  const int cap = a.max_pages * a.page_size;
+  const long long slot = (long long)pos + t.s;
+  t.page = -1, t.row = 0;
+  if (t.s < fresh && slot >= 0 && slot < cap) {
+    const int i = (int)((uint32_t)slot / (uint32_t)a.page_size);
+    t.row = (int)slot - i * a.page_size;
+    t.page = a.page_table[t.b * a.table_stride + i];
+    if (t.page >= a.num_pages) t.page = -1;
+  }
+  if (a.kv_lens_out != nullptr && t.s == 0 && threadIdx.x == 0)
+    a.kv_lens_out[t.b] = (int)min((long long)max(pos, 0) + fresh, (long long)cap);
+  const CS* cp = static_cast<const CS*>(a.cos) + t.b * a.cs_stride_b + t.s * a.cs_stride_s + t.c;
+  const CS* sp = static_cast<const CS*>(a.sin) + t.b * a.cs_stride_b + t.s * a.cs_stride_s + t.c;
+  load_floats<CS, kV>(cp, t.c1);
+  load_floats<CS, kV>(cp + D / 2, t.c2);
+  load_floats<CS, kV>(sp, t.s1);
+  load_floats<CS, kV>(sp + D / 2, t.s2);
+  const int r0 = threadIdx.x / kTpr;
+  if constexpr (PROMPT) {
+    for (int h = 0; h < hq; h += 4 * kSlots) token_rows<T, CS, D, HALVES, 0, 4>(a, t, h + r0, kSlots, hq);
+    for (int h = 0; h < hkv; h += 2 * kSlots) token_rows<T, CS, D, HALVES, 1, 2>(a, t, h + r0, kSlots, hkv);
+    for (int h = 0; h < hkv; h += 2 * kSlots) token_rows<T, CS, D, HALVES, 2, 2>(a, t, h + r0, kSlots, hkv);
+  } else {
+    for (int r = r0; r < hq + 2 * hkv; r += kSlots) {
+      if (r < hq)
+        token_rows<T, CS, D, HALVES, 0, 1>(a, t, r, 0, hq);
+      else if (r < hq + hkv)
+        token_rows<T, CS, D, HALVES, 1, 1>(a, t, r - hq, 0, hkv);
+      else
+        token_rows<T, CS, D, HALVES, 2, 1>(a, t, r - hq - hkv, 0, hkv);
+    }
+  }
+}
+
+constexpr int kPromptTokens = 384;
 
 template <typename T, typename CS, int D, bool HALVES>
 cudaError_t launch_append_sized(const aicas_paged_append_int4_params& p, cudaStream_t st) {
   const dim3 grid((unsigned)(p.batch * p.seq_len));
-  // as paged_append.cu chooses: the shortest way for a decode step, more CTAs and rows in flight for prompts
-  return p.batch * p.seq_len <= 384
-             ? launch_pdl(paged_append_int4_kernel<T, CS, D, HALVES, 256, 1>, grid, dim3(256), 0, st, p)
-             : launch_pdl(paged_append_int4_kernel<T, CS, D, HALVES, 32, 4>, grid, dim3(32), 0, st, p);
+  return p.batch * p.seq_len <= kPromptTokens
+             ? launch_pdl(paged_append_int4_kernel<T, CS, D, HALVES, false>, grid, dim3(256), 0, st, p)
+             : launch_pdl(paged_append_int4_kernel<T, CS, D, HALVES, true>, grid, dim3(32), 0, st, p);
 }
 
 template <typename T, typename CS>
@@ -207,49 +263,76 @@ cudaError_t launch_append(const aicas_paged_append_int4_params& p, cudaStream_t 
 
 // ------------------------------------------------------------------ reads
 
-// HBM bound: 8 elements a thread, 4 bytes of codes in and 16 bytes out.
-template <typename T, int D, bool HALVES>
-__global__ void __launch_bounds__(256) paged_read_int4_kernel(const __grid_constant__ aicas_paged_read_int4_params a) {
-  constexpr int kTpr = D / 8, kSlots = 256 / kTpr;
+// HBM bound: 8 elements a thread, 4 bytes of codes in and 16 bytes out, of ROWS rows of one
+// request, side and head, so that their page numbers, codes and pairs are on the way at once.
+template <typename T, int D, bool HALVES, int ROWS>
+__global__ void __launch_bounds__(256) paged_read_int4_kernel(const __grid_constant__ aicas_paged_read_int4_params a, int chunks) {
+  constexpr int kTpr = D / 8;
+  const int slots = blockDim.x / kTpr;
+  const int b = blockIdx.x / chunks, h = blockIdx.y >> 1, side = blockIdx.y & 1;
+  const int c = threadIdx.x % kTpr * 8, s0 = (blockIdx.x - b * chunks) * slots * ROWS + threadIdx.x / kTpr;
   grid_launch_dependents();
   grid_dependency_wait();
-  const int64_t total = (int64_t)a.batch * 2 * a.num_kv_heads * a.seq_len;
-  for (int64_t r = (int64_t)blockIdx.x * kSlots + threadIdx.x / kTpr; r < total; r += (int64_t)gridDim.x * kSlots) {
-    const int s = (int)(r % a.seq_len);
-    const int64_t head = r / a.seq_len;
-    const int h = (int)(head % a.num_kv_heads), side = (int)(head / a.num_kv_heads) & 1;
-    const int b = (int)(head / (2 * a.num_kv_heads));
-    const int c = threadIdx.x % kTpr * 8;
-    const int fresh = a.num_tokens != nullptr ? a.num_tokens[b] : a.seq_len;
-    const long long slot = (long long)a.positions[b] + s;
-    float f[8] = {};
-    if (s < fresh && slot >= 0 && slot < (long long)a.max_pages * a.page_size) {
-      const int i = (int)slot / a.page_size, row = (int)slot - i * a.page_size;
-      const int page = a.page_table[b * a.table_stride + i];
-      if (page >= 0 && page < a.num_pages) {
-        const aicas_int4_pages& from = a.kv[side];
-        const uint32_t u = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(from.codes) + page * from.cs_p +
-                                                              h * from.cs_h + row * from.cs_t + c / 2);
-        const T* pair = static_cast<const T*>(from.scales) + page * from.ss_p + h * from.ss_h + row * from.ss_t +
-                        (HALVES && c >= D / 2 ? 2 : 0);
-        const float scale = Elem<T>::to_float(pair[0]), least = Elem<T>::to_float(pair[1]);
+  const int fresh = a.num_tokens != nullptr ? min(a.num_tokens[b], a.seq_len) : a.seq_len;
+  const int pos = a.positions[b], cap = a.max_pages * a.page_size;
+  const aicas_int4_pages& from = a.kv[side];
+  const uint8_t* codes = static_cast<const uint8_t*>(from.codes) + h * from.cs_h + c / 2;
+  const T* pairs = static_cast<const T*>(from.scales) + h * from.ss_h + (HALVES && c >= D / 2 ? 2 : 0);
+  int page[ROWS], row[ROWS];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = fmaf(scale, (float)(u >> (4 * e) & 15u), least);
-      }
+  for (int j = 0; j < ROWS; ++j) {
+    const int s = s0 + j * slots;
+    const long long slot = (long long)pos + s;
+    page[j] = -1, row[j] = 0;
+    if (s < fresh && slot >= 0 && slot < cap) {
+      const int i = (int)((uint32_t)slot / (uint32_t)a.page_size);
+      row[j] = (int)slot - i * a.page_size;
+      page[j] = a.page_table[b * a.table_stride + i];
     }
-    *reinterpret_cast<uint4*>(static_cast<T*>(a.out[side]) + b * a.out_stride_b + h * a.out_stride_h + s * a.out_stride_s + c) =
-        pack_vec<T>(f);
   }
+  uint32_t u[ROWS], p[ROWS];
+#pragma unroll
+  for (int j = 0; j < ROWS; ++j) {
+    u[j] = p[j] = 0;
+    if (page[j] >= 0 && page[j] < a.num_pages) {
+      u[j] = *reinterpret_cast<const uint32_t*>(codes + page[j] * from.cs_p + row[j] * from.cs_t);
+      p[j] = *reinterpret_cast<const uint32_t*>(pairs + page[j] * from.ss_p + row[j] * from.ss_t);
+    }
+  }
+  T* out = static_cast<T*>(a.out[side]) + b * a.out_stride_b + h * a.out_stride_h + c;
+#pragma unroll
+  for (int j = 0; j < ROWS; ++j) {
+    const int s = s0 + j * slots;
+    if (s >= a.seq_len) break;
+    union {
+      uint32_t u;
+      T t[2];
+    } pair;
+    pair.u = p[j];
+    const float scale = Elem<T>::to_float(pair.t[0]), least = Elem<T>::to_float(pair.t[1]);
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = fmaf(scale, (float)(u[j] >> (4 * e) & 15u), least);
+    *reinterpret_cast<uint4*>(out + (int64_t)s * a.out_stride_s) = pack_vec<T>(f);
+  }
+}
+
+template <typename T, int D, bool HALVES>
+cudaError_t launch_read_sized(const aicas_paged_read_int4_params& p, cudaStream_t st) {
+  constexpr int kTpr = D / 8;
+  // few rows a request (a decode step): CTAs as small as they go; many: four rows a thread
+  const bool few = p.seq_len * kTpr <= 256;
+  const int threads = few ? (p.seq_len * kTpr + 31) / 32 * 32 : 256;
+  const int64_t rows = (int64_t)threads / kTpr * (few ? 1 : 4), chunks = (p.seq_len + rows - 1) / rows;
+  const dim3 grid((unsigned)(chunks * p.batch), 2u * p.num_kv_heads);
+  return few ? launch_pdl(paged_read_int4_kernel<T, D, HALVES, 1>, grid, dim3(threads), 0, st, p, (int)chunks)
+             : launch_pdl(paged_read_int4_kernel<T, D, HALVES, 4>, grid, dim3(threads), 0, st, p, (int)chunks);
 }
 
 template <typename T>
 cudaError_t launch_read(const aicas_paged_read_int4_params& p, cudaStream_t st) {
-  const int64_t rows = (int64_t)p.batch * 2 * p.num_kv_heads * p.seq_len, slots = 256 / (p.head_dim / 8);
-  const int64_t ctas = (rows + slots - 1) / slots;
-  const dim3 grid((unsigned)(ctas < 1 << 20 ? ctas : 1 << 20)), block(256);
-  if (p.head_dim == 64) return launch_pdl(paged_read_int4_kernel<T, 64, false>, grid, block, 0, st, p);
-  return p.group_size == 64 ? launch_pdl(paged_read_int4_kernel<T, 128, true>, grid, block, 0, st, p)
-                            : launch_pdl(paged_read_int4_kernel<T, 128, false>, grid, block, 0, st, p);
+  if (p.head_dim == 64) return launch_read_sized<T, 64, false>(p, st);
+  return p.group_size == 64 ? launch_read_sized<T, 128, true>(p, st) : launch_read_sized<T, 128, false>(p, st);
 }
 
 int status(cudaError_t e, const char* what, char* err, size_t errlen) {

@@ -78,7 +78,8 @@ def quantize_kv_int4(rows: torch.Tensor, group_size: int | None = None) -> Int4P
     bad = ~(scale.float().abs() < torch.inf)
     scale, lo = scale.masked_fill(bad, torch.nan), lo.masked_fill(bad, torch.nan)
     step, least = scale.float()[..., None], lo.float()[..., None]
-    q = torch.where(step > 0, (x - least) / torch.where(step > 0, step, 1.0), 0.0).nan_to_num(0.0)
+    fine = step >= torch.finfo(torch.float32).tiny
+    q = torch.where(fine, (x - least) / torch.where(fine, step, 1.0), 0.0)
     q = q.round().clamp(0, 15).to(torch.uint8).flatten(-2)
     return Int4Pages(q[..., 0::2] | (q[..., 1::2] << 4), torch.stack([scale, lo], -1))
 
