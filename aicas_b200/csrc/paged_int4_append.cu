@@ -56,10 +56,13 @@ struct Levels {
   __device__ __forceinline__ void set(float lo, float hi) {
     const T l = Elem<T>::from_float(lo);
     least = Elem<T>::to_float(l);
-    const T s = Elem<T>::from_float((hi - least) / 15.f);
+    constexpr float kFifteenth = 1.f / 15.f;
+    const float range = hi - least, near = range * kFifteenth;
+    const T s = Elem<T>::from_float(fmaf(fmaf(-15.f, near, range), kFifteenth, near));  // range / 15, rounded once
     scale = Elem<T>::to_float(s);
     if (!(fabsf(scale) < INFINITY)) scale = least = __int_as_float(0x7fc00000);  // an infinity or NaN among the elements
-    inv = scale >= 0x1p-126f ? __frcp_rn(scale) : 0.f;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
+    inv = scale >= 0x1p-126f ? inv : 0.f;
     union {
       T t[2];
       uint32_t u;
@@ -81,14 +84,12 @@ struct Levels {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float d = x[i] - least;
-      float w;
+      float w = d * inv;
       if constexpr (EXACT) {
         const float near = fmaf(x[i], inv, at) - kWhole;
-        w = fmaf(fmaf(-near, scale, d), inv, near) + kWhole;
-      } else {
-        w = fmaf(d, inv, kWhole);
+        w = fmaf(fmaf(-near, scale, d), inv, near);
       }
-      q[i] = __float_as_int(w) - 0x4b400000;
+      q[i] = __float_as_int(w * 0x1p-149f);  // as so many of the smallest steps: the number, rounded to a whole one
     }
     uint32_t u = 0;
 #pragma unroll
@@ -196,13 +197,17 @@ __device__ __forceinline__ void token_rows(const aicas_paged_append_int4_params&
 // second half, so that the rotation needs no exchange, and with groups of 64 in rows of 128
 // each half is a group.  PROMPT: one warp, and q's, k's and v's rows one after the other
 // with several in flight; else a row a thread, all at once.
+constexpr int kPromptWarps = 4;
+
 template <typename T, typename CS, int D, bool HALVES, bool PROMPT>
-__global__ void __launch_bounds__(PROMPT ? 32 : 256, PROMPT ? 18 : 1)
+__global__ void __launch_bounds__(PROMPT ? 32 * kPromptWarps : 256, PROMPT ? 16 / kPromptWarps : 1)
     paged_append_int4_kernel(const __grid_constant__ aicas_paged_append_int4_params a) {
   using K = Token<CS, D>;
   constexpr int kV = K::kV, kTpr = K::kTpr, kSlots = (PROMPT ? 32 : 256) / kTpr;
   K t;
-  t.b = blockIdx.x / a.seq_len, t.s = blockIdx.x - t.b * a.seq_len;
+  const int token = PROMPT ? blockIdx.x * kPromptWarps + threadIdx.x / 32 : blockIdx.x;
+  if (PROMPT && token >= a.batch * a.seq_len) return;
+  t.b = token / a.seq_len, t.s = token - t.b * a.seq_len;
   t.c = threadIdx.x % kTpr * kV;
   t.lanes = ((1u << kTpr) - 1u) << (threadIdx.x % 32 / kTpr * kTpr);
   const int hq = a.num_q_heads, hkv = a.num_kv_heads;
@@ -220,7 +225,7 @@ __global__ void __launch_bounds__(PROMPT ? 32 : 256, PROMPT ? 18 : 1)
     t.page = a.page_table[t.b * a.table_stride + i];
     if (t.page >= a.num_pages) t.page = -1;
   }
-  if (a.kv_lens_out != nullptr && t.s == 0 && threadIdx.x == 0)
+  if (a.kv_lens_out != nullptr && t.s == 0 && (PROMPT ? threadIdx.x % 32 : threadIdx.x) == 0)
     a.kv_lens_out[t.b] = (int)min((long long)max(pos, 0) + fresh, (long long)cap);
   const CS* cp = static_cast<const CS*>(a.cos) + t.b * a.cs_stride_b + t.s * a.cs_stride_s + t.c;
   const CS* sp = static_cast<const CS*>(a.sin) + t.b * a.cs_stride_b + t.s * a.cs_stride_s + t.c;
@@ -228,7 +233,7 @@ __global__ void __launch_bounds__(PROMPT ? 32 : 256, PROMPT ? 18 : 1)
   load_floats<CS, kV>(cp + D / 2, t.c2);
   load_floats<CS, kV>(sp, t.s1);
   load_floats<CS, kV>(sp + D / 2, t.s2);
-  const int r0 = threadIdx.x / kTpr;
+  const int r0 = (PROMPT ? threadIdx.x % 32 : threadIdx.x) / kTpr;
   if constexpr (PROMPT) {
     for (int h = 0; h < hq; h += 4 * kSlots) token_rows<T, CS, D, HALVES, 0, 4>(a, t, h + r0, kSlots, hq);
     for (int h = 0; h < hkv; h += 2 * kSlots) token_rows<T, CS, D, HALVES, 1, 2>(a, t, h + r0, kSlots, hkv);
@@ -245,14 +250,15 @@ __global__ void __launch_bounds__(PROMPT ? 32 : 256, PROMPT ? 18 : 1)
   }
 }
 
-constexpr int kPromptTokens = 384;
+constexpr int kPromptTokens = 600;  // see launch_append_sized
 
 template <typename T, typename CS, int D, bool HALVES>
 cudaError_t launch_append_sized(const aicas_paged_append_int4_params& p, cudaStream_t st) {
   const dim3 grid((unsigned)(p.batch * p.seq_len));
   return p.batch * p.seq_len <= kPromptTokens
              ? launch_pdl(paged_append_int4_kernel<T, CS, D, HALVES, false>, grid, dim3(256), 0, st, p)
-             : launch_pdl(paged_append_int4_kernel<T, CS, D, HALVES, true>, grid, dim3(32), 0, st, p);
+             : launch_pdl(paged_append_int4_kernel<T, CS, D, HALVES, true>, dim3((grid.x + kPromptWarps - 1) / kPromptWarps),
+                          dim3(32 * kPromptWarps), 0, st, p);
 }
 
 template <typename T, typename CS>
@@ -263,70 +269,100 @@ cudaError_t launch_append(const aicas_paged_append_int4_params& p, cudaStream_t 
 
 // ------------------------------------------------------------------ reads
 
-// HBM bound: 8 elements a thread, 4 bytes of codes in and 16 bytes out, of ROWS rows of one
+// 4 bytes of codes and the row's pair to 8 elements.
+template <typename T>
+__device__ __forceinline__ uint4 widened(uint32_t u, uint32_t p) {
+  union {
+    uint32_t u;
+    T t[2];
+  } pair;
+  pair.u = p;
+  const float scale = Elem<T>::to_float(pair.t[0]), least = Elem<T>::to_float(pair.t[1]);
+  float f[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = fmaf(scale, (float)(u >> (4 * e) & 15u), least);
+  return pack_vec<T>(f);
+}
+
+// The row of slot pos + s, if it is to be read: page (else -1) and row in it.
+__device__ __forceinline__ int2 row_at(const aicas_paged_read_int4_params& a, int b, int pos, int fresh, int s) {
+  const long long slot = (long long)pos + s;
+  if (s >= fresh || slot < 0 || slot >= a.max_pages * a.page_size) return make_int2(-1, 0);
+  const int i = (int)((uint32_t)slot / (uint32_t)a.page_size);
+  const int page = a.page_table[b * a.table_stride + i];
+  return make_int2(page < a.num_pages ? page : -1, (int)slot - i * a.page_size);
+}
+
+// HBM bound: 16 elements a thread, 8 bytes of codes in and 32 bytes out, of ROWS rows of one
 // request, side and head, so that their page numbers, codes and pairs are on the way at once.
 template <typename T, int D, bool HALVES, int ROWS>
 __global__ void __launch_bounds__(256) paged_read_int4_kernel(const __grid_constant__ aicas_paged_read_int4_params a, int chunks) {
-  constexpr int kTpr = D / 8;
-  const int slots = blockDim.x / kTpr;
+  constexpr int kTpr = D / 16, kSlots = 256 / kTpr;
   const int b = blockIdx.x / chunks, h = blockIdx.y >> 1, side = blockIdx.y & 1;
-  const int c = threadIdx.x % kTpr * 8, s0 = (blockIdx.x - b * chunks) * slots * ROWS + threadIdx.x / kTpr;
+  const int c = threadIdx.x % kTpr * 16, s0 = (blockIdx.x - b * chunks) * kSlots * ROWS + threadIdx.x / kTpr;
   grid_launch_dependents();
   grid_dependency_wait();
   const int fresh = a.num_tokens != nullptr ? min(a.num_tokens[b], a.seq_len) : a.seq_len;
-  const int pos = a.positions[b], cap = a.max_pages * a.page_size;
+  const int pos = a.positions[b];
   const aicas_int4_pages& from = a.kv[side];
   const uint8_t* codes = static_cast<const uint8_t*>(from.codes) + h * from.cs_h + c / 2;
   const T* pairs = static_cast<const T*>(from.scales) + h * from.ss_h + (HALVES && c >= D / 2 ? 2 : 0);
-  int page[ROWS], row[ROWS];
+  int2 at[ROWS];
+#pragma unroll
+  for (int j = 0; j < ROWS; ++j) at[j] = row_at(a, b, pos, fresh, s0 + j * kSlots);
+  uint2 u[ROWS];
+  uint32_t p[ROWS];
 #pragma unroll
   for (int j = 0; j < ROWS; ++j) {
-    const int s = s0 + j * slots;
-    const long long slot = (long long)pos + s;
-    page[j] = -1, row[j] = 0;
-    if (s < fresh && slot >= 0 && slot < cap) {
-      const int i = (int)((uint32_t)slot / (uint32_t)a.page_size);
-      row[j] = (int)slot - i * a.page_size;
-      page[j] = a.page_table[b * a.table_stride + i];
-    }
-  }
-  uint32_t u[ROWS], p[ROWS];
-#pragma unroll
-  for (int j = 0; j < ROWS; ++j) {
-    u[j] = p[j] = 0;
-    if (page[j] >= 0 && page[j] < a.num_pages) {
-      u[j] = *reinterpret_cast<const uint32_t*>(codes + page[j] * from.cs_p + row[j] * from.cs_t);
-      p[j] = *reinterpret_cast<const uint32_t*>(pairs + page[j] * from.ss_p + row[j] * from.ss_t);
+    u[j] = make_uint2(0, 0), p[j] = 0;
+    if (at[j].x >= 0) {
+      u[j] = *reinterpret_cast<const uint2*>(codes + at[j].x * from.cs_p + at[j].y * from.cs_t);
+      p[j] = *reinterpret_cast<const uint32_t*>(pairs + at[j].x * from.ss_p + at[j].y * from.ss_t);
     }
   }
   T* out = static_cast<T*>(a.out[side]) + b * a.out_stride_b + h * a.out_stride_h + c;
 #pragma unroll
   for (int j = 0; j < ROWS; ++j) {
-    const int s = s0 + j * slots;
+    const int s = s0 + j * kSlots;
     if (s >= a.seq_len) break;
-    union {
-      uint32_t u;
-      T t[2];
-    } pair;
-    pair.u = p[j];
-    const float scale = Elem<T>::to_float(pair.t[0]), least = Elem<T>::to_float(pair.t[1]);
-    float f[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = fmaf(scale, (float)(u[j] >> (4 * e) & 15u), least);
-    *reinterpret_cast<uint4*>(out + (int64_t)s * a.out_stride_s) = pack_vec<T>(f);
+    uint4* to = reinterpret_cast<uint4*>(out + (int64_t)s * a.out_stride_s);
+    to[0] = widened<T>(u[j].x, p[j]);
+    to[1] = widened<T>(u[j].y, p[j]);
+  }
+}
+
+// The few rows of a decode step: a CTA a request, all its rows at once.
+template <typename T, int D, bool HALVES>
+__global__ void __launch_bounds__(256) paged_read_few_int4_kernel(const __grid_constant__ aicas_paged_read_int4_params a) {
+  constexpr int kTpr = D / 8, kSlots = 256 / kTpr;
+  const int b = blockIdx.x, c = threadIdx.x % kTpr * 8;
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int fresh = a.num_tokens != nullptr ? min(a.num_tokens[b], a.seq_len) : a.seq_len;
+  const int pos = a.positions[b];
+  for (int r = threadIdx.x / kTpr; r < 2 * a.num_kv_heads * a.seq_len; r += kSlots) {
+    const int head = a.seq_len == 1 ? r : r / a.seq_len, s = r - head * a.seq_len, h = head >> 1, side = head & 1;
+    const aicas_int4_pages& from = a.kv[side];
+    const int2 at = row_at(a, b, pos, fresh, s);
+    uint32_t u = 0, p = 0;
+    if (at.x >= 0) {
+      u = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(from.codes) + at.x * from.cs_p + h * from.cs_h +
+                                             at.y * from.cs_t + c / 2);
+      p = *reinterpret_cast<const uint32_t*>(static_cast<const T*>(from.scales) + at.x * from.ss_p + h * from.ss_h +
+                                             at.y * from.ss_t + (HALVES && c >= D / 2 ? 2 : 0));
+    }
+    *reinterpret_cast<uint4*>(static_cast<T*>(a.out[side]) + b * a.out_stride_b + h * a.out_stride_h + s * a.out_stride_s + c) =
+        widened<T>(u, p);
   }
 }
 
 template <typename T, int D, bool HALVES>
 cudaError_t launch_read_sized(const aicas_paged_read_int4_params& p, cudaStream_t st) {
-  constexpr int kTpr = D / 8;
-  // few rows a request (a decode step): CTAs as small as they go; many: four rows a thread
-  const bool few = p.seq_len * kTpr <= 256;
-  const int threads = few ? (p.seq_len * kTpr + 31) / 32 * 32 : 256;
-  const int64_t rows = (int64_t)threads / kTpr * (few ? 1 : 4), chunks = (p.seq_len + rows - 1) / rows;
+  if ((int64_t)p.num_kv_heads * p.seq_len * (D / 8) <= 512)
+    return launch_pdl(paged_read_few_int4_kernel<T, D, HALVES>, dim3((unsigned)p.batch), dim3(256), 0, st, p);
+  const int64_t rows = 256 / (D / 16) * 2, chunks = (p.seq_len + rows - 1) / rows;
   const dim3 grid((unsigned)(chunks * p.batch), 2u * p.num_kv_heads);
-  return few ? launch_pdl(paged_read_int4_kernel<T, D, HALVES, 1>, grid, dim3(threads), 0, st, p, (int)chunks)
-             : launch_pdl(paged_read_int4_kernel<T, D, HALVES, 4>, grid, dim3(threads), 0, st, p, (int)chunks);
+  return launch_pdl(paged_read_int4_kernel<T, D, HALVES, 2>, grid, dim3(256), 0, st, p, (int)chunks);
 }
 
 template <typename T>
