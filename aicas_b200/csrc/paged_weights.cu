@@ -2,111 +2,483 @@
 //   w[b, h, t] += sum over queries s and heads j of the group of 2^(c q[b, j, s].k[b, h, t] - lse[b, j, s]),
 // c = scale log2(e), for the slots start <= t <= len - S + s that query s sees.
 //
-// A slot has one writer and its sum one order, so results repeat to the bit.  A thread a
-// slot, its row of K read once for each block of 8 queries.
+// A slot has one writer and its sum one order, so results repeat to the bit.
+//
+// 16-bit and 4-bit pages: K is read once, straight into the fragments of mma.sync
+// m16n8k16 (16 slots as rows, 8 queries as columns): a sum over the dims may take them
+// in any order, so a lane takes 16 bytes (or 8 of codes) of its row, and q's fragments are
+// laid out to match, in shared memory, once for the runs of slots of one (request, KV head).  A
+// warp's next rows are on their way while it multiplies.  Codes enter as paged_int4_decode.cu
+// says.  Queries beyond 8 reuse the fragments of K.
+//   * Work: tiles of kTile slots of all (request, KV head) pairs in equal runs a warp, cut
+//     on the device from the lengths.
+//   * Rounding: products of 16-bit numbers are exact, sums and weights fp32.
+//
+// fp32 pages: a thread a slot, its row read once for each block of 8 queries.
 #include <cstdio>
+#include <cstring>
 #include <type_traits>
 
 #include "common.cuh"
 #include "paged_int4.cuh"
+#include "paged_split.cuh"
 
 namespace aicas {
 namespace {
 
-constexpr int kThreads = 128, kBlock = 8;
+constexpr int kLogWarps = 3, kWarps = 1 << kLogWarps, kThreads = kWarps * 32;
+constexpr int kCols = 8;        // queries a product
+constexpr int kMostCols = 128;  // queries whose fragments shared memory holds at once
+constexpr float kCodeUnit = 16777216.f;  // 2^24: a code in an fp16's low bits is code / kCodeUnit
 
-// 8 elements d.. of a cached row, as floats.
-template <typename T, bool INT4>
-__device__ __forceinline__ void load_row8(const aicas_paged_weights_params& a, int page, int h, int row, int d, float* f) {
-  if constexpr (INT4) {
-    const uint32_t u = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.k_pages) + page * a.kp_stride_p +
-                                                          h * a.kp_stride_h + row * a.kp_stride_t + d / 2);
-    const T* pair = static_cast<const T*>(a.k_scales) + page * a.ks_stride_p + h * a.ks_stride_h + row * a.ks_stride_t +
-                    d / a.group_size * 2;
-    const float s = Elem<T>::to_float(pair[0]), least = Elem<T>::to_float(pair[1]);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = fmaf(s, (float)(u >> (4 * e) & 15u), least);
+struct WeighArgs {
+  aicas_paged_weights_params p;
+  // what paged_split.cuh asks for
+  const int32_t* lens;
+  const int32_t* starts;
+  int batch, hkv, row_blocks, cap, few;
+  int group, cols;       // queries of a KV head: heads of the group times window
+  int octets;            // of 8 rows a page has
+  uint32_t octets_mul;   // n / octets = (umulhi(n, octets_mul) + n) >> octets_shift
+  int octets_shift;
+  float scale_log2;
+};
+
+template <typename T> struct Mma;
+template <> struct Mma<__nv_bfloat16> {
+  __device__ __forceinline__ static void run(float c[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+};
+template <> struct Mma<__half> {
+  __device__ __forceinline__ static void run(float c[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T>
+__device__ __forceinline__ float2 pair_of(uint32_t u) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
   } else {
-    const T* p = static_cast<const T*>(a.k_pages) + page * a.kp_stride_p + h * a.kp_stride_h + row * a.kp_stride_t + d;
-#pragma unroll
-    for (int e = 0; e < 8; e += Elem<T>::kPerVec) Elem<T>::unpack(*reinterpret_cast<const uint4*>(p + e), f + e);
+    return __half22float2(*reinterpret_cast<const __half2*>(&u));
   }
 }
 
-template <typename T, bool INT4>
-__global__ void __launch_bounds__(kThreads) paged_weights_kernel(const __grid_constant__ aicas_paged_weights_params a) {
-  __shared__ float q_s[kBlock][128], lse_s[kBlock];
-  __shared__ int end_s[kBlock];
+__device__ __forceinline__ uint32_t pack_half(float x, float y) {
+  union {
+    __half2 h;
+    uint32_t u;
+  } r;
+  r.h = __floats2half2_rn(x, y);
+  return r.u;
+}
+
+// GD: groups a row of 4-bit pages; 0: 16-bit pages.  A lane's share of a row in words: pairs
+// of dims (16-bit; it has 16 bytes of each 64, of heads of 16 all in 8), or 8 codes (8 bytes of each 32).
+template <int D, int GD>
+struct WeighCfg {
+  static constexpr bool k4 = GD > 0;
+  static constexpr int kG = k4 ? GD : 1;
+  static constexpr int kMt = k4 ? 2 : 1;            // products' 16 slots a tile
+  static constexpr int kTile = 16 * kMt, kOct = 2 * kMt;
+  static constexpr int kWords = k4 ? D / 32 : D / 8;
+  static constexpr int kSteps = D / 16;
+  static constexpr int kFrag = 2 * kSteps;          // words of q's fragments a lane and 8 queries
+};
+
+// What a lane has of a column of 8 queries: of its scores, factor, addends by group, -lse.
+template <int G>
+struct Column {
+  float factor, least[G], minus_lse;
+  int end;  // it sees slots below
+};
+
+// The fragments of query `col` of a pair (request b, head kvh), of which the four lanes i have a share each.
+template <typename T, int D, int GD>
+__device__ __forceinline__ void load_query(const WeighArgs& a, int b, int kvh, int len, int col, uint32_t* q,
+                                           Column<WeighCfg<D, GD>::kG>& m) {
+  using C = WeighCfg<D, GD>;
+  const int i = threadIdx.x & 3, S = a.p.seq_len;
+  const bool there = col < a.cols;
+  const int j = there ? col / S : 0, s = there ? col - j * S : 0, head = kvh * a.group + j;
+  const T* src = static_cast<const T*>(a.p.q) + b * a.p.q_stride_b + head * a.p.q_stride_h + s * a.p.q_stride_s;
+  const float lse = a.p.lse[b * a.p.lse_stride_b + head * a.p.lse_stride_h + s * a.p.lse_stride_s];
+  // a query that saw nothing, and columns that are none, add 2^-inf
+  m.minus_lse = there && lse != -INFINITY ? -lse : -INFINITY;
+  m.end = len - S + 1 + s;
+  m.factor = a.scale_log2;
+#pragma unroll
+  for (int e = 0; e < C::kG; ++e) m.least[e] = 0.f;
+  if constexpr (!C::k4) {
+    if constexpr (D == 16) {
+      const uint2 u = *reinterpret_cast<const uint2*>(src + 4 * i);
+      q[0] = u.x, q[1] = u.y;
+    } else {
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        const uint4 u = *reinterpret_cast<const uint4*>(src + 32 * c + 8 * i);
+        q[4 * c] = u.x, q[4 * c + 1] = u.y, q[4 * c + 2] = u.z, q[4 * c + 3] = u.w;
+      }
+    }
+  } else {
+    float x[C::kWords][8], top = 0.f, sum[GD] = {};
+#pragma unroll
+    for (int w = 0; w < C::kWords; ++w) {  // dims 64 (w / 2) + 16 i + 8 (w % 2)
+      Elem<T>::unpack(*reinterpret_cast<const uint4*>(src + 64 * (w / 2) + 16 * i + 8 * (w % 2)), x[w]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        top = fmaxf(top, fabsf(x[w][e]));
+        sum[w * GD / C::kWords] += x[w][e];
+      }
+    }
+#pragma unroll
+    for (int off = 1; off < 4; off <<= 1) {
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+#pragma unroll
+      for (int e = 0; e < GD; ++e) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], off);
+    }
+    // scaled by a power of two, so that the largest is in [2^14, 2^15): paged_int4_decode.cu
+    const int E = (int)(__float_as_uint(top) >> 23) - 127;
+    const int up = top > 0.f && E < 128 && E > -100 ? 14 - E : 0;
+    const float by = __uint_as_float((uint32_t)(up + 127) << 23);
+    m.factor = __uint_as_float((uint32_t)(127 - up) << 23) * kCodeUnit * a.scale_log2;
+#pragma unroll
+    for (int e = 0; e < GD; ++e) m.least[e] = sum[e] * a.scale_log2;
+#pragma unroll
+    for (int w = 0; w < C::kWords; ++w) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[w][e] *= by;
+      q[4 * w] = pack_half(x[w][0], x[w][4]);
+      q[4 * w + 1] = pack_half(x[w][1] * 0.0625f, x[w][5] * 0.0625f);
+      q[4 * w + 2] = pack_half(x[w][2], x[w][6]);
+      q[4 * w + 3] = pack_half(x[w][3] * 0.0625f, x[w][7] * 0.0625f);
+    }
+  }
+}
+
+// A lane's share of a tile: rows g and g + 8 of each 16 slots.
+template <int D, int GD>
+struct WeighTile {
+  using C = WeighCfg<D, GD>;
+  uint32_t k[C::kMt][2][C::kWords], pair[C::kMt][2][C::kG];
+
+  // page, row: of octet o of the tile in the four lanes' `from + o`.
+  __device__ __forceinline__ void load(const WeighArgs& a, int head, int page, int row, int from) {
+    const int g = (threadIdx.x & 31) >> 2, i = threadIdx.x & 3;
+#pragma unroll
+    for (int o = 0; o < C::kOct; ++o) {
+      const int pg = __shfl_sync(0xffffffffu, page, from + o), r = __shfl_sync(0xffffffffu, row, from + o) + g;
+      uint32_t* w = k[o >> 1][o & 1];
+#pragma unroll
+      for (int e = 0; e < C::kWords; ++e) w[e] = 0u;
+#pragma unroll
+      for (int e = 0; e < C::kG; ++e) pair[o >> 1][o & 1][e] = 0u;
+      if (pg < 0) continue;
+      const int64_t at = pg * a.p.kp_stride_p + head * a.p.kp_stride_h + r * a.p.kp_stride_t;
+      if constexpr (C::k4) {
+        const uint8_t* p = static_cast<const uint8_t*>(a.p.k_pages) + at + 8 * i;
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h) {
+          const uint2 u = __ldg(reinterpret_cast<const uint2*>(p + 32 * h));
+          w[2 * h] = u.x, w[2 * h + 1] = u.y;
+        }
+        const uint16_t* s = static_cast<const uint16_t*>(a.p.k_scales) + pg * a.p.ks_stride_p + head * a.p.ks_stride_h + r * a.p.ks_stride_t;
+        if constexpr (GD == 2) {
+          const uint2 u = __ldg(reinterpret_cast<const uint2*>(s));
+          pair[o >> 1][o & 1][0] = u.x, pair[o >> 1][o & 1][1] = u.y;
+        } else {
+          pair[o >> 1][o & 1][0] = __ldg(reinterpret_cast<const uint32_t*>(s));
+        }
+      } else {
+        const uint16_t* p = static_cast<const uint16_t*>(a.p.k_pages) + at;
+        if constexpr (D == 16) {
+          const uint2 u = __ldg(reinterpret_cast<const uint2*>(p + 4 * i));
+          w[0] = u.x, w[1] = u.y;
+        } else {
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4*>(p + 32 * c + 8 * i));
+            w[4 * c] = u.x, w[4 * c + 1] = u.y, w[4 * c + 2] = u.z, w[4 * c + 3] = u.w;
+          }
+        }
+      }
+    }
+  }
+
+  // The products' operand of 16 slots.
+  __device__ __forceinline__ void operand(int mt, uint32_t (&f)[C::kSteps][4]) const {
+#pragma unroll
+    for (int s = 0; s < C::kSteps; ++s) {
+      if constexpr (C::k4) {  // half a word of codes
+        const uint32_t w0 = k[mt][0][s / 2] >> (s & 1 ? 8 : 0), w1 = k[mt][1][s / 2] >> (s & 1 ? 8 : 0);
+        f[s][0] = w0 & 0x000f000fu, f[s][1] = w1 & 0x000f000fu, f[s][2] = w0 & 0x00f000f0u, f[s][3] = w1 & 0x00f000f0u;
+      } else {
+        f[s][0] = k[mt][0][2 * s], f[s][1] = k[mt][1][2 * s], f[s][2] = k[mt][0][2 * s + 1], f[s][3] = k[mt][1][2 * s + 1];
+      }
+    }
+  }
+};
+
+// Adds the weights of 8 queries (of which a lane has columns c[0] and c[1]) for 16 slots to s0 (row g) and s1 (row g + 8).
+template <typename T, int D, int GD>
+__device__ __forceinline__ void add_columns(const uint32_t (&f)[WeighCfg<D, GD>::kSteps][4], const uint32_t* q,
+                                            const uint32_t (&pair)[2][WeighCfg<D, GD>::kG],
+                                            const Column<WeighCfg<D, GD>::kG> (&c)[2], int slot, bool causal, float& s0, float& s1) {
+  using C = WeighCfg<D, GD>;
+  using M = typename std::conditional<C::k4, __half, T>::type;
+  float acc[C::kG][4] = {};
+#pragma unroll
+  for (int s = 0; s < C::kSteps; ++s)
+    Mma<M>::run(acc[s * C::kG / C::kSteps], f[s][0], f[s][1], f[s][2], f[s][3], q[2 * s], q[2 * s + 1]);
+#pragma unroll
+  for (int half = 0; half < 2; ++half)
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      float s = c[n].minus_lse;
+      if constexpr (C::k4) {
+#pragma unroll
+        for (int e = 0; e < C::kG; ++e) {
+          const float2 k = pair_of<T>(pair[half][e]);
+          s = fmaf(acc[e][2 * half + n] * c[n].factor, k.x, fmaf(k.y, c[n].least[e], s));
+        }
+      } else {
+        s = fmaf(acc[0][2 * half + n], c[n].factor, s);
+      }
+      float p = exp2_fast(s);
+      if (causal && slot + 8 * half >= c[n].end) p = 0.f;
+      (half ? s1 : s0) += p;
+    }
+}
+
+template <typename T, int D, int GD, bool MANY>
+__global__ void __launch_bounds__(kThreads, 2) paged_weights_kernel(const __grid_constant__ WeighArgs a) {
+  using C = WeighCfg<D, GD>;
+  using Col = Column<C::kG>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  // MANY: [8 queries][lane][kFrag] words of q, then the columns
+  uint32_t* q_s = reinterpret_cast<uint32_t*>(smem);
+  Col* col_s = reinterpret_cast<Col*>(smem + (MANY ? min(a.cols, kMostCols) + kCols - 1 : 0) / kCols * 32 * C::kFrag * 4);
+  constexpr int kVec = C::kFrag < 4 ? C::kFrag : 4;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, i = lane & 3;
+  grid_launch_dependents();
+  grid_dependency_wait();
+  Split<C::kTile> split = {};
+  // one warp for itself, or (MANY) a CTA on one pair at a time
+  split.template find<kLogWarps, kLogWarps, MANY ? 0 : (1 << 20), 1, 0>(a);
+  if (!split.busy) return;
+  const int team = 1 << split.log, rank = warp & (team - 1);
+  Segment<C::kTile> seg = split.seg;
+  for (bool more = true; more; more = seg.next(a)) {
+    if (seg.t0 == seg.t1) continue;
+    const int kvh = seg.pair, b = seg.b;
+    for (int c0 = 0; c0 < a.cols; c0 += MANY ? kMostCols : kCols) {
+      const int blocks = MANY ? (min(a.cols - c0, kMostCols) + kCols - 1) / kCols : 1;
+      uint32_t q[C::kFrag];
+      Col mine, c[2];
+      if constexpr (MANY) {
+        __syncthreads();  // the last ones are done with
+        for (int n = warp; n < blocks; n += kWarps) {
+          load_query<T, D, GD>(a, b, kvh, seg.len, c0 + n * kCols + g, q, mine);
+#pragma unroll
+          for (int e = 0; e < C::kFrag; ++e) q_s[(n * C::kFrag + e / kVec * kVec) * 32 + kVec * lane + e % kVec] = q[e];
+          if (i == 0) col_s[n * kCols + g] = mine;
+        }
+        __syncthreads();
+      } else {
+        load_query<T, D, GD>(a, b, kvh, seg.len, c0 + g, q, mine);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const int from = 4 * (2 * i + n);
+          c[n].factor = __shfl_sync(0xffffffffu, mine.factor, from);
+          c[n].minus_lse = __shfl_sync(0xffffffffu, mine.minus_lse, from);
+          c[n].end = __shfl_sync(0xffffffffu, mine.end, from);
+#pragma unroll
+          for (int e = 0; e < C::kG; ++e) c[n].least[e] = __shfl_sync(0xffffffffu, mine.least[e], from);
+        }
+      }
+      float* w = a.p.weights + b * a.p.w_stride_b + kvh * a.p.w_stride_h;
+      // the tiles' page numbers, 32 octets at once: octet lane % kOct of tile lane / kOct
+      int page = -1, row = 0, known = 0;
+      const auto look = [&](int t) {
+        const int n = (seg.first_tile + t + lane / C::kOct * team) * C::kOct + lane % C::kOct;
+        const int at = (int)((__umulhi((uint32_t)n, a.octets_mul) + (uint32_t)n) >> a.octets_shift);
+        row = 8 * (n - at * a.octets);
+        page = -1;
+        if (8 * n < seg.len && 8 * n + 8 > seg.start) page = a.p.page_table[b * a.p.table_stride + at];
+        if (page >= a.p.num_pages) page = -1;
+        known = 32 / C::kOct;
+      };
+      int t = seg.t0 + rank;
+      WeighTile<D, GD> tile;
+      if (t < seg.t1) {
+        look(t);
+        tile.load(a, kvh, page, row, 32 - known * C::kOct);
+        --known;
+      }
+      for (; t < seg.t1; t += team) {
+        const int slot = (seg.first_tile + t) * C::kTile;
+        // this lane's slot of the tile's sums
+        const int own = slot + (C::kMt == 2 ? 8 * i + g : 8 * (i & 1) + g);
+        const bool writes = own >= seg.start && own < seg.len && (C::kMt == 2 || i < 2);
+        const float old = writes ? w[own] : 0.f;
+        WeighTile<D, GD> next = {};
+        if (t + team < seg.t1) {
+          if (known == 0) look(t + team);
+          next.load(a, kvh, page, row, 32 - known * C::kOct);
+          --known;
+        }
+        const bool causal = a.p.seq_len > 1 && slot + C::kTile > seg.len - a.p.seq_len + 1;
+        float s = 0.f;
+#pragma unroll
+        for (int mt = 0; mt < C::kMt; ++mt) {
+          uint32_t f[C::kSteps][4];
+          tile.operand(mt, f);
+          float s0 = 0.f, s1 = 0.f;
+          if constexpr (MANY) {
+#pragma unroll 1
+            for (int n = 0; n < blocks; ++n) {
+#pragma unroll
+              for (int e = 0; e < C::kFrag; e += kVec) {
+                const uint32_t* from = q_s + (n * C::kFrag + e) * 32 + kVec * lane;
+                if constexpr (kVec == 4) {
+                  const uint4 u = *reinterpret_cast<const uint4*>(from);
+                  q[e] = u.x, q[e + 1] = u.y, q[e + 2] = u.z, q[e + 3] = u.w;
+                } else {
+                  const uint2 u = *reinterpret_cast<const uint2*>(from);
+                  q[e] = u.x, q[e + 1] = u.y;
+                }
+              }
+              c[0] = col_s[n * kCols + 2 * i], c[1] = col_s[n * kCols + 2 * i + 1];
+              add_columns<T, D, GD>(f, q, tile.pair[mt], c, slot + 16 * mt + g, causal, s0, s1);
+            }
+          } else {
+            add_columns<T, D, GD>(f, q, tile.pair[mt], c, slot + 16 * mt + g, causal, s0, s1);
+          }
+          s0 += __shfl_xor_sync(0xffffffffu, s0, 1), s1 += __shfl_xor_sync(0xffffffffu, s1, 1);
+          s0 += __shfl_xor_sync(0xffffffffu, s0, 2), s1 += __shfl_xor_sync(0xffffffffu, s1, 2);
+          if (C::kMt == 1 || (i >> 1) == mt) s = i & 1 ? s1 : s0;
+        }
+        if (writes) w[own] = old + s;
+        tile = next;
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ fp32 pages
+
+constexpr int kSlots32 = 128, kBlock32 = 8;
+
+__global__ void __launch_bounds__(kSlots32) paged_weights_f32_kernel(const __grid_constant__ aicas_paged_weights_params a) {
+  __shared__ float q_s[kBlock32][128], lse_s[kBlock32];
+  __shared__ int end_s[kBlock32];
   const int group = a.num_q_heads / a.num_kv_heads, D = a.head_dim, cap = a.max_pages * a.page_size;
-  const int chunks = (cap + kThreads - 1) / kThreads;
+  const int chunks = (cap + kSlots32 - 1) / kSlots32;
   const int kvh = blockIdx.x / chunks % a.num_kv_heads, b = blockIdx.x / chunks / a.num_kv_heads;
   grid_launch_dependents();
   grid_dependency_wait();
   const int len = a.kv_lens != nullptr ? min(max(a.kv_lens[b], 0), cap) : cap;
   const int start = a.kv_starts != nullptr ? max(a.kv_starts[b], 0) : 0;
-  const int t0 = blockIdx.x % chunks * kThreads, t = t0 + threadIdx.x;
-  if (t0 >= len || t0 + kThreads <= start) return;
-  int page = -1, row = 0;
-  if (t >= start && t < len) {
-    const int i = t / a.page_size;
-    row = t - i * a.page_size;
-    page = a.page_table[b * a.table_stride + i];
+  const int t0 = blockIdx.x % chunks * kSlots32, t = t0 + threadIdx.x;
+  if (t0 >= len || t0 + kSlots32 <= start) return;
+  const bool mine = t >= start && t < len;
+  const float* k = nullptr;
+  if (mine) {
+    const int i = t / a.page_size, page = a.page_table[b * a.table_stride + i];
+    if (page >= 0 && page < a.num_pages)
+      k = static_cast<const float*>(a.k_pages) + page * a.kp_stride_p + kvh * a.kp_stride_h + (t - i * a.page_size) * a.kp_stride_t;
   }
   const float c = a.sm_scale * 1.4426950408889634f;
   float sum = 0.f;
-  for (int r0 = 0; r0 < group * a.seq_len; r0 += kBlock) {
+  for (int r0 = 0; r0 < group * a.seq_len; r0 += kBlock32) {
     __syncthreads();
-    for (int x = threadIdx.x; x < kBlock * D; x += kThreads) {
+    for (int x = threadIdx.x; x < kBlock32 * D; x += kSlots32) {
       const int r = r0 + x / D, j = kvh * group + r / a.seq_len, s = r % a.seq_len;
-      if (r < group * a.seq_len) {
-        q_s[x / D][x % D] = Elem<T>::to_float(static_cast<const T*>(a.q)[b * a.q_stride_b + j * a.q_stride_h + s * a.q_stride_s + x % D]);
-        if (x % D == 0) {
-          lse_s[x / D] = a.lse[b * a.lse_stride_b + j * a.lse_stride_h + s * a.lse_stride_s];
-          end_s[x / D] = len - a.seq_len + 1 + s;
-        }
-      } else {
-        q_s[x / D][x % D] = 0.f;
-        if (x % D == 0) end_s[x / D] = 0;
+      const bool there = r < group * a.seq_len;
+      q_s[x / D][x % D] = there ? static_cast<const float*>(a.q)[b * a.q_stride_b + j * a.q_stride_h + s * a.q_stride_s + x % D] : 0.f;
+      if (x % D == 0) {
+        lse_s[x / D] = there ? a.lse[b * a.lse_stride_b + j * a.lse_stride_h + s * a.lse_stride_s] : -INFINITY;
+        end_s[x / D] = len - a.seq_len + 1 + s;
       }
     }
     __syncthreads();
-    if (t >= start && t < len) {
-      float s[kBlock] = {};
-      if (page >= 0 && page < a.num_pages)
-        for (int d = 0; d < D; d += 8) {
-          float k[8];
-          load_row8<T, INT4>(a, page, kvh, row, d, k);
+    if (!mine) continue;
+    float s[kBlock32] = {};
+    if (k != nullptr)
+      for (int d = 0; d < D; d += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(k + d);
 #pragma unroll
-          for (int r = 0; r < kBlock; ++r)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) s[r] = fmaf(q_s[r][d + e], k[e], s[r]);
+        for (int r = 0; r < kBlock32; ++r) {
+          const float4 y = *reinterpret_cast<const float4*>(&q_s[r][d]);
+          s[r] = fmaf(y.x, x.x, fmaf(y.y, x.y, fmaf(y.z, x.z, fmaf(y.w, x.w, s[r]))));
         }
+      }
 #pragma unroll
-      for (int r = 0; r < kBlock; ++r)
-        if (t < end_s[r] && lse_s[r] != -INFINITY) sum += exp2f(fmaf(s[r], c, -lse_s[r]));
-    }
+    for (int r = 0; r < kBlock32; ++r)
+      if (t < end_s[r] && lse_s[r] != -INFINITY) sum += exp2f(fmaf(s[r], c, -lse_s[r]));
   }
-  if (t >= start && t < len) a.weights[b * a.w_stride_b + kvh * a.w_stride_h + t] += sum;
+  if (mine) a.weights[b * a.w_stride_b + kvh * a.w_stride_h + t] += sum;
+}
+
+// ------------------------------------------------------------------ host side
+
+template <typename T, int D, int GD>
+cudaError_t launch_weigh(const WeighArgs& a, int sms, cudaStream_t st) {
+  using C = WeighCfg<D, GD>;
+  const int64_t tiles = ((int64_t)a.cap + C::kTile - 1) / C::kTile * a.batch * a.hkv;
+  const int64_t ctas = (tiles + kWarps - 1) / kWarps;
+  const dim3 grid((unsigned)(ctas < 2 * sms ? ctas : 2 * sms)), block(kThreads);
+  if (a.cols <= kCols) return launch_pdl(paged_weights_kernel<T, D, GD, false>, grid, block, 0, st, a);
+  const int cols = ((a.cols < kMostCols ? a.cols : kMostCols) + kCols - 1) / kCols * kCols;
+  const size_t smem = (size_t)cols / kCols * 32 * C::kFrag * 4 + (size_t)cols * sizeof(Column<C::kG>);
+  return launch_pdl(paged_weights_kernel<T, D, GD, true>, grid, block, smem, st, a);
 }
 
 template <typename T>
-cudaError_t launch_weights(const aicas_paged_weights_params& p, cudaStream_t st) {
-  const int64_t chunks = ((int64_t)p.max_pages * p.page_size + kThreads - 1) / kThreads;
-  const dim3 grid((unsigned)(chunks * p.batch * p.num_kv_heads)), block(kThreads);
-  if constexpr (!std::is_same<T, float>::value) {
-    if (p.group_size != 0) return launch_pdl(paged_weights_kernel<T, true>, grid, block, 0, st, p);
+cudaError_t dispatch_weigh(const WeighArgs& a, int sms, cudaStream_t st) {
+  const int D = a.p.head_dim;
+  if (a.p.group_size != 0)
+    return D == 64 ? launch_weigh<T, 64, 1>(a, sms, st) : a.p.group_size == 64 ? launch_weigh<T, 128, 2>(a, sms, st) : launch_weigh<T, 128, 1>(a, sms, st);
+  switch (D) {
+    case 16: return launch_weigh<T, 16, 0>(a, sms, st);
+    case 32: return launch_weigh<T, 32, 0>(a, sms, st);
+    case 64: return launch_weigh<T, 64, 0>(a, sms, st);
+    case 128: return launch_weigh<T, 128, 0>(a, sms, st);
   }
-  return launch_pdl(paged_weights_kernel<T, false>, grid, block, 0, st, p);
+  return cudaErrorInvalidValue;
 }
 
 }  // namespace
 
-int run_paged_weights(const aicas_paged_weights_params* p, int, cudaStream_t stream, char* err, size_t errlen) {
+int run_paged_weights(const aicas_paged_weights_params* p, int sms, cudaStream_t stream, char* err, size_t errlen) {
   cudaError_t e = cudaErrorInvalidValue;
-  switch (p->dtype) {
-    case AICAS_DTYPE_F32: e = launch_weights<float>(*p, stream); break;
-    case AICAS_DTYPE_F16: e = launch_weights<__half>(*p, stream); break;
-    case AICAS_DTYPE_BF16: e = launch_weights<__nv_bfloat16>(*p, stream); break;
+  if (p->dtype == AICAS_DTYPE_F32) {
+    const int64_t chunks = ((int64_t)p->max_pages * p->page_size + kSlots32 - 1) / kSlots32;
+    e = launch_pdl(paged_weights_f32_kernel, dim3((unsigned)(chunks * p->batch * p->num_kv_heads)), dim3(kSlots32), 0, stream, *p);
+  } else {
+    WeighArgs a;
+    memset(&a, 0, sizeof(a));
+    a.p = *p;
+    a.lens = p->kv_lens, a.starts = p->kv_starts;
+    a.batch = p->batch, a.hkv = p->num_kv_heads, a.row_blocks = 1, a.cap = p->max_pages * p->page_size;
+    a.group = p->num_q_heads / p->num_kv_heads, a.cols = a.group * p->seq_len;
+    // n / d for n < 2^28, as in paged_int4_decode.cu
+    a.octets = p->page_size / 8;
+    while ((1ll << a.octets_shift) < a.octets) ++a.octets_shift;
+    a.octets_mul = (uint32_t)((((1ull << a.octets_shift) - a.octets) << 32) / a.octets + 1);
+    a.scale_log2 = p->sm_scale * 1.4426950408889634f;
+    e = p->dtype == AICAS_DTYPE_F16 ? dispatch_weigh<__half>(a, sms, stream) : dispatch_weigh<__nv_bfloat16>(a, sms, stream);
   }
   if (e == cudaSuccess) return AICAS_OK;
   snprintf(err, errlen, "paged weights launch: %s (%s)", cudaGetErrorString(e), cudaGetErrorName(e));
