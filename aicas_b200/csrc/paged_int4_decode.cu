@@ -32,12 +32,12 @@
 
 #include "common.cuh"
 #include "paged_int4.cuh"
-#include "paged_split.cuh"
+#include "paged_int4_tiles.cuh"
 
 namespace aicas {
 namespace {
 
-constexpr int kTile = 32;      // slots a tile
+constexpr int kTile = kInt4Tile;
 constexpr int kRanges = 4;     // ranges that a pair is cut into, about
 constexpr int kPairCost = 3;   // what beginning and ending a pair costs a warp, in tiles
 constexpr int kSmallTiles = 32;  // most tiles a CTA of a launch that gives pairs whole CTAs
@@ -45,31 +45,16 @@ constexpr int kLogWarps = 4, kMaxWarps = 1 << kLogWarps;
 constexpr int kSmallLog = 2;   // warps of a team in a small launch
 constexpr int kHeads = 8;      // query heads of a block
 constexpr size_t kWsCounters = (size_t)1 << 20;  // counter region shared with the other decode kernels
-constexpr float kCodeUnit = 16777216.f;  // 2^24: a code in an fp16's low bits is code / kCodeUnit
-
-// One side's pages: strides of the codes in 16 bytes, of the pairs in kPair bytes.
-struct Side {
-  const uint8_t* codes;
-  const uint8_t* pairs;
-  uint32_t cs_p, cs_h, cs_t, ss_p, ss_h, ss_t;
-};
-
 struct Int4Args {
-  Side kv[2];
+  Int4Source src;
   const void* q;
   void* out;
   float* lse;
-  const int32_t* table;
   const int32_t* lens;
   const int32_t* starts;
-  int64_t q_sb, q_sh, o_sb, o_sh, table_stride;
-  int batch, hq, hkv, group, row_blocks;
-  int num_pages, cap;
-  int octets;              // of 8 rows a page has
-  uint32_t octets_mul;     // n / octets = (umulhi(n, octets_mul) + n) >> octets_shift
-  int octets_shift;
+  int64_t q_sb, q_sh, o_sb, o_sh;
+  int batch, hq, hkv, group, row_blocks, cap;
   int few;                 // at most half as many pairs as CTAs
-  int dense;               // rows follow one another within a page and head, on both sides
   int part_heads;          // heads that a partial result has room for
   float scale_log2;
   float* ws_o;             // [2 * teams][part_heads][D]
@@ -78,17 +63,11 @@ struct Int4Args {
 };
 
 template <int D, int GD>
-struct Int4Cfg {
-  static constexpr int kRow = D / 2;          // bytes of a row's codes
-  static constexpr int kChunks = kRow / 16;   // its 16-byte chunks
-  static constexpr int kPair = 4 * GD;        // bytes of a row's pairs
-  static constexpr int kOffV = kTile * kRow;
-  static constexpr int kOffPairs = 2 * kTile * kRow;  // a slot's pairs of K, then of V
-  static constexpr int kStage = kOffPairs + 2 * kTile * kPair;
+struct Int4Cfg : Int4Stage<D, GD, 2> {
   static constexpr int kWarps = kMaxWarps, kThreads = kWarps * 32;
   static constexpr int kStages = 2;
   static constexpr int kRedRow = D + 4;
-  static constexpr int kOffRed = kWarps * kStages * kStage;
+  static constexpr int kOffRed = kWarps * kStages * Int4Cfg::kStage;
   static constexpr int kOffVars = kOffRed + kWarps * kHeads * kRedRow * 4;
   static constexpr int kSmem = kOffVars + 4 * kWarps;
   static_assert(kSmem <= 232448, "shared memory");
@@ -96,61 +75,10 @@ struct Int4Cfg {
 
 using Seg = Segment<kTile>;
 
-// The 16-byte chunk where chunk c of row r is kept: the same chunk of 8 rows, which a
-// fragment load takes, lies in all banks once.
-template <int D>
-__device__ __forceinline__ int swizzled(int r, int c) {
-  return c ^ (D == 128 ? (r >> 1) & 3 : (r >> 2) & 1);
-}
-
-__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t r[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t r[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-
-template <int BYTES>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool there) {
-  if constexpr (BYTES == 16) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-  } else {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(there ? BYTES : 0)
-                 : "memory");
-  }
-}
-
-__device__ __forceinline__ void mma(float c[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
-}
-
-__device__ __forceinline__ uint32_t pack_half(float x, float y) {
-  union {
-    __half2 h;
-    uint32_t u;
-  } r;
-  r.h = __floats2half2_rn(x, y);
-  return r.u;
 }
 
 // hi = fp16(x), lo = fp16(x - hi) of two numbers: hi's and lo's packed.
@@ -164,108 +92,6 @@ __device__ __forceinline__ void split_half(float x, float y, uint32_t& hi, uint3
   hi = r.u;
   lo = pack_half(x - f.x, y - f.y);
 }
-
-template <typename T>
-__device__ __forceinline__ float2 pair_of(uint32_t u) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
-  } else {
-    return __half22float2(*reinterpret_cast<const __half2*>(&u));
-  }
-}
-
-// ------------------------------------------------------------------ copies
-
-// A warp's way through its tiles, ahead of the products.  The pages of 8 of its tiles are
-// looked up at once, a lane an octet (8 rows) of slots, so that the page table's way and the
-// division are paid once for them.
-template <int D, int GD>
-struct Cursor {
-  using C = Int4Cfg<D, GD>;
-  Seg seg;
-  int t;      // its next tile, in seg
-  int turn;   // the warp that takes seg's first tile
-  int known;  // tiles from t on whose pages are looked up; -1: no tile left
-  int page;   // of lane's octet lane % 4 of the tile lane / 4 of those 8: page number, -1: nothing to copy,
-  int row;    // and first row in the page
-
-  __device__ __forceinline__ void look(const Int4Args& a, int team) {
-    const int lane = threadIdx.x & 31;
-    const int n = (seg.first_tile + t + (lane >> 2) * team) * (kTile / 8) + (lane & 3);
-    const int i = (int)((__umulhi((uint32_t)n, a.octets_mul) + (uint32_t)n) >> a.octets_shift);
-    row = 8 * (n - i * a.octets);
-    page = -1;
-    if (8 * n < seg.len && 8 * n + 8 > seg.start) page = a.table[seg.b * a.table_stride + i];
-    if (page >= a.num_pages) page = -1;
-    known = 8;
-  }
-
-  // To the warp's first tile at or after the segment.
-  __device__ __forceinline__ void settle(const Int4Args& a, int rank, int team) {
-    for (;;) {
-      t = seg.t0 + ((rank - turn) & (team - 1));
-      if (t < seg.t1) return look(a, team);
-      turn = (turn + seg.t1 - seg.t0) & (team - 1);
-      if (!seg.next(a)) {
-        known = -1;
-        return;
-      }
-    }
-  }
-
-  __device__ __forceinline__ void begin(const Int4Args& a, const Seg& first, int rank, int team) {
-    seg = first, turn = 0;
-    settle(a, rank, team);
-  }
-
-  template <bool DENSE>
-  __device__ __forceinline__ void rows(const Int4Args& a, uint32_t stage, int pg, int first_row) {
-    const int lane = threadIdx.x & 31, o = lane >> 3, sub = lane & 7;
-    const uint32_t head = a.row_blocks == 1 ? seg.pair : seg.pair / a.row_blocks;
-    const bool there = pg >= 0;
-    const uint32_t at = there ? pg : 0;
-    constexpr int kAtOnce = 8 / C::kChunks;  // rows of an octet in one go
-    const int r = sub / C::kChunks, c = sub % C::kChunks;
-#pragma unroll
-    for (int side = 0; side < 2; ++side) {
-      const Side& p = a.kv[side];
-      const uint64_t unit = (uint64_t)at * p.cs_p + (uint64_t)head * p.cs_h +
-                            (DENSE ? (uint64_t)(uint32_t)((first_row + r) * C::kChunks + c) : (uint64_t)(uint32_t)(first_row + r) * p.cs_t + c);
-      const uint8_t* codes = p.codes + 16 * unit;
-      const uint64_t step = DENSE ? kAtOnce * C::kRow : (uint64_t)p.cs_t * (16 * kAtOnce);
-      const uint32_t dst = stage + side * C::kOffV + (8 * o + r) * C::kRow;
-#pragma unroll
-      for (int k = 0; k < C::kChunks; ++k)
-        copy_async<16>(dst + kAtOnce * k * C::kRow + 16 * swizzled<D>(r + kAtOnce * k, c), codes + k * step, there);
-      const uint64_t pair = (uint64_t)at * p.ss_p + (uint64_t)head * p.ss_h +
-                            (DENSE ? (uint64_t)(uint32_t)(first_row + sub) : (uint64_t)(uint32_t)(first_row + sub) * p.ss_t);
-      copy_async<C::kPair>(stage + C::kOffPairs + (2 * lane + side) * C::kPair, p.pairs + C::kPair * pair, there);
-    }
-  }
-
-  // Asks for the tile and goes on to the next one.
-  __device__ __forceinline__ void copy(const Int4Args& a, uint32_t stage, int rank, int team) {
-    if (known >= 0) {
-      const int from = 4 * (8 - known) + ((threadIdx.x & 31) >> 3);
-      const int pg = __shfl_sync(0xffffffffu, page, from), first_row = __shfl_sync(0xffffffffu, row, from);
-      if (a.dense)
-        rows<true>(a, stage, pg, first_row);
-      else
-        rows<false>(a, stage, pg, first_row);
-      t += team;
-      if (t >= seg.t1) {
-        turn = (turn + seg.t1 - seg.t0) & (team - 1);
-        if (seg.next(a))
-          settle(a, rank, team);
-        else
-          known = -1;
-      } else if (--known == 0) {
-        look(a, team);
-      }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  }
-};
 
 // ------------------------------------------------------------------ a warp's state
 
@@ -597,7 +423,7 @@ __global__ void __launch_bounds__(Int4Cfg<D, GD>::kThreads, 1) paged_decode_int4
   const uint32_t ring = smem_u32(smem) + warp * C::kStages * C::kStage;
   using State = Int4State<T, D, GD, WIDE>;
   uint4 raw[State::kWords];
-  Cursor<D, GD> ahead;
+  Cursor<D, GD, 2, Int4Args> ahead;
   if (split.busy) {
     State::ask(a, split.seg, raw);  // on its way while the tiles are asked for
     ahead.begin(a, split.seg, rank, team);
@@ -798,33 +624,16 @@ int run_paged_decode_int4(const aicas_paged_decode_int4_params* p, int sms, void
   const size_t workspace_bytes = paged_decode_int4_workspace(p, sms);
   Int4Args a;
   memset(&a, 0, sizeof(a));
-  for (int i = 0; i < 2; ++i) {
-    const aicas_int4_pages& from = p->kv[i];
-    const int64_t pair = 2 * (p->head_dim / p->group_size);  // elements
-    const int64_t st[] = {from.cs_p / 16, from.cs_h / 16, from.cs_t / 16, from.ss_p / pair, from.ss_h / pair, from.ss_t / pair};
-    for (int64_t s : st)
-      if (s > (int64_t)UINT32_MAX) {
-        snprintf(err, errlen, "page strides of 64 GB or more are not supported");
-        return AICAS_ERR_UNSUPPORTED;
-      }
-    a.kv[i] = {static_cast<const uint8_t*>(from.codes), static_cast<const uint8_t*>(from.scales), (uint32_t)st[0], (uint32_t)st[1],
-               (uint32_t)st[2], (uint32_t)st[3], (uint32_t)st[4], (uint32_t)st[5]};
-  }
+  if (!a.src.set(p->kv, 2, p->page_table, p->table_stride, p->head_dim, p->group_size, p->num_pages, p->page_size, err, errlen))
+    return AICAS_ERR_UNSUPPORTED;
   a.q = p->q, a.out = p->out, a.lse = p->lse;
-  a.table = p->page_table, a.lens = p->kv_lens, a.starts = p->kv_starts;
+  a.lens = p->kv_lens, a.starts = p->kv_starts;
   a.q_sb = p->q_stride_b, a.q_sh = p->q_stride_h, a.o_sb = p->o_stride_b, a.o_sh = p->o_stride_h;
-  a.table_stride = p->table_stride;
   a.batch = p->batch, a.hq = p->num_q_heads, a.hkv = p->num_kv_heads;
   a.group = p->num_q_heads / p->num_kv_heads;
   a.row_blocks = (a.group + kHeads - 1) / kHeads;
-  a.num_pages = p->num_pages, a.cap = p->max_pages * p->page_size;
-  // n / d for n < 2^28: with s = ceil(log2 d), (n + floor(n M / 2^32)) >> s, M = floor(2^32 (2^s - d) / d) + 1
-  a.octets = p->page_size / 8;
-  while ((1ll << a.octets_shift) < a.octets) ++a.octets_shift;
-  a.octets_mul = (uint32_t)((((1ull << a.octets_shift) - a.octets) << 32) / a.octets + 1);
+  a.cap = p->max_pages * p->page_size;
   a.scale_log2 = p->sm_scale * 1.4426950408889634f;
-  a.dense = 1;
-  for (const Side& x : a.kv) a.dense &= x.cs_t == (uint32_t)p->head_dim / 32 && x.ss_t == 1;
   const int grid = decode_grid(p, sms);
   a.few = 2 * (int64_t)a.batch * a.hkv * a.row_blocks <= grid;
   uint8_t* ws = static_cast<uint8_t*>(workspace);

@@ -4,14 +4,15 @@
 //
 // A slot has one writer and its sum one order, so results repeat to the bit.
 //
-// 16-bit and 4-bit pages: K is read once, straight into the fragments of mma.sync
-// m16n8k16 (16 slots as rows, 8 queries as columns): a sum over the dims may take them
-// in any order, so a lane takes 16 bytes (or 8 of codes) of its row, and q's fragments are
-// laid out to match, in shared memory, once for the runs of slots of one (request, KV head).  A
-// warp's next rows are on their way while it multiplies.  Codes enter as paged_int4_decode.cu
-// says.  Queries beyond 8 reuse the fragments of K.
-//   * Work: tiles of kTile slots of all (request, KV head) pairs in equal runs a warp, cut
-//     on the device from the lengths.
+// 16-bit and 4-bit pages: mma.sync m16n8k16 with 16 slots as rows and 8 queries as columns;
+// queries beyond 8 reuse K's fragments.  A sum over the dims may take them in any order,
+// so 16-bit rows go from global memory straight into fragments (16 bytes of a row a lane,
+// the next tile's on their way while a warp multiplies), with q's laid out to match.
+// 4-bit rows, four times as many in flight for the same bytes, come through a ring in
+// shared memory (paged_int4_tiles.cuh); the codes enter as paged_int4_decode.cu says.
+//   * Work: the tiles of all (request, KV head) pairs in equal runs, cut on the device from
+//     the lengths: a run a warp, or, with more than 8 queries, whose fragments the warps
+//     of a CTA share, a run a CTA.
 //   * Rounding: products of 16-bit numbers are exact, sums and weights fp32.
 //
 // fp32 pages: a thread a slot, its row read once for each block of 8 queries.
@@ -21,7 +22,7 @@
 
 #include "common.cuh"
 #include "paged_int4.cuh"
-#include "paged_split.cuh"
+#include "paged_int4_tiles.cuh"
 
 namespace aicas {
 namespace {
@@ -29,7 +30,6 @@ namespace {
 constexpr int kLogWarps = 3, kWarps = 1 << kLogWarps, kThreads = kWarps * 32;
 constexpr int kCols = 8;        // queries a product
 constexpr int kMostCols = 128;  // queries whose fragments shared memory holds at once
-constexpr float kCodeUnit = 16777216.f;  // 2^24: a code in an fp16's low bits is code / kCodeUnit
 
 struct WeighArgs {
   aicas_paged_weights_params p;
@@ -38,9 +38,7 @@ struct WeighArgs {
   const int32_t* starts;
   int batch, hkv, row_blocks, cap, few;
   int group, cols;       // queries of a KV head: heads of the group times window
-  int octets;            // of 8 rows a page has
-  uint32_t octets_mul;   // n / octets = (umulhi(n, octets_mul) + n) >> octets_shift
-  int octets_shift;
+  Int4Source src;        // 4-bit pages; of 16-bit ones the division by the octets of a page
   float scale_log2;
 };
 
@@ -60,41 +58,20 @@ template <> struct Mma<__half> {
   }
 };
 
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-template <typename T>
-__device__ __forceinline__ float2 pair_of(uint32_t u) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
-  } else {
-    return __half22float2(*reinterpret_cast<const __half2*>(&u));
-  }
-}
-
-__device__ __forceinline__ uint32_t pack_half(float x, float y) {
-  union {
-    __half2 h;
-    uint32_t u;
-  } r;
-  r.h = __floats2half2_rn(x, y);
-  return r.u;
-}
-
-// GD: groups a row of 4-bit pages; 0: 16-bit pages.  A lane's share of a row in words: pairs
-// of dims (16-bit; it has 16 bytes of each 64, of heads of 16 all in 8), or 8 codes (8 bytes of each 32).
+// GD: groups a row of 4-bit pages; 0: 16-bit pages.  Of each 32 dims a lane has 8, as words
+// of two dims or of 8 codes (of 16-bit heads of 16 it has 4 dims in all).
 template <int D, int GD>
 struct WeighCfg {
   static constexpr bool k4 = GD > 0;
   static constexpr int kG = k4 ? GD : 1;
   static constexpr int kMt = k4 ? 2 : 1;            // products' 16 slots a tile
-  static constexpr int kTile = 16 * kMt, kOct = 2 * kMt;
+  static constexpr int kTile = 16 * kMt;
   static constexpr int kWords = k4 ? D / 32 : D / 8;
   static constexpr int kSteps = D / 16;
   static constexpr int kFrag = 2 * kSteps;          // words of q's fragments a lane and 8 queries
+  using Stage = Int4Stage<k4 ? D : 64, kG, 1>;
+  static constexpr int kStages = 2;
+  static constexpr int kRing = k4 ? kWarps * kStages * Stage::kStage : 0;
 };
 
 // What a lane has of a column of 8 queries: of its scores, factor, addends by group, -lse.
@@ -134,8 +111,8 @@ __device__ __forceinline__ void load_query(const WeighArgs& a, int b, int kvh, i
   } else {
     float x[C::kWords][8], top = 0.f, sum[GD] = {};
 #pragma unroll
-    for (int w = 0; w < C::kWords; ++w) {  // dims 64 (w / 2) + 16 i + 8 (w % 2)
-      Elem<T>::unpack(*reinterpret_cast<const uint4*>(src + 64 * (w / 2) + 16 * i + 8 * (w % 2)), x[w]);
+    for (int w = 0; w < C::kWords; ++w) {
+      Elem<T>::unpack(*reinterpret_cast<const uint4*>(src + 32 * w + 8 * i), x[w]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         top = fmaxf(top, fabsf(x[w][e]));
@@ -173,45 +150,57 @@ struct WeighTile {
   using C = WeighCfg<D, GD>;
   uint32_t k[C::kMt][2][C::kWords], pair[C::kMt][2][C::kG];
 
-  // page, row: of octet o of the tile in the four lanes' `from + o`.
+  // 16-bit rows.  page, row: of octet o of the tile in lane from + o.
   __device__ __forceinline__ void load(const WeighArgs& a, int head, int page, int row, int from) {
     const int g = (threadIdx.x & 31) >> 2, i = threadIdx.x & 3;
 #pragma unroll
-    for (int o = 0; o < C::kOct; ++o) {
+    for (int o = 0; o < 2; ++o) {
       const int pg = __shfl_sync(0xffffffffu, page, from + o), r = __shfl_sync(0xffffffffu, row, from + o) + g;
-      uint32_t* w = k[o >> 1][o & 1];
+      uint32_t* w = k[0][o];
 #pragma unroll
       for (int e = 0; e < C::kWords; ++e) w[e] = 0u;
-#pragma unroll
-      for (int e = 0; e < C::kG; ++e) pair[o >> 1][o & 1][e] = 0u;
       if (pg < 0) continue;
-      const int64_t at = pg * a.p.kp_stride_p + head * a.p.kp_stride_h + r * a.p.kp_stride_t;
-      if constexpr (C::k4) {
-        const uint8_t* p = static_cast<const uint8_t*>(a.p.k_pages) + at + 8 * i;
-#pragma unroll
-        for (int h = 0; h < D / 64; ++h) {
-          const uint2 u = __ldg(reinterpret_cast<const uint2*>(p + 32 * h));
-          w[2 * h] = u.x, w[2 * h + 1] = u.y;
-        }
-        const uint16_t* s = static_cast<const uint16_t*>(a.p.k_scales) + pg * a.p.ks_stride_p + head * a.p.ks_stride_h + r * a.p.ks_stride_t;
-        if constexpr (GD == 2) {
-          const uint2 u = __ldg(reinterpret_cast<const uint2*>(s));
-          pair[o >> 1][o & 1][0] = u.x, pair[o >> 1][o & 1][1] = u.y;
-        } else {
-          pair[o >> 1][o & 1][0] = __ldg(reinterpret_cast<const uint32_t*>(s));
-        }
+      const uint16_t* p = static_cast<const uint16_t*>(a.p.k_pages) + pg * a.p.kp_stride_p + head * a.p.kp_stride_h + r * a.p.kp_stride_t;
+      if constexpr (D == 16) {
+        const uint2 u = __ldg(reinterpret_cast<const uint2*>(p + 4 * i));
+        w[0] = u.x, w[1] = u.y;
       } else {
-        const uint16_t* p = static_cast<const uint16_t*>(a.p.k_pages) + at;
-        if constexpr (D == 16) {
-          const uint2 u = __ldg(reinterpret_cast<const uint2*>(p + 4 * i));
-          w[0] = u.x, w[1] = u.y;
-        } else {
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            const uint4 u = __ldg(reinterpret_cast<const uint4*>(p + 32 * c + 8 * i));
-            w[4 * c] = u.x, w[4 * c + 1] = u.y, w[4 * c + 2] = u.z, w[4 * c + 3] = u.w;
-          }
+        for (int c = 0; c < D / 32; ++c) {
+          const uint4 u = __ldg(reinterpret_cast<const uint4*>(p + 32 * c + 8 * i));
+          w[4 * c] = u.x, w[4 * c + 1] = u.y, w[4 * c + 2] = u.z, w[4 * c + 3] = u.w;
         }
+      }
+    }
+  }
+
+  // 4-bit rows from a stage.
+  __device__ __forceinline__ void take(uint32_t at) {
+    using St = typename C::Stage;
+    const int lane = threadIdx.x & 31, mat = lane >> 3, r = lane & 7;
+    // D = 128: chunk mat of rows 0..7; D = 64: chunk mat / 2 of rows 0..7 and 8..15
+    const uint32_t from = at + (D == 128 ? r * St::kRow + 16 * swizzled<D>(r, mat)
+                                         : (r + 8 * (mat & 1)) * St::kRow + 16 * swizzled<D>(r, mat >> 1));
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+      uint32_t u[4];
+      ldsm_x4(from + 16 * mt * St::kRow, u);
+      if constexpr (D == 128) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) k[mt][0][e] = u[e];
+        ldsm_x4(from + (16 * mt + 8) * St::kRow, u);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) k[mt][1][e] = u[e];
+      } else {
+        k[mt][0][0] = u[0], k[mt][1][0] = u[1], k[mt][0][1] = u[2], k[mt][1][1] = u[3];
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t p = at + St::kOffPairs + (16 * mt + 8 * half + (lane >> 2)) * St::kPair;
+        if constexpr (GD == 2)
+          asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(pair[mt][half][0]), "=r"(pair[mt][half][1]) : "r"(p) : "memory");
+        else
+          asm volatile("ld.shared.u32 %0, [%1];" : "=r"(pair[mt][half][0]) : "r"(p) : "memory");
       }
     }
   }
@@ -230,60 +219,84 @@ struct WeighTile {
   }
 };
 
+// q(s): the words of steps s and s + 1 of q's fragments.
 // Adds the weights of 8 queries (of which a lane has columns c[0] and c[1]) for 16 slots to s0 (row g) and s1 (row g + 8).
-template <typename T, int D, int GD>
-__device__ __forceinline__ void add_columns(const uint32_t (&f)[WeighCfg<D, GD>::kSteps][4], const uint32_t* q,
+template <typename T, int D, int GD, typename Q>
+__device__ __forceinline__ void add_columns(const uint32_t (&f)[WeighCfg<D, GD>::kSteps][4], const Q& q,
                                             const uint32_t (&pair)[2][WeighCfg<D, GD>::kG],
                                             const Column<WeighCfg<D, GD>::kG> (&c)[2], int slot, bool causal, float& s0, float& s1) {
   using C = WeighCfg<D, GD>;
   using M = typename std::conditional<C::k4, __half, T>::type;
-  float acc[C::kG][4] = {};
+  constexpr int kChains = C::kG == 2 || C::kSteps == 1 ? C::kG : 2;  // of products that wait for one another
+  float acc[kChains][4] = {};
 #pragma unroll
-  for (int s = 0; s < C::kSteps; ++s)
-    Mma<M>::run(acc[s * C::kG / C::kSteps], f[s][0], f[s][1], f[s][2], f[s][3], q[2 * s], q[2 * s + 1]);
+  for (int s = 0; s < C::kSteps; s += 2) {
+    const uint4 u = q(s);  // of two steps
+    Mma<M>::run(acc[s * kChains / C::kSteps], f[s][0], f[s][1], f[s][2], f[s][3], u.x, u.y);
+    if (s + 1 < C::kSteps)
+      Mma<M>::run(acc[(s + 1) * kChains / C::kSteps], f[s + 1][0], f[s + 1][1], f[s + 1][2], f[s + 1][3], u.z, u.w);
+  }
+  float s[2][2];
 #pragma unroll
   for (int half = 0; half < 2; ++half)
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
-      float s = c[n].minus_lse;
+      float x = c[n].minus_lse;
       if constexpr (C::k4) {
 #pragma unroll
         for (int e = 0; e < C::kG; ++e) {
           const float2 k = pair_of<T>(pair[half][e]);
-          s = fmaf(acc[e][2 * half + n] * c[n].factor, k.x, fmaf(k.y, c[n].least[e], s));
+          const float sum = C::kG == kChains ? acc[e][2 * half + n] : acc[0][2 * half + n] + acc[kChains - 1][2 * half + n];
+          x = fmaf(sum * c[n].factor, k.x, fmaf(k.y, c[n].least[e], x));
         }
       } else {
-        s = fmaf(acc[0][2 * half + n], c[n].factor, s);
+        const float sum = kChains == 1 ? acc[0][2 * half + n] : acc[0][2 * half + n] + acc[kChains - 1][2 * half + n];
+        x = fmaf(sum, c[n].factor, x);
       }
-      float p = exp2_fast(s);
-      if (causal && slot + 8 * half >= c[n].end) p = 0.f;
-      (half ? s1 : s0) += p;
+      s[half][n] = x;
     }
+  if (causal) {  // the window's own tokens are in the tile
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+        if (slot + 8 * half >= c[n].end) s[half][n] = -INFINITY;
+  }
+  s0 += exp2_fast(s[0][0]) + exp2_fast(s[0][1]);
+  s1 += exp2_fast(s[1][0]) + exp2_fast(s[1][1]);
 }
 
 template <typename T, int D, int GD, bool MANY>
 __global__ void __launch_bounds__(kThreads, 2) paged_weights_kernel(const __grid_constant__ WeighArgs a) {
   using C = WeighCfg<D, GD>;
   using Col = Column<C::kG>;
-  extern __shared__ __align__(16) uint8_t smem[];
-  // MANY: [8 queries][lane][kFrag] words of q, then the columns
-  uint32_t* q_s = reinterpret_cast<uint32_t*>(smem);
-  Col* col_s = reinterpret_cast<Col*>(smem + (MANY ? min(a.cols, kMostCols) + kCols - 1 : 0) / kCols * 32 * C::kFrag * 4);
+  extern __shared__ __align__(128) uint8_t smem[];
+  // the ring of 4-bit rows; MANY: [8 queries][lane][kFrag] words of q, then the columns
+  uint32_t* q_s = reinterpret_cast<uint32_t*>(smem + C::kRing);
+  Col* col_s = reinterpret_cast<Col*>(smem + C::kRing + (MANY ? min(a.cols, kMostCols) + kCols - 1 : 0) / kCols * 32 * C::kFrag * 4);
   constexpr int kVec = C::kFrag < 4 ? C::kFrag : 4;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, i = lane & 3;
+  const uint32_t ring = smem_u32(smem) + warp * C::kStages * C::Stage::kStage;
   grid_launch_dependents();
   grid_dependency_wait();
   Split<C::kTile> split = {};
-  // one warp for itself, or (MANY) a CTA on one pair at a time
+  // a run a warp, or (MANY) a CTA
   split.template find<kLogWarps, kLogWarps, MANY ? 0 : (1 << 20), 1, 0>(a);
   if (!split.busy) return;
   const int team = 1 << split.log, rank = warp & (team - 1);
-  Segment<C::kTile> seg = split.seg;
-  for (bool more = true; more; more = seg.next(a)) {
-    if (seg.t0 == seg.t1) continue;
-    const int kvh = seg.pair, b = seg.b;
-    for (int c0 = 0; c0 < a.cols; c0 += MANY ? kMostCols : kCols) {
-      const int blocks = MANY ? (min(a.cols - c0, kMostCols) + kCols - 1) / kCols : 1;
+  for (int c0 = 0; c0 < a.cols; c0 += MANY ? kMostCols : kCols) {
+    const int blocks = MANY ? (min(a.cols - c0, kMostCols) + kCols - 1) / kCols : 1;
+    Segment<C::kTile> seg = split.seg;
+    Cursor<C::k4 ? D : 64, C::kG, 1, WeighArgs> ahead;
+    int stage = 0, turn = 0;  // turn: the warp that takes the segment's first tile
+    if constexpr (C::k4) {
+      ahead.begin(a, seg, rank, team);
+#pragma unroll
+      for (int k = 0; k < C::kStages; ++k) ahead.copy(a, ring + k * C::Stage::kStage, rank, team);
+    }
+    for (bool more = true; more; more = seg.next(a)) {
+      if (seg.t0 == seg.t1) continue;
+      const int kvh = seg.pair, b = seg.b;
       uint32_t q[C::kFrag];
       Col mine, c[2];
       if constexpr (MANY) {
@@ -307,47 +320,68 @@ __global__ void __launch_bounds__(kThreads, 2) paged_weights_kernel(const __grid
           for (int e = 0; e < C::kG; ++e) c[n].least[e] = __shfl_sync(0xffffffffu, mine.least[e], from);
         }
       }
+      // the words of two steps of q's fragments
+      const auto get = [&](int s) {
+        return make_uint4(q[2 * s], q[2 * s + 1], 2 * s + 2 < C::kFrag ? q[(2 * s + 2) % C::kFrag] : 0u,
+                          2 * s + 3 < C::kFrag ? q[(2 * s + 3) % C::kFrag] : 0u);
+      };
       float* w = a.p.weights + b * a.p.w_stride_b + kvh * a.p.w_stride_h;
-      // the tiles' page numbers, 32 octets at once: octet lane % kOct of tile lane / kOct
+      // 16-bit pages: the page numbers of 16 tiles at once, octet lane % 2 of tile lane / 2
       int page = -1, row = 0, known = 0;
       const auto look = [&](int t) {
-        const int n = (seg.first_tile + t + lane / C::kOct * team) * C::kOct + lane % C::kOct;
-        const int at = (int)((__umulhi((uint32_t)n, a.octets_mul) + (uint32_t)n) >> a.octets_shift);
-        row = 8 * (n - at * a.octets);
+        const int n = (seg.first_tile + t + (lane >> 1) * team) * 2 + (lane & 1);
+        const int at = (int)((__umulhi((uint32_t)n, a.src.octets_mul) + (uint32_t)n) >> a.src.octets_shift);
+        row = 8 * (n - at * a.src.octets);
         page = -1;
         if (8 * n < seg.len && 8 * n + 8 > seg.start) page = a.p.page_table[b * a.p.table_stride + at];
         if (page >= a.p.num_pages) page = -1;
-        known = 32 / C::kOct;
+        known = 16;
+      };
+      // a lane writes the sum of one slot: row g of half a product, which of 2 kMt halves by i; what it holds so far
+      const int place = 8 * i + g;
+      const auto held = [&](int t) {
+        const int own = (seg.first_tile + t) * C::kTile + place;
+        return i < 2 * C::kMt && t < seg.t1 && own >= seg.start && own < seg.len ? w[own] : 0.f;
       };
       int t = seg.t0 + rank;
-      WeighTile<D, GD> tile;
-      if (t < seg.t1) {
-        look(t);
-        tile.load(a, kvh, page, row, 32 - known * C::kOct);
-        --known;
+      if constexpr (C::k4) {  // in the order in which the tiles were asked for
+        t = seg.t0 + ((rank - turn) & (team - 1));
+        turn = (turn + seg.t1 - seg.t0) & (team - 1);
       }
+      float old = held(t);
+      WeighTile<D, GD> tile;
+      if (!C::k4 && t < seg.t1) {
+        look(t);
+        tile.load(a, kvh, page, row, 32 - 2 * known--);
+      }
+#pragma unroll 1
       for (; t < seg.t1; t += team) {
         const int slot = (seg.first_tile + t) * C::kTile;
-        // this lane's slot of the tile's sums
-        const int own = slot + (C::kMt == 2 ? 8 * i + g : 8 * (i & 1) + g);
-        const bool writes = own >= seg.start && own < seg.len && (C::kMt == 2 || i < 2);
-        const float old = writes ? w[own] : 0.f;
-        WeighTile<D, GD> next = {};
-        if (t + team < seg.t1) {
+        const float coming = held(t + team);
+        float mine_of_tile = 0.f;
+        WeighTile<D, GD> next;
+        if constexpr (C::k4) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 1) : "memory");
+          __syncwarp();  // every lane's copies have landed
+          const uint32_t at = ring + stage * C::Stage::kStage;
+          tile.take(at);
+          __syncwarp();  // every lane has read the stage
+          ahead.copy(a, at, rank, team);
+          if (++stage == C::kStages) stage = 0;
+        } else if (t + team < seg.t1) {
           if (known == 0) look(t + team);
-          next.load(a, kvh, page, row, 32 - known * C::kOct);
-          --known;
+          next.load(a, kvh, page, row, 32 - 2 * known--);
         }
         const bool causal = a.p.seq_len > 1 && slot + C::kTile > seg.len - a.p.seq_len + 1;
-        float s = 0.f;
 #pragma unroll
         for (int mt = 0; mt < C::kMt; ++mt) {
           uint32_t f[C::kSteps][4];
           tile.operand(mt, f);
           float s0 = 0.f, s1 = 0.f;
           if constexpr (MANY) {
-#pragma unroll 1
+#pragma unroll 2
             for (int n = 0; n < blocks; ++n) {
+              c[0] = col_s[n * kCols + 2 * i], c[1] = col_s[n * kCols + 2 * i + 1];
 #pragma unroll
               for (int e = 0; e < C::kFrag; e += kVec) {
                 const uint32_t* from = q_s + (n * C::kFrag + e) * 32 + kVec * lane;
@@ -359,20 +393,21 @@ __global__ void __launch_bounds__(kThreads, 2) paged_weights_kernel(const __grid
                   q[e] = u.x, q[e + 1] = u.y;
                 }
               }
-              c[0] = col_s[n * kCols + 2 * i], c[1] = col_s[n * kCols + 2 * i + 1];
-              add_columns<T, D, GD>(f, q, tile.pair[mt], c, slot + 16 * mt + g, causal, s0, s1);
+              add_columns<T, D, GD>(f, get, tile.pair[mt], c, slot + 16 * mt + g, causal, s0, s1);
             }
           } else {
-            add_columns<T, D, GD>(f, q, tile.pair[mt], c, slot + 16 * mt + g, causal, s0, s1);
+            add_columns<T, D, GD>(f, get, tile.pair[mt], c, slot + 16 * mt + g, causal, s0, s1);
           }
           s0 += __shfl_xor_sync(0xffffffffu, s0, 1), s1 += __shfl_xor_sync(0xffffffffu, s1, 1);
           s0 += __shfl_xor_sync(0xffffffffu, s0, 2), s1 += __shfl_xor_sync(0xffffffffu, s1, 2);
-          if (C::kMt == 1 || (i >> 1) == mt) s = i & 1 ? s1 : s0;
+          if ((i >> 1) == mt) mine_of_tile = i & 1 ? s1 : s0;
         }
-        if (writes) w[own] = old + s;
-        tile = next;
+        if (i < 2 * C::kMt && slot + place >= seg.start && slot + place < seg.len) w[slot + place] = old + mine_of_tile;
+        old = coming;
+        if constexpr (!C::k4) tile = next;
       }
     }
+    if (MANY && c0 + kMostCols < a.cols) __syncthreads();  // the slots' sums so far, before others add to them
   }
 }
 
@@ -436,13 +471,26 @@ __global__ void __launch_bounds__(kSlots32) paged_weights_f32_kernel(const __gri
 template <typename T, int D, int GD>
 cudaError_t launch_weigh(const WeighArgs& a, int sms, cudaStream_t st) {
   using C = WeighCfg<D, GD>;
+  const auto launch = [&](auto kernel, dim3 grid, size_t smem, bool (&attr_set)[64]) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (smem > 48 * 1024 && (dev < 0 || dev >= 64 || !attr_set[dev])) {
+      constexpr int kMost = C::kRing + kMostCols / kCols * 32 * C::kFrag * 4 + kMostCols * (int)sizeof(Column<C::kG>);
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+      if (e != cudaSuccess) return e;
+      if (dev >= 0 && dev < 64) attr_set[dev] = true;
+    }
+    return launch_pdl(kernel, grid, dim3(kThreads), smem, st, a);
+  };
+  static bool attr_few[64] = {false}, attr_many[64] = {false};
   const int64_t tiles = ((int64_t)a.cap + C::kTile - 1) / C::kTile * a.batch * a.hkv;
   const int64_t ctas = (tiles + kWarps - 1) / kWarps;
-  const dim3 grid((unsigned)(ctas < 2 * sms ? ctas : 2 * sms)), block(kThreads);
-  if (a.cols <= kCols) return launch_pdl(paged_weights_kernel<T, D, GD, false>, grid, block, 0, st, a);
+  const dim3 grid((unsigned)(ctas < 2 * sms ? ctas : 2 * sms));
+  if (a.cols <= kCols) return launch(paged_weights_kernel<T, D, GD, false>, grid, C::kRing, attr_few);
   const int cols = ((a.cols < kMostCols ? a.cols : kMostCols) + kCols - 1) / kCols * kCols;
-  const size_t smem = (size_t)cols / kCols * 32 * C::kFrag * 4 + (size_t)cols * sizeof(Column<C::kG>);
-  return launch_pdl(paged_weights_kernel<T, D, GD, true>, grid, block, smem, st, a);
+  const size_t smem = C::kRing + (size_t)cols / kCols * 32 * C::kFrag * 4 + (size_t)cols * sizeof(Column<C::kG>);
+  return launch(paged_weights_kernel<T, D, GD, true>, grid, smem, attr_many);
 }
 
 template <typename T>
@@ -473,10 +521,14 @@ int run_paged_weights(const aicas_paged_weights_params* p, int sms, cudaStream_t
     a.lens = p->kv_lens, a.starts = p->kv_starts;
     a.batch = p->batch, a.hkv = p->num_kv_heads, a.row_blocks = 1, a.cap = p->max_pages * p->page_size;
     a.group = p->num_q_heads / p->num_kv_heads, a.cols = a.group * p->seq_len;
-    // n / d for n < 2^28, as in paged_int4_decode.cu
-    a.octets = p->page_size / 8;
-    while ((1ll << a.octets_shift) < a.octets) ++a.octets_shift;
-    a.octets_mul = (uint32_t)((((1ull << a.octets_shift) - a.octets) << 32) / a.octets + 1);
+    if (p->group_size != 0) {
+      const aicas_int4_pages pages = {const_cast<void*>(p->k_pages), const_cast<void*>(p->k_scales), p->kp_stride_p, p->kp_stride_h,
+                                      p->kp_stride_t, p->ks_stride_p, p->ks_stride_h, p->ks_stride_t};
+      if (!a.src.set(&pages, 1, p->page_table, p->table_stride, p->head_dim, p->group_size, p->num_pages, p->page_size, err, errlen))
+        return AICAS_ERR_UNSUPPORTED;
+    } else {
+      a.src.set_division(p->page_size);
+    }
     a.scale_log2 = p->sm_scale * 1.4426950408889634f;
     e = p->dtype == AICAS_DTYPE_F16 ? dispatch_weigh<__half>(a, sms, stream) : dispatch_weigh<__nv_bfloat16>(a, sms, stream);
   }
