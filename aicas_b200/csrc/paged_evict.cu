@@ -2,12 +2,11 @@
 // last keep_last, and of those between the ones of the largest weights, moved to the front
 // in their order.
 //
-// Two launches.  paged_select_kernel finds the weight of the last slot that stays by radix
-// selection (exact: equal weights go to the lower slot), lists the kept slots in order and
-// moves their weights.  paged_move_kernel moves the rows: slot i of the cut cache was slot
-// kept[i] >= i, so a CTA that reads a run of rows before it writes them, run after run,
-// never reads what it has overwritten; the columns of a row are independent, so they are
-// given to CTAs of their own.
+// Two launches.  The select kernel finds the weight of the last slot that stays (exact: equal
+// weights go to the lower slot), lists the kept slots in order and moves their weights.  The
+// move kernel moves the rows: slot i of the cut cache was slot kept[i] >= i, so a CTA that
+// reads a run of rows before it writes them, run after run, never reads what it has
+// overwritten; the columns of a row are independent, so each 32 bytes of them are a CTA's.
 #include <cstdio>
 
 #include "common.cuh"
@@ -16,19 +15,206 @@
 namespace aicas {
 namespace {
 
-constexpr int kSelectThreads = 512, kSelectWarps = kSelectThreads / 32;
-
-// A weight as a whole number of the same order; NaN below all numbers, -0 as 0.
+// A weight as a whole number of the same order; NaN below all numbers, -0 as 0.  Never 0.
 __device__ __forceinline__ uint32_t order_of(float w) {
-  if (w != w) return 0u;
+  if (w != w) return 1u;
   const uint32_t u = __float_as_uint(w + 0.f);
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float weight_of(uint32_t key) {
+  return key == 1u ? __int_as_float(0x7fc00000) : __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
+}
 
-__global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const __grid_constant__ aicas_paged_evict_params a) {
+// A cache that is not cut: its slots, and its weights where they are wanted elsewhere.
+__device__ __forceinline__ void keep_all(const aicas_paged_evict_params& a, int n, const float* w, float* wo, int32_t* kept, int from,
+                                         int step) {
+  for (int i = from; i < a.keep; i += step) kept[i] = i < n ? i : -1;
+  if (wo != w)
+    for (int i = from; i < n; i += step) wo[i] = w[i];
+}
+
+// ------------------------------------------------------------------ caches whose weights fit the registers of a cluster
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Writes to the word at this CTA's shared-memory address `at`, of CTA `rank` of the cluster.
+__device__ __forceinline__ void store_peer(uint32_t at, uint32_t rank, uint4 v) {
+  uint32_t there;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
+  asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(there), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// One cluster of CTAS CTAs a (request, KV head); each has a run of slots, KEYS a thread in
+// registers.  The key of the last slot that stays is found two bits at a time: how many keys
+// are not below each of three candidates, counted in registers, over a warp, through shared
+// memory and, between the CTAs, distributed shared memory: 16 short rounds, whatever the
+// weights are (counting them by their bytes meets the same few counters again and again).
+template <int THREADS, int KEYS>
+struct Select {
+  static constexpr int kWarps = THREADS / 32, kCells = KEYS * kWarps;
+  static_assert(KEYS <= 16 && kCells % 32 == 0, "a warp's count has 10 bits");
+  uint32_t cells[kCells];    // per (key of a thread, warp): flags counted, then those before
+  uint32_t packed[2][kWarps];
+  uint4 peers[2][8];         // counts of the cluster's CTAs
+  uint32_t total;
+};
+
+template <int THREADS, int KEYS>
+__global__ void __launch_bounds__(THREADS) paged_select_kernel(const __grid_constant__ aicas_paged_evict_params a, int ctas) {
+  using S = Select<THREADS, KEYS>;
+  __shared__ S sm;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, rank = ctas > 1 ? (int)cluster_rank() : 0;
+  const int pair = blockIdx.x / ctas, b = pair / a.num_kv_heads, h = pair - b * a.num_kv_heads;
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int n = min(max(a.kv_lens[b], 0), a.max_pages * a.page_size);
+  const float* w = a.weights + b * a.w_stride_b + h * a.w_stride_h;
+  float* wo = a.weights_out + b * a.wo_stride_b + h * a.wo_stride_h;
+  int32_t* kept = a.kept + (int64_t)pair * a.keep;
+  if (n <= a.longer_than) return keep_all(a, n, w, wo, kept, rank * THREADS + tid, ctas * THREADS);
+
+  if (ctas > 1) cluster_sync();  // every CTA runs before another writes to its shared memory
+  const int run = (n + ctas - 1) / ctas, t0 = rank * run, t1 = min(n, t0 + run);  // this CTA's slots
+  const int lo = a.keep_first, hi = n - a.keep_last;
+  uint32_t key[KEYS];  // 0 past the run's end
+#pragma unroll
+  for (int j = 0; j < KEYS; ++j) {
+    const int t = t0 + j * THREADS + tid;
+    key[j] = t < t1 ? order_of(w[t]) : 0u;
+  }
+  uint32_t candidate = 0u;  // bit j: key j is of a slot that stays or goes by its weight
+#pragma unroll
+  for (int j = 0; j < KEYS; ++j) {
+    const int t = t0 + j * THREADS + tid;
+    candidate |= (uint32_t)(t >= lo && t < hi && t < t1) << j;
+  }
+
+  int round = 0;
+  // Sums of three numbers over the cluster; a thread's at most KEYS each.  before: over the CTAs of lower rank.
+  const auto sums = [&](uint32_t x, uint32_t y, uint32_t z, uint3* before) {
+    const int buf = round++ & 1;
+    const uint32_t packed = __reduce_add_sync(0xffffffffu, x | y << 10 | z << 20);
+    if (lane == 0) sm.packed[buf][warp] = packed;
+    __syncthreads();
+    const uint32_t p = lane < S::kWarps ? sm.packed[buf][lane] : 0u;
+    uint3 s = make_uint3(__reduce_add_sync(0xffffffffu, p & 1023u), __reduce_add_sync(0xffffffffu, p >> 10 & 1023u),
+                         __reduce_add_sync(0xffffffffu, p >> 20));
+    if (before != nullptr) *before = make_uint3(0u, 0u, 0u);
+    if (ctas > 1) {
+      if (warp == 0 && lane < ctas) store_peer(smem_u32(&sm.peers[buf][rank]), lane, make_uint4(s.x, s.y, s.z, 0u));
+      __syncwarp();
+      cluster_sync();
+      s = make_uint3(0u, 0u, 0u);
+      for (int r = 0; r < ctas; ++r) {
+        const uint4 v = sm.peers[buf][r];
+        if (before != nullptr && r == rank) *before = s;
+        s.x += v.x, s.y += v.y, s.z += v.z;
+      }
+    }
+    return s;
+  };
+  const auto at_least = [&](uint32_t than) {
+    uint32_t c = 0u;
+#pragma unroll
+    for (int j = 0; j < KEYS; ++j) c += (candidate >> j & 1u) && key[j] >= than;
+    return c;
+  };
+  // The places of the flagged keys in the order of slots, from `base` on.
+  uint32_t place[KEYS];
+  const auto places = [&](uint32_t flags, uint32_t base) {
+    __syncthreads();  // the last ones are read
+#pragma unroll
+    for (int j = 0; j < KEYS; ++j) {
+      const uint32_t bits = __ballot_sync(0xffffffffu, flags >> j & 1u);
+      place[j] = __popc(bits & ((1u << lane) - 1u));
+      if (lane == 0) sm.cells[j * S::kWarps + warp] = __popc(bits);
+    }
+    __syncthreads();
+    if (warp == 0) {
+      constexpr int kEach = S::kCells / 32;
+      uint32_t c[kEach], sum = 0u;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) sum += c[e] = sm.cells[lane * kEach + e];
+      uint32_t before = sum;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, before, off);
+        if (lane >= off) before += v;
+      }
+      before -= sum;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        sm.cells[lane * kEach + e] = before;
+        before += c[e];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < KEYS; ++j) place[j] += base + sm.cells[j * S::kWarps + warp];
+  };
+
+  const uint32_t need = (uint32_t)(a.keep - a.keep_first - a.keep_last);
+  uint32_t least = 0u;  // the largest key that `need` candidates are not below
+  uint32_t stays = 0u;  // bit j: key j's slot stays
+#pragma unroll
+  for (int j = 0; j < KEYS; ++j) {
+    const int t = t0 + j * THREADS + tid;
+    stays |= (uint32_t)(t < t1 && (t < lo || t >= hi)) << j;
+  }
+  if (need > 0) {
+    uint32_t enough = 0u;  // how many are not below it
+    for (int shift = 30; shift >= 0; shift -= 2) {
+      const uint3 c = sums(at_least(least | 1u << shift), at_least(least | 2u << shift), at_least(least | 3u << shift), nullptr);
+      const uint32_t digit = c.z >= need ? 3u : c.y >= need ? 2u : c.x >= need ? 1u : 0u;
+      if (digit != 0u) enough = digit == 3u ? c.z : digit == 2u ? c.y : c.x;
+      least |= digit << shift;
+    }
+    uint32_t equal = 0u, above = 0u;
+#pragma unroll
+    for (int j = 0; j < KEYS; ++j) {
+      equal |= (candidate >> j & 1u && key[j] == least) << j;
+      above |= (candidate >> j & 1u && key[j] > least) << j;
+    }
+    if (enough > need) {  // of the equal ones the lower slots
+      uint3 before;
+      const uint3 c = sums(__popc(equal), __popc(above), 0u, &before);
+      places(equal, before.x);
+#pragma unroll
+      for (int j = 0; j < KEYS; ++j)
+        if (place[j] >= need - c.y) equal &= ~(1u << j);
+    }
+    stays |= equal | above;
+  }
+  uint3 before;
+  sums(__popc(stays), 0u, 0u, &before);
+  places(stays, before.x);
+#pragma unroll
+  for (int j = 0; j < KEYS; ++j) {
+    const int t = t0 + j * THREADS + tid;
+    if (stays >> j & 1u) {
+      kept[place[j]] = t;
+      wo[place[j]] = weight_of(key[j]);  // below keep; every CTA's weights are read
+    }
+    if (t >= a.keep && t < t1) wo[t] = 0.f;
+  }
+}
+
+// ------------------------------------------------------------------ longer caches
+
+// One CTA a (request, KV head); the key of the last slot that stays by its bytes, from
+// counts of all weights' bytes, read anew for each.
+constexpr int kLongThreads = 1024, kLongWarps = kLongThreads / 32;
+
+__global__ void __launch_bounds__(kLongThreads) paged_select_long_kernel(const __grid_constant__ aicas_paged_evict_params a) {
   __shared__ int hist[256];
   __shared__ uint32_t s_key;
-  __shared__ int s_need, s_eq[kSelectWarps], s_kept[kSelectWarps];
+  __shared__ int s_need, s_eq[kLongWarps], s_kept[kLongWarps];
   const int b = blockIdx.x / a.num_kv_heads, h = blockIdx.x - b * a.num_kv_heads;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   grid_launch_dependents();
@@ -37,13 +223,7 @@ __global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const __gr
   const float* w = a.weights + b * a.w_stride_b + h * a.w_stride_h;
   float* wo = a.weights_out + b * a.wo_stride_b + h * a.wo_stride_h;
   int32_t* kept = a.kept + (int64_t)blockIdx.x * a.keep;
-  if (n <= a.longer_than) {
-    for (int i = tid; i < a.keep; i += kSelectThreads) kept[i] = i < n ? i : -1;
-    if (wo != w)
-      for (int i = tid; i < n; i += kSelectThreads) wo[i] = w[i];
-    return;
-  }
-  // the key of the last slot that stays for its weight, a byte at a time
+  if (n <= a.longer_than) return keep_all(a, n, w, wo, kept, tid, kLongThreads);
   const int lo = a.keep_first, hi = n - a.keep_last;
   int need = a.keep - a.keep_first - a.keep_last;
   uint32_t key = 0;
@@ -51,7 +231,7 @@ __global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const __gr
     for (int shift = 24; shift >= 0; shift -= 8) {
       if (tid < 256) hist[tid] = 0;
       __syncthreads();
-      for (int t = lo + tid; t < hi; t += kSelectThreads) {
+      for (int t = lo + tid; t < hi; t += kLongThreads) {
         const uint32_t u = order_of(w[t]);
         if (shift == 24 || u >> (shift + 8) == key >> (shift + 8)) atomicAdd(&hist[u >> shift & 255u], 1);
       }
@@ -83,7 +263,7 @@ __global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const __gr
     }
   // need: how many of the slots with that key stay, the lower ones first
   int eq_base = 0, kept_base = 0;
-  for (int t0 = 0; t0 < n; t0 += kSelectThreads) {
+  for (int t0 = 0; t0 < n; t0 += kLongThreads) {
     const int t = t0 + tid;
     const float x = t < n ? w[t] : 0.f;
     const bool forced = t < lo || t >= hi, in = t < n;
@@ -92,69 +272,84 @@ __global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const __gr
     const uint32_t eq = __ballot_sync(0xffffffffu, equal), below = (1u << lane) - 1u;
     if (lane == 0) s_eq[warp] = __popc(eq);
     __syncthreads();
-    int eq_before = eq_base + __popc(eq & below);
-    for (int i = 0; i < kSelectWarps; ++i) {
-      if (i < warp) eq_before += s_eq[i];
-      eq_base += s_eq[i];
-    }
+    const int e = s_eq[lane];  // as many warps as lanes
+    const int eq_before = eq_base + __reduce_add_sync(0xffffffffu, lane < warp ? e : 0) + __popc(eq & below);
+    eq_base += __reduce_add_sync(0xffffffffu, e);
     const bool stays = in && (forced || (need > 0 && (u > key || (equal && eq_before < need))));
     const uint32_t st = __ballot_sync(0xffffffffu, stays);
     if (lane == 0) s_kept[warp] = __popc(st);
     __syncthreads();
-    int at = kept_base + __popc(st & below);
-    for (int i = 0; i < kSelectWarps; ++i) {
-      if (i < warp) at += s_kept[i];
-      kept_base += s_kept[i];
-    }
+    const int k = s_kept[lane];
+    const int at = kept_base + __reduce_add_sync(0xffffffffu, lane < warp ? k : 0) + __popc(st & below);
+    kept_base += __reduce_add_sync(0xffffffffu, k);
     if (stays) {  // at <= t, and this run's weights are read
       kept[at] = t;
       wo[at] = x;
     }
   }
   __syncthreads();
-  for (int t = a.keep + tid; t < n; t += kSelectThreads) wo[t] = 0.f;
+  for (int t = a.keep + tid; t < n; t += kLongThreads) wo[t] = 0.f;
 }
 
-constexpr int kMoveThreads = 256, kMoveRows = 4;
+// ------------------------------------------------------------------ rows
+
+constexpr int kMoveThreads = 256;
+constexpr int kPart = 32;  // bytes of a row that a CTA moves; rows of 4, 8 and 16 bytes are one part
 
 struct MoveArgs {
   aicas_paged_evict_params p;
   int parts[AICAS_EVICT_MAX_PLANES + 1];  // the planes' first column parts
-  int part_bytes[AICAS_EVICT_MAX_PLANES];
+  uint32_t octets_mul;                    // n / octets of a page = (umulhi(n, octets_mul) + n) >> octets_shift
+  int octets_shift;
 };
 
-template <typename V>
-__device__ void move_rows(const aicas_paged_evict_params& a, const aicas_evict_plane& pl, const int32_t* kept, int b, int h,
-                          int part_bytes, int part) {
-  const int tpr = part_bytes / (int)sizeof(V), rows = kMoveThreads / tpr;
-  const int r = threadIdx.x / tpr;
-  const int64_t col = (int64_t)part * part_bytes + (threadIdx.x - r * tpr) * (int)sizeof(V);
-  char* data = static_cast<char*>(pl.data) + h * pl.stride_h + col;
+// N vectors a row: one row a thread, ROWS at a time; the rows of the next run are looked up meanwhile.
+template <typename V, int N, int ROWS>
+__device__ __forceinline__ void move_rows(const MoveArgs& m, const aicas_evict_plane& pl, const int32_t* kept, int b, int h, int part) {
+  const aicas_paged_evict_params& a = m.p;
+  char* data = static_cast<char*>(pl.data) + h * pl.stride_h + (int64_t)part * kPart;
   const int32_t* table = a.page_table + b * a.table_stride;
-  const auto at = [&](int slot) -> char* {
-    const int i = slot / a.page_size, page = table[i];
-    return page >= 0 && page < a.num_pages ? data + page * pl.stride_p + (slot - i * a.page_size) * pl.stride_t : nullptr;
+  const auto at = [&](int slot, int& page) -> int64_t {  // page and place in it
+    const uint32_t n = (uint32_t)slot >> 3, i = (__umulhi(n, m.octets_mul) + n) >> m.octets_shift;
+    page = table[i];
+    return (int64_t)(slot - (int)i * a.page_size) * pl.stride_t;
   };
-  for (int i0 = 0; i0 < a.keep; i0 += rows * kMoveRows) {
-    V v[kMoveRows] = {};
-    char* to[kMoveRows];
+  constexpr int kRun = kMoveThreads * ROWS;
+  for (int i0 = 0; i0 < a.keep; i0 += kRun) {
+    const int last = min(a.keep, i0 + kRun) - 1;
+    if (kept[last] == last) continue;  // nothing of the run moves, nor of what is before it
+    V v[ROWS][N] = {};
+    char* to[ROWS];
+    int from[ROWS];
 #pragma unroll
-    for (int k = 0; k < kMoveRows; ++k) {
-      const int i = i0 + k * rows + r;
-      to[k] = nullptr;
-      if (r < rows && i < a.keep) {
-        const int from = kept[i];
-        if (from > i) {
-          const char* src = at(from);
-          to[k] = at(i);
-          if (src != nullptr) v[k] = *reinterpret_cast<const V*>(src);
-        }
+    for (int k = 0; k < ROWS; ++k) {
+      const int i = i0 + k * kMoveThreads + threadIdx.x;
+      from[k] = i <= last ? kept[i] : -1;
+    }
+    int src_page[ROWS], dst_page[ROWS];
+    int64_t src[ROWS], dst[ROWS];
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      const int i = i0 + k * kMoveThreads + threadIdx.x;
+      src_page[k] = dst_page[k] = -1, src[k] = dst[k] = 0;
+      if (from[k] > i) src[k] = at(from[k], src_page[k]), dst[k] = at(i, dst_page[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      to[k] = dst_page[k] >= 0 && dst_page[k] < a.num_pages ? data + dst_page[k] * pl.stride_p + dst[k] : nullptr;
+      if (src_page[k] >= 0 && src_page[k] < a.num_pages) {
+        const V* p = reinterpret_cast<const V*>(data + src_page[k] * pl.stride_p + src[k]);
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[k][e] = p[e];
       }
     }
     __syncthreads();  // the run is read
 #pragma unroll
-    for (int k = 0; k < kMoveRows; ++k)
-      if (to[k] != nullptr) *reinterpret_cast<V*>(to[k]) = v[k];
+    for (int k = 0; k < ROWS; ++k)
+      if (to[k] != nullptr) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) reinterpret_cast<V*>(to[k])[e] = v[k][e];
+      }
   }
 }
 
@@ -169,29 +364,58 @@ __global__ void __launch_bounds__(kMoveThreads) paged_move_kernel(const __grid_c
     const int n = min(max(a.kv_lens[b], 0), a.max_pages * a.page_size);
     a.kv_lens_out[b] = n > a.longer_than ? a.keep : n;
   }
+  // kv_lens_out may be kv_lens: the others go by the list of slots alone
+  const int32_t* kept = a.kept + (int64_t)pair * a.keep;
   int i = 0;
   while (at >= m.parts[i + 1]) ++i;
   const aicas_evict_plane& pl = a.plane[i];
-  const int32_t* kept = a.kept + (int64_t)pair * a.keep;
-  const int bytes = m.part_bytes[i], part = at - m.parts[i];
-  if (bytes % 16 == 0) move_rows<uint4>(a, pl, kept, b, h, bytes, part);
-  else if (bytes == 8) move_rows<uint2>(a, pl, kept, b, h, bytes, part);
-  else move_rows<uint32_t>(a, pl, kept, b, h, bytes, part);
+  const int part = at - m.parts[i];
+  const int bytes = min((int)pl.row_bytes - part * kPart, kPart);
+  if (bytes == 32) move_rows<uint4, 2, 2>(m, pl, kept, b, h, part);
+  else if (bytes == 16) move_rows<uint4, 1, 2>(m, pl, kept, b, h, part);
+  else if (bytes == 8) move_rows<uint2, 1, 2>(m, pl, kept, b, h, part);
+  else move_rows<uint32_t, 1, 2>(m, pl, kept, b, h, part);
+}
+
+template <int THREADS, int KEYS>
+cudaError_t launch_select(const aicas_paged_evict_params& p, int ctas, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.batch * p.num_kv_heads * ctas));
+  cfg.blockDim = dim3(THREADS);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)ctas, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = ctas > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, paged_select_kernel<THREADS, KEYS>, p, ctas);
+}
+
+cudaError_t launch_select_for(const aicas_paged_evict_params& p, cudaStream_t st) {
+  const int64_t slots = (int64_t)p.max_pages * p.page_size;
+  if (slots <= 512 * 4) return launch_select<512, 4>(p, 1, st);
+  if (slots <= 512 * 8) return launch_select<512, 8>(p, 1, st);
+  for (int ctas = 1; ctas <= 8; ctas *= 2)
+    if (slots <= (int64_t)1024 * 16 * ctas) return launch_select<1024, 16>(p, ctas, st);
+  return launch_pdl(paged_select_long_kernel, dim3((unsigned)(p.batch * p.num_kv_heads)), dim3(kLongThreads), 0, st, p);
 }
 
 }  // namespace
 
 int run_paged_evict(const aicas_paged_evict_params* p, cudaStream_t stream, char* err, size_t errlen) {
   const unsigned pairs = (unsigned)(p->batch * p->num_kv_heads);
-  cudaError_t e = launch_pdl(paged_select_kernel, dim3(pairs), dim3(kSelectThreads), 0, stream, *p);
+  cudaError_t e = launch_select_for(*p, stream);
   MoveArgs m;
   m.p = *p;
   m.parts[0] = 0;
-  for (int i = 0; i < p->num_planes; ++i) {
-    const int bytes = (int)p->plane[i].row_bytes;
-    m.part_bytes[i] = bytes > 128 ? 128 : bytes;
-    m.parts[i + 1] = m.parts[i] + (bytes + m.part_bytes[i] - 1) / m.part_bytes[i];
-  }
+  for (int i = 0; i < p->num_planes; ++i) m.parts[i + 1] = m.parts[i] + ((int)p->plane[i].row_bytes + kPart - 1) / kPart;
+  // n / d for n < 2^28, as in paged_int4_tiles.cuh
+  const int octets = p->page_size / 8;
+  m.octets_shift = 0;
+  while ((1ll << m.octets_shift) < octets) ++m.octets_shift;
+  m.octets_mul = (uint32_t)((((1ull << m.octets_shift) - octets) << 32) / octets + 1);
   if (e == cudaSuccess)
     e = launch_pdl(paged_move_kernel, dim3(pairs * m.parts[p->num_planes]), dim3(kMoveThreads), 0, stream, m);
   if (e == cudaSuccess) return AICAS_OK;

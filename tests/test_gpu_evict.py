@@ -269,6 +269,17 @@ def test_evict_long_caches(cuda_device):
     _evict_case(cuda_device, "fp16", 64, 64, 2, [40001], 64, 1500, 4, 500, seed=2)
 
 
+@pytest.mark.parametrize("n,keep", [(4097, 4000), (16384, 9000), (16400, 3), (33000, 32999), (70000, 35000), (131073, 70000)])
+def test_evict_caches_of_many_slots(cuda_device, n, keep):
+    """A thread's slots, clusters of CTAs and the way for still longer caches; many equal weights."""
+
+    def coarse(w):
+        w[:] = (w * 16).floor() / 16
+
+    _evict_case(cuda_device, "bf16", 16, 0, 1, [n, n - 1, 5], 64, keep, 1, 2, edit=coarse, seed=n)
+    _evict_case(cuda_device, "bf16", 16, 0, 1, [n], 64, keep, 0, 0, seed=n, out=True)
+
+
 def test_evict_refusals(cuda_device):
     kp = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16, device=cuda_device)
     pool = ab.int4_pages(4, 2, 16, 64, dtype=torch.float16, device=cuda_device)
