@@ -1169,7 +1169,7 @@ int aicas_paged_weights(const aicas_paged_weights_params* p, void* stream) {
 int aicas_paged_evict(const aicas_paged_evict_params* p, void* stream) {
   const int rc = check_paged_evict(p);
   if (rc != AICAS_OK) return rc;
-  return aicas::run_paged_evict(p, static_cast<cudaStream_t>(stream), g_err, sizeof(g_err));
+  return aicas::run_paged_evict(p, sm_count(), static_cast<cudaStream_t>(stream), g_err, sizeof(g_err));
 }
 
 int aicas_linear_int4(const aicas_linear_int4_params* p, void* stream) {

@@ -6,7 +6,8 @@
 // weights go to the lower slot), lists the kept slots in order and moves their weights.  The
 // move kernel moves the rows: slot i of the cut cache was slot kept[i] >= i, so a CTA that
 // reads a run of rows before it writes them, run after run, never reads what it has
-// overwritten; the columns of a row are independent, so each 32 bytes of them are a CTA's.
+// overwritten; the columns of a row are independent, so where there are few pairs, CTAs share
+// a row by its columns.
 #include <cstdio>
 
 #include "common.cuh"
@@ -20,9 +21,6 @@ __device__ __forceinline__ uint32_t order_of(float w) {
   if (w != w) return 1u;
   const uint32_t u = __float_as_uint(w + 0.f);
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
-}
-__device__ __forceinline__ float weight_of(uint32_t key) {
-  return key == 1u ? __int_as_float(0x7fc00000) : __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
 }
 
 // A cache that is not cut: its slots, and its weights where they are wanted elsewhere.
@@ -82,17 +80,11 @@ __global__ void __launch_bounds__(THREADS) paged_select_kernel(const __grid_cons
   if (ctas > 1) cluster_sync();  // every CTA runs before another writes to its shared memory
   const int run = (n + ctas - 1) / ctas, t0 = rank * run, t1 = min(n, t0 + run);  // this CTA's slots
   const int lo = a.keep_first, hi = n - a.keep_last;
-  uint32_t key[KEYS];  // 0 past the run's end
+  uint32_t key[KEYS];  // above all weights' for the slots that stay whatever theirs is, 0 past the run's end
 #pragma unroll
   for (int j = 0; j < KEYS; ++j) {
     const int t = t0 + j * THREADS + tid;
-    key[j] = t < t1 ? order_of(w[t]) : 0u;
-  }
-  uint32_t candidate = 0u;  // bit j: key j is of a slot that stays or goes by its weight
-#pragma unroll
-  for (int j = 0; j < KEYS; ++j) {
-    const int t = t0 + j * THREADS + tid;
-    candidate |= (uint32_t)(t >= lo && t < hi && t < t1) << j;
+    key[j] = t >= t1 ? 0u : t < lo || t >= hi ? 0xffffffffu : order_of(w[t]);
   }
 
   int round = 0;
@@ -122,7 +114,7 @@ __global__ void __launch_bounds__(THREADS) paged_select_kernel(const __grid_cons
   const auto at_least = [&](uint32_t than) {
     uint32_t c = 0u;
 #pragma unroll
-    for (int j = 0; j < KEYS; ++j) c += (candidate >> j & 1u) && key[j] >= than;
+    for (int j = 0; j < KEYS; ++j) c += key[j] >= than;
     return c;
   };
   // The places of the flagged keys in the order of slots, from `base` on.
@@ -159,38 +151,32 @@ __global__ void __launch_bounds__(THREADS) paged_select_kernel(const __grid_cons
     for (int j = 0; j < KEYS; ++j) place[j] += base + sm.cells[j * S::kWarps + warp];
   };
 
-  const uint32_t need = (uint32_t)(a.keep - a.keep_first - a.keep_last);
-  uint32_t least = 0u;  // the largest key that `need` candidates are not below
+  const uint32_t need = (uint32_t)a.keep;
+  uint32_t least = 0u;   // the largest key that `need` keys are not below
+  uint32_t enough = 0u;  // how many are not below it
+  for (int shift = 30; shift >= 0 && enough != need; shift -= 2) {
+    const uint3 c = sums(at_least(least | 1u << shift), at_least(least | 2u << shift), at_least(least | 3u << shift), nullptr);
+    const uint32_t digit = c.z >= need ? 3u : c.y >= need ? 2u : c.x >= need ? 1u : 0u;
+    if (digit != 0u) enough = digit == 3u ? c.z : digit == 2u ? c.y : c.x;
+    least |= digit << shift;
+  }
   uint32_t stays = 0u;  // bit j: key j's slot stays
 #pragma unroll
-  for (int j = 0; j < KEYS; ++j) {
-    const int t = t0 + j * THREADS + tid;
-    stays |= (uint32_t)(t < t1 && (t < lo || t >= hi)) << j;
-  }
-  if (need > 0) {
-    uint32_t enough = 0u;  // how many are not below it
-    for (int shift = 30; shift >= 0; shift -= 2) {
-      const uint3 c = sums(at_least(least | 1u << shift), at_least(least | 2u << shift), at_least(least | 3u << shift), nullptr);
-      const uint32_t digit = c.z >= need ? 3u : c.y >= need ? 2u : c.x >= need ? 1u : 0u;
-      if (digit != 0u) enough = digit == 3u ? c.z : digit == 2u ? c.y : c.x;
-      least |= digit << shift;
-    }
-    uint32_t equal = 0u, above = 0u;
+  for (int j = 0; j < KEYS; ++j) stays |= (uint32_t)(key[j] >= least) << j;
+  if (enough > need) {  // of those with the least key the lower slots
+    uint32_t equal = 0u;
 #pragma unroll
-    for (int j = 0; j < KEYS; ++j) {
-      equal |= (candidate >> j & 1u && key[j] == least) << j;
-      above |= (candidate >> j & 1u && key[j] > least) << j;
-    }
-    if (enough > need) {  // of the equal ones the lower slots
-      uint3 before;
-      const uint3 c = sums(__popc(equal), __popc(above), 0u, &before);
-      places(equal, before.x);
+    for (int j = 0; j < KEYS; ++j) equal |= (uint32_t)(key[j] == least) << j;
+    uint3 before;
+    const uint3 c = sums(__popc(equal), __popc(stays & ~equal), 0u, &before);
+    places(equal, before.x);
 #pragma unroll
-      for (int j = 0; j < KEYS; ++j)
-        if (place[j] >= need - c.y) equal &= ~(1u << j);
-    }
-    stays |= equal | above;
+    for (int j = 0; j < KEYS; ++j)
+      if ((equal >> j & 1u) && place[j] >= need - c.y) stays &= ~(1u << j);
   }
+  float x[KEYS];
+#pragma unroll
+  for (int j = 0; j < KEYS; ++j) x[j] = stays >> j & 1u ? w[t0 + j * THREADS + tid] : 0.f;
   uint3 before;
   sums(__popc(stays), 0u, 0u, &before);
   places(stays, before.x);
@@ -199,7 +185,7 @@ __global__ void __launch_bounds__(THREADS) paged_select_kernel(const __grid_cons
     const int t = t0 + j * THREADS + tid;
     if (stays >> j & 1u) {
       kept[place[j]] = t;
-      wo[place[j]] = weight_of(key[j]);  // below keep; every CTA's weights are read
+      wo[place[j]] = x[j];  // below keep; every CTA's weights are read
     }
     if (t >= a.keep && t < t1) wo[t] = 0.f;
   }
@@ -294,66 +280,76 @@ __global__ void __launch_bounds__(kLongThreads) paged_select_long_kernel(const _
 // ------------------------------------------------------------------ rows
 
 constexpr int kMoveThreads = 256;
-constexpr int kPart = 32;  // bytes of a row that a CTA moves; rows of 4, 8 and 16 bytes are one part
+constexpr int kMostRows = 512;  // of a run
+constexpr int kMoveCtas = 3;    // an SM, at least, as far as columns of 32 bytes go
 
 struct MoveArgs {
   aicas_paged_evict_params p;
   int parts[AICAS_EVICT_MAX_PLANES + 1];  // the planes' first column parts
+  int part_bytes[AICAS_EVICT_MAX_PLANES];
   uint32_t octets_mul;                    // n / octets of a page = (umulhi(n, octets_mul) + n) >> octets_shift
   int octets_shift;
 };
 
-// N vectors a row: one row a thread, ROWS at a time; the rows of the next run are looked up meanwhile.
-template <typename V, int N, int ROWS>
-__device__ __forceinline__ void move_rows(const MoveArgs& m, const aicas_evict_plane& pl, const int32_t* kept, int b, int h, int part) {
+struct Move {
+  int64_t src, dst;  // places in the plane, in bytes; -1: none (zeros; nothing to write)
+};
+
+// A row has LANES threads with a V each; ROWS rows a thread and run.  While a run's rows are
+// on their way, where the next one's lie is looked up, a row a thread.
+template <typename V, int LANES, int ROWS>
+__device__ __forceinline__ void move_rows(const MoveArgs& m, const aicas_evict_plane& pl, const int32_t* kept, int b, int h, int part,
+                                          Move (*where)[kMostRows]) {
   const aicas_paged_evict_params& a = m.p;
-  char* data = static_cast<char*>(pl.data) + h * pl.stride_h + (int64_t)part * kPart;
+  constexpr int kSlots = kMoveThreads / LANES, kRun = kSlots * ROWS;
+  static_assert(kRun <= kMostRows, "a run's places");
+  const int r = threadIdx.x / LANES;
+  char* data = static_cast<char*>(pl.data) + h * pl.stride_h + (int64_t)part * (LANES * sizeof(V)) + threadIdx.x % LANES * sizeof(V);
   const int32_t* table = a.page_table + b * a.table_stride;
-  const auto at = [&](int slot, int& page) -> int64_t {  // page and place in it
+  const auto at = [&](int slot) -> int64_t {
     const uint32_t n = (uint32_t)slot >> 3, i = (__umulhi(n, m.octets_mul) + n) >> m.octets_shift;
-    page = table[i];
-    return (int64_t)(slot - (int)i * a.page_size) * pl.stride_t;
+    const int page = table[i];
+    return page >= 0 && page < a.num_pages ? page * pl.stride_p + (slot - (int)i * a.page_size) * pl.stride_t : -1;
   };
-  constexpr int kRun = kMoveThreads * ROWS;
-  for (int i0 = 0; i0 < a.keep; i0 += kRun) {
-    const int last = min(a.keep, i0 + kRun) - 1;
-    if (kept[last] == last) continue;  // nothing of the run moves, nor of what is before it
-    V v[ROWS][N] = {};
-    char* to[ROWS];
-    int from[ROWS];
+  const auto look = [&](int run) {
+    for (int x = threadIdx.x; x < kRun; x += kMoveThreads) {
+      const int i = run * kRun + x, from = i < a.keep ? kept[i] : -1;
+      Move w = {-1, -1};
+      if (from > i) w.src = at(from), w.dst = at(i);
+      where[run % 3][x] = w;
+    }
+  };
+  const int runs = (a.keep + kRun - 1) / kRun;
+  int run = 0;
+  while (run < runs && kept[min(a.keep, (run + 1) * kRun) - 1] <= min(a.keep, (run + 1) * kRun) - 1) ++run;  // what stays in place
+  if (run == runs) return;
+  V v[ROWS], next[ROWS];
+  const auto load = [&](int run, V (&x)[ROWS]) {
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
-      const int i = i0 + k * kMoveThreads + threadIdx.x;
-      from[k] = i <= last ? kept[i] : -1;
+      const int64_t src = where[run % 3][k * kSlots + r].src;
+      x[k] = V{};
+      if (src >= 0) x[k] = *reinterpret_cast<const V*>(data + src);
     }
-    int src_page[ROWS], dst_page[ROWS];
-    int64_t src[ROWS], dst[ROWS];
+  };
+  look(run);
+  __syncthreads();
+  load(run, v);
+  for (; run < runs; ++run) {
+    if (run + 1 < runs) look(run + 1);
+    __syncthreads();  // this run is read; the next one's rows are not among those written now
+    if (run + 1 < runs) load(run + 1, next);
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
-      const int i = i0 + k * kMoveThreads + threadIdx.x;
-      src_page[k] = dst_page[k] = -1, src[k] = dst[k] = 0;
-      if (from[k] > i) src[k] = at(from[k], src_page[k]), dst[k] = at(i, dst_page[k]);
+      const int64_t dst = where[run % 3][k * kSlots + r].dst;
+      if (dst >= 0) *reinterpret_cast<V*>(data + dst) = v[k];
+      v[k] = next[k];
     }
-#pragma unroll
-    for (int k = 0; k < ROWS; ++k) {
-      to[k] = dst_page[k] >= 0 && dst_page[k] < a.num_pages ? data + dst_page[k] * pl.stride_p + dst[k] : nullptr;
-      if (src_page[k] >= 0 && src_page[k] < a.num_pages) {
-        const V* p = reinterpret_cast<const V*>(data + src_page[k] * pl.stride_p + src[k]);
-#pragma unroll
-        for (int e = 0; e < N; ++e) v[k][e] = p[e];
-      }
-    }
-    __syncthreads();  // the run is read
-#pragma unroll
-    for (int k = 0; k < ROWS; ++k)
-      if (to[k] != nullptr) {
-#pragma unroll
-        for (int e = 0; e < N; ++e) reinterpret_cast<V*>(to[k])[e] = v[k][e];
-      }
   }
 }
 
 __global__ void __launch_bounds__(kMoveThreads) paged_move_kernel(const __grid_constant__ MoveArgs m) {
+  __shared__ Move where[3][kMostRows];
   const aicas_paged_evict_params& a = m.p;
   const int parts = m.parts[a.num_planes];
   const int pair = blockIdx.x / parts, at = blockIdx.x - pair * parts;
@@ -370,11 +366,15 @@ __global__ void __launch_bounds__(kMoveThreads) paged_move_kernel(const __grid_c
   while (at >= m.parts[i + 1]) ++i;
   const aicas_evict_plane& pl = a.plane[i];
   const int part = at - m.parts[i];
-  const int bytes = min((int)pl.row_bytes - part * kPart, kPart);
-  if (bytes == 32) move_rows<uint4, 2, 2>(m, pl, kept, b, h, part);
-  else if (bytes == 16) move_rows<uint4, 1, 2>(m, pl, kept, b, h, part);
-  else if (bytes == 8) move_rows<uint2, 1, 2>(m, pl, kept, b, h, part);
-  else move_rows<uint32_t, 1, 2>(m, pl, kept, b, h, part);
+  switch (m.part_bytes[i]) {
+    case 256: return move_rows<uint4, 16, 8>(m, pl, kept, b, h, part, where);
+    case 128: return move_rows<uint4, 8, 8>(m, pl, kept, b, h, part, where);
+    case 64: return move_rows<uint4, 4, 8>(m, pl, kept, b, h, part, where);
+    case 32: return move_rows<uint4, 2, 4>(m, pl, kept, b, h, part, where);
+    case 16: return move_rows<uint4, 1, 2>(m, pl, kept, b, h, part, where);
+    case 8: return move_rows<uint2, 1, 2>(m, pl, kept, b, h, part, where);
+    default: return move_rows<uint32_t, 1, 2>(m, pl, kept, b, h, part, where);
+  }
 }
 
 template <int THREADS, int KEYS>
@@ -404,13 +404,27 @@ cudaError_t launch_select_for(const aicas_paged_evict_params& p, cudaStream_t st
 
 }  // namespace
 
-int run_paged_evict(const aicas_paged_evict_params* p, cudaStream_t stream, char* err, size_t errlen) {
+int run_paged_evict(const aicas_paged_evict_params* p, int sms, cudaStream_t stream, char* err, size_t errlen) {
   const unsigned pairs = (unsigned)(p->batch * p->num_kv_heads);
   cudaError_t e = launch_select_for(*p, stream);
   MoveArgs m;
   m.p = *p;
-  m.parts[0] = 0;
-  for (int i = 0; i < p->num_planes; ++i) m.parts[i + 1] = m.parts[i] + ((int)p->plane[i].row_bytes + kPart - 1) / kPart;
+  // whole rows, or as many parts of them as give each SM a few CTAs
+  int most = 256;
+  for (;; most /= 2) {
+    m.parts[0] = 0;
+    for (int i = 0; i < p->num_planes; ++i) {
+      const int bytes = (int)p->plane[i].row_bytes;
+      int part = 16;
+      if (bytes < 16)
+        part = bytes;
+      else
+        while (part < most && bytes % (2 * part) == 0) part *= 2;
+      m.part_bytes[i] = part;
+      m.parts[i + 1] = m.parts[i] + bytes / part;
+    }
+    if (most == 32 || (int64_t)pairs * m.parts[p->num_planes] >= kMoveCtas * sms) break;
+  }
   // n / d for n < 2^28, as in paged_int4_tiles.cuh
   const int octets = p->page_size / 8;
   m.octets_shift = 0;

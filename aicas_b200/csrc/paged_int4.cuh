@@ -19,6 +19,6 @@ int run_paged_decode_int4(const aicas_paged_decode_int4_params* p, int sms, void
                           char* err, size_t errlen);
 
 int run_paged_weights(const aicas_paged_weights_params* p, int sms, cudaStream_t stream, char* err, size_t errlen);
-int run_paged_evict(const aicas_paged_evict_params* p, cudaStream_t stream, char* err, size_t errlen);
+int run_paged_evict(const aicas_paged_evict_params* p, int sms, cudaStream_t stream, char* err, size_t errlen);
 
 }  // namespace aicas
