@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(kLongThreads) paged_select_long_kernel(const _
 
 constexpr int kMoveThreads = 256;
 constexpr int kMostRows = 512;  // of a run
-constexpr int kMoveCtas = 3;    // an SM, at least, as far as columns of 32 bytes go
+constexpr int kMoveCtas = 1;    // an SM, at least, as far as columns of 32 bytes go
 
 struct MoveArgs {
   aicas_paged_evict_params p;
@@ -348,6 +348,8 @@ __device__ __forceinline__ void move_rows(const MoveArgs& m, const aicas_evict_p
   }
 }
 
+// ROWS: 8 a thread where an SM has few CTAs, 4 (and twice the CTAs) where it has many.
+template <int ROWS>
 __global__ void __launch_bounds__(kMoveThreads) paged_move_kernel(const __grid_constant__ MoveArgs m) {
   __shared__ Move where[3][kMostRows];
   const aicas_paged_evict_params& a = m.p;
@@ -367,9 +369,9 @@ __global__ void __launch_bounds__(kMoveThreads) paged_move_kernel(const __grid_c
   const aicas_evict_plane& pl = a.plane[i];
   const int part = at - m.parts[i];
   switch (m.part_bytes[i]) {
-    case 256: return move_rows<uint4, 16, 8>(m, pl, kept, b, h, part, where);
-    case 128: return move_rows<uint4, 8, 8>(m, pl, kept, b, h, part, where);
-    case 64: return move_rows<uint4, 4, 8>(m, pl, kept, b, h, part, where);
+    case 256: return move_rows<uint4, 16, ROWS>(m, pl, kept, b, h, part, where);
+    case 128: return move_rows<uint4, 8, ROWS>(m, pl, kept, b, h, part, where);
+    case 64: return move_rows<uint4, 4, ROWS>(m, pl, kept, b, h, part, where);
     case 32: return move_rows<uint4, 2, 4>(m, pl, kept, b, h, part, where);
     case 16: return move_rows<uint4, 1, 2>(m, pl, kept, b, h, part, where);
     case 8: return move_rows<uint2, 1, 2>(m, pl, kept, b, h, part, where);
@@ -396,9 +398,10 @@ cudaError_t launch_select(const aicas_paged_evict_params& p, int ctas, cudaStrea
 cudaError_t launch_select_for(const aicas_paged_evict_params& p, cudaStream_t st) {
   const int64_t slots = (int64_t)p.max_pages * p.page_size;
   if (slots <= 512 * 4) return launch_select<512, 4>(p, 1, st);
-  if (slots <= 512 * 8) return launch_select<512, 8>(p, 1, st);
   for (int ctas = 1; ctas <= 8; ctas *= 2)
-    if (slots <= (int64_t)1024 * 16 * ctas) return launch_select<1024, 16>(p, ctas, st);
+    if (slots <= (int64_t)512 * 8 * ctas) return launch_select<512, 8>(p, ctas, st);
+  if (slots <= 512 * 16 * 8) return launch_select<512, 16>(p, 8, st);
+  if (slots <= 1024 * 16 * 8) return launch_select<1024, 16>(p, 8, st);
   return launch_pdl(paged_select_long_kernel, dim3((unsigned)(p.batch * p.num_kv_heads)), dim3(kLongThreads), 0, st, p);
 }
 
@@ -431,7 +434,9 @@ int run_paged_evict(const aicas_paged_evict_params* p, int sms, cudaStream_t str
   while ((1ll << m.octets_shift) < octets) ++m.octets_shift;
   m.octets_mul = (uint32_t)((((1ull << m.octets_shift) - octets) << 32) / octets + 1);
   if (e == cudaSuccess)
-    e = launch_pdl(paged_move_kernel, dim3(pairs * m.parts[p->num_planes]), dim3(kMoveThreads), 0, stream, m);
+    // 32 caches cut to 1024 slots (512 CTAs) 65.2 us with 8, 62.6 with 4; 4 caches cut to 8192 (256 CTAs) 97, 133
+    e = launch_pdl(pairs * m.parts[p->num_planes] <= 2u * sms ? paged_move_kernel<8> : paged_move_kernel<4>,
+                   dim3(pairs * m.parts[p->num_planes]), dim3(kMoveThreads), 0, stream, m);
   if (e == cudaSuccess) return AICAS_OK;
   snprintf(err, errlen, "paged evict launch: %s (%s)", cudaGetErrorString(e), cudaGetErrorName(e));
   return AICAS_ERR_CUDA;
