@@ -56,9 +56,7 @@ struct Levels {
   __device__ __forceinline__ void set(float lo, float hi) {
     const T l = Elem<T>::from_float(lo);
     least = Elem<T>::to_float(l);
-    constexpr float kFifteenth = 1.f / 15.f;
-    const float range = hi - least, near = range * kFifteenth;
-    const T s = Elem<T>::from_float(fmaf(fmaf(-15.f, near, range), kFifteenth, near));  // range / 15, rounded once
+    const T s = Elem<T>::from_float((hi - least) * (1.f / 15.f));
     scale = Elem<T>::to_float(s);
     if (!(fabsf(scale) < INFINITY)) scale = least = __int_as_float(0x7fc00000);  // an infinity or NaN among the elements
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
@@ -71,10 +69,9 @@ struct Levels {
     pair = r.u;
   }
 
-  // The codes of 8 elements, 4 bits each.  EXACT: elements that are 16-bit values often lie
-  // on the border between two codes, where the quotient by the reciprocal may fall on
-  // either side; what a nearby code leaves, which fma gives exactly, corrects it.
-  template <bool EXACT>
+  // The codes of 8 elements, 4 bits each.  The quotient by the reciprocal may fall on the
+  // other side of a border between two codes, on which 16-bit values often lie: what a
+  // nearby code leaves, which fma gives exactly, corrects it.
   __device__ __forceinline__ uint32_t codes(const float* x) const {
     if (inv == 0.f) return 0u;  // one value, or NaN
     // 1.5 x 2^23: a sum with it has the number, rounded to a whole one, in its low bits
@@ -83,12 +80,8 @@ struct Levels {
     int q[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float d = x[i] - least;
-      float w = d * inv;
-      if constexpr (EXACT) {
-        const float near = fmaf(x[i], inv, at) - kWhole;
-        w = fmaf(fmaf(-near, scale, d), inv, near);
-      }
+      const float near = fmaf(x[i], inv, at) - kWhole;
+      const float w = fmaf(fmaf(-near, scale, x[i] - least), inv, near);
       q[i] = __float_as_int(w * 0x1p-149f);  // as so many of the smallest steps: the number, rounded to a whole one
     }
     uint32_t u = 0;
@@ -98,6 +91,37 @@ struct Levels {
     return u;
   }
 };
+
+// The sum of a row's squares, added in the order of torch's sums of 64 and 128 contiguous
+// numbers on the GPU: x1, x2 are 8 elements each of the row's halves.
+template <int D>
+__device__ __forceinline__ float torch_sum(uint32_t lanes, const float* x1, const float* x2) {
+  if constexpr (D == 128) {  // fours one after the other; then the halves of the 32 sums, of those, and so on
+    float a[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float s[2];
+#pragma unroll
+      for (int side = 0; side < 2; ++side) {
+        const float* x = (side == 0 ? x1 : x2) + 4 * h;
+        s[side] = __fadd_rn(__fadd_rn(__fadd_rn(__fmul_rn(x[0], x[0]), __fmul_rn(x[1], x[1])), __fmul_rn(x[2], x[2])), __fmul_rn(x[3], x[3]));
+      }
+      a[h] = s[0] + s[1];
+#pragma unroll
+      for (int off = 4; off >= 1; off >>= 1) a[h] += __shfl_xor_sync(lanes, a[h], off);
+    }
+    return a[0] + a[1];
+  } else {  // the halves of the 64 squares, of their sums, and so on
+    float a[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      a[i] = __fadd_rn(__fmul_rn(x1[i], x1[i]), __fmul_rn(x2[i], x2[i]));
+#pragma unroll
+      for (int off = 2; off >= 1; off >>= 1) a[i] += __shfl_xor_sync(lanes, a[i], off);
+    }
+    return ((a[0] + a[4]) + (a[2] + a[6])) + ((a[1] + a[5]) + (a[3] + a[7]));
+  }
+}
 
 // The lane's part of one token: c is its place in a row's halves, lanes those of its row.
 template <typename CS, int D>
@@ -115,6 +139,9 @@ __device__ __forceinline__ void token_rows(const aicas_paged_append_int4_params&
   using K = Token<CS, D>;
   constexpr int kV = K::kV, kTpr = K::kTpr;
   constexpr bool kRoundEach = std::is_same<T, CS>::value;
+  // Keys in fp32: every operation rounded as torch's, so that they get the codes that torch's keys
+  // would get (a fused product and sum puts some on the other side of a border).
+  constexpr bool kAsTorch = KIND == 1 && !kRoundEach;
   const T* src = static_cast<const T*>(KIND == 0 ? a.q_in : KIND == 1 ? a.k_in : a.v_in) +
                  t.b * (KIND == 0 ? a.qi_stride_b : KIND == 1 ? a.k_stride_b : a.v_stride_b) +
                  t.s * (KIND == 0 ? a.qi_stride_s : KIND == 1 ? a.k_stride_s : a.v_stride_s) + t.c;
@@ -147,13 +174,35 @@ __device__ __forceinline__ void token_rows(const aicas_paged_append_int4_params&
         Elem<T>::unpack(w1, f1);
         Elem<T>::unpack(w2, f2);
         float ss = 0.f;
+        if constexpr (kAsTorch) {
+          ss = torch_sum<D>(t.lanes, x1, x2);
+        } else {
 #pragma unroll
-        for (int i = 0; i < kV; ++i) ss += x1[i] * x1[i] + x2[i] * x2[i];
+          for (int i = 0; i < kV; ++i) ss += x1[i] * x1[i] + x2[i] * x2[i];
 #pragma unroll
-        for (int off = kTpr / 2; off >= 1; off >>= 1) ss += __shfl_xor_sync(t.lanes, ss, off);
-        normed_pair<T, kRoundEach, kV>(x1, x2, f1, f2, rsqrtf(ss / (float)D + a.norm_eps));
+          for (int off = kTpr / 2; off >= 1; off >>= 1) ss += __shfl_xor_sync(t.lanes, ss, off);
+        }
+        const float inv = rsqrtf(ss / (float)D + a.norm_eps);
+        if constexpr (kAsTorch) {
+#pragma unroll
+          for (int i = 0; i < kV; ++i) {
+            x1[i] = __fmul_rn(__fmul_rn(x1[i], inv), f1[i]);
+            x2[i] = __fmul_rn(__fmul_rn(x2[i], inv), f2[i]);
+          }
+        } else {
+          normed_pair<T, kRoundEach, kV>(x1, x2, f1, f2, inv);
+        }
       }
-      rotated_pair<T, kRoundEach, kV>(x1, x2, t.c1, t.c2, t.s1, t.s2);
+      if constexpr (kAsTorch) {
+#pragma unroll
+        for (int i = 0; i < kV; ++i) {
+          const float p1 = x1[i], p2 = x2[i];
+          x1[i] = __fadd_rn(__fmul_rn(p1, t.c1[i]), __fmul_rn(-p2, t.s1[i]));
+          x2[i] = __fadd_rn(__fmul_rn(p2, t.c2[i]), __fmul_rn(p1, t.s2[i]));
+        }
+      } else {
+        rotated_pair<T, kRoundEach, kV>(x1, x2, t.c1, t.c2, t.s1, t.s2);
+      }
     }
     if constexpr (KIND == 0) {
       T* dst = static_cast<T*>(a.q_out) + t.b * a.qo_stride_b + t.s * a.qo_stride_s + head * a.qo_stride_h + t.c;
@@ -164,7 +213,6 @@ __device__ __forceinline__ void token_rows(const aicas_paged_append_int4_params&
 #pragma unroll
         for (int i = 0; i < kV; ++i) x1[i] = rounded<T>(x1[i]), x2[i] = rounded<T>(x2[i]);
       }
-      constexpr bool kExact = KIND == 2 || kRoundEach;
       const aicas_int4_pages& to = a.kv[KIND - 1];
       uint8_t* codes = static_cast<uint8_t*>(to.codes) + t.page * to.cs_p + t.row * to.cs_t + head * to.cs_h + t.c / 2;
       T* pair = static_cast<T*>(to.scales) + t.page * to.ss_p + t.row * to.ss_t + head * to.ss_h;
@@ -185,8 +233,8 @@ __device__ __forceinline__ void token_rows(const aicas_paged_append_int4_params&
         v2 = v1;
         if (t.c == 0) *reinterpret_cast<uint32_t*>(pair) = v1.pair;
       }
-      *reinterpret_cast<uint32_t*>(codes) = v1.codes<kExact>(x1);
-      *reinterpret_cast<uint32_t*>(codes + D / 4) = v2.codes<kExact>(x2);
+      *reinterpret_cast<uint32_t*>(codes) = v1.codes(x1);
+      *reinterpret_cast<uint32_t*>(codes + D / 4) = v2.codes(x2);
     }
   }
 }
