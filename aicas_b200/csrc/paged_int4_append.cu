@@ -379,16 +379,19 @@ __global__ void __launch_bounds__(256) paged_read_int4_kernel(const __grid_const
   }
 }
 
-// The few rows of a decode step: a CTA a request, all its rows at once.
+// The few rows of a decode step: all of a request's at once, in CTAs of kFewThreads.
+constexpr int kFewThreads = 32;
+
 template <typename T, int D, bool HALVES>
-__global__ void __launch_bounds__(256) paged_read_few_int4_kernel(const __grid_constant__ aicas_paged_read_int4_params a) {
-  constexpr int kTpr = D / 8, kSlots = 256 / kTpr;
+__global__ void __launch_bounds__(kFewThreads) paged_read_few_int4_kernel(const __grid_constant__ aicas_paged_read_int4_params a) {
+  constexpr int kTpr = D / 8;
   const int b = blockIdx.x, c = threadIdx.x % kTpr * 8;
   grid_launch_dependents();
   grid_dependency_wait();
   const int fresh = a.num_tokens != nullptr ? min(a.num_tokens[b], a.seq_len) : a.seq_len;
   const int pos = a.positions[b];
-  for (int r = threadIdx.x / kTpr; r < 2 * a.num_kv_heads * a.seq_len; r += kSlots) {
+  const int r = (blockIdx.y * kFewThreads + threadIdx.x) / kTpr;
+  if (r < 2 * a.num_kv_heads * a.seq_len) {
     const int head = a.seq_len == 1 ? r : r / a.seq_len, s = r - head * a.seq_len, h = head >> 1, side = head & 1;
     const aicas_int4_pages& from = a.kv[side];
     const int2 at = row_at(a, b, pos, fresh, s);
@@ -407,7 +410,9 @@ __global__ void __launch_bounds__(256) paged_read_few_int4_kernel(const __grid_c
 template <typename T, int D, bool HALVES>
 cudaError_t launch_read_sized(const aicas_paged_read_int4_params& p, cudaStream_t st) {
   if ((int64_t)p.num_kv_heads * p.seq_len * (D / 8) <= 512)
-    return launch_pdl(paged_read_few_int4_kernel<T, D, HALVES>, dim3((unsigned)p.batch), dim3(256), 0, st, p);
+    return launch_pdl(paged_read_few_int4_kernel<T, D, HALVES>,
+                      dim3((unsigned)p.batch, (2 * p.num_kv_heads * p.seq_len * (D / 8) + kFewThreads - 1) / kFewThreads), dim3(kFewThreads), 0,
+                      st, p);
   const int64_t rows = 256 / (D / 16) * 2, chunks = (p.seq_len + rows - 1) / rows;
   const dim3 grid((unsigned)(chunks * p.batch), 2u * p.num_kv_heads);
   return launch_pdl(paged_read_int4_kernel<T, D, HALVES, 2>, grid, dim3(256), 0, st, p, (int)chunks);
