@@ -624,7 +624,8 @@ int run_paged_decode_int4(const aicas_paged_decode_int4_params* p, int sms, void
   const size_t workspace_bytes = paged_decode_int4_workspace(p, sms);
   Int4Args a;
   memset(&a, 0, sizeof(a));
-  if (!a.src.set(p->kv, 2, p->page_table, p->table_stride, p->head_dim, p->group_size, p->num_pages, p->page_size, err, errlen))
+  if (!a.src.set(p->kv, 2, p->page_table, p->table_stride, p->head_dim, p->group_size, p->num_kv_heads, p->num_pages,
+                 p->page_size, err, errlen))
     return AICAS_ERR_UNSUPPORTED;
   a.q = p->q, a.out = p->out, a.lse = p->lse;
   a.lens = p->kv_lens, a.starts = p->kv_starts;

@@ -29,11 +29,13 @@ struct Int4Source {
   int octets;              // of 8 rows a page has
   uint32_t octets_mul;     // n / octets = (umulhi(n, octets_mul) + n) >> octets_shift
   int octets_shift;
-  int dense;               // rows follow one another within a page and head
+  // Rows follow one another within a page and head, both sides have the same strides, and
+  // places in them, in units of 16 bytes and of a row's pairs, fit 32 bits.
+  int dense;
 
   // Of `sides` sides; false, with a message, for strides that are too large.
   bool set(const aicas_int4_pages* pages, int sides, const int32_t* page_table, int64_t stride, int head_dim, int group_size,
-           int pages_in_pool, int page_size, char* err, size_t errlen) {
+           int heads, int pages_in_pool, int page_size, char* err, size_t errlen) {
     dense = 1;
     for (int i = 0; i < sides; ++i) {
       const aicas_int4_pages& from = pages[i];
@@ -46,7 +48,12 @@ struct Int4Source {
         }
       kv[i] = {static_cast<const uint8_t*>(from.codes), static_cast<const uint8_t*>(from.scales), (uint32_t)st[0], (uint32_t)st[1],
                (uint32_t)st[2], (uint32_t)st[3], (uint32_t)st[4], (uint32_t)st[5]};
-      dense &= kv[i].cs_t == (uint32_t)head_dim / 32 && kv[i].ss_t == 1;
+      const Side &a = kv[0], &b = kv[i];
+      dense &= b.cs_t == (uint32_t)head_dim / 32 && b.ss_t == 1 && a.cs_p == b.cs_p && a.cs_h == b.cs_h && a.ss_p == b.ss_p && a.ss_h == b.ss_h;
+      // the last row's place; products of numbers below 2^32
+      const double last = (double)pages_in_pool * b.cs_p + (double)heads * b.cs_h + (double)page_size * b.cs_t;
+      const double last_pair = (double)pages_in_pool * b.ss_p + (double)heads * b.ss_h + (double)page_size * b.ss_t;
+      dense &= last < 4e9 && last_pair < 4e9;
     }
     table = page_table, table_stride = stride, num_pages = pages_in_pool;
     set_division(page_size);
@@ -147,8 +154,11 @@ struct Cursor {
   int t;      // its next tile, in seg
   int turn;   // the warp that takes seg's first tile
   int known;  // tiles from t on whose pages are looked up; -1: no tile left
-  int page;   // of lane's octet lane % 4 of the tile lane / 4 of those 8: page number, -1: nothing to copy,
-  int row;    // and first row in the page
+  // Of the lane's octet lane % 4 of the tile lane / 4 of those 8: page number (-1: nothing to
+  // copy) and first row in the page; of dense pages the places of its codes (-1) and pairs.
+  int page, row;
+
+  __device__ __forceinline__ uint32_t head(const A& a) const { return a.row_blocks == 1 ? seg.pair : seg.pair / a.row_blocks; }
 
   __device__ __forceinline__ void look(const A& a, int team) {
     const int lane = threadIdx.x & 31;
@@ -157,7 +167,14 @@ struct Cursor {
     row = 8 * (n - i * a.src.octets);
     page = -1;
     if (8 * n < seg.len && 8 * n + 8 > seg.start) page = a.src.table[seg.b * a.src.table_stride + i];
-    if (page >= a.src.num_pages) page = -1;
+    if (page >= a.src.num_pages || page < 0) {
+      page = -1;
+    } else if (a.src.dense) {
+      const Side& p = a.src.kv[0];
+      const uint32_t at = page, h = head(a);
+      page = (int)(at * p.cs_p + h * p.cs_h + (uint32_t)row * C::kChunks);
+      row = (int)(at * p.ss_p + h * p.ss_h + (uint32_t)row);
+    }
     known = 8;
   }
 
@@ -179,28 +196,34 @@ struct Cursor {
     settle(a, rank, team);
   }
 
+  // One tile's rows: page and row of the lane's octet, as above.
   template <bool DENSE>
   __device__ __forceinline__ void rows(const A& a, uint32_t stage, int pg, int first_row) {
     const int lane = threadIdx.x & 31, o = lane >> 3, sub = lane & 7;
-    const uint32_t head = a.row_blocks == 1 ? seg.pair : seg.pair / a.row_blocks;
-    const bool there = pg >= 0;
-    const uint32_t at = there ? pg : 0;
+    const bool there = pg != -1;
     constexpr int kAtOnce = 8 / C::kChunks;  // rows of an octet in one go
     const int r = sub / C::kChunks, c = sub % C::kChunks;
+    const uint32_t h = DENSE ? 0u : head(a);
 #pragma unroll
     for (int side = 0; side < SIDES; ++side) {
       const Side& p = a.src.kv[side];
-      const uint64_t unit = (uint64_t)at * p.cs_p + (uint64_t)head * p.cs_h +
-                            (DENSE ? (uint64_t)(uint32_t)((first_row + r) * C::kChunks + c) : (uint64_t)(uint32_t)(first_row + r) * p.cs_t + c);
-      const uint8_t* codes = p.codes + 16 * unit;
-      const uint64_t step = DENSE ? kAtOnce * C::kRow : (uint64_t)p.cs_t * (16 * kAtOnce);
+      const uint8_t *codes = p.codes, *pair = p.pairs;
+      uint64_t step = kAtOnce * C::kRow;
+      if constexpr (DENSE) {
+        // this lane's 16 bytes of the octet are the sub-th, and 8 further ones each
+        codes += 16ull * (uint32_t)(there ? pg + sub : 0);
+        pair += (uint64_t)C::kPair * (uint32_t)(there ? first_row + sub : 0);
+      } else {
+        const uint32_t at = there ? pg : 0;
+        codes += 16 * ((uint64_t)at * p.cs_p + (uint64_t)h * p.cs_h + (uint64_t)(uint32_t)(first_row + r) * p.cs_t + c);
+        pair += C::kPair * ((uint64_t)at * p.ss_p + (uint64_t)h * p.ss_h + (uint64_t)(uint32_t)(first_row + sub) * p.ss_t);
+        step = (uint64_t)p.cs_t * (16 * kAtOnce);
+      }
       const uint32_t dst = stage + side * C::kOffV + (8 * o + r) * C::kRow;
 #pragma unroll
       for (int k = 0; k < C::kChunks; ++k)
         copy_async<16>(dst + kAtOnce * k * C::kRow + 16 * swizzled<D>(r + kAtOnce * k, c), codes + k * step, there);
-      const uint64_t pair = (uint64_t)at * p.ss_p + (uint64_t)head * p.ss_h +
-                            (DENSE ? (uint64_t)(uint32_t)(first_row + sub) : (uint64_t)(uint32_t)(first_row + sub) * p.ss_t);
-      copy_async<C::kPair>(stage + C::kOffPairs + (SIDES * lane + side) * C::kPair, p.pairs + C::kPair * pair, there);
+      copy_async<C::kPair>(stage + C::kOffPairs + (SIDES * lane + side) * C::kPair, pair, there);
     }
   }
 

@@ -524,7 +524,8 @@ int run_paged_weights(const aicas_paged_weights_params* p, int sms, cudaStream_t
     if (p->group_size != 0) {
       const aicas_int4_pages pages = {const_cast<void*>(p->k_pages), const_cast<void*>(p->k_scales), p->kp_stride_p, p->kp_stride_h,
                                       p->kp_stride_t, p->ks_stride_p, p->ks_stride_h, p->ks_stride_t};
-      if (!a.src.set(&pages, 1, p->page_table, p->table_stride, p->head_dim, p->group_size, p->num_pages, p->page_size, err, errlen))
+      if (!a.src.set(&pages, 1, p->page_table, p->table_stride, p->head_dim, p->group_size, p->num_kv_heads, p->num_pages,
+                     p->page_size, err, errlen))
         return AICAS_ERR_UNSUPPORTED;
     } else {
       a.src.set_division(p->page_size);
