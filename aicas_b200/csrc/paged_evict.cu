@@ -80,11 +80,15 @@ __global__ void __launch_bounds__(THREADS) paged_select_kernel(const __grid_cons
   if (ctas > 1) cluster_sync();  // every CTA runs before another writes to its shared memory
   const int run = (n + ctas - 1) / ctas, t0 = rank * run, t1 = min(n, t0 + run);  // this CTA's slots
   const int lo = a.keep_first, hi = n - a.keep_last;
+  // The weights stay in registers where these hold them beside the keys.
+  constexpr bool kHeld = KEYS <= 8;
+  float x[KEYS];
   uint32_t key[KEYS];  // above all weights' for the slots that stay whatever theirs is, 0 past the run's end
 #pragma unroll
   for (int j = 0; j < KEYS; ++j) {
     const int t = t0 + j * THREADS + tid;
-    key[j] = t >= t1 ? 0u : t < lo || t >= hi ? 0xffffffffu : order_of(w[t]);
+    x[j] = t < t1 ? w[t] : 0.f;
+    key[j] = t >= t1 ? 0u : t < lo || t >= hi ? 0xffffffffu : order_of(x[j]);
   }
 
   int round = 0;
@@ -174,9 +178,9 @@ __global__ void __launch_bounds__(THREADS) paged_select_kernel(const __grid_cons
     for (int j = 0; j < KEYS; ++j)
       if ((equal >> j & 1u) && place[j] >= need - c.y) stays &= ~(1u << j);
   }
-  float x[KEYS];
+  if constexpr (!kHeld)
 #pragma unroll
-  for (int j = 0; j < KEYS; ++j) x[j] = stays >> j & 1u ? w[t0 + j * THREADS + tid] : 0.f;
+    for (int j = 0; j < KEYS; ++j) x[j] = stays >> j & 1u ? w[t0 + j * THREADS + tid] : 0.f;
   uint3 before;
   sums(__popc(stays), 0u, 0u, &before);
   places(stays, before.x);
@@ -321,7 +325,8 @@ __device__ __forceinline__ void move_rows(const MoveArgs& m, const aicas_evict_p
   };
   const int runs = (a.keep + kRun - 1) / kRun;
   int run = 0;
-  while (run < runs && kept[min(a.keep, (run + 1) * kRun) - 1] <= min(a.keep, (run + 1) * kRun) - 1) ++run;  // what stays in place
+  // what stays in place, where it may be worth a look
+  while (run < runs && runs > 2 && kept[min(a.keep, (run + 1) * kRun) - 1] <= min(a.keep, (run + 1) * kRun) - 1) ++run;  // what stays in place
   if (run == runs) return;
   V v[ROWS], next[ROWS];
   const auto load = [&](int run, V (&x)[ROWS]) {
