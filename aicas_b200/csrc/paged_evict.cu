@@ -2,12 +2,12 @@
 // last keep_last, and of those between the ones of the largest weights, moved to the front
 // in their order.
 //
-// Two launches.  The select kernel finds the weight of the last slot that stays (exact: equal
-// weights go to the lower slot), lists the kept slots in order and moves their weights.  The
-// move kernel moves the rows: slot i of the cut cache was slot kept[i] >= i, so a CTA that
-// reads a run of rows before it writes them, run after run, never reads what it has
-// overwritten; the columns of a row are independent, so where there are few pairs, CTAs share
-// a row by its columns.
+// The selection finds the weight of the last slot that stays (exact: equal weights go to the
+// lower slot), lists the kept slots in order and moves their weights; then the rows are moved.
+// Slot i of the cut cache was slot kept[i] >= i, so a CTA that reads a run of rows before it
+// writes them, run after run, never reads what it has overwritten; the columns of a row are
+// independent, so where there are few pairs, CTAs share a row by its columns.  Short caches of
+// few pairs do both in one launch, a cluster of CTAs a pair; the others in two.
 #include <cstdio>
 
 #include "common.cuh"
@@ -31,6 +31,95 @@ __device__ __forceinline__ void keep_all(const aicas_paged_evict_params& a, int 
     for (int i = from; i < n; i += step) wo[i] = w[i];
 }
 
+// ------------------------------------------------------------------ rows
+
+constexpr int kMostRows = 512;  // of a run
+
+struct MoveArgs {
+  aicas_paged_evict_params p;
+  int parts[AICAS_EVICT_MAX_PLANES + 1];  // the planes' first column parts
+  int part_bytes[AICAS_EVICT_MAX_PLANES];
+  uint32_t octets_mul;                    // n / octets of a page = (umulhi(n, octets_mul) + n) >> octets_shift
+  int octets_shift;
+};
+
+struct Move {
+  int64_t src, dst;  // places in the plane, in bytes; -1: none (zeros; nothing to write)
+};
+
+// A row has LANES threads with a V each; ROWS rows a thread and run.  While a run's rows are
+// on their way, where the next one's lie is looked up, a row a thread.
+template <int THREADS, typename V, int LANES, int ROWS>
+__device__ __forceinline__ void move_rows(const MoveArgs& m, const aicas_evict_plane& pl, const int32_t* kept, int b, int h, int part,
+                                          Move (*where)[kMostRows]) {
+  const aicas_paged_evict_params& a = m.p;
+  constexpr int kSlots = THREADS / LANES, kRun = kSlots * ROWS;
+  static_assert(kRun <= kMostRows, "a run's places");
+  const int r = threadIdx.x / LANES;
+  char* data = static_cast<char*>(pl.data) + h * pl.stride_h + (int64_t)part * (LANES * sizeof(V)) + threadIdx.x % LANES * sizeof(V);
+  const int32_t* table = a.page_table + b * a.table_stride;
+  const auto at = [&](int slot) -> int64_t {
+    const uint32_t n = (uint32_t)slot >> 3, i = (__umulhi(n, m.octets_mul) + n) >> m.octets_shift;
+    const int page = table[i];
+    return page >= 0 && page < a.num_pages ? page * pl.stride_p + (slot - (int)i * a.page_size) * pl.stride_t : -1;
+  };
+  const auto look = [&](int run) {
+    for (int x = threadIdx.x; x < kRun; x += THREADS) {
+      const int i = run * kRun + x, from = i < a.keep ? kept[i] : -1;
+      Move w = {-1, -1};
+      if (from > i) w.src = at(from), w.dst = at(i);
+      where[run % 3][x] = w;
+    }
+  };
+  const int runs = (a.keep + kRun - 1) / kRun;
+  int run = 0;
+  // what stays in place, where it may be worth a look
+  while (run < runs && runs > 2 && kept[min(a.keep, (run + 1) * kRun) - 1] <= min(a.keep, (run + 1) * kRun) - 1) ++run;  // what stays in place
+  if (run == runs) return;
+  V v[ROWS], next[ROWS];
+  const auto load = [&](int run, V (&x)[ROWS]) {
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      const int64_t src = where[run % 3][k * kSlots + r].src;
+      x[k] = V{};
+      if (src >= 0) x[k] = *reinterpret_cast<const V*>(data + src);
+    }
+  };
+  look(run);
+  __syncthreads();
+  load(run, v);
+  for (; run < runs; ++run) {
+    if (run + 1 < runs) look(run + 1);
+    __syncthreads();  // this run is read; the next one's rows are not among those written now
+    if (run + 1 < runs) load(run + 1, next);
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      const int64_t dst = where[run % 3][k * kSlots + r].dst;
+      if (dst >= 0) *reinterpret_cast<V*>(data + dst) = v[k];
+      v[k] = next[k];
+    }
+  }
+}
+
+// Part `at` of a pair's parts.  ROWS: vectors a thread has in flight, twice.
+template <int THREADS, int ROWS>
+__device__ __forceinline__ void move_part(const MoveArgs& m, const int32_t* kept, int b, int h, int at, Move (*where)[kMostRows]) {
+  int i = 0;
+  while (at >= m.parts[i + 1]) ++i;
+  const aicas_evict_plane& pl = m.p.plane[i];
+  const int part = at - m.parts[i];
+  constexpr int kFew = kMostRows / THREADS;  // rows of a thread that a run has places for
+  switch (m.part_bytes[i]) {
+    case 256: return move_rows<THREADS, uint4, 16, ROWS>(m, pl, kept, b, h, part, where);
+    case 128: return move_rows<THREADS, uint4, 8, ROWS>(m, pl, kept, b, h, part, where);
+    case 64: return move_rows<THREADS, uint4, 4, (4 * kFew < ROWS ? 4 * kFew : ROWS)>(m, pl, kept, b, h, part, where);
+    case 32: return move_rows<THREADS, uint4, 2, (2 * kFew < ROWS ? 2 * kFew : ROWS)>(m, pl, kept, b, h, part, where);
+    case 16: return move_rows<THREADS, uint4, 1, kFew>(m, pl, kept, b, h, part, where);
+    case 8: return move_rows<THREADS, uint2, 1, kFew>(m, pl, kept, b, h, part, where);
+    default: return move_rows<THREADS, uint32_t, 1, kFew>(m, pl, kept, b, h, part, where);
+  }
+}
+
 // ------------------------------------------------------------------ caches whose weights fit the registers of a cluster
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -48,10 +137,11 @@ __device__ __forceinline__ void store_peer(uint32_t at, uint32_t rank, uint4 v) 
   asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(there), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
-// One cluster of CTAS CTAs a (request, KV head); each has a run of slots, KEYS a thread in
-// registers.  The key of the last slot that stays is found two bits at a time: how many keys
-// are not below each of three candidates, counted in registers, over a warp, through shared
-// memory and, between the CTAs, distributed shared memory: 16 short rounds, whatever the
+// KEYS slots a thread in registers; each CTA of a cluster has a run of the slots, or, where the
+// kernel MOVES the rows too, has them all and finds by itself what the others find.  The key of
+// the last slot that stays is found two bits at a time: how many keys are not below each of
+// three candidates, counted in registers, over a warp, through shared memory and, between the
+// CTAs that share the slots, distributed shared memory: at most 16 short rounds, whatever the
 // weights are (counting them by their bytes meets the same few counters again and again).
 template <int THREADS, int KEYS>
 struct Select {
@@ -59,14 +149,14 @@ struct Select {
   static_assert(KEYS <= 16 && kCells % 32 == 0, "a warp's count has 10 bits");
   uint32_t cells[kCells];    // per (key of a thread, warp): flags counted, then those before
   uint32_t packed[2][kWarps];
-  uint4 peers[2][8];         // counts of the cluster's CTAs
-  uint32_t total;
+  uint4 peers[2][8];         // counts of the CTAs that share the slots
 };
 
-template <int THREADS, int KEYS>
-__global__ void __launch_bounds__(THREADS) paged_select_kernel(const __grid_constant__ aicas_paged_evict_params a, int ctas) {
+template <int THREADS, int KEYS, bool MOVES>
+__global__ void __launch_bounds__(THREADS) paged_select_kernel(const __grid_constant__ MoveArgs m, int ctas) {
   using S = Select<THREADS, KEYS>;
   __shared__ S sm;
+  const aicas_paged_evict_params& a = m.p;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, rank = ctas > 1 ? (int)cluster_rank() : 0;
   const int pair = blockIdx.x / ctas, b = pair / a.num_kv_heads, h = pair - b * a.num_kv_heads;
   grid_launch_dependents();
@@ -75,10 +165,11 @@ __global__ void __launch_bounds__(THREADS) paged_select_kernel(const __grid_cons
   const float* w = a.weights + b * a.w_stride_b + h * a.w_stride_h;
   float* wo = a.weights_out + b * a.wo_stride_b + h * a.wo_stride_h;
   int32_t* kept = a.kept + (int64_t)pair * a.keep;
+  if (MOVES && a.kv_lens_out != nullptr && h == 0 && rank == 0 && tid == 0) a.kv_lens_out[b] = n > a.longer_than ? a.keep : n;
   if (n <= a.longer_than) return keep_all(a, n, w, wo, kept, rank * THREADS + tid, ctas * THREADS);
 
-  if (ctas > 1) cluster_sync();  // every CTA runs before another writes to its shared memory
-  const int run = (n + ctas - 1) / ctas, t0 = rank * run, t1 = min(n, t0 + run);  // this CTA's slots
+  if (!MOVES && ctas > 1) cluster_sync();  // every CTA runs before another writes to its shared memory
+  const int run = MOVES ? n : (n + ctas - 1) / ctas, t0 = MOVES ? 0 : rank * run, t1 = min(n, t0 + run);  // this CTA's slots
   const int lo = a.keep_first, hi = n - a.keep_last;
   // The weights stay in registers where these hold them beside the keys.
   constexpr bool kHeld = KEYS <= 8;
@@ -102,7 +193,7 @@ __global__ void __launch_bounds__(THREADS) paged_select_kernel(const __grid_cons
     uint3 s = make_uint3(__reduce_add_sync(0xffffffffu, p & 1023u), __reduce_add_sync(0xffffffffu, p >> 10 & 1023u),
                          __reduce_add_sync(0xffffffffu, p >> 20));
     if (before != nullptr) *before = make_uint3(0u, 0u, 0u);
-    if (ctas > 1) {
+    if (!MOVES && ctas > 1) {
       if (warp == 0 && lane < ctas) store_peer(smem_u32(&sm.peers[buf][rank]), lane, make_uint4(s.x, s.y, s.z, 0u));
       __syncwarp();
       cluster_sync();
@@ -181,17 +272,31 @@ __global__ void __launch_bounds__(THREADS) paged_select_kernel(const __grid_cons
   if constexpr (!kHeld)
 #pragma unroll
     for (int j = 0; j < KEYS; ++j) x[j] = stays >> j & 1u ? w[t0 + j * THREADS + tid] : 0.f;
-  uint3 before;
-  sums(__popc(stays), 0u, 0u, &before);
+  uint3 before = make_uint3(0u, 0u, 0u);
+  if (!MOVES)
+    sums(__popc(stays), 0u, 0u, &before);
+  else if (ctas > 1)
+    cluster_sync();  // all CTAs have read the weights
   places(stays, before.x);
+  __shared__ int32_t list[MOVES ? THREADS * KEYS : 1];
 #pragma unroll
   for (int j = 0; j < KEYS; ++j) {
     const int t = t0 + j * THREADS + tid;
     if (stays >> j & 1u) {
-      kept[place[j]] = t;
-      wo[place[j]] = x[j];  // below keep; every CTA's weights are read
+      if (MOVES) list[place[j]] = t;
+      if (!MOVES || rank == 0) {
+        kept[place[j]] = t;
+        wo[place[j]] = x[j];  // below keep
+      }
     }
-    if (t >= a.keep && t < t1) wo[t] = 0.f;
+    if ((!MOVES || rank == 0) && t >= a.keep && t < t1) wo[t] = 0.f;
+  }
+  if constexpr (MOVES) {
+    __shared__ Move where[3][kMostRows];
+    for (int at = rank; at < m.parts[a.num_planes]; at += ctas) {
+      __syncthreads();  // the list is written, the places of the part before are done with
+      move_part<THREADS, 4>(m, list, b, h, at, where);
+    }
   }
 }
 
@@ -281,79 +386,8 @@ __global__ void __launch_bounds__(kLongThreads) paged_select_long_kernel(const _
   for (int t = a.keep + tid; t < n; t += kLongThreads) wo[t] = 0.f;
 }
 
-// ------------------------------------------------------------------ rows
-
 constexpr int kMoveThreads = 256;
-constexpr int kMostRows = 512;  // of a run
-constexpr int kMoveCtas = 1;    // an SM, at least, as far as columns of 32 bytes go
 
-struct MoveArgs {
-  aicas_paged_evict_params p;
-  int parts[AICAS_EVICT_MAX_PLANES + 1];  // the planes' first column parts
-  int part_bytes[AICAS_EVICT_MAX_PLANES];
-  uint32_t octets_mul;                    // n / octets of a page = (umulhi(n, octets_mul) + n) >> octets_shift
-  int octets_shift;
-};
-
-struct Move {
-  int64_t src, dst;  // places in the plane, in bytes; -1: none (zeros; nothing to write)
-};
-
-// A row has LANES threads with a V each; ROWS rows a thread and run.  While a run's rows are
-// on their way, where the next one's lie is looked up, a row a thread.
-template <typename V, int LANES, int ROWS>
-__device__ __forceinline__ void move_rows(const MoveArgs& m, const aicas_evict_plane& pl, const int32_t* kept, int b, int h, int part,
-                                          Move (*where)[kMostRows]) {
-  const aicas_paged_evict_params& a = m.p;
-  constexpr int kSlots = kMoveThreads / LANES, kRun = kSlots * ROWS;
-  static_assert(kRun <= kMostRows, "a run's places");
-  const int r = threadIdx.x / LANES;
-  char* data = static_cast<char*>(pl.data) + h * pl.stride_h + (int64_t)part * (LANES * sizeof(V)) + threadIdx.x % LANES * sizeof(V);
-  const int32_t* table = a.page_table + b * a.table_stride;
-  const auto at = [&](int slot) -> int64_t {
-    const uint32_t n = (uint32_t)slot >> 3, i = (__umulhi(n, m.octets_mul) + n) >> m.octets_shift;
-    const int page = table[i];
-    return page >= 0 && page < a.num_pages ? page * pl.stride_p + (slot - (int)i * a.page_size) * pl.stride_t : -1;
-  };
-  const auto look = [&](int run) {
-    for (int x = threadIdx.x; x < kRun; x += kMoveThreads) {
-      const int i = run * kRun + x, from = i < a.keep ? kept[i] : -1;
-      Move w = {-1, -1};
-      if (from > i) w.src = at(from), w.dst = at(i);
-      where[run % 3][x] = w;
-    }
-  };
-  const int runs = (a.keep + kRun - 1) / kRun;
-  int run = 0;
-  // what stays in place, where it may be worth a look
-  while (run < runs && runs > 2 && kept[min(a.keep, (run + 1) * kRun) - 1] <= min(a.keep, (run + 1) * kRun) - 1) ++run;  // what stays in place
-  if (run == runs) return;
-  V v[ROWS], next[ROWS];
-  const auto load = [&](int run, V (&x)[ROWS]) {
-#pragma unroll
-    for (int k = 0; k < ROWS; ++k) {
-      const int64_t src = where[run % 3][k * kSlots + r].src;
-      x[k] = V{};
-      if (src >= 0) x[k] = *reinterpret_cast<const V*>(data + src);
-    }
-  };
-  look(run);
-  __syncthreads();
-  load(run, v);
-  for (; run < runs; ++run) {
-    if (run + 1 < runs) look(run + 1);
-    __syncthreads();  // this run is read; the next one's rows are not among those written now
-    if (run + 1 < runs) load(run + 1, next);
-#pragma unroll
-    for (int k = 0; k < ROWS; ++k) {
-      const int64_t dst = where[run % 3][k * kSlots + r].dst;
-      if (dst >= 0) *reinterpret_cast<V*>(data + dst) = v[k];
-      v[k] = next[k];
-    }
-  }
-}
-
-// ROWS: 8 a thread where an SM has few CTAs, 4 (and twice the CTAs) where it has many.
 template <int ROWS>
 __global__ void __launch_bounds__(kMoveThreads) paged_move_kernel(const __grid_constant__ MoveArgs m) {
   __shared__ Move where[3][kMostRows];
@@ -368,26 +402,36 @@ __global__ void __launch_bounds__(kMoveThreads) paged_move_kernel(const __grid_c
     a.kv_lens_out[b] = n > a.longer_than ? a.keep : n;
   }
   // kv_lens_out may be kv_lens: the others go by the list of slots alone
-  const int32_t* kept = a.kept + (int64_t)pair * a.keep;
-  int i = 0;
-  while (at >= m.parts[i + 1]) ++i;
-  const aicas_evict_plane& pl = a.plane[i];
-  const int part = at - m.parts[i];
-  switch (m.part_bytes[i]) {
-    case 256: return move_rows<uint4, 16, ROWS>(m, pl, kept, b, h, part, where);
-    case 128: return move_rows<uint4, 8, ROWS>(m, pl, kept, b, h, part, where);
-    case 64: return move_rows<uint4, 4, ROWS>(m, pl, kept, b, h, part, where);
-    case 32: return move_rows<uint4, 2, 4>(m, pl, kept, b, h, part, where);
-    case 16: return move_rows<uint4, 1, 2>(m, pl, kept, b, h, part, where);
-    case 8: return move_rows<uint2, 1, 2>(m, pl, kept, b, h, part, where);
-    default: return move_rows<uint32_t, 1, 2>(m, pl, kept, b, h, part, where);
+  move_part<kMoveThreads, ROWS>(m, a.kept + (int64_t)pair * a.keep, b, h, at, where);
+}
+
+// One launch for as many pairs as have their clusters of 8 at once.  One launch, two:
+// 8 pairs cut from 1500 to 1024 slots of 256 bytes 8.5 us, 11.8, from 4096 to 2900 16.4, 24.5;
+// 14 from 1501 to 333 11.7, 14.0; 16 from 1500 to 1024 14.8, 12.0, from 4096 to 1024 20.0, 15.5.
+constexpr int kOneLaunch = 10;  // SMs a pair
+
+// Columns that the planes' rows are moved by: as wide as leaves `least` parts, at most 256 bytes.
+void set_parts(MoveArgs& m, int64_t least) {
+  for (int most = 256;; most /= 2) {
+    m.parts[0] = 0;
+    for (int i = 0; i < m.p.num_planes; ++i) {
+      const int bytes = (int)m.p.plane[i].row_bytes;
+      int part = 16;
+      if (bytes < 16)
+        part = bytes;
+      else
+        while (part < most && bytes % (2 * part) == 0) part *= 2;
+      m.part_bytes[i] = part;
+      m.parts[i + 1] = m.parts[i] + bytes / part;
+    }
+    if (most == 32 || m.parts[m.p.num_planes] >= least) return;
   }
 }
 
-template <int THREADS, int KEYS>
-cudaError_t launch_select(const aicas_paged_evict_params& p, int ctas, cudaStream_t st) {
+template <int THREADS, int KEYS, bool MOVES>
+cudaError_t launch_select(const MoveArgs& m, int ctas, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.batch * p.num_kv_heads * ctas));
+  cfg.gridDim = dim3((unsigned)(m.p.batch * m.p.num_kv_heads * ctas));
   cfg.blockDim = dim3(THREADS);
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -397,51 +441,44 @@ cudaError_t launch_select(const aicas_paged_evict_params& p, int ctas, cudaStrea
   attr[1].val.clusterDim.x = (unsigned)ctas, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = ctas > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, paged_select_kernel<THREADS, KEYS>, p, ctas);
+  return cudaLaunchKernelEx(&cfg, paged_select_kernel<THREADS, KEYS, MOVES>, m, ctas);
 }
 
-cudaError_t launch_select_for(const aicas_paged_evict_params& p, cudaStream_t st) {
-  const int64_t slots = (int64_t)p.max_pages * p.page_size;
-  if (slots <= 512 * 4) return launch_select<512, 4>(p, 1, st);
+cudaError_t launch_select_for(const MoveArgs& m, cudaStream_t st) {
+  const int64_t slots = (int64_t)m.p.max_pages * m.p.page_size;
+  if (slots <= 512 * 4) return launch_select<512, 4, false>(m, 1, st);
   for (int ctas = 1; ctas <= 8; ctas *= 2)
-    if (slots <= (int64_t)512 * 8 * ctas) return launch_select<512, 8>(p, ctas, st);
-  if (slots <= 512 * 16 * 8) return launch_select<512, 16>(p, 8, st);
-  if (slots <= 1024 * 16 * 8) return launch_select<1024, 16>(p, 8, st);
-  return launch_pdl(paged_select_long_kernel, dim3((unsigned)(p.batch * p.num_kv_heads)), dim3(kLongThreads), 0, st, p);
+    if (slots <= (int64_t)512 * 8 * ctas) return launch_select<512, 8, false>(m, ctas, st);
+  if (slots <= 512 * 16 * 8) return launch_select<512, 16, false>(m, 8, st);
+  if (slots <= 1024 * 16 * 8) return launch_select<1024, 16, false>(m, 8, st);
+  return launch_pdl(paged_select_long_kernel, dim3((unsigned)(m.p.batch * m.p.num_kv_heads)), dim3(kLongThreads), 0, st, m.p);
 }
 
 }  // namespace
 
 int run_paged_evict(const aicas_paged_evict_params* p, int sms, cudaStream_t stream, char* err, size_t errlen) {
-  const unsigned pairs = (unsigned)(p->batch * p->num_kv_heads);
-  cudaError_t e = launch_select_for(*p, stream);
+  const int64_t pairs = (int64_t)p->batch * p->num_kv_heads, slots = (int64_t)p->max_pages * p->page_size;
   MoveArgs m;
   m.p = *p;
-  // whole rows, or as many parts of them as give each SM a few CTAs
-  int most = 256;
-  for (;; most /= 2) {
-    m.parts[0] = 0;
-    for (int i = 0; i < p->num_planes; ++i) {
-      const int bytes = (int)p->plane[i].row_bytes;
-      int part = 16;
-      if (bytes < 16)
-        part = bytes;
-      else
-        while (part < most && bytes % (2 * part) == 0) part *= 2;
-      m.part_bytes[i] = part;
-      m.parts[i + 1] = m.parts[i] + bytes / part;
-    }
-    if (most == 32 || (int64_t)pairs * m.parts[p->num_planes] >= kMoveCtas * sms) break;
-  }
   // n / d for n < 2^28, as in paged_int4_tiles.cuh
   const int octets = p->page_size / 8;
   m.octets_shift = 0;
   while ((1ll << m.octets_shift) < octets) ++m.octets_shift;
   m.octets_mul = (uint32_t)((((1ull << m.octets_shift) - octets) << 32) / octets + 1);
-  if (e == cudaSuccess)
-    // 32 caches cut to 1024 slots (512 CTAs) 65.2 us with 8, 62.6 with 4; 4 caches cut to 8192 (256 CTAs) 97, 133
-    e = launch_pdl(pairs * m.parts[p->num_planes] <= 2u * sms ? paged_move_kernel<8> : paged_move_kernel<4>,
-                   dim3(pairs * m.parts[p->num_planes]), dim3(kMoveThreads), 0, stream, m);
+  cudaError_t e;
+  if (slots <= 512 * 8 && pairs * kOneLaunch <= sms && (p->kv_lens_out == nullptr || p->kv_lens_out != p->kv_lens)) {
+    set_parts(m, 8);
+    const int ctas = m.parts[p->num_planes] >= 8 ? 8 : m.parts[p->num_planes] >= 4 ? 4 : 2;
+    e = slots <= 512 * 4 ? launch_select<512, 4, true>(m, ctas, stream) : launch_select<512, 8, true>(m, ctas, stream);
+  } else {
+    e = launch_select_for(m, stream);
+    // whole rows, or as many parts of them as give each SM a CTA
+    set_parts(m, (sms + pairs - 1) / pairs);
+    const int64_t ctas = pairs * m.parts[p->num_planes];
+    if (e == cudaSuccess)
+      // 32 caches cut to 1024 slots (512 CTAs) 65.2 us with 8, 62.6 with 4; 4 caches cut to 8192 (256 CTAs) 97, 133
+      e = launch_pdl(ctas <= 2 * sms ? paged_move_kernel<8> : paged_move_kernel<4>, dim3((unsigned)ctas), dim3(kMoveThreads), 0, stream, m);
+  }
   if (e == cudaSuccess) return AICAS_OK;
   snprintf(err, errlen, "paged evict launch: %s (%s)", cudaGetErrorString(e), cudaGetErrorName(e));
   return AICAS_ERR_CUDA;
