@@ -460,6 +460,17 @@ int run_paged_evict(const aicas_paged_evict_params* p, int sms, cudaStream_t str
   const int64_t pairs = (int64_t)p->batch * p->num_kv_heads, slots = (int64_t)p->max_pages * p->page_size;
   MoveArgs m;
   m.p = *p;
+  // rows that are keys and values at once move once
+  m.p.num_planes = 0;
+  for (int i = 0; i < p->num_planes; ++i) {
+    const aicas_evict_plane& x = p->plane[i];
+    bool there = false;
+    for (int j = 0; j < m.p.num_planes; ++j) {
+      const aicas_evict_plane& y = m.p.plane[j];
+      there |= x.data == y.data && x.stride_p == y.stride_p && x.stride_h == y.stride_h && x.stride_t == y.stride_t && x.row_bytes == y.row_bytes;
+    }
+    if (!there) m.p.plane[m.p.num_planes++] = x;
+  }
   // n / d for n < 2^28, as in paged_int4_tiles.cuh
   const int octets = p->page_size / 8;
   m.octets_shift = 0;
@@ -468,13 +479,13 @@ int run_paged_evict(const aicas_paged_evict_params* p, int sms, cudaStream_t str
   cudaError_t e;
   if (slots <= 512 * 8 && pairs * kOneLaunch <= sms && (p->kv_lens_out == nullptr || p->kv_lens_out != p->kv_lens)) {
     set_parts(m, 8);
-    const int ctas = m.parts[p->num_planes] >= 8 ? 8 : m.parts[p->num_planes] >= 4 ? 4 : 2;
+    const int ctas = m.parts[m.p.num_planes] >= 8 ? 8 : m.parts[m.p.num_planes] >= 4 ? 4 : 2;
     e = slots <= 512 * 4 ? launch_select<512, 4, true>(m, ctas, stream) : launch_select<512, 8, true>(m, ctas, stream);
   } else {
     e = launch_select_for(m, stream);
     // whole rows, or as many parts of them as give each SM a CTA
     set_parts(m, (sms + pairs - 1) / pairs);
-    const int64_t ctas = pairs * m.parts[p->num_planes];
+    const int64_t ctas = pairs * m.parts[m.p.num_planes];
     if (e == cudaSuccess)
       // 32 caches cut to 1024 slots (512 CTAs) 65.2 us with 8, 62.6 with 4; 4 caches cut to 8192 (256 CTAs) 97, 133
       e = launch_pdl(ctas <= 2 * sms ? paged_move_kernel<8> : paged_move_kernel<4>, dim3((unsigned)ctas), dim3(kMoveThreads), 0, stream, m);

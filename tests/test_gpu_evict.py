@@ -299,6 +299,25 @@ def test_evict_refusals(cuda_device):
             case()
 
 
+@pytest.mark.parametrize("group,batch", [(0, 2), (128, 2), (64, 40)])
+def test_evict_of_one_pool_as_keys_and_values(cuda_device, group, batch):
+    """Rows that are both move once (batches of the one launch, and of the two)."""
+    g = torch.Generator().manual_seed(5)
+    per, hkv = 20, 2
+    pool = _pages(g, batch * per, hkv, 16, 128, group, "bf16", cuda_device)
+    copy = ab.Int4Pages(*(t.clone() for t in pool)) if group else pool.clone()
+    table = _table(g, batch, per, batch * per, cuda_device)
+    w = torch.rand(batch, hkv, per * 16, generator=g).to(cuda_device)
+    lens = torch.full((batch,), per * 16, dtype=torch.int32, device=cuda_device)
+    kept = ab.paged_kv_evict(pool, pool, table, w, lens, keep=100, keep_first=4, keep_last=20)
+    for now, was in zip(pool, copy) if group else [(pool, copy)]:
+        for b in range(batch):
+            new, old = (t[table[b].long()].transpose(0, 1).flatten(1, 2) for t in (now, was))
+            for h in range(hkv):
+                assert torch.equal(new[h, :100], old[h, kept[b, h].long()])
+                assert torch.equal(new[h, 100:], old[h, 100:])
+
+
 # ------------------------------------------------------------------ together
 
 
