@@ -47,6 +47,28 @@ __device__ __forceinline__ void group_range(uint32_t lanes, float& lo, float& hi
   }
 }
 
+// Two numbers, two operations an instruction, each rounded as one of its own (8 prompts of 2048
+// tokens written and read back 80 -> 78 us).
+struct Two {
+  uint64_t u;
+  Two() = default;
+  __device__ __forceinline__ Two(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(u) : "f"(x), "f"(y)); }
+  __device__ __forceinline__ explicit Two(float x) : Two(x, x) {}
+  __device__ __forceinline__ void get(float& x, float& y) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(u)); }
+};
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(a.u) : "l"(b.u));
+  return a;
+}
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+  asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(a.u) : "l"(b.u));
+  return a;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c.u) : "l"(a.u), "l"(b.u));
+  return c;
+}
+
 // A group's (scale, least) as the cache holds them, and what its codes are taken by.
 struct Levels {
   float scale, least, inv;
@@ -76,18 +98,18 @@ struct Levels {
     if (inv == 0.f) return 0u;  // one value, or NaN
     // 1.5 x 2^23: a sum with it has the number, rounded to a whole one, in its low bits
     constexpr float kWhole = 12582912.f;
-    const float at = fmaf(-least, inv, kWhole);
-    int q[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float near = fmaf(x[i], inv, at) - kWhole;
-      const float w = fmaf(fmaf(-near, scale, x[i] - least), inv, near);
-      q[i] = __float_as_int(w * 0x1p-149f);  // as so many of the smallest steps: the number, rounded to a whole one
-    }
+    const Two at(fmaf(-least, inv, kWhole)), by(inv), down(-scale), from(-least);
     uint32_t u = 0;
 #pragma unroll
-    for (int i = 6; i >= 0; i -= 2)  // two numbers, held to 0..15, below what is there
-      asm("cvt.pack.sat.u4.s32.b32 %0, %1, %2, %0;" : "+r"(u) : "r"(q[i + 1]), "r"(q[i]));
+    for (int i = 6; i >= 0; i -= 2) {
+      const Two v(x[i], x[i + 1]), near = fma2(v, by, at) + Two(-kWhole);
+      // as so many of the smallest steps: the number, rounded to a whole one
+      const Two w = fma2(fma2(near, down, v + from), by, near) * Two(0x1p-149f);
+      float a, b;
+      w.get(a, b);
+      // two numbers, held to 0..15, below what is there
+      asm("cvt.pack.sat.u4.s32.b32 %0, %1, %2, %0;" : "+r"(u) : "r"(__float_as_int(b)), "r"(__float_as_int(a)));
+    }
     return u;
   }
 };
@@ -195,10 +217,10 @@ __device__ __forceinline__ void token_rows(const aicas_paged_append_int4_params&
       }
       if constexpr (kAsTorch) {
 #pragma unroll
-        for (int i = 0; i < kV; ++i) {
-          const float p1 = x1[i], p2 = x2[i];
-          x1[i] = __fadd_rn(__fmul_rn(p1, t.c1[i]), __fmul_rn(-p2, t.s1[i]));
-          x2[i] = __fadd_rn(__fmul_rn(p2, t.c2[i]), __fmul_rn(p1, t.s2[i]));
+        for (int i = 0; i < kV; i += 2) {
+          const Two p1(x1[i], x1[i + 1]), p2(x2[i], x2[i + 1]);
+          (p1 * Two(t.c1[i], t.c1[i + 1]) + p2 * Two(-t.s1[i], -t.s1[i + 1])).get(x1[i], x1[i + 1]);
+          (p2 * Two(t.c2[i], t.c2[i + 1]) + p1 * Two(t.s2[i], t.s2[i + 1])).get(x2[i], x2[i + 1]);
         }
       } else {
         rotated_pair<T, kRoundEach, kV>(x1, x2, t.c1, t.c2, t.s1, t.s2);
@@ -239,12 +261,18 @@ __device__ __forceinline__ void token_rows(const aicas_paged_append_int4_params&
   }
 }
 
-// HBM bound: the token's rows are read once, q written in 16 and k and v in 4 bits.  One
-// CTA a token, as in paged_append.cu: a row (one head of q, k or v) belongs to D / 16
-// threads, each with one 16-byte vector of the row's first half and the matching one of its
-// second half, so that the rotation needs no exchange, and with groups of 64 in rows of 128
-// each half is a group.  PROMPT: one warp, and q's, k's and v's rows one after the other
-// with several in flight; else a row a thread, all at once.
+// The token's rows are read once, q is written in 16 and k and v in 4 bits.  As in
+// paged_append.cu a row (one head of q, k or v) belongs to D / 16 threads, each with one
+// 16-byte vector of the row's first half and the matching one of its second half, so that the
+// rotation needs no exchange, and with groups of 64 in rows of 128 each half is a group.
+// PROMPT: a warp a token, and q's, k's and v's rows one after the other with several in
+// flight; else a CTA a token, a row a thread, all at once.
+//
+// One token of 16 query and 8 KV heads of 128 and its read back 4.0 us, 64 tokens 4.3: two
+// launches.  8 prompts of 2048 tokens and their read back 78 us, 3.9 TB/s: about 2200
+// instructions a token, whose chains 16 warps an SM (of 128 registers a thread) cover to 57% of
+// the issue slots, while the memory is at 40%.  Rows asked for a token ahead (85 -> 92 us),
+// 18 to 28 resident warps and larger CTAs were slower.
 constexpr int kPromptWarps = 4;
 
 template <typename T, typename CS, int D, bool HALVES, bool PROMPT>
@@ -298,7 +326,9 @@ __global__ void __launch_bounds__(PROMPT ? 32 * kPromptWarps : 256, PROMPT ? 16 
   }
 }
 
-constexpr int kPromptTokens = 600;  // see launch_append_sized
+// Tokens up to which each gets a CTA: the append and read of 16 x 16 tokens of 8 KV heads
+// 5.3 us, a warp each 7.3; of 512 8.3, 11.1; of 1024 13.2, 12.1; of 2 x 2048 45.8, 24.5.
+constexpr int kPromptTokens = 600;
 
 template <typename T, typename CS, int D, bool HALVES>
 cudaError_t launch_append_sized(const aicas_paged_append_int4_params& p, cudaStream_t st) {
@@ -326,9 +356,16 @@ __device__ __forceinline__ uint4 widened(uint32_t u, uint32_t p) {
   } pair;
   pair.u = p;
   const float scale = Elem<T>::to_float(pair.t[0]), least = Elem<T>::to_float(pair.t[1]);
+  // a byte below the exponent of 2^23 is 2^23 and the byte
+  constexpr float kWhole = 8388608.f;
+  const Two by(scale), from(least);
+  const uint32_t even = u & 0x0f0f0f0fu, odd = u >> 4 & 0x0f0f0f0fu;
   float f[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) f[e] = fmaf(scale, (float)(u >> (4 * e) & 15u), least);
+  for (int k = 0; k < 4; ++k) {
+    const Two code(__uint_as_float(__byte_perm(even, 0x4b000000u, 0x7440 + k)), __uint_as_float(__byte_perm(odd, 0x4b000000u, 0x7440 + k)));
+    fma2(code + Two(-kWhole), by, from).get(f[2 * k], f[2 * k + 1]);
+  }
   return pack_vec<T>(f);
 }
 
@@ -341,8 +378,9 @@ __device__ __forceinline__ int2 row_at(const aicas_paged_read_int4_params& a, in
   return make_int2(page < a.num_pages ? page : -1, (int)slot - i * a.page_size);
 }
 
-// HBM bound: 16 elements a thread, 8 bytes of codes in and 32 bytes out, of ROWS rows of one
-// request, side and head, so that their page numbers, codes and pairs are on the way at once.
+// HBM bound, by what it writes: 16 elements a thread, 8 bytes of codes in and 32 bytes out, of
+// ROWS rows of one request, side and head, so that their page numbers, codes and pairs are on
+// the way at once.
 template <typename T, int D, bool HALVES, int ROWS>
 __global__ void __launch_bounds__(256) paged_read_int4_kernel(const __grid_constant__ aicas_paged_read_int4_params a, int chunks) {
   constexpr int kTpr = D / 16, kSlots = 256 / kTpr;
@@ -409,7 +447,9 @@ __global__ void __launch_bounds__(kFewThreads) paged_read_few_int4_kernel(const 
 
 template <typename T, int D, bool HALVES>
 cudaError_t launch_read_sized(const aicas_paged_read_int4_params& p, cudaStream_t st) {
-  if ((int64_t)p.num_kv_heads * p.seq_len * (D / 8) <= 512)
+  // with the append of as many: 16 x 16 tokens of 8 heads (2048) 5.3 us, 5.7 in the other kernel, 256 x 1 5.5, 8.5;
+  // 1 x 512 (65536) 9.0, 8.1
+  if ((int64_t)p.num_kv_heads * p.seq_len * (D / 8) <= 2048)
     return launch_pdl(paged_read_few_int4_kernel<T, D, HALVES>,
                       dim3((unsigned)p.batch, (2 * p.num_kv_heads * p.seq_len * (D / 8) + kFewThreads - 1) / kFewThreads), dim3(kFewThreads), 0,
                       st, p);

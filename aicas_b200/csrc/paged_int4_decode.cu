@@ -23,9 +23,17 @@
 //     the operand layout by a transposing 8 x 8 move in registers.
 //   * Rounding: a 16-bit q is exact in one fp16 after scaling by a power of two a head (down
 //     to 2^-29 of its largest element).  A probability times its scale enters P V as two
-//     fp16 parts (22 bits; down to 2^-37 of the largest), scaled by a power of two that
-//     follows the largest scale.  Everything else is fp32.
+//     fp16 parts, 22 bits, or to within 2^-25 of numbers that a power of two brings to 2^7 and
+//     more for the largest scale of V so far: 2^-32 of that scale, whatever its slot's
+//     probability.  Everything else is fp32.
 //   * Slots out of range: score -inf, V's scale and least 0.
+//   * Bound: HBM, from a few thousand tiles on.  16 query and 8 KV heads of 128 in bf16: 4
+//     caches of 131072 slots, groups of 128, 105 us, 5.75 TB/s; 64 of up to 4096 37 us, 4.15
+//     TB/s, of which about 5 us pass before the first products and 6 after the copies end.
+//     One of 1024 7.1 us: the chain lengths, page table, rows, products, join.
+//   * Taken and dropped (64 of up to 4096): masks after multiplies instead of shifts 41 -> 44
+//     us; rings of 3 stages no faster than 2; 8 warps of twice the registers 10% slower; two
+//     partial results joined at once 37 -> 52 (spills).
 #include <cstdio>
 #include <cstring>
 #include <type_traits>
@@ -38,11 +46,18 @@ namespace aicas {
 namespace {
 
 constexpr int kTile = kInt4Tile;
-constexpr int kRanges = 4;     // ranges that a pair is cut into, about
-constexpr int kPairCost = 3;   // what beginning and ending a pair costs a warp, in tiles
-constexpr int kSmallTiles = 32;  // most tiles a CTA of a launch that gives pairs whole CTAs
+// Ranges that a pair is cut into, about: 64 caches of up to 4096 slots, with 1 41.2 us, 2 38.0,
+// 4 36.9, 8 38.1.
+constexpr int kRanges = 4;
+// What beginning and ending a pair costs a warp, in tiles: the same with 1 38.2, 3 36.9, 6 38.1;
+// 256 caches of up to 512 30.4, 28.3, 29.9.
+constexpr int kPairCost = 3;
+// Most tiles a CTA of a launch that gives pairs whole teams: 8 caches of up to 2048 slots 10.4
+// us, in equal ranges 11.9 (with 8 already), one of 8192 10.2, 10.9.
+constexpr int kSmallTiles = 32;
 constexpr int kLogWarps = 4, kMaxWarps = 1 << kLogWarps;
-constexpr int kSmallLog = 2;   // warps of a team in a small launch
+// Warps of a team in a small launch, as a power of two: one cache of 1024 slots with 2 8.1 us, 4 7.1, 16 8.4.
+constexpr int kSmallLog = 2;
 constexpr int kHeads = 8;      // query heads of a block
 constexpr size_t kWsCounters = (size_t)1 << 20;  // counter region shared with the other decode kernels
 struct Int4Args {
@@ -96,7 +111,8 @@ __device__ __forceinline__ void split_half(float x, float y, uint32_t& hi, uint3
 // ------------------------------------------------------------------ a warp's state
 
 // WIDE: up to 8 heads, a column each, lo parts in products of their own; else up to 4
-// heads, head j's hi and lo parts in columns 2 j and 2 j + 1 of the same products.
+// heads, head j's hi and lo parts in columns 2 j and 2 j + 1 of the same products (2 heads, 4
+// caches of 131072 slots: 105 us, as WIDE 129).
 // A lane's heads: WIDE 2 i and 2 i + 1, else i; its slots of 16: rows g and g + 8 of a product.
 // K's fragments are words: lane i has 8 dims of each 32.  V's are 16-bit units of 4 dims,
 // paired over two slots by the transposing load: lane g has units g of each 32.
