@@ -1134,7 +1134,7 @@ int aicas_paged_decode_gqa(const aicas_paged_decode_params* p, void* workspace, 
 int aicas_paged_append_int4(const aicas_paged_append_int4_params* p, void* stream) {
   const int rc = check_paged_append_int4(p);
   if (rc != AICAS_OK) return rc;
-  return aicas::run_paged_append_int4(p, static_cast<cudaStream_t>(stream), g_err, sizeof(g_err));
+  return aicas::run_paged_append_int4(p, sm_count(), static_cast<cudaStream_t>(stream), g_err, sizeof(g_err));
 }
 
 int aicas_paged_read_int4(const aicas_paged_read_int4_params* p, void* stream) {

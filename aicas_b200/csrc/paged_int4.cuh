@@ -10,7 +10,7 @@ namespace aicas {
 
 // Each launches its kernel for validated parameters, returns an AICAS_* status
 // and writes a message into err on failure.
-int run_paged_append_int4(const aicas_paged_append_int4_params* p, cudaStream_t stream, char* err, size_t errlen);
+int run_paged_append_int4(const aicas_paged_append_int4_params* p, int sms, cudaStream_t stream, char* err, size_t errlen);
 int run_paged_read_int4(const aicas_paged_read_int4_params* p, cudaStream_t stream, char* err, size_t errlen);
 
 // Bytes of workspace run_paged_decode_int4 needs on a device with `sms` SMs.

@@ -155,28 +155,26 @@ struct Token {
   float c1[kV], c2[kV], s1[kV], s2[kV];
 };
 
-// Rows h, h + step, ... (COUNT of them, below `heads`) of the token's q (KIND 0), k (1) or v (2).
+// Where row 0 of token s of request b is, of q (kind 0), k (1) or v (2), and how far the next one.
+template <typename T>
+__device__ __forceinline__ const T* row_source(const aicas_paged_append_int4_params& a, int kind, int b, int s, int64_t& step) {
+  step = kind == 0 ? a.qi_stride_h : kind == 1 ? a.k_stride_h : a.v_stride_h;
+  return static_cast<const T*>(kind == 0 ? a.q_in : kind == 1 ? a.k_in : a.v_in) +
+         b * (kind == 0 ? a.qi_stride_b : kind == 1 ? a.k_stride_b : a.v_stride_b) +
+         s * (kind == 0 ? a.qi_stride_s : kind == 1 ? a.k_stride_s : a.v_stride_s);
+}
+
+// Rows h, h + step, ... (COUNT of them, below `heads`) of the token's q (KIND 0), k (1) or v (2);
+// u1, u2: the lane's vectors of them.
 template <typename T, typename CS, int D, bool HALVES, int KIND, int COUNT>
-__device__ __forceinline__ void token_rows(const aicas_paged_append_int4_params& a, const Token<CS, D>& t, int h, int step, int heads) {
+__device__ __forceinline__ void token_rows(const aicas_paged_append_int4_params& a, const Token<CS, D>& t, int h, int step, int heads,
+                                           const uint4 (&u1)[COUNT], const uint4 (&u2)[COUNT]) {
   using K = Token<CS, D>;
   constexpr int kV = K::kV, kTpr = K::kTpr;
   constexpr bool kRoundEach = std::is_same<T, CS>::value;
   // Keys in fp32: every operation rounded as torch's, so that they get the codes that torch's keys
   // would get (a fused product and sum puts some on the other side of a border).
   constexpr bool kAsTorch = KIND == 1 && !kRoundEach;
-  const T* src = static_cast<const T*>(KIND == 0 ? a.q_in : KIND == 1 ? a.k_in : a.v_in) +
-                 t.b * (KIND == 0 ? a.qi_stride_b : KIND == 1 ? a.k_stride_b : a.v_stride_b) +
-                 t.s * (KIND == 0 ? a.qi_stride_s : KIND == 1 ? a.k_stride_s : a.v_stride_s) + t.c;
-  const int64_t src_h = KIND == 0 ? a.qi_stride_h : KIND == 1 ? a.k_stride_h : a.v_stride_h;
-  uint4 u1[COUNT], u2[COUNT];
-#pragma unroll
-  for (int j = 0; j < COUNT; ++j) {
-    u1[j] = u2[j] = make_uint4(0, 0, 0, 0);
-    if (h + j * step >= heads) continue;
-    const T* p = src + (h + j * step) * src_h;
-    u1[j] = *reinterpret_cast<const uint4*>(p);
-    u2[j] = *reinterpret_cast<const uint4*>(p + D / 2);
-  }
   const T* w = static_cast<const T*>(KIND == 0 ? a.q_norm_weight : a.k_norm_weight);
   uint4 w1 = {}, w2 = {};
   if (KIND < 2 && w != nullptr) {
@@ -265,30 +263,23 @@ __device__ __forceinline__ void token_rows(const aicas_paged_append_int4_params&
 // paged_append.cu a row (one head of q, k or v) belongs to D / 16 threads, each with one
 // 16-byte vector of the row's first half and the matching one of its second half, so that the
 // rotation needs no exchange, and with groups of 64 in rows of 128 each half is a group.
-// PROMPT: a warp a token, and q's, k's and v's rows one after the other with several in
-// flight; else a CTA a token, a row a thread, all at once.
+// PROMPT: a warp walks through tokens, a unit of two rows a lane at a time; the units are
+// copied into shared memory kUnits ahead, each lane's vectors by itself, so that the lanes wait
+// for no one.  Else a CTA a token, a row a thread, all at once.
 //
 // One token of 16 query and 8 KV heads of 128 and its read back 4.0 us, 64 tokens 4.3: two
-// launches.  8 prompts of 2048 tokens and their read back 78 us, 3.9 TB/s: about 2200
-// instructions a token, whose chains 16 warps an SM (of 128 registers a thread) cover to 57% of
-// the issue slots, while the memory is at 40%.  Rows asked for a token ahead (85 -> 92 us),
-// 18 to 28 resident warps and larger CTAs were slower.
-constexpr int kPromptWarps = 4;
+// launches.  8 prompts of 2048 tokens and their read back 74 us, 4.1 TB/s: about 2200
+// instructions a token, whose chains 16 warps an SM (of 128 registers a thread) cover to 62% of
+// the issue slots, while the memory is at 43%.  Without the copies ahead 78 us; rows asked for
+// ahead in registers 92, 20 and 24 warps an SM 79 and 104.
+constexpr int kPromptWarps = 4, kPromptCtas = 4;  // of a CTA, of an SM
+constexpr int kUnits = 2;  // 8 prompts of 2048 tokens with 2 74.0 us, 4 74.8, 6 76.8
 
-template <typename T, typename CS, int D, bool HALVES, bool PROMPT>
-__global__ void __launch_bounds__(PROMPT ? 32 * kPromptWarps : 256, PROMPT ? 16 / kPromptWarps : 1)
-    paged_append_int4_kernel(const __grid_constant__ aicas_paged_append_int4_params a) {
-  using K = Token<CS, D>;
-  constexpr int kV = K::kV, kTpr = K::kTpr, kSlots = (PROMPT ? 32 : 256) / kTpr;
-  K t;
-  const int token = PROMPT ? blockIdx.x * kPromptWarps + threadIdx.x / 32 : blockIdx.x;
-  if (PROMPT && token >= a.batch * a.seq_len) return;
+// The lane's part of token `token`, but for what of it is its own.
+template <typename T, typename CS, int D>
+__device__ __forceinline__ void begin_token(const aicas_paged_append_int4_params& a, Token<CS, D>& t, int token, bool first_lane) {
+  constexpr int kV = Token<CS, D>::kV;
   t.b = token / a.seq_len, t.s = token - t.b * a.seq_len;
-  t.c = threadIdx.x % kTpr * kV;
-  t.lanes = ((1u << kTpr) - 1u) << (threadIdx.x % 32 / kTpr * kTpr);
-  const int hq = a.num_q_heads, hkv = a.num_kv_heads;
-  grid_launch_dependents();
-  grid_dependency_wait();
   // the token's slot; asked for first, needed last
   const int pos = a.positions[t.b];
   const int fresh = a.num_new != nullptr ? min(max(a.num_new[t.b], 0), a.seq_len) : a.seq_len;
@@ -301,7 +292,7 @@ __global__ void __launch_bounds__(PROMPT ? 32 * kPromptWarps : 256, PROMPT ? 16 
     t.page = a.page_table[t.b * a.table_stride + i];
     if (t.page >= a.num_pages) t.page = -1;
   }
-  if (a.kv_lens_out != nullptr && t.s == 0 && (PROMPT ? threadIdx.x % 32 : threadIdx.x) == 0)
+  if (a.kv_lens_out != nullptr && t.s == 0 && first_lane)
     a.kv_lens_out[t.b] = (int)min((long long)max(pos, 0) + fresh, (long long)cap);
   const CS* cp = static_cast<const CS*>(a.cos) + t.b * a.cs_stride_b + t.s * a.cs_stride_s + t.c;
   const CS* sp = static_cast<const CS*>(a.sin) + t.b * a.cs_stride_b + t.s * a.cs_stride_s + t.c;
@@ -309,40 +300,115 @@ __global__ void __launch_bounds__(PROMPT ? 32 * kPromptWarps : 256, PROMPT ? 16 
   load_floats<CS, kV>(cp + D / 2, t.c2);
   load_floats<CS, kV>(sp, t.s1);
   load_floats<CS, kV>(sp + D / 2, t.s2);
-  const int r0 = (PROMPT ? threadIdx.x % 32 : threadIdx.x) / kTpr;
-  if constexpr (PROMPT) {
-    for (int h = 0; h < hq; h += 4 * kSlots) token_rows<T, CS, D, HALVES, 0, 4>(a, t, h + r0, kSlots, hq);
-    for (int h = 0; h < hkv; h += 2 * kSlots) token_rows<T, CS, D, HALVES, 1, 2>(a, t, h + r0, kSlots, hkv);
-    for (int h = 0; h < hkv; h += 2 * kSlots) token_rows<T, CS, D, HALVES, 2, 2>(a, t, h + r0, kSlots, hkv);
-  } else {
-    for (int r = r0; r < hq + 2 * hkv; r += kSlots) {
-      if (r < hq)
-        token_rows<T, CS, D, HALVES, 0, 1>(a, t, r, 0, hq);
-      else if (r < hq + hkv)
-        token_rows<T, CS, D, HALVES, 1, 1>(a, t, r - hq, 0, hkv);
-      else
-        token_rows<T, CS, D, HALVES, 2, 1>(a, t, r - hq - hkv, 0, hkv);
+}
+
+template <typename T, typename CS, int D, bool HALVES>
+__global__ void __launch_bounds__(256, 1) paged_append_int4_kernel(const __grid_constant__ aicas_paged_append_int4_params a) {
+  using K = Token<CS, D>;
+  constexpr int kTpr = K::kTpr, kSlots = 256 / kTpr;
+  K t;
+  t.c = threadIdx.x % kTpr * K::kV;
+  t.lanes = ((1u << kTpr) - 1u) << (threadIdx.x % 32 / kTpr * kTpr);
+  const int hq = a.num_q_heads, hkv = a.num_kv_heads;
+  grid_launch_dependents();
+  grid_dependency_wait();
+  begin_token<T>(a, t, blockIdx.x, threadIdx.x == 0);
+  const auto row = [&](auto kind, int h, int heads) {
+    constexpr int kKind = decltype(kind)::value;
+    int64_t step;
+    const T* p = row_source<T>(a, kKind, t.b, t.s, step) + t.c;
+    p += h * step;
+    const uint4 u1[1] = {*reinterpret_cast<const uint4*>(p)}, u2[1] = {*reinterpret_cast<const uint4*>(p + D / 2)};
+    token_rows<T, CS, D, HALVES, kKind, 1>(a, t, h, 0, heads, u1, u2);
+  };
+  for (int r = threadIdx.x / kTpr; r < hq + 2 * hkv; r += kSlots) {
+    if (r < hq)
+      row(std::integral_constant<int, 0>(), r, hq);
+    else if (r < hq + hkv)
+      row(std::integral_constant<int, 1>(), r - hq, hkv);
+    else
+      row(std::integral_constant<int, 2>(), r - hq - hkv, hkv);
+  }
+}
+
+template <typename T, typename CS, int D, bool HALVES>
+__global__ void __launch_bounds__(32 * kPromptWarps, kPromptCtas)
+    paged_append_int4_prompt_kernel(const __grid_constant__ aicas_paged_append_int4_params a) {
+  using K = Token<CS, D>;
+  constexpr int kTpr = K::kTpr, kSlots = 32 / kTpr, kRows = 2 * kSlots;  // rows of a unit
+  __shared__ uint4 ring[kPromptWarps][kUnits][4][32];  // [first and second half of row 0, of row 1]
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, r0 = lane / kTpr;
+  const int tokens = a.batch * a.seq_len, warps = (int)gridDim.x * kPromptWarps;
+  const int hq = a.num_q_heads, hkv = a.num_kv_heads, nq = (hq + kRows - 1) / kRows, nk = (hkv + kRows - 1) / kRows;
+  K t;
+  t.c = lane % kTpr * K::kV;
+  t.lanes = ((1u << kTpr) - 1u) << (r0 * kTpr);
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int first = blockIdx.x * kPromptWarps + warp;
+  // the unit that is copied next
+  int64_t to_come = first;
+  int unit = 0, b = 0, s = 0;
+  const auto copy = [&](uint4 (&stage)[4][32]) {
+    if (to_come < tokens) {
+      if (unit == 0) b = (int)to_come / a.seq_len, s = (int)to_come - b * a.seq_len;
+      const int kind = unit < nq ? 0 : unit < nq + nk ? 1 : 2, of_kind = unit - (kind == 0 ? 0 : kind == 1 ? nq : nq + nk);
+      int64_t step;
+      const T* src = row_source<T>(a, kind, b, s, step) + t.c;
+      const int h = of_kind * kRows + r0, heads = kind == 0 ? hq : hkv;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        if (h + j * kSlots < heads) {
+          const T* p = src + (h + j * kSlots) * step;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(&stage[2 * j][lane])), "l"(p) : "memory");
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(&stage[2 * j + 1][lane])), "l"(p + D / 2) : "memory");
+        }
+      if (++unit == nq + 2 * nk) unit = 0, to_come += warps;
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int k = 0; k < kUnits; ++k) copy(ring[warp][k]);
+  int at = 0;
+  const auto rows = [&](auto kind, int n, int heads) {
+    constexpr int kKind = decltype(kind)::value;
+#pragma unroll 1
+    for (int u = 0; u < n; ++u) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kUnits - 1) : "memory");
+      uint4(&stage)[4][32] = ring[warp][at];
+      const uint4 u1[2] = {stage[0][lane], stage[2][lane]}, u2[2] = {stage[1][lane], stage[3][lane]};
+      token_rows<T, CS, D, HALVES, kKind, 2>(a, t, u * kRows + r0, kSlots, heads, u1, u2);
+      copy(stage);
+      at = at + 1 == kUnits ? 0 : at + 1;
+    }
+  };
+#pragma unroll 1
+  for (int64_t token = first; token < tokens; token += warps) {
+    begin_token<T>(a, t, (int)token, lane == 0);
+    rows(std::integral_constant<int, 0>(), nq, hq);
+    rows(std::integral_constant<int, 1>(), nk, hkv);
+    rows(std::integral_constant<int, 2>(), nk, hkv);
   }
 }
 
 // Tokens up to which each gets a CTA: the append and read of 16 x 16 tokens of 8 KV heads
-// 5.3 us, a warp each 7.3; of 512 8.3, 11.1; of 1024 13.2, 12.1; of 2 x 2048 45.8, 24.5.
+// 5.3 us, a warp each 7.3; of 512 8.4, 11.1; of 1024 13.2 both; of 2 x 2048 45.8, 24.7.
 constexpr int kPromptTokens = 600;
 
 template <typename T, typename CS, int D, bool HALVES>
-cudaError_t launch_append_sized(const aicas_paged_append_int4_params& p, cudaStream_t st) {
-  const dim3 grid((unsigned)(p.batch * p.seq_len));
-  return p.batch * p.seq_len <= kPromptTokens
-             ? launch_pdl(paged_append_int4_kernel<T, CS, D, HALVES, false>, grid, dim3(256), 0, st, p)
-             : launch_pdl(paged_append_int4_kernel<T, CS, D, HALVES, true>, dim3((grid.x + kPromptWarps - 1) / kPromptWarps),
-                          dim3(32 * kPromptWarps), 0, st, p);
+cudaError_t launch_append_sized(const aicas_paged_append_int4_params& p, int sms, cudaStream_t st) {
+  const int64_t tokens = (int64_t)p.batch * p.seq_len;
+  if (tokens <= kPromptTokens)
+    return launch_pdl(paged_append_int4_kernel<T, CS, D, HALVES>, dim3((unsigned)tokens), dim3(256), 0, st, p);
+  const int64_t ctas = (tokens + kPromptWarps - 1) / kPromptWarps;
+  return launch_pdl(paged_append_int4_prompt_kernel<T, CS, D, HALVES>, dim3((unsigned)(ctas < kPromptCtas * sms ? ctas : kPromptCtas * sms)),
+                    dim3(32 * kPromptWarps), 0, st, p);
 }
 
 template <typename T, typename CS>
-cudaError_t launch_append(const aicas_paged_append_int4_params& p, cudaStream_t st) {
-  if (p.head_dim == 64) return launch_append_sized<T, CS, 64, false>(p, st);
-  return p.group_size == 64 ? launch_append_sized<T, CS, 128, true>(p, st) : launch_append_sized<T, CS, 128, false>(p, st);
+cudaError_t launch_append(const aicas_paged_append_int4_params& p, int sms, cudaStream_t st) {
+  if (p.head_dim == 64) return launch_append_sized<T, CS, 64, false>(p, sms, st);
+  return p.group_size == 64 ? launch_append_sized<T, CS, 128, true>(p, sms, st) : launch_append_sized<T, CS, 128, false>(p, sms, st);
 }
 
 // ------------------------------------------------------------------ reads
@@ -472,13 +538,13 @@ int status(cudaError_t e, const char* what, char* err, size_t errlen) {
 
 }  // namespace
 
-int run_paged_append_int4(const aicas_paged_append_int4_params* p, cudaStream_t stream, char* err, size_t errlen) {
+int run_paged_append_int4(const aicas_paged_append_int4_params* p, int sms, cudaStream_t stream, char* err, size_t errlen) {
   const bool f32cs = p->cs_dtype == AICAS_DTYPE_F32;
   cudaError_t e = cudaErrorInvalidValue;
   if (p->dtype == AICAS_DTYPE_F16)
-    e = f32cs ? launch_append<__half, float>(*p, stream) : launch_append<__half, __half>(*p, stream);
+    e = f32cs ? launch_append<__half, float>(*p, sms, stream) : launch_append<__half, __half>(*p, sms, stream);
   else if (p->dtype == AICAS_DTYPE_BF16)
-    e = f32cs ? launch_append<__nv_bfloat16, float>(*p, stream) : launch_append<__nv_bfloat16, __nv_bfloat16>(*p, stream);
+    e = f32cs ? launch_append<__nv_bfloat16, float>(*p, sms, stream) : launch_append<__nv_bfloat16, __nv_bfloat16>(*p, sms, stream);
   return status(e, "paged 4-bit append", err, errlen);
 }
 
