@@ -78,7 +78,7 @@ __device__ __forceinline__ void move_rows(const MoveArgs& m, const aicas_evict_p
   const int runs = (a.keep + kRun - 1) / kRun;
   int run = 0;
   // what stays in place, where it may be worth a look
-  while (run < runs && runs > 2 && kept[min(a.keep, (run + 1) * kRun) - 1] <= min(a.keep, (run + 1) * kRun) - 1) ++run;  // what stays in place
+  while (run < runs && runs > 2 && kept[min(a.keep, (run + 1) * kRun) - 1] <= min(a.keep, (run + 1) * kRun) - 1) ++run;
   if (run == runs) return;
   V v[ROWS], next[ROWS];
   const auto load = [&](int run, V (&x)[ROWS]) {
@@ -405,8 +405,9 @@ __global__ void __launch_bounds__(kMoveThreads) paged_move_kernel(const __grid_c
     const int n = min(max(a.kv_lens[b], 0), a.max_pages * a.page_size);
     a.kv_lens_out[b] = n > a.longer_than ? a.keep : n;
   }
-  // kv_lens_out may be kv_lens: the others go by the list of slots alone
-  move_part<kMoveThreads, ROWS>(m, a.kept + (int64_t)pair * a.keep, b, h, at, where);
+  // kv_lens_out may be kv_lens: the others go by the list of slots alone, whose last says whether any slot moves
+  const int32_t* kept = a.kept + (int64_t)pair * a.keep;
+  if (kept[a.keep - 1] >= a.keep) move_part<kMoveThreads, ROWS>(m, kept, b, h, at, where);
 }
 
 // One launch for as many pairs as have their clusters of 8 at once.  One launch, two:
