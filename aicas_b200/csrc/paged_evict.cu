@@ -9,9 +9,9 @@
 // independent, so where there are few pairs, CTAs share a row by its columns.  Short caches of
 // few pairs do both in one launch, a cluster of CTAs a pair; the others in two.
 //
-// Bound: HBM, for the rows, after the selection's about 12 us.  8 KV heads of 128 in bf16: 32
-// caches of up to 4096 slots cut to 1024 62 us (4.2 TB/s while rows move), 4 of 32768 cut to
-// 8192 96 us, 64 4-bit ones of 2048 cut to 1024 and read back 120 us.
+// Bound: HBM, for the rows, after a selection of about 14 us.  8 KV heads of 128 in bf16: 32
+// caches of up to 4096 slots cut to 1024 62 us (5.3 TB/s while rows move), 4 of 32768 cut to
+// 8192 97 us, 64 4-bit ones of 2048 cut to 1024 and read back 118 us.
 #include <cstdio>
 
 #include "common.cuh"
