@@ -19,7 +19,8 @@
 //     of 16 queries over 4 4-bit caches of 16384 18.5 us, 4.1 for the bytes: the products, four
 //     blocks of 8 columns a tile, and 32 exponentials a slot and head.
 //   * Taken and dropped (64 of up to 4096): 3 CTAs an SM 52 -> 77 us (spills), tiles of 64 slots
-//     63; rings of 4 or 6 stages no faster.
+//     63; rings of 4 or 6 stages no faster; for the window, queries as rows with 32 of them in a
+//     warp's registers 18.4 -> 20.5 us, both 16 slots of a tile for one load of q 19.9 (spills).
 //
 // fp32 pages: a thread a slot, its row read once for each block of 8 queries (products of fp32
 // numbers in full; the pages that float checks use).

@@ -375,3 +375,61 @@ def test_steps_with_evictions(cuda_device, group):
                 assert int(lens[b]) == int(now[b])
     assert cuts >= 5
     assert nat.device_error_flags() == 0
+
+
+@pytest.mark.parametrize("group", [0, 128])
+def test_two_streams_at_once(cuda_device, group):
+    """Attention, weights and eviction on two streams, eager and from two graphs, many times over: the
+    same bits as alone."""
+    g = torch.Generator().manual_seed(21)
+    B, hq, hkv, D, per = 3, 8, 4, 128, 40
+    attend = ab.paged_gqa_decode_attention_int4 if group else ab.paged_gqa_decode_attention
+    sets = []
+    for _ in range(2):
+        kp, vp = (_pages(g, B * per, hkv, 16, D, group, "bf16", cuda_device) for _ in range(2))
+        table = _table(g, B, per, B * per, cuda_device)
+        q = torch.randn(B, hq, 1, D, generator=g).to(torch.bfloat16).to(cuda_device)
+        lens = torch.tensor([640, 17, 500], dtype=torch.int32, device=cuda_device)
+        held = [t.clone() for p in (kp, vp) for t in (p if group else (p,))]
+        w0 = torch.rand(B, hkv, per * 16, generator=g).to(cuda_device)
+        sets.append((kp, vp, table, q, lens, held, w0))
+
+    def run(kp, vp, table, q, lens, held, w0):
+        for t, was in zip([t for p in (kp, vp) for t in (p if group else (p,))], held):
+            t.copy_(was)
+        w = w0.clone()
+        kw = dict(sm_scale=0.09, num_key_value_groups=hq // hkv, kv_lens=lens)
+        out, lse = attend(q, kp, vp, table, return_lse=True, **kw)
+        ab.paged_attention_weights(q, kp, table, lse, w, **kw)
+        now = torch.empty_like(lens)
+        kept = ab.paged_kv_evict(kp, vp, table, w, lens, keep=200, keep_first=4, keep_last=30, kv_lens_out=now)
+        after = attend(q, kp, vp, table, sm_scale=0.09, num_key_value_groups=hq // hkv, kv_lens=now)
+        return out, lse, w, kept, now, after
+
+    alone = [[t.clone() for t in run(*s)] for s in sets]
+    torch.cuda.synchronize()
+    streams, graphs, results = [torch.cuda.Stream() for _ in sets], [], []
+    for s, stream in zip(sets, streams):
+        with torch.cuda.stream(stream):
+            run(*s)
+            stream.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                results.append(run(*s))
+            graphs.append(graph)
+    for _ in range(20):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for got, want in zip(results, alone):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for _ in range(5):
+        eager = []
+        for s, stream in zip(sets, streams):
+            with torch.cuda.stream(stream):
+                eager.append(run(*s))
+        torch.cuda.synchronize()
+        for got, want in zip(eager, alone):
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert nat.device_error_flags() == 0
