@@ -435,20 +435,32 @@ __device__ __forceinline__ uint4 widened(uint32_t u, uint32_t p) {
   return pack_vec<T>(f);
 }
 
+// n / (page_size / 8) for n < 2^28, as in paged_int4_tiles.cuh.
+struct ByOctets {
+  uint32_t mul;
+  int shift;
+};
+ByOctets by_octets(int page_size) {
+  const int octets = page_size / 8;
+  int shift = 0;
+  while ((1ll << shift) < octets) ++shift;
+  return {(uint32_t)((((1ull << shift) - octets) << 32) / octets + 1), shift};
+}
+
 // The row of slot pos + s, if it is to be read: page (else -1) and row in it.
-__device__ __forceinline__ int2 row_at(const aicas_paged_read_int4_params& a, int b, int pos, int fresh, int s) {
+__device__ __forceinline__ int2 row_at(const aicas_paged_read_int4_params& a, ByOctets by, int b, int pos, int fresh, int s) {
   const long long slot = (long long)pos + s;
   if (s >= fresh || slot < 0 || slot >= a.max_pages * a.page_size) return make_int2(-1, 0);
-  const int i = (int)((uint32_t)slot / (uint32_t)a.page_size);
+  const uint32_t n = (uint32_t)slot >> 3, i = (__umulhi(n, by.mul) + n) >> by.shift;
   const int page = a.page_table[b * a.table_stride + i];
-  return make_int2(page < a.num_pages ? page : -1, (int)slot - i * a.page_size);
+  return make_int2(page < a.num_pages ? page : -1, (int)((uint32_t)slot - i * (uint32_t)a.page_size));
 }
 
 // HBM bound, by what it writes: 16 elements a thread, 8 bytes of codes in and 32 bytes out, of
 // ROWS rows of one request, side and head, so that their page numbers, codes and pairs are on
 // the way at once.
 template <typename T, int D, bool HALVES, int ROWS>
-__global__ void __launch_bounds__(256) paged_read_int4_kernel(const __grid_constant__ aicas_paged_read_int4_params a, int chunks) {
+__global__ void __launch_bounds__(256) paged_read_int4_kernel(const __grid_constant__ aicas_paged_read_int4_params a, ByOctets by, int chunks) {
   constexpr int kTpr = D / 16, kSlots = 256 / kTpr;
   const int b = blockIdx.x / chunks, h = blockIdx.y >> 1, side = blockIdx.y & 1;
   const int c = threadIdx.x % kTpr * 16, s0 = (blockIdx.x - b * chunks) * kSlots * ROWS + threadIdx.x / kTpr;
@@ -461,7 +473,7 @@ __global__ void __launch_bounds__(256) paged_read_int4_kernel(const __grid_const
   const T* pairs = static_cast<const T*>(from.scales) + h * from.ss_h + (HALVES && c >= D / 2 ? 2 : 0);
   int2 at[ROWS];
 #pragma unroll
-  for (int j = 0; j < ROWS; ++j) at[j] = row_at(a, b, pos, fresh, s0 + j * kSlots);
+  for (int j = 0; j < ROWS; ++j) at[j] = row_at(a, by, b, pos, fresh, s0 + j * kSlots);
   uint2 u[ROWS];
   uint32_t p[ROWS];
 #pragma unroll
@@ -487,7 +499,7 @@ __global__ void __launch_bounds__(256) paged_read_int4_kernel(const __grid_const
 constexpr int kFewThreads = 32;
 
 template <typename T, int D, bool HALVES>
-__global__ void __launch_bounds__(kFewThreads) paged_read_few_int4_kernel(const __grid_constant__ aicas_paged_read_int4_params a) {
+__global__ void __launch_bounds__(kFewThreads) paged_read_few_int4_kernel(const __grid_constant__ aicas_paged_read_int4_params a, ByOctets by) {
   constexpr int kTpr = D / 8;
   const int b = blockIdx.x, c = threadIdx.x % kTpr * 8;
   grid_launch_dependents();
@@ -498,7 +510,7 @@ __global__ void __launch_bounds__(kFewThreads) paged_read_few_int4_kernel(const 
   if (r < 2 * a.num_kv_heads * a.seq_len) {
     const int head = a.seq_len == 1 ? r : r / a.seq_len, s = r - head * a.seq_len, h = head >> 1, side = head & 1;
     const aicas_int4_pages& from = a.kv[side];
-    const int2 at = row_at(a, b, pos, fresh, s);
+    const int2 at = row_at(a, by, b, pos, fresh, s);
     uint32_t u = 0, p = 0;
     if (at.x >= 0) {
       u = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(from.codes) + at.x * from.cs_p + h * from.cs_h +
@@ -518,10 +530,10 @@ cudaError_t launch_read_sized(const aicas_paged_read_int4_params& p, cudaStream_
   if ((int64_t)p.num_kv_heads * p.seq_len * (D / 8) <= 2048)
     return launch_pdl(paged_read_few_int4_kernel<T, D, HALVES>,
                       dim3((unsigned)p.batch, (2 * p.num_kv_heads * p.seq_len * (D / 8) + kFewThreads - 1) / kFewThreads), dim3(kFewThreads), 0,
-                      st, p);
+                      st, p, by_octets(p.page_size));
   const int64_t rows = 256 / (D / 16) * 2, chunks = (p.seq_len + rows - 1) / rows;
   const dim3 grid((unsigned)(chunks * p.batch), 2u * p.num_kv_heads);
-  return launch_pdl(paged_read_int4_kernel<T, D, HALVES, 2>, grid, dim3(256), 0, st, p, (int)chunks);
+  return launch_pdl(paged_read_int4_kernel<T, D, HALVES, 2>, grid, dim3(256), 0, st, p, by_octets(p.page_size), (int)chunks);
 }
 
 template <typename T>
