@@ -152,7 +152,7 @@ struct Token {
   int b, s, c;
   uint32_t lanes;
   int page, row;  // page -1: nowhere to write
-  float c1[kV], c2[kV], s1[kV], s2[kV];
+  float c1[kV], c2[kV], s1[kV], s2[kV];  // s1 negated where tables are wider than T
 };
 
 // Where row 0 of token s of request b is, of q (kind 0), k (1) or v (2), and how far the next one.
@@ -209,19 +209,26 @@ __device__ __forceinline__ void token_rows(const aicas_paged_append_int4_params&
             x1[i] = __fmul_rn(__fmul_rn(x1[i], inv), f1[i]);
             x2[i] = __fmul_rn(__fmul_rn(x2[i], inv), f2[i]);
           }
+        } else if constexpr (kRoundEach) {
+          normed_pair<T, true, kV>(x1, x2, f1, f2, inv);
         } else {
-          normed_pair<T, kRoundEach, kV>(x1, x2, f1, f2, inv);
+#pragma unroll
+          for (int i = 0; i < kV; i += 2) {
+            (Two(x1[i], x1[i + 1]) * (Two(inv) * Two(f1[i], f1[i + 1]))).get(x1[i], x1[i + 1]);
+            (Two(x2[i], x2[i + 1]) * (Two(inv) * Two(f2[i], f2[i + 1]))).get(x2[i], x2[i + 1]);
+          }
         }
       }
-      if constexpr (kAsTorch) {
+      if constexpr (kRoundEach) {
+        rotated_pair<T, true, kV>(x1, x2, t.c1, t.c2, t.s1, t.s2);
+      } else {
 #pragma unroll
         for (int i = 0; i < kV; i += 2) {
           const Two p1(x1[i], x1[i + 1]), p2(x2[i], x2[i + 1]);
-          (p1 * Two(t.c1[i], t.c1[i + 1]) + p2 * Two(-t.s1[i], -t.s1[i + 1])).get(x1[i], x1[i + 1]);
-          (p2 * Two(t.c2[i], t.c2[i + 1]) + p1 * Two(t.s2[i], t.s2[i + 1])).get(x2[i], x2[i + 1]);
+          const Two c1(t.c1[i], t.c1[i + 1]), c2(t.c2[i], t.c2[i + 1]), m1(t.s1[i], t.s1[i + 1]), s2(t.s2[i], t.s2[i + 1]);
+          (kAsTorch ? p1 * c1 + p2 * m1 : fma2(p1, c1, p2 * m1)).get(x1[i], x1[i + 1]);
+          (kAsTorch ? p2 * c2 + p1 * s2 : fma2(p2, c2, p1 * s2)).get(x2[i], x2[i + 1]);
         }
-      } else {
-        rotated_pair<T, kRoundEach, kV>(x1, x2, t.c1, t.c2, t.s1, t.s2);
       }
     }
     if constexpr (KIND == 0) {
@@ -268,7 +275,7 @@ __device__ __forceinline__ void token_rows(const aicas_paged_append_int4_params&
 // for no one.  Else a CTA a token, a row a thread, all at once.
 //
 // One token of 16 query and 8 KV heads of 128 and its read back 4.0 us, 64 tokens 4.3: two
-// launches.  8 prompts of 2048 tokens and their read back 74 us, 4.1 TB/s: about 2200
+// launches.  8 prompts of 2048 tokens and their read back 72.5 us, 4.2 TB/s: about 2100
 // instructions a token, whose chains 16 warps an SM (of 128 registers a thread) cover to 62% of
 // the issue slots, while the memory is at 43%.  Without the copies ahead 78 us; rows asked for
 // ahead in registers 92, 20 and 24 warps an SM 79 and 104.
@@ -299,6 +306,9 @@ __device__ __forceinline__ void begin_token(const aicas_paged_append_int4_params
   load_floats<CS, kV>(cp, t.c1);
   load_floats<CS, kV>(cp + D / 2, t.c2);
   load_floats<CS, kV>(sp, t.s1);
+  if constexpr (!std::is_same<T, CS>::value)
+#pragma unroll
+    for (int i = 0; i < kV; ++i) t.s1[i] = -t.s1[i];
   load_floats<CS, kV>(sp + D / 2, t.s2);
 }
 

@@ -156,6 +156,21 @@ def test_append_many_tokens(cuda_device):
     _append_case(cuda_device, "bf16", 128, 128, 16, 8, 3, 200, 16, 14, norm=True, counts=[200, 0, 77])
 
 
+@pytest.mark.parametrize("dtype,dim,group,tables", [("bf16", 128, 128, "fp32"), ("fp16", 128, 64, "fp32"), ("bf16", 64, 64, "fp32"),
+                                                    ("fp16", 128, 128, "own"), ("bf16", 64, 64, "own")])
+@pytest.mark.parametrize("heads", [(6, 2), (20, 1), (7, 7), (34, 17)])
+def test_append_long_prompts(cuda_device, dtype, dim, group, tables, heads):
+    """More tokens than warps, heads that do not fill a unit of rows, requests with fewer and no new tokens."""
+    _append_case(cuda_device, dtype, dim, group, *heads, 5, 523, 16, 34, norm=True, tables=dtype if tables == "own" else "fp32",
+                 counts=[523, 0, 77, 523, 522], one_table=heads[0] == 7, seed=heads[0] + dim)
+
+
+@pytest.mark.parametrize("layout", ["hnd", "nhd", "wide"])
+def test_append_long_prompts_layouts(cuda_device, layout):
+    _append_case(cuda_device, "bf16", 128, 64, 4, 2, 3, 331, 24, 14, layout=layout, positions=[0, 5, 300], seed=9)
+    _append_case(cuda_device, "bf16", 64, 64, 1, 1, 1, 3001, 8, 376, layout=layout, norm=True, seed=10)
+
+
 def test_append_single_tokens_at_page_edges(cuda_device):
     _append_case(cuda_device, "fp16", 64, 64, 16, 8, 6, 1, 16, 4, positions=[0, 15, 16, 31, 62, 63], norm=True)
 
