@@ -47,8 +47,9 @@ __device__ __forceinline__ void group_range(uint32_t lanes, float& lo, float& hi
   }
 }
 
-// Two numbers, two operations an instruction, each rounded as one of its own (8 prompts of 2048
-// tokens written and read back 80 -> 78 us).
+// Two numbers, two operations an instruction (8 prompts of 2048 tokens written and read back 80 ->
+// 78 us).  The assembler may fuse a product that is added to something, .rn or not: where both
+// roundings are wanted it takes the operations of single numbers.
 struct Two {
   uint64_t u;
   Two() = default;
@@ -221,13 +222,20 @@ __device__ __forceinline__ void token_rows(const aicas_paged_append_int4_params&
       }
       if constexpr (kRoundEach) {
         rotated_pair<T, true, kV>(x1, x2, t.c1, t.c2, t.s1, t.s2);
+      } else if constexpr (kAsTorch) {
+#pragma unroll
+        for (int i = 0; i < kV; ++i) {
+          const float p1 = x1[i], p2 = x2[i];
+          x1[i] = __fadd_rn(__fmul_rn(p1, t.c1[i]), __fmul_rn(p2, t.s1[i]));
+          x2[i] = __fadd_rn(__fmul_rn(p2, t.c2[i]), __fmul_rn(p1, t.s2[i]));
+        }
       } else {
 #pragma unroll
         for (int i = 0; i < kV; i += 2) {
           const Two p1(x1[i], x1[i + 1]), p2(x2[i], x2[i + 1]);
           const Two c1(t.c1[i], t.c1[i + 1]), c2(t.c2[i], t.c2[i + 1]), m1(t.s1[i], t.s1[i + 1]), s2(t.s2[i], t.s2[i + 1]);
-          (kAsTorch ? p1 * c1 + p2 * m1 : fma2(p1, c1, p2 * m1)).get(x1[i], x1[i + 1]);
-          (kAsTorch ? p2 * c2 + p1 * s2 : fma2(p2, c2, p1 * s2)).get(x2[i], x2[i + 1]);
+          fma2(p1, c1, p2 * m1).get(x1[i], x1[i + 1]);
+          fma2(p2, c2, p1 * s2).get(x2[i], x2[i + 1]);
         }
       }
     }
@@ -275,7 +283,7 @@ __device__ __forceinline__ void token_rows(const aicas_paged_append_int4_params&
 // for no one.  Else a CTA a token, a row a thread, all at once.
 //
 // One token of 16 query and 8 KV heads of 128 and its read back 4.0 us, 64 tokens 4.3: two
-// launches.  8 prompts of 2048 tokens and their read back 72.5 us, 4.2 TB/s: about 2100
+// launches.  8 prompts of 2048 tokens and their read back 73 us, 4.2 TB/s: about 2100
 // instructions a token, whose chains 16 warps an SM (of 128 registers a thread) cover to 62% of
 // the issue slots, while the memory is at 43%.  Without the copies ahead 78 us; rows asked for
 // ahead in registers 92, 20 and 24 warps an SM 79 and 104.

@@ -165,6 +165,35 @@ def test_append_long_prompts(cuda_device, dtype, dim, group, tables, heads):
                  counts=[523, 0, 77, 523, 522], one_table=heads[0] == 7, seed=heads[0] + dim)
 
 
+@pytest.mark.parametrize("dim,group", [(64, 64), (128, 64), (128, 128)])
+@pytest.mark.parametrize("dtype,norm", [("bf16", True), ("bf16", False), ("fp16", True), ("fp16", False)])
+@pytest.mark.parametrize("batch,seq", [(8, 2048), (500, 1)])
+def test_append_keys_get_the_codes_of_torchs_keys(cuda_device, dim, group, dtype, norm, batch, seq):
+    """Codes and pairs to the bit: those of the keys that torch's operations give on the GPU."""
+    g = torch.Generator(device=cuda_device).manual_seed(dim + seq)
+    dt, hq, hkv, per = DT[dtype], 8, 8, -(-seq // 16)
+    q, k, v = (torch.randn(batch, seq, h, dim, generator=g, device=cuda_device).to(dt).transpose(1, 2) for h in (hq, hkv, hkv))
+    ang = 3 * torch.randn(batch, seq, dim, generator=g, device=cuda_device)
+    cos, sin = ang.cos(), ang.sin()
+    w = (1 + 0.3 * torch.randn(dim, generator=g, device=cuda_device)).to(dt) if norm else None
+    kp, vp = (ab.int4_pages(batch * per, hkv, 16, dim, group, dtype=dt, device=cuda_device) for _ in range(2))
+    table = torch.arange(batch * per, dtype=torch.int32, device=cuda_device).view(batch, per)
+    ab.paged_rope_kv_append_int4(q, k, v, cos, sin, kp, vp, table, torch.zeros(batch, dtype=torch.int32, device=cuda_device),
+                                 q_norm_weight=w, k_norm_weight=w)
+    x = k.float()
+    if norm:
+        x = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + 1e-6) * w.float()
+    x = x * cos[:, None] + torch.cat([-x[..., dim // 2:], x[..., : dim // 2]], -1) * sin[:, None]
+    for pool, rows in ((kp, x), (vp, v.float())):
+        y = rows.unflatten(-1, (-1, group))
+        least = y.amin(-1).to(dt)
+        scale = ((y.amax(-1) - least.float()) / 15).to(dt)
+        code = ((y - least.float()[..., None]) / scale.float()[..., None]).round().clamp(0, 15).to(torch.uint8).flatten(-2)
+        for part, want in zip(pool, (code[..., 0::2] | (code[..., 1::2] << 4), torch.stack([scale, least], -1))):
+            got = part.view(batch, per, *part.shape[1:]).transpose(1, 2).flatten(2, 3)[:, :, :seq]
+            assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("layout", ["hnd", "nhd", "wide"])
 def test_append_long_prompts_layouts(cuda_device, layout):
     _append_case(cuda_device, "bf16", 128, 64, 4, 2, 3, 331, 24, 14, layout=layout, positions=[0, 5, 300], seed=9)
