@@ -279,45 +279,44 @@ __device__ __forceinline__ void token_rows(const aicas_paged_append_int4_params&
 // 16-byte vector of the row's first half and the matching one of its second half, so that the
 // rotation needs no exchange, and with groups of 64 in rows of 128 each half is a group.
 // PROMPT: a warp walks through tokens, a unit of two rows a lane at a time; the units are
-// copied into shared memory kUnits ahead, each lane's vectors by itself, so that the lanes wait
-// for no one.  Else a CTA a token, a row a thread, all at once.
+// copied into shared memory kUnits ahead, and the next token's tables, each lane's vectors by
+// itself, so that the lanes wait for no one.  Else a CTA a token, a row a thread, all at once.
 //
 // One token of 16 query and 8 KV heads of 128 and its read back 4.0 us, 64 tokens 4.3: two
-// launches.  8 prompts of 2048 tokens and their read back 73 us, 4.2 TB/s: about 2100
+// launches.  8 prompts of 2048 tokens and their read back 72 us, 4.2 TB/s: about 2100
 // instructions a token, whose chains 16 warps an SM (of 128 registers a thread) cover to 62% of
 // the issue slots, while the memory is at 43%.  Without the copies ahead 78 us; rows asked for
 // ahead in registers 92, 20 and 24 warps an SM 79 and 104.
 constexpr int kPromptWarps = 4, kPromptCtas = 4;  // of a CTA, of an SM
 constexpr int kUnits = 2;  // 8 prompts of 2048 tokens with 2 74.0 us, 4 74.8, 6 76.8
 
-// The lane's part of token `token`, but for what of it is its own.
-template <typename T, typename CS, int D>
-__device__ __forceinline__ void begin_token(const aicas_paged_append_int4_params& a, Token<CS, D>& t, int token, bool first_lane) {
-  constexpr int kV = Token<CS, D>::kV;
-  t.b = token / a.seq_len, t.s = token - t.b * a.seq_len;
-  // the token's slot; asked for first, needed last
-  const int pos = a.positions[t.b];
-  const int fresh = a.num_new != nullptr ? min(max(a.num_new[t.b], 0), a.seq_len) : a.seq_len;
+// A token's page (-1: nowhere to write) and row in it; its request's length, where one is asked for.
+__device__ __forceinline__ int2 place_of(const aicas_paged_append_int4_params& a, int b, int s, bool first_lane) {
+  const int pos = a.positions[b];
+  const int fresh = a.num_new != nullptr ? min(max(a.num_new[b], 0), a.seq_len) : a.seq_len;
   const int cap = a.max_pages * a.page_size;
-  const long long slot = (long long)pos + t.s;
-  t.page = -1, t.row = 0;
-  if (t.s < fresh && slot >= 0 && slot < cap) {
+  const long long slot = (long long)pos + s;
+  int2 at = make_int2(-1, 0);
+  if (s < fresh && slot >= 0 && slot < cap) {
     const int i = (int)((uint32_t)slot / (uint32_t)a.page_size);
-    t.row = (int)slot - i * a.page_size;
-    t.page = a.page_table[t.b * a.table_stride + i];
-    if (t.page >= a.num_pages) t.page = -1;
+    at = make_int2(a.page_table[b * a.table_stride + i], (int)slot - i * a.page_size);
+    if (at.x >= a.num_pages) at.x = -1;
   }
-  if (a.kv_lens_out != nullptr && t.s == 0 && first_lane)
-    a.kv_lens_out[t.b] = (int)min((long long)max(pos, 0) + fresh, (long long)cap);
-  const CS* cp = static_cast<const CS*>(a.cos) + t.b * a.cs_stride_b + t.s * a.cs_stride_s + t.c;
-  const CS* sp = static_cast<const CS*>(a.sin) + t.b * a.cs_stride_b + t.s * a.cs_stride_s + t.c;
-  load_floats<CS, kV>(cp, t.c1);
-  load_floats<CS, kV>(cp + D / 2, t.c2);
-  load_floats<CS, kV>(sp, t.s1);
+  if (a.kv_lens_out != nullptr && s == 0 && first_lane) a.kv_lens_out[b] = (int)min((long long)max(pos, 0) + fresh, (long long)cap);
+  return at;
+}
+
+// cos and sin of a token's dims c .. c + 7 and D / 2 + c .. as the rotation takes them, from the four places.
+template <typename T, typename CS, int D>
+__device__ __forceinline__ void take_tables(Token<CS, D>& t, const CS* c1, const CS* c2, const CS* s1, const CS* s2) {
+  constexpr int kV = Token<CS, D>::kV;
+  load_floats<CS, kV>(c1, t.c1);
+  load_floats<CS, kV>(c2, t.c2);
+  load_floats<CS, kV>(s1, t.s1);
+  load_floats<CS, kV>(s2, t.s2);
   if constexpr (!std::is_same<T, CS>::value)
 #pragma unroll
     for (int i = 0; i < kV; ++i) t.s1[i] = -t.s1[i];
-  load_floats<CS, kV>(sp + D / 2, t.s2);
 }
 
 template <typename T, typename CS, int D, bool HALVES>
@@ -330,7 +329,12 @@ __global__ void __launch_bounds__(256, 1) paged_append_int4_kernel(const __grid_
   const int hq = a.num_q_heads, hkv = a.num_kv_heads;
   grid_launch_dependents();
   grid_dependency_wait();
-  begin_token<T>(a, t, blockIdx.x, threadIdx.x == 0);
+  t.b = (int)blockIdx.x / a.seq_len, t.s = (int)blockIdx.x - t.b * a.seq_len;
+  const int2 place = place_of(a, t.b, t.s, threadIdx.x == 0);  // asked for first, needed last
+  t.page = place.x, t.row = place.y;
+  const CS* cp = static_cast<const CS*>(a.cos) + t.b * a.cs_stride_b + t.s * a.cs_stride_s + t.c;
+  const CS* sp = static_cast<const CS*>(a.sin) + t.b * a.cs_stride_b + t.s * a.cs_stride_s + t.c;
+  take_tables<T>(t, cp, cp + D / 2, sp, sp + D / 2);
   const auto row = [&](auto kind, int h, int heads) {
     constexpr int kKind = decltype(kind)::value;
     int64_t step;
@@ -355,6 +359,8 @@ __global__ void __launch_bounds__(32 * kPromptWarps, kPromptCtas)
   using K = Token<CS, D>;
   constexpr int kTpr = K::kTpr, kSlots = 32 / kTpr, kRows = 2 * kSlots;  // rows of a unit
   __shared__ uint4 ring[kPromptWarps][kUnits][4][32];  // [first and second half of row 0, of row 1]
+  constexpr int kTabVecs = K::kV * (int)sizeof(CS) / 16;
+  __shared__ uint4 tables[kPromptWarps][32][4 * kTabVecs + 1];  // a lane's cos and sin; 1: to turn the banks
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, r0 = lane / kTpr;
   const int tokens = a.batch * a.seq_len, warps = (int)gridDim.x * kPromptWarps;
   const int hq = a.num_q_heads, hkv = a.num_kv_heads, nq = (hq + kRows - 1) / kRows, nk = (hkv + kRows - 1) / kRows;
@@ -385,8 +391,21 @@ __global__ void __launch_bounds__(32 * kPromptWarps, kPromptCtas)
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  uint4* const mine = tables[warp][lane];
+  const auto copy_tables = [&](int b, int s) {
+    const CS* from[2] = {static_cast<const CS*>(a.cos) + b * a.cs_stride_b + s * a.cs_stride_s + t.c,
+                         static_cast<const CS*>(a.sin) + b * a.cs_stride_b + s * a.cs_stride_s + t.c};
+#pragma unroll
+    for (int e = 0; e < 4 * kTabVecs; ++e)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(smem_u32(mine + e)),
+                   "l"(from[e / (2 * kTabVecs)] + e / kTabVecs % 2 * (D / 2) + e % kTabVecs * (16 / (int)sizeof(CS))) : "memory");
+  };
+  if (first >= tokens) return;
+  t.b = first / a.seq_len, t.s = first - t.b * a.seq_len;
+  copy_tables(t.b, t.s);  // in the first unit's group
 #pragma unroll
   for (int k = 0; k < kUnits; ++k) copy(ring[warp][k]);
+  int2 place = place_of(a, t.b, t.s, lane == 0);
   int at = 0;
   const auto rows = [&](auto kind, int n, int heads) {
     constexpr int kKind = decltype(kind)::value;
@@ -401,16 +420,28 @@ __global__ void __launch_bounds__(32 * kPromptWarps, kPromptCtas)
     }
   };
 #pragma unroll 1
-  for (int64_t token = first; token < tokens; token += warps) {
-    begin_token<T>(a, t, (int)token, lane == 0);
+  for (int64_t token = first; token < tokens;) {
+    // the tables' group is not the last one
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    const CS* tab = reinterpret_cast<const CS*>(mine);
+    constexpr int kEach = K::kV;
+    take_tables<T>(t, tab, tab + kEach, tab + 2 * kEach, tab + 3 * kEach);
+    t.page = place.x, t.row = place.y;
     rows(std::integral_constant<int, 0>(), nq, hq);
+    token += warps;
+    const int nb = token < tokens ? (int)token / a.seq_len : t.b, ns = token < tokens ? (int)token - nb * a.seq_len : t.s;
+    if (token < tokens) {
+      copy_tables(nb, ns);  // q's rows are done, so these are read; they go into the next unit's group
+      place = place_of(a, nb, ns, lane == 0);
+    }
     rows(std::integral_constant<int, 1>(), nk, hkv);
     rows(std::integral_constant<int, 2>(), nk, hkv);
+    t.b = nb, t.s = ns;
   }
 }
 
 // Tokens up to which each gets a CTA: the append and read of 16 x 16 tokens of 8 KV heads
-// 5.3 us, a warp each 7.3; of 512 8.4, 11.1; of 1024 13.2 both; of 2 x 2048 45.8, 24.7.
+// 5.3 us, a warp each 7.3; of 512 8.4, 11.1; of 1024 13.2, 12.7; of 2 x 2048 45.8, 24.3.
 constexpr int kPromptTokens = 600;
 
 template <typename T, typename CS, int D, bool HALVES>
