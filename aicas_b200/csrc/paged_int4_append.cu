@@ -283,9 +283,9 @@ __device__ __forceinline__ void token_rows(const aicas_paged_append_int4_params&
 // itself, so that the lanes wait for no one.  Else a CTA a token, a row a thread, all at once.
 //
 // One token of 16 query and 8 KV heads of 128 and its read back 4.0 us, 64 tokens 4.3: two
-// launches.  8 prompts of 2048 tokens and their read back 72 us, 4.2 TB/s: about 2100
-// instructions a token, whose chains 16 warps an SM (of 128 registers a thread) cover to 62% of
-// the issue slots, while the memory is at 43%.  Without the copies ahead 78 us; rows asked for
+// launches.  8 prompts of 2048 tokens and their read back 72 us, 4.2 TB/s: about 2200
+// instructions a token, whose chains 16 warps an SM (of 128 registers a thread) cover to 63% of
+// the issue slots, while the memory is at 44%.  Without the copies ahead 78 us; rows asked for
 // ahead in registers 92, 20 and 24 warps an SM 79 and 104.
 constexpr int kPromptWarps = 4, kPromptCtas = 4;  // of a CTA, of an SM
 constexpr int kUnits = 2;  // 8 prompts of 2048 tokens with 2 74.0 us, 4 74.8, 6 76.8
