@@ -535,10 +535,8 @@ __global__ void __launch_bounds__(Int4Cfg<D, GD>::kThreads, 1) paged_decode_int4
         last = __shfl_sync(0xffffffffu, last, 0);
         if (team > 1 && lane_id == 0) s_last[warp] = last;
       }
-      if (team > 1) {
-        team_sync();
-        last = s_last[warp - rank];
-      }
+      team_sync();  // lane 0's acquire holds for the team behind a barrier (a shuffle orders no memory)
+      if (team > 1) last = s_last[warp - rank];
       if (last) {
         const int first_slot = small || c0 * chunk >= pair0 ? 0 : 1;  // of team c0; the others hold it as their first
         for (int x = lane_id; x < heads * (D / 4); x += threads) {
