@@ -56,7 +56,7 @@ def _check_weights(what: str, name: str, weights, B: int, Hkv: int, slots: int, 
                          "page table")
     s = steps(weights)
     C = weights.shape[2]
-    if s[2] not in (0, 1) or (Hkv > 1 and s[1] < C) or (B > 1 and s[0] < C) \
+    if (C > 1 and s[2] != 1) or (Hkv > 1 and s[1] < C) or (B > 1 and s[0] < C) \
             or (Hkv > 1 and B > 1 and s[0] < s[1] * Hkv and s[1] < s[0] * B):
         raise ValueError(f"{what}: {name} must have contiguous slots and rows apart from one another")
     return s[0], s[1]
