@@ -232,7 +232,8 @@ struct Int4State {
       // scores are less the old reference; the first tile sets it, down too
       const float up = mt == -INFINITY ? 0.f : first ? mt : fmaxf(mt, 0.f);
       ref[n] += up;
-      const float alpha = exp2_fast(-up);
+      // nothing is added up before the first tile, and 2^-up overflows where its scores are far below 0
+      const float alpha = first ? 1.f : exp2_fast(-up);
       l[n] *= alpha;
 #pragma unroll
       for (int e = 0; e < GD; ++e) z[n][e] *= alpha;
