@@ -3,7 +3,7 @@
 //   y = x * rsqrt(mean x^2 + eps) * w        (with a norm weight, else y = x)
 //   r = y * cos + rotate_half(y) * sin,      rotate_half(y) = cat(-y[D/2:], y[:D/2])
 //   of each group of 64 (or D) elements of r (keys) and v:
-//     least = T(min r),  scale = T((max r - least) / 15)
+//     least = T(min r),  scale = T((max r - least) * (1 / 15)), an fp32 product with fp32's 1 / 15
 //     code  = (r - least) / scale to the nearest of 0..15   (0 where scale is no normal fp32 number)
 //   read back as fma(scale, code, least), rounded to T.
 //

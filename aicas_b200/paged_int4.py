@@ -74,7 +74,7 @@ def quantize_kv_int4(rows: torch.Tensor, group_size: int | None = None) -> Int4P
         raise ValueError(f"quantize_kv_int4 needs fp16 or bf16 rows (got {rows.dtype})")
     x = rows.detach().float().unflatten(-1, (d // group_size, group_size))
     lo = x.amin(-1).to(rows.dtype)
-    scale = ((x.amax(-1) - lo.float()) / 15).to(rows.dtype)
+    scale = ((x.amax(-1) - lo.float()) * (1 / 15)).to(rows.dtype)  # on a GPU torch's "/ 15" is this product too
     bad = ~(scale.float().abs() < torch.inf)
     scale, lo = scale.masked_fill(bad, torch.nan), lo.masked_fill(bad, torch.nan)
     step, least = scale.float()[..., None], lo.float()[..., None]
@@ -163,8 +163,8 @@ def paged_rope_kv_append_int4(
     arguments, rotation, rounding, drops and lengths, but for the pages, whose scales
     are of the query's dtype (fp16 or bf16).
 
-    A group's least value, and a fifteenth of its range above it, are rounded to that
-    dtype; each element becomes the nearest of the 16 levels.  A group that is all one
+    A group's least value, and its range above that times 1/15 (an fp32 product), are
+    rounded to that dtype; each element becomes the nearest of the 16 levels.  A group that is all one
     value gets that value, one with an element that is not finite reads back as NaN."""
     done = fast("append_int4", query, key, value, cos, sin, k_pages, v_pages, page_table, positions, num_new, q_out,
                 kv_lens_out, q_norm_weight, k_norm_weight, eps)

@@ -521,8 +521,8 @@ typedef struct aicas_paged_append_int4_params {
 } aicas_paged_append_int4_params;
 
 /* aicas_paged_rope_append with rounded rows: of a group's values (keys after norm and
-   rotation) least = their least and scale = (their largest - least) / 15, each rounded to
-   dtype, code = (value - least) / scale to the nearest of 0..15 (0 where scale is below
+   rotation) least = their least and scale = (their largest - least) * (1 / 15), a product in
+   fp32 with fp32's 1 / 15, each rounded to dtype, code = (value - least) / scale to the nearest of 0..15 (0 where scale is below
    2^-126, fp32's least normal number).  A group with a value that is not finite, or a range past fp32's, has scale and least NaN. */
 AICAS_API int aicas_paged_append_int4(const aicas_paged_append_int4_params* p, void* stream);
 

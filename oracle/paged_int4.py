@@ -25,10 +25,12 @@ def pack(q: np.ndarray) -> np.ndarray:
 
 def levels(x: np.ndarray, group: int, dtype: str):
     """(scale, least, code before it is rounded) of rows [..., D]: pairs [..., D / g],
-    rounded to ``dtype``; codes [..., D] in float64."""
+    rounded to ``dtype``, the scale after an fp32 difference and an fp32 product with 1 / 15;
+    codes [..., D] in float64."""
     y = x.astype(np.float64).reshape(*x.shape[:-1], -1, group)
     least = round_to(y.min(-1), dtype)
-    scale = round_to((y.max(-1) - least) / 15, dtype)
+    with np.errstate(over="ignore", invalid="ignore"):
+        scale = round_to((y.max(-1).astype(np.float32) - least.astype(np.float32)) * np.float32(1 / 15), dtype)
     bad = ~np.isfinite(scale)
     scale[bad] = least[bad] = np.nan
     s, lo = scale[..., None].astype(np.float64), least[..., None].astype(np.float64)
