@@ -1,5 +1,5 @@
 """Codes and pairs of the 4-bit append, to the bit: groups whose scale lies at a border, and
-keys with tables of the tensors' own type.
+keys with tables of the tensors' own type."""
 from __future__ import annotations
 
 import numpy as np
