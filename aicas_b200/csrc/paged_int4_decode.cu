@@ -25,7 +25,12 @@
 //     to 2^-29 of its largest element).  A probability times its scale enters P V as two
 //     fp16 parts, 22 bits, or to within 2^-25 of numbers that a power of two brings to 2^7 and
 //     more for the largest scale of V so far: 2^-32 of that scale, whatever its slot's
-//     probability.  Everything else is fp32.
+//     probability.  Everything else is fp32, but a product's sum is cut off, not rounded, and
+//     codes are all positive, so that a long chain of products into o drifts: with values around 0,
+//     whose sums of scale times code and of least cancel, by 2.6e-4 of the result over 131072
+//     slots a request in a batch of 4, growing with the tiles a warp has.  So o is emptied into a
+//     rounded sum in shared memory every kHoldTiles tiles: in fp16 2.2e-4 off the 64-bit result (its
+//     own rounding is 2.06e-4), without 3.4e-4.
 //   * Slots out of range: score -inf, V's scale and least 0.
 //   * Bound: HBM, from a few thousand tiles on.  16 query and 8 KV heads of 128 in bf16: 4
 //     caches of 131072 slots, groups of 128, 105 us, 5.75 TB/s; 64 of up to 4096 37 us, 4.15
@@ -59,6 +64,9 @@ constexpr int kLogWarps = 4, kMaxWarps = 1 << kLogWarps;
 // Warps of a team in a small launch, as a power of two: one cache of 1024 slots with 2 8.1 us, 4 7.1, 16 8.4.
 constexpr int kSmallLog = 2;
 constexpr int kHeads = 8;      // query heads of a block
+// Tiles of a warp whose products are added up in the tensor cores alone: 4 caches of 131072 slots
+// 109.6 us with 8, 109.1 with 16, 105.3 without an end (64 of up to 4096 37.8, 37.6, 36.9).
+constexpr int kHoldTiles = 8;
 constexpr size_t kWsCounters = (size_t)1 << 20;  // counter region shared with the other decode kernels
 struct Int4Args {
   Int4Source src;
@@ -86,6 +94,7 @@ struct Int4Cfg : Int4Stage<D, GD, 2> {
   static constexpr int kOffVars = kOffRed + kWarps * kHeads * kRedRow * 4;
   static constexpr int kSmem = kOffVars + 4 * kWarps;
   static_assert(kSmem <= 232448, "shared memory");
+  static_assert(32 * D <= kHeads * kRedRow * 4, "a warp's sums");
 };
 
 using Seg = Segment<kTile>;
@@ -128,11 +137,18 @@ struct Int4State {
   float l[kN], z[kN][GD];  // the lane's shares of sum p, sum p least
   float lift;              // power of two on scales of V
   float bound;             // the largest scale of V that lift is good for; -1: no tile yet
+  bool holds;              // the warp's part of the reduction buffer has what was added up before o was last emptied
 
   // p stays below 2^kSlack: the reference is moved when a score passes it by more.
   static constexpr float kSlack = 4.f;
 
   uint32_t k_off, v_off, p_off;  // this lane's places in a stage: rows of the fragment loads, pairs
+
+  // The lane's place in the warp's part of the reduction buffer, which is free until put.
+  __device__ __forceinline__ static float4* place() {
+    extern __shared__ __align__(128) uint8_t smem[];
+    return reinterpret_cast<float4*>(smem + C::kOffRed + (threadIdx.x >> 5) * (kHeads * C::kRedRow * 4)) + (threadIdx.x & 31);
+  }
 
   __device__ __forceinline__ void init() {
     const int lane = threadIdx.x & 31, mat = lane >> 3, r = lane & 7;
@@ -197,7 +213,7 @@ struct Int4State {
 #pragma unroll
       for (int e = 0; e < GD; ++e) z[n][e] = 0.f;
     }
-    lift = 0.f, bound = -1.f;
+    lift = 0.f, bound = -1.f, holds = false;
 #pragma unroll
     for (int n = 0; n < D / 16; ++n)
 #pragma unroll
@@ -247,6 +263,28 @@ struct Int4State {
 #pragma unroll
     for (int n = 0; n < D / 16; ++n)
       o[n][0] *= f[0], o[n][1] *= f[kN - 1], o[n][2] *= f[0], o[n][3] *= f[kN - 1];
+    if (holds) {
+      float4* const held = place();
+#pragma unroll 1
+      for (int n = 0; n < D / 16; ++n) {
+        const float4 x = held[32 * n];
+        held[32 * n] = make_float4(x.x * f[0], x.y * f[kN - 1], x.z * f[0], x.w * f[kN - 1]);
+      }
+    }
+  }
+
+  // Adds o to what is held, rounding the sum, and empties it.
+  __device__ __forceinline__ void hold() {
+    float4* const held = place();
+#pragma unroll
+    for (int n = 0; n < D / 16; ++n) {
+      float4 x = holds ? held[32 * n] : make_float4(0.f, 0.f, 0.f, 0.f);
+      x.x += o[n][0], x.y += o[n][1], x.z += o[n][2], x.w += o[n][3];
+      held[32 * n] = x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+    }
+    holds = true;
   }
 
   // One tile at shared-memory address `at`; lo..hi: its slots in range.
@@ -372,6 +410,15 @@ struct Int4State {
   __device__ __forceinline__ void put(int heads, float* red) {
     const int lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3;
     const float unit = lift == 0.f ? 0.f : kCodeUnit / lift;
+    if (holds) {
+      float4* const held = place();
+#pragma unroll
+      for (int n = 0; n < D / 16; ++n) {
+        const float4 x = held[32 * n];
+        o[n][0] += x.x, o[n][1] += x.y, o[n][2] += x.z, o[n][3] += x.w;
+      }
+      __syncwarp();  // every lane has read its share of the buffer
+    }
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
       const int h = WIDE ? 2 * i + n : i;
@@ -478,6 +525,7 @@ __global__ void __launch_bounds__(Int4Cfg<D, GD>::kThreads, 1) paged_decode_int4
       const uint32_t at = ring + stage * C::kStage;
       const int slot = (seg.first_tile + t) * kTile;
       st.tile(at, seg.start - slot, seg.len - slot);
+      if ((~t & (kHoldTiles - 1) * team) == 0) st.hold();
       __syncwarp();  // every lane has read the stage
       ahead.copy(a, at, rank, team);
       if (++stage == C::kStages) stage = 0;

@@ -37,3 +37,35 @@ def test_joins_repeat_to_the_bit(cuda_device, batch, hkv, hi):
     first = run()
     again = [run() for _ in range(200)]
     assert all(torch.equal(a, b) for other in again for a, b in zip(first, other))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim,group,groups", [(128, 128, 2), (128, 64, 2), (64, 64, 2), (128, 128, 8), (128, 64, 8)])
+def test_long_sums_do_not_drift(cuda_device, dtype, dim, group, groups):
+    """A large batch over long caches of values around 0: a warp adds up hundreds of tiles, and
+    what scales times codes come to cancels with the least values.
+
+    Tolerance: products are added up in chains of 16 steps, each of which may cut off 2^-23 of the
+    largest number in it, at most what all codes at 15 come to: 16 x 2^-23 x 15 scale, 1.3e-5 for the
+    values here; the mean over all outputs within that, each output within twice that (the
+    chains' sums are rounded, 2^-24 each) and half a unit of its own rounding."""
+    g = torch.Generator(device=cuda_device).manual_seed(dim + group + groups)
+    B, hkv, n, size, dt = 128, 4, 65536, 64, DT[dtype]
+    hq = hkv * groups
+    rows = [torch.randn(n // size, hkv, size, dim, generator=g, device=cuda_device).to(dt) for _ in range(2)]
+    kp, vp = (ab.quantize_kv_int4(r, group) for r in rows)
+    table = torch.randperm(n // size, generator=g, device=cuda_device).int().expand(B, -1)  # all requests read the same pages
+    q = torch.randn(B, hq, 1, dim, generator=g, device=cuda_device).to(dt)
+    out = ab.paged_gqa_decode_attention_int4(q, kp, vp, table, sm_scale=dim ** -0.5, num_key_value_groups=groups)
+    total, count = 0.0, 0
+    bound = 16 * 2.0 ** -23 * 15 * float(vp.scales[..., 0].float().max())
+    half = torch.finfo(dt).eps / 2
+    for h in range(hkv):
+        k, v = (p.dequantize()[:, h].flatten(0, 1).double() for p in (kp, vp))
+        for b in range(0, B, 32):
+            mine = q[b:b + 32, h * groups:(h + 1) * groups, 0].double()
+            ref = torch.softmax(mine @ k.t() * dim ** -0.5, -1) @ v
+            off = out[b:b + 32, h * groups:(h + 1) * groups, 0].double() - ref
+            assert (off.abs() <= half * ref.abs() + 2 * bound).all()
+            total, count = total + float(off.sum()), count + off.numel()
+    assert abs(total / count) <= bound
