@@ -409,7 +409,7 @@ struct Int4State {
   // The block's heads into this warp's part of the reduction buffer.
   __device__ __forceinline__ void put(int heads, float* red) {
     const int lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3;
-    const float unit = lift == 0.f ? 0.f : kCodeUnit / lift;
+    const float drop = lift == 0.f ? 0.f : 1.f / lift;  // times kCodeUnit it would overflow for scales of 2^111
     if (holds) {
       float4* const held = place();
 #pragma unroll
@@ -441,7 +441,7 @@ struct Int4State {
 #pragma unroll
           for (int t = 0; t < 4; ++t) {
             const float* c = o[4 * cp + t] + 2 * half;
-            x[t] = fmaf(WIDE ? c[n] : c[0] + c[1], t & 1 ? unit * 0.0625f : unit, least[GD == 2 ? cp : 0]);
+            x[t] = fmaf((WIDE ? c[n] : c[0] + c[1]) * (t & 1 ? kCodeUnit / 16.f : kCodeUnit), drop, least[GD == 2 ? cp : 0]);
           }
           *reinterpret_cast<float4*>(row + 64 * cp + 32 * half + 4 * g) = make_float4(x[0], x[1], x[2], x[3]);
         }

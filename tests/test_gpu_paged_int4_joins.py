@@ -69,3 +69,25 @@ def test_long_sums_do_not_drift(cuda_device, dtype, dim, group, groups):
             assert (off.abs() <= half * ref.abs() + 2 * bound).all()
             total, count = total + float(off.sum()), count + off.numel()
     assert abs(total / count) <= bound
+
+
+@pytest.mark.parametrize("to", [1e-35, 1e-20, 1e20, 1e34, 4e36])
+@pytest.mark.parametrize("group", [64, 128])
+@pytest.mark.parametrize("groups", [2, 8])
+def test_values_over_the_range_of_bf16(cuda_device, to, group, groups):
+    """Values of any size that their sums leave room for, against the same in 64 bits."""
+    g = torch.Generator().manual_seed(groups)
+    B, hkv, per, dim = 3, 2, 8, 128
+    rows = [torch.randn(B * per, hkv, 16, dim, generator=g).to(DT["bf16"]) for _ in range(2)]
+    rows[1] = (rows[1].double() * to).to(DT["bf16"])
+    kp, vp = (ab.Int4Pages(*(t.to(cuda_device) for t in ab.quantize_kv_int4(r, group))) for r in rows)
+    table = torch.randperm(B * per, generator=g).view(B, per).int().to(cuda_device)
+    q = torch.randn(B, hkv * groups, 1, dim, generator=g).to(DT["bf16"]).to(cuda_device)
+    lens = [1, 33, 128]
+    out = ab.paged_gqa_decode_attention_int4(q, kp, vp, table, sm_scale=dim ** -0.5, num_key_value_groups=groups, kv_lens=lens)
+    for b, n in enumerate(lens):
+        k, v = (p.dequantize()[table[b].long()].transpose(0, 1).flatten(1, 2)[:, :n].double() for p in (kp, vp))
+        mine = q[b, :, 0].double().view(hkv, groups, dim)
+        ref = (torch.softmax(mine @ k.transpose(1, 2) * dim ** -0.5, -1) @ v).view(-1, dim)
+        # 2e-4 of values around 1, as at the top; below fp32's normal numbers sums keep fewer bits (a scale is 0.3 to)
+        assert ((out[b, :, 0].double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 2e-4 * to + 2.0 ** -133).all()
