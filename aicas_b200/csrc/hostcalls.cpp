@@ -542,7 +542,8 @@ PyObject* evict(PyObject*, PyObject* const* args, Py_ssize_t count) {
       !table_ok(table, table.size(0), table.get_device()))
     return none();
   const int64_t B = table.size(0), index = table.get_device();
-  if (keep < 1 || keep > INT32_MAX || first < 0 || last < 0 || first + last > keep || longer < keep || longer > INT32_MAX) return none();
+  if (keep < 1 || keep > INT32_MAX || first < 0 || last < 0 || first > keep || last > keep - first || longer < keep || longer > INT32_MAX)
+    return none();
   aicas_paged_evict_params p;
   memset(&p, 0, sizeof(p));
   Pool4 shapes[2];

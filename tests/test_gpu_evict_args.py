@@ -1,0 +1,38 @@
+"""Arguments of the eviction's operators at their edges: refused, or taken as they are meant, on the compiled way
+and in Python."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import aicas_b200 as ab
+from aicas_b200 import _hostpath as hp
+from aicas_b200 import eviction
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(params=["compiled", "python"])
+def way(request, monkeypatch):
+    hp.library()
+    if request.param == "python":
+        monkeypatch.setattr(eviction, "fast", lambda *args: None)
+
+
+def _state(device, B=2, hkv=2, per=4):
+    g = torch.Generator().manual_seed(0)
+    kp, vp = (torch.randn(B * per, hkv, 16, 64, generator=g).to(torch.bfloat16).to(device) for _ in range(2))
+    table = torch.arange(B * per, dtype=torch.int32, device=device).view(B, per)
+    w = torch.rand(B, hkv, per * 16, generator=g).to(device)
+    lens = torch.full((B,), per * 16, dtype=torch.int32, device=device)
+    return kp, vp, table, w, lens
+
+
+@pytest.mark.parametrize("first,last", [(2 ** 62, 2 ** 62), (2 ** 63 - 1, 2 ** 63 - 1), (2 ** 63 - 1, 1), (2 ** 62, 0), (0, 2 ** 63 - 1),
+                                        (2 ** 32, 0), (2 ** 70, 0)])
+def test_counts_whose_sum_overflows_are_refused(cuda_device, way, first, last):
+    kp, vp, table, w, lens = _state(cuda_device)
+    before = [t.clone() for t in (kp, vp, w)]
+    with pytest.raises(ValueError, match="keep"):
+        ab.paged_kv_evict(kp, vp, table, w, lens, keep=20, keep_first=first, keep_last=last)
+    assert all(torch.equal(a, b) for a, b in zip((kp, vp, w), before))
