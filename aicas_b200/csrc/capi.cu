@@ -664,6 +664,12 @@ int check_paged_evict(const aicas_paged_evict_params* p) {
   for (int64_t s : st)
     if (s < 0) return fail(AICAS_ERR_INVALID, "strides of the weights must not be negative");
   if ((int64_t)p->batch * p->num_kv_heads > (1 << 24)) return fail(AICAS_ERR_UNSUPPORTED, "batch=%d of %d heads", p->batch, p->num_kv_heads);
+  const auto extent = [&](int64_t sb, int64_t sh) {
+    return (p->batch - 1) * sb + (p->num_kv_heads - 1) * sh + (int64_t)p->max_pages * p->page_size;
+  };
+  if ((p->weights_out != p->weights || p->wo_stride_b != p->w_stride_b || p->wo_stride_h != p->w_stride_h) &&
+      p->weights < p->weights_out + extent(p->wo_stride_b, p->wo_stride_h) && p->weights_out < p->weights + extent(p->w_stride_b, p->w_stride_h))
+    return fail(AICAS_ERR_INVALID, "weights_out must be weights or memory apart from it");
   if (lengths_overlap(p->kv_lens_out, p->batch, p->page_table, (p->batch - 1) * p->table_stride + p->max_pages) ||
       (p->kv_lens_out != p->kv_lens && lengths_overlap(p->kv_lens_out, p->batch, p->kv_lens, p->batch)))
     return fail(AICAS_ERR_INVALID, "kv_lens_out must be kv_lens or share no memory with it, nor with page_table");

@@ -197,9 +197,10 @@ def paged_kv_evict(
     if weights_out is None:
         weights_out = weights
     ob, oh = _check_weights(what, "weights_out", weights_out, B, Hkv, slots, index)
-    if weights_out is not weights and weights_out.untyped_storage().data_ptr() == weights.untyped_storage().data_ptr() \
-            and (weights_out.data_ptr(), ob, oh) != (weights.data_ptr(), wb, wh):
-        raise ValueError(f"{what}: weights_out must be weights or memory of its own")
+    at, to = ((t.data_ptr(), t.data_ptr() + 4 * (max(B - 1, 0) * sb + max(Hkv - 1, 0) * sh + slots))
+              for t, sb, sh in ((weights, wb, wh), (weights_out, ob, oh)))
+    if (at[0], wb, wh) != (to[0], ob, oh) and at[0] < to[1] and to[0] < at[1]:
+        raise ValueError(f"{what}: weights_out must be weights or memory apart from it")
     lens = lengths(kv_lens, B, device)
     if lens is None:
         raise ValueError(f"{what}: kv_lens are required")

@@ -605,7 +605,7 @@ typedef struct aicas_evict_plane {
 typedef struct aicas_paged_evict_params {
   aicas_evict_plane plane[AICAS_EVICT_MAX_PLANES]; /* what a slot has: keys, values, their scales */
   const float* weights;     /* [B, Hkv, C], C >= max_pages * page_size */
-  float* weights_out;       /* the same shape; may be weights */
+  float* weights_out;       /* the same shape; weights, with its strides, or memory apart from it */
   int32_t* kept;            /* [B, Hkv, keep], contiguous */
   const int32_t* page_table;
   const int32_t* kv_lens;   /* [B], clamped to 0..capacity */

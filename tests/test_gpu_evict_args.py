@@ -36,3 +36,26 @@ def test_counts_whose_sum_overflows_are_refused(cuda_device, way, first, last):
     with pytest.raises(ValueError, match="keep"):
         ab.paged_kv_evict(kp, vp, table, w, lens, keep=20, keep_first=first, keep_last=last)
     assert all(torch.equal(a, b) for a, b in zip((kp, vp, w), before))
+
+
+@pytest.mark.parametrize("B,hkv", [(2, 2), (1, 1), (1, 3)])
+def test_weights_of_one_buffer_in_turn(cuda_device, way, B, hkv):
+    """Two halves of one buffer share no element: one may receive what the other becomes."""
+    kp, vp, table, w, lens = _state(cuda_device, B, hkv)
+    both = torch.full((2, B, hkv, 64), -5.0, device=cuda_device)
+    both[0] = w
+    pools = [(kp.clone(), vp.clone()) for _ in range(3)]
+    apart = torch.full_like(w, -5.0)
+    want = ab.paged_kv_evict(*pools[0], table, w, lens, keep=20, keep_last=3, weights_out=apart)
+    got = ab.paged_kv_evict(*pools[1], table, both[0], lens, keep=20, keep_last=3, weights_out=both[1])
+    assert torch.equal(got, want) and torch.equal(both[1], apart) and torch.equal(both[0], w)
+    both[1], both[0] = w, -5.0
+    got = ab.paged_kv_evict(*pools[2], table, both[1], lens, keep=20, keep_last=3, weights_out=both[0])
+    assert torch.equal(got, want) and torch.equal(both[0], apart)
+    for other in pools[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(other, pools[0]))
+    flat = both.view(-1)
+    n = B * hkv * 64
+    for shift in (1, 16, n - 1):
+        with pytest.raises(ValueError, match="weights_out"):
+            ab.paged_kv_evict(kp, vp, table, both[0], lens, keep=20, weights_out=flat[shift:shift + n].view(B, hkv, 64))

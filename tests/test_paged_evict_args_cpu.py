@@ -2,9 +2,12 @@
 is not what their shape says."""
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
+from aicas_b200 import _native as nat
 from aicas_b200.eviction import _check_weights
 
 
@@ -30,3 +33,22 @@ def test_weights_of_contiguous_slots_are_taken(shape):
     assert _check(torch.zeros(h, b, 32).transpose(0, 1), 32) == (step(b, 32), step(h, 32 * b))
     odd = torch.zeros(32).as_strided((1, 1, 32), (7, 5, 1))
     assert _check(odd, 32) == (0, 0)
+
+
+@pytest.mark.parametrize("at,strides,taken", [
+    (0, (4096, 512), True), (2 * 4096, (4096, 512), True), (-2 * 4096, (4096, 512), True),  # in place, behind, before
+    (64, (4096, 512), False), (2 * 4096 - 1, (4096, 512), False), (1 - 2 * 4096, (4096, 512), False), (0, (4096, 256), False),
+    (256, (4096, 512), False)])
+def test_weights_out_of_the_c_entry(native_lib, at, strides, taken):
+    """The entry's checks come before any launch: what passes this one fails at the lengths' own."""
+    p = nat.PagedEvictParams()
+    base = 1 << 20  # fake addresses, never dereferenced
+    pl = p.plane[0]
+    pl.data, pl.stride_p, pl.stride_h, pl.stride_t, pl.row_bytes = base * 8, 8 * 16 * 256, 16 * 256, 256, 256
+    p.num_planes, p.weights, p.weights_out, p.kept, p.page_table = 1, base * 2, base * 2 + 4 * at, base * 3, base * 5
+    p.kv_lens, p.kv_lens_out = base * 6, base * 6 + 4  # refused, last of all
+    p.w_stride_b, p.w_stride_h, p.wo_stride_b, p.wo_stride_h, p.table_stride = 4096, 512, *strides, 64
+    p.batch, p.num_kv_heads, p.num_pages, p.page_size, p.max_pages = 2, 8, 100, 16, 32
+    p.keep, p.longer_than = 100, 100
+    assert native_lib.aicas_paged_evict(ctypes.byref(p), None) == nat.ERR_INVALID
+    assert ("kv_lens_out" if taken else "weights_out") in nat.last_error()
