@@ -192,10 +192,10 @@ def paged_kv_evict(
         raise ValueError(f"{what}: keep must be below 2^31")
     slots = max_pages * size
     wb, wh = _check_weights(what, "weights", weights, B, Hkv, slots, index)
-    if weights.requires_grad:
-        _reject_grad(weights)
     if weights_out is None:
         weights_out = weights
+    if weights.requires_grad or weights_out.requires_grad:
+        _reject_grad(weights, weights_out)
     ob, oh = _check_weights(what, "weights_out", weights_out, B, Hkv, slots, index)
     at, to = ((t.data_ptr(), t.data_ptr() + 4 * (max(B - 1, 0) * sb + max(Hkv - 1, 0) * sh + slots))
               for t, sb, sh in ((weights, wb, wh), (weights_out, ob, oh)))

@@ -59,3 +59,14 @@ def test_weights_of_one_buffer_in_turn(cuda_device, way, B, hkv):
     for shift in (1, 16, n - 1):
         with pytest.raises(ValueError, match="weights_out"):
             ab.paged_kv_evict(kp, vp, table, both[0], lens, keep=20, weights_out=flat[shift:shift + n].view(B, hkv, 64))
+
+
+def test_weights_out_that_needs_a_gradient_is_refused(cuda_device, way):
+    kp, vp, table, w, lens = _state(cuda_device)
+    out = torch.zeros_like(w).requires_grad_()
+    with pytest.raises(ValueError):
+        ab.paged_kv_evict(kp, vp, table, w, lens, keep=20, weights_out=out)
+    assert not out.any()
+    with torch.no_grad():
+        ab.paged_kv_evict(kp, vp, table, w, lens, keep=20, weights_out=out)
+    assert out[..., :20].all() and not out[..., 20:].any()
