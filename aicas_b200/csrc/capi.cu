@@ -630,7 +630,8 @@ int check_paged_weights(const aicas_paged_weights_params* p) {
     if (s < 0) return fail(AICAS_ERR_INVALID, "strides of lse and weights must not be negative");
   if (((reinterpret_cast<uintptr_t>(p->lse) | reinterpret_cast<uintptr_t>(p->weights)) & 3u) != 0)
     return fail(AICAS_ERR_INVALID, "lse and weights must be 4-byte aligned");
-  const int64_t tiles = (((int64_t)p->max_pages * p->page_size + 15) / 16 + 1) * p->batch * p->num_kv_heads;
+  // tiles of (request, KV head), one more for a start inside a tile and 8 for what a pair costs, are numbered with 32-bit ints
+  const int64_t tiles = (((int64_t)p->max_pages * p->page_size + 15) / 16 + 9) * p->batch * p->num_kv_heads;
   if (tiles > (int64_t)INT32_MAX / 2)
     return fail(AICAS_ERR_UNSUPPORTED, "%lld tiles of 16 slots exceed the 2^30 of one launch", (long long)tiles);
   return check_scale(p->sm_scale);

@@ -52,3 +52,19 @@ def test_weights_out_of_the_c_entry(native_lib, at, strides, taken):
     p.keep, p.longer_than = 100, 100
     assert native_lib.aicas_paged_evict(ctypes.byref(p), None) == nat.ERR_INVALID
     assert ("kv_lens_out" if taken else "weights_out") in nat.last_error()
+
+
+@pytest.mark.parametrize("batch,heads,max_pages,taken", [(1 << 24, 8, 1, False), (14_000_000, 8, 1, False), (12_000_000, 8, 1, True), (1 << 16, 8, 128, True),
+                                                         (1 << 16, 8, 4096, False)])
+def test_pairs_whose_units_exceed_32_bits_are_refused(native_lib, batch, heads, max_pages, taken):
+    """Pairs of few tiles count by what beginning and ending them costs (8 tiles of a block of warps)."""
+    p = nat.PagedWeightsParams()
+    base = 1 << 20  # fake addresses, never dereferenced
+    p.q, p.k_pages, p.lse, p.weights, p.page_table, p.table_stride = base, base * 2, base * 3, base * 4, base * 5, 0
+    p.q_stride_b, p.q_stride_h, p.q_stride_s = 2048, 128, 128
+    p.kp_stride_p, p.kp_stride_h, p.kp_stride_t = 8 * 8 * 128, 8 * 128, 128
+    p.batch, p.num_q_heads, p.num_kv_heads, p.seq_len, p.head_dim = batch, 2 * heads, heads, 9, 128
+    p.num_pages, p.page_size, p.max_pages, p.dtype = 100, 8, max_pages, nat.DTYPE_BF16
+    p.sm_scale = float("inf")  # refused, last of all
+    assert native_lib.aicas_paged_weights(ctypes.byref(p), None) == (nat.ERR_INVALID if taken else nat.ERR_UNSUPPORTED)
+    assert ("finite" if taken else "2^30") in nat.last_error()
