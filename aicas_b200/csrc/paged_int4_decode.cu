@@ -21,8 +21,9 @@
 //   * Products: m16n8k16 with K (16 slots) and V^T (16 dims) as the 16-row operand and the
 //     heads as the 8 columns; a probability moves from the scores' accumulator layout to
 //     the operand layout by a transposing 8 x 8 move in registers.
-//   * Rounding: a 16-bit q is exact in one fp16 after scaling by a power of two a head (down
-//     to 2^-29 of its largest element).  A probability times its scale enters P V as two
+//   * Rounding: a 16-bit q enters as one fp16 after scaling by a power of two a head.  In the
+//     dims that are taken by 1 / 16 an element is exact down to 2^-24 (of fp16; bf16 2^-27) of its head's largest and
+//     off by at most 2^-35 of that below, in the others down to 2^-28 (2^-31) and 2^-39.  A probability times its scale enters P V as two
 //     fp16 parts, 22 bits, or to within 2^-25 of numbers that a power of two brings to 2^7 and
 //     more for the largest scale of V so far: 2^-32 of that scale, whatever its slot's
 //     probability.  Everything else is fp32, but a product's sum is cut off, not rounded, and

@@ -132,7 +132,7 @@ def _table(what: str, page_table, batch: int, index: int):
     return page_table, t_shape[1], page_table.stride(0)
 
 
-def _check_query(what: str, query, k_pages) -> None:
+def _check_query(what: str, query) -> None:
     if query.ndim != 4:
         raise ValueError(f"{what}: query must be 4-D")
     if query.device.type != "cuda":
@@ -173,7 +173,7 @@ def paged_rope_kv_append_int4(
     if query.requires_grad or key.requires_grad or value.requires_grad:
         _reject_grad(query, key, value)
     what = "paged_rope_kv_append_int4"
-    _check_query(what, query, k_pages)
+    _check_query(what, query)
     B, Hq, S, D = query.shape
     (P, Hkv, size, dim, group), refs, page_table, max_pages, table_stride = _pools(
         what, query, k_pages, v_pages, page_table, B, query.dtype)
@@ -254,7 +254,7 @@ def paged_gqa_decode_attention_int4(
     if query.requires_grad:
         _reject_grad(query)
     what = "paged_gqa_decode_attention_int4"
-    _check_query(what, query, k_pages)
+    _check_query(what, query)
     B, Hq, q_len, D = query.shape
     (P, Hkv, size, dim, group), refs, page_table, max_pages, table_stride = _pools(
         what, query, k_pages, v_pages, page_table, B, query.dtype)
