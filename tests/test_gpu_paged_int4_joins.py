@@ -71,6 +71,64 @@ def test_long_sums_do_not_drift(cuda_device, dtype, dim, group, groups):
     assert abs(total / count) <= bound
 
 
+def _late_case(device, dtype, dim, group, groups, edit):
+    """Many pairs of some 70 tiles, about 28 a warp, whose first and later halves `edit` sets apart; against
+    64 bits on the device, with the tolerances of test_gpu_paged_far_scores.py."""
+    g = torch.Generator(device=device).manual_seed(group + groups)
+    B, hkv, n, size, dt = 90, 8, 2400, 16, DT[dtype]
+    per = n // size
+    rows = [torch.randn(B * per, hkv, size, dim, generator=g, device=device) for _ in range(2)]
+    q = torch.randn(B, hkv * groups, 1, dim, generator=g, device=device)
+    edit(q, *(r.view(B, 2, per // 2, hkv, size, dim) for r in rows))  # [request, half of its pages]
+    kp, vp = (ab.quantize_kv_int4(r.to(dt), group) for r in rows)
+    q, table = q.to(dt), torch.arange(B * per, dtype=torch.int32, device=device).view(B, per)
+    lens = [n - 7 * b for b in range(B)]
+    out, lse = ab.paged_gqa_decode_attention_int4(q, kp, vp, table, sm_scale=dim ** -0.5, num_key_value_groups=groups,
+                                                  kv_lens=lens, return_lse=True)
+    scale, log2 = dim ** -0.5, 0.6931471805599453
+    k_all, v_all = (p.dequantize().view(B, per, hkv, size, dim).transpose(1, 2).flatten(2, 3) for p in (kp, vp))
+    for b, length in enumerate(lens):
+        k, v = (x[b, :, :length].double() for x in (k_all, v_all))
+        mine = q[b, :, 0].double().view(hkv, groups, dim)
+        s = mine @ k.transpose(1, 2) * scale
+        # scale code + |least| is at most three times a row's largest |k|
+        e = 40 * 2.0 ** -24 * 3 * (mine.abs().sum(-1) * k.abs().amax((1, 2))[:, None]).flatten() * scale / log2
+        ref = (torch.softmax(s, -1) @ v).view(-1, dim)
+        ref_lse = torch.logsumexp(s, -1).flatten() / log2
+        top = v.abs().max()
+        bound = torch.finfo(dt).eps / 2 * ref.abs() + 2e-4 * top + 2 * torch.expm1(e * log2)[:, None] * top
+        assert ((out[b, :, 0].double() - ref).abs() <= bound).all()
+        assert ((lse[b].double() - ref_lse).abs() <= e + 1e-4 + 2.0 ** -22 * ref_lse.abs()).all()
+
+
+LATE = pytest.mark.parametrize("dtype,dim,group,groups", [("bf16", 128, 128, 2), ("bf16", 128, 64, 8), ("fp16", 64, 64, 6)])
+
+
+@LATE
+@pytest.mark.parametrize("far", [-100.0, -6.0, 6.0])
+def test_references_that_move_late(cuda_device, dtype, dim, group, groups, far):
+    """The first half of each cache scores far below or above the second: sums that are held by then are
+    scaled with the rest."""
+
+    def edit(q, k, v):
+        k[:, 0, :, 0] += 3.0
+        q[:, :groups] = 0.1 * q[:, :groups] + far / (dim ** -0.5 * 3.0 * dim)
+
+    _late_case(cuda_device, dtype, dim, group, groups, edit)
+
+
+@LATE
+@pytest.mark.parametrize("early,late", [(2.0 ** -7, 1.0), (2.0 ** -12, 1.0), (1.0, 2.0 ** -7)])
+def test_scales_that_grow_late(cuda_device, dtype, dim, group, groups, early, late):
+    """Values of another size from the middle of each cache on."""
+
+    def edit(q, k, v):
+        v[:, 0] *= early
+        v[:, 1] *= late
+
+    _late_case(cuda_device, dtype, dim, group, groups, edit)
+
+
 @pytest.mark.parametrize("to", [1e-35, 1e-20, 1e20, 1e34, 4e36])
 @pytest.mark.parametrize("group", [64, 128])
 @pytest.mark.parametrize("groups", [2, 8])
