@@ -154,7 +154,10 @@ def paged_kv_evict(
     and -1 past its length.
 
     A page that a cut request holds must be in one place of one row of the page table:
-    pages that requests share have to be copied first."""
+    pages that requests share have to be copied first.  All slots below ``kv_lens[b]`` are
+    tokens here: a request that is attended to from a ``kv_starts[b]`` above 0 has to be
+    left out (its masked slots would be kept as its first ones, and others by their weight
+    of 0, as many as each head chances to have, and no start would hold for the cut cache)."""
     done = fast("evict", k_pages, v_pages, page_table, weights, kv_lens, keep, keep_first, keep_last, longer_than, kv_lens_out,
                 weights_out)
     if done is not None:

@@ -626,7 +626,8 @@ typedef struct aicas_paged_evict_params {
    are equal; NaN counts as less than all numbers) move to slots 0 .. keep - 1 in their order, with
    their weights; the weights of the slots behind become 0.  kept[b, h, i] is the slot that became i;
    in a cache that is not cut, i, and -1 past its length.  Rows behind the kept ones stay as they
-   were.  A page is in one place of one request's row of the table. */
+   were.  A page is in one place of one request's row of the table.  All slots below kv_lens are
+   tokens: a cache that is attended to from a kv_starts above 0 is not to be cut. */
 AICAS_API int aicas_paged_evict(const aicas_paged_evict_params* p, void* stream);
 
 /* ------------------------------------------------------------------------ */
