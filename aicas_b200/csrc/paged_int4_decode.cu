@@ -27,19 +27,20 @@
 //     fp16 parts, 22 bits, or to within 2^-25 of numbers that a power of two brings to 2^7 and
 //     more for the largest scale of V so far: 2^-32 of that scale, whatever its slot's
 //     probability.  Everything else is fp32, but a product's sum is cut off, not rounded, and
-//     codes are all positive, so that a long chain of products into o drifts: with values around 0,
-//     whose sums of scale times code and of least cancel, by 2.6e-4 of the result over 131072
-//     slots a request in a batch of 4, growing with the tiles a warp has.  So o is emptied into a
-//     rounded sum in shared memory every kHoldTiles tiles: in fp16 2.2e-4 off the 64-bit result (its
-//     own rounding is 2.06e-4), without 3.4e-4.
+//     codes are all positive, so that a long chain of products into o drifts, and with values around
+//     0 the sums of scale times code and of least cancel.  So o is emptied into a rounded sum
+//     in shared memory every kHoldTiles tiles: 128 fp16 caches of 65536 slots 2.3e-4 off the 64-bit
+//     result (its own rounding is 2.07e-4), without 1.5e-2; 4 of 131072 2.2e-4, 3.4e-4.
 //   * Slots out of range: score -inf, V's scale and least 0.
 //   * Bound: HBM, from a few thousand tiles on.  16 query and 8 KV heads of 128 in bf16: 4
-//     caches of 131072 slots, groups of 128, 105 us, 5.75 TB/s; 64 of up to 4096 37 us, 4.15
-//     TB/s, of which about 5 us pass before the first products and 6 after the copies end.
-//     One of 1024 7.1 us: the chain lengths, page table, rows, products, join.
+//     caches of 131072 slots, groups of 64, 110 us, 5.5 TB/s; 64 of up to 4096, groups of 128,
+//     38 us, 4.0 TB/s, of which about 5 us pass before the first products and 6 after the copies end.
+//     One of 1024 7.3 us: the chain lengths, page table, rows, products, join.
 //   * Taken and dropped (64 of up to 4096): masks after multiplies instead of shifts 41 -> 44
 //     us; rings of 3 stages no faster than 2; 8 warps of twice the registers 10% slower; two
-//     partial results joined at once 37 -> 52 (spills).
+//     partial results joined at once 37 -> 52 (spills).  Against the drift of o, V's codes centred
+//     at 8, by products with a constant (4 x 131072 111 us) or the lanes' own sums (109.5): codes
+//     that do not average 8 drift on.
 #include <cstdio>
 #include <cstring>
 #include <type_traits>
@@ -52,21 +53,21 @@ namespace aicas {
 namespace {
 
 constexpr int kTile = kInt4Tile;
-// Ranges that a pair is cut into, about: 64 caches of up to 4096 slots, with 1 41.2 us, 2 38.0,
-// 4 36.9, 8 38.1.
+// Ranges that a pair is cut into, about: 64 caches of up to 4096 slots, with 1 42.6 us, 2 38.9,
+// 4 38.1, 8 38.9.
 constexpr int kRanges = 4;
-// What beginning and ending a pair costs a warp, in tiles: the same with 1 38.2, 3 36.9, 6 38.1;
-// 256 caches of up to 512 30.4, 28.3, 29.9.
+// What beginning and ending a pair costs a warp, in tiles: the same with 1 39.8, 3 38.1, 6 39.4;
+// 256 caches of up to 512 31.4, 28.8, 31.0.
 constexpr int kPairCost = 3;
 // Most tiles a CTA of a launch that gives pairs whole teams: 8 caches of up to 2048 slots 10.4
-// us, in equal ranges 11.9 (with 8 already), one of 8192 10.2, 10.9.
+// us, in equal ranges 11.9 (with 8 already), one of 8192 10.4, 11.0.
 constexpr int kSmallTiles = 32;
 constexpr int kLogWarps = 4, kMaxWarps = 1 << kLogWarps;
-// Warps of a team in a small launch, as a power of two: one cache of 1024 slots with 2 8.1 us, 4 7.1, 16 8.4.
+// Warps of a team in a small launch, as a power of two: one cache of 1024 slots with 2 8.2 us, 4 7.3, 16 8.5.
 constexpr int kSmallLog = 2;
 constexpr int kHeads = 8;      // query heads of a block
 // Tiles of a warp whose products are added up in the tensor cores alone: 4 caches of 131072 slots
-// 109.6 us with 8, 109.1 with 16, 105.3 without an end (64 of up to 4096 37.8, 37.6, 36.9).
+// 109.9 us with 8, 109.0 with 16, 105.3 without an end (64 of up to 4096 38.1, 37.8, 36.9).
 constexpr int kHoldTiles = 8;
 constexpr size_t kWsCounters = (size_t)1 << 20;  // counter region shared with the other decode kernels
 struct Int4Args {
@@ -122,7 +123,7 @@ __device__ __forceinline__ void split_half(float x, float y, uint32_t& hi, uint3
 
 // WIDE: up to 8 heads, a column each, lo parts in products of their own; else up to 4
 // heads, head j's hi and lo parts in columns 2 j and 2 j + 1 of the same products (2 heads, 4
-// caches of 131072 slots: 105 us, as WIDE 129).
+// caches of 131072 slots: 110 us, as WIDE 132).
 // A lane's heads: WIDE 2 i and 2 i + 1, else i; its slots of 16: rows g and g + 8 of a product.
 // K's fragments are words: lane i has 8 dims of each 32.  V's are 16-bit units of 4 dims,
 // paired over two slots by the transposing load: lane g has units g of each 32.
