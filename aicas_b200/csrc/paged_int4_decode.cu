@@ -22,10 +22,11 @@
 //     heads as the 8 columns; a probability moves from the scores' accumulator layout to
 //     the operand layout by a transposing 8 x 8 move in registers.
 //   * Rounding: a 16-bit q enters as one fp16 after scaling by a power of two a head.  In the
-//     dims that are taken by 1 / 16 an element is exact down to 2^-24 (of fp16; bf16 2^-27) of its head's largest and
-//     off by at most 2^-35 of that below, in the others down to 2^-28 (2^-31) and 2^-39.  A probability times its scale enters P V as two
-//     fp16 parts, 22 bits, or to within 2^-25 of numbers that a power of two brings to 2^7 and
-//     more for the largest scale of V so far: 2^-32 of that scale, whatever its slot's
+//     dims that are taken by 1 / 16 an element is exact down to 2^-24 (of fp16; bf16 2^-27) of its
+//     head's largest and off by at most 2^-35 of that below, in the others down to 2^-28 (2^-31)
+//     and 2^-39.  A probability times its scale enters P V as two fp16 parts, 22 bits, or to
+//     within 2^-25 of numbers that a power of two brings to 2^7 and more for the largest scale
+//     of V so far: 2^-32 of that scale, whatever its slot's
 //     probability.  Everything else is fp32, but a product's sum is cut off, not rounded, and
 //     codes are all positive, so that a long chain of products into o drifts, and with values around
 //     0 the sums of scale times code and of least cancel.  So o is emptied into a rounded sum
